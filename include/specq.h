@@ -44,10 +44,21 @@ extern "C" {
 #define SPECQ_STATUS_TIMEOUT_TEST 0x04     /* specq_selftest_wait_timeout's deliberate wait         */
 #define SPECQ_STATUS_TIMEOUT_PEER 0x08     /* a peer GPU's exchange signal did not arrive in time   */
 #define SPECQ_STATUS_PLAN_CLAMPED 0x100    /* a plan value was outside [0, max] and was clamped     */
+#define SPECQ_STATUS_KV_NONFINITE 0x200    /* an appended K or V value was infinite or NaN           */
+#define SPECQ_STATUS_BAD_INDEX 0x400       /* a page, row or draft index read on the device was out of range and skipped */
 
 /* ---- dtypes for scale tensors ----------------------------------------------------------- */
 #define SPECQ_DTYPE_F16 0
 #define SPECQ_DTYPE_F32 1
+#define SPECQ_DTYPE_BF16 2
+
+/* ---- the numbers of a block-scaled KV cache --------------------------------------------- */
+#define SPECQ_CACHE_INT8 0 /* -127 .. 127  */
+#define SPECQ_CACHE_E4M3 1 /* e4m3, +-448  */
+
+/* ---- pair layouts of the rotary positions ------------------------------------------------ */
+#define SPECQ_ROPE_HALF 0        /* pairs (i, i + rot/2) */
+#define SPECQ_ROPE_INTERLEAVED 1 /* pairs (2i, 2i + 1)   */
 
 /*
  * W8A8 GEMM.  out[m, n] = fp16( (fp32(sum_k a[m,k] * w[n,k]) * sa[m]) * sw[n] )
@@ -268,6 +279,105 @@ int specq_w8a8_peer(const int8_t* a, int64_t lda, const float* sa, const int8_t*
 int specq_quant_rows_peer(const void* x, int64_t ldx, void* r, int64_t ldr, int8_t* q, int64_t ldq, float* s,
                           const int32_t* plan, const float* amax_in, float* amax_out, int M, int N, int mode,
                           const uint32_t* wait_flags, int rank, int world, void* stream);
+
+/* ==== the block-scaled KV cache: 8 bits, one fp32 scale for each page and KV head ============
+ * No reference counterpart (the reference's cache has a scale for each token and head, and no
+ * rotary positions, page pool or draft trees).
+ *   kc, vc   int8 or e4m3 numbers [P, page, H_KV, D], strides (kv_sp, kv_so, kv_sh), unit
+ *            stride along D; D is 64 or 128, page a power of two in 8..128
+ *   ks, vs   fp32 [P, H_KV], strides (s_sp, s_sh): the value is number * scale, scales positive
+ *   block_tbl int32 [B, bt_cols], row stride bt_sb; ctx_len int32 [B] as for attention above
+ */
+
+/* Rotary positions of the first `rot` elements of every head:
+ *   pair i of row t turns by the angle whose cosine and sine are table[pos[t], i] and
+ *   table[pos[t], rot/2 + i]; elements past rot are copied.
+ *   x, out   [T, H, D] of SPECQ_DTYPE_* `dtype`, strides (xt, xh) / (ot, oh), unit along D;
+ *            out may be x (same strides)
+ *   table    fp32 [n_pos, rot], contiguous (cosines | sines); rot even
+ *   pos      int32 [T]; one outside the table is clamped (SPECQ_STATUS_PLAN_CLAMPED)
+ *   layout   SPECQ_ROPE_*; inverse != 0 turns back (the gradient)
+ *   plan     optional, plan[0] = the active rows
+ */
+int specq_rope(const void* x, int64_t xt, int64_t xh, void* out, int64_t ot, int64_t oh, int dtype,
+               const int32_t* pos, const float* table, int n_pos, int T, int H, int D, int rot, int layout,
+               int inverse, const int32_t* plan, void* stream);
+
+/* Write the K and V of the q_len newest tokens of each sequence into their pages, and turn the
+ * same tokens' queries.  Rows are packed: token t of sequence b is row b * q_len + t and goes
+ * to position ctx_len[b] - q_len + t.
+ *   k, v     fp16 or bf16 (dtype) [T, H_KV, D], strides (kt, kh), (vt, vh)
+ *   q        optional [T, H, D], strides (qt, qh) -> q_out (may be q), strides (ot, oh)
+ *   table    optional (null: no rotation, no q); rot a multiple of 16
+ *   pos      optional int32 [T]: rotary positions (null: the tokens' cache positions)
+ * With a = max |x| of a page's new tokens (K after its turn) and qmax = 127 or 448:
+ *   need = max(a, 1e-8) / qmax;  s' = need when the page's slot 0 is new, else max(s, need)
+ *   older tokens of the page become rn(q * (s / s')), the new ones rn(x / s').
+ * NaN is stored as 0 and an infinity as +-qmax, without part in a (SPECQ_STATUS_KV_NONFINITE).
+ * Slots past the new tokens are not touched.  A page that other rows share must not be written
+ * (specq_pages_fork copies a part-filled page).  plan[0] = n_seqs, plan[1] = q_len.
+ */
+int specq_block_append(const void* k, int64_t kt, int64_t kh, const void* v, int64_t vt, int64_t vh, const void* q,
+                       int64_t qt, int64_t qh, void* q_out, int64_t ot, int64_t oh, int dtype, const float* table,
+                       int n_pos, int rot, int layout, const int32_t* pos, void* kc, void* vc, int64_t kv_sp,
+                       int64_t kv_so, int64_t kv_sh, int cache_dtype, int n_pages, float* ks, float* vs,
+                       int64_t s_sp, int64_t s_sh, const int32_t* block_tbl, int64_t bt_sb, int bt_cols,
+                       const int32_t* ctx_len, const int32_t* plan, int B, int n_seqs, int q_len, int ql_max, int H,
+                       int H_KV, int D, int page, void* stream);
+
+/* Attention of the q_len newest tokens of each sequence over the block-scaled cache.
+ *   q, out   fp16 or bf16 (dtype) [B, q_len, H, D] with strides; q_sb = 0 (o_sb = 0): packed rows
+ *   tree     optional uint64 [B, q_len] (strides tree_sb, tree_st): row qi sees draft token j when
+ *            bit j is set (and every token before the drafts); null: the causal window of
+ *            specq_paged_attention.  q_len <= 64 with a tree.
+ *   workspace  16-byte aligned device memory of at least the bytes that
+ *            specq_block_attention_workspace gives for the same sizes; nothing is kept in it
+ * A row that sees no token is 0.  Bytes at and past ctx_len may hold anything.  The result for
+ * given sizes does not depend on timing; under a plan the work is cut by the active sizes, so it
+ * equals the eager call's up to the order of fp32 sums.
+ */
+int specq_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, const void* kc,
+                          const void* vc, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int cache_dtype, int n_pages,
+                          const float* ks, const float* vs, int64_t s_sp, int64_t s_sh, const int32_t* block_tbl,
+                          int64_t bt_sb, int bt_cols, const int32_t* ctx_len, const uint64_t* tree, int64_t tree_sb,
+                          int64_t tree_st, float sm_scale, void* out, int64_t o_sb, int64_t o_st, int64_t o_sh,
+                          const int32_t* plan, int B, int n_seqs, int q_len, int ql_max, int H, int H_KV, int D,
+                          int page, void* workspace, int64_t workspace_bytes, void* stream);
+int specq_block_attention_workspace(int B, int n_seqs, int q_len, int ql_max, int H, int H_KV, int D, int page,
+                                    int bt_cols, int plan, int64_t* bytes);
+
+/* Move the accepted drafts of each sequence together: accept[b, j] (strictly growing, < q_len),
+ * j < n_accept[b], goes from position ctx_len[b] - q_len + accept[b, j] to ctx_len[b] - q_len + j,
+ * in every one of L layers (kv_sl, s_sl: layer strides); ctx_out[b] = ctx_len[b] - q_len +
+ * n_accept[b] (ctx_out is not ctx_len).  A page's scale grows to hold what arrives from pages of
+ * larger scale, and numbers whose scale differs are requantised.  A sequence with a bad index
+ * keeps its tokens and its length (SPECQ_STATUS_BAD_INDEX).
+ */
+int specq_block_compact(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t kv_so, int64_t kv_sh,
+                        int cache_dtype, int L, int n_pages, float* ks, float* vs, int64_t s_sl, int64_t s_sp,
+                        int64_t s_sh, const int32_t* block_tbl, int64_t bt_sb, int bt_cols, const int32_t* ctx_len,
+                        const int32_t* accept, int64_t acc_sb, int acc_cols, const int32_t* n_accept,
+                        int32_t* ctx_out, int B, int q_len, int H_KV, int D, int page, void* stream);
+
+/* The page pool.  ref int32 [P] = rows that hold a page (0: free), tbl int32 [S, C] (row stride
+ * ld) = the rows' pages (-1: none), held int32 [S] = how many each holds.  ref is 16-byte
+ * aligned.  Results are functions of the state alone: free pages are taken lowest first.
+ *   release  rows with drop[r] != 0 (uint8 [S]) give up their pages
+ *   reserve  row r grows to ceil(want[r] / page) pages; every row or none
+ *   fork     row r with parent[r] = p >= 0, p != r becomes row p's first length[p] tokens: full
+ *            pages shared, a part-filled last page copied (all L layers, filled slots and scales);
+ *            every row or none, all at once (a permutation of beams is allowed).  scratch: int32
+ *            [S * (C + 1)] device memory.
+ * short_out (device int32): pages missing, 0 when the call was carried out.
+ */
+int specq_pages_release(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C,
+                        const uint8_t* drop, void* stream);
+int specq_pages_reserve(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C,
+                        const int32_t* want, int page, int32_t* short_out, void* stream);
+int specq_pages_fork(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int L, float* ks,
+                     float* vs, int64_t s_sl, int64_t s_sp, int64_t s_sh, int32_t* ref, int P, int32_t* tbl,
+                     int64_t ld, int32_t* held, int S, int C, const int32_t* parent, const int32_t* length,
+                     int32_t* scratch, int32_t* short_out, int H_KV, int D, int page, void* stream);
 
 /*
  * Pipeline tracing (builds compiled with -DSPECQ_TRACE only; other builds return

@@ -1,0 +1,592 @@
+// block_cache.cuh -- writing a KV cache held in 8 bits with one fp32 scale for each page and
+// KV head: the append of new tokens and the compaction of a verified draft tree.
+//
+// Cache: kc, vc [P, page, H_KV, D] of int8 or e4m3 numbers q (q_max = 127 or 448) and ks, vs
+// [P, H_KV] fp32 scales s; the value is q * s.
+//
+// append.  Token t of sequence b (row b * q_len + t) goes to position ctx_len[b] - q_len + t.
+// For each page that receives tokens and each KV head, with a = max |x| over its new tokens
+// (K after its rotary turn, in fp32):
+//   need = max(a, 1e-8) * fp32(1 / q_max)
+//   s'   = need               if the page's first slot is among the new tokens
+//          max(s, need)       otherwise; the page's older tokens become rn(q * (s / s'))
+//   q'   = rn(x * (1 / s'))   saturated, for the new tokens
+// Older tokens are rewritten only when the scale grows; slots past the new tokens are not
+// touched.  An 8-bit number has no NaN or infinity here: a NaN is stored as 0, an infinity as
+// +-q_max, neither takes part in a, and SPECQ_STATUS_KV_NONFINITE is reported.
+//
+// A warp holds up to 16 slots of one page and head in registers (64 fp32 a thread at D = 128),
+// so the rotated values are made once and used twice, for the maximum and for the numbers; a
+// page of more than 16 tokens is shared by page / 16 warps of one CTA, which exchange their
+// maxima through shared memory.  The same launch turns the tokens' queries: they come from the
+// same rows, and a launch of their own costs a short verification step as much as the work.
+// Bound by HBM for prompts and by latency for a few tokens.
+//
+// compact.  After verification the accepted drafts of sequence b sit at base + accept[b, j]
+// (base = ctx_len - q_len); they move to base + j.  A target page's scale becomes
+//   s' = max(s, max over its arriving tokens of (max |q| * fp32(1 / q_max)) * s_source)
+// and numbers whose scale differs are requantised, rn(q * (s_source / s')).  One warp per
+// (layer, sequence, head, K or V) walks its tokens in order, 4 or 8 at a time: accept[j] >= j
+// and both grow, so a token never lands on one that has yet to be read.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "rope.cuh"
+
+namespace specq {
+
+constexpr int kAppendThreads = 256;
+constexpr int kAppendSlots = 16;     // slots of a page that one warp holds
+constexpr float kKvFloor = 1e-8f;
+
+template <int CT>   // 0 = int8, 1 = e4m3
+__host__ __device__ constexpr float cache_inv_max() { return CT == 0 ? 1.0f / 127.0f : 1.0f / 448.0f; }
+
+// Four fp32 to four saturated 8-bit numbers (round to nearest even); none of v is NaN.
+template <int CT>
+__device__ __forceinline__ uint32_t pack_cache4(float a, float b, float c, float d) {
+  if constexpr (CT == 0) {
+    const float v[4] = {a, b, c, d};
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int q = static_cast<int>(rintf(fminf(fmaxf(v[i], -127.f), 127.f)));
+      w |= (static_cast<uint32_t>(q) & 0xFFu) << (8 * i);
+    }
+    return w;
+  } else {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  }
+}
+
+template <int CT>
+__device__ __forceinline__ void unpack_cache4(uint32_t w, float (&v)[4]) {
+  if constexpr (CT == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = static_cast<float>(static_cast<int8_t>((w >> (8 * i)) & 0xFFu));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w >> (16 * i)) & 0xFFFFu), __NV_E4M3);
+      const float2 f = __half22float2(__half2(r));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+
+// rn(q * r) of four stored numbers
+template <int CT>
+__device__ __forceinline__ uint32_t requant4(uint32_t w, float r) {
+  float v[4];
+  unpack_cache4<CT>(w, v);
+  return pack_cache4<CT>(v[0] * r, v[1] * r, v[2] * r, v[3] * r);
+}
+
+template <int CT>
+__device__ __forceinline__ float absmax4(uint32_t w) {
+  float v[4];
+  unpack_cache4<CT>(w, v);
+  return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+}
+
+struct BlockAppendParams {
+  const void* k;         // [T, H_KV, D] packed token rows
+  const void* v;
+  const void* q;         // optional [T, H, D]: turned into q_out
+  void* q_out;
+  const float* table;    // optional [n_pos, rot]
+  const int32_t* pos;    // optional [T] rotary positions (default: the token's cache position)
+  uint8_t* kc;
+  uint8_t* vc;
+  float* ks;
+  float* vs;
+  const int32_t* bt;
+  const int32_t* ctx;
+  const int32_t* plan;   // plan[0] = n_seqs, plan[1] = q_len
+  int* status;
+  int64_t kt, kh, vt, vh, qt, qh, ot, oh, kv_sp, kv_so, kv_sh, s_sp, s_sh, bt_sb;
+  int n_seqs, q_len, b_grid, ql_max, h_kv, h_q, page_log2, n_pages, bt_cols, rot, n_pos, half;
+  int n_win, win_blocks, kv_blocks;   // pages a sequence may touch, blocks of one of them, blocks of all
+  int q_items, q_groups;
+};
+
+template <typename T>
+__device__ __forceinline__ void load_row4(const T* p, float* v) {
+  const uint2 u = *reinterpret_cast<const uint2*>(p);
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = weight_to_f32<T>(e[i]);
+}
+
+__device__ __forceinline__ void append_extents(const BlockAppendParams& p, int& n_seqs, int& q_len) {
+  n_seqs = p.n_seqs;
+  q_len = p.q_len;
+  if (p.plan != nullptr) {
+    const int a = __ldg(p.plan), b = __ldg(p.plan + 1);
+    n_seqs = min(max(a, 0), p.b_grid);
+    q_len = min(max(b, 0), p.ql_max);
+    if ((a != n_seqs || b != q_len) && blockIdx.x == 0 && threadIdx.x == 0)
+      report_status(p.status, SPECQ_STATUS_PLAN_CLAMPED);
+  }
+}
+
+template <typename T, int D, int CT, int HP>
+__global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __grid_constant__ BlockAppendParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  __shared__ float red[kAppendThreads / 32];
+  int n_seqs, q_len;
+  append_extents(p, n_seqs, q_len);
+
+  if (static_cast<int>(blockIdx.x) >= p.kv_blocks) {   // ---- queries
+    const uint32_t id = (blockIdx.x - p.kv_blocks) * kAppendThreads + threadIdx.x;
+    const uint32_t th = id / static_cast<uint32_t>(p.q_items);
+    const int item = static_cast<int>(id - th * p.q_items);
+    const int t = static_cast<int>(th / static_cast<uint32_t>(p.q_groups));
+    const int h0 = static_cast<int>(th - static_cast<uint32_t>(t) * p.q_groups) * HP;
+    if (t >= n_seqs * q_len) return;
+    int pos;
+    if (p.pos != nullptr) {
+      pos = __ldg(p.pos + t);
+    } else {
+      const int b = t / q_len;
+      pos = __ldg(p.ctx + b) - q_len + (t - b * q_len);
+    }
+    const float* row = rope_row(p.table, pos, p.n_pos, p.rot, p.status);
+    const T* x = static_cast<const T*>(p.q) + t * p.qt + h0 * p.qh;
+    T* out = static_cast<T*>(p.q_out) + t * p.ot + h0 * p.oh;
+    const int n = min(HP, p.h_q - h0);
+    if (p.half) rope_item<T, true, HP>(x, p.qh, out, p.oh, row, p.rot, 1.f, item, n);
+    else rope_item<T, false, HP>(x, p.qh, out, p.oh, row, p.rot, 1.f, item, n);
+    return;
+  }
+
+  // ---- keys and values: (sequence, page of its window, group of (head, K|V) units)
+  const int page = 1 << p.page_log2;
+  const int wpu = max(1, page / kAppendSlots);              // warps of a unit
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  const int bw = static_cast<int>(blockIdx.x) / p.win_blocks;
+  const int part = static_cast<int>(blockIdx.x) - bw * p.win_blocks;
+  const int b = bw / p.n_win, win = bw - b * p.n_win;
+  if (b >= n_seqs || q_len == 0) return;
+  const int ctx = __ldg(p.ctx + b);
+  const int base = ctx - q_len;
+  if (base < 0 || ctx > p.bt_cols * page) {                 // tokens outside the table: not written
+    if (threadIdx.x == 0 && win == 0 && part == 0) report_status(p.status, SPECQ_STATUS_PLAN_CLAMPED);
+    return;
+  }
+  const int col = (base >> p.page_log2) + win;
+  const int start = col << p.page_log2;                     // position of the page's slot 0
+  if (start >= ctx) return;
+  const int pg = __ldg(p.bt + b * p.bt_sb + col);
+  if (pg < 0 || pg >= p.n_pages) {
+    if (threadIdx.x == 0 && part == 0) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+    return;
+  }
+  const int unit = part * ((kAppendThreads / 32) / wpu) + warp / wpu;
+  const bool live = unit < 2 * p.h_kv;
+  const bool is_v = unit >= p.h_kv;
+  const int head = is_v ? unit - p.h_kv : unit;
+  const int sub = warp % wpu;                               // this warp's 16 slots of the page
+
+  constexpr int LPT = D / 8;            // lanes of a token
+  constexpr int TPS = 32 / LPT;         // tokens of a step
+  constexpr int STEPS = kAppendSlots / TPS;
+  const int l = lane % LPT;
+  const bool turn = !is_v && p.table != nullptr && 8 * l < p.rot;
+  // the thread's 8 elements are two runs of 4: partners in the half layout
+  const int o1 = turn && p.half ? 4 * l : 8 * l;
+  const int o2 = turn && p.half ? (p.rot >> 1) + 4 * l : 8 * l + 4;
+  const int slot0 = sub * kAppendSlots + lane / LPT;
+  float x[STEPS][8];
+  float amax = 0.f;
+  bool odd = false;
+  float s_old = 0.f;
+  float* scale = nullptr;
+  uint8_t* dst = nullptr;
+  if (live) {
+    scale = (is_v ? p.vs : p.ks) + static_cast<int64_t>(pg) * p.s_sp + head * p.s_sh;
+    dst = (is_v ? p.vc : p.kc) + static_cast<int64_t>(pg) * p.kv_sp + head * p.kv_sh;
+    s_old = *scale;
+    const T* src = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.vh : p.kh);
+    const int64_t st = is_v ? p.vt : p.kt;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int slot = slot0 + i * TPS;
+      const int tok = start + slot;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+      if (slot < page && tok >= base && tok < ctx) {
+        const T* r = src + static_cast<int64_t>(b * q_len + tok - base) * st;
+        load_row4<T>(r + o1, x[i]);
+        load_row4<T>(r + o2, x[i] + 4);
+      }
+    }
+    if (turn) {
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const int slot = slot0 + i * TPS;
+        const int tok = start + slot;
+        if (slot < page && tok >= base && tok < ctx) {
+          const int pos = p.pos != nullptr ? __ldg(p.pos + b * q_len + tok - base) : tok;
+          const float* row = rope_row(p.table, pos, p.n_pos, p.rot, p.status);
+          float c[4], s[4];
+          load_f32_run<4>(row + 4 * l, c);
+          load_f32_run<4>(row + (p.rot >> 1) + 4 * l, s);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // pairs: (e, e + 4) of the two runs, or neighbours
+            const float a = p.half ? x[i][e] : x[i][2 * e];
+            const float bb = p.half ? x[i][e + 4] : x[i][2 * e + 1];
+            const float y = fmaf(a, c[e], -bb * s[e]), z = fmaf(bb, c[e], a * s[e]);
+            c[e] = y;
+            s[e] = z;
+          }
+          if (p.half) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[i][e] = c[e]; x[i][e + 4] = s[e]; }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[i][2 * e] = c[e]; x[i][2 * e + 1] = s[e]; }
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float a = fabsf(x[i][e]);
+        if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
+        else odd = true;
+      }
+  }
+  amax = warp_max_f32(amax);
+  if (wpu > 1) {
+    if (lane == 0) red[warp] = amax;
+    __syncthreads();                    // also: every warp has read the old scale
+    for (int w = 0; w < wpu; ++w) amax = fmaxf(amax, red[warp - sub + w]);
+  } else {
+    __syncwarp();
+  }
+  if (!live) return;
+  const float need = fmaxf(amax, kKvFloor) * cache_inv_max<CT>();
+  const bool fresh = start >= base;
+  const float s_new = fresh ? need : fmaxf(s_old, need);
+  const float rs = __frcp_rn(s_new);
+  if (odd) report_status(p.status, SPECQ_STATUS_KV_NONFINITE);
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i) {
+    const int slot = slot0 + i * TPS;
+    const int tok = start + slot;
+    if (slot < page && tok >= base && tok < ctx) {
+      float y[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        y[e] = x[i][e] * rs;
+        if (odd && !(y[e] == y[e])) y[e] = 0.f;
+      }
+      uint8_t* d = dst + static_cast<int64_t>(slot) * p.kv_so;
+      *reinterpret_cast<uint32_t*>(d + o1) = pack_cache4<CT>(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<uint32_t*>(d + o2) = pack_cache4<CT>(y[4], y[5], y[6], y[7]);
+    }
+  }
+  if (!fresh && s_new > s_old) {        // the page's older tokens under the grown scale
+    const float r = __fdiv_rn(s_old, s_new);
+    for (int slot = slot0; slot < min(base - start, (sub + 1) * kAppendSlots); slot += TPS) {
+      uint2* d = reinterpret_cast<uint2*>(dst + static_cast<int64_t>(slot) * p.kv_so + 8 * l);
+      uint2 w = *d;
+      w.x = requant4<CT>(w.x, r);
+      w.y = requant4<CT>(w.y, r);
+      *d = w;
+    }
+  }
+  if (sub == 0 && lane == 0 && s_new != s_old) *scale = s_new;
+}
+
+inline bool page_ok(int page) { return page >= 8 && page <= 128 && (page & (page - 1)) == 0; }
+
+inline int run_block_append(const void* k, int64_t kt, int64_t kh, const void* v, int64_t vt, int64_t vh,
+                            const void* q, int64_t qt, int64_t qh, void* q_out, int64_t ot, int64_t oh, int dtype,
+                            const float* table, int n_pos, int rot, int layout, const int32_t* pos, void* kc,
+                            void* vc, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int cache_dtype, int n_pages,
+                            float* ks, float* vs, int64_t s_sp, int64_t s_sh, const int32_t* bt, int64_t bt_sb,
+                            int bt_cols, const int32_t* ctx, const int32_t* plan, int B, int n_seqs, int q_len,
+                            int ql_max, int H, int H_KV, int D, int page, void* stream) {
+  if (B < 0 || n_seqs < 0 || q_len < 0 || ql_max < 0 || H < 0 || H_KV <= 0 || n_pages < 0 || bt_cols < 0)
+    return fail(SPECQ_ERR_INVALID_ARG, "block_append: negative size");
+  if (dtype != 0 && dtype != 2) return fail(SPECQ_ERR_INVALID_ARG, "block_append: row dtype code %d", dtype);
+  if (cache_dtype != SPECQ_CACHE_INT8 && cache_dtype != SPECQ_CACHE_E4M3)
+    return fail(SPECQ_ERR_INVALID_ARG, "block_append: cache dtype code %d", cache_dtype);
+  if (D != 64 && D != 128) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: head_dim %d (this build supports 64 and 128)", D);
+  if (!page_ok(page)) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: page %d (a power of two in 8..128)", page);
+  if (plan == nullptr && (n_seqs > B || q_len > ql_max))
+    return fail(SPECQ_ERR_INVALID_ARG, "block_append: n_seqs/q_len exceed the grid");
+  if (layout < 0 || layout > 1) return fail(SPECQ_ERR_INVALID_ARG, "block_append: layout %d", layout);
+  if (table != nullptr && (rot < 2 || rot > D || n_pos <= 0))
+    return fail(SPECQ_ERR_INVALID_ARG, "block_append: rot=%d n_pos=%d", rot, n_pos);
+  if (table != nullptr && rot % 16)
+    return fail(SPECQ_ERR_UNSUPPORTED, "block_append: rot=%d must be a multiple of 16 (rope takes any even one)", rot);
+  if (table == nullptr && (q != nullptr || pos != nullptr))
+    return fail(SPECQ_ERR_INVALID_ARG, "block_append: queries and positions need a rotary table");
+  const int b_grid = plan ? B : n_seqs;
+  const int ql = plan ? ql_max : q_len;
+  if (b_grid == 0 || ql == 0) return SPECQ_OK;
+  if (k == nullptr || v == nullptr || kc == nullptr || vc == nullptr || ks == nullptr || vs == nullptr ||
+      bt == nullptr || ctx == nullptr || (q != nullptr && q_out == nullptr))
+    return fail(SPECQ_ERR_INVALID_ARG, "block_append: null pointer");
+  if (!aligned(k, 8) || !aligned(v, 8) || kt % 4 || kh % 4 || vt % 4 || vh % 4)
+    return fail(SPECQ_ERR_UNSUPPORTED, "block_append: K and V rows must be 8-byte aligned");
+  if (!aligned(kc, 8) || !aligned(vc, 8) || kv_sp % 8 || kv_so % 8 || kv_sh % 8)
+    return fail(SPECQ_ERR_UNSUPPORTED, "block_append: cache rows must be 8-byte aligned");
+  if (table != nullptr && !aligned(table, 16)) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: table not 16-byte aligned");
+  if (q != nullptr && H > 0 && (!aligned(q, 16) || !aligned(q_out, 16) || qt % 8 || qh % 8 || ot % 8 || oh % 8))
+    return fail(SPECQ_ERR_UNSUPPORTED, "block_append: query rows must be 16-byte aligned");
+  if (q != nullptr && q == q_out && (qt != ot || qh != oh))
+    return fail(SPECQ_ERR_INVALID_ARG, "block_append: in place, the strides of q and q_out must be the same");
+  if (static_cast<int64_t>(b_grid) * ql > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: too many tokens");
+  DeviceState* dev = nullptr;
+  if (int rc = get_device_state(&dev)) return rc;
+  BlockAppendParams p = {};
+  p.k = k; p.v = v; p.q = q; p.q_out = q_out; p.table = table; p.pos = pos;
+  p.kc = static_cast<uint8_t*>(kc); p.vc = static_cast<uint8_t*>(vc); p.ks = ks; p.vs = vs;
+  p.bt = bt; p.ctx = ctx; p.plan = plan; p.status = dev->status;
+  p.kt = kt; p.kh = kh; p.vt = vt; p.vh = vh; p.qt = qt; p.qh = qh; p.ot = ot; p.oh = oh;
+  p.kv_sp = kv_sp; p.kv_so = kv_so; p.kv_sh = kv_sh; p.s_sp = s_sp; p.s_sh = s_sh; p.bt_sb = bt_sb;
+  p.n_seqs = n_seqs; p.q_len = q_len; p.b_grid = b_grid; p.ql_max = ql; p.h_kv = H_KV; p.h_q = H;
+  p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
+  p.n_pages = n_pages; p.bt_cols = bt_cols; p.rot = rot; p.n_pos = n_pos; p.half = layout == 0;
+  const int wpu = std::max(1, page / kAppendSlots);
+  p.n_win = (ql - 1) / page + 2;
+  p.win_blocks = ceil_div(2 * H_KV, (kAppendThreads / 32) / wpu);
+  const int64_t kv_blocks = static_cast<int64_t>(b_grid) * p.n_win * p.win_blocks;
+  int64_t q_blocks = 0;
+  bool many = false;
+  if (q != nullptr && H > 0) {
+    const int64_t tokens = static_cast<int64_t>(b_grid) * ql;
+    const bool tail = q_out != q;
+    p.q_items = rope_items<__half>(D, rot, p.half != 0, tail);
+    many = tokens * H * p.q_items >= static_cast<int64_t>(dev->sm_count) * 2048;
+    p.q_groups = ceil_div(H, many ? kRopeHeads : 1);
+    const int64_t threads = tokens * p.q_groups * p.q_items;
+    if (threads > 0x7FFFFF00ll) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: too many query rows");
+    q_blocks = (threads + kAppendThreads - 1) / kAppendThreads;
+  }
+  if (kv_blocks + q_blocks > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: too many tokens");
+  p.kv_blocks = static_cast<int>(kv_blocks);
+  const dim3 grid(static_cast<unsigned>(kv_blocks + q_blocks));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto launch = [&](auto t, auto d, auto c, auto hp) {
+    return launch_plain(block_append_kernel<decltype(t), decltype(d)::value, decltype(c)::value, decltype(hp)::value>,
+                        grid, dim3(kAppendThreads), st, p);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Many = std::integral_constant<int, kRopeHeads>;
+  auto by_hp = [&](auto t, auto d, auto c) { return many ? launch(t, d, c, Many{}) : launch(t, d, c, One{}); };
+  auto by_cache = [&](auto t, auto d) {
+    return cache_dtype == SPECQ_CACHE_INT8 ? by_hp(t, d, std::integral_constant<int, 0>{})
+                                           : by_hp(t, d, std::integral_constant<int, 1>{});
+  };
+  auto by_dim = [&](auto t) {
+    return D == 64 ? by_cache(t, std::integral_constant<int, 64>{}) : by_cache(t, std::integral_constant<int, 128>{});
+  };
+  SPECQ_CUDA_TRY(dtype == 0 ? by_dim(__half{}) : by_dim(__nv_bfloat16{}));
+  return SPECQ_OK;
+}
+
+struct BlockCompactParams {
+  uint8_t* kc;
+  uint8_t* vc;
+  float* ks;
+  float* vs;
+  const int32_t* bt;
+  const int32_t* ctx;
+  const int32_t* accept;   // [B, A]
+  const int32_t* n_accept; // [B]
+  int32_t* ctx_out;        // [B]
+  int* status;
+  int64_t kv_sl, kv_sp, kv_so, kv_sh, s_sl, s_sp, s_sh, bt_sb, acc_sb;
+  int L, B, h_kv, q_len, acc_cols, page_log2, n_pages, bt_cols;
+};
+
+constexpr int kCompactThreads = 128;
+
+template <int D, int CT>
+__global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __grid_constant__ BlockCompactParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t id = (blockIdx.x * kCompactThreads + threadIdx.x) >> 5;
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const uint32_t hu = 2u * p.h_kv;
+  const uint32_t lb = id / hu;
+  const int unit = static_cast<int>(id - lb * hu);
+  const int layer = static_cast<int>(lb / static_cast<uint32_t>(p.B));
+  const int b = static_cast<int>(lb - static_cast<uint32_t>(layer) * p.B);
+  if (layer >= p.L) return;
+  const int page = 1 << p.page_log2;
+  const bool first_unit = layer == 0 && unit == 0 && lane == 0;
+  const int ctx = __ldg(p.ctx + b);
+  const int base = ctx - p.q_len;
+  const int n_raw = __ldg(p.n_accept + b);
+  const int n = min(max(n_raw, 0), min(p.acc_cols, p.q_len));
+  // accept must grow strictly within the drafts, and the drafts lie in the table
+  const int32_t* acc = p.accept + b * p.acc_sb;
+  bool ok = base >= 0 && ctx <= p.bt_cols * page && n == n_raw;
+  int same = n;                 // leading tokens that already stand where they belong
+  for (int j0 = 0; j0 < n; j0 += 32) {
+    const int j = j0 + lane;
+    bool good = true, moves = false;
+    if (j < n) {
+      const int a = __ldg(acc + j);
+      const int before = j > 0 ? __ldg(acc + j - 1) : -1;
+      good = a > before && a < p.q_len;
+      moves = a != j;
+    }
+    ok = ok && __all_sync(0xffffffffu, good);
+    const unsigned m = __ballot_sync(0xffffffffu, moves);
+    if (m != 0u && same == n) same = j0 + __ffs(m) - 1;
+  }
+  const int32_t* bt = p.bt + b * p.bt_sb;
+  if (ok && same < n) {         // and every page of theirs is one of the cache
+    bool good = true;
+    for (int c = (base >> p.page_log2) + lane; c <= (ctx - 1) >> p.page_log2; c += 32) {
+      const int pg = __ldg(bt + c);
+      good = good && pg >= 0 && pg < p.n_pages;
+    }
+    ok = __all_sync(0xffffffffu, good);
+  }
+  if (first_unit) {
+    p.ctx_out[b] = ok ? base + n : ctx;
+    if (!ok) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+  }
+  if (!ok || same == n) return;   // not ok: nothing of this sequence moves
+
+  const bool is_v = unit >= p.h_kv;
+  const int head = is_v ? unit - p.h_kv : unit;
+  uint8_t* cache = (is_v ? p.vc : p.kc) + layer * p.kv_sl + head * p.kv_sh;
+  float* scale = (is_v ? p.vs : p.ks) + layer * p.s_sl + head * p.s_sh;
+  constexpr int LPT = D / 16, TPS = 32 / LPT;   // lanes of a token (16 bytes each), tokens of a step
+  constexpr int BATCH = 4;                      // steps in flight
+  const int sub = lane / LPT;
+  const int byte = (lane % LPT) * 16;
+  const int mask = page - 1;
+
+  for (int j0 = same; j0 < n;) {
+    const int dpos = base + j0;
+    const int dcol = dpos >> p.page_log2;
+    const int j1 = min(n, ((dcol + 1) << p.page_log2) - base);   // this target page takes tokens j0 .. j1 - 1
+    const int dpg = __ldg(bt + dcol);
+    uint8_t* dst = cache + static_cast<int64_t>(dpg) * p.kv_sp;
+    float* s_at = scale + static_cast<int64_t>(dpg) * p.s_sp;
+    const float s_old = *s_at;
+    // the arriving tokens' need; those of the page itself fit its scale already
+    float need = 0.f;
+    for (int j = j0 + sub; j < j1; j += TPS) {
+      const int pos = base + __ldg(acc + j);
+      const int scol = pos >> p.page_log2;
+      if (scol == dcol) continue;
+      const int spg = __ldg(bt + scol);
+      const uint4 w = *reinterpret_cast<const uint4*>(cache + static_cast<int64_t>(spg) * p.kv_sp +
+                                                      static_cast<int64_t>(pos & mask) * p.kv_so + byte);
+      const float a = fmaxf(fmaxf(absmax4<CT>(w.x), absmax4<CT>(w.y)), fmaxf(absmax4<CT>(w.z), absmax4<CT>(w.w)));
+      need = fmaxf(need, a * cache_inv_max<CT>() * scale[static_cast<int64_t>(spg) * p.s_sp]);
+    }
+    need = warp_max_f32(need);
+    const float s_new = fmaxf(s_old, need);
+    if (s_new > s_old) {        // what the page held before the arriving tokens
+      const float r = __fdiv_rn(s_old, s_new);
+      const int keep = dpos & mask;
+      for (int slot = sub; slot < keep; slot += TPS) {
+        uint4* d = reinterpret_cast<uint4*>(dst + static_cast<int64_t>(slot) * p.kv_so + byte);
+        uint4 w = *d;
+        w.x = requant4<CT>(w.x, r); w.y = requant4<CT>(w.y, r);
+        w.z = requant4<CT>(w.z, r); w.w = requant4<CT>(w.w, r);
+        *d = w;
+      }
+    }
+    for (int jb = j0; jb < j1; jb += BATCH * TPS) {
+      uint4 w[BATCH];
+      float r[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int j = jb + i * TPS + sub;
+        w[i] = make_uint4(0u, 0u, 0u, 0u);
+        r[i] = 1.f;
+        if (j < j1) {
+          const int pos = base + __ldg(acc + j);
+          const int scol = pos >> p.page_log2;
+          const int spg = __ldg(bt + scol);
+          w[i] = *reinterpret_cast<const uint4*>(cache + static_cast<int64_t>(spg) * p.kv_sp +
+                                                 static_cast<int64_t>(pos & mask) * p.kv_so + byte);
+          const float ss = scol == dcol ? s_old : scale[static_cast<int64_t>(spg) * p.s_sp];
+          if (ss != s_new) r[i] = __fdiv_rn(ss, s_new);
+        }
+      }
+      __syncwarp();             // every read of the batch before its writes
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int j = jb + i * TPS + sub;
+        if (j < j1) {
+          if (r[i] != 1.f) {
+            w[i].x = requant4<CT>(w[i].x, r[i]); w[i].y = requant4<CT>(w[i].y, r[i]);
+            w[i].z = requant4<CT>(w[i].z, r[i]); w[i].w = requant4<CT>(w[i].w, r[i]);
+          }
+          *reinterpret_cast<uint4*>(dst + static_cast<int64_t>((base + j) & mask) * p.kv_so + byte) = w[i];
+        }
+      }
+      __syncwarp();
+    }
+    if (lane == 0 && s_new != s_old) *s_at = s_new;
+    __syncwarp();
+    j0 = j1;
+  }
+}
+
+inline int run_block_compact(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t kv_so, int64_t kv_sh,
+                             int cache_dtype, int L, int n_pages, float* ks, float* vs, int64_t s_sl, int64_t s_sp,
+                             int64_t s_sh, const int32_t* bt, int64_t bt_sb, int bt_cols, const int32_t* ctx,
+                             const int32_t* accept, int64_t acc_sb, int acc_cols, const int32_t* n_accept,
+                             int32_t* ctx_out, int B, int q_len, int H_KV, int D, int page, void* stream) {
+  if (B < 0 || q_len < 0 || H_KV <= 0 || n_pages < 0 || bt_cols < 0 || L <= 0 || acc_cols < 0)
+    return fail(SPECQ_ERR_INVALID_ARG, "block_compact: negative size");
+  if (cache_dtype != SPECQ_CACHE_INT8 && cache_dtype != SPECQ_CACHE_E4M3)
+    return fail(SPECQ_ERR_INVALID_ARG, "block_compact: cache dtype code %d", cache_dtype);
+  if (D != 64 && D != 128) return fail(SPECQ_ERR_UNSUPPORTED, "block_compact: head_dim %d (this build supports 64 and 128)", D);
+  if (!page_ok(page)) return fail(SPECQ_ERR_UNSUPPORTED, "block_compact: page %d (a power of two in 8..128)", page);
+  if (B == 0) return SPECQ_OK;
+  if (kc == nullptr || vc == nullptr || ks == nullptr || vs == nullptr || bt == nullptr || ctx == nullptr ||
+      n_accept == nullptr || ctx_out == nullptr || (acc_cols > 0 && accept == nullptr))
+    return fail(SPECQ_ERR_INVALID_ARG, "block_compact: null pointer");
+  if (ctx == ctx_out) return fail(SPECQ_ERR_INVALID_ARG, "block_compact: ctx_out must not be ctx_len (every warp reads ctx_len)");
+  if (!aligned(kc, 16) || !aligned(vc, 16) || kv_sl % 16 || kv_sp % 16 || kv_so % 16 || kv_sh % 16)
+    return fail(SPECQ_ERR_UNSUPPORTED, "block_compact: cache rows must be 16-byte aligned");
+  const int64_t warps = static_cast<int64_t>(L) * B * 2 * H_KV;
+  if (warps > (0x7FFFFFFFll >> 5)) return fail(SPECQ_ERR_UNSUPPORTED, "block_compact: too many (layer, sequence, head) units");
+  DeviceState* dev = nullptr;
+  if (int rc = get_device_state(&dev)) return rc;
+  BlockCompactParams p = {};
+  p.kc = static_cast<uint8_t*>(kc); p.vc = static_cast<uint8_t*>(vc); p.ks = ks; p.vs = vs; p.bt = bt; p.ctx = ctx;
+  p.accept = accept; p.n_accept = n_accept; p.ctx_out = ctx_out; p.status = dev->status;
+  p.kv_sl = kv_sl; p.kv_sp = kv_sp; p.kv_so = kv_so; p.kv_sh = kv_sh;
+  p.s_sl = s_sl; p.s_sp = s_sp; p.s_sh = s_sh; p.bt_sb = bt_sb; p.acc_sb = acc_sb;
+  p.L = L; p.B = B; p.h_kv = H_KV; p.q_len = q_len; p.acc_cols = acc_cols;
+  p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
+  p.n_pages = n_pages; p.bt_cols = bt_cols;
+  const dim3 grid(static_cast<unsigned>((warps + kCompactThreads / 32 - 1) / (kCompactThreads / 32)));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (cache_dtype == SPECQ_CACHE_INT8)
+    e = D == 64 ? launch_plain(block_compact_kernel<64, 0>, grid, dim3(kCompactThreads), st, p)
+                : launch_plain(block_compact_kernel<128, 0>, grid, dim3(kCompactThreads), st, p);
+  else
+    e = D == 64 ? launch_plain(block_compact_kernel<64, 1>, grid, dim3(kCompactThreads), st, p)
+                : launch_plain(block_compact_kernel<128, 1>, grid, dim3(kCompactThreads), st, p);
+  SPECQ_CUDA_TRY(e);
+  return SPECQ_OK;
+}
+
+}  // namespace specq

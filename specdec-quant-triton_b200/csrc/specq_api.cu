@@ -12,6 +12,10 @@
 #include "rowops.cuh"
 #include "mma_peak.cuh"
 #include "peer_gather.cuh"
+#include "rope.cuh"
+#include "block_cache.cuh"
+#include "block_attn.cuh"
+#include "pages.cuh"
 
 namespace specq {
 
@@ -495,6 +499,79 @@ int specq_pack_int4(const void* w, int w_dtype, int64_t ldw, int N, int K, int g
   last_launch_ref() = LaunchRecord();
   return run_pack_int4(w, w_dtype, ldw, N, K, group, wp, ldwp, sc, ldsc, deq, lddeq, stream);
 }
+
+int specq_rope(const void* x, int64_t xt, int64_t xh, void* out, int64_t ot, int64_t oh, int dtype, const int32_t*
+               pos, const float* table, int n_pos, int T, int H, int D, int rot, int layout, int inverse, const
+               int32_t* plan, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_rope(x, xt, xh, out, ot, oh, dtype, pos, table, n_pos, T, H, D, rot, layout, inverse, plan, stream);
+}
+
+int specq_block_append(const void* k, int64_t kt, int64_t kh, const void* v, int64_t vt, int64_t vh, const void* q,
+                       int64_t qt, int64_t qh, void* q_out, int64_t ot, int64_t oh, int dtype, const float* table,
+                       int n_pos, int rot, int layout, const int32_t* pos, void* kc, void* vc, int64_t kv_sp,
+                       int64_t kv_so, int64_t kv_sh, int cache_dtype, int n_pages, float* ks, float* vs, int64_t
+                       s_sp, int64_t s_sh, const int32_t* block_tbl, int64_t bt_sb, int bt_cols, const int32_t*
+                       ctx_len, const int32_t* plan, int B, int n_seqs, int q_len, int ql_max, int H, int H_KV, int
+                       D, int page, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_block_append(k, kt, kh, v, vt, vh, q, qt, qh, q_out, ot, oh, dtype, table, n_pos, rot, layout, pos, kc,
+                          vc, kv_sp, kv_so, kv_sh, cache_dtype, n_pages, ks, vs, s_sp, s_sh, block_tbl, bt_sb,
+                          bt_cols, ctx_len, plan, B, n_seqs, q_len, ql_max, H, H_KV, D, page, stream);
+}
+
+int specq_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, const void* kc, const
+                          void* vc, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int cache_dtype, int n_pages, const
+                          float* ks, const float* vs, int64_t s_sp, int64_t s_sh, const int32_t* block_tbl, int64_t
+                          bt_sb, int bt_cols, const int32_t* ctx_len, const uint64_t* tree, int64_t tree_sb, int64_t
+                          tree_st, float sm_scale, void* out, int64_t o_sb, int64_t o_st, int64_t o_sh, const
+                          int32_t* plan, int B, int n_seqs, int q_len, int ql_max, int H, int H_KV, int D, int page,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_block_attention(q, q_sb, q_st, q_sh, dtype, kc, vc, kv_sp, kv_so, kv_sh, cache_dtype, n_pages, ks, vs,
+                             s_sp, s_sh, block_tbl, bt_sb, bt_cols, ctx_len, tree, tree_sb, tree_st, sm_scale, out,
+                             o_sb, o_st, o_sh, plan, B, n_seqs, q_len, ql_max, H, H_KV, D, page, workspace,
+                             workspace_bytes, stream);
+}
+
+int specq_block_attention_workspace(int B, int n_seqs, int q_len, int ql_max, int H, int H_KV, int D, int page, int
+                                    bt_cols, int plan, int64_t* bytes) {
+  last_launch_ref() = LaunchRecord();
+  return run_block_attention_workspace(B, n_seqs, q_len, ql_max, H, H_KV, D, page, bt_cols, plan, bytes);
+}
+
+int specq_block_compact(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int
+                        cache_dtype, int L, int n_pages, float* ks, float* vs, int64_t s_sl, int64_t s_sp, int64_t
+                        s_sh, const int32_t* block_tbl, int64_t bt_sb, int bt_cols, const int32_t* ctx_len, const
+                        int32_t* accept, int64_t acc_sb, int acc_cols, const int32_t* n_accept, int32_t* ctx_out,
+                        int B, int q_len, int H_KV, int D, int page, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_block_compact(kc, vc, kv_sl, kv_sp, kv_so, kv_sh, cache_dtype, L, n_pages, ks, vs, s_sl, s_sp, s_sh,
+                           block_tbl, bt_sb, bt_cols, ctx_len, accept, acc_sb, acc_cols, n_accept, ctx_out, B,
+                           q_len, H_KV, D, page, stream);
+}
+
+int specq_pages_release(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C, const uint8_t*
+                        drop, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_pages_release(ref, P, tbl, ld, held, S, C, drop, stream);
+}
+
+int specq_pages_reserve(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C, const int32_t*
+                        want, int page, int32_t* short_out, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_pages_reserve(ref, P, tbl, ld, held, S, C, want, page, short_out, stream);
+}
+
+int specq_pages_fork(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int L, float*
+                     ks, float* vs, int64_t s_sl, int64_t s_sp, int64_t s_sh, int32_t* ref, int P, int32_t* tbl,
+                     int64_t ld, int32_t* held, int S, int C, const int32_t* parent, const int32_t* length, int32_t*
+                     scratch, int32_t* short_out, int H_KV, int D, int page, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_pages_fork(kc, vc, kv_sl, kv_sp, kv_so, kv_sh, L, ks, vs, s_sl, s_sp, s_sh, ref, P, tbl, ld, held, S,
+                        C, parent, length, scratch, short_out, H_KV, D, page, stream);
+}
+
 
 int specq_kernel_info(int which, int variant, int* num_regs, int* local_bytes, int* static_smem, int* dynamic_smem,
                       int* max_threads) {

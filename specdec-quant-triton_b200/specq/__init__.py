@@ -9,6 +9,8 @@ import torch
 
 from . import _lib
 from . import fixtures
+from .blocks import (kv_append_blocks, kv_compact_blocks, paged_attention_blocks, pages_fork, pages_release,
+                     pages_reserve, rope, rope_table)
 from .fixtures import make_paged_kv, paged_attention_ref, quantize_weight_int8
 from .ops import (QUANT_PLAIN, QUANT_RESIDUAL, QUANT_SILU_MUL, KernelHandle, _paged_attn_kernel, _w4a16_kernel,
                   _w8a8_kernel, kv_append, pack_int4, paged_attention, paged_attention_packed, quant_rows,
@@ -51,4 +53,6 @@ __all__ = [
     "quantize_act_int8", "quantize_weight_int8", "quantize_weight_int4", "make_paged_kv", "paged_attention_ref",
     "KernelHandle", "get_status", "SpecqError",
     "quant_rows", "kv_append", "pack_int4", "fixtures", "paged_attention_packed", "QUANT_PLAIN", "QUANT_RESIDUAL", "QUANT_SILU_MUL",
+    "rope", "rope_table", "kv_append_blocks", "paged_attention_blocks", "kv_compact_blocks", "pages_release",
+    "pages_reserve", "pages_fork",
 ]

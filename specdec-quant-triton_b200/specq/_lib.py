@@ -24,9 +24,18 @@ SPECQ_STATUS_TIMEOUT_MMA = 0x02
 SPECQ_STATUS_TIMEOUT_TEST = 0x04
 SPECQ_STATUS_TIMEOUT_PEER = 0x08
 SPECQ_STATUS_PLAN_CLAMPED = 0x100
+SPECQ_STATUS_KV_NONFINITE = 0x200
+SPECQ_STATUS_BAD_INDEX = 0x400
 
 SPECQ_DTYPE_F16 = 0
 SPECQ_DTYPE_F32 = 1
+SPECQ_DTYPE_BF16 = 2
+
+SPECQ_CACHE_INT8 = 0
+SPECQ_CACHE_E4M3 = 1
+
+SPECQ_ROPE_HALF = 0
+SPECQ_ROPE_INTERLEAVED = 1
 
 _i32, _i64, _u64, _vp = C.c_int, C.c_int64, C.c_uint64, C.c_void_p
 _pi32 = C.POINTER(C.c_int)
@@ -58,6 +67,22 @@ SIGNATURES = {
                                _vp]),
     "specq_quant_rows_peer": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp,
                                      _i32, _i32, _vp]),
+    "specq_rope": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                    _vp, _vp]),
+    "specq_block_append": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i32,
+                    _i32, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp, _i64, _i64, _vp, _i64, _i32,
+                    _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "specq_block_attention": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _vp,
+                    _i64, _i64, _vp, _i64, _i32, _vp, _vp, _i64, _i64, C.c_float, _vp, _i64, _i64, _i64, _vp, _i32,
+                    _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "specq_block_attention_workspace": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                    C.POINTER(C.c_int64)]),
+    "specq_block_compact": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _i64, _i64,
+                    _vp, _i64, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "specq_pages_release": (_i32, [_vp, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp]),
+    "specq_pages_reserve": (_i32, [_vp, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _i32, _vp, _vp]),
+    "specq_pages_fork": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _vp,
+                    _i64, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
     "specq_trace_configure": (_i32, [_vp, _i32]),
 }
 
