@@ -52,6 +52,8 @@ constexpr int kBAWarps = kBAThreads / 32;
 constexpr int kBATok = 16;              // tokens of a warp's tile
 constexpr int kBAMaxStages = 8;
 constexpr float kBARaise = 8.f;         // log2 of how far p may pass 1 before the maximum is raised
+constexpr float kBANone = -1e30f;        // the running maximum of a row that has seen no token: finite, so that a
+                                         // masked score, -inf, less it is -inf and not NaN
 constexpr float kBALeastV = 8.077935669463161e-28f;   // 2^-90: a smaller V scale reads as this
 
 struct BlockAttnParams {
@@ -222,27 +224,359 @@ __device__ __forceinline__ int64_t ba_out_at(const BlockAttnParams& p, const BAL
   return b * p.o_sb + tok * p.o_st + static_cast<int64_t>(h * p.group + g) * p.o_sh;
 }
 
-template <int D, int NT, int RG>
-constexpr int ba_merge_bytes() { return (kBAWarps / RG) * (RG * NT * 8) * (D + 12) * 4; }
+// One block's view of the segment it works on.
+struct BASeg {
+  int b, h, row_lo;        // sequence, KV head, first row of the chunk
+  int ctx, old;            // tokens; tokens before the drafts (every row sees them)
+  int ta, tb, nt;          // tiles of this piece, tiles of the segment
+};
+
+// A group's place in its ring, carried from segment to segment.
+struct BARing {
+  uint64_t* full;          // [stages]
+  uint64_t* empty;
+  uint8_t* base;
+  int get, put;            // next stage to read, to fill
+  uint32_t get_ph, put_ph; // their phases
+  bool ok;                 // no wait has run out
+};
+
+// One warp's part of a segment: its rows (NT groups of 8 from row lr0 of the chunk, nts of them
+// in use), its group's tokens; leaves its part of O in the merge buffer, m and l beside it.
+template <int D, int CT, int NT, int RG>
+__device__ __forceinline__ void ba_segment(const BlockAttnParams& p, const CUtensorMap& mk, const CUtensorMap& mv,
+                                           const BALine& a, const BASeg& sg, BARing& ring, int tg, int rg, int lr0, int nts,
+                                           float* sm_m, float* sm_l, float* merge) {
+  constexpr int TG = kBAWarps / RG;
+  constexpr int KC = D / 16;                 // 16-byte pieces of a token
+  constexpr int KB = kBATok * D;             // bytes of a K (or V) tile
+  constexpr int PITCH = D + 12;              // of the merge buffer, in floats: its stores hit each bank once
+  const int lane = static_cast<int>(threadIdx.x & 31);
+  const int gq = lane >> 2, tq = lane & 3;
+  const int stages = p.stages;
+
+  // ---- boxes: box e of the group's tile i (page 8: two boxes a tile) and their registers
+  const int two = p.page_log2 == 3 ? 1 : 0;
+  const int first_tok = sg.ta * p.tile + tg * kBATok;
+  int n_tiles = sg.tb - sg.ta;                                 // of this group, those with a token
+  if (n_tiles > 0 && first_tok + (n_tiles - 1) * p.tile >= sg.ctx) --n_tiles;
+  const int boxes = n_tiles << two;
+  const int32_t* bt = p.bt + sg.b * p.bt_sb;
+  int pg_c = 0, pg_n = 0;
+  float ck_c = 0.f, lv_c = 0.f, iv_c = 0.f, ck_n = 0.f, lv_n = 0.f, iv_n = 0.f;
+  auto load_batch = [&](int e0, int& pg, float& ck, float& lv, float& iv) {
+    const int e = e0 + lane;
+    pg = 0;
+    ck = 1e-37f; lv = -INFINITY; iv = 0.f;     // a box that is not there weighs nothing
+    if (e < boxes) {
+      const int tok = first_tok + (e >> two) * p.tile + (two ? (e & 1) * 8 : 0);
+      if (tok < sg.ctx) {
+        const int x = __ldg(bt + (tok >> p.page_log2));
+        if (x >= 0 && x < p.n_pages) {
+          pg = x;
+          const int64_t at = static_cast<int64_t>(x) * p.s_sp + sg.h * p.s_sh;
+          ck = __ldg(p.ks + at) * p.scale_log2;
+          if (ck < 1e-37f) ck = 1e-37f;        // a masked score, -inf, times it stays -inf
+          float v = __ldg(p.vs + at);
+          v = v < kBALeastV ? kBALeastV : v;
+          lv = __log2f(v);
+          iv = 1.f / v;
+        } else {
+          report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+        }
+      }
+    }
+  };
+  load_batch(0, pg_c, ck_c, lv_c, iv_c);
+  load_batch(32, pg_n, ck_n, lv_n, iv_n);
+  int batch0 = 0;                                              // first box of the current batch
+
+  auto issue = [&](int i) {                                    // tile i into the next stage (rg 0's warp)
+    const int e = i << two;
+    const int pg = e - batch0 < 32 ? pg_c : pg_n;
+    const int p0 = __shfl_sync(0xffffffffu, pg, e & 31);
+    const int p1 = two ? __shfl_sync(0xffffffffu, pg, (e + 1) & 31) : 0;
+    if (RG > 1)
+      ring.ok = ring.ok && mbar_wait(&ring.empty[ring.put], ring.put_ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+    if (lane == 0 && ring.ok) {
+      uint8_t* d = ring.base + ring.put * 2 * KB;
+      uint64_t* bar = &ring.full[ring.put];
+      const int slot = two ? 0 : (first_tok + i * p.tile) & ((1 << p.page_log2) - 1);
+      mbar_arrive_expect_tx(bar, 2 * KB);
+      tma_box(d, &mk, bar, sg.h, slot, p0);
+      tma_box(d + KB, &mv, bar, sg.h, slot, p0);
+      if (two) {
+        tma_box(d + KB / 2, &mk, bar, sg.h, 0, p1);
+        tma_box(d + KB + KB / 2, &mv, bar, sg.h, 0, p1);
+      }
+    }
+    __syncwarp();
+    if (++ring.put == stages) {
+      ring.put = 0;
+      ring.put_ph ^= 1u;
+    }
+  };
+  if (rg == 0)
+    for (int i = 0; i < min(stages - 1, n_tiles); ++i) issue(i);
+
+  // ---- Q^T as the B operand: thread (gq, tq) holds row gq of each group, d = 16 c + 4 tq + 0..3
+  uint32_t qf[NT][KC][2];
+  float fac = 1.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const int lr = lr0 + n * 8 + gq;
+    const int rr = sg.row_lo + lr;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) qf[n][c][0] = qf[n][c][1] = 0u;
+    if (n < nts && lr < a.chunk_rows && rr < a.q_rows) {
+      const int qi = rr / p.group, g = rr - qi * p.group;
+      const int64_t tok = p.q_sb == 0 ? static_cast<int64_t>(sg.b) * a.q_len + qi : qi;
+      const int64_t off = sg.b * p.q_sb + tok * p.q_st + static_cast<int64_t>(sg.h * p.group + g) * p.q_sh;
+      const uint2* src = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + off + 4 * tq);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint2 w = __ldg(src + 4 * c);
+        qf[n][c][0] = w.x;
+        qf[n][c][1] = w.y;
+      }
+    }
+  }
+  if (p.bf16) {
+    // to fp16 under one power of two that brings the warp's largest to [1, 2): bf16's 8 bits are
+    // exact down to 2^-17 of it, and what is smaller is off by 2^-25 of it at most
+    float top = 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(qf[n][c][i] << 16)), fabsf(__uint_as_float(qf[n][c][i] & 0xffff0000u))));
+    top = warp_max_f32(top);
+    const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+    fac = __uint_as_float(ex << 23);
+    const float inv = __uint_as_float((254u - ex) << 23);
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const __half2 y = __floats2half2_rn(__uint_as_float(qf[n][c][i] << 16) * inv,
+                                              __uint_as_float(qf[n][c][i] & 0xffff0000u) * inv);
+          qf[n][c][i] = *reinterpret_cast<const uint32_t*>(&y);
+        }
+  }
+
+  float o[KC][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = kBANone;
+    l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
+  }
+  // this lane's ldmatrix row: matrix lane / 8 = (token half, piece), swizzled as the box was stored
+  const int mr = (lane & 7) + ((lane >> 3) & 1) * 8, mc = lane >> 4;
+  const uint32_t row_off = static_cast<uint32_t>(mr * D + ((mc ^ (D == 128 ? (mr & 7) : ((mr >> 1) & 3))) << 4));
+  const uint32_t ring_s = smem_u32(ring.base) + row_off;
+
+  for (int i = 0; i < n_tiles; ++i) {
+    const int e = (i << two) & 31;
+    if (e == 0 && i > 0) {                                      // the next batch of boxes
+      batch0 += 32;
+      pg_c = pg_n; ck_c = ck_n; lv_c = lv_n; iv_c = iv_n;
+      load_batch(batch0 + 32, pg_n, ck_n, lv_n, iv_n);
+    }
+    if (rg == 0 && i + stages - 1 < n_tiles) issue(i + stages - 1);
+    const int s = ring.get;
+    ring.ok = ring.ok && mbar_wait(&ring.full[s], ring.get_ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+    if (++ring.get == stages) {
+      ring.get = 0;
+      ring.get_ph ^= 1u;
+    }
+    const uint32_t kt = ring_s + static_cast<uint32_t>(s * 2 * KB), vt = kt + KB;
+
+    // S^T = K Q^T
+    float sc[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < KC; c += 2) {
+      uint32_t r[4];
+      ldsm4(kt ^ static_cast<uint32_t>(c << 4), r);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t l0, h0, l1, h1;
+        widen4<CT, false>(r[2 * hf], l0, h0);
+        widen4<CT, false>(r[2 * hf + 1], l1, h1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(sc[n], l0, l1, h0, h1, qf[n][c + hf][0], qf[n][c + hf][1]);
+      }
+    }
+
+    // softmax of the tile: rows 2 tq, 2 tq + 1 of each group, tokens gq and gq + 8
+    const float ck = __shfl_sync(0xffffffffu, ck_c, e) * fac;
+    const float lv = __shfl_sync(0xffffffffu, lv_c, e);
+    const float iv = __shfl_sync(0xffffffffu, iv_c, e);
+    float lv1 = lv, iv_rel = 1.f;                               // tokens 8 .. 15: the same page, or
+    if (two) {                                                  // another one with its own scales
+      const float ck1 = __shfl_sync(0xffffffffu, ck_c, e + 1) * fac;
+      lv1 = __shfl_sync(0xffffffffu, lv_c, e + 1);
+      const float iv1 = __shfl_sync(0xffffffffu, iv_c, e + 1);
+      const float rel = ck1 / ck;
+      iv_rel = iv > 0.f ? iv1 / iv : 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        sc[n][2] *= rel;
+        sc[n][3] *= rel;
+      }
+    }
+    const int t0 = first_tok + i * p.tile;
+    if (t0 + kBATok > sg.old) {                                 // some row may not see some token
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int rr = sg.row_lo + lr0 + n * 8 + 2 * tq + r;
+          const int qi = rr / p.group;
+          if (p.tree == nullptr) {
+            const int lim = min(sg.ctx, sg.old + qi + 1);
+            if (t0 + gq >= lim) sc[n][r] = -INFINITY;
+            if (t0 + gq + 8 >= lim) sc[n][2 + r] = -INFINITY;
+          } else {
+            const uint64_t word = qi < a.q_len ? __ldg(reinterpret_cast<const unsigned long long*>(p.tree) + sg.b * p.tree_sb + qi * p.tree_st) : 0ull;
+            const int j0 = t0 + gq - sg.old, j1 = j0 + 8;
+            if (j0 >= a.q_len || (j0 >= 0 && ((word >> (j0 & 63)) & 1ull) == 0ull)) sc[n][r] = -INFINITY;
+            if (j1 >= a.q_len || (j1 >= 0 && ((word >> (j1 & 63)) & 1ull) == 0ull)) sc[n][2 + r] = -INFINITY;
+          }
+        }
+      if (CT == 1 && t0 + kBATok > sg.ctx) {
+        // slots past the last token may hold anything, NaN bytes too: their V reads as 0
+        uint8_t* v = ring.base + s * 2 * KB + KB;
+        for (int x = max(sg.ctx - t0, 0) * KC + lane; x < kBATok * KC; x += 32) *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();                               // before the stage is filled again
+        __syncwarp();
+      }
+    }
+    // x - m in log2 units, x = score + log2(sV)
+    float y[NT][4], top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        y[n][r] = fmaf(sc[n][r], ck, lv - m[n][r]);
+        y[n][2 + r] = fmaf(sc[n][2 + r], ck, lv1 - m[n][r]);
+        top = fmaxf(top, fmaxf(y[n][r], y[n][2 + r]));
+      }
+    if (__any_sync(0xffffffffu, top > kBARaise)) {              // raise the maxima and what they scale
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float x0 = fmaf(sc[n][r], ck, lv), x1 = fmaf(sc[n][2 + r], ck, lv1);
+          float v = fmaxf(x0, x1);
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+          const float mn = fmaxf(m[n][r], v);
+          const float f = ex2(m[n][r] - mn);
+          m[n][r] = mn;
+          l[n][r] *= f;
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            o[c][n][r] *= f;
+            o[c][n][2 + r] *= f;
+          }
+          y[n][r] = x0 - mn;
+          y[n][2 + r] = x1 - mn;
+        }
+    }
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        y[n][r] = ex2(y[n][r]);
+        y[n][2 + r] = ex2(y[n][2 + r]);
+        l[n][r] = fmaf(fmaf(y[n][2 + r], iv_rel, y[n][r]), iv, l[n][r]);
+      }
+      const __half2 h0 = __floats2half2_rn(y[n][0], y[n][1]), h1 = __floats2half2_rn(y[n][2], y[n][3]);
+      pb[n][0] = movm_t(*reinterpret_cast<const uint32_t*>(&h0));
+      pb[n][1] = movm_t(*reinterpret_cast<const uint32_t*>(&h1));
+    }
+
+    // O^T += V^T P^T
+#pragma unroll
+    for (int c = 0; c < KC; c += 2) {
+      uint32_t r[4];
+      ldsm4_t(vt ^ static_cast<uint32_t>(c << 4), r);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t e0, d0, e1, d1;
+        widen4<CT, true>(r[2 * hf], e0, d0);
+        widen4<CT, true>(r[2 * hf + 1], e1, d1);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(o[c + hf][n], e0, d0, e1, d1, pb[n][0], pb[n][1]);
+      }
+    }
+    __syncwarp();                                               // every lane has read the stage
+    if (RG > 1 && lane == 0) mbar_arrive(&ring.empty[s]);
+  }
+
+  // ---- this warp's part of the join
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float v = l[n][r];
+      v += __shfl_xor_sync(0xffffffffu, v, 4);
+      v += __shfl_xor_sync(0xffffffffu, v, 8);
+      v += __shfl_xor_sync(0xffffffffu, v, 16);
+      const int lr = lr0 + n * 8 + 2 * tq + r;
+      if (gq == 0 && n < nts) {
+        sm_m[tg * p.rows + lr] = m[n][r];
+        sm_l[tg * p.rows + lr] = v;
+      }
+    }
+  named_barrier_sync(1, kBAThreads);                            // also: every group is done with the ring
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+    if (n < nts) {
+      float f[2];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const int lr = lr0 + n * 8 + 2 * tq + r;
+        float top = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < TG; ++t) top = fmaxf(top, sm_m[t * p.rows + lr]);
+        f[r] = ex2(m[n][r] - top);
+      }
+      float* d0 = merge + (tg * p.rows + lr0 + n * 8 + 2 * tq) * PITCH + 2 * gq;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        *reinterpret_cast<float2*>(d0 + 16 * c) = make_float2(o[c][n][0] * f[0], o[c][n][2] * f[0]);
+        *reinterpret_cast<float2*>(d0 + PITCH + 16 * c) = make_float2(o[c][n][1] * f[1], o[c][n][3] * f[1]);
+      }
+    }
+}
 
 template <int D, int CT, int NT, int RG>
 __global__ void __launch_bounds__(kBAThreads, NT == 1 ? 2 : 1)
 block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_constant__ CUtensorMap mk,
                   const __grid_constant__ CUtensorMap mv) {
   constexpr int TG = kBAWarps / RG;          // groups of warps with tokens of their own
-  constexpr int KC = D / 16;                 // 16-byte pieces of a token
-  constexpr int KB = kBATok * D;             // bytes of a K (or V) tile
+  constexpr int KB = kBATok * D;
   constexpr int ROWS = RG * NT * 8;
-  constexpr int PITCH = D + 12;              // of the merge buffer, in floats: its stores hit each bank once
+  constexpr int PITCH = D + 12;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ float sm_m[TG][ROWS], sm_l[TG][ROWS];
+  __shared__ float sm_m[TG * ROWS], sm_l[TG * ROWS];
   __shared__ __align__(8) uint64_t full[TG][kBAMaxStages], empty[TG][kBAMaxStages];
-  uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float* merge = reinterpret_cast<float*>(ring);
+  uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* merge = reinterpret_cast<float*>(base);
 
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   const int tg = warp % TG, rg = warp / TG;
-  const int gq = lane >> 2, tq = lane & 3;
   const int stages = p.stages;
   if (threadIdx.x == 0) {
     for (int t = 0; t < TG; ++t)
@@ -259,330 +593,45 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
 
   const BALine a = ba_line(p, blockIdx.x == 0 && warp == 0);
   const int64_t u0 = a.total * blockIdx.x / p.grid, u1 = a.total * (blockIdx.x + 1) / p.grid;
-  bool ok = true;
-  uint32_t cnt = 0;                          // tiles this group has consumed (stage and phase)
-  uint8_t* my_ring = ring + tg * stages * 2 * KB;
-  const uint32_t my_ring_s = smem_u32(my_ring);
-
-  int b = 0;
+  BARing ring = {full[tg], empty[tg], base + tg * stages * 2 * KB, 0, 0, 0u, 0u, true};
+  BASeg sg = {};
   int64_t seq_begin = 0;
-  if (u0 < u1) b = ba_find(p, a, u0, &seq_begin);
+  if (u0 < u1) sg.b = ba_find(p, a, u0, &seq_begin);
   for (int64_t u = u0; u < u1;) {
-    const int ctx = ba_ctx(p, b);
-    const int nt = ba_tiles(p, ctx);
+    sg.ctx = ba_ctx(p, sg.b);
+    sg.old = sg.ctx - a.q_len;
+    sg.nt = ba_tiles(p, sg.ctx);
     const int in_seq = static_cast<int>(u - seq_begin);
-    const int hr = in_seq / nt, ta = in_seq - hr * nt;       // (KV head, row chunk), first tile
-    const int h = hr / a.rc, rc = hr - h * a.rc;
-    const int64_t seg_begin = u - ta;
-    const int tb = static_cast<int>(min(static_cast<int64_t>(nt), u1 - seg_begin));
+    const int hr = in_seq / sg.nt;                             // (KV head, row chunk)
+    sg.ta = in_seq - hr * sg.nt;
+    sg.h = hr / a.rc;
+    sg.row_lo = (hr - sg.h * a.rc) * a.chunk_rows;
+    const int64_t seg_begin = u - sg.ta;
+    sg.tb = static_cast<int>(min(static_cast<int64_t>(sg.nt), u1 - seg_begin));
 
-    // ---- rows of this warp: groups of 8 dealt evenly over the RG warps
-    const int row_lo = rc * a.chunk_rows;
-    const int groups = min(a.chunk_rows, a.q_rows - row_lo + 7) >> 3;
-    const int nts = RG == 1 ? groups : groups / RG + (rg < groups % RG ? 1 : 0);
-    const int lr0 = RG == 1 ? 0 : 8 * (rg * (groups / RG) + min(rg, groups % RG));   // first row in the chunk
-
-    // ---- boxes: box e of the group's tile i (page 8: two boxes a tile) and their registers
-    const int two = p.page_log2 == 3 ? 1 : 0;
-    const int first_tok = ta * p.tile + tg * kBATok;
-    int n_tiles = tb - ta;                                     // of this group, those with a token
-    if (n_tiles > 0 && first_tok + (n_tiles - 1) * p.tile >= ctx) --n_tiles;
-    const int boxes = n_tiles << two;
-    const int32_t* bt = p.bt + b * p.bt_sb;
-    int pg_c = 0, pg_n = 0;
-    float ck_c = 0.f, lv_c = 0.f, iv_c = 0.f, ck_n = 0.f, lv_n = 0.f, iv_n = 0.f;
-    auto load_batch = [&](int e0, int& pg, float& ck, float& lv, float& iv) {
-      const int e = e0 + lane;
-      pg = 0;
-      ck = 0.f; lv = -INFINITY; iv = 0.f;      // a box that is not there weighs nothing
-      if (e < boxes) {
-        const int tok = first_tok + (e >> two) * p.tile + (two ? (e & 1) * 8 : 0);
-        if (tok < ctx) {
-          const int x = __ldg(bt + (tok >> p.page_log2));
-          if (x >= 0 && x < p.n_pages) {
-            pg = x;
-            const int64_t at = static_cast<int64_t>(x) * p.s_sp + h * p.s_sh;
-            ck = __ldg(p.ks + at) * p.scale_log2;
-            float v = __ldg(p.vs + at);
-            v = v < kBALeastV ? kBALeastV : v;
-            lv = __log2f(v);
-            iv = 1.f / v;
-          } else {
-            report_status(p.status, SPECQ_STATUS_BAD_INDEX);
-          }
-        }
-      }
-    };
-    load_batch(0, pg_c, ck_c, lv_c, iv_c);
-    load_batch(32, pg_n, ck_n, lv_n, iv_n);
-    int batch0 = 0;                                            // first box of the current batch
-
-    auto issue = [&](int i) {                                  // tile i into its stage (rg 0's warp)
-      const uint32_t c = cnt + static_cast<uint32_t>(i);       // cnt: the count at the segment's tile 0
-      const int s = static_cast<int>(c % static_cast<uint32_t>(stages));
-      const uint32_t lap = c / static_cast<uint32_t>(stages);
-      const int e = i << two;
-      const int p0 = __shfl_sync(0xffffffffu, e - batch0 < 32 ? pg_c : pg_n, e & 31);
-      const int p1 = __shfl_sync(0xffffffffu, e - batch0 < 32 ? pg_c : pg_n, (e + two) & 31);
-      if (RG > 1 && lap > 0u) ok = ok && mbar_wait(&empty[tg][s], (lap - 1u) & 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-      if (lane == 0 && ok) {
-        uint8_t* d = my_ring + s * 2 * KB;
-        const int slot = (first_tok + i * p.tile) & ((1 << p.page_log2) - 1);
-        mbar_arrive_expect_tx(&full[tg][s], 2 * KB);
-        tma_box(d, &mk, &full[tg][s], h, two ? 0 : slot, p0);
-        tma_box(d + KB, &mv, &full[tg][s], h, two ? 0 : slot, p0);
-        if (two) {
-          tma_box(d + KB / 2, &mk, &full[tg][s], h, 0, p1);
-          tma_box(d + KB + KB / 2, &mv, &full[tg][s], h, 0, p1);
-        }
-      }
-      __syncwarp();
-    };
-    if (rg == 0)
-      for (int i = 0; i < min(stages - 1, n_tiles); ++i) issue(i);
-
-    // ---- Q^T as the B operand: thread (gq, tq) holds row gq of each group, d = 16 c + 4 tq + 0..3
-    uint32_t qf[NT][KC][2];
-    float fac[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int lr = lr0 + n * 8 + gq;
-      const int rr = row_lo + lr;
-      float f = 1.f;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) qf[n][c][0] = qf[n][c][1] = 0u;
-      if (n < nts && lr < a.chunk_rows && rr < a.q_rows) {
-        const int qi = rr / p.group, g = rr - qi * p.group;
-        const int64_t tok = p.q_sb == 0 ? static_cast<int64_t>(b) * a.q_len + qi : qi;
-        const int64_t off = b * p.q_sb + tok * p.q_st + static_cast<int64_t>(h * p.group + g) * p.q_sh;
-        const uint2* src = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + off + 4 * tq);
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const uint2 w = __ldg(src + 4 * c);
-          qf[n][c][0] = w.x;
-          qf[n][c][1] = w.y;
-        }
-      }
-      if (p.bf16) {     // to fp16 under a power of two that brings the row's largest to [1, 4)
-        float top = 0.f;
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(qf[n][c][i] << 16)), fabsf(__uint_as_float(qf[n][c][i] & 0xffff0000u))));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-        f = __uint_as_float(ex << 23);
-        const float inv = __uint_as_float((254u - ex) << 23);
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const __half2 y = __floats2half2_rn(__uint_as_float(qf[n][c][i] << 16) * inv,
-                                                __uint_as_float(qf[n][c][i] & 0xffff0000u) * inv);
-            qf[n][c][i] = *reinterpret_cast<const uint32_t*>(&y);
-          }
-      }
-      // the accumulator's columns: rows 2 tq and 2 tq + 1
-      fac[n][0] = __shfl_sync(0xffffffffu, f, 8 * tq);
-      fac[n][1] = __shfl_sync(0xffffffffu, f, 8 * tq + 4);
-    }
-
-    float o[KC][NT][4], m[NT][2], l[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      m[n][0] = m[n][1] = -INFINITY;
-      l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
-    }
-    const int old = ctx - a.q_len;                              // tokens before the drafts: every row sees them
-
-    for (int i = 0; i < n_tiles; ++i) {
-      if (((i << two) & 31) == 0 && i > 0) {                    // the next batch of boxes
-        batch0 += 32;
-        pg_c = pg_n; ck_c = ck_n; lv_c = lv_n; iv_c = iv_n;
-        load_batch(batch0 + 32, pg_n, ck_n, lv_n, iv_n);
-      }
-      if (rg == 0 && i + stages - 1 < n_tiles) issue(i + stages - 1);
-      const uint32_t c0 = cnt + static_cast<uint32_t>(i);
-      const int s = static_cast<int>(c0 % static_cast<uint32_t>(stages));
-      ok = ok && mbar_wait(&full[tg][s], (c0 / static_cast<uint32_t>(stages)) & 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-      const uint32_t kt = my_ring_s + s * 2 * KB, vt = kt + KB;
-
-      // S^T = K Q^T
-      float sc[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-      // the row of this lane's ldmatrix address: matrix lane / 8 = (token half, piece)
-      const int mr = (lane & 7) + ((lane >> 3) & 1) * 8, mc = lane >> 4;
-      auto at = [&](uint32_t tile, int c) {                     // swizzled address of piece c of token mr
-        const int x = D == 128 ? (mr & 7) : ((mr >> 1) & 3);
-        return tile + static_cast<uint32_t>(mr * D + ((c ^ x) << 4));
-      };
-#pragma unroll
-      for (int c = 0; c < KC; c += 2) {
-        uint32_t r[4];
-        ldsm4(at(kt, c + mc), r);
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t l0, h0, l1, h1;
-          widen4<CT, false>(r[2 * hf], l0, h0);
-          widen4<CT, false>(r[2 * hf + 1], l1, h1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            if (n < nts) mma16816(sc[n], l0, l1, h0, h1, qf[n][c + hf][0], qf[n][c + hf][1]);
-        }
-      }
-
-      // softmax of the tile: rows 2 tq, 2 tq + 1 of each group, tokens gq and gq + 8
-      const int e = (i << two) & 31;
-      const float ck0 = __shfl_sync(0xffffffffu, ck_c, e), ck1 = __shfl_sync(0xffffffffu, ck_c, e + two);
-      const float lv0 = __shfl_sync(0xffffffffu, lv_c, e), lv1 = __shfl_sync(0xffffffffu, lv_c, e + two);
-      const float iv0 = __shfl_sync(0xffffffffu, iv_c, e), iv1 = __shfl_sync(0xffffffffu, iv_c, e + two);
-      const int t0 = first_tok + i * p.tile;
-      const bool edge = t0 + kBATok > old;                      // some row may not see some token
-      if (edge) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const int rr = row_lo + lr0 + n * 8 + 2 * tq + r;
-            const int qi = rr / p.group;
-            if (p.tree == nullptr) {
-              const int lim = min(ctx, old + qi + 1);
-              if (t0 + gq >= lim) sc[n][r] = -INFINITY;
-              if (t0 + gq + 8 >= lim) sc[n][2 + r] = -INFINITY;
-            } else {
-              const uint64_t word = qi < a.q_len ? __ldg(reinterpret_cast<const unsigned long long*>(p.tree) + b * p.tree_sb + qi * p.tree_st) : 0ull;
-              const int j0 = t0 + gq - old, j1 = j0 + 8;
-              if (j0 >= a.q_len || (j0 >= 0 && ((word >> (j0 & 63)) & 1ull) == 0ull)) sc[n][r] = -INFINITY;
-              if (j1 >= a.q_len || (j1 >= 0 && ((word >> (j1 & 63)) & 1ull) == 0ull)) sc[n][2 + r] = -INFINITY;
-            }
-          }
-      }
-      // x = score in log2 units + log2(sV); a masked score stays -inf (ck > 0 or the box is absent)
-      float top = -INFINITY;
-      float x[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float a0 = sc[n][r], a1 = sc[n][2 + r];
-          x[n][r] = a0 == -INFINITY ? -INFINITY : fmaf(a0, ck0 * fac[n][r], lv0);
-          x[n][2 + r] = a1 == -INFINITY ? -INFINITY : fmaf(a1, ck1 * fac[n][r], lv1);
-          if (n < nts) top = fmaxf(top, fmaxf(x[n][r], x[n][2 + r]) - m[n][r]);
-        }
-      if (__any_sync(0xffffffffu, top > kBARaise)) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float v = fmaxf(x[n][r], x[n][2 + r]);
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-            const float mn = fmaxf(m[n][r], v);
-            const float f = mn == m[n][r] ? 1.f : ex2(m[n][r] - mn);   // -inf before the first: 0
-            m[n][r] = mn;
-            l[n][r] *= f;
-#pragma unroll
-            for (int c = 0; c < KC; ++c) {
-              o[c][n][r] *= f;
-              o[c][n][2 + r] *= f;
-            }
-          }
-      }
-      uint32_t pb[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float y[4];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float mm = m[n][r] == -INFINITY ? 0.f : m[n][r];
-          y[r] = ex2(x[n][r] - mm);
-          y[2 + r] = ex2(x[n][2 + r] - mm);
-          l[n][r] += fmaf(y[r], iv0, y[2 + r] * iv1);
-        }
-        const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
-        pb[n][0] = movm_t(*reinterpret_cast<const uint32_t*>(&h0));
-        pb[n][1] = movm_t(*reinterpret_cast<const uint32_t*>(&h1));
-      }
-
-      // O^T += V^T P^T; slots past the last token may hold anything: they read as 0
-      const bool tail = t0 + kBATok > ctx;
-      uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;
-      if (tail) {
-        const int t = t0 + 2 * tq;
-        keep0 = (t < ctx ? 0xffffu : 0u) | (t + 1 < ctx ? 0xffff0000u : 0u);
-        keep1 = (t + 8 < ctx ? 0xffffu : 0u) | (t + 9 < ctx ? 0xffff0000u : 0u);
-      }
-#pragma unroll
-      for (int c = 0; c < KC; c += 2) {
-        uint32_t r[4];
-        ldsm4_t(at(vt, c + mc), r);
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t e0, d0, e1, d1;
-          widen4<CT, true>(r[2 * hf] & keep0, e0, d0);
-          widen4<CT, true>(r[2 * hf + 1] & keep1, e1, d1);
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            if (n < nts) mma16816(o[c + hf][n], e0, d0, e1, d1, pb[n][0], pb[n][1]);
-        }
-      }
-      __syncwarp();                                             // every lane has read the stage
-      if (RG > 1 && lane == 0) mbar_arrive(&empty[tg][s]);
-    }
-    cnt += static_cast<uint32_t>(n_tiles);
-
-    // ---- join the groups' parts
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float v = l[n][r];
-        v += __shfl_xor_sync(0xffffffffu, v, 4);
-        v += __shfl_xor_sync(0xffffffffu, v, 8);
-        v += __shfl_xor_sync(0xffffffffu, v, 16);
-        const int lr = lr0 + n * 8 + 2 * tq + r;
-        if (gq == 0 && n < nts) {
-          sm_m[tg][lr] = m[n][r];
-          sm_l[tg][lr] = v;
-        }
-      }
-    __syncthreads();                                            // also: every group is done with the ring
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-      if (n < nts) {
-        float f[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int lr = lr0 + n * 8 + 2 * tq + r;
-          float top = -INFINITY;
-#pragma unroll
-          for (int t = 0; t < TG; ++t) top = fmaxf(top, sm_m[t][lr]);
-          f[r] = m[n][r] == -INFINITY ? 0.f : ex2(m[n][r] - top);
-        }
-        float* d0 = merge + (tg * ROWS + lr0 + n * 8 + 2 * tq) * PITCH + 2 * gq;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          *reinterpret_cast<float2*>(d0 + 16 * c) = make_float2(o[c][n][0] * f[0], o[c][n][2] * f[0]);
-          *reinterpret_cast<float2*>(d0 + PITCH + 16 * c) = make_float2(o[c][n][1] * f[1], o[c][n][3] * f[1]);
-        }
-      }
+    // rows of this warp: groups of 8 dealt evenly over the RG warps, so NT or NT - 1 (fewer only
+    // under a plan whose q_len is below the largest: the spare groups then compute on zeros)
+    const int groups = min(a.chunk_rows, a.q_rows - sg.row_lo + 7) >> 3;
+    const int nts = groups / RG + (rg < groups % RG ? 1 : 0);
+    const int lr0 = 8 * (rg * (groups / RG) + min(rg, groups % RG));
+    if (NT == 1 || RG == 1 || nts == NT)
+      ba_segment<D, CT, NT, RG>(p, mk, mv, a, sg, ring, tg, rg, lr0, nts, sm_m, sm_l, merge);
+    else
+      ba_segment<D, CT, NT == 1 ? 1 : NT - 1, RG>(p, mk, mv, a, sg, ring, tg, rg, lr0, nts, sm_m, sm_l, merge);
     __syncthreads();
-    const bool whole = ta == 0 && tb == nt;
-    const int slot = 2 * static_cast<int>(blockIdx.x) + (ta == 0 ? 1 : 0);
-    const int live = min(a.chunk_rows, a.q_rows - row_lo);
+
+    const bool whole = sg.ta == 0 && sg.tb == sg.nt;
+    const int slot = 2 * static_cast<int>(blockIdx.x) + (sg.ta == 0 ? 1 : 0);
+    const int live = min(a.chunk_rows, a.q_rows - sg.row_lo);
     for (int x = static_cast<int>(threadIdx.x); x < live * (D / 4); x += kBAThreads) {
       const int lr = x / (D / 4), d = (x - lr * (D / 4)) * 4;
       float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int t = 0; t < TG; ++t) top = fmaxf(top, sm_m[t][lr]);
+      for (int t = 0; t < TG; ++t) top = fmaxf(top, sm_m[t * ROWS + lr]);
 #pragma unroll
-      for (int t = 0; t < TG; ++t) sum += sm_m[t][lr] == -INFINITY ? 0.f : ex2(sm_m[t][lr] - top) * sm_l[t][lr];
+      for (int t = 0; t < TG; ++t) {
+        sum += ex2(sm_m[t * ROWS + lr] - top) * sm_l[t * ROWS + lr];
+      }
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int t = 0; t < TG; ++t) {
@@ -591,7 +640,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       }
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        ba_store(p, ba_out_at(p, a, b, h, row_lo + lr) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+        ba_store(p, ba_out_at(p, a, sg.b, sg.h, sg.row_lo + lr) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
       } else {
         *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * ROWS + lr) * D + d) = v;
         if (d == 0)
@@ -601,14 +650,14 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     fence_proxy_async_smem();                                   // the merge buffer becomes a TMA target again
     __syncthreads();
 
-    u = seg_begin + tb;
-    if (hr + 1 == p.h_kv * a.rc && tb == nt) {
+    u = seg_begin + sg.tb;
+    if (hr + 1 == p.h_kv * a.rc && sg.tb == sg.nt) {
       seq_begin = u;
-      ++b;
+      ++sg.b;
     }
   }
   pdl_launch_dependents();
-  if (!ok && rg == 0 && lane == 0) {   // a wait ran out: leave no copy of this block in flight
+  if (!ring.ok && rg == 0 && lane == 0) {   // a wait ran out: leave no copy of this block in flight
     for (int s = 0; s < stages; ++s) {
       (void)mbar_wait(&full[tg][s], 0u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
       (void)mbar_wait(&full[tg][s], 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
@@ -656,7 +705,6 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
     if (empty_piece(c)) continue;
     const int64_t at = static_cast<int64_t>(slot_of(c)) * p.rows + lr;
     const float2 ml = __ldg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
-    if (ml.x == -INFINITY) continue;
     const float f = ex2(ml.x - top);
     sum += f * ml.y;
     const float* src = p.part_o + at * D + lane * V;
@@ -780,6 +828,7 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
                                int H_KV, int D, int page, void* workspace, int64_t workspace_bytes, void* stream) {
   if (int rc = check_block_attn_sizes(B, n_seqs, q_len, ql_max, H, H_KV, D, page, bt_cols, plan != nullptr)) return rc;
   if (dtype != 0 && dtype != 2) return fail(SPECQ_ERR_INVALID_ARG, "block_attention: query dtype code %d", dtype);
+  if (!(sm_scale > 0.f)) return fail(SPECQ_ERR_INVALID_ARG, "block_attention: sm_scale %g must be positive", sm_scale);
   if (cache_dtype != SPECQ_CACHE_INT8 && cache_dtype != SPECQ_CACHE_E4M3)
     return fail(SPECQ_ERR_INVALID_ARG, "block_attention: cache dtype code %d", cache_dtype);
   const int bg = plan ? B : n_seqs, ql = plan ? ql_max : q_len;

@@ -270,6 +270,8 @@ def paged_attention_blocks(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=None, tr
         raise ValueError(f"{name}: out must be {q.dtype} {tuple(q.shape)}, got {out.dtype} {tuple(out.shape)}")
     if q.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError(f"{name}: q and out need unit stride along D")
+    if sm_scale is not None and not sm_scale > 0:
+        raise ValueError(f"{name}: sm_scale={sm_scale} must be positive")
     if tree is not None:
         if tree.dtype != torch.int64 or tree.dim() != 2 or tree.shape[0] < B or tree.shape[1] < ql_max:
             raise ValueError(f"{name}: tree must be int64 [>= {B}, >= {ql_max}], got {tree.dtype} {tuple(tree.shape)}")
