@@ -14,23 +14,28 @@
 // products accumulate in fp32.  m lags: p may reach 2^8 before the running maximum is raised
 // (one warp vote a tile), which fp16 holds without loss.
 //
-// Tile.  A warp owns 16 tokens at a time and up to 24 query rows, and works alone:
-//   S^T [16 tokens x rows] = K Q^T      mma.m16n8k16, K converted 8 -> 16 bits in registers
-//   P^T = 2^(S^T - m)                   in the accumulator's registers
-//   O^T [D x rows] += V^T P^T           P^T turned by movmatrix, V by a transposing ldmatrix
-// Rows are the N side of both products, so they pad to 8 and not to 16 or 128.  Everything
-// but the 8-bit tiles stays in registers; no barrier joins the warps inside the loop.  Tiles
-// arrive by TMA (one box of 16 slots of a page for K, one for V) in a ring of its own for each
-// group of warps that shares tokens; the lane that issues takes page numbers from a register
-// file of the next 32 boxes, loaded a batch ahead with their scales.  Groups of more than 24
-// rows split their rows over 2 or 4 warps that read the same ring; rows beyond 96 go to other
-// blocks, which find the pages in L2.
+// Tile.  A tile is 128 tokens (64 up to 16 rows) and up to 40 query rows, worked on by a group of four warps; a
+// block has two groups, which take tiles in turn, each with its own running maxima, so that one
+// group's exponentials overlap the other's products.  Within a group
+//   S^T [tokens x rows] = K Q^T         each warp its own quarter of the tokens; Q^T stays in registers, K is
+//                                       converted 8 -> 16 bits in registers, once
+//   P^T = 2^(S^T - m)                   in the accumulator's registers, turned by movmatrix and
+//                                       left in shared memory as the fragments the next step reads
+//   O^T [D x rows] += V^T P^T           each warp its own quarter of the D elements over all of
+//                                       the tokens; V by a transposing ldmatrix, converted once
+// so O costs 8 registers for 8 rows (D = 128), and a segment ends with a sum of two halves.  Two
+// barriers of the group a tile: one carries the vote that raises the running maxima, one joins
+// the products.  Rows are the N side of both products and pad to 8.  Feeding warps walk the same
+// segments ahead of the others: they read page numbers and scales, start the TMA boxes (up to 64
+// slots of a page) into a ring and copy the next queries, so a new segment finds its first tiles
+// in shared memory.
 //
-// Why mma.sync: a 16-token tile is 16 x 8n x 128 twice, 16 n instructions.  The warp-level
-// tensor pipe makes one every 2 cycles an SM (measured; 1024 multiply-adds a cycle), so one
-// token costs 2 n cycles an SM for 8 n rows, against the 11.6 cycles in which HBM delivers its
-// 256 bytes: up to 5 groups of 8 rows stay below the memory time, without the round trips
-// through tensor memory and the block-wide hand-overs of a tcgen05 pipeline.
+// Why mma.sync: a 16-token tile of 8n rows is 16 n instructions, and the warp-level tensor pipe
+// takes one every 2 cycles an SM (measured; 1024 multiply-adds a cycle): 2 n cycles a token,
+// against the 11.6 in which HBM delivers its 256 bytes.  Up to n = 5 the products fit under the
+// memory time, and rows cost what they are: the tcgen05 tile would be 128 tokens x 16n padded rows
+// at 64-76 cycles an instruction, with round trips through tensor memory between the steps.
+// More than 40 rows go to several blocks, which find the pages in L2.
 //
 // Work.  The tiles of all (sequence, KV head, row chunk) segments form one line, cut into equal
 // pieces, one for each resident block, whatever the sequences' lengths; each block finds its
@@ -47,9 +52,20 @@
 
 namespace specq {
 
-constexpr int kBAThreads = 256;
-constexpr int kBAWarps = kBAThreads / 32;
-constexpr int kBATok = 16;              // tokens of a warp's tile
+constexpr int kBAGroupWarps = 4;                  // of a group
+constexpr int kBAWarps = 2 * kBAGroupWarps;       // that compute
+constexpr int kBACompute = 32 * kBAWarps;
+// And those that feed them.  A box costs its warp some 90 cycles to start, so a block that has an
+// SM to itself has four.  The registers of an SM's quarter divide among whole warps: from 3 row
+// groups on the block launches 12 warps of 168 and splits their 64,512 as 224 for the computing
+// ones (8 x 32 x 224) and 56 for the feeding ones (4 x 32 x 56).
+__host__ __device__ constexpr bool ba_split(int nt) { return nt >= 3; }
+__host__ __device__ constexpr int ba_feeders(int nt) { return ba_split(nt) ? 4 : 1; }
+__host__ __device__ constexpr int ba_threads(int nt) { return kBACompute + 32 * ba_feeders(nt); }
+// Tokens of a tile: up to 16 rows two blocks share an SM, and half as many tokens leave each a ring
+// of six stages.
+__host__ __device__ constexpr int ba_tile(int nt) { return ba_split(nt) ? 128 : 64; }
+constexpr int kBAMaxGroups = 5;                   // groups of 8 query rows a block holds at most
 constexpr int kBAMaxStages = 8;
 constexpr float kBARaise = 8.f;         // log2 of how far p may pass 1 before the maximum is raised
 constexpr float kBANone = -1e30f;        // the running maximum of a row that has seen no token: finite, so that a
@@ -71,7 +87,9 @@ struct BlockAttnParams {
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, s_sp, s_sh, bt_sb, tree_sb, tree_st;
   float scale_log2;         // sm_scale * log2(e)
   int n_seqs, q_len, b_max, ql_max, h_kv, group, page_log2, n_pages, bt_cols;
-  int bf16, stages, grid, rows, tile;   // rows: of a block's chunk; tile: tokens of a block's tile
+  int bf16, stages, grid, rows, box;    // rows: of a block's chunk; box: slots of a TMA box
+  int tile;                             // tokens of a tile
+  uint32_t group_magic;                 // ceil(2^32 / group), for group > 1
 };
 
 __device__ __forceinline__ void tma_box(void* dst, const CUtensorMap* map, uint64_t* bar, int head, int slot, int page) {
@@ -135,11 +153,23 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   }
 }
 
-// Where the segments of a call lie on the line of tiles.
+// qi of query row rr = qi * group + g (rr * group < 2^32)
+__device__ __forceinline__ int ba_token(const BlockAttnParams& p, int rr) {
+  return p.group == 1 ? rr : static_cast<int>(__umulhi(static_cast<uint32_t>(rr), p.group_magic));
+}
+
+// Where the segments of a call lie on the line of tiles.  Piece c of the line (one a block) is
+// [start(c), start(c + 1)): the first `more` pieces have one tile more than the others.
 struct BALine {
   int n_seqs, q_len, q_rows, rc;   // rc: row chunks of a (sequence, KV head)
   int chunk_rows;                  // rows of a chunk (a multiple of 8)
-  int64_t total;                   // tiles in all
+  int total;                       // tiles in all
+  int each, more;
+  __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
+  __device__ __forceinline__ int piece_of(int u) const {
+    const int wide = more * (each + 1);
+    return u < wide ? u / (each + 1) : more + (u - wide) / each;   // each > 0 past the wide ones
+  }
 };
 
 __device__ __forceinline__ int ba_ctx(const BlockAttnParams& p, int b) {
@@ -158,11 +188,7 @@ __device__ __forceinline__ BALine ba_line(const BlockAttnParams& p, bool tell) {
     a.q_len = min(max(q, 0), p.ql_max);
     if (tell && (n != a.n_seqs || q != a.q_len)) report_status(p.status, SPECQ_STATUS_PLAN_CLAMPED);
   }
-  a.q_rows = a.q_len * p.group;
-  const int groups = (a.q_rows + 7) >> 3;
-  a.rc = (groups * 8 + p.rows - 1) / p.rows;
-  a.chunk_rows = a.rc > 0 ? (groups + a.rc - 1) / a.rc * 8 : 0;
-  int64_t t = 0;
+  int t = 0;
   const int lane = static_cast<int>(threadIdx.x & 31);
   for (int b0 = 0; b0 < a.n_seqs; b0 += 32) {
     const int b = b0 + lane;
@@ -174,52 +200,50 @@ __device__ __forceinline__ BALine ba_line(const BlockAttnParams& p, bool tell) {
     }
     t += __reduce_add_sync(0xffffffffu, n);
   }
+  a.q_rows = a.q_len * p.group;
+  const int groups = (a.q_rows + 7) >> 3;
+  a.rc = (groups * 8 + p.rows - 1) / p.rows;
+  a.chunk_rows = a.rc > 0 ? (groups + a.rc - 1) / a.rc * 8 : 0;
   a.total = t * (p.h_kv * a.rc);
+  a.each = a.total / p.grid;
+  a.more = a.total - a.each * p.grid;
   return a;
 }
 
 // The sequence that holds line position u (every lane of the warp calls), and where it begins.
-__device__ __forceinline__ int ba_find(const BlockAttnParams& p, const BALine& a, int64_t u, int64_t* begin) {
+__device__ __forceinline__ int ba_find(const BlockAttnParams& p, const BALine& a, int u, int* begin) {
   const int lane = static_cast<int>(threadIdx.x & 31);
   const int per = p.h_kv * a.rc;
-  int64_t at = 0;
+  int at = 0;
   for (int b0 = 0; b0 < a.n_seqs; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < a.n_seqs ? ba_tiles(p, ba_ctx(p, b)) : 0;
+    const int n = b < a.n_seqs ? ba_tiles(p, ba_ctx(p, b)) * per : 0;
     int inc = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, inc, d);
       if (lane >= d) inc += up;
     }
-    const int64_t end = at + static_cast<int64_t>(inc) * per;
-    const unsigned over = __ballot_sync(0xffffffffu, b < a.n_seqs && end > u);
+    const unsigned over = __ballot_sync(0xffffffffu, b < a.n_seqs && at + inc > u);
     if (over != 0u) {
       const int first = __ffs(over) - 1;
-      *begin = at + static_cast<int64_t>(__shfl_sync(0xffffffffu, inc - n, first)) * per;
+      *begin = at + __shfl_sync(0xffffffffu, inc - n, first);
       return b0 + first;
     }
-    at += static_cast<int64_t>(__shfl_sync(0xffffffffu, inc, 31)) * per;
+    at += __shfl_sync(0xffffffffu, inc, 31);
   }
   *begin = at;
   return a.n_seqs;
 }
 
-__device__ __forceinline__ void ba_store(const BlockAttnParams& p, int64_t off, float a, float b, float c, float d) {
-  if (p.bf16) {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(a, b), y = __floats2bfloat162_rn(c, d);
-    *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + off) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-  } else {
-    const __half2 x = __floats2half2_rn(a, b), y = __floats2half2_rn(c, d);
-    *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + off) =
-        make_uint2(*reinterpret_cast<const uint32_t*>(&x), *reinterpret_cast<const uint32_t*>(&y));
-  }
+__device__ __forceinline__ void ba_store2(const BlockAttnParams& p, int64_t off, float a, float b) {
+  if (p.bf16) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + off) = __floats2bfloat162_rn(a, b);
+  else *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + off) = __floats2half2_rn(a, b);
 }
 
 // Row rr of (sequence b, KV head h) in out, in elements.  o_sb = 0: packed token rows.
 __device__ __forceinline__ int64_t ba_out_at(const BlockAttnParams& p, const BALine& a, int b, int h, int rr) {
-  const int qi = rr / p.group, g = rr - qi * p.group;
+  const int qi = ba_token(p, rr), g = rr - qi * p.group;
   const int64_t tok = p.o_sb == 0 ? static_cast<int64_t>(b) * a.q_len + qi : qi;
   return b * p.o_sb + tok * p.o_st + static_cast<int64_t>(h * p.group + g) * p.o_sh;
 }
@@ -231,438 +255,528 @@ struct BASeg {
   int ta, tb, nt;          // tiles of this piece, tiles of the segment
 };
 
-// A group's place in its ring, carried from segment to segment.
-struct BARing {
-  uint64_t* full;          // [stages]
-  uint64_t* empty;
-  uint8_t* base;
-  int get, put;            // next stage to read, to fill
-  uint32_t get_ph, put_ph; // their phases
-  bool ok;                 // no wait has run out
+// The segments of a block's piece [u, u1) of the line, in order.
+struct BAWalk {
+  int u, u1, seq_begin, b;
+  __device__ __forceinline__ void start(const BlockAttnParams& p, const BALine& a) {
+    u = a.start(static_cast<int>(blockIdx.x));
+    u1 = a.start(static_cast<int>(blockIdx.x) + 1);
+    seq_begin = 0;
+    b = u < u1 ? ba_find(p, a, u, &seq_begin) : 0;
+  }
+  __device__ __forceinline__ bool next(const BlockAttnParams& p, const BALine& a, BASeg& s) {
+    if (u >= u1) return false;
+    s.b = b;
+    s.ctx = ba_ctx(p, b);
+    s.old = s.ctx - a.q_len;
+    s.nt = ba_tiles(p, s.ctx);
+    const int in_seq = u - seq_begin;
+    const int hr = in_seq / s.nt;                              // (KV head, row chunk)
+    s.ta = in_seq - hr * s.nt;
+    s.h = hr / a.rc;
+    s.row_lo = (hr - s.h * a.rc) * a.chunk_rows;
+    s.tb = min(s.nt, u1 - u + s.ta);
+    u += s.tb - s.ta;
+    if (s.tb == s.nt && hr + 1 == p.h_kv * a.rc) {
+      seq_begin = u;
+      ++b;
+    }
+    return true;
+  }
 };
 
-// One warp's part of a segment: its rows (NT groups of 8 from row lr0 of the chunk, nts of them
-// in use), its group's tokens; leaves its part of O in the merge buffer, m and l beside it.
-template <int D, int CT, int NT, int RG>
-__device__ __forceinline__ void ba_segment(const BlockAttnParams& p, const CUtensorMap& mk, const CUtensorMap& mv,
-                                           const BALine& a, const BASeg& sg, BARing& ring, int tg, int rg, int lr0, int nts,
-                                           float* sm_m, float* sm_l, float* merge) {
-  constexpr int TG = kBAWarps / RG;
-  constexpr int KC = D / 16;                 // 16-byte pieces of a token
-  constexpr int KB = kBATok * D;             // bytes of a K (or V) tile
-  constexpr int PITCH = D + 12;              // of the merge buffer, in floats: its stores hit each bank once
-  const int lane = static_cast<int>(threadIdx.x & 31);
-  const int gq = lane >> 2, tq = lane & 3;
-  const int stages = p.stages;
-
-  // ---- boxes: box e of the group's tile i (page 8: two boxes a tile) and their registers
-  const int two = p.page_log2 == 3 ? 1 : 0;
-  const int first_tok = sg.ta * p.tile + tg * kBATok;
-  int n_tiles = sg.tb - sg.ta;                                 // of this group, those with a token
-  if (n_tiles > 0 && first_tok + (n_tiles - 1) * p.tile >= sg.ctx) --n_tiles;
-  const int boxes = n_tiles << two;
-  const int32_t* bt = p.bt + sg.b * p.bt_sb;
-  int pg_c = 0, pg_n = 0;
-  float ck_c = 0.f, lv_c = 0.f, iv_c = 0.f, ck_n = 0.f, lv_n = 0.f, iv_n = 0.f;
-  auto load_batch = [&](int e0, int& pg, float& ck, float& lv, float& iv) {
-    const int e = e0 + lane;
-    pg = 0;
-    ck = 1e-37f; lv = -INFINITY; iv = 0.f;     // a box that is not there weighs nothing
-    if (e < boxes) {
-      const int tok = first_tok + (e >> two) * p.tile + (two ? (e & 1) * 8 : 0);
-      if (tok < sg.ctx) {
-        const int x = __ldg(bt + (tok >> p.page_log2));
-        if (x >= 0 && x < p.n_pages) {
-          pg = x;
-          const int64_t at = static_cast<int64_t>(x) * p.s_sp + sg.h * p.s_sh;
-          ck = __ldg(p.ks + at) * p.scale_log2;
-          if (ck < 1e-37f) ck = 1e-37f;        // a masked score, -inf, times it stays -inf
-          float v = __ldg(p.vs + at);
-          v = v < kBALeastV ? kBALeastV : v;
-          lv = __log2f(v);
-          iv = 1.f / v;
-        } else {
-          report_status(p.status, SPECQ_STATUS_BAD_INDEX);
-        }
-      }
-    }
-  };
-  load_batch(0, pg_c, ck_c, lv_c, iv_c);
-  load_batch(32, pg_n, ck_n, lv_n, iv_n);
-  int batch0 = 0;                                              // first box of the current batch
-
-  auto issue = [&](int i) {                                    // tile i into the next stage (rg 0's warp)
-    const int e = i << two;
-    const int pg = e - batch0 < 32 ? pg_c : pg_n;
-    const int p0 = __shfl_sync(0xffffffffu, pg, e & 31);
-    const int p1 = two ? __shfl_sync(0xffffffffu, pg, (e + 1) & 31) : 0;
-    if (RG > 1)
-      ring.ok = ring.ok && mbar_wait(&ring.empty[ring.put], ring.put_ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-    if (lane == 0 && ring.ok) {
-      uint8_t* d = ring.base + ring.put * 2 * KB;
-      uint64_t* bar = &ring.full[ring.put];
-      const int slot = two ? 0 : (first_tok + i * p.tile) & ((1 << p.page_log2) - 1);
-      mbar_arrive_expect_tx(bar, 2 * KB);
-      tma_box(d, &mk, bar, sg.h, slot, p0);
-      tma_box(d + KB, &mv, bar, sg.h, slot, p0);
-      if (two) {
-        tma_box(d + KB / 2, &mk, bar, sg.h, 0, p1);
-        tma_box(d + KB + KB / 2, &mv, bar, sg.h, 0, p1);
-      }
-    }
-    __syncwarp();
-    if (++ring.put == stages) {
-      ring.put = 0;
-      ring.put_ph ^= 1u;
-    }
-  };
-  if (rg == 0)
-    for (int i = 0; i < min(stages - 1, n_tiles); ++i) issue(i);
-
-  // ---- Q^T as the B operand: thread (gq, tq) holds row gq of each group, d = 16 c + 4 tq + 0..3
-  uint32_t qf[NT][KC][2];
-  float fac = 1.f;
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int lr = lr0 + n * 8 + gq;
-    const int rr = sg.row_lo + lr;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) qf[n][c][0] = qf[n][c][1] = 0u;
-    if (n < nts && lr < a.chunk_rows && rr < a.q_rows) {
-      const int qi = rr / p.group, g = rr - qi * p.group;
-      const int64_t tok = p.q_sb == 0 ? static_cast<int64_t>(sg.b) * a.q_len + qi : qi;
-      const int64_t off = sg.b * p.q_sb + tok * p.q_st + static_cast<int64_t>(sg.h * p.group + g) * p.q_sh;
-      const uint2* src = reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.q) + off + 4 * tq);
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const uint2 w = __ldg(src + 4 * c);
-        qf[n][c][0] = w.x;
-        qf[n][c][1] = w.y;
-      }
+// A place in the ring of stages.  The number of stages is a multiple of 2 and of the feeding warps, and
+// tile n of a piece goes to group n % 2 and comes from warp n % feeders: so a stage has one reader and
+// one writer for good.  (With others in between, a waiter would not see every phase of a barrier,
+// and a parity would name two.)
+struct BAPlace {
+  int s;
+  uint32_t ph;
+  __device__ __forceinline__ void step(int stages) {
+    if (++s == stages) {
+      s = 0;
+      ph ^= 1u;
     }
   }
-  if (p.bf16) {
-    // to fp16 under one power of two that brings the warp's largest to [1, 2): bf16's 8 bits are
-    // exact down to 2^-17 of it, and what is smaller is off by 2^-25 of it at most
-    float top = 0.f;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(qf[n][c][i] << 16)), fabsf(__uint_as_float(qf[n][c][i] & 0xffff0000u))));
-    top = warp_max_f32(top);
-    const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-    fac = __uint_as_float(ex << 23);
-    const float inv = __uint_as_float((254u - ex) << 23);
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const __half2 y = __floats2half2_rn(__uint_as_float(qf[n][c][i] << 16) * inv,
-                                              __uint_as_float(qf[n][c][i] & 0xffff0000u) * inv);
-          qf[n][c][i] = *reinterpret_cast<const uint32_t*>(&y);
-        }
-  }
+};
 
-  float o[KC][NT][4], m[NT][2], l[NT][2];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = kBANone;
-    l[n][0] = l[n][1] = 0.f;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
-  }
-  // this lane's ldmatrix row: matrix lane / 8 = (token half, piece), swizzled as the box was stored
-  const int mr = (lane & 7) + ((lane >> 3) & 1) * 8, mc = lane >> 4;
-  const uint32_t row_off = static_cast<uint32_t>(mr * D + ((mc ^ (D == 128 ? (mr & 7) : ((mr >> 1) & 3))) << 4));
-  const uint32_t ring_s = smem_u32(ring.base) + row_off;
-
-  for (int i = 0; i < n_tiles; ++i) {
-    const int e = (i << two) & 31;
-    if (e == 0 && i > 0) {                                      // the next batch of boxes
-      batch0 += 32;
-      pg_c = pg_n; ck_c = ck_n; lv_c = lv_n; iv_c = iv_n;
-      load_batch(batch0 + 32, pg_n, ck_n, lv_n, iv_n);
-    }
-    if (rg == 0 && i + stages - 1 < n_tiles) issue(i + stages - 1);
-    const int s = ring.get;
-    ring.ok = ring.ok && mbar_wait(&ring.full[s], ring.get_ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-    if (++ring.get == stages) {
-      ring.get = 0;
-      ring.get_ph ^= 1u;
-    }
-    const uint32_t kt = ring_s + static_cast<uint32_t>(s * 2 * KB), vt = kt + KB;
-
-    // S^T = K Q^T
-    float sc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-    for (int c = 0; c < KC; c += 2) {
-      uint32_t r[4];
-      ldsm4(kt ^ static_cast<uint32_t>(c << 4), r);
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t l0, h0, l1, h1;
-        widen4<CT, false>(r[2 * hf], l0, h0);
-        widen4<CT, false>(r[2 * hf + 1], l1, h1);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816(sc[n], l0, l1, h0, h1, qf[n][c + hf][0], qf[n][c + hf][1]);
-      }
-    }
-
-    // softmax of the tile: rows 2 tq, 2 tq + 1 of each group, tokens gq and gq + 8
-    const float ck = __shfl_sync(0xffffffffu, ck_c, e) * fac;
-    const float lv = __shfl_sync(0xffffffffu, lv_c, e);
-    const float iv = __shfl_sync(0xffffffffu, iv_c, e);
-    float lv1 = lv, iv_rel = 1.f;                               // tokens 8 .. 15: the same page, or
-    if (two) {                                                  // another one with its own scales
-      const float ck1 = __shfl_sync(0xffffffffu, ck_c, e + 1) * fac;
-      lv1 = __shfl_sync(0xffffffffu, lv_c, e + 1);
-      const float iv1 = __shfl_sync(0xffffffffu, iv_c, e + 1);
-      const float rel = ck1 / ck;
-      iv_rel = iv > 0.f ? iv1 / iv : 0.f;
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        sc[n][2] *= rel;
-        sc[n][3] *= rel;
-      }
-    }
-    const int t0 = first_tok + i * p.tile;
-    if (t0 + kBATok > sg.old) {                                 // some row may not see some token
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int rr = sg.row_lo + lr0 + n * 8 + 2 * tq + r;
-          const int qi = rr / p.group;
-          if (p.tree == nullptr) {
-            const int lim = min(sg.ctx, sg.old + qi + 1);
-            if (t0 + gq >= lim) sc[n][r] = -INFINITY;
-            if (t0 + gq + 8 >= lim) sc[n][2 + r] = -INFINITY;
-          } else {
-            const uint64_t word = qi < a.q_len ? __ldg(reinterpret_cast<const unsigned long long*>(p.tree) + sg.b * p.tree_sb + qi * p.tree_st) : 0ull;
-            const int j0 = t0 + gq - sg.old, j1 = j0 + 8;
-            if (j0 >= a.q_len || (j0 >= 0 && ((word >> (j0 & 63)) & 1ull) == 0ull)) sc[n][r] = -INFINITY;
-            if (j1 >= a.q_len || (j1 >= 0 && ((word >> (j1 & 63)) & 1ull) == 0ull)) sc[n][2 + r] = -INFINITY;
-          }
-        }
-      if (CT == 1 && t0 + kBATok > sg.ctx) {
-        // slots past the last token may hold anything, NaN bytes too: their V reads as 0
-        uint8_t* v = ring.base + s * 2 * KB + KB;
-        for (int x = max(sg.ctx - t0, 0) * KC + lane; x < kBATok * KC; x += 32) *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async_smem();                               // before the stage is filled again
-        __syncwarp();
-      }
-    }
-    // x - m in log2 units, x = score + log2(sV)
-    float y[NT][4], top = -INFINITY;
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        y[n][r] = fmaf(sc[n][r], ck, lv - m[n][r]);
-        y[n][2 + r] = fmaf(sc[n][2 + r], ck, lv1 - m[n][r]);
-        top = fmaxf(top, fmaxf(y[n][r], y[n][2 + r]));
-      }
-    if (__any_sync(0xffffffffu, top > kBARaise)) {              // raise the maxima and what they scale
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float x0 = fmaf(sc[n][r], ck, lv), x1 = fmaf(sc[n][2 + r], ck, lv1);
-          float v = fmaxf(x0, x1);
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-          v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-          const float mn = fmaxf(m[n][r], v);
-          const float f = ex2(m[n][r] - mn);
-          m[n][r] = mn;
-          l[n][r] *= f;
-#pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            o[c][n][r] *= f;
-            o[c][n][2 + r] *= f;
-          }
-          y[n][r] = x0 - mn;
-          y[n][2 + r] = x1 - mn;
-        }
-    }
-    uint32_t pb[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        y[n][r] = ex2(y[n][r]);
-        y[n][2 + r] = ex2(y[n][2 + r]);
-        l[n][r] = fmaf(fmaf(y[n][2 + r], iv_rel, y[n][r]), iv, l[n][r]);
-      }
-      const __half2 h0 = __floats2half2_rn(y[n][0], y[n][1]), h1 = __floats2half2_rn(y[n][2], y[n][3]);
-      pb[n][0] = movm_t(*reinterpret_cast<const uint32_t*>(&h0));
-      pb[n][1] = movm_t(*reinterpret_cast<const uint32_t*>(&h1));
-    }
-
-    // O^T += V^T P^T
-#pragma unroll
-    for (int c = 0; c < KC; c += 2) {
-      uint32_t r[4];
-      ldsm4_t(vt ^ static_cast<uint32_t>(c << 4), r);
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t e0, d0, e1, d1;
-        widen4<CT, true>(r[2 * hf], e0, d0);
-        widen4<CT, true>(r[2 * hf + 1], e1, d1);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma16816(o[c + hf][n], e0, d0, e1, d1, pb[n][0], pb[n][1]);
-      }
-    }
-    __syncwarp();                                               // every lane has read the stage
-    if (RG > 1 && lane == 0) mbar_arrive(&ring.empty[s]);
-  }
-
-  // ---- this warp's part of the join
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float v = l[n][r];
-      v += __shfl_xor_sync(0xffffffffu, v, 4);
-      v += __shfl_xor_sync(0xffffffffu, v, 8);
-      v += __shfl_xor_sync(0xffffffffu, v, 16);
-      const int lr = lr0 + n * 8 + 2 * tq + r;
-      if (gq == 0 && n < nts) {
-        sm_m[tg * p.rows + lr] = m[n][r];
-        sm_l[tg * p.rows + lr] = v;
-      }
-    }
-  named_barrier_sync(1, kBAThreads);                            // also: every group is done with the ring
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-    if (n < nts) {
-      float f[2];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const int lr = lr0 + n * 8 + 2 * tq + r;
-        float top = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < TG; ++t) top = fmaxf(top, sm_m[t * p.rows + lr]);
-        f[r] = ex2(m[n][r] - top);
-      }
-      float* d0 = merge + (tg * p.rows + lr0 + n * 8 + 2 * tq) * PITCH + 2 * gq;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        *reinterpret_cast<float2*>(d0 + 16 * c) = make_float2(o[c][n][0] * f[0], o[c][n][2] * f[0]);
-        *reinterpret_cast<float2*>(d0 + PITCH + 16 * c) = make_float2(o[c][n][1] * f[1], o[c][n][3] * f[1]);
-      }
-    }
+// A group's barrier that also tells whether any of its threads says so.
+__device__ __forceinline__ bool ba_vote(int id, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(x ? 1u : 0u), "r"(id), "n"(32 * kBAGroupWarps)
+      : "memory");
+  return r != 0u;
 }
 
-template <int D, int CT, int NT, int RG>
-__global__ void __launch_bounds__(kBAThreads, NT == 1 ? 2 : 1)
+template <int D, int NT>
+struct BASmem {
+  static constexpr int TOK = ba_tile(NT);
+  static constexpr int U = TOK / 16 / kBAGroupWarps;           // 16 tokens that a warp multiplies with Q
+  static constexpr int MT = D / 16 / kBAGroupWarps;            // 16-element pieces of D a warp accumulates
+  static constexpr int ROWS = NT * 8;
+  static constexpr int KB = TOK * D;                       // bytes of a K (or V) tile
+  static constexpr int STAGE = 2 * KB;
+  static constexpr int P = (TOK / 16) * NT * 32 * 8;       // a tile's P^T: [16 tokens][group][lane] b0, b1
+  static constexpr int QPITCH = 2 * D + 16;
+  static constexpr int Q = ROWS * QPITCH;
+  static constexpr int SC = TOK / 8;                           // scales of a stage: ck, lv, iv for each 8 tokens
+  static constexpr int SCALES = SC * 16;
+  static constexpr int MERGE = kBAGroupWarps * MT * NT * 32 * 16;   // one group's O
+  static constexpr int fixed = 2 * P + MERGE + 2 * Q + kBAMaxStages * SCALES + 2 * kBAWarps * ROWS * 4 + 256;
+};
+
+template <int D, int CT, int NT>
+__global__ void __launch_bounds__(ba_threads(NT), ba_split(NT) ? 1 : 2)
 block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_constant__ CUtensorMap mk,
                   const __grid_constant__ CUtensorMap mv) {
-  constexpr int TG = kBAWarps / RG;          // groups of warps with tokens of their own
-  constexpr int KB = kBATok * D;
-  constexpr int ROWS = RG * NT * 8;
-  constexpr int PITCH = D + 12;
+  SPECQ_TRACE_INIT();
+  if (threadIdx.x == 0) SPECQ_TRACE_POINT(0, 0);
+  using S = BASmem<D, NT>;
+  constexpr int KC = D / 16;                 // 16-byte pieces of a token
+  constexpr int MT = S::MT, U = S::U, TOK = S::TOK, ROWS = S::ROWS, NF = ba_feeders(NT);
   extern __shared__ uint8_t smem_raw[];
-  __shared__ float sm_m[TG * ROWS], sm_l[TG * ROWS];
-  __shared__ __align__(8) uint64_t full[TG][kBAMaxStages], empty[TG][kBAMaxStages];
   uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  float* merge = reinterpret_cast<float*>(base);
+  const int stages = p.stages;
+  uint8_t* ring = base;
+  uint8_t* pbuf = ring + stages * S::STAGE;                    // one for each group
+  float4* merge = reinterpret_cast<float4*>(pbuf + 2 * S::P);
+  uint8_t* qbuf = pbuf + 2 * S::P + S::MERGE;
+  float4* scales = reinterpret_cast<float4*>(qbuf + 2 * S::Q);
+  float* sm_l = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scales) + kBAMaxStages * S::SCALES);   // [warp][row]
+  float* sm_m = sm_l + kBAWarps * ROWS;                                                                   // [warp][row]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm_m + kBAWarps * ROWS);
+  uint64_t* empty = full + kBAMaxStages;
+  uint64_t* q_full = empty + kBAMaxStages;
+  uint64_t* q_empty = q_full + 2;
 
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
-  const int tg = warp % TG, rg = warp / TG;
-  const int stages = p.stages;
   if (threadIdx.x == 0) {
-    for (int t = 0; t < TG; ++t)
-      for (int s = 0; s < stages; ++s) {
-        mbar_init(&full[t][s], 1u);
-        mbar_init(&empty[t][s], RG);
-      }
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 2u);               // the boxes' expected bytes, and the scales
+      mbar_init(&empty[s], kBAGroupWarps);   // the group that reads it
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&q_full[s], 32u * NF);
+      mbar_init(&q_empty[s], kBAWarps);
+    }
     fence_barrier_init();
     tma_prefetch_desc(&mk);
     tma_prefetch_desc(&mv);
   }
   __syncthreads();
   pdl_wait();
-
+  if (threadIdx.x == 0) SPECQ_TRACE_POINT(1, 0);
   const BALine a = ba_line(p, blockIdx.x == 0 && warp == 0);
-  const int64_t u0 = a.total * blockIdx.x / p.grid, u1 = a.total * (blockIdx.x + 1) / p.grid;
-  BARing ring = {full[tg], empty[tg], base + tg * stages * 2 * KB, 0, 0, 0u, 0u, true};
+  BAWalk walk;
+  walk.start(p, a);
+  if (threadIdx.x == 0) SPECQ_TRACE_POINT(2, 0);
   BASeg sg = {};
-  int64_t seq_begin = 0;
-  if (u0 < u1) sg.b = ba_find(p, a, u0, &seq_begin);
-  for (int64_t u = u0; u < u1;) {
-    sg.ctx = ba_ctx(p, sg.b);
-    sg.old = sg.ctx - a.q_len;
-    sg.nt = ba_tiles(p, sg.ctx);
-    const int in_seq = static_cast<int>(u - seq_begin);
-    const int hr = in_seq / sg.nt;                             // (KV head, row chunk)
-    sg.ta = in_seq - hr * sg.nt;
-    sg.h = hr / a.rc;
-    sg.row_lo = (hr - sg.h * a.rc) * a.chunk_rows;
-    const int64_t seg_begin = u - sg.ta;
-    sg.tb = static_cast<int>(min(static_cast<int64_t>(sg.nt), u1 - seg_begin));
+  BAPlace at = {0, 0u}, qat = {0, 0u};       // stage of the piece's next tile, of its next queries
+  bool ok = true;
 
-    // rows of this warp: groups of 8 dealt evenly over the RG warps, so NT or NT - 1 (fewer only
-    // under a plan whose q_len is below the largest: the spare groups then compute on zeros)
-    const int groups = min(a.chunk_rows, a.q_rows - sg.row_lo + 7) >> 3;
-    const int nts = groups / RG + (rg < groups % RG ? 1 : 0);
-    const int lr0 = 8 * (rg * (groups / RG) + min(rg, groups % RG));
-    if (NT == 1 || RG == 1 || nts == NT)
-      ba_segment<D, CT, NT, RG>(p, mk, mv, a, sg, ring, tg, rg, lr0, nts, sm_m, sm_l, merge);
-    else
-      ba_segment<D, CT, NT == 1 ? 1 : NT - 1, RG>(p, mk, mv, a, sg, ring, tg, rg, lr0, nts, sm_m, sm_l, merge);
-    __syncthreads();
-
-    const bool whole = sg.ta == 0 && sg.tb == sg.nt;
-    const int slot = 2 * static_cast<int>(blockIdx.x) + (sg.ta == 0 ? 1 : 0);
-    const int live = min(a.chunk_rows, a.q_rows - sg.row_lo);
-    for (int x = static_cast<int>(threadIdx.x); x < live * (D / 4); x += kBAThreads) {
-      const int lr = x / (D / 4), d = (x - lr * (D / 4)) * 4;
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < TG; ++t) top = fmaxf(top, sm_m[t * ROWS + lr]);
-#pragma unroll
-      for (int t = 0; t < TG; ++t) {
-        sum += ex2(sm_m[t * ROWS + lr] - top) * sm_l[t * ROWS + lr];
+  if (warp >= kBAWarps) {                    // ---- the feeding warps: warp f takes tiles f, f + NF, ... of the piece
+    if constexpr (ba_split(NT)) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    const int f = warp - kBAWarps;
+    const int nb = TOK / p.box;          // boxes of a tile; a batch of 32 is `tpb` of the warp's tiles
+    const int tpb = 32 / nb;
+    const int lt = lane / nb, lb = lane - lt * nb;
+    int skip = f;                            // tiles of the segment before the warp's next one
+    while (walk.next(p, a, sg)) {
+      const int32_t* bt = p.bt + sg.b * p.bt_sb;
+      bool q_done = false;
+      auto copy_queries = [&]() {
+        q_done = true;
+        ok = ok && mbar_wait(&q_empty[qat.s], qat.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+        const int rows = min(a.chunk_rows, a.q_rows - sg.row_lo);
+        constexpr int CH = D / 8;            // 16-byte pieces of a query row: a lane keeps its piece
+        const int c = lane % CH;
+        for (int lr = f * (32 / CH) + lane / CH; lr < ROWS; lr += NF * (32 / CH)) {
+          uint8_t* d = qbuf + qat.s * S::Q + lr * S::QPITCH + c * 16;
+          const int rr = sg.row_lo + min(lr, rows - 1);
+          const int qi = ba_token(p, rr), g = rr - qi * p.group;
+          const int64_t row = p.q_sb == 0 ? static_cast<int64_t>(sg.b) * a.q_len + qi : qi;
+          const uint16_t* src = static_cast<const uint16_t*>(p.q) + sg.b * p.q_sb + row * p.q_st +
+                                static_cast<int64_t>(sg.h * p.group + g) * p.q_sh + c * 8;
+          // padding rows take 0 of the 16 bytes: zeros
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(d)), "l"(src), "r"(lr < rows ? 16 : 0)
+                       : "memory");
+        }
+        cp_async_mbar_arrive(&q_full[qat.s]);
+        if (lane == 0 && f == 0) SPECQ_TRACE_POINT(4, qat.s);
+        qat.step(2);
+      };
+      int t0 = sg.ta + skip;                 // the batch's first tile
+      int pg = -1, tok = 0;
+      auto load_pages = [&]() {
+        const int t = t0 + lt * NF;
+        tok = t * TOK + lb * p.box;
+        pg = t < sg.tb && tok < sg.ctx ? __ldg(bt + (tok >> p.page_log2)) : -1;
+      };
+      load_pages();
+      int stepped = sg.ta;                   // `at` is the stage of this tile
+      for (; t0 < sg.tb;) {
+        const int my_tile = t0 + lt * NF, my_tok = tok;
+        const bool load = my_tile < sg.tb && tok < sg.ctx;
+        const bool there = pg >= 0 && pg < p.n_pages;          // a bad page reads page 0 and weighs nothing
+        if (load && !there) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+        const int page = there ? pg : 0;
+        float ks = 0.f, vs = 0.f;
+        if (there) {
+          const int64_t x = static_cast<int64_t>(page) * p.s_sp + sg.h * p.s_sh;
+          ks = __ldg(p.ks + x);
+          vs = __ldg(p.vs + x);
+        }
+        const int t1 = min(sg.tb, t0 + tpb * NF);
+        const int tb0 = t0;
+        t0 += tpb * NF;
+        if (t0 < sg.tb) load_pages();
+        for (int t = tb0; t < t1; t += NF) {
+          for (; stepped < t; ++stepped) at.step(stages);
+          ok = ok && mbar_wait(&empty[at.s], at.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+          const bool mine = t == my_tile;
+          const unsigned boxes = __ballot_sync(0xffffffffu, mine && load);
+          if (ok) {
+            if (lane == 0) mbar_arrive_expect_tx(&full[at.s], 2u * __popc(boxes) * p.box * D);
+            __syncwarp();
+            if (mine && load) {
+              uint8_t* dk = ring + at.s * S::STAGE + lb * p.box * D;
+              const int slot = my_tok & ((1 << p.page_log2) - 1);
+              tma_box(dk, &mk, &full[at.s], sg.h, slot, page);
+              tma_box(dk + S::KB, &mv, &full[at.s], sg.h, slot, page);
+            }
+            if (mine) {
+              // a masked score, -inf, times ck stays -inf; what is not there weighs nothing
+              float4 w = make_float4(1e-37f, -INFINITY, 0.f, 0.f);
+              if (there) {
+                const float v = vs < kBALeastV ? kBALeastV : vs;
+                w.x = fmaxf(ks * p.scale_log2, 1e-37f);
+                w.y = __log2f(v);
+                w.z = __frcp_rn(v);
+              }
+              float4* d = scales + at.s * S::SC + lb * (p.box >> 3);
+              for (int i = 0; i < p.box >> 3; ++i) d[i] = w;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[at.s]);
+            if (lane == 0) SPECQ_TRACE_POINT(5, t);
+          }
+          if (!q_done) copy_queries();       // after the first tile is on its way
+        }
       }
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int t = 0; t < TG; ++t) {
-        const float4 w = *reinterpret_cast<const float4*>(merge + (t * ROWS + lr) * PITCH + d);
-        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-      }
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        ba_store(p, ba_out_at(p, a, sg.b, sg.h, sg.row_lo + lr) + d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * ROWS + lr) * D + d) = v;
-        if (d == 0)
-          *reinterpret_cast<float2*>(p.part_ml + (static_cast<int64_t>(slot) * ROWS + lr) * 2) = make_float2(top, sum);
+      if (!q_done) copy_queries();
+      for (; stepped < sg.tb; ++stepped) at.step(stages);
+      skip = (skip + NF - (sg.tb - sg.ta) % NF) % NF;
+    }
+    if (!ok) {                               // a wait ran out: leave no copy of this block in flight
+      for (int s = 0; s < stages; ++s) {
+        (void)mbar_wait(&full[s], 0u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+        (void)mbar_wait(&full[s], 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
       }
     }
-    fence_proxy_async_smem();                                   // the merge buffer becomes a TMA target again
-    __syncthreads();
+    pdl_launch_dependents();
+    return;
+  }
 
-    u = seg_begin + sg.tb;
-    if (hr + 1 == p.h_kv * a.rc && sg.tb == sg.nt) {
-      seq_begin = u;
-      ++sg.b;
+  // ---- the computing warps
+  if constexpr (ba_split(NT)) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+  const int grp = warp >> 2, gw = warp & 3;  // group, warp of the group
+  const int gq = lane >> 2, tq = lane & 3;
+  // ldmatrix rows of this lane: matrix lane / 8 = (token half, piece); pieces are swizzled
+  const int mr = (lane & 7) + ((lane >> 3) & 1) * 8, mc = lane >> 4;
+  const uint32_t ring_s = smem_u32(ring);
+  const uint32_t k_off = ring_s + static_cast<uint32_t>((gw * 16 * U + mr) * D + ((mc ^ (D == 128 ? (mr & 7) : ((mr >> 1) & 3))) << 4));
+  // V: MT = 2, matrices (token half, piece); MT = 1, (token half, next 16 tokens)
+  const int vr = MT == 2 ? mr : mr + mc * 16;
+  const int vc = MT == 2 ? 2 * gw + mc : gw;
+  const uint32_t v_off = ring_s + S::KB + static_cast<uint32_t>(vr * D + ((vc ^ (D == 128 ? (vr & 7) : ((vr >> 1) & 3))) << 4));
+  uint8_t* my_p = pbuf + grp * S::P + lane * 8;
+
+  int tile_no = 0;                           // of the piece
+  while (walk.next(p, a, sg)) {
+    // ---- Q^T as the B operand: thread (gq, tq) holds row gq of each group, d = 16 c + 4 tq + 0..3
+    uint32_t qf[NT][KC][2];
+    float fac = 1.f;
+    ok = ok && mbar_wait(&q_full[qat.s], qat.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const uint8_t* src = qbuf + qat.s * S::Q + (n * 8 + gq) * S::QPITCH + 8 * tq;
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        const uint2 w = *reinterpret_cast<const uint2*>(src + 32 * c);
+        qf[n][c][0] = w.x;
+        qf[n][c][1] = w.y;
+      }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&q_empty[qat.s]);
+    qat.step(2);
+    if (threadIdx.x == 0) SPECQ_TRACE_POINT(9, sg.ta);
+    if (p.bf16) {
+      // to fp16 under one power of two that brings the largest to [1, 2): bf16's 8 bits are exact
+      // down to 2^-17 of it, and what is smaller is off by 2^-25 of it at most
+      float top = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(qf[n][c][i] << 16)), fabsf(__uint_as_float(qf[n][c][i] & 0xffff0000u))));
+      top = warp_max_f32(top);
+      const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      fac = __uint_as_float(ex << 23);
+      const float inv = __uint_as_float((254u - ex) << 23);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const __half2 y = __floats2half2_rn(__uint_as_float(qf[n][c][i] << 16) * inv,
+                                                __uint_as_float(qf[n][c][i] & 0xffff0000u) * inv);
+            qf[n][c][i] = *reinterpret_cast<const uint32_t*>(&y);
+          }
+    }
+    float o[MT][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = kBANone;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int c = 0; c < MT; ++c) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
+    }
+
+    for (int t = sg.ta; t < sg.tb; ++t, at.step(stages)) {
+      if ((tile_no++ & 1) != grp) continue;                     // the other group's
+      ok = ok && mbar_wait(&full[at.s], at.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+      const uint32_t stage = static_cast<uint32_t>(at.s * S::STAGE);
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(10, t);
+
+      // S^T = K Q^T for tokens 16 (U gw + u) + 0..15
+      float sc[U][NT][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sc[u][n][0] = sc[u][n][1] = sc[u][n][2] = sc[u][n][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < KC; c += 2) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          uint32_t r[4];
+          ldsm4(((k_off + stage) ^ static_cast<uint32_t>(c << 4)) + static_cast<uint32_t>(u * 16 * D), r);
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            uint32_t l0, h0, l1, h1;
+            widen4<CT, false>(r[2 * hf], l0, h0);
+            widen4<CT, false>(r[2 * hf + 1], l1, h1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816(sc[u][n], l0, l1, h0, h1, qf[n][c + hf][0], qf[n][c + hf][1]);
+          }
+        }
+      }
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(11, t);
+
+      // softmax: rows 2 tq, 2 tq + 1 of each group, tokens gq and gq + 8 of each 16
+      float ck[U], lv[U], lv1[U], iv[U], iv_rel[U];
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float4 w0 = scales[at.s * S::SC + 2 * (U * gw + u)];
+        ck[u] = w0.x * fac;
+        lv[u] = lv1[u] = w0.y;
+        iv[u] = w0.z;
+        iv_rel[u] = 1.f;
+        if (p.page_log2 == 3) {              // tokens 8 .. 15 are another page's, with its own scales
+          const float4 w1 = scales[at.s * S::SC + 2 * (U * gw + u) + 1];
+          lv1[u] = w1.y;
+          iv_rel[u] = iv[u] > 0.f ? w1.z / iv[u] : 0.f;
+          const float rel = w1.x / w0.x;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            sc[u][n][2] *= rel;
+            sc[u][n][3] *= rel;
+          }
+        }
+        const int t0 = t * TOK + 16 * (U * gw + u);
+        if (t0 + 16 > sg.old) {              // some row may not see some token
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int qi = ba_token(p, sg.row_lo + n * 8 + 2 * tq + r);
+              if (p.tree == nullptr) {
+                const int lim = min(sg.ctx, sg.old + qi + 1);
+                if (t0 + gq >= lim) sc[u][n][r] = -INFINITY;
+                if (t0 + gq + 8 >= lim) sc[u][n][2 + r] = -INFINITY;
+              } else {
+                const uint64_t word = qi < a.q_len ? __ldg(reinterpret_cast<const unsigned long long*>(p.tree) + sg.b * p.tree_sb + qi * p.tree_st) : 0ull;
+                const int j0 = t0 + gq - sg.old, j1 = j0 + 8;
+                if (j0 >= a.q_len || (j0 >= 0 && ((word >> (j0 & 63)) & 1ull) == 0ull)) sc[u][n][r] = -INFINITY;
+                if (j1 >= a.q_len || (j1 >= 0 && ((word >> (j1 & 63)) & 1ull) == 0ull)) sc[u][n][2 + r] = -INFINITY;
+              }
+            }
+          if (CT == 1 && t0 + 16 > sg.ctx) {
+            // slots past the last token may hold anything, NaN bytes too: their V reads as 0
+            uint8_t* v = ring + stage + S::KB + 16 * (U * gw + u) * D;
+            for (int x = max(sg.ctx - t0, 0) * KC + lane; x < 16 * KC; x += 32)
+              *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+            fence_proxy_async_smem();        // before the stage is filled again
+          }
+        }
+        // x = score in log2 units + log2(sV), against the lagging m
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            sc[u][n][r] = fmaf(sc[u][n][r], ck[u], lv[u]);
+            sc[u][n][2 + r] = fmaf(sc[u][n][2 + r], ck[u], lv1[u]);
+            top = fmaxf(top, fmaxf(sc[u][n][r], sc[u][n][2 + r]) - m[n][r]);
+          }
+      }
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(12, t);
+      // the vote is also the barrier after which the group's P buffer may be written again
+      if (ba_vote(1 + grp, top > kBARaise)) {                   // raise the maxima and what they scale
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float v = fmaxf(sc[0][n][r], sc[0][n][2 + r]);
+            if constexpr (U == 2) v = fmaxf(v, fmaxf(sc[U - 1][n][r], sc[U - 1][n][2 + r]));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+            if (gq == 0) sm_m[warp * ROWS + n * 8 + 2 * tq + r] = v;
+          }
+        named_barrier_sync(1 + grp, 32 * kBAGroupWarps);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float mn = m[n][r];
+#pragma unroll
+            for (int w = 0; w < kBAGroupWarps; ++w) mn = fmaxf(mn, sm_m[(grp * kBAGroupWarps + w) * ROWS + n * 8 + 2 * tq + r]);
+            const float f = ex2(m[n][r] - mn);
+            m[n][r] = mn;
+            l[n][r] *= f;
+#pragma unroll
+            for (int c = 0; c < MT; ++c) {
+              o[c][n][r] *= f;
+              o[c][n][2 + r] *= f;
+            }
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float y[4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            y[r] = ex2(sc[u][n][r] - m[n][r]);
+            y[2 + r] = ex2(sc[u][n][2 + r] - m[n][r]);
+            l[n][r] = fmaf(fmaf(y[2 + r], iv_rel[u], y[r]), iv[u], l[n][r]);
+          }
+          const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
+          *reinterpret_cast<uint2*>(my_p + ((U * gw + u) * NT + n) * 256) =
+              make_uint2(movm_t(*reinterpret_cast<const uint32_t*>(&h0)), movm_t(*reinterpret_cast<const uint32_t*>(&h1)));
+        }
+      named_barrier_sync(1 + grp, 32 * kBAGroupWarps);
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, t);
+
+      // O^T += V^T P^T
+#pragma unroll
+      for (int k = 0; k < TOK / 16; k += (MT == 2 ? 1 : 2)) {
+        uint32_t r[4];
+        ldsm4_t(v_off + stage + static_cast<uint32_t>(k * 16 * D), r);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          uint32_t e0, d0, e1, d1;
+          widen4<CT, true>(r[2 * hf], e0, d0);
+          widen4<CT, true>(r[2 * hf + 1], e1, d1);
+          const int kk = MT == 2 ? k : k + hf;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint2 b = *reinterpret_cast<const uint2*>(my_p + (kk * NT + n) * 256);
+            mma16816(o[MT == 2 ? hf : 0][n], e0, d0, e1, d1, b.x, b.y);
+          }
+        }
+      }
+      __syncwarp();                                             // every lane has read the stage
+      if (lane == 0) mbar_arrive(&empty[at.s]);
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(14, t);
+    }
+
+    // ---- the segment's rows: the second group's part to the first, then out or the workspace
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float v = l[n][r];
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+        if (gq == 0) {
+          sm_l[warp * ROWS + n * 8 + 2 * tq + r] = v;
+          if (warp == kBAGroupWarps) sm_m[warp * ROWS + n * 8 + 2 * tq + r] = m[n][r];
+        }
+      }
+    if (grp == 1) {
+#pragma unroll
+      for (int c = 0; c < MT; ++c)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          merge[((gw * MT + c) * NT + n) * 32 + lane] = make_float4(o[c][n][0], o[c][n][1], o[c][n][2], o[c][n][3]);
+    }
+    named_barrier_sync(3, kBACompute);
+    if (grp == 0) {
+      const bool whole = sg.ta == 0 && sg.tb == sg.nt;
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (sg.ta == 0 ? 1 : 0);
+      const int live = min(a.chunk_rows, a.q_rows - sg.row_lo);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float4 w[MT];
+#pragma unroll
+        for (int c = 0; c < MT; ++c) w[c] = merge[((gw * MT + c) * NT + n) * 32 + lane];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int lr = n * 8 + 2 * tq + r;
+          const float m1 = sm_m[kBAGroupWarps * ROWS + lr];
+          const float mx = fmaxf(m[n][r], m1), f0 = ex2(m[n][r] - mx), f1 = ex2(m1 - mx);
+          float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+          for (int x = 0; x < kBAGroupWarps; ++x) {
+            l0 += sm_l[x * ROWS + lr];
+            l1 += sm_l[(kBAGroupWarps + x) * ROWS + lr];
+          }
+          const float sum = l0 * f0 + l1 * f1;
+          if (lr < live) {
+            if (whole) {
+              const float inv = sum == 0.f ? 0.f : 1.f / sum;
+              const int64_t off = ba_out_at(p, a, sg.b, sg.h, sg.row_lo + lr) + gw * MT * 16 + 2 * gq;
+#pragma unroll
+              for (int c = 0; c < MT; ++c)
+                ba_store2(p, off + 16 * c, (o[c][n][r] * f0 + (r == 0 ? w[c].x : w[c].y) * f1) * inv,
+                          (o[c][n][2 + r] * f0 + (r == 0 ? w[c].z : w[c].w) * f1) * inv);
+            } else {
+              float* d = p.part_o + (slot * ROWS + lr) * D + gw * MT * 16 + 2 * gq;
+#pragma unroll
+              for (int c = 0; c < MT; ++c)
+                *reinterpret_cast<float2*>(d + 16 * c) = make_float2(o[c][n][r] * f0 + (r == 0 ? w[c].x : w[c].y) * f1,
+                                                                    o[c][n][2 + r] * f0 + (r == 0 ? w[c].z : w[c].w) * f1);
+              if (gw == 0 && gq == 0)
+                *reinterpret_cast<float2*>(p.part_ml + (slot * ROWS + lr) * 2) = make_float2(mx, sum);
+            }
+          }
+        }
+      }
+    }
+    named_barrier_sync(3, kBACompute);                          // sm_l, sm_m and the merge buffer may be written again
+    if (threadIdx.x == 0) SPECQ_TRACE_POINT(16, sg.ta);
   }
   pdl_launch_dependents();
-  if (!ring.ok && rg == 0 && lane == 0) {   // a wait ran out: leave no copy of this block in flight
-    for (int s = 0; s < stages; ++s) {
-      (void)mbar_wait(&full[tg][s], 0u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-      (void)mbar_wait(&full[tg][s], 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-    }
-  }
 }
 
 // Join the parts of cut segments: block (segment, group of 8 rows), one warp a row.
@@ -673,103 +787,127 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   const BALine a = ba_line(p, false);
   if (a.rc == 0) return;
-  const int seg = blockIdx.x;
-  const int b = seg / (p.h_kv * a.rc), hr = seg - b * (p.h_kv * a.rc);
+  const int per = p.h_kv * a.rc;
+  const int b = static_cast<int>(blockIdx.x) / per, hr = static_cast<int>(blockIdx.x) - b * per;
   if (b >= a.n_seqs) return;
-  const int h = hr / a.rc, rc = hr - h * a.rc;
+  const int h = hr / a.rc, row_lo = (hr - h * a.rc) * a.chunk_rows;
+  const int lr = blockIdx.y * 8 + warp;
+  if (lr >= min(a.chunk_rows, a.q_rows - row_lo)) return;
   // where the segment lies on the line
-  int64_t before = 0;
+  int before = 0;
   for (int b0 = 0; b0 < b; b0 += 32) {
     const int x = b0 + lane;
     before += __reduce_add_sync(0xffffffffu, x < b ? ba_tiles(p, ba_ctx(p, x)) : 0);
   }
   const int nt = ba_tiles(p, ba_ctx(p, b));
-  const int64_t s0 = before * (p.h_kv * a.rc) + static_cast<int64_t>(hr) * nt, s1 = s0 + nt;
-  const int c0 = static_cast<int>(((s0 + 1) * p.grid - 1) / a.total), c1 = static_cast<int>((s1 * p.grid - 1) / a.total);
+  const int s0 = before * per + hr * nt;
+  const int c0 = a.piece_of(s0), c1 = a.piece_of(s0 + nt - 1);
   if (c0 == c1) return;                                         // inside one piece: written already
-  const int row_lo = rc * a.chunk_rows;
-  const int lr = blockIdx.y * 8 + warp;
-  if (lr >= min(a.chunk_rows, a.q_rows - row_lo)) return;
-  auto slot_of = [&](int c) { return 2 * c + (a.total * c / p.grid <= s0 ? 1 : 0); };
-  auto empty_piece = [&](int c) { return a.total * c / p.grid == a.total * (c + 1) / p.grid; };
-  float top = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32)
-    if (!empty_piece(c)) top = fmaxf(top, __ldg(p.part_ml + (static_cast<int64_t>(slot_of(c)) * p.rows + lr) * 2));
-  top = warp_max_f32(top);
+  // piece c0 holds the segment's beginning (its second slot), the others begin inside it
   constexpr int V = D / 32;
   float v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = 0.f;
-  float sum = 0.f;
-  for (int c = c0; c <= c1; ++c) {
-    if (empty_piece(c)) continue;
-    const int64_t at = static_cast<int64_t>(slot_of(c)) * p.rows + lr;
-    const float2 ml = __ldg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
-    const float f = ex2(ml.x - top);
-    sum += f * ml.y;
-    const float* src = p.part_o + at * D + lane * V;
-    if constexpr (V == 4) {
-      const float4 w = __ldg(reinterpret_cast<const float4*>(src));
-      v[0] += f * w.x; v[1] += f * w.y; v[2] += f * w.z; v[3] += f * w.w;
-    } else {
-      const float2 w = __ldg(reinterpret_cast<const float2*>(src));
-      v[0] += f * w.x; v[1] += f * w.y;
+  float sum = 0.f, top = kBANone;
+  constexpr int U = 4;                                          // parts in flight
+  for (int cb = c0; cb <= c1; cb += U) {
+    float2 ml[U];
+    float w[U][V];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int c = cb + i;
+      ml[i] = make_float2(kBANone, 0.f);
+#pragma unroll
+      for (int x = 0; x < V; ++x) w[i][x] = 0.f;
+      if (c <= c1) {
+        const int64_t at = static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * p.rows + lr;
+        ml[i] = __ldg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
+        const float* src = p.part_o + at * D + lane * V;
+        if constexpr (V == 4) {
+          const float4 u = __ldg(reinterpret_cast<const float4*>(src));
+          w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
+        } else {
+          const float2 u = __ldg(reinterpret_cast<const float2*>(src));
+          w[i][0] = u.x; w[i][1] = u.y;
+        }
+      }
     }
+    float mx = top;
+#pragma unroll
+    for (int i = 0; i < U; ++i) mx = fmaxf(mx, ml[i].x);
+    const float f0 = ex2(top - mx);
+    sum *= f0;
+#pragma unroll
+    for (int x = 0; x < V; ++x) v[x] *= f0;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const float f = ex2(ml[i].x - mx);
+      sum = fmaf(f, ml[i].y, sum);
+#pragma unroll
+      for (int x = 0; x < V; ++x) v[x] = fmaf(f, w[i][x], v[x]);
+    }
+    top = mx;
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t off = ba_out_at(p, a, b, h, row_lo + lr) + lane * V;
-  if constexpr (V == 4) {
-    ba_store(p, off, v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  } else if (p.bf16) {
-    *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(p.out) + off) = __floats2bfloat162_rn(v[0] * inv, v[1] * inv);
-  } else {
-    *reinterpret_cast<__half2*>(static_cast<__half*>(p.out) + off) = __floats2half2_rn(v[0] * inv, v[1] * inv);
-  }
+#pragma unroll
+  for (int i = 0; i < V; i += 2) ba_store2(p, off + i, v[i] * inv, v[i + 1] * inv);
 }
 
 // How a call is launched: the variant for its rows, the grid and the workspace, from the sizes
 // that the host knows (maxima under a plan).
 struct BAShape {
-  int nt, rg, rows, tile, rc, grid, stages, smem;
+  int nt, rows, tile, rc, grid, stages, smem;
   bool join;
   int64_t o_floats, ml_floats;
 };
 
+template <int D>
+inline void ba_smem(int nt, int* fixed, int* stage) {
+  switch (nt) {
+    case 1: *fixed = BASmem<D, 1>::fixed; break;
+    case 2: *fixed = BASmem<D, 2>::fixed; break;
+    case 3: *fixed = BASmem<D, 3>::fixed; break;
+    case 4: *fixed = BASmem<D, 4>::fixed; break;
+    default: *fixed = BASmem<D, 5>::fixed; break;
+  }
+  *stage = 2 * ba_tile(nt) * D;
+}
+
 inline int ba_shape(int B, int ql, int H_KV, int group, int D, int page, int bt_cols, int sm_count, BAShape* s) {
   const int groups = ceil_div(ql * group, 8);
-  s->rc = ceil_div(groups, 12);
-  const int g = ceil_div(groups, s->rc);
-  // up to 3 groups of 8 rows are one warp's (its accumulators and Q fill the registers); more
-  // are dealt to 2 or 4 warps that share a ring
-  s->rg = g <= 3 ? 1 : g <= 6 ? 2 : 4;
-  s->nt = std::max(g <= 3 ? 1 : 2, ceil_div(g, s->rg));
-  s->rows = s->rg * s->nt * 8;
-  const int tg = kBAWarps / s->rg;
-  s->tile = tg * kBATok;
-  const int per_sm = s->nt == 1 ? 2 : 1;
+  s->rc = ceil_div(groups, kBAMaxGroups);
+  s->nt = ceil_div(groups, s->rc);
+  s->rows = s->nt * 8;
+  // up to 16 rows two blocks fit an SM's registers and fill each other's pauses
+  const int per_sm = ba_split(s->nt) ? 1 : 2;
+  s->tile = ba_tile(s->nt);
   const int64_t max_tiles = std::max<int64_t>(1, (static_cast<int64_t>(bt_cols) * page + s->tile - 1) / s->tile);
   const int64_t line = static_cast<int64_t>(B) * H_KV * s->rc * max_tiles;
+  if (line > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %lld tiles", (long long)line);
   s->grid = static_cast<int>(std::min<int64_t>(line, static_cast<int64_t>(per_sm) * sm_count));
   s->join = max_tiles > 1;
-  const int stage = tg * 2 * kBATok * D;
-  const int merge = tg * s->rows * (D + 12) * 4;
-  const int room = (per_sm == 2 ? 110 * 1024 : 216 * 1024);
-  s->stages = std::min(kBAMaxStages, room / stage);
-  s->smem = 1024 + std::max(s->stages * stage, merge);
-  if (s->smem > 224 * 1024) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: shared memory %d", s->smem);
+  int fixed, stage;
+  if (D == 64) ba_smem<64>(s->nt, &fixed, &stage);
+  else ba_smem<128>(s->nt, &fixed, &stage);
+  const int room = (per_sm == 2 ? 112 * 1024 : 226 * 1024) - 1024 - fixed;
+  const int of = std::max(2, ba_feeders(s->nt));               // stages have one reader and one writer each
+  s->stages = std::min(kBAMaxStages, room / stage) / of * of;
+  if (s->stages < of) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %d rows do not fit shared memory", s->rows);
+  s->smem = 1024 + fixed + s->stages * stage;
   s->o_floats = s->join ? 2ll * s->grid * s->rows * D : 0;
   s->ml_floats = s->join ? 2ll * s->grid * s->rows * 2 : 0;
   return SPECQ_OK;
 }
 
-template <int D, int CT, int NT, int RG>
+template <int D, int CT, int NT>
 inline int launch_block_attn(const BlockAttnParams& p, const BAShape& s, const CUtensorMap& mk, const CUtensorMap& mv,
                              cudaStream_t st) {
-  auto kern = block_attn_kernel<D, CT, NT, RG>;
+  auto kern = block_attn_kernel<D, CT, NT>;
   SPECQ_CUDA_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(kern), s.smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(s.grid));
-  cfg.blockDim = dim3(kBAThreads);
+  cfg.blockDim = dim3(ba_threads(NT));
   cfg.dynamicSmemBytes = static_cast<size_t>(s.smem);
   cfg.stream = st;
   LaunchAttrs at(1);
@@ -781,13 +919,13 @@ inline int launch_block_attn(const BlockAttnParams& p, const BAShape& s, const C
 template <int D, int CT>
 inline int launch_block_attn_rows(const BlockAttnParams& p, const BAShape& s, const CUtensorMap& mk,
                                   const CUtensorMap& mv, cudaStream_t st) {
-  if (s.rg == 1) {
-    if (s.nt == 1) return launch_block_attn<D, CT, 1, 1>(p, s, mk, mv, st);
-    if (s.nt == 2) return launch_block_attn<D, CT, 2, 1>(p, s, mk, mv, st);
-    return launch_block_attn<D, CT, 3, 1>(p, s, mk, mv, st);
+  switch (s.nt) {
+    case 1: return launch_block_attn<D, CT, 1>(p, s, mk, mv, st);
+    case 2: return launch_block_attn<D, CT, 2>(p, s, mk, mv, st);
+    case 3: return launch_block_attn<D, CT, 3>(p, s, mk, mv, st);
+    case 4: return launch_block_attn<D, CT, 4>(p, s, mk, mv, st);
+    default: return launch_block_attn<D, CT, 5>(p, s, mk, mv, st);
   }
-  if (s.rg == 2) return s.nt == 2 ? launch_block_attn<D, CT, 2, 2>(p, s, mk, mv, st) : launch_block_attn<D, CT, 3, 2>(p, s, mk, mv, st);
-  return s.nt == 2 ? launch_block_attn<D, CT, 2, 4>(p, s, mk, mv, st) : launch_block_attn<D, CT, 3, 4>(p, s, mk, mv, st);
 }
 
 inline int check_block_attn_sizes(int B, int n_seqs, int q_len, int ql_max, int H, int H_KV, int D, int page, int bt_cols,
@@ -838,8 +976,8 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
       ctx == nullptr || (bt == nullptr && bt_cols > 0))
     return fail(SPECQ_ERR_INVALID_ARG, "block_attention: null pointer");
   if (n_pages <= 0) return fail(SPECQ_ERR_INVALID_ARG, "block_attention: a cache of %d pages", n_pages);
-  if (!aligned(q, 8) || q_sb % 4 || q_st % 4 || q_sh % 4 || !aligned(out, 8) || o_sb % 4 || o_st % 4 || o_sh % 4)
-    return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: query and output rows must be 8-byte aligned");
+  if (!aligned(q, 16) || q_sb % 8 || q_st % 8 || q_sh % 8 || !aligned(out, 4) || o_sb % 2 || o_st % 2 || o_sh % 2)
+    return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: query rows must be 16-byte aligned, output rows 4-byte");
   if (!aligned(kc, 16) || !aligned(vc, 16) || kv_sp % 16 || kv_so % 16 || kv_sh % 16 || kv_sp <= 0 || kv_so <= 0 || kv_sh <= 0)
     return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: cache rows must be 16-byte aligned (TMA)");
   DeviceState* dev = nullptr;
@@ -854,7 +992,7 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
   const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(H_KV), static_cast<uint64_t>(page),
                             static_cast<uint64_t>(n_pages)};
   const uint64_t strides[3] = {static_cast<uint64_t>(kv_sh), static_cast<uint64_t>(kv_so), static_cast<uint64_t>(kv_sp)};
-  const uint32_t box[4] = {static_cast<uint32_t>(D), 1, static_cast<uint32_t>(std::min(kBATok, page)), 1};
+  const uint32_t box[4] = {static_cast<uint32_t>(D), 1, static_cast<uint32_t>(std::min(64, page)), 1};
   const CUtensorMapSwizzle sw = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   if (int rc = encode_tiled(&mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, kc, dims, strides, box, sw)) return rc;
   if (int rc = encode_tiled(&mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, vc, dims, strides, box, sw)) return rc;
@@ -869,7 +1007,8 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
   p.n_seqs = n_seqs; p.q_len = q_len; p.b_max = bg; p.ql_max = ql; p.h_kv = H_KV; p.group = H / H_KV;
   p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.n_pages = n_pages; p.bt_cols = bt_cols;
-  p.bf16 = dtype == 2; p.stages = s.stages; p.grid = s.grid; p.rows = s.rows; p.tile = s.tile;
+  p.bf16 = dtype == 2; p.stages = s.stages; p.grid = s.grid; p.rows = s.rows; p.box = std::min(64, page); p.tile = s.tile;
+  p.group_magic = p.group > 1 ? 0xFFFFFFFFu / static_cast<uint32_t>(p.group) + 1u : 0u;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
   if (D == 128)
