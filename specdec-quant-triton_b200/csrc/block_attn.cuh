@@ -47,6 +47,7 @@
 #include <cuda_fp8.h>
 
 #include "block_cache.cuh"
+#include "paged_attn.cuh"
 #include "sm100.cuh"
 #include "specq_host.cuh"
 
@@ -55,12 +56,13 @@ namespace specq {
 constexpr int kBAGroupWarps = 4;                  // of a group
 constexpr int kBAWarps = 2 * kBAGroupWarps;       // that compute
 constexpr int kBACompute = 32 * kBAWarps;
-// And those that feed them.  A box costs its warp some 90 cycles to start, so a block that has an
-// SM to itself has four.  The registers of an SM's quarter divide among whole warps: from 3 row
+// And those that feed them.  A TMA box holds its warp for some 180 cycles whatever its size
+// (measured: 2 KB boxes from one warp an SM come at 2.8 TB/s, from two at 4.7, from four at 5.1), so an SM
+// has four of them, two a block where two blocks share it.  The registers of an SM's quarter divide among whole warps: from 3 row
 // groups on the block launches 12 warps of 168 and splits their 64,512 as 224 for the computing
 // ones (8 x 32 x 224) and 56 for the feeding ones (4 x 32 x 56).
 __host__ __device__ constexpr bool ba_split(int nt) { return nt >= 3; }
-__host__ __device__ constexpr int ba_feeders(int nt) { return ba_split(nt) ? 4 : 1; }
+__host__ __device__ constexpr int ba_feeders(int nt) { return ba_split(nt) ? 4 : 2; }
 __host__ __device__ constexpr int ba_threads(int nt) { return kBACompute + 32 * ba_feeders(nt); }
 // Tokens of a tile: up to 16 rows two blocks share an SM, and half as many tokens leave each a ring
 // of six stages.
@@ -92,12 +94,9 @@ struct BlockAttnParams {
   uint32_t group_magic;                 // ceil(2^32 / group), for group > 1
 };
 
-__device__ __forceinline__ void tma_box(void* dst, const CUtensorMap* map, uint64_t* bar, int head, int slot, int page) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(head), "r"(slot), "r"(page)
-      : "memory");
+__device__ __forceinline__ void tma_box(void* dst, const CUtensorMap* map, uint64_t* bar, int head, int slot, int page,
+                                        uint64_t hint) {
+  tma_load_4d(dst, map, bar, 0, head, slot, page, hint);
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -114,13 +113,12 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
 }
 __device__ __forceinline__ uint32_t movm_t(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -384,6 +382,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     const int tpb = 32 / nb;
     const int lt = lane / nb, lb = lane - lt * nb;
     int skip = f;                            // tiles of the segment before the warp's next one
+    // pages that one block reads are read once; of several row chunks the first leaves them in L2
+    const uint64_t hint = a.rc == 1 ? policy_evict_first() : policy_evict_last();
     while (walk.next(p, a, sg)) {
       const int32_t* bt = p.bt + sg.b * p.bt_sb;
       bool q_done = false;
@@ -441,11 +441,19 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
           if (ok) {
             if (lane == 0) mbar_arrive_expect_tx(&full[at.s], 2u * __popc(boxes) * p.box * D);
             __syncwarp();
-            if (mine && load) {
-              uint8_t* dk = ring + at.s * S::STAGE + lb * p.box * D;
-              const int slot = my_tok & ((1 << p.page_log2) - 1);
-              tma_box(dk, &mk, &full[at.s], sg.h, slot, page);
-              tma_box(dk + S::KB, &mv, &full[at.s], sg.h, slot, page);
+            // one lane starts all boxes: their operands are the warp's, not a lane's
+            const int first = (t - tb0) / NF * nb;
+            uint8_t* dk = ring + at.s * S::STAGE;
+            int slot = (t * TOK) & ((1 << p.page_log2) - 1);
+            const int n_box = __popc(boxes);
+            for (int x = 0; x < n_box; ++x) {
+              const int pgx = __shfl_sync(0xffffffffu, page, first + x);
+              if (elect_one()) {
+                tma_box(dk, &mk, &full[at.s], sg.h, slot, pgx, hint);
+                tma_box(dk + S::KB, &mv, &full[at.s], sg.h, slot, pgx, hint);
+              }
+              dk += p.box * D;
+              slot = (slot + p.box) & ((1 << p.page_log2) - 1);
             }
             if (mine) {
               // a masked score, -inf, times ck stays -inf; what is not there weighs nothing
@@ -562,19 +570,18 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
 #pragma unroll
         for (int n = 0; n < NT; ++n) sc[u][n][0] = sc[u][n][1] = sc[u][n][2] = sc[u][n][3] = 0.f;
 #pragma unroll
-      for (int c = 0; c < KC; c += 2) {
+      for (int u = 0; u < U; ++u) {
+        uint32_t r[KC / 2][4];               // the whole 16 tokens are on their way before the first product
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          uint32_t r[4];
-          ldsm4(((k_off + stage) ^ static_cast<uint32_t>(c << 4)) + static_cast<uint32_t>(u * 16 * D), r);
+        for (int c = 0; c < KC / 2; ++c)
+          ldsm4(((k_off + stage) ^ static_cast<uint32_t>(c << 5)) + static_cast<uint32_t>(u * 16 * D), r[c]);
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            uint32_t l0, h0, l1, h1;
-            widen4<CT, false>(r[2 * hf], l0, h0);
-            widen4<CT, false>(r[2 * hf + 1], l1, h1);
+        for (int c = 0; c < KC; ++c) {
+          uint32_t l0, h0, l1, h1;
+          widen4<CT, false>(r[c >> 1][2 * (c & 1)], l0, h0);
+          widen4<CT, false>(r[c >> 1][2 * (c & 1) + 1], l1, h1);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma16816(sc[u][n], l0, l1, h0, h1, qf[n][c + hf][0], qf[n][c + hf][1]);
-          }
+          for (int n = 0; n < NT; ++n) mma16816(sc[u][n], l0, l1, h0, h1, qf[n][c][0], qf[n][c][1]);
         }
       }
       if (threadIdx.x == 0) SPECQ_TRACE_POINT(11, t);
@@ -687,16 +694,20 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, t);
 
       // O^T += V^T P^T
+      constexpr int KSTEP = MT == 2 ? 1 : 2, NK = TOK / 16 / KSTEP, AHEAD = NK < 4 ? NK : 4;
+      uint32_t vr4[AHEAD][4];
 #pragma unroll
-      for (int k = 0; k < TOK / 16; k += (MT == 2 ? 1 : 2)) {
-        uint32_t r[4];
-        ldsm4_t(v_off + stage + static_cast<uint32_t>(k * 16 * D), r);
+      for (int k = 0; k < AHEAD; ++k) ldsm4_t(v_off + stage + static_cast<uint32_t>(k * KSTEP * 16 * D), vr4[k]);
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        uint32_t r[4] = {vr4[k % AHEAD][0], vr4[k % AHEAD][1], vr4[k % AHEAD][2], vr4[k % AHEAD][3]};
+        if (k + AHEAD < NK) ldsm4_t(v_off + stage + static_cast<uint32_t>((k + AHEAD) * KSTEP * 16 * D), vr4[k % AHEAD]);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           uint32_t e0, d0, e1, d1;
           widen4<CT, true>(r[2 * hf], e0, d0);
           widen4<CT, true>(r[2 * hf + 1], e1, d1);
-          const int kk = MT == 2 ? k : k + hf;
+          const int kk = MT == 2 ? k : 2 * k + hf;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const uint2 b = *reinterpret_cast<const uint2*>(my_p + (kk * NT + n) * 256);
