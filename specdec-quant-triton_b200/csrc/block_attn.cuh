@@ -40,7 +40,7 @@
 // Work.  The tiles of all (sequence, KV head, row chunk) segments form one line, cut into equal
 // pieces, one for each resident block, whatever the sequences' lengths; each block finds its
 // piece from ctx_len on the device.  A segment inside one piece is written at once; the parts of
-// a cut one go to the workspace and a second, dependent launch joins them in the pieces' order.
+// a cut one, two groups' for each piece, go to the workspace and a second, dependent launch joins them in the pieces' order.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -83,14 +83,14 @@ struct BlockAttnParams {
   const int32_t* ctx;
   const uint64_t* tree;     // optional [B, q_len] bit sets
   const int32_t* plan;      // plan[0] = n_seqs, plan[1] = q_len
-  float* part_o;            // [2 grid][rows][D]
-  float* part_ml;           // [2 grid][rows][2]
+  float* part_o;            // [grid][2 cut segments][2 groups][rows][ba_part(D)]
   int* status;
   int64_t q_sb, q_st, q_sh, o_sb, o_st, o_sh, s_sp, s_sh, bt_sb, tree_sb, tree_st;
   float scale_log2;         // sm_scale * log2(e)
   int n_seqs, q_len, b_max, ql_max, h_kv, group, page_log2, n_pages, bt_cols;
   int bf16, stages, grid, rows, box;    // rows: of a block's chunk; box: slots of a TMA box
   int tile;                             // tokens of a tile
+  int rc, chunk_rows;                   // row chunks of a (sequence, KV head) and their rows, without a plan
   uint32_t group_magic;                 // ceil(2^32 / group), for group > 1
 };
 
@@ -156,6 +156,18 @@ __device__ __forceinline__ int ba_token(const BlockAttnParams& p, int rr) {
   return p.group == 1 ? rr : static_cast<int>(__umulhi(static_cast<uint32_t>(rr), p.group_magic));
 }
 
+// a / b for non-negative a and positive b.  A launch executes its set-up code once, from cold
+// instruction caches, so its length is its time: the quotient by the reciprocal is a third of an
+// integer division's (exact after one correction below 2^22, where the product is off by < 1).
+__device__ __forceinline__ int ba_div(int a, int b) {
+  if (a >= (1 << 22)) return a / b;
+  int q = static_cast<int>(__fmul_rz(static_cast<float>(a), __frcp_rn(static_cast<float>(b))));
+  const int r = a - q * b;
+  if (r >= b) ++q;
+  if (r < 0) --q;
+  return q;
+}
+
 // Where the segments of a call lie on the line of tiles.  Piece c of the line (one a block) is
 // [start(c), start(c + 1)): the first `more` pieces have one tile more than the others.
 struct BALine {
@@ -166,7 +178,7 @@ struct BALine {
   __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
   __device__ __forceinline__ int piece_of(int u) const {
     const int wide = more * (each + 1);
-    return u < wide ? u / (each + 1) : more + (u - wide) / each;   // each > 0 past the wide ones
+    return u < wide ? ba_div(u, each + 1) : more + ba_div(u - wide, each);   // each > 0 past the wide ones
   }
 };
 
@@ -199,11 +211,15 @@ __device__ __forceinline__ BALine ba_line(const BlockAttnParams& p, bool tell) {
     t += __reduce_add_sync(0xffffffffu, n);
   }
   a.q_rows = a.q_len * p.group;
-  const int groups = (a.q_rows + 7) >> 3;
-  a.rc = (groups * 8 + p.rows - 1) / p.rows;
-  a.chunk_rows = a.rc > 0 ? (groups + a.rc - 1) / a.rc * 8 : 0;
+  a.rc = p.rc;
+  a.chunk_rows = p.chunk_rows;
+  if (p.plan != nullptr) {
+    const int groups = (a.q_rows + 7) >> 3;
+    a.rc = ba_div(groups * 8 + p.rows - 1, p.rows);
+    a.chunk_rows = a.rc > 0 ? ba_div(groups + a.rc - 1, a.rc) * 8 : 0;
+  }
   a.total = t * (p.h_kv * a.rc);
-  a.each = a.total / p.grid;
+  a.each = ba_div(a.total, p.grid);
   a.more = a.total - a.each * p.grid;
   return a;
 }
@@ -269,9 +285,9 @@ struct BAWalk {
     s.old = s.ctx - a.q_len;
     s.nt = ba_tiles(p, s.ctx);
     const int in_seq = u - seq_begin;
-    const int hr = in_seq / s.nt;                              // (KV head, row chunk)
+    const int hr = ba_div(in_seq, s.nt);                       // (KV head, row chunk)
     s.ta = in_seq - hr * s.nt;
-    s.h = hr / a.rc;
+    s.h = a.rc == 1 ? hr : ba_div(hr, a.rc);
     s.row_lo = (hr - s.h * a.rc) * a.chunk_rows;
     s.tb = min(s.nt, u1 - u + s.ta);
     u += s.tb - s.ta;
@@ -309,6 +325,9 @@ __device__ __forceinline__ bool ba_vote(int id, bool x) {
   return r != 0u;
 }
 
+// A row's part in the workspace: O [D], l of the group's four warps, m, and padding to 16 bytes.
+__host__ __device__ constexpr int ba_part(int D) { return D + 8; }
+
 template <int D, int NT>
 struct BASmem {
   static constexpr int TOK = ba_tile(NT);
@@ -322,6 +341,7 @@ struct BASmem {
   static constexpr int Q = ROWS * QPITCH;
   static constexpr int SC = TOK / 8;                           // scales of a stage: ck, lv, iv for each 8 tokens
   static constexpr int SCALES = SC * 16;
+  static constexpr int PART = ba_part(D);                      // floats of a row's part
   static constexpr int MERGE = kBAGroupWarps * MT * NT * 32 * 16;   // one group's O
   static constexpr int fixed = 2 * P + MERGE + 2 * Q + kBAMaxStages * SCALES + 2 * kBAWarps * ROWS * 4 + 256;
 };
@@ -378,9 +398,9 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   if (warp >= kBAWarps) {                    // ---- the feeding warps: warp f takes tiles f, f + NF, ... of the piece
     if constexpr (ba_split(NT)) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     const int f = warp - kBAWarps;
-    const int nb = TOK / p.box;          // boxes of a tile; a batch of 32 is `tpb` of the warp's tiles
-    const int tpb = 32 / nb;
-    const int lt = lane / nb, lb = lane - lt * nb;
+    const int nb = TOK >> (31 - __clz(p.box));          // boxes of a tile; a batch of 32 is `tpb` of the warp's tiles
+    const int tpb = 32 / nb;                 // (all powers of two)
+    const int lt = lane >> (31 - __clz(nb)), lb = lane & (nb - 1);
     int skip = f;                            // tiles of the segment before the warp's next one
     // pages that one block reads are read once; of several row chunks the first leaves them in L2
     const uint64_t hint = a.rc == 1 ? policy_evict_first() : policy_evict_last();
@@ -557,8 +577,10 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       for (int c = 0; c < MT; ++c) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
     }
 
+    int n_mine = 0;
     for (int t = sg.ta; t < sg.tb; ++t, at.step(stages)) {
       if ((tile_no++ & 1) != grp) continue;                     // the other group's
+      ++n_mine;
       ok = ok && mbar_wait(&full[at.s], at.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
       const uint32_t stage = static_cast<uint32_t>(at.s * S::STAGE);
       if (threadIdx.x == 0) SPECQ_TRACE_POINT(10, t);
@@ -694,14 +716,17 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, t);
 
       // O^T += V^T P^T
-      constexpr int KSTEP = MT == 2 ? 1 : 2, NK = TOK / 16 / KSTEP, AHEAD = NK < 4 ? NK : 4;
+      constexpr int KSTEP = MT == 2 ? 1 : 2, NK = TOK / 16 / KSTEP, AHEAD = NK < 2 ? NK : 2;
       uint32_t vr4[AHEAD][4];
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) ldsm4_t(v_off + stage + static_cast<uint32_t>(k * KSTEP * 16 * D), vr4[k]);
+#pragma unroll 1
+      for (int kb = 0; kb < NK; kb += AHEAD)
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        uint32_t r[4] = {vr4[k % AHEAD][0], vr4[k % AHEAD][1], vr4[k % AHEAD][2], vr4[k % AHEAD][3]};
-        if (k + AHEAD < NK) ldsm4_t(v_off + stage + static_cast<uint32_t>((k + AHEAD) * KSTEP * 16 * D), vr4[k % AHEAD]);
+      for (int ka = 0; ka < AHEAD; ++ka) {
+        const int k = kb + ka;
+        uint32_t r[4] = {vr4[ka][0], vr4[ka][1], vr4[ka][2], vr4[ka][3]};
+        if (k + AHEAD < NK) ldsm4_t(v_off + stage + static_cast<uint32_t>((k + AHEAD) * KSTEP * 16 * D), vr4[ka]);
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           uint32_t e0, d0, e1, d1;
@@ -720,7 +745,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       if (threadIdx.x == 0) SPECQ_TRACE_POINT(14, t);
     }
 
-    // ---- the segment's rows: the second group's part to the first, then out or the workspace
+    // ---- the group's part of the segment
+    const int live = min(a.chunk_rows, a.q_rows - sg.row_lo);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -729,62 +755,76 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
         v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         v += __shfl_xor_sync(0xffffffffu, v, 16);
-        if (gq == 0) {
-          sm_l[warp * ROWS + n * 8 + 2 * tq + r] = v;
-          if (warp == kBAGroupWarps) sm_m[warp * ROWS + n * 8 + 2 * tq + r] = m[n][r];
-        }
+        l[n][r] = v;
       }
-    if (grp == 1) {
-#pragma unroll
-      for (int c = 0; c < MT; ++c)
+    if (sg.ta > 0 || sg.tb < sg.nt) {
+      // a piece of a cut segment: a group that had a tile writes its part to the workspace (O of each
+      // warp's elements, l of each warp's tokens, m) and goes on
+      if (n_mine > 0) {
+        float* part = p.part_o + (2 * (2 * static_cast<int64_t>(blockIdx.x) + (sg.ta == 0 ? 1 : 0)) + grp) * (ROWS * S::PART);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
-          merge[((gw * MT + c) * NT + n) * 32 + lane] = make_float4(o[c][n][0], o[c][n][1], o[c][n][2], o[c][n][3]);
-    }
-    named_barrier_sync(3, kBACompute);
-    if (grp == 0) {
-      const bool whole = sg.ta == 0 && sg.tb == sg.nt;
-      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (sg.ta == 0 ? 1 : 0);
-      const int live = min(a.chunk_rows, a.q_rows - sg.row_lo);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float4 w[MT];
-#pragma unroll
-        for (int c = 0; c < MT; ++c) w[c] = merge[((gw * MT + c) * NT + n) * 32 + lane];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int lr = n * 8 + 2 * tq + r;
-          const float m1 = sm_m[kBAGroupWarps * ROWS + lr];
-          const float mx = fmaxf(m[n][r], m1), f0 = ex2(m[n][r] - mx), f1 = ex2(m1 - mx);
-          float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-          for (int x = 0; x < kBAGroupWarps; ++x) {
-            l0 += sm_l[x * ROWS + lr];
-            l1 += sm_l[(kBAGroupWarps + x) * ROWS + lr];
-          }
-          const float sum = l0 * f0 + l1 * f1;
-          if (lr < live) {
-            if (whole) {
-              const float inv = sum == 0.f ? 0.f : 1.f / sum;
-              const int64_t off = ba_out_at(p, a, sg.b, sg.h, sg.row_lo + lr) + gw * MT * 16 + 2 * gq;
+          for (int r = 0; r < 2; ++r) {
+            float* d = part + (n * 8 + 2 * tq + r) * S::PART;
+            if (n * 8 + 2 * tq + r < live) {
 #pragma unroll
               for (int c = 0; c < MT; ++c)
-                ba_store2(p, off + 16 * c, (o[c][n][r] * f0 + (r == 0 ? w[c].x : w[c].y) * f1) * inv,
-                          (o[c][n][2 + r] * f0 + (r == 0 ? w[c].z : w[c].w) * f1) * inv);
-            } else {
-              float* d = p.part_o + (slot * ROWS + lr) * D + gw * MT * 16 + 2 * gq;
-#pragma unroll
-              for (int c = 0; c < MT; ++c)
-                *reinterpret_cast<float2*>(d + 16 * c) = make_float2(o[c][n][r] * f0 + (r == 0 ? w[c].x : w[c].y) * f1,
-                                                                    o[c][n][2 + r] * f0 + (r == 0 ? w[c].z : w[c].w) * f1);
-              if (gw == 0 && gq == 0)
-                *reinterpret_cast<float2*>(p.part_ml + (slot * ROWS + lr) * 2) = make_float2(mx, sum);
+                *reinterpret_cast<float2*>(d + (gw * MT + c) * 16 + 2 * gq) = make_float2(o[c][n][r], o[c][n][2 + r]);
+              if (gq == 0) {
+                d[D + gw] = l[n][r];
+                if (gw == 0) d[D + kBAGroupWarps] = m[n][r];
+              }
             }
           }
-        }
       }
+    } else {
+      // all of it: the second group's part goes to the first, and out
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (gq == 0) {
+            sm_l[warp * ROWS + n * 8 + 2 * tq + r] = l[n][r];
+            if (warp == kBAGroupWarps) sm_m[warp * ROWS + n * 8 + 2 * tq + r] = m[n][r];
+          }
+      if (grp == 1) {
+#pragma unroll
+        for (int c = 0; c < MT; ++c)
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+            merge[((gw * MT + c) * NT + n) * 32 + lane] = make_float4(o[c][n][0], o[c][n][1], o[c][n][2], o[c][n][3]);
+      }
+      named_barrier_sync(3, kBACompute);
+      if (grp == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const int lr = n * 8 + 2 * tq + r;
+            const float m1 = sm_m[kBAGroupWarps * ROWS + lr];
+            const float mx = fmaxf(m[n][r], m1), f0 = ex2(m[n][r] - mx), f1 = ex2(m1 - mx);
+            float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+            for (int x = 0; x < kBAGroupWarps; ++x) {
+              l0 += sm_l[x * ROWS + lr];
+              l1 += sm_l[(kBAGroupWarps + x) * ROWS + lr];
+            }
+            const float sum = l0 * f0 + l1 * f1;
+            const float inv = sum == 0.f ? 0.f : __frcp_rn(sum);
+            if (lr < live) {
+              const int64_t off = ba_out_at(p, a, sg.b, sg.h, sg.row_lo + lr) + gw * MT * 16 + 2 * gq;
+#pragma unroll
+              for (int c = 0; c < MT; ++c) {
+                const float4 w = merge[((gw * MT + c) * NT + n) * 32 + lane];
+                ba_store2(p, off + 16 * c, (o[c][n][r] * f0 + (r == 0 ? w.x : w.y) * f1) * inv,
+                          (o[c][n][2 + r] * f0 + (r == 0 ? w.z : w.w) * f1) * inv);
+              }
+            }
+          }
+      }
+      named_barrier_sync(3, kBACompute);                        // sm_l, sm_m and the merge buffer may be written again
     }
-    named_barrier_sync(3, kBACompute);                          // sm_l, sm_m and the merge buffer may be written again
     if (threadIdx.x == 0) SPECQ_TRACE_POINT(16, sg.ta);
   }
   pdl_launch_dependents();
@@ -799,9 +839,9 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
   const BALine a = ba_line(p, false);
   if (a.rc == 0) return;
   const int per = p.h_kv * a.rc;
-  const int b = static_cast<int>(blockIdx.x) / per, hr = static_cast<int>(blockIdx.x) - b * per;
+  const int b = ba_div(static_cast<int>(blockIdx.x), per), hr = static_cast<int>(blockIdx.x) - b * per;
   if (b >= a.n_seqs) return;
-  const int h = hr / a.rc, row_lo = (hr - h * a.rc) * a.chunk_rows;
+  const int h = ba_div(hr, a.rc), row_lo = (hr - h * a.rc) * a.chunk_rows;
   const int lr = blockIdx.y * 8 + warp;
   if (lr >= min(a.chunk_rows, a.q_rows - row_lo)) return;
   // where the segment lies on the line
@@ -814,48 +854,51 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
   const int s0 = before * per + hr * nt;
   const int c0 = a.piece_of(s0), c1 = a.piece_of(s0 + nt - 1);
   if (c0 == c1) return;                                         // inside one piece: written already
-  // piece c0 holds the segment's beginning (its second slot), the others begin inside it
-  constexpr int V = D / 32;
+  // piece c0 holds the segment's beginning (its second slot), the others begin inside it; tile n of a
+  // piece is group n % 2's, so a group has a part unless the segment has one tile there, the other's
+  constexpr int V = D / 32, PART = ba_part(D);
   float v[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = 0.f;
   float sum = 0.f, top = kBANone;
   constexpr int U = 4;                                          // parts in flight
-  for (int cb = c0; cb <= c1; cb += U) {
-    float2 ml[U];
-    float w[U][V];
+  for (int x0 = 2 * c0; x0 <= 2 * c1 + 1; x0 += U) {
+    float m[U], l[U], w[U][V];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int c = cb + i;
-      ml[i] = make_float2(kBANone, 0.f);
+      const int x = x0 + i, c = x >> 1, grp = x & 1;
+      m[i] = kBANone;
+      l[i] = 0.f;
 #pragma unroll
-      for (int x = 0; x < V; ++x) w[i][x] = 0.f;
-      if (c <= c1) {
-        const int64_t at = static_cast<int64_t>(2 * c + (c == c0 ? 1 : 0)) * p.rows + lr;
-        ml[i] = __ldg(reinterpret_cast<const float2*>(p.part_ml + at * 2));
-        const float* src = p.part_o + at * D + lane * V;
+      for (int y = 0; y < V; ++y) w[i][y] = 0.f;
+      const int from = max(s0, a.start(c)), to = min(s0 + nt, a.start(c + 1));
+      if (c <= c1 && (to - from > 1 || ((from - a.start(c)) & 1) == grp)) {
+        const float* src = p.part_o + (static_cast<int64_t>(2 * (2 * c + (c == c0 ? 1 : 0)) + grp) * p.rows + lr) * PART;
+        const float4 l4 = __ldg(reinterpret_cast<const float4*>(src + D));
+        m[i] = __ldg(src + D + kBAGroupWarps);
+        l[i] = (l4.x + l4.y) + (l4.z + l4.w);
         if constexpr (V == 4) {
-          const float4 u = __ldg(reinterpret_cast<const float4*>(src));
+          const float4 u = __ldg(reinterpret_cast<const float4*>(src + lane * V));
           w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
         } else {
-          const float2 u = __ldg(reinterpret_cast<const float2*>(src));
+          const float2 u = __ldg(reinterpret_cast<const float2*>(src + lane * V));
           w[i][0] = u.x; w[i][1] = u.y;
         }
       }
     }
     float mx = top;
 #pragma unroll
-    for (int i = 0; i < U; ++i) mx = fmaxf(mx, ml[i].x);
+    for (int i = 0; i < U; ++i) mx = fmaxf(mx, m[i]);
     const float f0 = ex2(top - mx);
     sum *= f0;
 #pragma unroll
-    for (int x = 0; x < V; ++x) v[x] *= f0;
+    for (int y = 0; y < V; ++y) v[y] *= f0;
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const float f = ex2(ml[i].x - mx);
-      sum = fmaf(f, ml[i].y, sum);
+      const float f = ex2(m[i] - mx);
+      sum = fmaf(f, l[i], sum);
 #pragma unroll
-      for (int x = 0; x < V; ++x) v[x] = fmaf(f, w[i][x], v[x]);
+      for (int y = 0; y < V; ++y) v[y] = fmaf(f, w[i][y], v[y]);
     }
     top = mx;
   }
@@ -870,7 +913,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
 struct BAShape {
   int nt, rows, tile, rc, grid, stages, smem;
   bool join;
-  int64_t o_floats, ml_floats;
+  int64_t ws_floats;
 };
 
 template <int D>
@@ -906,8 +949,7 @@ inline int ba_shape(int B, int ql, int H_KV, int group, int D, int page, int bt_
   s->stages = std::min(kBAMaxStages, room / stage) / of * of;
   if (s->stages < of) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %d rows do not fit shared memory", s->rows);
   s->smem = 1024 + fixed + s->stages * stage;
-  s->o_floats = s->join ? 2ll * s->grid * s->rows * D : 0;
-  s->ml_floats = s->join ? 2ll * s->grid * s->rows * 2 : 0;
+  s->ws_floats = s->join ? 4ll * s->grid * s->rows * ba_part(D) : 0;
   return SPECQ_OK;
 }
 
@@ -964,7 +1006,7 @@ inline int run_block_attention_workspace(int B, int n_seqs, int q_len, int ql_ma
   if (int rc = get_device_state(&dev)) return rc;
   BAShape s;
   if (int rc = ba_shape(bg, ql, H_KV, H / H_KV, D, page, bt_cols, dev->sm_count, &s)) return rc;
-  *bytes = (s.o_floats + s.ml_floats) * static_cast<int64_t>(sizeof(float));
+  *bytes = s.ws_floats * static_cast<int64_t>(sizeof(float));
   return SPECQ_OK;
 }
 
@@ -995,7 +1037,7 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
   if (int rc = get_device_state(&dev)) return rc;
   BAShape s;
   if (int rc = ba_shape(bg, ql, H_KV, H / H_KV, D, page, bt_cols, dev->sm_count, &s)) return rc;
-  const int64_t need = (s.o_floats + s.ml_floats) * static_cast<int64_t>(sizeof(float));
+  const int64_t need = s.ws_floats * static_cast<int64_t>(sizeof(float));
   if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(SPECQ_ERR_INVALID_ARG, "block_attention: a 16-byte aligned workspace of %lld bytes is needed, got %lld",
                 (long long)need, (long long)workspace_bytes);
@@ -1010,7 +1052,6 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
   BlockAttnParams p = {};
   p.q = q; p.out = out; p.ks = ks; p.vs = vs; p.bt = bt; p.ctx = ctx; p.tree = tree; p.plan = plan;
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + s.o_floats;
   p.status = dev->status;
   p.q_sb = q_sb; p.q_st = q_st; p.q_sh = q_sh; p.o_sb = o_sb; p.o_st = o_st; p.o_sh = o_sh;
   p.s_sp = s_sp; p.s_sh = s_sh; p.bt_sb = bt_sb; p.tree_sb = tree_sb; p.tree_st = tree_st;
@@ -1019,6 +1060,7 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
   p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.n_pages = n_pages; p.bt_cols = bt_cols;
   p.bf16 = dtype == 2; p.stages = s.stages; p.grid = s.grid; p.rows = s.rows; p.box = std::min(64, page); p.tile = s.tile;
+  p.rc = s.rc; p.chunk_rows = ceil_div(ceil_div(ql * p.group, 8), s.rc) * 8;
   p.group_magic = p.group > 1 ? 0xFFFFFFFFu / static_cast<uint32_t>(p.group) + 1u : 0u;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
