@@ -1,4 +1,5 @@
-"""Build libspecq.so (the sm_100a kernels behind the C ABI of include/specq.h) in-tree.
+"""Build libspecq.so (the sm_100a kernels behind the C ABI of include/specq.h) and _native.so (the
+Python binding of the block-scaled cache's operators) in-tree.
 
     python specdec-quant-triton_b200/build.py [--verbose-ptxas] [--force]
 
@@ -10,16 +11,20 @@ from __future__ import annotations
 
 import argparse
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 OUT = os.path.join(PKG_DIR, "specq", "libspecq.so")
+BINDING = os.path.join(CSRC, "py_blocks.cpp")
+BINDING_OUT = os.path.join(PKG_DIR, "specq", "_native.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -49,8 +54,31 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(s) <= t for s in sources())
 
 
+def build_binding(force: bool = False, quiet: bool = False) -> str:
+    """Build _native.so against the installed torch's headers (it holds no kernel)."""
+    t = os.path.getmtime(BINDING_OUT) if os.path.exists(BINDING_OUT) else 0.0
+    if not force and all(os.path.getmtime(s) <= t for s in (BINDING, os.path.join(INCLUDE, "specq.h"))):
+        return BINDING_OUT
+    torch_dir = os.path.dirname(importlib.util.find_spec("torch").origin)
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc_path())))
+    cmd = [os.environ.get("CXX") or shutil.which("c++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-I", INCLUDE, "-I", os.path.join(torch_dir, "include"),
+           "-I", os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"), "-I", os.path.join(cuda, "include"),
+           "-I", sysconfig.get_paths()["include"], BINDING, "-o", BINDING_OUT + ".tmp", "-L", os.path.join(torch_dir, "lib"),
+           "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    if not quiet:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError("the C++ compiler failed building _native.so")
+    os.replace(BINDING_OUT + ".tmp", BINDING_OUT)
+    return BINDING_OUT
+
+
 def build(force: bool = False, verbose_ptxas: bool = False, quiet: bool = False, trace: bool = False) -> str:
     """Build libspecq.so; trace=True builds libspecq_trace.so with the pipeline trace points."""
+    build_binding(force=force and not trace, quiet=quiet)
     out = OUT.replace("libspecq.so", "libspecq_trace.so") if trace else OUT
     if not force and not trace and up_to_date():
         return OUT

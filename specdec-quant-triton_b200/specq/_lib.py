@@ -88,6 +88,7 @@ SIGNATURES = {
 
 _lock = threading.Lock()
 _lib = None
+_native = None
 
 
 class SpecqError(RuntimeError):
@@ -116,6 +117,24 @@ def load():
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def native():
+    """The compiled binding of the block-scaled cache's operators, bound to the loaded library."""
+    global _native
+    if _native is not None:
+        return _native
+    lib = load()
+    with _lock:
+        if _native is None:
+            path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_native.so")
+            if not os.path.exists(path):
+                raise ImportError(f"_native.so not found at {path}; build it with "
+                                  "`python specdec-quant-triton_b200/build.py` (there is no fallback path)")
+            from . import _native as mod
+            mod.bind({name: C.cast(getattr(lib, name), C.c_void_p).value for name in SIGNATURES}, SpecqError)
+            _native = mod
+    return _native
 
 
 def check(rc: int):
