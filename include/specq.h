@@ -348,7 +348,8 @@ int specq_block_attention_workspace(int B, int n_seqs, int q_len, int ql_max, in
 
 /* Move the accepted drafts of each sequence together: accept[b, j] (strictly growing, < q_len),
  * j < n_accept[b], goes from position ctx_len[b] - q_len + accept[b, j] to ctx_len[b] - q_len + j,
- * in every one of L layers (kv_sl, s_sl: layer strides); ctx_out[b] = ctx_len[b] - q_len +
+ * in every one of L layers (kv_sl, s_sl: layer strides), acc_cols <= 64 and the drafts on at most 32
+ * pages; ctx_out[b] = ctx_len[b] - q_len +
  * n_accept[b] (ctx_out is not ctx_len).  A page's scale grows to hold what arrives from pages of
  * larger scale, and numbers whose scale differs are requantised.  A sequence with a bad index
  * keeps its tokens and its length (SPECQ_STATUS_BAD_INDEX).
@@ -367,7 +368,7 @@ int specq_block_compact(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_
  *   fork     row r with parent[r] = p >= 0, p != r becomes row p's first length[p] tokens: full
  *            pages shared, a part-filled last page copied (all L layers, filled slots and scales);
  *            every row or none, all at once (a permutation of beams is allowed).  scratch: int32
- *            [S * (C + 1)] device memory.
+ *            [S * (C + 2)] device memory.
  * short_out (device int32): pages missing, 0 when the call was carried out.
  */
 int specq_pages_release(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C,

@@ -15,10 +15,9 @@
 // touched.  An 8-bit number has no NaN or infinity here: a NaN is stored as 0, an infinity as
 // +-q_max, neither takes part in a, and SPECQ_STATUS_KV_NONFINITE is reported.
 //
-// A warp holds up to 16 slots of one page and head in registers (64 fp32 a thread at D = 128),
-// so the rotated values are made once and used twice, for the maximum and for the numbers; a
-// page of more than 16 tokens is shared by page / 16 warps of one CTA, which exchange their
-// maxima through shared memory.  The same launch turns the tokens' queries: they come from the
+// A warp holds 8 (16 at D = 64) slots of one page and head in registers, 32 fp32 a thread,
+// so the rotated values are made once and used twice, for the maximum and for the numbers; the
+// warps that share a larger page are of one CTA and exchange their maxima through shared memory.  The same launch turns the tokens' queries: they come from the
 // same rows, and a launch of their own costs a short verification step as much as the work.
 // Bound by HBM for prompts and by latency for a few tokens.
 //
@@ -37,7 +36,10 @@
 namespace specq {
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendSlots = 16;     // slots of a page that one warp holds
+constexpr int kAppendWarps = kAppendThreads / 32;
+// Slots of a page that one warp holds: 8 x 128 or 16 x 64 values are 32 fp32 a thread, which leaves
+// room for four blocks an SM (64 for 16 x 128 left room for two); a page of 128 slots of 128 needs 16.
+__host__ __device__ constexpr int append_slots(int D, int page) { return D == 128 && page <= 64 ? 8 : 16; }
 constexpr float kKvFloor = 1e-8f;
 
 template <int CT>   // 0 = int8, 1 = e4m3
@@ -134,40 +136,53 @@ __device__ __forceinline__ void append_extents(const BlockAppendParams& p, int& 
   }
 }
 
-template <typename T, int D, int CT, int HP>
+// Thread id of the tokens' queries: one 16-byte item of HP heads of a token.
+template <typename T, int HP>
+__device__ __forceinline__ void append_queries(const BlockAppendParams& p, uint32_t id, int n_seqs, int q_len) {
+  const uint32_t th = id / static_cast<uint32_t>(p.q_items);
+  const int item = static_cast<int>(id - th * p.q_items);
+  const int t = static_cast<int>(th / static_cast<uint32_t>(p.q_groups));
+  const int h0 = static_cast<int>(th - static_cast<uint32_t>(t) * p.q_groups) * HP;
+  if (t >= n_seqs * q_len) return;
+  int pos;
+  if (p.pos != nullptr) {
+    pos = __ldg(p.pos + t);
+  } else {
+    const int b = t / q_len;
+    pos = __ldg(p.ctx + b) - q_len + (t - b * q_len);
+  }
+  const float* row = rope_row(p.table, pos, p.n_pos, p.rot, p.status);
+  const T* x = static_cast<const T*>(p.q) + t * p.qt + h0 * p.qh;
+  T* out = static_cast<T*>(p.q_out) + t * p.ot + h0 * p.oh;
+  const int n = min(HP, p.h_q - h0);
+  if (p.half) rope_item<T, true, HP>(x, p.qh, out, p.oh, row, p.rot, 1.f, item, n);
+  else rope_item<T, false, HP>(x, p.qh, out, p.oh, row, p.rot, 1.f, item, n);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRopeThreads) block_append_queries_kernel(const __grid_constant__ BlockAppendParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  int n_seqs, q_len;
+  append_extents(p, n_seqs, q_len);
+  append_queries<T, kRopeHeads>(p, blockIdx.x * kRopeThreads + threadIdx.x, n_seqs, q_len);
+}
+
+template <typename T, int D, int CT, int SLOTS>
 __global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __grid_constant__ BlockAppendParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  __shared__ float red[kAppendThreads / 32];
+  __shared__ float red[kAppendWarps];
   int n_seqs, q_len;
   append_extents(p, n_seqs, q_len);
-
-  if (static_cast<int>(blockIdx.x) >= p.kv_blocks) {   // ---- queries
-    const uint32_t id = (blockIdx.x - p.kv_blocks) * kAppendThreads + threadIdx.x;
-    const uint32_t th = id / static_cast<uint32_t>(p.q_items);
-    const int item = static_cast<int>(id - th * p.q_items);
-    const int t = static_cast<int>(th / static_cast<uint32_t>(p.q_groups));
-    const int h0 = static_cast<int>(th - static_cast<uint32_t>(t) * p.q_groups) * HP;
-    if (t >= n_seqs * q_len) return;
-    int pos;
-    if (p.pos != nullptr) {
-      pos = __ldg(p.pos + t);
-    } else {
-      const int b = t / q_len;
-      pos = __ldg(p.ctx + b) - q_len + (t - b * q_len);
-    }
-    const float* row = rope_row(p.table, pos, p.n_pos, p.rot, p.status);
-    const T* x = static_cast<const T*>(p.q) + t * p.qt + h0 * p.qh;
-    T* out = static_cast<T*>(p.q_out) + t * p.ot + h0 * p.oh;
-    const int n = min(HP, p.h_q - h0);
-    if (p.half) rope_item<T, true, HP>(x, p.qh, out, p.oh, row, p.rot, 1.f, item, n);
-    else rope_item<T, false, HP>(x, p.qh, out, p.oh, row, p.rot, 1.f, item, n);
+  if (static_cast<int>(blockIdx.x) >= p.kv_blocks) {
+    append_queries<T, 1>(p, (blockIdx.x - p.kv_blocks) * kAppendThreads + threadIdx.x, n_seqs, q_len);
     return;
   }
 
   // ---- keys and values: (sequence, page of its window, group of (head, K|V) units)
   const int page = 1 << p.page_log2;
-  const int wpu = max(1, page / kAppendSlots);              // warps of a unit
+  const int wpu = max(1, page / SLOTS);                     // warps of a unit
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   const int bw = static_cast<int>(blockIdx.x) / p.win_blocks;
   const int part = static_cast<int>(blockIdx.x) - bw * p.win_blocks;
@@ -182,26 +197,22 @@ __global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __gr
   const int col = (base >> p.page_log2) + win;
   const int start = col << p.page_log2;                     // position of the page's slot 0
   if (start >= ctx) return;
-  const int pg = __ldg(p.bt + b * p.bt_sb + col);
-  if (pg < 0 || pg >= p.n_pages) {
-    if (threadIdx.x == 0 && part == 0) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
-    return;
-  }
-  const int unit = part * ((kAppendThreads / 32) / wpu) + warp / wpu;
+  const int pg = __ldg(p.bt + b * p.bt_sb + col);           // looked at after the rows' loads
+  const int unit = part * (kAppendWarps / wpu) + warp / wpu;
   const bool live = unit < 2 * p.h_kv;
   const bool is_v = unit >= p.h_kv;
   const int head = is_v ? unit - p.h_kv : unit;
-  const int sub = warp % wpu;                               // this warp's 16 slots of the page
+  const int sub = warp % wpu;                               // this warp's slots of the page
 
   constexpr int LPT = D / 8;            // lanes of a token
   constexpr int TPS = 32 / LPT;         // tokens of a step
-  constexpr int STEPS = kAppendSlots / TPS;
+  constexpr int STEPS = SLOTS / TPS;
   const int l = lane % LPT;
   const bool turn = !is_v && p.table != nullptr && 8 * l < p.rot;
   // the thread's 8 elements are two runs of 4: partners in the half layout
   const int o1 = turn && p.half ? 4 * l : 8 * l;
   const int o2 = turn && p.half ? (p.rot >> 1) + 4 * l : 8 * l + 4;
-  const int slot0 = sub * kAppendSlots + lane / LPT;
+  const int slot0 = sub * SLOTS + lane / LPT;
   float x[STEPS][8];
   float amax = 0.f;
   bool odd = false;
@@ -209,9 +220,6 @@ __global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __gr
   float* scale = nullptr;
   uint8_t* dst = nullptr;
   if (live) {
-    scale = (is_v ? p.vs : p.ks) + static_cast<int64_t>(pg) * p.s_sp + head * p.s_sh;
-    dst = (is_v ? p.vc : p.kc) + static_cast<int64_t>(pg) * p.kv_sp + head * p.kv_sh;
-    s_old = *scale;
     const T* src = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.vh : p.kh);
     const int64_t st = is_v ? p.vt : p.kt;
 #pragma unroll
@@ -226,6 +234,15 @@ __global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __gr
         load_row4<T>(r + o2, x[i] + 4);
       }
     }
+  }
+  if (pg < 0 || pg >= p.n_pages) {
+    if (threadIdx.x == 0 && part == 0) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+    return;
+  }
+  if (live) {
+    scale = (is_v ? p.vs : p.ks) + static_cast<int64_t>(pg) * p.s_sp + head * p.s_sh;
+    dst = (is_v ? p.vc : p.kc) + static_cast<int64_t>(pg) * p.kv_sp + head * p.kv_sh;
+    s_old = *scale;
     if (turn) {
 #pragma unroll
       for (int i = 0; i < STEPS; ++i) {
@@ -297,7 +314,7 @@ __global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __gr
   }
   if (!fresh && s_new > s_old) {        // the page's older tokens under the grown scale
     const float r = __fdiv_rn(s_old, s_new);
-    for (int slot = slot0; slot < min(base - start, (sub + 1) * kAppendSlots); slot += TPS) {
+    for (int slot = slot0; slot < min(base - start, (sub + 1) * SLOTS); slot += TPS) {
       uint2* d = reinterpret_cast<uint2*>(dst + static_cast<int64_t>(slot) * p.kv_so + 8 * l);
       uint2 w = *d;
       w.x = requant4<CT>(w.x, r);
@@ -360,9 +377,10 @@ inline int run_block_append(const void* k, int64_t kt, int64_t kh, const void* v
   p.n_seqs = n_seqs; p.q_len = q_len; p.b_grid = b_grid; p.ql_max = ql; p.h_kv = H_KV; p.h_q = H;
   p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.n_pages = n_pages; p.bt_cols = bt_cols; p.rot = rot; p.n_pos = n_pos; p.half = layout == 0;
-  const int wpu = std::max(1, page / kAppendSlots);
+  const int slots = append_slots(D, page);
+  const int wpu = std::max(1, page / slots);
   p.n_win = (ql - 1) / page + 2;
-  p.win_blocks = ceil_div(2 * H_KV, (kAppendThreads / 32) / wpu);
+  p.win_blocks = ceil_div(2 * H_KV, kAppendWarps / wpu);
   const int64_t kv_blocks = static_cast<int64_t>(b_grid) * p.n_win * p.win_blocks;
   int64_t q_blocks = 0;
   bool many = false;
@@ -374,27 +392,36 @@ inline int run_block_append(const void* k, int64_t kt, int64_t kh, const void* v
     p.q_groups = ceil_div(H, many ? kRopeHeads : 1);
     const int64_t threads = tokens * p.q_groups * p.q_items;
     if (threads > 0x7FFFFF00ll) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: too many query rows");
-    q_blocks = (threads + kAppendThreads - 1) / kAppendThreads;
+    // a few tokens' queries ride in the same launch; many go in one of their own, whose threads need
+    // half the registers (the prompt of 4 x 2047 tokens: 63 us in one launch)
+    const int block = many ? kRopeThreads : kAppendThreads;
+    q_blocks = (threads + block - 1) / block;
   }
   if (kv_blocks + q_blocks > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: too many tokens");
   p.kv_blocks = static_cast<int>(kv_blocks);
-  const dim3 grid(static_cast<unsigned>(kv_blocks + q_blocks));
+  const dim3 grid(static_cast<unsigned>(kv_blocks + (many ? 0 : q_blocks)));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto launch = [&](auto t, auto d, auto c, auto hp) {
-    return launch_plain(block_append_kernel<decltype(t), decltype(d)::value, decltype(c)::value, decltype(hp)::value>,
-                        grid, dim3(kAppendThreads), st, p);
+  auto launch = [&](auto t, auto d, auto c) -> cudaError_t {
+    using T = decltype(t);
+    constexpr int DD = decltype(d)::value, CT = decltype(c)::value;
+    if constexpr (DD == 128) {
+      if (slots == 8) return launch_plain(block_append_kernel<T, DD, CT, 8>, grid, dim3(kAppendThreads), st, p);
+    }
+    return launch_plain(block_append_kernel<T, DD, CT, 16>, grid, dim3(kAppendThreads), st, p);
   };
-  using One = std::integral_constant<int, 1>;
-  using Many = std::integral_constant<int, kRopeHeads>;
-  auto by_hp = [&](auto t, auto d, auto c) { return many ? launch(t, d, c, Many{}) : launch(t, d, c, One{}); };
   auto by_cache = [&](auto t, auto d) {
-    return cache_dtype == SPECQ_CACHE_INT8 ? by_hp(t, d, std::integral_constant<int, 0>{})
-                                           : by_hp(t, d, std::integral_constant<int, 1>{});
+    return cache_dtype == SPECQ_CACHE_INT8 ? launch(t, d, std::integral_constant<int, 0>{})
+                                           : launch(t, d, std::integral_constant<int, 1>{});
   };
   auto by_dim = [&](auto t) {
     return D == 64 ? by_cache(t, std::integral_constant<int, 64>{}) : by_cache(t, std::integral_constant<int, 128>{});
   };
   SPECQ_CUDA_TRY(dtype == 0 ? by_dim(__half{}) : by_dim(__nv_bfloat16{}));
+  if (many) {
+    const dim3 qg(static_cast<unsigned>(q_blocks));
+    SPECQ_CUDA_TRY(dtype == 0 ? launch_plain(block_append_queries_kernel<__half>, qg, dim3(kRopeThreads), st, p)
+                              : launch_plain(block_append_queries_kernel<__nv_bfloat16>, qg, dim3(kRopeThreads), st, p));
+  }
   return SPECQ_OK;
 }
 
@@ -414,7 +441,11 @@ struct BlockCompactParams {
 };
 
 constexpr int kCompactThreads = 128;
+constexpr int kCompactTokens = 64;   // accepted ones, whose indices a warp holds, two a lane
 
+// The indices, page numbers and scales of a warp's drafts stand in its lanes' registers, so the
+// chain of dependent loads is: lengths and indices; page numbers; scales and tokens.  Up to 16
+// (D = 128) or 32 (D = 64) moving tokens are read once, before the first is written.
 template <int D, int CT>
 __global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __grid_constant__ BlockCompactParams p) {
   pdl_launch_dependents();
@@ -427,38 +458,31 @@ __global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __
   const int layer = static_cast<int>(lb / static_cast<uint32_t>(p.B));
   const int b = static_cast<int>(lb - static_cast<uint32_t>(layer) * p.B);
   if (layer >= p.L) return;
-  const int page = 1 << p.page_log2;
+  const int page = 1 << p.page_log2, mask = page - 1;
   const bool first_unit = layer == 0 && unit == 0 && lane == 0;
-  const int ctx = __ldg(p.ctx + b);
-  const int base = ctx - p.q_len;
-  const int n_raw = __ldg(p.n_accept + b);
-  const int n = min(max(n_raw, 0), min(p.acc_cols, p.q_len));
-  // accept must grow strictly within the drafts, and the drafts lie in the table
   const int32_t* acc = p.accept + b * p.acc_sb;
-  bool ok = base >= 0 && ctx <= p.bt_cols * page && n == n_raw;
-  int same = n;                 // leading tokens that already stand where they belong
-  for (int j0 = 0; j0 < n; j0 += 32) {
-    const int j = j0 + lane;
-    bool good = true, moves = false;
-    if (j < n) {
-      const int a = __ldg(acc + j);
-      const int before = j > 0 ? __ldg(acc + j - 1) : -1;
-      good = a > before && a < p.q_len;
-      moves = a != j;
-    }
-    ok = ok && __all_sync(0xffffffffu, good);
-    const unsigned m = __ballot_sync(0xffffffffu, moves);
-    if (m != 0u && same == n) same = j0 + __ffs(m) - 1;
-  }
-  const int32_t* bt = p.bt + b * p.bt_sb;
-  if (ok && same < n) {         // and every page of theirs is one of the cache
-    bool good = true;
-    for (int c = (base >> p.page_log2) + lane; c <= (ctx - 1) >> p.page_log2; c += 32) {
-      const int pg = __ldg(bt + c);
-      good = good && pg >= 0 && pg < p.n_pages;
-    }
-    ok = __all_sync(0xffffffffu, good);
-  }
+  const int a0 = lane < p.acc_cols ? __ldg(acc + lane) : 0;
+  const int a1 = lane + 32 < p.acc_cols ? __ldg(acc + lane + 32) : 0;
+  const int ctx = __ldg(p.ctx + b);
+  const int n_raw = __ldg(p.n_accept + b);
+  const int base = ctx - p.q_len;
+  const int n = min(max(n_raw, 0), min(p.acc_cols, p.q_len));
+  const bool in_table = base >= 0 && ctx <= p.bt_cols * page;
+  // the drafts' pages, one a lane
+  const int col0 = base >> p.page_log2, n_win = ((ctx - 1) >> p.page_log2) - col0 + 1;
+  int pg = 0;
+  if (in_table && lane < n_win) pg = __ldg(p.bt + b * p.bt_sb + col0 + lane);
+  // accept must grow strictly within the drafts, the drafts lie in the table on pages of the cache
+  const int before0 = __shfl_up_sync(0xffffffffu, a0, 1), last0 = __shfl_sync(0xffffffffu, a0, 31);
+  const int before1 = __shfl_up_sync(0xffffffffu, a1, 1);
+  const bool good0 = lane >= n || (a0 > (lane == 0 ? -1 : before0) && a0 < p.q_len);
+  const bool good1 = lane + 32 >= n || (a1 > (lane == 0 ? last0 : before1) && a1 < p.q_len);
+  const unsigned moves0 = __ballot_sync(0xffffffffu, lane < n && a0 != lane);
+  const unsigned moves1 = __ballot_sync(0xffffffffu, lane + 32 < n && a1 != lane + 32);
+  // leading tokens that already stand where they belong
+  const int same = moves0 != 0u ? __ffs(moves0) - 1 : moves1 != 0u ? 31 + __ffs(moves1) : n;
+  bool ok = in_table && n == n_raw && __all_sync(0xffffffffu, good0 && good1);
+  if (same < n) ok = ok && __all_sync(0xffffffffu, lane >= n_win || (pg >= 0 && pg < p.n_pages));
   if (first_unit) {
     p.ctx_out[b] = ok ? base + n : ctx;
     if (!ok) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
@@ -469,31 +493,53 @@ __global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __
   const int head = is_v ? unit - p.h_kv : unit;
   uint8_t* cache = (is_v ? p.vc : p.kc) + layer * p.kv_sl + head * p.kv_sh;
   float* scale = (is_v ? p.vs : p.ks) + layer * p.s_sl + head * p.s_sh;
-  constexpr int LPT = D / 16, TPS = 32 / LPT;   // lanes of a token (16 bytes each), tokens of a step
-  constexpr int BATCH = 4;                      // steps in flight
+  float sc = 0.f;                                // of window page `lane`
+  if (lane < n_win) sc = scale[static_cast<int64_t>(pg) * p.s_sp];
+  constexpr int LPT = D / 16, TPS = 32 / LPT;    // lanes of a token (16 bytes each), tokens of a step
+  constexpr int BATCH = 4;                       // steps in flight
   const int sub = lane / LPT;
   const int byte = (lane % LPT) * 16;
-  const int mask = page - 1;
 
+  uint4 w[BATCH];
+  int swin[BATCH];
+  auto load = [&](int jb, int end) {
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int j = jb + i * TPS + sub;
+      const int lo = __shfl_sync(0xffffffffu, a0, j & 31), hi = __shfl_sync(0xffffffffu, a1, j & 31);
+      const int pos = base + (j < 32 ? lo : hi);
+      const int win = j < end ? (pos >> p.page_log2) - col0 : 0;
+      const int spg = __shfl_sync(0xffffffffu, pg, win);
+      swin[i] = win;
+      w[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (j < end)
+        w[i] = *reinterpret_cast<const uint4*>(cache + static_cast<int64_t>(spg) * p.kv_sp +
+                                               static_cast<int64_t>(pos & mask) * p.kv_so + byte);
+    }
+  };
+  // few enough tokens: all are read at once, for every target page
+  const bool once = n - same <= BATCH * TPS;
+  if (once) load(same, n);
   for (int j0 = same; j0 < n;) {
     const int dpos = base + j0;
-    const int dcol = dpos >> p.page_log2;
-    const int j1 = min(n, ((dcol + 1) << p.page_log2) - base);   // this target page takes tokens j0 .. j1 - 1
-    const int dpg = __ldg(bt + dcol);
-    uint8_t* dst = cache + static_cast<int64_t>(dpg) * p.kv_sp;
-    float* s_at = scale + static_cast<int64_t>(dpg) * p.s_sp;
-    const float s_old = *s_at;
+    const int dwin = (dpos >> p.page_log2) - col0;
+    const int j1 = min(n, ((col0 + dwin + 1) << p.page_log2) - base);   // this target page takes tokens j0 .. j1 - 1
+    uint8_t* dst = cache + static_cast<int64_t>(__shfl_sync(0xffffffffu, pg, dwin)) * p.kv_sp;
+    const float s_old = __shfl_sync(0xffffffffu, sc, dwin);
     // the arriving tokens' need; those of the page itself fit its scale already
     float need = 0.f;
-    for (int j = j0 + sub; j < j1; j += TPS) {
-      const int pos = base + __ldg(acc + j);
-      const int scol = pos >> p.page_log2;
-      if (scol == dcol) continue;
-      const int spg = __ldg(bt + scol);
-      const uint4 w = *reinterpret_cast<const uint4*>(cache + static_cast<int64_t>(spg) * p.kv_sp +
-                                                      static_cast<int64_t>(pos & mask) * p.kv_so + byte);
-      const float a = fmaxf(fmaxf(absmax4<CT>(w.x), absmax4<CT>(w.y)), fmaxf(absmax4<CT>(w.z), absmax4<CT>(w.w)));
-      need = fmaxf(need, a * cache_inv_max<CT>() * scale[static_cast<int64_t>(spg) * p.s_sp]);
+    const int jf = once ? same : j0;             // the first batch's first token
+    for (int jb = jf; jb < j1; jb += BATCH * TPS) {
+      if (!once) load(jb, j1);
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const float ss = __shfl_sync(0xffffffffu, sc, swin[i]);
+        const int j = jb + i * TPS + sub;
+        if (j >= j0 && j < j1 && swin[i] != dwin) {
+          const float a = fmaxf(fmaxf(absmax4<CT>(w[i].x), absmax4<CT>(w[i].y)), fmaxf(absmax4<CT>(w[i].z), absmax4<CT>(w[i].w)));
+          need = fmaxf(need, a * cache_inv_max<CT>() * ss);
+        }
+      }
     }
     need = warp_max_f32(need);
     const float s_new = fmaxf(s_old, need);
@@ -502,46 +548,32 @@ __global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __
       const int keep = dpos & mask;
       for (int slot = sub; slot < keep; slot += TPS) {
         uint4* d = reinterpret_cast<uint4*>(dst + static_cast<int64_t>(slot) * p.kv_so + byte);
-        uint4 w = *d;
-        w.x = requant4<CT>(w.x, r); w.y = requant4<CT>(w.y, r);
-        w.z = requant4<CT>(w.z, r); w.w = requant4<CT>(w.w, r);
-        *d = w;
+        uint4 x = *d;
+        x.x = requant4<CT>(x.x, r); x.y = requant4<CT>(x.y, r);
+        x.z = requant4<CT>(x.z, r); x.w = requant4<CT>(x.w, r);
+        *d = x;
       }
     }
-    for (int jb = j0; jb < j1; jb += BATCH * TPS) {
-      uint4 w[BATCH];
-      float r[BATCH];
-#pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        const int j = jb + i * TPS + sub;
-        w[i] = make_uint4(0u, 0u, 0u, 0u);
-        r[i] = 1.f;
-        if (j < j1) {
-          const int pos = base + __ldg(acc + j);
-          const int scol = pos >> p.page_log2;
-          const int spg = __ldg(bt + scol);
-          w[i] = *reinterpret_cast<const uint4*>(cache + static_cast<int64_t>(spg) * p.kv_sp +
-                                                 static_cast<int64_t>(pos & mask) * p.kv_so + byte);
-          const float ss = scol == dcol ? s_old : scale[static_cast<int64_t>(spg) * p.s_sp];
-          if (ss != s_new) r[i] = __fdiv_rn(ss, s_new);
-        }
-      }
+    for (int jb = jf; jb < j1; jb += BATCH * TPS) {
+      if (!once && j1 - j0 > BATCH * TPS) load(jb, j1);   // otherwise they are in the registers still
       __syncwarp();             // every read of the batch before its writes
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
         const int j = jb + i * TPS + sub;
-        if (j < j1) {
-          if (r[i] != 1.f) {
-            w[i].x = requant4<CT>(w[i].x, r[i]); w[i].y = requant4<CT>(w[i].y, r[i]);
-            w[i].z = requant4<CT>(w[i].z, r[i]); w[i].w = requant4<CT>(w[i].w, r[i]);
+        const float ss = __shfl_sync(0xffffffffu, sc, swin[i]);
+        if (j >= j0 && j < j1) {
+          uint4 x = w[i];
+          if (ss != s_new) {
+            const float r = __fdiv_rn(ss, s_new);
+            x.x = requant4<CT>(x.x, r); x.y = requant4<CT>(x.y, r);
+            x.z = requant4<CT>(x.z, r); x.w = requant4<CT>(x.w, r);
           }
-          *reinterpret_cast<uint4*>(dst + static_cast<int64_t>((base + j) & mask) * p.kv_so + byte) = w[i];
+          *reinterpret_cast<uint4*>(dst + static_cast<int64_t>((base + j) & mask) * p.kv_so + byte) = x;
         }
       }
       __syncwarp();
     }
-    if (lane == 0 && s_new != s_old) *s_at = s_new;
-    __syncwarp();
+    if (lane == dwin && s_new != s_old) scale[static_cast<int64_t>(pg) * p.s_sp] = s_new;
     j0 = j1;
   }
 }
@@ -557,6 +589,9 @@ inline int run_block_compact(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, i
     return fail(SPECQ_ERR_INVALID_ARG, "block_compact: cache dtype code %d", cache_dtype);
   if (D != 64 && D != 128) return fail(SPECQ_ERR_UNSUPPORTED, "block_compact: head_dim %d (this build supports 64 and 128)", D);
   if (!page_ok(page)) return fail(SPECQ_ERR_UNSUPPORTED, "block_compact: page %d (a power of two in 8..128)", page);
+  if (acc_cols > kCompactTokens || (q_len - 1) / page + 2 > 32)
+    return fail(SPECQ_ERR_UNSUPPORTED, "block_compact: %d accepted tokens > %d, or %d drafts over more than 32 pages of %d",
+                acc_cols, kCompactTokens, q_len, page);
   if (B == 0) return SPECQ_OK;
   if (kc == nullptr || vc == nullptr || ks == nullptr || vs == nullptr || bt == nullptr || ctx == nullptr ||
       n_accept == nullptr || ctx_out == nullptr || (acc_cols > 0 && accept == nullptr))

@@ -1,7 +1,7 @@
 // pages.cuh -- the page pool of a paged KV cache on the device: release, reserve, fork.
 //
 // State: ref [P] (how many rows hold a page; 0 = free), tbl [S, C] (the rows' pages, -1 past
-// the held ones) and held [S] (pages a row holds).  There is no free list: a page is free when
+// the held ones, which every call keeps so) and held [S] (pages a row holds).  There is no free list: a page is free when
 // its count is 0, and pages are handed out lowest index first, row by row, so the result of
 // every call is a function of the state alone (the atomics below add integers, whose order
 // does not matter, or claim nothing).
@@ -16,10 +16,11 @@
 //          were, so beams can be permuted.  Again all or none, short = the missing pages.
 //
 // The work is a few kilobytes of integers, so what counts is the number of dependent steps.
-// reserve is one CTA that reads ref in runs of 16 counts a thread (16,384 pages a step, one
-// block scan each) and stops when it has found enough.  fork is that CTA, then a grid that
-// snapshots the parents' rows and copies the pages (bound by HBM), then a grid that writes the
-// rows; the kernels follow one another by programmatic launch.
+// reserve is one CTA that reads ref in runs of 8 counts a thread (8,192 pages a step, one
+// block scan each, the free ones listed in shared memory and placed by a warp a row) and stops when it has found enough.  fork is that CTA, which up to
+// kForkSmall table cells also rewrites the rows between two barriers, and then a grid that copies
+// the pages (bound by HBM); a larger table is snapshot by the copying grid and rewritten by a
+// third.  The kernels follow one another by programmatic launch.
 #pragma once
 
 #include "sm100.cuh"
@@ -28,7 +29,7 @@
 namespace specq {
 
 constexpr int kPoolThreads = 1024;
-constexpr int kPoolRun = 16;       // counts a thread reads in one step
+constexpr int kPoolRun = 8;        // counts a thread reads in one step
 constexpr int kPoolMaxRows = 8192; // rows of a table: their prefix sums stand in shared memory
 
 struct PagePool {
@@ -50,14 +51,12 @@ __global__ void __launch_bounds__(128) pages_release_kernel(const __grid_constan
   if (drop[r] == 0) return;
   const int n = pool_held(p, r);
   int32_t* row = p.tbl + r * p.ld;
-  for (int c = threadIdx.x; c < p.C; c += 128) {
-    if (c < n) {
-      const int pg = row[c];
-      if (pg < 0 || pg >= p.P) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
-      else if (atomicSub(p.ref + pg, 1) <= 0) {   // a count that was already 0 stays 0
-        atomicAdd(p.ref + pg, 1);
-        report_status(p.status, SPECQ_STATUS_BAD_INDEX);
-      }
+  for (int c = threadIdx.x; c < n; c += 128) {
+    const int pg = row[c];
+    if (pg < 0 || pg >= p.P) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+    else if (atomicSub(p.ref + pg, 1) <= 0) {   // a count that was already 0 stays 0
+      atomicAdd(p.ref + pg, 1);
+      report_status(p.status, SPECQ_STATUS_BAD_INDEX);
     }
     row[c] = -1;
   }
@@ -111,11 +110,12 @@ __device__ __forceinline__ int pool_starts(int S, int* start, int* red, Need nee
   return total;
 }
 
-// Calls give(rank, page) for the `total` lowest free pages, in any order, if there are as many;
-// returns how many are missing.  The first pass only counts; a call whose first step already
-// finds enough pages counts and gives in that one step.
-template <typename Give>
-__device__ __forceinline__ int pool_take(const PagePool& p, int total, int* red, Give give) {
+// Finds the `total` lowest free pages, if there are as many, and hands them over a step at a time:
+// use(rank, list, count) by every thread, list[i] being the free page of rank `rank` + i.  Returns
+// how many pages are missing.  A call whose first step finds enough looks at the counts once;
+// others count first, since nothing may be handed over when pages are missing.
+template <typename Use>
+__device__ __forceinline__ int pool_take(const PagePool& p, int total, int* red, int* list, Use use) {
   const int step = kPoolThreads * kPoolRun;
   for (int pass = 0; pass < 2; ++pass) {
     int found = 0;
@@ -133,15 +133,14 @@ __device__ __forceinline__ int pool_take(const PagePool& p, int total, int* red,
           if (first + i < p.P && p.ref[first + i] == 0) free_bits |= 1u << i;
       }
       int sum;
-      int rank = found + block_exclusive(__popc(free_bits), red, &sum);
+      int at = block_exclusive(__popc(free_bits), red, &sum);
       if (pass == 1 || (p0 == 0 && sum >= total)) {
-        while (free_bits != 0u && rank < total) {
-          const int i = __ffs(free_bits) - 1;
-          free_bits &= free_bits - 1u;
-          give(rank++, first + i);
-        }
+        for (; free_bits != 0u; free_bits &= free_bits - 1u) list[at++] = first + __ffs(free_bits) - 1;
+        __syncthreads();
+        use(found, list, min(sum, total - found));
+        __syncthreads();
+        if (pass == 0) return 0;
       }
-      if (pass == 0 && p0 == 0 && sum >= total) return 0;
       found += sum;
     }
     if (found < total) return total - found;
@@ -149,23 +148,16 @@ __device__ __forceinline__ int pool_take(const PagePool& p, int total, int* red,
   return 0;
 }
 
-// The row whose pages include rank k: the last r with start[r] <= k among rows that take any.
-__device__ __forceinline__ int pool_row_of(const int* start, int S, int k) {
-  int lo = 0, hi = S;      // start[lo] <= k < start[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (start[mid] <= k) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
+inline size_t pool_smem(int S) { return (static_cast<size_t>(kPoolThreads) * kPoolRun + S + 1) * sizeof(int); }
 
 __global__ void __launch_bounds__(kPoolThreads) pages_reserve_kernel(const __grid_constant__ PagePool p, const int32_t* want,
                                                                      int page, int32_t* short_out) {
   pdl_launch_dependents();
   pdl_wait();
-  extern __shared__ int start[];          // [S + 1]
+  extern __shared__ int list[];           // [kPoolThreads * kPoolRun], then start [S + 1]
+  int* start = list + kPoolThreads * kPoolRun;
   __shared__ int red[33];
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   auto need = [&](int r) {
     const int w = want[r];
     int cols = w <= 0 ? 0 : (w - 1) / page + 1;
@@ -178,10 +170,17 @@ __global__ void __launch_bounds__(kPoolThreads) pages_reserve_kernel(const __gri
   const int total = pool_starts(p.S, start, red, need);
   int missing = 0;
   if (total > 0) {
-    missing = pool_take(p, total, red, [&](int k, int pg) {
-      const int r = pool_row_of(start, p.S, k);
-      p.tbl[r * p.ld + pool_held(p, r) + k - start[r]] = pg;
-      p.ref[pg] = 1;
+    missing = pool_take(p, total, red, list, [&](int rank, const int* pages, int count) {
+      for (int r = warp; r < p.S; r += kPoolThreads / 32) {
+        const int lo = max(start[r], rank), hi = min(start[r + 1], rank + count);
+        if (lo >= hi) continue;
+        int32_t* cell = p.tbl + r * p.ld + pool_held(p, r) - start[r];
+        for (int k = lo + lane; k < hi; k += 32) {
+          const int pg = pages[k - rank];
+          cell[k] = pg;
+          p.ref[pg] = 1;
+        }
+      }
     });
   }
   __syncthreads();                        // the pages are placed by the old held
@@ -199,6 +198,7 @@ struct PageForkParams {
   const int32_t* length;   // [S]
   int32_t* snap;           // [S, C] scratch: the rows to be
   int32_t* fresh;          // [S] scratch: the copied page, -1 without one, -2 where the row stays
+  int32_t* from;           // [S] scratch: the page it is copied from
   int32_t* short_out;
   uint8_t* kc;
   uint8_t* vc;
@@ -206,7 +206,44 @@ struct PageForkParams {
   float* vs;
   int64_t kv_sl, kv_sp, kv_so, kv_sh, s_sl, s_sp, s_sh;
   int page, h_kv, D, L;
+  int small;               // the table is rewritten by the planning CTA
+  int dense;               // a page's tokens and heads are contiguous
 };
+
+constexpr int kForkSmall = 2048;   // S * C: 2 cells a thread of the planning CTA (at 14,784 it takes 25 us for them)
+
+// Row r, which is forked with `to` as its copied page, takes its share of the parent's pages:
+// snapshot (before any row is rewritten) and rewrite, each by `step` threads from `c0`.
+__device__ __forceinline__ void fork_snapshot(const PageForkParams& f, int r, int c0, int step) {
+  const int p = f.parent[r], full = f.length[p] / f.page;
+  const int32_t* from_row = f.pool.tbl + p * f.pool.ld;
+  int32_t* snap = f.snap + static_cast<int64_t>(r) * f.pool.C;
+  for (int c = c0; c < full; c += step) {
+    const int pg = from_row[c];
+    snap[c] = pg;
+    if (pg < 0 || pg >= f.pool.P) report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
+    else atomicAdd(f.pool.ref + pg, 1);
+  }
+}
+__device__ __forceinline__ void fork_rewrite(const PageForkParams& f, int r, int to, int c0, int step) {
+  const int full = f.length[f.parent[r]] / f.page, had = pool_held(f.pool, r);
+  int32_t* row = f.pool.tbl + r * f.pool.ld;
+  const int32_t* snap = f.snap + static_cast<int64_t>(r) * f.pool.C;
+  for (int c = c0; c < max(had, full + (to >= 0 ? 1 : 0)); c += step) {
+    if (c < had) {
+      const int pg = row[c];
+      if (pg < 0 || pg >= f.pool.P) report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
+      else if (atomicSub(f.pool.ref + pg, 1) <= 0) {
+        atomicAdd(f.pool.ref + pg, 1);
+        report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
+      }
+    }
+    row[c] = c < full ? snap[c] : (c == full && to >= 0 ? to : -1);
+  }
+}
+__device__ __forceinline__ int fork_held(const PageForkParams& f, int r, int to) {
+  return f.length[f.parent[r]] / f.page + (to >= 0 ? 1 : 0);
+}
 
 // parent of row r, or -1 where the row stays as it is
 __device__ __forceinline__ int fork_parent(const PageForkParams& f, int r, bool tell) {
@@ -224,82 +261,103 @@ __device__ __forceinline__ int fork_parent(const PageForkParams& f, int r, bool 
 __global__ void __launch_bounds__(kPoolThreads) pages_fork_plan_kernel(const __grid_constant__ PageForkParams f) {
   pdl_launch_dependents();
   pdl_wait();
-  extern __shared__ int start[];
+  extern __shared__ int list[];
+  int* start = list + kPoolThreads * kPoolRun;
   __shared__ int red[33];
   auto need = [&](int r) {
     const int p = fork_parent(f, r, true);
     f.fresh[r] = p < 0 ? -2 : -1;
-    return p >= 0 && f.length[p] % f.page != 0 ? 1 : 0;
+    if (p < 0) return 0;
+    const int n = f.length[p], full = n / f.page;
+    if (n == full * f.page) return 0;
+    f.from[r] = f.pool.tbl[p * f.pool.ld + full];
+    return 1;
   };
   const int total = pool_starts(f.pool.S, start, red, need);
   int missing = 0;
   if (total > 0) {
-    missing = pool_take(f.pool, total, red, [&](int k, int pg) {
-      f.fresh[pool_row_of(start, f.pool.S, k)] = pg;
-      f.pool.ref[pg] = 1;
+    missing = pool_take(f.pool, total, red, list, [&](int rank, const int* pages, int count) {
+      for (int r = threadIdx.x; r < f.pool.S; r += kPoolThreads) {
+        const int k = start[r];
+        if (start[r + 1] > k && k >= rank && k < rank + count) {
+          f.fresh[r] = pages[k - rank];
+          f.pool.ref[pages[k - rank]] = 1;
+        }
+      }
     });
   }
   if (missing > 0)
     for (int r = threadIdx.x; r < f.pool.S; r += kPoolThreads) f.fresh[r] = -2;
   if (threadIdx.x == 0) *f.short_out = missing;
+  if (f.small == 0 || missing > 0) return;
+  __syncthreads();
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  for (int r = warp; r < f.pool.S; r += kPoolThreads / 32)
+    if (f.fresh[r] != -2) fork_snapshot(f, r, lane, 32);
+  __syncthreads();
+  for (int r = warp; r < f.pool.S; r += kPoolThreads / 32) {
+    const int to = f.fresh[r];
+    if (to == -2) continue;
+    fork_rewrite(f, r, to, lane, 32);
+    __syncwarp();          // every lane has read held[r]
+    if (lane == 0) f.pool.held[r] = fork_held(f, r, to);
+  }
 }
 
 constexpr int kForkThreads = 256;
 
-// block (row, 2 * layer + K|V), and one more y: the parents' rows
+// Block (row, y) copies the row's page in the (layer, K|V) pairs y, y + Y, ...; the blocks of y = 0
+// also snapshot the parents' rows of a large table.
 __global__ void __launch_bounds__(kForkThreads) pages_fork_copy_kernel(const __grid_constant__ PageForkParams f) {
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.x;
   const int to = f.fresh[r];
   if (to == -2) return;
-  const int p = f.parent[r];
-  const int n = f.length[p];
-  const int full = n / f.page, rest = n - full * f.page;
-  const int32_t* from_row = f.pool.tbl + p * f.pool.ld;
-  if (blockIdx.y == 0) {
-    int32_t* snap = f.snap + static_cast<int64_t>(r) * f.pool.C;
-    for (int c = threadIdx.x; c < full; c += kForkThreads) {
-      const int pg = from_row[c];
-      snap[c] = pg;
-      if (pg < 0 || pg >= f.pool.P) report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
-      else atomicAdd(f.pool.ref + pg, 1);
-    }
-    return;
-  }
-  if (rest == 0) return;
-  const int from = from_row[full];
+  if (f.small == 0 && blockIdx.y == 0) fork_snapshot(f, r, threadIdx.x, kForkThreads);
+  if (to < 0) return;
+  const int n = f.length[f.parent[r]];
+  const int rest = n - n / f.page * f.page;
+  const int from = f.from[r];
   if (from < 0 || from >= f.pool.P) {
     if (threadIdx.x == 0) report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
     return;
   }
-  const int layer = (blockIdx.y - 1) >> 1;
-  const bool is_v = (blockIdx.y - 1) & 1;
-  uint8_t* cache = (is_v ? f.vc : f.kc) + layer * f.kv_sl;
-  const uint8_t* src = cache + from * f.kv_sp;
-  uint8_t* dst = cache + to * f.kv_sp;
-  const int chunks = f.D >> 4, per_slot = f.h_kv * chunks, items = rest * per_slot;
-  constexpr int U = 4;
-  for (int i0 = threadIdx.x; i0 < items; i0 += U * kForkThreads) {
+  // all pairs' 16-byte pieces as one run, several loads in flight
+  const unsigned chunks = f.D >> 4, per_slot = f.h_kv * chunks, items = rest * per_slot;
+  const unsigned pairs = (2 * f.L - blockIdx.y + gridDim.y - 1) / gridDim.y;
+  constexpr int U = 8;
+  for (unsigned i0 = threadIdx.x; i0 < items * pairs; i0 += U * kForkThreads) {
     uint4 w[U];
-    int64_t at[U];
+    uint8_t* at[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kForkThreads;
-      if (i < items) {
-        const int slot = i / per_slot, in = i - slot * per_slot;
-        const int h = in / chunks, c = in - h * chunks;
-        at[u] = slot * f.kv_so + h * f.kv_sh + c * 16;
-        w[u] = *reinterpret_cast<const uint4*>(src + at[u]);
+      const unsigned i = i0 + u * kForkThreads;
+      at[u] = nullptr;
+      if (i < items * pairs) {
+        const unsigned pair = i / items, in = i - pair * items;
+        const unsigned y = blockIdx.y + pair * gridDim.y;
+        int64_t off;
+        if (f.dense) {
+          off = static_cast<int64_t>(in) * 16;
+        } else {
+          const unsigned slot = in / per_slot, rest_in = in - slot * per_slot, h = rest_in / chunks;
+          off = slot * f.kv_so + h * f.kv_sh + (rest_in - h * chunks) * 16;
+        }
+        uint8_t* base = ((y & 1) ? f.vc : f.kc) + (y >> 1) * f.kv_sl + off;
+        at[u] = base + to * f.kv_sp;
+        w[u] = *reinterpret_cast<const uint4*>(base + from * f.kv_sp);
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (i0 + u * kForkThreads < items) *reinterpret_cast<uint4*>(dst + at[u]) = w[u];
+      if (at[u] != nullptr) *reinterpret_cast<uint4*>(at[u]) = w[u];
   }
-  float* scale = (is_v ? f.vs : f.ks) + layer * f.s_sl;
-  for (int h = threadIdx.x; h < f.h_kv; h += kForkThreads)
-    scale[to * f.s_sp + h * f.s_sh] = scale[from * f.s_sp + h * f.s_sh];
+  for (unsigned i = threadIdx.x; i < pairs * f.h_kv; i += kForkThreads) {
+    const unsigned pair = i / f.h_kv, h = i - pair * f.h_kv, y = blockIdx.y + pair * gridDim.y;
+    float* scale = ((y & 1) ? f.vs : f.ks) + (y >> 1) * f.s_sl + h * f.s_sh;
+    scale[to * f.s_sp] = scale[from * f.s_sp];
+  }
 }
 
 __global__ void __launch_bounds__(128) pages_fork_rows_kernel(const __grid_constant__ PageForkParams f) {
@@ -308,24 +366,9 @@ __global__ void __launch_bounds__(128) pages_fork_rows_kernel(const __grid_const
   const int r = blockIdx.x;
   const int to = f.fresh[r];
   if (to == -2) return;
-  const int n = f.length[f.parent[r]];
-  const int full = n / f.page;
-  const int had = pool_held(f.pool, r);
-  int32_t* row = f.pool.tbl + r * f.pool.ld;
-  const int32_t* snap = f.snap + static_cast<int64_t>(r) * f.pool.C;
-  for (int c = threadIdx.x; c < f.pool.C; c += 128) {
-    if (c < had) {
-      const int pg = row[c];
-      if (pg < 0 || pg >= f.pool.P) report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
-      else if (atomicSub(f.pool.ref + pg, 1) <= 0) {
-        atomicAdd(f.pool.ref + pg, 1);
-        report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
-      }
-    }
-    row[c] = c < full ? snap[c] : (c == full && to >= 0 ? to : -1);
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) f.pool.held[r] = full + (to >= 0 ? 1 : 0);
+  fork_rewrite(f, r, to, threadIdx.x, 128);
+  __syncthreads();         // every thread has read held[r]
+  if (threadIdx.x == 0) f.pool.held[r] = fork_held(f, r, to);
 }
 
 inline int make_pool(const char* who, PagePool* p, int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held,
@@ -349,10 +392,12 @@ inline int pool_device(PagePool* p) {
 
 inline cudaError_t launch_pool(void (*kern)(PagePool, const int32_t*, int, int32_t*), const PagePool& p, const int32_t* want,
                                int page, int32_t* short_out, cudaStream_t st) {
+  const cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), static_cast<int>(pool_smem(p.S)));
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1);
   cfg.blockDim = dim3(kPoolThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(p.S + 1) * sizeof(int);
+  cfg.dynamicSmemBytes = pool_smem(p.S);
   cfg.stream = st;
   LaunchAttrs at(1);
   at.apply(cfg);
@@ -397,22 +442,30 @@ inline int run_pages_fork(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int6
   if (!aligned(kc, 16) || !aligned(vc, 16) || kv_sl % 16 || kv_sp % 16 || kv_so % 16 || kv_sh % 16)
     return fail(SPECQ_ERR_UNSUPPORTED, "pages_fork: cache rows must be 16-byte aligned");
   if (int rc = pool_device(&f.pool)) return rc;
-  f.parent = parent; f.length = length; f.fresh = scratch; f.snap = scratch + S; f.short_out = short_out;
+  f.parent = parent; f.length = length; f.short_out = short_out;
+  f.fresh = scratch; f.from = scratch + S; f.snap = scratch + 2 * static_cast<int64_t>(S);
   f.kc = static_cast<uint8_t*>(kc); f.vc = static_cast<uint8_t*>(vc); f.ks = ks; f.vs = vs;
   f.kv_sl = kv_sl; f.kv_sp = kv_sp; f.kv_so = kv_so; f.kv_sh = kv_sh; f.s_sl = s_sl; f.s_sp = s_sp; f.s_sh = s_sh;
   f.page = page; f.h_kv = H_KV; f.D = D; f.L = L;
+  f.small = static_cast<int64_t>(S) * C <= kForkSmall;
+  f.dense = kv_sh == D && kv_so == static_cast<int64_t>(H_KV) * D;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  SPECQ_CUDA_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(pages_fork_plan_kernel), static_cast<int>(pool_smem(S))));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(1);
   cfg.blockDim = dim3(kPoolThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(S + 1) * sizeof(int);
+  cfg.dynamicSmemBytes = pool_smem(S);
   cfg.stream = st;
   LaunchAttrs at(1);
   at.apply(cfg);
   SPECQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, pages_fork_plan_kernel, f));
   if (S == 0) return SPECQ_OK;
-  SPECQ_CUDA_TRY(launch_plain(pages_fork_copy_kernel, dim3(S, 1 + 2 * L), dim3(kForkThreads), st, f));
-  SPECQ_CUDA_TRY(launch_plain(pages_fork_rows_kernel, dim3(S), dim3(128), st, f));
+  // enough blocks for eight an SM; each then copies several layers' pages with its loads in flight
+  DeviceState* dev = nullptr;
+  if (int rc = get_device_state(&dev)) return rc;
+  const int y = std::max(1, std::min(2 * L, ceil_div(8 * dev->sm_count, S)));
+  if (L > 0 || f.small == 0) SPECQ_CUDA_TRY(launch_plain(pages_fork_copy_kernel, dim3(S, y), dim3(kForkThreads), st, f));
+  if (f.small == 0) SPECQ_CUDA_TRY(launch_plain(pages_fork_rows_kernel, dim3(S), dim3(128), st, f));
   return SPECQ_OK;
 }
 

@@ -418,7 +418,7 @@ PyObject* pages_fork(PyObject* const* a) {
   if (given != nullptr) int32s(who, "short", *given, 1, 1);
   same_device(who, {&p.ref, &c.kc, &c.vc, &c.ks, &c.vs, &p.tbl, &p.held, &parent, &length, given});
   const Tensor out = given != nullptr ? *given : new_int32(p.ref, 1);
-  const Tensor scratch = new_int32(p.ref, static_cast<int64_t>(p.S) * (p.C + 1));
+  const Tensor scratch = new_int32(p.ref, static_cast<int64_t>(p.S) * (p.C + 2));
   const int d = c.d;
   check(lib.pages_fork(c.kc.data_ptr(), c.vc.data_ptr(), c.sl(), c.kc.stride(d), c.kc.stride(d + 1), c.kc.stride(d + 2), size32(who, c.L),
                        ptr<float>(c.ks), ptr<float>(c.vs), c.s_sl(), c.ks.stride(d), c.ks.stride(d + 1), ptr<int32_t>(p.ref), p.P,

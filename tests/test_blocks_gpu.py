@@ -512,7 +512,7 @@ def _pool_state(gen, S, C, P):
     return [t.to(torch.int32) for t in (ref, tbl, held)]
 
 
-@pytest.mark.parametrize("S,C,P,page", [(1, 1, 2, 16), (5, 7, 60, 8), (40, 33, 2000, 16), (1100, 9, 20011, 16),
+@pytest.mark.parametrize("S,C,P,page", [(1, 1, 2, 16), (5, 7, 60, 8), (40, 33, 2000, 16), (1100, 9, 20011, 16), (700, 40, 30000, 8),
                                         (64, 20, 40000, 32)])
 def test_pool_against_the_oracle(cuda, S, C, P, page):
     import specq
