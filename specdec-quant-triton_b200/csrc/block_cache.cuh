@@ -45,17 +45,14 @@ constexpr float kKvFloor = 1e-8f;
 template <int CT>   // 0 = int8, 1 = e4m3
 __host__ __device__ constexpr float cache_inv_max() { return CT == 0 ? 1.0f / 127.0f : 1.0f / 448.0f; }
 
-// Four fp32 to four saturated 8-bit numbers (round to nearest even); none of v is NaN.
+// Four fp32 to four 8-bit numbers (round to nearest even).  None of them is NaN; int8: none rounds
+// to more than 127 in magnitude.
 template <int CT>
 __device__ __forceinline__ uint32_t pack_cache4(float a, float b, float c, float d) {
   if constexpr (CT == 0) {
-    const float v[4] = {a, b, c, d};
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int q = static_cast<int>(rintf(fminf(fmaxf(v[i], -127.f), 127.f)));
-      w |= (static_cast<uint32_t>(q) & 0xFFu) << (8 * i);
-    }
+    uint32_t lo, w;
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, 0;" : "=r"(lo) : "r"(__float2int_rn(d)), "r"(__float2int_rn(c)));
+    asm("cvt.pack.sat.s8.s32.b32 %0, %1, %2, %3;" : "=r"(w) : "r"(__float2int_rn(b)), "r"(__float2int_rn(a)), "r"(lo));
     return w;
   } else {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
@@ -80,7 +77,7 @@ __device__ __forceinline__ void unpack_cache4(uint32_t w, float (&v)[4]) {
   }
 }
 
-// rn(q * r) of four stored numbers
+// rn(q * r) of four stored numbers, r <= 1 (a stored -128 is not one of this cache's)
 template <int CT>
 __device__ __forceinline__ uint32_t requant4(uint32_t w, float r) {
   float v[4];
@@ -88,11 +85,27 @@ __device__ __forceinline__ uint32_t requant4(uint32_t w, float r) {
   return pack_cache4<CT>(v[0] * r, v[1] * r, v[2] * r, v[3] * r);
 }
 
+// The largest magnitude of 16 stored numbers; exact in fp16, two at a time.
 template <int CT>
-__device__ __forceinline__ float absmax4(uint32_t w) {
-  float v[4];
-  unpack_cache4<CT>(w, v);
-  return fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+__device__ __forceinline__ float absmax16(const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  __half2 m = __half2(__half_raw{0}, __half_raw{0});
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __half2 a, b;
+    if constexpr (CT == 0) {          // 1024 + (byte ^ 0x80), less 1152
+      const uint32_t x = w[i] ^ 0x80808080u;
+      const uint32_t lo = __byte_perm(x, 0x64646464u, 0x4140), hi = __byte_perm(x, 0x64646464u, 0x4342);
+      const __half2 off = __half2(__half_raw{0x6480}, __half_raw{0x6480});
+      a = __hsub2(*reinterpret_cast<const __half2*>(&lo), off);
+      b = __hsub2(*reinterpret_cast<const __half2*>(&hi), off);
+    } else {
+      a = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] & 0xFFFFu), __NV_E4M3));
+      b = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w[i] >> 16), __NV_E4M3));
+    }
+    m = __hmax2(m, __hmax2(__habs2(a), __habs2(b)));
+  }
+  return __half2float(__hmax(__low2half(m), __high2half(m)));
 }
 
 struct BlockAppendParams {
@@ -159,24 +172,16 @@ __device__ __forceinline__ void append_queries(const BlockAppendParams& p, uint3
   else rope_item<T, false, HP>(x, p.qh, out, p.oh, row, p.rot, 1.f, item, n);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRopeThreads) block_append_queries_kernel(const __grid_constant__ BlockAppendParams p) {
-  pdl_launch_dependents();
-  pdl_wait();
-  int n_seqs, q_len;
-  append_extents(p, n_seqs, q_len);
-  append_queries<T, kRopeHeads>(p, blockIdx.x * kRopeThreads + threadIdx.x, n_seqs, q_len);
-}
-
-template <typename T, int D, int CT, int SLOTS>
-__global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __grid_constant__ BlockAppendParams p) {
+template <typename T, int D, int CT, int SLOTS, int HP>
+__global__ void __launch_bounds__(kAppendThreads, SLOTS * D <= 1024 ? 4 : 2)
+block_append_kernel(const __grid_constant__ BlockAppendParams p) {
   pdl_launch_dependents();
   pdl_wait();
   __shared__ float red[kAppendWarps];
   int n_seqs, q_len;
   append_extents(p, n_seqs, q_len);
   if (static_cast<int>(blockIdx.x) >= p.kv_blocks) {
-    append_queries<T, 1>(p, (blockIdx.x - p.kv_blocks) * kAppendThreads + threadIdx.x, n_seqs, q_len);
+    append_queries<T, HP>(p, (blockIdx.x - p.kv_blocks) * kAppendThreads + threadIdx.x, n_seqs, q_len);
     return;
   }
 
@@ -213,25 +218,23 @@ __global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __gr
   const int o1 = turn && p.half ? 4 * l : 8 * l;
   const int o2 = turn && p.half ? (p.rot >> 1) + 4 * l : 8 * l + 4;
   const int slot0 = sub * SLOTS + lane / LPT;
+  // steps i with a new token: lo <= i < hi (slots past a small page are past every token)
+  const int first = start + slot0;
+  const int lo = max(0, (base - first + TPS - 1) / TPS);
+  const int end = min(ctx, start + page);
+  const int hi = live ? min(STEPS, max(0, (end - first + TPS - 1) / TPS)) : 0;
   float x[STEPS][8];
-  float amax = 0.f;
-  bool odd = false;
-  float s_old = 0.f;
-  float* scale = nullptr;
-  uint8_t* dst = nullptr;
-  if (live) {
-    const T* src = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.vh : p.kh);
+  const int64_t row0 = b * q_len + (first - base);
+  {
     const int64_t st = is_v ? p.vt : p.kt;
+    const T* r = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.vh : p.kh) + row0 * st;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      const int slot = slot0 + i * TPS;
-      const int tok = start + slot;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-      if (slot < page && tok >= base && tok < ctx) {
-        const T* r = src + static_cast<int64_t>(b * q_len + tok - base) * st;
-        load_row4<T>(r + o1, x[i]);
-        load_row4<T>(r + o2, x[i] + 4);
+      if (i >= lo && i < hi) {
+        load_row4<T>(r + i * TPS * st + o1, x[i]);
+        load_row4<T>(r + i * TPS * st + o2, x[i] + 4);
       }
     }
   }
@@ -239,48 +242,57 @@ __global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __gr
     if (threadIdx.x == 0 && part == 0) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
     return;
   }
+  float s_old = 0.f;
+  float* scale = nullptr;
+  uint8_t* dst = nullptr;
   if (live) {
     scale = (is_v ? p.vs : p.ks) + static_cast<int64_t>(pg) * p.s_sp + head * p.s_sh;
     dst = (is_v ? p.vc : p.kc) + static_cast<int64_t>(pg) * p.kv_sp + head * p.kv_sh;
     s_old = *scale;
-    if (turn) {
+  }
+  if (turn) {
+    auto each = [&](auto is_half) {
+      constexpr bool HALF = decltype(is_half)::value;
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int slot = slot0 + i * TPS;
-        const int tok = start + slot;
-        if (slot < page && tok >= base && tok < ctx) {
-          const int pos = p.pos != nullptr ? __ldg(p.pos + b * q_len + tok - base) : tok;
+      for (int i = 0; i < STEPS; ++i)
+        if (i >= lo && i < hi) {
+          const int pos = p.pos != nullptr ? __ldg(p.pos + row0 + i * TPS) : first + i * TPS;
           const float* row = rope_row(p.table, pos, p.n_pos, p.rot, p.status);
           float c[4], s[4];
           load_f32_run<4>(row + 4 * l, c);
           load_f32_run<4>(row + (p.rot >> 1) + 4 * l, s);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            // pairs: (e, e + 4) of the two runs, or neighbours
-            const float a = p.half ? x[i][e] : x[i][2 * e];
-            const float bb = p.half ? x[i][e + 4] : x[i][2 * e + 1];
-            const float y = fmaf(a, c[e], -bb * s[e]), z = fmaf(bb, c[e], a * s[e]);
-            c[e] = y;
-            s[e] = z;
-          }
-          if (p.half) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { x[i][e] = c[e]; x[i][e + 4] = s[e]; }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { x[i][2 * e] = c[e]; x[i][2 * e + 1] = s[e]; }
+            float& xa = x[i][HALF ? e : 2 * e];
+            float& xb = x[i][HALF ? e + 4 : 2 * e + 1];
+            const float a = xa, bb = xb;
+            xa = fmaf(a, c[e], -bb * s[e]);
+            xb = fmaf(bb, c[e], a * s[e]);
           }
         }
-      }
-    }
+    };
+    if (p.half) each(std::true_type{});
+    else each(std::false_type{});
+  }
+  // the maximum of the magnitudes as bits: a NaN or an infinity shows as 0x7f800000 or more
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[i][e]) & 0x7fffffffu);
+  float amax = __uint_as_float(top);
+  const bool odd = __any_sync(0xffffffffu, top >= 0x7f800000u);
+  if (odd) {                            // NaN becomes 0; infinities have no part in the maximum
+    amax = 0.f;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
+        if (!(x[i][e] == x[i][e])) x[i][e] = 0.f;
         const float a = fabsf(x[i][e]);
         if (a <= 3.402823466e38f) amax = fmaxf(amax, a);
-        else odd = true;
       }
+    if (lane == 0) report_status(p.status, SPECQ_STATUS_KV_NONFINITE);
   }
   amax = warp_max_f32(amax);
   if (wpu > 1) {
@@ -295,22 +307,30 @@ __global__ void __launch_bounds__(kAppendThreads) block_append_kernel(const __gr
   const bool fresh = start >= base;
   const float s_new = fresh ? need : fmaxf(s_old, need);
   const float rs = __frcp_rn(s_new);
-  if (odd) report_status(p.status, SPECQ_STATUS_KV_NONFINITE);
+  if (odd) {                            // an infinity is stored as the largest number
+    const float lim = s_new * (1.f / cache_inv_max<CT>());
 #pragma unroll
-  for (int i = 0; i < STEPS; ++i) {
-    const int slot = slot0 + i * TPS;
-    const int tok = start + slot;
-    if (slot < page && tok >= base && tok < ctx) {
-      float y[8];
+    for (int i = 0; i < STEPS; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        y[e] = x[i][e] * rs;
-        if (odd && !(y[e] == y[e])) y[e] = 0.f;
+      for (int e = 0; e < 8; ++e)
+        if (fabsf(x[i][e]) > 3.402823466e38f) x[i][e] = copysignf(lim, x[i][e]);
+  }
+  {
+    uint8_t* d = dst + static_cast<int64_t>(slot0) * p.kv_so;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+      if (i >= lo && i < hi) {
+        const float* y = x[i];
+        const uint32_t w0 = pack_cache4<CT>(y[0] * rs, y[1] * rs, y[2] * rs, y[3] * rs);
+        const uint32_t w1 = pack_cache4<CT>(y[4] * rs, y[5] * rs, y[6] * rs, y[7] * rs);
+        uint8_t* q = d + static_cast<int64_t>(i * TPS) * p.kv_so;
+        if (turn && p.half) {
+          *reinterpret_cast<uint32_t*>(q + o1) = w0;
+          *reinterpret_cast<uint32_t*>(q + o2) = w1;
+        } else {
+          *reinterpret_cast<uint2*>(q + o1) = make_uint2(w0, w1);
+        }
       }
-      uint8_t* d = dst + static_cast<int64_t>(slot) * p.kv_so;
-      *reinterpret_cast<uint32_t*>(d + o1) = pack_cache4<CT>(y[0], y[1], y[2], y[3]);
-      *reinterpret_cast<uint32_t*>(d + o2) = pack_cache4<CT>(y[4], y[5], y[6], y[7]);
-    }
   }
   if (!fresh && s_new > s_old) {        // the page's older tokens under the grown scale
     const float r = __fdiv_rn(s_old, s_new);
@@ -392,36 +412,31 @@ inline int run_block_append(const void* k, int64_t kt, int64_t kh, const void* v
     p.q_groups = ceil_div(H, many ? kRopeHeads : 1);
     const int64_t threads = tokens * p.q_groups * p.q_items;
     if (threads > 0x7FFFFF00ll) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: too many query rows");
-    // a few tokens' queries ride in the same launch; many go in one of their own, whose threads need
-    // half the registers (the prompt of 4 x 2047 tokens: 63 us in one launch)
-    const int block = many ? kRopeThreads : kAppendThreads;
-    q_blocks = (threads + block - 1) / block;
+    q_blocks = (threads + kAppendThreads - 1) / kAppendThreads;
   }
   if (kv_blocks + q_blocks > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_append: too many tokens");
   p.kv_blocks = static_cast<int>(kv_blocks);
-  const dim3 grid(static_cast<unsigned>(kv_blocks + (many ? 0 : q_blocks)));
+  const dim3 grid(static_cast<unsigned>(kv_blocks + q_blocks));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto launch = [&](auto t, auto d, auto c) -> cudaError_t {
+  auto launch = [&](auto t, auto d, auto c, auto hp) -> cudaError_t {
     using T = decltype(t);
-    constexpr int DD = decltype(d)::value, CT = decltype(c)::value;
+    constexpr int DD = decltype(d)::value, CT = decltype(c)::value, HP = decltype(hp)::value;
     if constexpr (DD == 128) {
-      if (slots == 8) return launch_plain(block_append_kernel<T, DD, CT, 8>, grid, dim3(kAppendThreads), st, p);
+      if (slots == 8) return launch_plain(block_append_kernel<T, DD, CT, 8, HP>, grid, dim3(kAppendThreads), st, p);
     }
-    return launch_plain(block_append_kernel<T, DD, CT, 16>, grid, dim3(kAppendThreads), st, p);
+    return launch_plain(block_append_kernel<T, DD, CT, 16, HP>, grid, dim3(kAppendThreads), st, p);
+  };
+  auto by_hp = [&](auto t, auto d, auto c) {
+    return many ? launch(t, d, c, std::integral_constant<int, kRopeHeads>{}) : launch(t, d, c, std::integral_constant<int, 1>{});
   };
   auto by_cache = [&](auto t, auto d) {
-    return cache_dtype == SPECQ_CACHE_INT8 ? launch(t, d, std::integral_constant<int, 0>{})
-                                           : launch(t, d, std::integral_constant<int, 1>{});
+    return cache_dtype == SPECQ_CACHE_INT8 ? by_hp(t, d, std::integral_constant<int, 0>{})
+                                           : by_hp(t, d, std::integral_constant<int, 1>{});
   };
   auto by_dim = [&](auto t) {
     return D == 64 ? by_cache(t, std::integral_constant<int, 64>{}) : by_cache(t, std::integral_constant<int, 128>{});
   };
   SPECQ_CUDA_TRY(dtype == 0 ? by_dim(__half{}) : by_dim(__nv_bfloat16{}));
-  if (many) {
-    const dim3 qg(static_cast<unsigned>(q_blocks));
-    SPECQ_CUDA_TRY(dtype == 0 ? launch_plain(block_append_queries_kernel<__half>, qg, dim3(kRopeThreads), st, p)
-                              : launch_plain(block_append_queries_kernel<__nv_bfloat16>, qg, dim3(kRopeThreads), st, p));
-  }
   return SPECQ_OK;
 }
 
@@ -526,7 +541,8 @@ __global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __
     const int j1 = min(n, ((col0 + dwin + 1) << p.page_log2) - base);   // this target page takes tokens j0 .. j1 - 1
     uint8_t* dst = cache + static_cast<int64_t>(__shfl_sync(0xffffffffu, pg, dwin)) * p.kv_sp;
     const float s_old = __shfl_sync(0xffffffffu, sc, dwin);
-    // the arriving tokens' need; those of the page itself fit its scale already
+    // the arriving tokens' need; a number is at most q_max, so those of pages whose scale is no larger
+    // (the page itself among them) fit already
     float need = 0.f;
     const int jf = once ? same : j0;             // the first batch's first token
     for (int jb = jf; jb < j1; jb += BATCH * TPS) {
@@ -535,10 +551,7 @@ __global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __
       for (int i = 0; i < BATCH; ++i) {
         const float ss = __shfl_sync(0xffffffffu, sc, swin[i]);
         const int j = jb + i * TPS + sub;
-        if (j >= j0 && j < j1 && swin[i] != dwin) {
-          const float a = fmaxf(fmaxf(absmax4<CT>(w[i].x), absmax4<CT>(w[i].y)), fmaxf(absmax4<CT>(w[i].z), absmax4<CT>(w[i].w)));
-          need = fmaxf(need, a * cache_inv_max<CT>() * ss);
-        }
+        if (j >= j0 && j < j1 && ss > s_old) need = fmaxf(need, absmax16<CT>(w[i]) * cache_inv_max<CT>() * ss);
       }
     }
     need = warp_max_f32(need);
