@@ -19,8 +19,8 @@
 // group's exponentials overlap the other's products.  Within a group
 //   S^T [tokens x rows] = K Q^T         each warp its own quarter of the tokens; Q^T stays in registers, K is
 //                                       converted 8 -> 16 bits in registers, once
-//   P^T = 2^(S^T - m)                   in the accumulator's registers, turned by movmatrix and
-//                                       left in shared memory as the fragments the next step reads
+//   P^T = 2^(S^T - m)                   in the accumulator's registers, turned by stmatrix on its
+//                                       way to shared memory, where every warp of the group reads it
 //   O^T [D x rows] += V^T P^T           each warp its own quarter of the D elements over all of
 //                                       the tokens; V by a transposing ldmatrix, converted once
 // so O costs 8 registers for 8 rows (D = 128), and a segment ends with a sum of two halves.  Two
@@ -111,10 +111,12 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ uint32_t movm_t(uint32_t a) {
-  uint32_t d;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
-  return d;
+__device__ __forceinline__ void stsm4_t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void stsm2_t(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -314,6 +316,10 @@ struct BAPlace {
   }
 };
 
+__device__ __forceinline__ void named_barrier_arrive(uint32_t id, uint32_t nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
+}
+
 // A group's barrier that also tells whether any of its threads says so.
 __device__ __forceinline__ bool ba_vote(int id, bool x) {
   uint32_t r;
@@ -336,14 +342,16 @@ struct BASmem {
   static constexpr int ROWS = NT * 8;
   static constexpr int KB = TOK * D;                       // bytes of a K (or V) tile
   static constexpr int STAGE = 2 * KB;
-  static constexpr int P = (TOK / 16) * NT * 32 * 8;       // a tile's P^T: [16 tokens][group][lane] b0, b1
+  static constexpr int PPITCH = 2 * TOK + 16;                  // rows of P shift by 4 banks
+  static constexpr int P = ROWS * PPITCH;  // a tile's P [row][token], fp16
   static constexpr int QPITCH = 2 * D + 16;
-  static constexpr int Q = ROWS * QPITCH;
+  static constexpr int TREE = ROWS * QPITCH;                   // behind the queries: the rows' tree words
+  static constexpr int Q = TREE + ROWS * 8;
   static constexpr int SC = TOK / 8;                           // scales of a stage: ck, lv, iv for each 8 tokens
   static constexpr int SCALES = SC * 16;
   static constexpr int PART = ba_part(D);                      // floats of a row's part
   static constexpr int MERGE = kBAGroupWarps * MT * NT * 32 * 16;   // one group's O
-  static constexpr int fixed = 2 * P + MERGE + 2 * Q + kBAMaxStages * SCALES + 2 * kBAWarps * ROWS * 4 + 256;
+  static constexpr int fixed = 2 * P + MERGE + 2 * Q + kBAMaxStages * SCALES + 2 * kBAWarps * ROWS * 4 + 512;
 };
 
 template <int D, int CT, int NT>
@@ -365,16 +373,22 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   float4* scales = reinterpret_cast<float4*>(qbuf + 2 * S::Q);
   float* sm_l = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scales) + kBAMaxStages * S::SCALES);   // [warp][row]
   float* sm_m = sm_l + kBAWarps * ROWS;                                                                   // [warp][row]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm_m + kBAWarps * ROWS);
-  uint64_t* empty = full + kBAMaxStages;
-  uint64_t* q_full = empty + kBAMaxStages;
+  // K and V tiles have rings of their own: a K stage is free once the scores are made, a whole turn
+  // before its V
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(sm_m + kBAWarps * ROWS);
+  uint64_t* k_empty = k_full + kBAMaxStages;
+  uint64_t* v_full = k_empty + kBAMaxStages;
+  uint64_t* v_empty = v_full + kBAMaxStages;
+  uint64_t* q_full = v_empty + kBAMaxStages;
   uint64_t* q_empty = q_full + 2;
 
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 2u);               // the boxes' expected bytes, and the scales
-      mbar_init(&empty[s], kBAGroupWarps);   // the group that reads it
+      mbar_init(&k_full[s], 2u);             // the boxes' expected bytes, and the scales
+      mbar_init(&v_full[s], 1u);
+      mbar_init(&k_empty[s], kBAGroupWarps); // the group that reads it
+      mbar_init(&v_empty[s], kBAGroupWarps);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&q_full[s], 32u * NF);
@@ -401,6 +415,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     const int nb = TOK >> (31 - __clz(p.box));          // boxes of a tile; a batch of 32 is `tpb` of the warp's tiles
     const int tpb = 32 / nb;                 // (all powers of two)
     const int lt = lane >> (31 - __clz(nb)), lb = lane & (nb - 1);
+    int segment = 0;
     int skip = f;                            // tiles of the segment before the warp's next one
     // pages that one block reads are read once; of several row chunks the first leaves them in L2
     const uint64_t hint = a.rc == 1 ? policy_evict_first() : policy_evict_last();
@@ -424,6 +439,13 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(d)), "l"(src), "r"(lr < rows ? 16 : 0)
                        : "memory");
         }
+        if (p.tree != nullptr && f == NF - 1) {
+          for (int lr = lane; lr < ROWS; lr += 32) {
+            const int qi = ba_token(p, sg.row_lo + min(lr, rows - 1));
+            const uint64_t* src = p.tree + sg.b * p.tree_sb + qi * p.tree_st;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(qbuf + qat.s * S::Q + S::TREE + lr * 8)), "l"(src) : "memory");
+          }
+        }
         cp_async_mbar_arrive(&q_full[qat.s]);
         if (lane == 0 && f == 0) SPECQ_TRACE_POINT(4, qat.s);
         qat.step(2);
@@ -436,6 +458,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
         pg = t < sg.tb && tok < sg.ctx ? __ldg(bt + (tok >> p.page_log2)) : -1;
       };
       load_pages();
+      if (segment++ > 0) copy_queries();     // the piece's first tile goes before its queries
       int stepped = sg.ta;                   // `at` is the stage of this tile
       for (; t0 < sg.tb;) {
         const int my_tile = t0 + lt * NF, my_tok = tok;
@@ -455,26 +478,26 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
         if (t0 < sg.tb) load_pages();
         for (int t = tb0; t < t1; t += NF) {
           for (; stepped < t; ++stepped) at.step(stages);
-          ok = ok && mbar_wait(&empty[at.s], at.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+          ok = ok && mbar_wait(&k_empty[at.s], at.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
           const bool mine = t == my_tile;
           const unsigned boxes = __ballot_sync(0xffffffffu, mine && load);
           if (ok) {
-            if (lane == 0) mbar_arrive_expect_tx(&full[at.s], 2u * __popc(boxes) * p.box * D);
+            if (lane == 0) mbar_arrive_expect_tx(&k_full[at.s], __popc(boxes) * p.box * D);
             __syncwarp();
             // one lane starts all boxes: their operands are the warp's, not a lane's
             const int first = (t - tb0) / NF * nb;
-            uint8_t* dk = ring + at.s * S::STAGE;
-            int slot = (t * TOK) & ((1 << p.page_log2) - 1);
+            const int slot0 = (t * TOK) & ((1 << p.page_log2) - 1);
             const int n_box = __popc(boxes);
-            for (int x = 0; x < n_box; ++x) {
-              const int pgx = __shfl_sync(0xffffffffu, page, first + x);
-              if (elect_one()) {
-                tma_box(dk, &mk, &full[at.s], sg.h, slot, pgx, hint);
-                tma_box(dk + S::KB, &mv, &full[at.s], sg.h, slot, pgx, hint);
+            auto start = [&](uint8_t* d, const CUtensorMap* map, uint64_t* bar) {
+              int slot = slot0;
+              for (int x = 0; x < n_box; ++x) {
+                const int pgx = __shfl_sync(0xffffffffu, page, first + x);
+                if (elect_one()) tma_box(d, map, bar, sg.h, slot, pgx, hint);
+                d += p.box * D;
+                slot = (slot + p.box) & ((1 << p.page_log2) - 1);
               }
-              dk += p.box * D;
-              slot = (slot + p.box) & ((1 << p.page_log2) - 1);
-            }
+            };
+            start(ring + at.s * S::KB, &mk, &k_full[at.s]);
             if (mine) {
               // a masked score, -inf, times ck stays -inf; what is not there weighs nothing
               float4 w = make_float4(1e-37f, -INFINITY, 0.f, 0.f);
@@ -488,10 +511,16 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
               for (int i = 0; i < p.box >> 3; ++i) d[i] = w;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&full[at.s]);
+            if (lane == 0) mbar_arrive(&k_full[at.s]);
             if (lane == 0) SPECQ_TRACE_POINT(5, t);
+            ok = ok && mbar_wait(&v_empty[at.s], at.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+            if (ok) {
+              if (lane == 0) mbar_arrive_expect_tx(&v_full[at.s], __popc(boxes) * p.box * D);
+              __syncwarp();
+              start(ring + (stages + at.s) * S::KB, &mv, &v_full[at.s]);
+            }
           }
-          if (!q_done) copy_queries();       // after the first tile is on its way
+          if (!q_done) copy_queries();
         }
       }
       if (!q_done) copy_queries();
@@ -500,8 +529,10 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     }
     if (!ok) {                               // a wait ran out: leave no copy of this block in flight
       for (int s = 0; s < stages; ++s) {
-        (void)mbar_wait(&full[s], 0u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-        (void)mbar_wait(&full[s], 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+        for (uint32_t ph = 0; ph < 2u; ++ph) {
+          (void)mbar_wait(&k_full[s], ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+          (void)mbar_wait(&v_full[s], ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+        }
       }
     }
     pdl_launch_dependents();
@@ -519,8 +550,11 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   // V: MT = 2, matrices (token half, piece); MT = 1, (token half, next 16 tokens)
   const int vr = MT == 2 ? mr : mr + mc * 16;
   const int vc = MT == 2 ? 2 * gw + mc : gw;
-  const uint32_t v_off = ring_s + S::KB + static_cast<uint32_t>(vr * D + ((vc ^ (D == 128 ? (vr & 7) : ((vr >> 1) & 3))) << 4));
-  uint8_t* my_p = pbuf + grp * S::P + lane * 8;
+  const uint32_t v_off = ring_s + static_cast<uint32_t>(stages * S::KB) + static_cast<uint32_t>(vr * D + ((vc ^ (D == 128 ? (vr & 7) : ((vr >> 1) & 3))) << 4));
+  // P: this lane's row of the matrices that it stores (group pair, token half) and loads (32 tokens of a group)
+  const uint32_t p_base = smem_u32(pbuf + grp * S::P);
+  const uint32_t p_put = p_base + static_cast<uint32_t>(((lane >> 4) * 8 + (lane & 7)) * S::PPITCH + (U * gw * 16 + ((lane >> 3) & 1) * 8) * 2);
+  const uint32_t p_get = p_base + static_cast<uint32_t>((lane & 7) * S::PPITCH + (lane >> 3) * 16);
 
   int tile_no = 0;                           // of the piece
   while (walk.next(p, a, sg)) {
@@ -538,9 +572,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
         qf[n][c][1] = w.y;
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&q_empty[qat.s]);
-    qat.step(2);
+    const uint64_t* tree_rows = reinterpret_cast<const uint64_t*>(qbuf + qat.s * S::Q + S::TREE);
     if (threadIdx.x == 0) SPECQ_TRACE_POINT(9, sg.ta);
     if (p.bf16) {
       // to fp16 under one power of two that brings the largest to [1, 2): bf16's 8 bits are exact
@@ -577,16 +609,9 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       for (int c = 0; c < MT; ++c) o[c][n][0] = o[c][n][1] = o[c][n][2] = o[c][n][3] = 0.f;
     }
 
-    int n_mine = 0;
-    for (int t = sg.ta; t < sg.tb; ++t, at.step(stages)) {
-      if ((tile_no++ & 1) != grp) continue;                     // the other group's
-      ++n_mine;
-      ok = ok && mbar_wait(&full[at.s], at.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-      const uint32_t stage = static_cast<uint32_t>(at.s * S::STAGE);
-      if (threadIdx.x == 0) SPECQ_TRACE_POINT(10, t);
-
+    float sc[U][NT][4];                      // a tile's scores
+    auto scores = [&](uint32_t stage) {
       // S^T = K Q^T for tokens 16 (U gw + u) + 0..15
-      float sc[U][NT][4];
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -606,67 +631,92 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
           for (int n = 0; n < NT; ++n) mma16816(sc[u][n], l0, l1, h0, h1, qf[n][c][0], qf[n][c][1]);
         }
       }
-      if (threadIdx.x == 0) SPECQ_TRACE_POINT(11, t);
-
+    };
+    // masks, raises the maxima where the vote says so, leaves P in shared memory (after the vote, which is
+    // also the barrier after which the group has read the P before)
+    BAPlace pl = at;
+    auto softmax = [&](int t) {              // of tile t, whose place is pl
       // softmax: rows 2 tq, 2 tq + 1 of each group, tokens gq and gq + 8 of each 16
       float ck[U], lv[U], lv1[U], iv[U], iv_rel[U];
-      float top = -INFINITY;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float4 w0 = scales[at.s * S::SC + 2 * (U * gw + u)];
+        const float4 w0 = scales[pl.s * S::SC + 2 * (U * gw + u)];
         ck[u] = w0.x * fac;
         lv[u] = lv1[u] = w0.y;
         iv[u] = w0.z;
         iv_rel[u] = 1.f;
-        if (p.page_log2 == 3) {              // tokens 8 .. 15 are another page's, with its own scales
-          const float4 w1 = scales[at.s * S::SC + 2 * (U * gw + u) + 1];
-          lv1[u] = w1.y;
-          iv_rel[u] = iv[u] > 0.f ? w1.z / iv[u] : 0.f;
-          const float rel = w1.x / w0.x;
+      }
+      const int tw = t * TOK + 16 * U * gw;  // the warp's first token
+      if (p.page_log2 == 3 || tw + 16 * U > sg.old) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            sc[u][n][2] *= rel;
-            sc[u][n][3] *= rel;
-          }
-        }
-        const int t0 = t * TOK + 16 * (U * gw + u);
-        if (t0 + 16 > sg.old) {              // some row may not see some token
+        for (int u = 0; u < U; ++u) {
+          if (p.page_log2 == 3) {            // tokens 8 .. 15 are another page's, with its own scales
+            const float ck0 = scales[pl.s * S::SC + 2 * (U * gw + u)].x;
+            const float4 w1 = scales[pl.s * S::SC + 2 * (U * gw + u) + 1];
+            lv1[u] = w1.y;
+            iv_rel[u] = iv[u] > 0.f ? w1.z / iv[u] : 0.f;
+            const float rel = w1.x / ck0;
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int qi = ba_token(p, sg.row_lo + n * 8 + 2 * tq + r);
-              if (p.tree == nullptr) {
-                const int lim = min(sg.ctx, sg.old + qi + 1);
-                if (t0 + gq >= lim) sc[u][n][r] = -INFINITY;
-                if (t0 + gq + 8 >= lim) sc[u][n][2 + r] = -INFINITY;
-              } else {
-                const uint64_t word = qi < a.q_len ? __ldg(reinterpret_cast<const unsigned long long*>(p.tree) + sg.b * p.tree_sb + qi * p.tree_st) : 0ull;
-                const int j0 = t0 + gq - sg.old, j1 = j0 + 8;
-                if (j0 >= a.q_len || (j0 >= 0 && ((word >> (j0 & 63)) & 1ull) == 0ull)) sc[u][n][r] = -INFINITY;
-                if (j1 >= a.q_len || (j1 >= 0 && ((word >> (j1 & 63)) & 1ull) == 0ull)) sc[u][n][2 + r] = -INFINITY;
-              }
+            for (int n = 0; n < NT; ++n) {
+              sc[u][n][2] *= rel;
+              sc[u][n][3] *= rel;
             }
-          if (CT == 1 && t0 + 16 > sg.ctx) {
-            // slots past the last token may hold anything, NaN bytes too: their V reads as 0
-            uint8_t* v = ring + stage + S::KB + 16 * (U * gw + u) * D;
-            for (int x = max(sg.ctx - t0, 0) * KC + lane; x < 16 * KC; x += 32)
-              *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0u, 0u, 0u, 0u);
-            fence_proxy_async_smem();        // before the stage is filled again
+          }
+          const int t0 = tw + 16 * u;
+          if (t0 + 16 > sg.old) {            // some row may not see some token
+            // bits 4n + 2r + half of what this thread's rows see of its two tokens
+            uint32_t sees = 0;
+            const int j0 = t0 + gq - sg.old, j1 = j0 + 8;       // draft numbers
+#pragma unroll 1
+            for (int x = 0; x < 2 * NT; ++x) {
+              const int lr = (x >> 1) * 8 + 2 * tq + (x & 1);
+              uint32_t s0, s1;
+              if (p.tree == nullptr) {
+                const int qi = min(ba_token(p, sg.row_lo + lr), a.q_len - 1);
+                s0 = j0 <= qi;
+                s1 = j1 <= qi;
+              } else {
+                const uint64_t word = tree_rows[lr];
+                s0 = j0 < 0 || (j0 < a.q_len && ((word >> (j0 & 63)) & 1ull) != 0ull);
+                s1 = j1 < 0 || (j1 < a.q_len && ((word >> (j1 & 63)) & 1ull) != 0ull);
+              }
+              sees |= (s0 | s1 << 1) << (2 * x);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                if (((sees >> (4 * n + 2 * r)) & 1u) == 0u) sc[u][n][r] = -INFINITY;
+                if (((sees >> (4 * n + 2 * r)) & 2u) == 0u) sc[u][n][2 + r] = -INFINITY;
+              }
+            if (CT == 1 && t0 + 16 > sg.ctx) {
+              // slots past the last token may hold anything, NaN bytes too: their V reads as 0
+              ok = ok && mbar_wait(&v_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+              uint8_t* v = ring + (stages + pl.s) * S::KB + 16 * (U * gw + u) * D;
+              for (int x = max(sg.ctx - t0, 0) * KC + lane; x < 16 * KC; x += 32)
+                *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0u, 0u, 0u, 0u);
+              fence_proxy_async_smem();      // before the stage is filled again
+            }
           }
         }
-        // x = score in log2 units + log2(sV), against the lagging m
+      }
+      // x = score in log2 units + log2(sV), against the lagging m; one chain of maxima a group of rows
+      float tops[NT];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        tops[n] = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             sc[u][n][r] = fmaf(sc[u][n][r], ck[u], lv[u]);
             sc[u][n][2 + r] = fmaf(sc[u][n][2 + r], ck[u], lv1[u]);
-            top = fmaxf(top, fmaxf(sc[u][n][r], sc[u][n][2 + r]) - m[n][r]);
+            tops[n] = fmaxf(tops[n], fmaxf(sc[u][n][r], sc[u][n][2 + r]) - m[n][r]);
           }
       }
-      if (threadIdx.x == 0) SPECQ_TRACE_POINT(12, t);
-      // the vote is also the barrier after which the group's P buffer may be written again
+      float top = tops[0];
+#pragma unroll
+      for (int n = 1; n < NT; ++n) top = fmaxf(top, tops[n]);
       if (ba_vote(1 + grp, top > kBARaise)) {                   // raise the maxima and what they scale
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -698,7 +748,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
           }
       }
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        uint32_t h[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float y[4];
@@ -709,41 +760,110 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
             l[n][r] = fmaf(fmaf(y[2 + r], iv_rel[u], y[r]), iv[u], l[n][r]);
           }
           const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
-          *reinterpret_cast<uint2*>(my_p + ((U * gw + u) * NT + n) * 256) =
-              make_uint2(movm_t(*reinterpret_cast<const uint32_t*>(&h0)), movm_t(*reinterpret_cast<const uint32_t*>(&h1)));
+          h[n][0] = *reinterpret_cast<const uint32_t*>(&h0);
+          h[n][1] = *reinterpret_cast<const uint32_t*>(&h1);
         }
-      named_barrier_sync(1 + grp, 32 * kBAGroupWarps);
-      if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, t);
-
-      // O^T += V^T P^T
-      constexpr int KSTEP = MT == 2 ? 1 : 2, NK = TOK / 16 / KSTEP, AHEAD = NK < 2 ? NK : 2;
-      uint32_t vr4[AHEAD][4];
+        // (token, row) fragments turned on the way to P [row][token]
+        const uint32_t d = p_put + static_cast<uint32_t>(u * 32);
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) ldsm4_t(v_off + stage + static_cast<uint32_t>(k * KSTEP * 16 * D), vr4[k]);
-#pragma unroll 1
-      for (int kb = 0; kb < NK; kb += AHEAD)
-#pragma unroll
-      for (int ka = 0; ka < AHEAD; ++ka) {
-        const int k = kb + ka;
-        uint32_t r[4] = {vr4[ka][0], vr4[ka][1], vr4[ka][2], vr4[ka][3]};
-        if (k + AHEAD < NK) ldsm4_t(v_off + stage + static_cast<uint32_t>((k + AHEAD) * KSTEP * 16 * D), vr4[ka]);
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          uint32_t e0, d0, e1, d1;
-          widen4<CT, true>(r[2 * hf], e0, d0);
-          widen4<CT, true>(r[2 * hf + 1], e1, d1);
-          const int kk = MT == 2 ? k : 2 * k + hf;
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint2 b = *reinterpret_cast<const uint2*>(my_p + (kk * NT + n) * 256);
-            mma16816(o[MT == 2 ? hf : 0][n], e0, d0, e1, d1, b.x, b.y);
-          }
-        }
+        for (int n = 0; n + 1 < NT; n += 2) stsm4_t(d + static_cast<uint32_t>(n * 8 * S::PPITCH), h[n][0], h[n][1], h[n + 1][0], h[n + 1][1]);
+        if constexpr (NT % 2 == 1) stsm2_t(d + static_cast<uint32_t>((NT - 1) * 8 * S::PPITCH), h[NT - 1][0], h[NT - 1][1]);
       }
-      __syncwarp();                                             // every lane has read the stage
-      if (lane == 0) mbar_arrive(&empty[at.s]);
-      if (threadIdx.x == 0) SPECQ_TRACE_POINT(14, t);
+    };
+    auto products = [&](uint32_t stage) {
+      // O^T += V^T P^T
+      // 32 tokens at a time; V of the next 32 is on its way
+      constexpr int NK = TOK / 32;
+      uint32_t vn[MT][4];
+#pragma unroll
+      for (int c = 0; c < MT; ++c) ldsm4_t(v_off + stage + static_cast<uint32_t>(c * 16 * D), vn[c]);
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        uint32_t pf[NT][4], r[MT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) ldsm4(p_get + static_cast<uint32_t>(n * 8 * S::PPITCH + k * 64), pf[n]);
+#pragma unroll
+        for (int c = 0; c < MT; ++c) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[c][i] = vn[c][i];
+          if (k + 1 < NK) ldsm4_t(v_off + stage + static_cast<uint32_t>(((k + 1) * 2 + c) * 16 * D), vn[c]);
+        }
+        // MT = 2: r[s] is 16-token step s, two pieces of D; MT = 1: both steps of the one piece
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int c = 0; c < MT; ++c) {
+            uint32_t e0, d0, e1, d1;
+            widen4<CT, true>(r[MT == 2 ? s : 0][2 * (MT == 2 ? c : s)], e0, d0);
+            widen4<CT, true>(r[MT == 2 ? s : 0][2 * (MT == 2 ? c : s) + 1], e1, d1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16816(o[c][n], e0, d0, e1, d1, pf[n][2 * s], pf[n][2 * s + 1]);
+          }
+      }
+    };
+    auto release = [&](uint64_t* bar) {
+      __syncwarp();                          // every lane has read the stage
+      if (lane == 0) mbar_arrive(bar);
+    };
+
+    // the group's tiles are every other one of the piece
+    const int n_all = sg.tb - sg.ta, first_mine = ((tile_no & 1) != grp) ? 1 : 0;
+    const int n_mine = (n_all - first_mine + 1) >> 1;
+    tile_no += n_all;
+    if (first_mine) pl.step(stages);
+    auto next = [&]() {
+      pl.step(stages);
+      pl.step(stages);
+    };
+    if constexpr (ba_split(NT)) {
+      // A tile's scores follow the products of the tile before, so that the tensor pipe has one long
+      // stretch and then the exponentials'; the second group starts its first stretch when the first
+      // group has ended its own, and from then on each runs its exponentials under the other's products.
+      BAPlace before = pl;                   // of the tile before
+      if (grp == 1) named_barrier_sync(4, kBACompute);
+      for (int x = 0; x <= n_mine; ++x) {
+        if (threadIdx.x == 0) SPECQ_TRACE_POINT(10, x);
+        if (x > 0) {
+          ok = ok && mbar_wait(&v_full[before.s], before.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+          named_barrier_sync(1 + grp, 32 * kBAGroupWarps);      // the group's P is written
+          products(static_cast<uint32_t>(before.s * S::KB));
+          release(&v_empty[before.s]);
+        }
+        if (threadIdx.x == 0) SPECQ_TRACE_POINT(11, x);
+        if (x < n_mine) {
+          ok = ok && mbar_wait(&k_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+          scores(static_cast<uint32_t>(pl.s * S::KB));
+        }
+        if (threadIdx.x == 0) SPECQ_TRACE_POINT(12, x);
+        if (grp == 0 && x == 0) named_barrier_arrive(4, kBACompute);
+        if (x < n_mine) {
+          softmax(sg.ta + first_mine + 2 * x);
+          release(&k_empty[pl.s]);           // its scales are read too
+          before = pl;
+          next();
+        }
+        if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, x);
+      }
+    } else {
+      for (int x = 0; x < n_mine; ++x) {
+        ok = ok && mbar_wait(&k_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+        if (threadIdx.x == 0) SPECQ_TRACE_POINT(10, x);
+        scores(static_cast<uint32_t>(pl.s * S::KB));
+        softmax(sg.ta + first_mine + 2 * x);
+        release(&k_empty[pl.s]);
+        named_barrier_sync(1 + grp, 32 * kBAGroupWarps);
+        if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, x);
+        ok = ok && mbar_wait(&v_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+        products(static_cast<uint32_t>(pl.s * S::KB));
+        release(&v_empty[pl.s]);
+        next();
+      }
     }
+    for (int x = 0; x < n_all; ++x) at.step(stages);
+
+    __syncwarp();                            // the queries' buffer (and its tree words) may be filled again
+    if (lane == 0) mbar_arrive(&q_empty[qat.s]);
+    qat.step(2);
 
     // ---- the group's part of the segment
     const int live = min(a.chunk_rows, a.q_rows - sg.row_lo);
