@@ -316,10 +316,6 @@ struct BAPlace {
   }
 };
 
-__device__ __forceinline__ void named_barrier_arrive(uint32_t id, uint32_t nthreads) {
-  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
-}
-
 // A group's barrier that also tells whether any of its threads says so.
 __device__ __forceinline__ bool ba_vote(int id, bool x) {
   uint32_t r;
@@ -373,8 +369,9 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   float4* scales = reinterpret_cast<float4*>(qbuf + 2 * S::Q);
   float* sm_l = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(scales) + kBAMaxStages * S::SCALES);   // [warp][row]
   float* sm_m = sm_l + kBAWarps * ROWS;                                                                   // [warp][row]
-  // K and V tiles have rings of their own: a K stage is free once the scores are made, a whole turn
-  // before its V
+  // A block that has the SM to itself has few stages, and frees a tile's K when its scores are made;
+  // where two share it, a tile is one stage with one barrier (59 -> 56 us for B=32 q=1 ctx 4096)
+  constexpr bool TWO = ba_split(NT);
   uint64_t* k_full = reinterpret_cast<uint64_t*>(sm_m + kBAWarps * ROWS);
   uint64_t* k_empty = k_full + kBAMaxStages;
   uint64_t* v_full = k_empty + kBAMaxStages;
@@ -400,6 +397,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   }
   __syncthreads();
   pdl_wait();
+  pdl_launch_dependents();                   // the joining blocks set themselves up as these leave the SMs
   if (threadIdx.x == 0) SPECQ_TRACE_POINT(1, 0);
   const BALine a = ba_line(p, blockIdx.x == 0 && warp == 0);
   BAWalk walk;
@@ -482,7 +480,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
           const bool mine = t == my_tile;
           const unsigned boxes = __ballot_sync(0xffffffffu, mine && load);
           if (ok) {
-            if (lane == 0) mbar_arrive_expect_tx(&k_full[at.s], __popc(boxes) * p.box * D);
+            if (lane == 0) mbar_arrive_expect_tx(&k_full[at.s], (TWO ? 1u : 2u) * __popc(boxes) * p.box * D);
             __syncwarp();
             // one lane starts all boxes: their operands are the warp's, not a lane's
             const int first = (t - tb0) / NF * nb;
@@ -498,6 +496,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
               }
             };
             start(ring + at.s * S::KB, &mk, &k_full[at.s]);
+            if constexpr (!TWO) start(ring + (stages + at.s) * S::KB, &mv, &k_full[at.s]);
             if (mine) {
               // a masked score, -inf, times ck stays -inf; what is not there weighs nothing
               float4 w = make_float4(1e-37f, -INFINITY, 0.f, 0.f);
@@ -513,8 +512,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_full[at.s]);
             if (lane == 0) SPECQ_TRACE_POINT(5, t);
-            ok = ok && mbar_wait(&v_empty[at.s], at.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-            if (ok) {
+            if constexpr (TWO) ok = ok && mbar_wait(&v_empty[at.s], at.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+            if (TWO && ok) {
               if (lane == 0) mbar_arrive_expect_tx(&v_full[at.s], __popc(boxes) * p.box * D);
               __syncwarp();
               start(ring + (stages + at.s) * S::KB, &mv, &v_full[at.s]);
@@ -531,11 +530,10 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       for (int s = 0; s < stages; ++s) {
         for (uint32_t ph = 0; ph < 2u; ++ph) {
           (void)mbar_wait(&k_full[s], ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-          (void)mbar_wait(&v_full[s], ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+          if (TWO) (void)mbar_wait(&v_full[s], ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
         }
       }
     }
-    pdl_launch_dependents();
     return;
   }
 
@@ -691,7 +689,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
               }
             if (CT == 1 && t0 + 16 > sg.ctx) {
               // slots past the last token may hold anything, NaN bytes too: their V reads as 0
-              ok = ok && mbar_wait(&v_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+              if constexpr (TWO) ok = ok && mbar_wait(&v_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
               uint8_t* v = ring + (stages + pl.s) * S::KB + 16 * (U * gw + u) * D;
               for (int x = max(sg.ctx - t0, 0) * KC + lane; x < 16 * KC; x += 32)
                 *reinterpret_cast<uint4*>(v + x * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -811,53 +809,21 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     const int n_mine = (n_all - first_mine + 1) >> 1;
     tile_no += n_all;
     if (first_mine) pl.step(stages);
-    auto next = [&]() {
+    for (int x = 0; x < n_mine; ++x) {
+      ok = ok && mbar_wait(&k_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(10, x);
+      scores(static_cast<uint32_t>(pl.s * S::KB));
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(11, x);
+      softmax(sg.ta + first_mine + 2 * x);
+      if constexpr (TWO) release(&k_empty[pl.s]);               // its scales are read too
+      named_barrier_sync(1 + grp, 32 * kBAGroupWarps);          // the group's P is written
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, x);
+      if constexpr (TWO) ok = ok && mbar_wait(&v_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+      products(static_cast<uint32_t>(pl.s * S::KB));
+      release(TWO ? &v_empty[pl.s] : &k_empty[pl.s]);
+      if (threadIdx.x == 0) SPECQ_TRACE_POINT(14, x);
       pl.step(stages);
       pl.step(stages);
-    };
-    if constexpr (ba_split(NT)) {
-      // A tile's scores follow the products of the tile before, so that the tensor pipe has one long
-      // stretch and then the exponentials'; the second group starts its first stretch when the first
-      // group has ended its own, and from then on each runs its exponentials under the other's products.
-      BAPlace before = pl;                   // of the tile before
-      if (grp == 1) named_barrier_sync(4, kBACompute);
-      for (int x = 0; x <= n_mine; ++x) {
-        if (threadIdx.x == 0) SPECQ_TRACE_POINT(10, x);
-        if (x > 0) {
-          ok = ok && mbar_wait(&v_full[before.s], before.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-          named_barrier_sync(1 + grp, 32 * kBAGroupWarps);      // the group's P is written
-          products(static_cast<uint32_t>(before.s * S::KB));
-          release(&v_empty[before.s]);
-        }
-        if (threadIdx.x == 0) SPECQ_TRACE_POINT(11, x);
-        if (x < n_mine) {
-          ok = ok && mbar_wait(&k_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-          scores(static_cast<uint32_t>(pl.s * S::KB));
-        }
-        if (threadIdx.x == 0) SPECQ_TRACE_POINT(12, x);
-        if (grp == 0 && x == 0) named_barrier_arrive(4, kBACompute);
-        if (x < n_mine) {
-          softmax(sg.ta + first_mine + 2 * x);
-          release(&k_empty[pl.s]);           // its scales are read too
-          before = pl;
-          next();
-        }
-        if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, x);
-      }
-    } else {
-      for (int x = 0; x < n_mine; ++x) {
-        ok = ok && mbar_wait(&k_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-        if (threadIdx.x == 0) SPECQ_TRACE_POINT(10, x);
-        scores(static_cast<uint32_t>(pl.s * S::KB));
-        softmax(sg.ta + first_mine + 2 * x);
-        release(&k_empty[pl.s]);
-        named_barrier_sync(1 + grp, 32 * kBAGroupWarps);
-        if (threadIdx.x == 0) SPECQ_TRACE_POINT(13, x);
-        ok = ok && mbar_wait(&v_full[pl.s], pl.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-        products(static_cast<uint32_t>(pl.s * S::KB));
-        release(&v_empty[pl.s]);
-        next();
-      }
     }
     for (int x = 0; x < n_all; ++x) at.step(stages);
 
@@ -947,33 +913,37 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     }
     if (threadIdx.x == 0) SPECQ_TRACE_POINT(16, sg.ta);
   }
-  pdl_launch_dependents();
 }
 
 // Join the parts of cut segments: block (segment, group of 8 rows), one warp a row.
 template <int D>
 __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_constant__ BlockAttnParams p) {
   pdl_launch_dependents();
-  pdl_wait();
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  // The lengths and the plan were there before the attention kernel started (these blocks start when
+  // all of its have passed their own wait), so the block finds its rows while that still runs.
   const BALine a = ba_line(p, false);
-  if (a.rc == 0) return;
-  const int per = p.h_kv * a.rc;
+  const int per = max(1, p.h_kv * a.rc);
   const int b = ba_div(static_cast<int>(blockIdx.x), per), hr = static_cast<int>(blockIdx.x) - b * per;
-  if (b >= a.n_seqs) return;
-  const int h = ba_div(hr, a.rc), row_lo = (hr - h * a.rc) * a.chunk_rows;
+  const int h = a.rc > 1 ? ba_div(hr, a.rc) : hr, row_lo = (hr - h * a.rc) * a.chunk_rows;
   const int lr = blockIdx.y * 8 + warp;
-  if (lr >= min(a.chunk_rows, a.q_rows - row_lo)) return;
-  // where the segment lies on the line
-  int before = 0;
-  for (int b0 = 0; b0 < b; b0 += 32) {
-    const int x = b0 + lane;
-    before += __reduce_add_sync(0xffffffffu, x < b ? ba_tiles(p, ba_ctx(p, x)) : 0);
+  bool work = a.rc > 0 && b < a.n_seqs && lr < min(a.chunk_rows, a.q_rows - row_lo);
+  int s0 = 0, nt = 0, c0 = 0, c1 = 0;
+  if (work) {
+    // where the segment lies on the line
+    int before = 0;
+    for (int b0 = 0; b0 < b; b0 += 32) {
+      const int x = b0 + lane;
+      before += __reduce_add_sync(0xffffffffu, x < b ? ba_tiles(p, ba_ctx(p, x)) : 0);
+    }
+    nt = ba_tiles(p, ba_ctx(p, b));
+    s0 = before * per + hr * nt;
+    c0 = a.piece_of(s0);
+    c1 = a.piece_of(s0 + nt - 1);
+    work = c0 != c1;                                            // else inside one piece: written already
   }
-  const int nt = ba_tiles(p, ba_ctx(p, b));
-  const int s0 = before * per + hr * nt;
-  const int c0 = a.piece_of(s0), c1 = a.piece_of(s0 + nt - 1);
-  if (c0 == c1) return;                                         // inside one piece: written already
+  pdl_wait();                                                   // every block, or the next kernel could pass this one
+  if (!work) return;
   // piece c0 holds the segment's beginning (its second slot), the others begin inside it; tile n of a
   // piece is group n % 2's, so a group has a part unless the segment has one tile there, the other's
   constexpr int V = D / 32, PART = ba_part(D);
