@@ -14,15 +14,15 @@
 // products accumulate in fp32.  m lags: p may reach 2^8 before the running maximum is raised
 // (one warp vote a tile), which fp16 holds without loss.
 //
-// Tile.  A tile is 128 tokens (64 up to 16 rows) and up to 40 query rows, worked on by a group of four warps; a
-// block has two groups, which take tiles in turn, each with its own running maxima, so that one
-// group's exponentials overlap the other's products.  Within a group
-//   S^T [tokens x rows] = K Q^T         each warp its own quarter of the tokens; Q^T stays in registers, K is
-//                                       converted 8 -> 16 bits in registers, once
-//   P^T = 2^(S^T - m)                   in the accumulator's registers, turned by stmatrix on its
-//                                       way to shared memory, where every warp of the group reads it
-//   O^T [D x rows] += V^T P^T           each warp its own quarter of the D elements over all of
-//                                       the tokens; V by a transposing ldmatrix, converted once
+// Tile.  A tile is 128 tokens (64 up to 16 rows) of one KV head against up to 40 query rows, the work of
+// a group of four warps.  A block has two groups, which take tiles in turn, each with its own
+// running maxima.  Within a group
+//   S^T [tokens x rows] = K Q^T   each warp its own quarter of the tokens; Q^T stays in registers, K
+//                                 is converted 8 -> 16 bits in registers, once
+//   P^T = 2^(S^T - m)             in the accumulator's registers, turned by stmatrix on its way to
+//                                 shared memory, where every warp of the group reads it
+//   O^T [D x rows] += V^T P^T     each warp its own quarter of D over all of the tokens; V by a
+//                                 transposing ldmatrix, converted once
 // so O costs 8 registers for 8 rows (D = 128), and a segment ends with a sum of two halves.  Two
 // barriers of the group a tile: one carries the vote that raises the running maxima, one joins
 // the products.  Rows are the N side of both products and pad to 8.  Feeding warps walk the same
@@ -32,15 +32,23 @@
 //
 // Why mma.sync: a 16-token tile of 8n rows is 16 n instructions, and the warp-level tensor pipe
 // takes one every 2 cycles an SM (measured; 1024 multiply-adds a cycle): 2 n cycles a token,
-// against the 11.6 in which HBM delivers its 256 bytes.  Up to n = 5 the products fit under the
-// memory time, and rows cost what they are: the tcgen05 tile would be 128 tokens x 16n padded rows
-// at 64-76 cycles an instruction, with round trips through tensor memory between the steps.
-// More than 40 rows go to several blocks, which find the pages in L2.
+// against the 11.6 in which HBM delivers its 256 bytes, so up to n = 5 the products fit under the
+// memory time.  A tcgen05 tile would be 128 tokens x 16n padded rows at 64-76 cycles an
+// instruction, with round trips through tensor memory between the steps.  More than 40 rows go to
+// several blocks, which find the pages in L2; there the products are the bound.
+//
+// Measured (D = 128, 8 KV heads, group 4, page 64): B = 32, q = 1, context 4096: 57.4 us, 4.7 TB/s (heads
+// before slots in a page: 50.2 us, 5.3 TB/s, of the 6.44 that a copy reaches), bound by HBM.  B = 8,
+// q = 9, context 4096: 42 us, of which some 20 are set-up and the join (a launch runs its set-up once,
+// from cold instruction caches), and 2,500 cycles a tile where the products alone would take 1,525: two
+// warps a quarter of the SM are all that the registers hold (Q and O of 40 rows), too few to cover
+// their own latencies.
 //
 // Work.  The tiles of all (sequence, KV head, row chunk) segments form one line, cut into equal
 // pieces, one for each resident block, whatever the sequences' lengths; each block finds its
-// piece from ctx_len on the device.  A segment inside one piece is written at once; the parts of
-// a cut one, two groups' for each piece, go to the workspace and a second, dependent launch joins them in the pieces' order.
+// piece from ctx_len on the device.  A segment inside one piece is written at once; the parts of a
+// cut one, two groups' for each piece, go to the workspace, and a second, dependent launch joins
+// them in the pieces' order.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -57,10 +65,10 @@ constexpr int kBAGroupWarps = 4;                  // of a group
 constexpr int kBAWarps = 2 * kBAGroupWarps;       // that compute
 constexpr int kBACompute = 32 * kBAWarps;
 // And those that feed them.  A TMA box holds its warp for some 180 cycles whatever its size
-// (measured: 2 KB boxes from one warp an SM come at 2.8 TB/s, from two at 4.7, from four at 5.1), so an SM
-// has four of them, two a block where two blocks share it.  The registers of an SM's quarter divide among whole warps: from 3 row
-// groups on the block launches 12 warps of 168 and splits their 64,512 as 224 for the computing
-// ones (8 x 32 x 224) and 56 for the feeding ones (4 x 32 x 56).
+// (measured: 2 KB boxes from one warp an SM come at 2.8 TB/s, from two at 4.7, from four at 5.1), so
+// an SM has four of them, two a block where two blocks share it.  The registers of an SM's quarter
+// divide among whole warps: from 3 row groups on the block launches 12 warps of 168 and splits
+// their 64,512 as 224 for the computing ones (8 x 32 x 224) and 56 for the feeding ones (4 x 32 x 56).
 __host__ __device__ constexpr bool ba_split(int nt) { return nt >= 3; }
 __host__ __device__ constexpr int ba_feeders(int nt) { return ba_split(nt) ? 4 : 2; }
 __host__ __device__ constexpr int ba_threads(int nt) { return kBACompute + 32 * ba_feeders(nt); }
@@ -573,18 +581,22 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     const uint64_t* tree_rows = reinterpret_cast<const uint64_t*>(qbuf + qat.s * S::Q + S::TREE);
     if (threadIdx.x == 0) SPECQ_TRACE_POINT(9, sg.ta);
     if (p.bf16) {
-      // to fp16 under one power of two that brings the largest to [1, 2): bf16's 8 bits are exact
-      // down to 2^-17 of it, and what is smaller is off by 2^-25 of it at most
-      float top = 0.f;
+      // to fp16 under one power of two that brings the largest finite one to [1, 2): bf16's 8 bits are
+      // exact down to 2^-17 of it, and what is smaller is off by 2^-25 of it at most
+      uint32_t top = 0;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            top = fmaxf(top, fmaxf(fabsf(__uint_as_float(qf[n][c][i] << 16)), fabsf(__uint_as_float(qf[n][c][i] & 0xffff0000u))));
-      top = warp_max_f32(top);
-      const uint32_t ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t mag = (half ? qf[n][c][i] >> 16 : qf[n][c][i]) & 0x7fffu;
+              top = max(top, mag >= 0x7f80u ? 0u : mag);
+            }
+      top = __reduce_max_sync(0xffffffffu, top);
+      const uint32_t ex = min(max(top >> 7, 1u), 253u);
       fac = __uint_as_float(ex << 23);
       const float inv = __uint_as_float((254u - ex) << 23);
 #pragma unroll
@@ -911,7 +923,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       }
       named_barrier_sync(3, kBACompute);                        // sm_l, sm_m and the merge buffer may be written again
     }
-    if (threadIdx.x == 0) SPECQ_TRACE_POINT(16, sg.ta);
+    if (threadIdx.x == 0) SPECQ_TRACE_POINT(15, sg.ta);
   }
 }
 

@@ -11,6 +11,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -146,8 +147,13 @@ void same_device(const char* who, std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) {
     if (t == nullptr) continue;
     if (!t->is_cuda()) BAD_VALUE("specq kernels take CUDA tensors (there is no CPU path)");
-    if (first == nullptr) first = t;
-    else if (t->get_device() != first->get_device()) BAD_VALUE("%s: tensors on different devices", who);
+    if (first == nullptr) {
+      first = t;
+      const int now = static_cast<int>(c10::cuda::current_device());   // whose stream the call uses
+      if (t->get_device() != now) BAD_VALUE("%s: tensors on cuda:%d, the current device is cuda:%d", who, t->get_device(), now);
+    } else if (t->get_device() != first->get_device()) {
+      BAD_VALUE("%s: tensors on different devices", who);
+    }
   }
 }
 

@@ -305,6 +305,20 @@ def test_attention_extreme_values(cuda):
     assert torch.equal(got, specq.paged_attention_blocks(q, kc, vc, ks, vs, tbl, cl))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_attention_rows_do_not_touch_each_other(cuda, dtype, bad):
+    """A query row that holds an infinity or a NaN changes no other row by a bit."""
+    import specq
+    q, kc, vc, ks, vs, tbl, cl = _attend_inputs(11, 2, 5, 2, 4, 64, 16, "e4m3", dtype, [400, 33])
+    ref = specq.paged_attention_blocks(q, kc, vc, ks, vs, tbl, cl)
+    q[0, 2, 1, 7] = bad
+    got = specq.paged_attention_blocks(q, kc, vc, ks, vs, tbl, cl)
+    keep = torch.ones(2, 5, 8, dtype=torch.bool)
+    keep[0, 2, 1] = False
+    assert torch.equal(got[keep.cuda()], ref[keep.cuda()])
+
+
 def test_attention_strides_heads_first_and_packed(cuda):
     """A cache laid out [P, H_KV, page, D], scales and queries with other strides, packed rows, out=."""
     import specq
