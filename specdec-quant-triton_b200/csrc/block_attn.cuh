@@ -75,6 +75,8 @@ __host__ __device__ constexpr int ba_threads(int nt) { return kBACompute + 32 * 
 // Tokens of a tile: up to 16 rows two blocks share an SM, and half as many tokens leave each a ring
 // of six stages.
 __host__ __device__ constexpr int ba_tile(int nt) { return ba_split(nt) ? 128 : 64; }
+// Places of the line that a segment takes before its tiles.
+constexpr int kBASwitch = 2;
 constexpr int kBAMaxGroups = 5;                   // groups of 8 query rows a block holds at most
 constexpr int kBAMaxStages = 8;
 constexpr float kBARaise = 8.f;         // log2 of how far p may pass 1 before the maximum is raised
@@ -97,7 +99,7 @@ struct BlockAttnParams {
   float scale_log2;         // sm_scale * log2(e)
   int n_seqs, q_len, b_max, ql_max, h_kv, group, page_log2, n_pages, bt_cols;
   int bf16, stages, grid, rows, box;    // rows: of a block's chunk; box: slots of a TMA box
-  int tile;                             // tokens of a tile
+  int tile, tile_log2;                  // tokens of a tile
   int rc, chunk_rows;                   // row chunks of a (sequence, KV head) and their rows, without a plan
   uint32_t group_magic;                 // ceil(2^32 / group), for group > 1
 };
@@ -178,12 +180,13 @@ __device__ __forceinline__ int ba_div(int a, int b) {
   return q;
 }
 
-// Where the segments of a call lie on the line of tiles.  Piece c of the line (one a block) is
-// [start(c), start(c + 1)): the first `more` pieces have one tile more than the others.
+// Where the segments of a call lie on the line.  A segment takes kBASwitch places, in which nothing
+// is done, and then one for each of its tiles: beginning a segment costs a block about as much.
+// Piece c of the line (one a block) is [start(c), start(c + 1)): the first `more` pieces have one
+// place more than the others.
 struct BALine {
   int n_seqs, q_len, q_rows, rc;   // rc: row chunks of a (sequence, KV head)
   int chunk_rows;                  // rows of a chunk (a multiple of 8)
-  int total;                       // tiles in all
   int each, more;
   __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
   __device__ __forceinline__ int piece_of(int u) const {
@@ -196,7 +199,8 @@ __device__ __forceinline__ int ba_ctx(const BlockAttnParams& p, int b) {
   const int c = __ldg(p.ctx + b);
   return min(max(c, 0), p.bt_cols << p.page_log2);
 }
-__device__ __forceinline__ int ba_tiles(const BlockAttnParams& p, int ctx) { return max(1, (ctx + p.tile - 1) / p.tile); }
+__device__ __forceinline__ int ba_tiles(const BlockAttnParams& p, int ctx) { return max(1, (ctx + p.tile - 1) >> p.tile_log2); }
+__device__ __forceinline__ int ba_places(const BlockAttnParams& p, int ctx) { return kBASwitch + ba_tiles(p, ctx); }
 
 __device__ __forceinline__ BALine ba_line(const BlockAttnParams& p, bool tell) {
   BALine a;
@@ -216,7 +220,7 @@ __device__ __forceinline__ BALine ba_line(const BlockAttnParams& p, bool tell) {
     if (b < a.n_seqs) {
       const int c = __ldg(p.ctx + b);
       if (tell && (c < 0 || c > (p.bt_cols << p.page_log2))) report_status(p.status, SPECQ_STATUS_PLAN_CLAMPED);
-      n = ba_tiles(p, ba_ctx(p, b));
+      n = ba_places(p, ba_ctx(p, b));
     }
     t += __reduce_add_sync(0xffffffffu, n);
   }
@@ -228,9 +232,9 @@ __device__ __forceinline__ BALine ba_line(const BlockAttnParams& p, bool tell) {
     a.rc = ba_div(groups * 8 + p.rows - 1, p.rows);
     a.chunk_rows = a.rc > 0 ? ba_div(groups + a.rc - 1, a.rc) * 8 : 0;
   }
-  a.total = t * (p.h_kv * a.rc);
-  a.each = ba_div(a.total, p.grid);
-  a.more = a.total - a.each * p.grid;
+  const int total = t * (p.h_kv * a.rc);
+  a.each = ba_div(total, p.grid);
+  a.more = total - a.each * p.grid;
   return a;
 }
 
@@ -241,7 +245,7 @@ __device__ __forceinline__ int ba_find(const BlockAttnParams& p, const BALine& a
   int at = 0;
   for (int b0 = 0; b0 < a.n_seqs; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < a.n_seqs ? ba_tiles(p, ba_ctx(p, b)) * per : 0;
+    const int n = b < a.n_seqs ? ba_places(p, ba_ctx(p, b)) * per : 0;
     int inc = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -282,30 +286,39 @@ struct BASeg {
 // The segments of a block's piece [u, u1) of the line, in order.
 struct BAWalk {
   int u, u1, seq_begin, b;
+  int ctx, ctx_next;       // of sequences b and b + 1, read before they are needed
   __device__ __forceinline__ void start(const BlockAttnParams& p, const BALine& a) {
     u = a.start(static_cast<int>(blockIdx.x));
     u1 = a.start(static_cast<int>(blockIdx.x) + 1);
     seq_begin = 0;
     b = u < u1 ? ba_find(p, a, u, &seq_begin) : 0;
+    ctx = u < u1 ? ba_ctx(p, b) : 0;
+    ctx_next = u < u1 && b + 1 < a.n_seqs ? ba_ctx(p, b + 1) : 0;
   }
   __device__ __forceinline__ bool next(const BlockAttnParams& p, const BALine& a, BASeg& s) {
-    if (u >= u1) return false;
-    s.b = b;
-    s.ctx = ba_ctx(p, b);
-    s.old = s.ctx - a.q_len;
-    s.nt = ba_tiles(p, s.ctx);
-    const int in_seq = u - seq_begin;
-    const int hr = ba_div(in_seq, s.nt);                       // (KV head, row chunk)
-    s.ta = in_seq - hr * s.nt;
-    s.h = a.rc == 1 ? hr : ba_div(hr, a.rc);
-    s.row_lo = (hr - s.h * a.rc) * a.chunk_rows;
-    s.tb = min(s.nt, u1 - u + s.ta);
-    u += s.tb - s.ta;
-    if (s.tb == s.nt && hr + 1 == p.h_kv * a.rc) {
-      seq_begin = u;
-      ++b;
+    while (u < u1) {
+      s.b = b;
+      s.ctx = ctx;
+      s.old = ctx - a.q_len;
+      s.nt = ba_tiles(p, ctx);
+      const int len = kBASwitch + s.nt;
+      const int in_seq = u - seq_begin;
+      const int hr = ba_div(in_seq, len);                      // (KV head, row chunk)
+      const int from = in_seq - hr * len, to = min(len, u1 - u + from);
+      s.h = a.rc == 1 ? hr : ba_div(hr, a.rc);
+      s.row_lo = (hr - s.h * a.rc) * a.chunk_rows;
+      s.ta = max(0, from - kBASwitch);
+      s.tb = max(0, to - kBASwitch);
+      u += to - from;
+      if (to == len && hr + 1 == p.h_kv * a.rc) {
+        seq_begin = u;
+        ++b;
+        ctx = ctx_next;
+        ctx_next = b + 1 < a.n_seqs ? ba_ctx(p, b + 1) : 0;
+      }
+      if (s.tb > s.ta) return true;                            // else the piece ends before the segment's first tile
     }
-    return true;
+    return false;
   }
 };
 
@@ -321,6 +334,13 @@ struct BAPlace {
       s = 0;
       ph ^= 1u;
     }
+  }
+  __device__ __forceinline__ void back(int stages) {
+    if (s == 0) {
+      s = stages;
+      ph ^= 1u;
+    }
+    --s;
   }
 };
 
@@ -414,6 +434,32 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   BASeg sg = {};
   BAPlace at = {0, 0u}, qat = {0, 0u};       // stage of the piece's next tile, of its next queries
   bool ok = true;
+  // The queries of segment s into the next buffer, a quarter (NF = 2: half) by each of NF warps.
+  auto copy_queries = [&](int f, const BASeg& s) {
+    const int rows = min(a.chunk_rows, a.q_rows - s.row_lo);
+    constexpr int CH = D / 8;                // 16-byte pieces of a query row: a lane keeps its piece
+    const int c = lane % CH;
+    for (int lr = f * (32 / CH) + lane / CH; lr < ROWS; lr += NF * (32 / CH)) {
+      uint8_t* d = qbuf + qat.s * S::Q + lr * S::QPITCH + c * 16;
+      const int rr = s.row_lo + min(lr, rows - 1);
+      const int qi = ba_token(p, rr), g = rr - qi * p.group;
+      const int64_t row = p.q_sb == 0 ? static_cast<int64_t>(s.b) * a.q_len + qi : qi;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + s.b * p.q_sb + row * p.q_st +
+                            static_cast<int64_t>(s.h * p.group + g) * p.q_sh + c * 8;
+      // padding rows take 0 of the 16 bytes: zeros
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(d)), "l"(src), "r"(lr < rows ? 16 : 0)
+                   : "memory");
+    }
+    if (p.tree != nullptr && f == NF - 1) {
+      for (int lr = lane; lr < ROWS; lr += 32) {
+        const int qi = ba_token(p, s.row_lo + min(lr, rows - 1));
+        const uint64_t* src = p.tree + s.b * p.tree_sb + qi * p.tree_st;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(qbuf + qat.s * S::Q + S::TREE + lr * 8)), "l"(src) : "memory");
+      }
+    }
+    cp_async_mbar_arrive(&q_full[qat.s]);
+    if (lane == 0 && f == 0) SPECQ_TRACE_POINT(4, qat.s);
+  };
 
   if (warp >= kBAWarps) {                    // ---- the feeding warps: warp f takes tiles f, f + NF, ... of the piece
     if constexpr (ba_split(NT)) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -421,41 +467,13 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     const int nb = TOK >> (31 - __clz(p.box));          // boxes of a tile; a batch of 32 is `tpb` of the warp's tiles
     const int tpb = 32 / nb;                 // (all powers of two)
     const int lt = lane >> (31 - __clz(nb)), lb = lane & (nb - 1);
-    int segment = 0;
+    bool q_done = true;                      // the computing warps copy the piece's first queries
+    qat.step(2);
     int skip = f;                            // tiles of the segment before the warp's next one
     // pages that one block reads are read once; of several row chunks the first leaves them in L2
     const uint64_t hint = a.rc == 1 ? policy_evict_first() : policy_evict_last();
     while (walk.next(p, a, sg)) {
       const int32_t* bt = p.bt + sg.b * p.bt_sb;
-      bool q_done = false;
-      auto copy_queries = [&]() {
-        q_done = true;
-        ok = ok && mbar_wait(&q_empty[qat.s], qat.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
-        const int rows = min(a.chunk_rows, a.q_rows - sg.row_lo);
-        constexpr int CH = D / 8;            // 16-byte pieces of a query row: a lane keeps its piece
-        const int c = lane % CH;
-        for (int lr = f * (32 / CH) + lane / CH; lr < ROWS; lr += NF * (32 / CH)) {
-          uint8_t* d = qbuf + qat.s * S::Q + lr * S::QPITCH + c * 16;
-          const int rr = sg.row_lo + min(lr, rows - 1);
-          const int qi = ba_token(p, rr), g = rr - qi * p.group;
-          const int64_t row = p.q_sb == 0 ? static_cast<int64_t>(sg.b) * a.q_len + qi : qi;
-          const uint16_t* src = static_cast<const uint16_t*>(p.q) + sg.b * p.q_sb + row * p.q_st +
-                                static_cast<int64_t>(sg.h * p.group + g) * p.q_sh + c * 8;
-          // padding rows take 0 of the 16 bytes: zeros
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(d)), "l"(src), "r"(lr < rows ? 16 : 0)
-                       : "memory");
-        }
-        if (p.tree != nullptr && f == NF - 1) {
-          for (int lr = lane; lr < ROWS; lr += 32) {
-            const int qi = ba_token(p, sg.row_lo + min(lr, rows - 1));
-            const uint64_t* src = p.tree + sg.b * p.tree_sb + qi * p.tree_st;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(qbuf + qat.s * S::Q + S::TREE + lr * 8)), "l"(src) : "memory");
-          }
-        }
-        cp_async_mbar_arrive(&q_full[qat.s]);
-        if (lane == 0 && f == 0) SPECQ_TRACE_POINT(4, qat.s);
-        qat.step(2);
-      };
       int t0 = sg.ta + skip;                 // the batch's first tile
       int pg = -1, tok = 0;
       auto load_pages = [&]() {
@@ -464,7 +482,12 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
         pg = t < sg.tb && tok < sg.ctx ? __ldg(bt + (tok >> p.page_log2)) : -1;
       };
       load_pages();
-      if (segment++ > 0) copy_queries();     // the piece's first tile goes before its queries
+      if (!q_done) {
+        ok = ok && mbar_wait(&q_empty[qat.s], qat.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+        copy_queries(f, sg);
+        qat.step(2);
+      }
+      q_done = false;
       int stepped = sg.ta;                   // `at` is the stage of this tile
       for (; t0 < sg.tb;) {
         const int my_tile = t0 + lt * NF, my_tok = tok;
@@ -473,11 +496,6 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
         if (load && !there) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
         const int page = there ? pg : 0;
         float ks = 0.f, vs = 0.f;
-        if (there) {
-          const int64_t x = static_cast<int64_t>(page) * p.s_sp + sg.h * p.s_sh;
-          ks = __ldg(p.ks + x);
-          vs = __ldg(p.vs + x);
-        }
         const int t1 = min(sg.tb, t0 + tpb * NF);
         const int tb0 = t0;
         t0 += tpb * NF;
@@ -504,6 +522,11 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
               }
             };
             start(ring + at.s * S::KB, &mk, &k_full[at.s]);
+            if (t == tb0 && there) {         // the batch's scales, behind its first boxes
+              const int64_t x = static_cast<int64_t>(page) * p.s_sp + sg.h * p.s_sh;
+              ks = __ldg(p.ks + x);
+              vs = __ldg(p.vs + x);
+            }
             if constexpr (!TWO) start(ring + (stages + at.s) * S::KB, &mv, &k_full[at.s]);
             if (mine) {
               // a masked score, -inf, times ck stays -inf; what is not there weighs nothing
@@ -527,10 +550,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
               start(ring + (stages + at.s) * S::KB, &mv, &v_full[at.s]);
             }
           }
-          if (!q_done) copy_queries();
         }
       }
-      if (!q_done) copy_queries();
       for (; stepped < sg.tb; ++stepped) at.step(stages);
       skip = (skip + NF - (sg.tb - sg.ta) % NF) % NF;
     }
@@ -563,7 +584,10 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   const uint32_t p_get = p_base + static_cast<uint32_t>((lane & 7) * S::PPITCH + (lane >> 3) * 16);
 
   int tile_no = 0;                           // of the piece
-  while (walk.next(p, a, sg)) {
+  for (bool first = true; walk.next(p, a, sg); first = false) {
+    // The piece's first queries are on their way before any tile, so they do not queue behind the
+    // ring's first filling; the feeding warps copy the others, ahead.
+    if (first && warp < NF) copy_queries(warp, sg);
     // ---- Q^T as the B operand: thread (gq, tq) holds row gq of each group, d = 16 c + 4 tq + 0..3
     uint32_t qf[NT][KC][2];
     float fac = 1.f;
@@ -741,12 +765,17 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
           }
         named_barrier_sync(1 + grp, 32 * kBAGroupWarps);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+          float2 top2 = make_float2(m[n][0], m[n][1]);
+#pragma unroll
+          for (int w = 0; w < kBAGroupWarps; ++w) {
+            const float2 v = *reinterpret_cast<const float2*>(&sm_m[(grp * kBAGroupWarps + w) * ROWS + n * 8 + 2 * tq]);
+            top2.x = fmaxf(top2.x, v.x);
+            top2.y = fmaxf(top2.y, v.y);
+          }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float mn = m[n][r];
-#pragma unroll
-            for (int w = 0; w < kBAGroupWarps; ++w) mn = fmaxf(mn, sm_m[(grp * kBAGroupWarps + w) * ROWS + n * 8 + 2 * tq + r]);
+            const float mn = r == 0 ? top2.x : top2.y;
             const float f = ex2(m[n][r] - mn);
             m[n][r] = mn;
             l[n][r] *= f;
@@ -756,6 +785,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
               o[c][n][2 + r] *= f;
             }
           }
+        }
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -837,7 +867,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       pl.step(stages);
       pl.step(stages);
     }
-    for (int x = 0; x < n_all; ++x) at.step(stages);
+    at = pl;                                 // of the tile after the segment's last:
+    if (first_mine + 2 * n_mine > n_all) at.back(stages);
 
     __syncwarp();                            // the queries' buffer (and its tree words) may be filled again
     if (lane == 0) mbar_arrive(&q_empty[qat.s]);
@@ -856,9 +887,9 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
         l[n][r] = v;
       }
     if (sg.ta > 0 || sg.tb < sg.nt) {
-      // a piece of a cut segment: a group that had a tile writes its part to the workspace (O of each
-      // warp's elements, l of each warp's tokens, m) and goes on
-      if (n_mine > 0) {
+      // a piece of a cut segment: each group writes its part to the workspace (O of each warp's
+      // elements, l of each warp's tokens, m; a group that had no tile has l = 0) and goes on
+      {
         float* part = p.part_o + (2 * (2 * static_cast<int64_t>(blockIdx.x) + (sg.ta == 0 ? 1 : 0)) + grp) * (ROWS * S::PART);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -940,24 +971,23 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
   const int h = a.rc > 1 ? ba_div(hr, a.rc) : hr, row_lo = (hr - h * a.rc) * a.chunk_rows;
   const int lr = blockIdx.y * 8 + warp;
   bool work = a.rc > 0 && b < a.n_seqs && lr < min(a.chunk_rows, a.q_rows - row_lo);
-  int s0 = 0, nt = 0, c0 = 0, c1 = 0;
+  int c0 = 0, c1 = 0;
   if (work) {
     // where the segment lies on the line
     int before = 0;
     for (int b0 = 0; b0 < b; b0 += 32) {
       const int x = b0 + lane;
-      before += __reduce_add_sync(0xffffffffu, x < b ? ba_tiles(p, ba_ctx(p, x)) : 0);
+      before += __reduce_add_sync(0xffffffffu, x < b ? ba_places(p, ba_ctx(p, x)) : 0);
     }
-    nt = ba_tiles(p, ba_ctx(p, b));
-    s0 = before * per + hr * nt;
+    const int nt = ba_tiles(p, ba_ctx(p, b));
+    const int s0 = before * per + hr * (kBASwitch + nt) + kBASwitch;      // its first tile
     c0 = a.piece_of(s0);
     c1 = a.piece_of(s0 + nt - 1);
     work = c0 != c1;                                            // else inside one piece: written already
   }
   pdl_wait();                                                   // every block, or the next kernel could pass this one
   if (!work) return;
-  // piece c0 holds the segment's beginning (its second slot), the others begin inside it; tile n of a
-  // piece is group n % 2's, so a group has a part unless the segment has one tile there, the other's
+  // piece c0 holds the segment's beginning (its second slot), the others begin inside it
   constexpr int V = D / 32, PART = ba_part(D);
   float v[V];
 #pragma unroll
@@ -973,8 +1003,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
       l[i] = 0.f;
 #pragma unroll
       for (int y = 0; y < V; ++y) w[i][y] = 0.f;
-      const int from = max(s0, a.start(c)), to = min(s0 + nt, a.start(c + 1));
-      if (c <= c1 && (to - from > 1 || ((from - a.start(c)) & 1) == grp)) {
+      if (c <= c1) {
         const float* src = p.part_o + (static_cast<int64_t>(2 * (2 * c + (c == c0 ? 1 : 0)) + grp) * p.rows + lr) * PART;
         const float4 l4 = __ldg(reinterpret_cast<const float4*>(src + D));
         m[i] = __ldg(src + D + kBAGroupWarps);
@@ -1040,7 +1069,7 @@ inline int ba_shape(int B, int ql, int H_KV, int group, int D, int page, int bt_
   s->tile = ba_tile(s->nt);
   const int64_t max_tiles = std::max<int64_t>(1, (static_cast<int64_t>(bt_cols) * page + s->tile - 1) / s->tile);
   const int64_t line = static_cast<int64_t>(B) * H_KV * s->rc * max_tiles;
-  if (line > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %lld tiles", (long long)line);
+  if (line + static_cast<int64_t>(B) * H_KV * s->rc * kBASwitch > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %lld tiles", (long long)line);
   s->grid = static_cast<int>(std::min<int64_t>(line, static_cast<int64_t>(per_sm) * sm_count));
   s->join = max_tiles > 1;
   int fixed, stage;
@@ -1162,6 +1191,7 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
   p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.n_pages = n_pages; p.bt_cols = bt_cols;
   p.bf16 = dtype == 2; p.stages = s.stages; p.grid = s.grid; p.rows = s.rows; p.box = std::min(64, page); p.tile = s.tile;
+  p.tile_log2 = 31 - __builtin_clz(static_cast<unsigned>(s.tile));
   p.rc = s.rc; p.chunk_rows = ceil_div(ceil_div(ql * p.group, 8), s.rc) * 8;
   p.group_magic = p.group > 1 ? 0xFFFFFFFFu / static_cast<uint32_t>(p.group) + 1u : 0u;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
