@@ -28,7 +28,8 @@
 // the products.  Rows are the N side of both products and pad to 8.  Feeding warps walk the same
 // segments ahead of the others: they read page numbers and scales, start the TMA boxes (up to 64
 // slots of a page) into a ring and copy the next queries, so a new segment finds its first tiles
-// in shared memory.
+// in shared memory.  The piece's first queries are copied by the computing warps: behind the ring's
+// first filling they came 2.5 us later.
 //
 // Why mma.sync: a 16-token tile of 8n rows is 16 n instructions, and the warp-level tensor pipe
 // takes one every 2 cycles an SM (measured; 1024 multiply-adds a cycle): 2 n cycles a token,
@@ -37,18 +38,19 @@
 // instruction, with round trips through tensor memory between the steps.  More than 40 rows go to
 // several blocks, which find the pages in L2; there the products are the bound.
 //
-// Measured (D = 128, 8 KV heads, group 4, page 64): B = 32, q = 1, context 4096: 57.4 us, 4.7 TB/s (heads
-// before slots in a page: 50.2 us, 5.3 TB/s, of the 6.44 that a copy reaches), bound by HBM.  B = 8,
-// q = 9, context 4096: 42 us, of which some 20 are set-up and the join (a launch runs its set-up once,
-// from cold instruction caches), and 2,500 cycles a tile where the products alone would take 1,525: two
+// Measured (D = 128, 8 KV heads, group 4, page 64): B = 32, q = 1, context 4096: 55.5 us, 4.8 TB/s (heads
+// before slots in a page: 49.5 us, 5.4 TB/s, of the 6.44 that a copy reaches), bound by HBM.  B = 8,
+// q = 9, context 4096: 36 us, of which some 16 are set-up and the join (a launch runs its set-up once,
+// from cold instruction caches), and 2,400 cycles a tile where the products alone would take 1,525: two
 // warps a quarter of the SM are all that the registers hold (Q and O of 40 rows), too few to cover
-// their own latencies.
+// their own latencies.  D = 64: two blocks of 24 rows an SM were 35 us for q = 9, one of 40 rows is 27.
 //
-// Work.  The tiles of all (sequence, KV head, row chunk) segments form one line, cut into equal
-// pieces, one for each resident block, whatever the sequences' lengths; each block finds its
-// piece from ctx_len on the device.  A segment inside one piece is written at once; the parts of a
-// cut one, two groups' for each piece, go to the workspace, and a second, dependent launch joins
-// them in the pieces' order.
+// Work.  The tiles of all (sequence, KV head, row chunk) segments form one line, each segment's after
+// some places that stand for the time its beginning takes; the line is cut into equal pieces, one
+// for each resident block, whatever the sequences' lengths, and each block finds its piece from
+// ctx_len on the device.  A segment inside one piece is written at once; the parts of a cut one,
+// two groups' for each piece, go to the workspace, and a second, dependent launch joins them in the
+// pieces' order.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -75,8 +77,11 @@ __host__ __device__ constexpr int ba_threads(int nt) { return kBACompute + 32 * 
 // Tokens of a tile: up to 16 rows two blocks share an SM, and half as many tokens leave each a ring
 // of six stages.
 __host__ __device__ constexpr int ba_tile(int nt) { return ba_split(nt) ? 128 : 64; }
-// Places of the line that a segment takes before its tiles.
-constexpr int kBASwitch = 2;
+// Places of the line that a segment takes before its tiles: a block that begins a segment spends
+// 6,000 to 8,000 cycles on it (the part before, the next queries, a first tile that raises the maxima),
+// a tile some 2,400 at D = 128 and 1,500 at D = 64.  Measured without, with these and with 6 and 8: B = 8
+// q = 9 ctx 4096 39 / 36.0 / 37.8 us; D = 64, 24 ragged lengths of up to 4000, q = 5: 48 / 30.4 / 31.7 us.
+__host__ __device__ constexpr int ba_switch(int d) { return d == 64 ? 4 : 3; }
 constexpr int kBAMaxGroups = 5;                   // groups of 8 query rows a block holds at most
 constexpr int kBAMaxStages = 8;
 constexpr float kBARaise = 8.f;         // log2 of how far p may pass 1 before the maximum is raised
@@ -100,6 +105,7 @@ struct BlockAttnParams {
   int n_seqs, q_len, b_max, ql_max, h_kv, group, page_log2, n_pages, bt_cols;
   int bf16, stages, grid, rows, box;    // rows: of a block's chunk; box: slots of a TMA box
   int tile, tile_log2;                  // tokens of a tile
+  int places;                           // of the line, before a segment's tiles
   int rc, chunk_rows;                   // row chunks of a (sequence, KV head) and their rows, without a plan
   uint32_t group_magic;                 // ceil(2^32 / group), for group > 1
 };
@@ -180,7 +186,7 @@ __device__ __forceinline__ int ba_div(int a, int b) {
   return q;
 }
 
-// Where the segments of a call lie on the line.  A segment takes kBASwitch places, in which nothing
+// Where the segments of a call lie on the line.  A segment takes p.places places, in which nothing
 // is done, and then one for each of its tiles: beginning a segment costs a block about as much.
 // Piece c of the line (one a block) is [start(c), start(c + 1)): the first `more` pieces have one
 // place more than the others.
@@ -200,7 +206,7 @@ __device__ __forceinline__ int ba_ctx(const BlockAttnParams& p, int b) {
   return min(max(c, 0), p.bt_cols << p.page_log2);
 }
 __device__ __forceinline__ int ba_tiles(const BlockAttnParams& p, int ctx) { return max(1, (ctx + p.tile - 1) >> p.tile_log2); }
-__device__ __forceinline__ int ba_places(const BlockAttnParams& p, int ctx) { return kBASwitch + ba_tiles(p, ctx); }
+__device__ __forceinline__ int ba_places(const BlockAttnParams& p, int ctx) { return p.places + ba_tiles(p, ctx); }
 
 __device__ __forceinline__ BALine ba_line(const BlockAttnParams& p, bool tell) {
   BALine a;
@@ -283,42 +289,51 @@ struct BASeg {
   int ta, tb, nt;          // tiles of this piece, tiles of the segment
 };
 
-// The segments of a block's piece [u, u1) of the line, in order.
+// The segments of a block's piece [u, u1) of the line, in order.  (The divisions are in start():
+// what a block executes once runs from cold instruction caches, some 20 cycles an instruction.)
 struct BAWalk {
-  int u, u1, seq_begin, b;
+  int u, u1;
+  int b, h, chunk, from;   // of the segment at u, and u's place in it
   int ctx, ctx_next;       // of sequences b and b + 1, read before they are needed
   __device__ __forceinline__ void start(const BlockAttnParams& p, const BALine& a) {
     u = a.start(static_cast<int>(blockIdx.x));
     u1 = a.start(static_cast<int>(blockIdx.x) + 1);
-    seq_begin = 0;
-    b = u < u1 ? ba_find(p, a, u, &seq_begin) : 0;
-    ctx = u < u1 ? ba_ctx(p, b) : 0;
-    ctx_next = u < u1 && b + 1 < a.n_seqs ? ba_ctx(p, b + 1) : 0;
+    b = h = chunk = from = ctx = ctx_next = 0;
+    if (u >= u1) return;
+    int begin;
+    b = ba_find(p, a, u, &begin);
+    ctx = ba_ctx(p, b);
+    if (b + 1 < a.n_seqs) ctx_next = ba_ctx(p, b + 1);
+    const int len = ba_places(p, ctx), hr = ba_div(u - begin, len);
+    from = u - begin - hr * len;
+    h = a.rc == 1 ? hr : ba_div(hr, a.rc);
+    chunk = hr - h * a.rc;
   }
   __device__ __forceinline__ bool next(const BlockAttnParams& p, const BALine& a, BASeg& s) {
-    while (u < u1) {
+    do {
+      if (u >= u1) return false;
       s.b = b;
+      s.h = h;
+      s.row_lo = chunk * a.chunk_rows;
       s.ctx = ctx;
       s.old = ctx - a.q_len;
       s.nt = ba_tiles(p, ctx);
-      const int len = kBASwitch + s.nt;
-      const int in_seq = u - seq_begin;
-      const int hr = ba_div(in_seq, len);                      // (KV head, row chunk)
-      const int from = in_seq - hr * len, to = min(len, u1 - u + from);
-      s.h = a.rc == 1 ? hr : ba_div(hr, a.rc);
-      s.row_lo = (hr - s.h * a.rc) * a.chunk_rows;
-      s.ta = max(0, from - kBASwitch);
-      s.tb = max(0, to - kBASwitch);
+      const int to = min(p.places + s.nt, from + u1 - u);
+      s.ta = max(0, from - p.places);
+      s.tb = max(0, to - p.places);
       u += to - from;
-      if (to == len && hr + 1 == p.h_kv * a.rc) {
-        seq_begin = u;
-        ++b;
-        ctx = ctx_next;
-        ctx_next = b + 1 < a.n_seqs ? ba_ctx(p, b + 1) : 0;
+      from = 0;
+      if (++chunk == a.rc) {
+        chunk = 0;
+        if (++h == p.h_kv) {
+          h = 0;
+          ++b;
+          ctx = ctx_next;
+          if (b + 1 < a.n_seqs) ctx_next = ba_ctx(p, b + 1);
+        }
       }
-      if (s.tb > s.ta) return true;                            // else the piece ends before the segment's first tile
-    }
-    return false;
+    } while (s.tb == s.ta);                  // the piece may end before the segment's first tile
+    return true;
   }
 };
 
@@ -980,7 +995,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
       before += __reduce_add_sync(0xffffffffu, x < b ? ba_places(p, ba_ctx(p, x)) : 0);
     }
     const int nt = ba_tiles(p, ba_ctx(p, b));
-    const int s0 = before * per + hr * (kBASwitch + nt) + kBASwitch;      // its first tile
+    const int s0 = before * per + hr * (p.places + nt) + p.places;      // its first tile
     c0 = a.piece_of(s0);
     c1 = a.piece_of(s0 + nt - 1);
     work = c0 != c1;                                            // else inside one piece: written already
@@ -1069,7 +1084,7 @@ inline int ba_shape(int B, int ql, int H_KV, int group, int D, int page, int bt_
   s->tile = ba_tile(s->nt);
   const int64_t max_tiles = std::max<int64_t>(1, (static_cast<int64_t>(bt_cols) * page + s->tile - 1) / s->tile);
   const int64_t line = static_cast<int64_t>(B) * H_KV * s->rc * max_tiles;
-  if (line + static_cast<int64_t>(B) * H_KV * s->rc * kBASwitch > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %lld tiles", (long long)line);
+  if (line + static_cast<int64_t>(B) * H_KV * s->rc * ba_switch(D) > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %lld tiles", (long long)line);
   s->grid = static_cast<int>(std::min<int64_t>(line, static_cast<int64_t>(per_sm) * sm_count));
   s->join = max_tiles > 1;
   int fixed, stage;
@@ -1191,6 +1206,7 @@ inline int run_block_attention(const void* q, int64_t q_sb, int64_t q_st, int64_
   p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.n_pages = n_pages; p.bt_cols = bt_cols;
   p.bf16 = dtype == 2; p.stages = s.stages; p.grid = s.grid; p.rows = s.rows; p.box = std::min(64, page); p.tile = s.tile;
+  p.places = ba_switch(D);
   p.tile_log2 = 31 - __builtin_clz(static_cast<unsigned>(s.tile));
   p.rc = s.rc; p.chunk_rows = ceil_div(ceil_div(ql * p.group, 8), s.rc) * 8;
   p.group_magic = p.group > 1 ? 0xFFFFFFFFu / static_cast<uint32_t>(p.group) + 1u : 0u;
