@@ -17,16 +17,20 @@
 //
 // A warp holds 8 (16 at D = 64) slots of one page and head in registers, 32 fp32 a thread,
 // so the rotated values are made once and used twice, for the maximum and for the numbers; the
-// warps that share a larger page are of one CTA and exchange their maxima through shared memory.  The same launch turns the tokens' queries: they come from the
-// same rows, and a launch of their own costs a short verification step as much as the work.
-// Bound by HBM for prompts and by latency for a few tokens.
+// warps that share a larger page are of one CTA and exchange their maxima through shared memory.
+// The same launch turns the tokens' queries: they come from the same rows, and a launch of their
+// own costs a short verification step as much as the work.  Bound by HBM for prompts and by latency
+// for a few tokens.  Measured (32 query and 8 KV heads of 128): 4 x 2047 tokens, page 64: 41 us,
+// 4.6 TB/s (with 64 values a thread and half the blocks an SM 47 us); 8 x 9 tokens: 4.5 us.
 //
 // compact.  After verification the accepted drafts of sequence b sit at base + accept[b, j]
 // (base = ctx_len - q_len); they move to base + j.  A target page's scale becomes
 //   s' = max(s, max over its arriving tokens of (max |q| * fp32(1 / q_max)) * s_source)
 // and numbers whose scale differs are requantised, rn(q * (s_source / s')).  One warp per
 // (layer, sequence, head, K or V) walks its tokens in order, 4 or 8 at a time: accept[j] >= j
-// and both grow, so a token never lands on one that has yet to be read.
+// and both grow, so a token never lands on one that has yet to be read.  Bound by HBM's and the
+// TLBs' handling of scattered 128-byte rows.  Measured: 48 trees of 33 nodes, 32 layers, 8 heads of
+// 128: 26.3 us for 83 MB, 3.2 TB/s; 8 chains of 9, one layer: 3.0 us, the three loads of its chain.
 #pragma once
 
 #include <cuda_fp8.h>

@@ -1,10 +1,10 @@
 // pages.cuh -- the page pool of a paged KV cache on the device: release, reserve, fork.
 //
 // State: ref [P] (how many rows hold a page; 0 = free), tbl [S, C] (the rows' pages, -1 past
-// the held ones, which every call keeps so) and held [S] (pages a row holds).  There is no free list: a page is free when
-// its count is 0, and pages are handed out lowest index first, row by row, so the result of
-// every call is a function of the state alone (the atomics below add integers, whose order
-// does not matter, or claim nothing).
+// the held ones, which every call keeps so) and held [S] (pages a row holds).  There is no free
+// list: a page is free when its count is 0, and pages are handed out lowest index first, row by
+// row, so the result of every call is a function of the state alone (the atomics below add
+// integers, whose order does not matter, or claim nothing).
 //
 // release  every held page of a dropped row counts one less; the row empties.
 // reserve  row r is extended to ceil(want[r] / page) pages.  All rows or, when the free pages
@@ -17,10 +17,12 @@
 //
 // The work is a few kilobytes of integers, so what counts is the number of dependent steps.
 // reserve is one CTA that reads ref in runs of 8 counts a thread (8,192 pages a step, one
-// block scan each, the free ones listed in shared memory and placed by a warp a row) and stops when it has found enough.  fork is that CTA, which up to
-// kForkSmall table cells also rewrites the rows between two barriers, and then a grid that copies
-// the pages (bound by HBM); a larger table is snapshot by the copying grid and rewritten by a
-// third.  The kernels follow one another by programmatic launch.
+// block scan each, the free ones listed in shared memory and placed by a warp a row) and stops when
+// it has found enough.  fork is that CTA, which up to kForkSmall table cells also rewrites the rows
+// between two barriers, and then a grid that copies the pages (bound by HBM); a larger table is
+// snapshot by the copying grid and rewritten by a third.  The kernels follow one another by
+// programmatic launch.  Measured, release + reserve + fork: 8 rows, one layer 11 us; 192 rows in
+// beams of 4, 16 layers of pages of 16 x 8 x 128: 27.6 us, of which the copies' bytes need 8.8.
 #pragma once
 
 #include "sm100.cuh"

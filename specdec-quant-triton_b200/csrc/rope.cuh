@@ -11,6 +11,8 @@
 // bytes (half layout: the 16 bytes of both partners) of kRopeHeads heads of one token, so the
 // pair's cosines and sines are loaded once for all of them and the heads' loads are in flight
 // together; short calls, whose time is the latency of one load, take one head a thread.
+// Measured (B200): 8190 x 40 x 128 bf16, interleaved, first 64 turned: 28.7 us, 5.9 TB/s of the 6.44
+// that a copy reaches; one token of 40 heads: 1.5 us in a stream of launches.
 #pragma once
 
 #include <cuda_bf16.h>
