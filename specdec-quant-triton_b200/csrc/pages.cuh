@@ -20,8 +20,8 @@
 // block scan each, the free ones listed in shared memory and placed by a warp a row) and stops when
 // it has found enough.  fork is that CTA, which up to kForkSmall table cells also rewrites the rows
 // between two barriers, and then a grid that copies the pages (bound by HBM); a larger table is
-// snapshot by the copying grid and rewritten by a third.  The kernels follow one another by
-// programmatic launch.  Measured, release + reserve + fork: 8 rows, one layer 11 us; 192 rows in
+// snapshot by other CTAs beside the planning one and rewritten by blocks of the copying grid.  The
+// kernels follow one another by programmatic launch.  Measured, release + reserve + fork: 8 rows, one layer 11 us; 192 rows in
 // beams of 4, 16 layers of pages of 16 x 8 x 128: 27.6 us, of which the copies' bytes need 8.8.
 #pragma once
 
@@ -209,23 +209,21 @@ struct PageForkParams {
   int64_t kv_sl, kv_sp, kv_so, kv_sh, s_sl, s_sp, s_sh;
   int page, h_kv, D, L;
   int small;               // the table is rewritten by the planning CTA
+  int planes;              // blocks that copy a row's page
   int dense;               // a page's tokens and heads are contiguous
 };
 
 constexpr int kForkSmall = 2048;   // S * C: 2 cells a thread of the planning CTA (at 14,784 it takes 25 us for them)
 
 // Row r, which is forked with `to` as its copied page, takes its share of the parent's pages:
-// snapshot (before any row is rewritten) and rewrite, each by `step` threads from `c0`.
+// snapshot (before any row is rewritten) and rewrite, each by `step` threads from `c0`.  The rows'
+// additions to the counts and subtractions from them may come in any order: a page is subtracted
+// at most once for each row that held it.
 __device__ __forceinline__ void fork_snapshot(const PageForkParams& f, int r, int c0, int step) {
   const int p = f.parent[r], full = f.length[p] / f.page;
   const int32_t* from_row = f.pool.tbl + p * f.pool.ld;
   int32_t* snap = f.snap + static_cast<int64_t>(r) * f.pool.C;
-  for (int c = c0; c < full; c += step) {
-    const int pg = from_row[c];
-    snap[c] = pg;
-    if (pg < 0 || pg >= f.pool.P) report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
-    else atomicAdd(f.pool.ref + pg, 1);
-  }
+  for (int c = c0; c < full; c += step) snap[c] = from_row[c];
 }
 __device__ __forceinline__ void fork_rewrite(const PageForkParams& f, int r, int to, int c0, int step) {
   const int full = f.length[f.parent[r]] / f.page, had = pool_held(f.pool, r);
@@ -240,7 +238,13 @@ __device__ __forceinline__ void fork_rewrite(const PageForkParams& f, int r, int
         report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
       }
     }
-    row[c] = c < full ? snap[c] : (c == full && to >= 0 ? to : -1);
+    int now = c == full && to >= 0 ? to : -1;
+    if (c < full) {
+      now = snap[c];
+      if (now < 0 || now >= f.pool.P) report_status(f.pool.status, SPECQ_STATUS_BAD_INDEX);
+      else atomicAdd(f.pool.ref + now, 1);
+    }
+    row[c] = now;
   }
 }
 __device__ __forceinline__ int fork_held(const PageForkParams& f, int r, int to) {
@@ -263,6 +267,12 @@ __device__ __forceinline__ int fork_parent(const PageForkParams& f, int r, bool 
 __global__ void __launch_bounds__(kPoolThreads) pages_fork_plan_kernel(const __grid_constant__ PageForkParams f) {
   pdl_launch_dependents();
   pdl_wait();
+  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
+  if (blockIdx.x > 0) {                   // beside the planning CTA: the parents' rows of a large table
+    const int r = (static_cast<int>(blockIdx.x) - 1) * (kPoolThreads / 32) + warp;
+    if (r < f.pool.S && fork_parent(f, r, false) >= 0) fork_snapshot(f, r, lane, 32);
+    return;
+  }
   extern __shared__ int list[];
   int* start = list + kPoolThreads * kPoolRun;
   __shared__ int red[33];
@@ -293,7 +303,6 @@ __global__ void __launch_bounds__(kPoolThreads) pages_fork_plan_kernel(const __g
   if (threadIdx.x == 0) *f.short_out = missing;
   if (f.small == 0 || missing > 0) return;
   __syncthreads();
-  const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
   for (int r = warp; r < f.pool.S; r += kPoolThreads / 32)
     if (f.fresh[r] != -2) fork_snapshot(f, r, lane, 32);
   __syncthreads();
@@ -308,15 +317,20 @@ __global__ void __launch_bounds__(kPoolThreads) pages_fork_plan_kernel(const __g
 
 constexpr int kForkThreads = 256;
 
-// Block (row, y) copies the row's page in the (layer, K|V) pairs y, y + Y, ...; the blocks of y = 0
-// also snapshot the parents' rows of a large table.
+// Block (row, y) copies the row's page in the (layer, K|V) pairs y, y + planes, ...; the blocks of
+// y = planes rewrite the rows of a large table.
 __global__ void __launch_bounds__(kForkThreads) pages_fork_copy_kernel(const __grid_constant__ PageForkParams f) {
   pdl_launch_dependents();
   pdl_wait();
   const int r = blockIdx.x;
   const int to = f.fresh[r];
   if (to == -2) return;
-  if (f.small == 0 && blockIdx.y == 0) fork_snapshot(f, r, threadIdx.x, kForkThreads);
+  if (blockIdx.y == static_cast<unsigned>(f.planes)) {
+    fork_rewrite(f, r, to, threadIdx.x, kForkThreads);
+    __syncthreads();       // every thread has read held[r]
+    if (threadIdx.x == 0) f.pool.held[r] = fork_held(f, r, to);
+    return;
+  }
   if (to < 0) return;
   const int n = f.length[f.parent[r]];
   const int rest = n - n / f.page * f.page;
@@ -327,7 +341,7 @@ __global__ void __launch_bounds__(kForkThreads) pages_fork_copy_kernel(const __g
   }
   // all pairs' 16-byte pieces as one run, several loads in flight
   const unsigned chunks = f.D >> 4, per_slot = f.h_kv * chunks, items = rest * per_slot;
-  const unsigned pairs = (2 * f.L - blockIdx.y + gridDim.y - 1) / gridDim.y;
+  const unsigned pairs = (2 * f.L - blockIdx.y + f.planes - 1) / f.planes;
   constexpr int U = 8;
   for (unsigned i0 = threadIdx.x; i0 < items * pairs; i0 += U * kForkThreads) {
     uint4 w[U];
@@ -338,7 +352,7 @@ __global__ void __launch_bounds__(kForkThreads) pages_fork_copy_kernel(const __g
       at[u] = nullptr;
       if (i < items * pairs) {
         const unsigned pair = i / items, in = i - pair * items;
-        const unsigned y = blockIdx.y + pair * gridDim.y;
+        const unsigned y = blockIdx.y + pair * f.planes;
         int64_t off;
         if (f.dense) {
           off = static_cast<int64_t>(in) * 16;
@@ -356,21 +370,10 @@ __global__ void __launch_bounds__(kForkThreads) pages_fork_copy_kernel(const __g
       if (at[u] != nullptr) *reinterpret_cast<uint4*>(at[u]) = w[u];
   }
   for (unsigned i = threadIdx.x; i < pairs * f.h_kv; i += kForkThreads) {
-    const unsigned pair = i / f.h_kv, h = i - pair * f.h_kv, y = blockIdx.y + pair * gridDim.y;
+    const unsigned pair = i / f.h_kv, h = i - pair * f.h_kv, y = blockIdx.y + pair * f.planes;
     float* scale = ((y & 1) ? f.vs : f.ks) + (y >> 1) * f.s_sl + h * f.s_sh;
     scale[to * f.s_sp] = scale[from * f.s_sp];
   }
-}
-
-__global__ void __launch_bounds__(128) pages_fork_rows_kernel(const __grid_constant__ PageForkParams f) {
-  pdl_launch_dependents();
-  pdl_wait();
-  const int r = blockIdx.x;
-  const int to = f.fresh[r];
-  if (to == -2) return;
-  fork_rewrite(f, r, to, threadIdx.x, 128);
-  __syncthreads();         // every thread has read held[r]
-  if (threadIdx.x == 0) f.pool.held[r] = fork_held(f, r, to);
 }
 
 inline int make_pool(const char* who, PagePool* p, int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held,
@@ -454,20 +457,19 @@ inline int run_pages_fork(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int6
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   SPECQ_CUDA_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(pages_fork_plan_kernel), static_cast<int>(pool_smem(S))));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(1);
+  cfg.gridDim = dim3(1 + (f.small ? 0 : ceil_div(S, kPoolThreads / 32)));
   cfg.blockDim = dim3(kPoolThreads);
   cfg.dynamicSmemBytes = pool_smem(S);
   cfg.stream = st;
   LaunchAttrs at(1);
   at.apply(cfg);
-  SPECQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, pages_fork_plan_kernel, f));
-  if (S == 0) return SPECQ_OK;
   // enough blocks for eight an SM; each then copies several layers' pages with its loads in flight
   DeviceState* dev = nullptr;
   if (int rc = get_device_state(&dev)) return rc;
-  const int y = std::max(1, std::min(2 * L, ceil_div(8 * dev->sm_count, S)));
-  if (L > 0 || f.small == 0) SPECQ_CUDA_TRY(launch_plain(pages_fork_copy_kernel, dim3(S, y), dim3(kForkThreads), st, f));
-  if (f.small == 0) SPECQ_CUDA_TRY(launch_plain(pages_fork_rows_kernel, dim3(S), dim3(128), st, f));
+  f.planes = S > 0 ? std::min(2 * L, std::max(1, ceil_div(8 * dev->sm_count, S))) : 0;
+  SPECQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, pages_fork_plan_kernel, f));
+  const int y = f.planes + (f.small ? 0 : 1);
+  if (S > 0 && y > 0) SPECQ_CUDA_TRY(launch_plain(pages_fork_copy_kernel, dim3(S, y), dim3(kForkThreads), st, f));
   return SPECQ_OK;
 }
 
