@@ -18,11 +18,10 @@
 // The work is a few kilobytes of integers, so what counts is the number of dependent steps.
 // reserve is one CTA that reads ref in runs of 8 counts a thread (8,192 pages a step, one
 // block scan each, the free ones listed in shared memory and placed by a warp a row) and stops when
-// it has found enough.  fork is that CTA, which up to kForkSmall table cells also rewrites the rows
-// between two barriers, and then a grid that copies the pages (bound by HBM); a larger table is
-// snapshot by other CTAs beside the planning one and rewritten by blocks of the copying grid.  The
-// kernels follow one another by programmatic launch.  Measured, release + reserve + fork: 8 rows, one layer 11 us; 192 rows in
-// beams of 4, 16 layers of pages of 16 x 8 x 128: 27.6 us, of which the copies' bytes need 8.8.
+// it has found enough.  fork is that CTA and beside it others that snapshot the parents' rows, and
+// then a grid that copies the pages (bound by HBM) and rewrites the rows.  The kernels follow one
+// another by programmatic launch.  Measured, release + reserve + fork: 8 rows, one layer 9.2 us; 192 rows in
+// beams of 4, 16 layers of pages of 16 x 8 x 128: 24.1 us, of which the copies' bytes need 8.8.
 #pragma once
 
 #include "sm100.cuh"
@@ -208,12 +207,9 @@ struct PageForkParams {
   float* vs;
   int64_t kv_sl, kv_sp, kv_so, kv_sh, s_sl, s_sp, s_sh;
   int page, h_kv, D, L;
-  int small;               // the table is rewritten by the planning CTA
   int planes;              // blocks that copy a row's page
   int dense;               // a page's tokens and heads are contiguous
 };
-
-constexpr int kForkSmall = 2048;   // S * C: 2 cells a thread of the planning CTA (at 14,784 it takes 25 us for them)
 
 // Row r, which is forked with `to` as its copied page, takes its share of the parent's pages:
 // snapshot (before any row is rewritten) and rewrite, each by `step` threads from `c0`.  The rows'
@@ -268,7 +264,7 @@ __global__ void __launch_bounds__(kPoolThreads) pages_fork_plan_kernel(const __g
   pdl_launch_dependents();
   pdl_wait();
   const int warp = static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31);
-  if (blockIdx.x > 0) {                   // beside the planning CTA: the parents' rows of a large table
+  if (blockIdx.x > 0) {                   // beside the planning CTA: the parents' rows
     const int r = (static_cast<int>(blockIdx.x) - 1) * (kPoolThreads / 32) + warp;
     if (r < f.pool.S && fork_parent(f, r, false) >= 0) fork_snapshot(f, r, lane, 32);
     return;
@@ -301,24 +297,12 @@ __global__ void __launch_bounds__(kPoolThreads) pages_fork_plan_kernel(const __g
   if (missing > 0)
     for (int r = threadIdx.x; r < f.pool.S; r += kPoolThreads) f.fresh[r] = -2;
   if (threadIdx.x == 0) *f.short_out = missing;
-  if (f.small == 0 || missing > 0) return;
-  __syncthreads();
-  for (int r = warp; r < f.pool.S; r += kPoolThreads / 32)
-    if (f.fresh[r] != -2) fork_snapshot(f, r, lane, 32);
-  __syncthreads();
-  for (int r = warp; r < f.pool.S; r += kPoolThreads / 32) {
-    const int to = f.fresh[r];
-    if (to == -2) continue;
-    fork_rewrite(f, r, to, lane, 32);
-    __syncwarp();          // every lane has read held[r]
-    if (lane == 0) f.pool.held[r] = fork_held(f, r, to);
-  }
 }
 
 constexpr int kForkThreads = 256;
 
 // Block (row, y) copies the row's page in the (layer, K|V) pairs y, y + planes, ...; the blocks of
-// y = planes rewrite the rows of a large table.
+// y = planes rewrite the rows.
 __global__ void __launch_bounds__(kForkThreads) pages_fork_copy_kernel(const __grid_constant__ PageForkParams f) {
   pdl_launch_dependents();
   pdl_wait();
@@ -452,12 +436,11 @@ inline int run_pages_fork(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int6
   f.kc = static_cast<uint8_t*>(kc); f.vc = static_cast<uint8_t*>(vc); f.ks = ks; f.vs = vs;
   f.kv_sl = kv_sl; f.kv_sp = kv_sp; f.kv_so = kv_so; f.kv_sh = kv_sh; f.s_sl = s_sl; f.s_sp = s_sp; f.s_sh = s_sh;
   f.page = page; f.h_kv = H_KV; f.D = D; f.L = L;
-  f.small = static_cast<int64_t>(S) * C <= kForkSmall;
   f.dense = kv_sh == D && kv_so == static_cast<int64_t>(H_KV) * D;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   SPECQ_CUDA_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(pages_fork_plan_kernel), static_cast<int>(pool_smem(S))));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(1 + (f.small ? 0 : ceil_div(S, kPoolThreads / 32)));
+  cfg.gridDim = dim3(1 + ceil_div(S, kPoolThreads / 32));
   cfg.blockDim = dim3(kPoolThreads);
   cfg.dynamicSmemBytes = pool_smem(S);
   cfg.stream = st;
@@ -468,8 +451,7 @@ inline int run_pages_fork(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int6
   if (int rc = get_device_state(&dev)) return rc;
   f.planes = S > 0 ? std::min(2 * L, std::max(1, ceil_div(8 * dev->sm_count, S))) : 0;
   SPECQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, pages_fork_plan_kernel, f));
-  const int y = f.planes + (f.small ? 0 : 1);
-  if (S > 0 && y > 0) SPECQ_CUDA_TRY(launch_plain(pages_fork_copy_kernel, dim3(S, y), dim3(kForkThreads), st, f));
+  if (S > 0) SPECQ_CUDA_TRY(launch_plain(pages_fork_copy_kernel, dim3(S, f.planes + 1), dim3(kForkThreads), st, f));
   return SPECQ_OK;
 }
 
