@@ -20,17 +20,20 @@
 // warps that share a larger page are of one CTA and exchange their maxima through shared memory.
 // The same launch turns the tokens' queries: they come from the same rows, and a launch of their
 // own costs a short verification step as much as the work.  Bound by HBM for prompts and by latency
-// for a few tokens.  Measured (32 query and 8 KV heads of 128): 4 x 2047 tokens, page 64: 41 us,
-// 4.6 TB/s (with 64 values a thread and half the blocks an SM 47 us); 8 x 9 tokens: 4.5 us.
+// for a few tokens.  Measured (32 query and 8 KV heads of 128): 4 x 2047 tokens, page 64: 36.9 us,
+// 5.1 TB/s (keys and values of 64 values a thread and half the blocks an SM took 6 us more, blocks of
+// queries among those of keys and values 0.7); 8 x 9 tokens: 4.5 us.
 //
 // compact.  After verification the accepted drafts of sequence b sit at base + accept[b, j]
 // (base = ctx_len - q_len); they move to base + j.  A target page's scale becomes
 //   s' = max(s, max over its arriving tokens of (max |q| * fp32(1 / q_max)) * s_source)
 // and numbers whose scale differs are requantised, rn(q * (s_source / s')).  One warp per
 // (layer, sequence, head, K or V) walks its tokens in order, 4 or 8 at a time: accept[j] >= j
-// and both grow, so a token never lands on one that has yet to be read.  Bound by HBM's and the
-// TLBs' handling of scattered 128-byte rows.  Measured: 48 trees of 33 nodes, 32 layers, 8 heads of
-// 128: 26.3 us for 83 MB, 3.2 TB/s; 8 chains of 9, one layer: 3.0 us, the three loads of its chain.
+// and both grow, so a token never lands on one that has yet to be read.  Bound by scattered reads
+// and writes of 128 bytes.  Measured: 48 trees of 33 nodes, 32 layers, 8 heads of 128: 26.3 us for
+// some 83 MB, 3.2 TB/s (40 warps an SM in place of 28: the same; two to eight heads a warp, the next
+// one's tokens read ahead: 31 to 46; half as many tokens in flight: 31); 8 chains of 9, one layer:
+// 3.0 us, the three loads of its chain.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -129,6 +132,7 @@ struct BlockAppendParams {
   int* status;
   int64_t kt, kh, vt, vh, qt, qh, ot, oh, kv_sp, kv_so, kv_sh, s_sp, s_sh, bt_sb;
   int n_seqs, q_len, b_grid, ql_max, h_kv, h_q, page_log2, n_pages, bt_cols, rot, n_pos, half;
+  int wide;                           // rows of K and V are 16-byte aligned
   int n_win, win_blocks, kv_blocks;   // pages a sequence may touch, blocks of one of them, blocks of all
   int q_items, q_groups;
 };
@@ -232,13 +236,24 @@ block_append_kernel(const __grid_constant__ BlockAppendParams p) {
   {
     const int64_t st = is_v ? p.vt : p.kt;
     const T* r = static_cast<const T*>(is_v ? p.v : p.k) + head * (is_v ? p.vh : p.kh) + row0 * st;
+    // one 16-byte load for both runs where they adjoin (41.0 -> 36.9 us for 4 x 2047 tokens)
+    if (p.wide && o2 == o1 + 4) {
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
+      for (int i = 0; i < STEPS; ++i) {
+        Row16<T> w;
+        w.raw = make_uint4(0u, 0u, 0u, 0u);
+        if (i >= lo && i < hi) w.load(r + i * TPS * st + o1);
+        w.get(x[i]);
+      }
+    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
-      if (i >= lo && i < hi) {
-        load_row4<T>(r + i * TPS * st + o1, x[i]);
-        load_row4<T>(r + i * TPS * st + o2, x[i] + 4);
+      for (int i = 0; i < STEPS; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] = 0.f;
+        if (i >= lo && i < hi) {
+          load_row4<T>(r + i * TPS * st + o1, x[i]);
+          load_row4<T>(r + i * TPS * st + o2, x[i] + 4);
+        }
       }
     }
   }
@@ -401,6 +416,7 @@ inline int run_block_append(const void* k, int64_t kt, int64_t kh, const void* v
   p.n_seqs = n_seqs; p.q_len = q_len; p.b_grid = b_grid; p.ql_max = ql; p.h_kv = H_KV; p.h_q = H;
   p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.n_pages = n_pages; p.bt_cols = bt_cols; p.rot = rot; p.n_pos = n_pos; p.half = layout == 0;
+  p.wide = aligned(k, 16) && aligned(v, 16) && kt % 8 == 0 && kh % 8 == 0 && vt % 8 == 0 && vh % 8 == 0;
   const int slots = append_slots(D, page);
   const int wpu = std::max(1, page / slots);
   p.n_win = (ql - 1) / page + 2;

@@ -182,6 +182,26 @@ def test_append_plan(cuda):
     assert _status() == 0
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("shift", [4, 12])
+def test_append_rows_of_eight_byte_alignment(cuda, layout, shift):
+    """K and V rows that begin off a 16-byte boundary, or whose stride leaves it, are stored as aligned ones are."""
+    import specq
+    gen = torch.Generator().manual_seed(shift)
+    B, Q, KV, D, page = 3, 19, 2, 128, 16
+    tbl = _table(gen, B, 4, 14)
+    ctx = torch.tensor([19, 33, 60], dtype=torch.int32).cuda()
+    table = specq.rope_table(64, 64, device="cuda")
+    wide = torch.randn(B * Q, 2 * KV * D + 2 * shift, generator=gen).half().cuda()
+    k, v = (wide[:, shift + i * KV * D: shift + (i + 1) * KV * D].unflatten(1, (KV, D)) for i in range(2))
+    base = [_stored(gen, (14, page, KV, D), "int8") for _ in range(2)] + [_scales(gen, (14, KV), "int8") for _ in range(2)]
+    a, b = [t.clone() for t in base], [t.clone() for t in base]
+    specq.kv_append_blocks(k, v, *a, tbl, ctx, Q, table=table, layout=layout)
+    specq.kv_append_blocks(k.contiguous(), v.contiguous(), *b, tbl, ctx, Q, table=table, layout=layout)
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
+    assert _status() == 0
+
+
 # ---- attention ---------------------------------------------------------------------------------
 UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
