@@ -82,6 +82,7 @@ __host__ __device__ constexpr int ba_tile(int nt) { return ba_split(nt) ? 128 : 
 // a tile some 2,400 at D = 128 and 1,500 at D = 64.  Measured without, with these and with 6 and 8: B = 8
 // q = 9 ctx 4096 39 / 36.0 / 37.8 us; D = 64, 24 ragged lengths of up to 4000, q = 5: 48 / 30.4 / 31.7 us.
 __host__ __device__ constexpr int ba_switch(int d) { return d == 64 ? 4 : 3; }
+constexpr int kBAComputeRegs = 224, kBAFeedRegs = 56;
 constexpr int kBAMaxGroups = 5;                   // groups of 8 query rows a block holds at most
 constexpr int kBAMaxStages = 8;
 constexpr float kBARaise = 8.f;         // log2 of how far p may pass 1 before the maximum is raised
@@ -477,7 +478,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   };
 
   if (warp >= kBAWarps) {                    // ---- the feeding warps: warp f takes tiles f, f + NF, ... of the piece
-    if constexpr (ba_split(NT)) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if constexpr (ba_split(NT)) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBAFeedRegs));
     const int f = warp - kBAWarps;
     const int nb = TOK >> (31 - __clz(p.box));          // boxes of a tile; a batch of 32 is `tpb` of the warp's tiles
     const int tpb = 32 / nb;                 // (all powers of two)
@@ -582,7 +583,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   }
 
   // ---- the computing warps
-  if constexpr (ba_split(NT)) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+  if constexpr (ba_split(NT)) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBAComputeRegs));
   const int grp = warp >> 2, gw = warp & 3;  // group, warp of the group
   const int gq = lane >> 2, tq = lane & 3;
   // ldmatrix rows of this lane: matrix lane / 8 = (token half, piece); pieces are swizzled
@@ -1103,6 +1104,15 @@ template <int D, int CT, int NT>
 inline int launch_block_attn(const BlockAttnParams& p, const BAShape& s, const CUtensorMap& mk, const CUtensorMap& mv,
                              cudaStream_t st) {
   auto kern = block_attn_kernel<D, CT, NT>;
+  if constexpr (ba_split(NT)) {
+    // The computing warps wait for registers that the launch has to bring: fewer would be waited for without end.
+    static const int regs = [&] {
+      cudaFuncAttributes fa = {};
+      return cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(kern)) == cudaSuccess ? fa.numRegs : 0;
+    }();
+    if (regs * ba_threads(NT) < 32 * (kBAWarps * kBAComputeRegs + ba_feeders(NT) * kBAFeedRegs))
+      return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: built with %d registers a thread, too few to split", regs);
+  }
   SPECQ_CUDA_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(kern), s.smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(s.grid));
