@@ -40,7 +40,7 @@
 //
 // Measured (D = 128, 8 KV heads, group 4, page 64): B = 32, q = 1, context 4096: 55.5 us, 4.8 TB/s (heads
 // before slots in a page: 49.5 us, 5.4 TB/s, of the 6.44 that a copy reaches), bound by HBM.  B = 8,
-// q = 9, context 4096: 36 us, of which some 16 are set-up and the join (a launch runs its set-up once,
+// q = 9, context 4096: 35 us, of which some 15 are set-up and the join (a launch runs its set-up once,
 // from cold instruction caches), and 2,400 cycles a tile where the products alone would take 1,525: two
 // warps a quarter of the SM are all that the registers hold (Q and O of 40 rows), too few to cover
 // their own latencies.  D = 64: two blocks of 24 rows an SM were 35 us for q = 9, one of 40 rows is 27.
@@ -82,6 +82,10 @@ __host__ __device__ constexpr int ba_tile(int nt) { return ba_split(nt) ? 128 : 
 // a tile some 2,400 at D = 128 and 1,500 at D = 64.  Measured without, with these and with 6 and 8: B = 8
 // q = 9 ctx 4096 39 / 36.0 / 37.8 us; D = 64, 24 ragged lengths of up to 4000, q = 5: 48 / 30.4 / 31.7 us.
 __host__ __device__ constexpr int ba_switch(int d) { return d == 64 ? 4 : 3; }
+// Fewest places of a piece.  Measured with 1, 2, 3, 4 and 6: one sequence of 3000 tokens, q = 1, D = 128
+// 29.0 / 18.7 / 15.7 / 14.3 / 13.3 us; 16 drafts on 2500 tokens, one KV head, D = 64 19.9 / 14.5 / 13.4 /
+// 13.1 / 14.0; 6 x 23 rows, context 286 10.0 / 10.0 / 10.5 / 12.2 / 10.4; one short sequence 5.1, with 6 7.0.
+constexpr int kBAPiece = 3;
 constexpr int kBAComputeRegs = 224, kBAFeedRegs = 56;
 constexpr int kBAMaxGroups = 5;                   // groups of 8 query rows a block holds at most
 constexpr int kBAMaxStages = 8;
@@ -190,11 +194,12 @@ __device__ __forceinline__ int ba_div(int a, int b) {
 // Where the segments of a call lie on the line.  A segment takes p.places places, in which nothing
 // is done, and then one for each of its tiles: beginning a segment costs a block about as much.
 // Piece c of the line (one a block) is [start(c), start(c + 1)): the first `more` pieces have one
-// place more than the others.
+// place more than the others.  A piece has kBAPiece places at least: a block's two groups take two
+// tiles in the time of one, and every piece is two more parts to join.
 struct BALine {
   int n_seqs, q_len, q_rows, rc;   // rc: row chunks of a (sequence, KV head)
   int chunk_rows;                  // rows of a chunk (a multiple of 8)
-  int each, more;
+  int pieces, each, more;
   __device__ __forceinline__ int start(int c) const { return each * c + min(c, more); }
   __device__ __forceinline__ int piece_of(int u) const {
     const int wide = more * (each + 1);
@@ -240,8 +245,9 @@ __device__ __forceinline__ BALine ba_line(const BlockAttnParams& p, bool tell) {
     a.chunk_rows = a.rc > 0 ? ba_div(groups + a.rc - 1, a.rc) * 8 : 0;
   }
   const int total = t * (p.h_kv * a.rc);
-  a.each = ba_div(total, p.grid);
-  a.more = total - a.each * p.grid;
+  a.pieces = min(p.grid, max(1, ba_div(total, kBAPiece)));
+  a.each = ba_div(total, a.pieces);
+  a.more = total - a.each * a.pieces;
   return a;
 }
 
@@ -300,6 +306,7 @@ struct BAWalk {
     u = a.start(static_cast<int>(blockIdx.x));
     u1 = a.start(static_cast<int>(blockIdx.x) + 1);
     b = h = chunk = from = ctx = ctx_next = 0;
+    if (static_cast<int>(blockIdx.x) >= a.pieces) u = u1;
     if (u >= u1) return;
     int begin;
     b = ba_find(p, a, u, &begin);
@@ -1009,7 +1016,7 @@ __global__ void __launch_bounds__(256) block_attn_join_kernel(const __grid_const
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] = 0.f;
   float sum = 0.f, top = kBANone;
-  constexpr int U = 4;                                          // parts in flight
+  constexpr int U = 8;                                          // parts in flight (4: verify 36.0 us, 8: 35.2, 16: 38.1)
   for (int x0 = 2 * c0; x0 <= 2 * c1 + 1; x0 += U) {
     float m[U], l[U], w[U][V];
 #pragma unroll
