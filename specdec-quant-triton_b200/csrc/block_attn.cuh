@@ -38,7 +38,7 @@
 // instruction, with round trips through tensor memory between the steps.  More than 40 rows go to
 // several blocks, which find the pages in L2; there the products are the bound.
 //
-// Measured (D = 128, 8 KV heads, group 4, page 64): B = 32, q = 1, context 4096: 55.5 us, 4.8 TB/s (heads
+// Measured (D = 128, 8 KV heads, group 4, page 64): B = 32, q = 1, context 4096: 55.0 us, 4.9 TB/s (heads
 // before slots in a page: 49.5 us, 5.4 TB/s, of the 6.44 that a copy reaches), bound by HBM.  B = 8,
 // q = 9, context 4096: 35 us, of which some 15 are set-up and the join (a launch runs its set-up once,
 // from cold instruction caches), and 2,400 cycles a tile where the products alone would take 1,525: two
@@ -477,7 +477,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       for (int lr = lane; lr < ROWS; lr += 32) {
         const int qi = ba_token(p, s.row_lo + min(lr, rows - 1));
         const uint64_t* src = p.tree + s.b * p.tree_sb + qi * p.tree_st;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(qbuf + qat.s * S::Q + S::TREE + lr * 8)), "l"(src) : "memory");
+        const uint32_t d = smem_u32(qbuf + qat.s * S::Q + S::TREE + lr * 8);
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
       }
     }
     cp_async_mbar_arrive(&q_full[qat.s]);
@@ -566,7 +567,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_full[at.s]);
             if (lane == 0) SPECQ_TRACE_POINT(5, t);
-            if constexpr (TWO) ok = ok && mbar_wait(&v_empty[at.s], at.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
+            if constexpr (TWO)
+              ok = ok && mbar_wait(&v_empty[at.s], at.ph ^ 1u, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
             if (TWO && ok) {
               if (lane == 0) mbar_arrive_expect_tx(&v_full[at.s], __popc(boxes) * p.box * D);
               __syncwarp();
@@ -596,14 +598,17 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
   // ldmatrix rows of this lane: matrix lane / 8 = (token half, piece); pieces are swizzled
   const int mr = (lane & 7) + ((lane >> 3) & 1) * 8, mc = lane >> 4;
   const uint32_t ring_s = smem_u32(ring);
-  const uint32_t k_off = ring_s + static_cast<uint32_t>((gw * 16 * U + mr) * D + ((mc ^ (D == 128 ? (mr & 7) : ((mr >> 1) & 3))) << 4));
+  const uint32_t k_off =
+      ring_s + static_cast<uint32_t>((gw * 16 * U + mr) * D + ((mc ^ (D == 128 ? (mr & 7) : ((mr >> 1) & 3))) << 4));
   // V: MT = 2, matrices (token half, piece); MT = 1, (token half, next 16 tokens)
   const int vr = MT == 2 ? mr : mr + mc * 16;
   const int vc = MT == 2 ? 2 * gw + mc : gw;
-  const uint32_t v_off = ring_s + static_cast<uint32_t>(stages * S::KB) + static_cast<uint32_t>(vr * D + ((vc ^ (D == 128 ? (vr & 7) : ((vr >> 1) & 3))) << 4));
+  const uint32_t v_off =
+      ring_s + static_cast<uint32_t>(stages * S::KB + vr * D + ((vc ^ (D == 128 ? (vr & 7) : ((vr >> 1) & 3))) << 4));
   // P: this lane's row of the matrices that it stores (group pair, token half) and loads (32 tokens of a group)
   const uint32_t p_base = smem_u32(pbuf + grp * S::P);
-  const uint32_t p_put = p_base + static_cast<uint32_t>(((lane >> 4) * 8 + (lane & 7)) * S::PPITCH + (U * gw * 16 + ((lane >> 3) & 1) * 8) * 2);
+  const uint32_t p_put =
+      p_base + static_cast<uint32_t>(((lane >> 4) * 8 + (lane & 7)) * S::PPITCH + (U * gw * 16 + ((lane >> 3) & 1) * 8) * 2);
   const uint32_t p_get = p_base + static_cast<uint32_t>((lane & 7) * S::PPITCH + (lane >> 3) * 16);
 
   int tile_no = 0;                           // of the piece
@@ -829,7 +834,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
         // (token, row) fragments turned on the way to P [row][token]
         const uint32_t d = p_put + static_cast<uint32_t>(u * 32);
 #pragma unroll
-        for (int n = 0; n + 1 < NT; n += 2) stsm4_t(d + static_cast<uint32_t>(n * 8 * S::PPITCH), h[n][0], h[n][1], h[n + 1][0], h[n + 1][1]);
+        for (int n = 0; n + 1 < NT; n += 2)
+          stsm4_t(d + static_cast<uint32_t>(n * 8 * S::PPITCH), h[n][0], h[n][1], h[n + 1][0], h[n + 1][1]);
         if constexpr (NT % 2 == 1) stsm2_t(d + static_cast<uint32_t>((NT - 1) * 8 * S::PPITCH), h[NT - 1][0], h[NT - 1][1]);
       }
     };
@@ -1092,7 +1098,8 @@ inline int ba_shape(int B, int ql, int H_KV, int group, int D, int page, int bt_
   s->tile = ba_tile(s->nt);
   const int64_t max_tiles = std::max<int64_t>(1, (static_cast<int64_t>(bt_cols) * page + s->tile - 1) / s->tile);
   const int64_t line = static_cast<int64_t>(B) * H_KV * s->rc * max_tiles;
-  if (line + static_cast<int64_t>(B) * H_KV * s->rc * ba_switch(D) > 0x7FFFFFFFll) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %lld tiles", (long long)line);
+  if (line + static_cast<int64_t>(B) * H_KV * s->rc * ba_switch(D) > 0x7FFFFFFFll)
+    return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %lld tiles", (long long)line);
   s->grid = static_cast<int>(std::min<int64_t>(line, static_cast<int64_t>(per_sm) * sm_count));
   s->join = max_tiles > 1;
   int fixed, stage;

@@ -198,8 +198,9 @@ def run(steps=20, rows=8, layers=4, nodes=21, seed=0, check=False, dtype=torch.i
     torch.cuda.synchronize()
     missing = max(int(x.item()) for x in shorts)
     status = _lib.get_status(clear=True)
-    return {"steps": steps, "rows": rows, "layers": layers, "nodes": nodes, "cache": str(dtype)[6:], "accepted_tokens": accepted,
-            "forks": forks, "ended": ended, "ms_per_step": (time.perf_counter() - t0) / steps * 1e3,
+    return {"steps": steps, "rows": rows, "layers": layers, "nodes": nodes, "cache": str(dtype)[6:],
+            "accepted_tokens": accepted, "forks": forks, "ended": ended,
+            "ms_per_step": (time.perf_counter() - t0) / steps * 1e3,
             "missing_pages": missing, "status": status, "max_abs_error": worst if check else None}
 
 
