@@ -699,30 +699,32 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     BAPlace pl = at;
     auto softmax = [&](int t) {              // of tile t, whose place is pl
       // softmax: rows 2 tq, 2 tq + 1 of each group, tokens gq and gq + 8 of each 16
-      float ck[U], lv[U], lv1[U], iv[U], iv_rel[U];
+      float ck[U], lv[U], lv1[U], iv[U], iv1[U];   // 1: of tokens gq + 8
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float4 w0 = scales[pl.s * S::SC + 2 * (U * gw + u)];
         ck[u] = w0.x * fac;
         lv[u] = lv1[u] = w0.y;
-        iv[u] = w0.z;
-        iv_rel[u] = 1.f;
+        iv[u] = iv1[u] = w0.z;
       }
       const int tw = t * TOK + 16 * U * gw;  // the warp's first token
       if (p.page_log2 == 3 || tw + 16 * U > sg.old) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           if (p.page_log2 == 3) {            // tokens 8 .. 15 are another page's, with its own scales
-            const float ck0 = scales[pl.s * S::SC + 2 * (U * gw + u)].x;
             const float4 w1 = scales[pl.s * S::SC + 2 * (U * gw + u) + 1];
             lv1[u] = w1.y;
-            iv_rel[u] = iv[u] > 0.f ? w1.z / iv[u] : 0.f;
-            const float rel = w1.x / ck0;
+            iv1[u] = w1.z;
+            // each half under its own page's scale here (either page may be one that weighs nothing)
+            const float ck1 = w1.x * fac;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              sc[u][n][2] *= rel;
-              sc[u][n][3] *= rel;
-            }
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                sc[u][n][r] *= ck[u];
+                sc[u][n][2 + r] *= ck1;
+              }
+            ck[u] = 1.f;
           }
           const int t0 = tw + 16 * u;
           if (t0 + 16 > sg.old) {            // some row may not see some token
@@ -825,7 +827,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
           for (int r = 0; r < 2; ++r) {
             y[r] = ex2(sc[u][n][r] - m[n][r]);
             y[2 + r] = ex2(sc[u][n][2 + r] - m[n][r]);
-            l[n][r] = fmaf(fmaf(y[2 + r], iv_rel[u], y[r]), iv[u], l[n][r]);
+            l[n][r] = fmaf(y[2 + r], iv1[u], fmaf(y[r], iv[u], l[n][r]));
           }
           const __half2 h0 = __floats2half2_rn(y[0], y[1]), h1 = __floats2half2_rn(y[2], y[3]);
           h[n][0] = *reinterpret_cast<const uint32_t*>(&h0);

@@ -1,0 +1,51 @@
+"""The block-scaled cache's operators at the edges of their inputs: tiny, zero and outlying queries, page numbers
+outside the cache, rows that a call does not reach, gradients of the rotation, kernels on each other's heels.
+
+Attention is compared with the 64-bit oracle under the bound derived in test_blocks_gpu.py; a page number
+outside the cache takes its tokens out of the window, so there the oracle gets the table without that page."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import block_oracle as BO
+from test_blocks_gpu import UNIT, _attend_check, _attend_inputs, _np, _status
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- page numbers outside the cache -------------------------------------------------------------------
+def _without_pages(q, kc, vc, ks, vs, tbl, cl, bad):
+    """The 64-bit result where the pages `bad` (lists of columns, one a sequence; whole pages before the
+    drafts) are not there, and the bound's parts."""
+    page, parts = kc.shape[1], []
+    for b, cols in enumerate(bad):
+        row = np.delete(tbl[b].cpu().numpy(), cols)[None]
+        parts.append(BO.attention(_np(q[b: b + 1]), _np(kc), _np(vc), _np(ks), _np(vs), row, [int(cl[b]) - page * len(cols)]))
+    return [np.concatenate(p) for p in zip(*parts)]
+
+
+def _attend_with_bad_pages(args, bad):
+    import specq
+    from specq import _lib
+    q, kc, vc, ks, vs, tbl, cl = args
+    ref, mag, size = _without_pages(q, kc, vc, ks, vs, tbl, cl, bad)
+    broken = tbl.clone()
+    for b, cols in enumerate(bad):
+        for i, c in enumerate(cols):
+            broken[b, c] = (-1, kc.shape[0], 1 << 30, -(1 << 31))[(b + i) % 4]
+    got = specq.paged_attention_blocks(q, kc, vc, ks, vs, broken, cl)
+    assert _status() == _lib.SPECQ_STATUS_BAD_INDEX
+    assert torch.isfinite(got).all()
+    lim = UNIT[q.dtype] * np.abs(ref) + (2.0 ** -11 + 2 * (132 * 2.0 ** -24 * size[..., None] + 2.0 ** -14)) * mag + 2.0 ** -24
+    err = np.abs(_np(got) - ref)
+    assert (err <= lim).all(), (err.max(), (err / lim).max())
+
+
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Q,KV,G,D", [(1, 2, 4, 128), (4, 1, 8, 64), (3, 2, 1, 128)])
+def test_attention_steps_over_a_bad_page_of_eight(cuda, kind, dtype, Q, KV, G, D):
+    """At page 8 two pages share 16 tokens of a tile: a bad even or odd one takes no weight from the other."""
+    args = _attend_inputs(31, 5, Q, KV, G, D, 8, kind, dtype, [40, 47, 90, 300, 24 + Q])
+    for bad in ([[2], [3], [0, 5], [4, 7, 10, 33], []], [[0, 2], [1], [1, 2], [16, 17, 18], [2]]):
+        _attend_with_bad_pages(args, bad)
