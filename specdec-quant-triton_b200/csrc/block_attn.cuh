@@ -92,6 +92,7 @@ constexpr int kBAMaxStages = 8;
 constexpr float kBARaise = 8.f;         // log2 of how far p may pass 1 before the maximum is raised
 constexpr float kBANone = -1e30f;        // the running maximum of a row that has seen no token: finite, so that a
                                          // masked score, -inf, less it is -inf and not NaN
+constexpr float kBALeastK = 1e-37f;              // the least factor of a score that may be masked
 constexpr float kBALeastV = 8.077935669463161e-28f;   // 2^-90: a smaller V scale reads as this
 
 struct BlockAttnParams {
@@ -553,11 +554,10 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
             }
             if constexpr (!TWO) start(ring + (stages + at.s) * S::KB, &mv, &k_full[at.s]);
             if (mine) {
-              // a masked score, -inf, times ck stays -inf; what is not there weighs nothing
-              float4 w = make_float4(1e-37f, -INFINITY, 0.f, 0.f);
+              float4 w = make_float4(0.f, -INFINITY, 0.f, 0.f);   // what is not there weighs nothing
               if (there) {
                 const float v = vs < kBALeastV ? kBALeastV : vs;
-                w.x = fmaxf(ks * p.scale_log2, 1e-37f);
+                w.x = ks * p.scale_log2;
                 w.y = __log2f(v);
                 w.z = __frcp_rn(v);
               }
@@ -703,29 +703,43 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const float4 w0 = scales[pl.s * S::SC + 2 * (U * gw + u)];
-        ck[u] = w0.x * fac;
+        ck[u] = w0.x;
         lv[u] = lv1[u] = w0.y;
         iv[u] = iv1[u] = w0.z;
       }
-      const int tw = t * TOK + 16 * U * gw;  // the warp's first token
-      if (p.page_log2 == 3 || tw + 16 * U > sg.old) {
+      // What the scores are multiplied by: one number for 16 tokens, in the sum with lv below.  At page 8 tokens
+      // 8 .. 15 are another page's, with its own scales, and bf16 queries bring their power of two; there the
+      // scores are multiplied here, before any of them is masked, since that number may underflow and 0 times
+      // a masked -inf is NaN (below, its floor keeps it from that: a score under it weighs as 0 does).
+      if (p.bf16 || p.page_log2 == 3) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          if (p.page_log2 == 3) {            // tokens 8 .. 15 are another page's, with its own scales
+          float c0 = ck[u], c1 = c0;
+          if (p.page_log2 == 3) {
             const float4 w1 = scales[pl.s * S::SC + 2 * (U * gw + u) + 1];
+            c1 = w1.x;
             lv1[u] = w1.y;
             iv1[u] = w1.z;
-            // each half under its own page's scale here (either page may be one that weighs nothing)
-            const float ck1 = w1.x * fac;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                sc[u][n][r] *= ck[u];
-                sc[u][n][2 + r] *= ck1;
-              }
-            ck[u] = 1.f;
           }
+          c0 *= fac;
+          c1 *= fac;
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              sc[u][n][r] *= c0;
+              sc[u][n][2 + r] *= c1;
+            }
+          ck[u] = 1.f;
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) ck[u] = fmaxf(ck[u], kBALeastK);
+      }
+      const int tw = t * TOK + 16 * U * gw;  // the warp's first token
+      if (tw + 16 * U > sg.old) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
           const int t0 = tw + 16 * u;
           if (t0 + 16 > sg.old) {            // some row may not see some token
             // bits 4n + 2r + half of what this thread's rows see of its two tokens

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import block_oracle as BO
-from test_blocks_gpu import UNIT, _attend_check, _attend_inputs, _np, _status
+from test_blocks_gpu import UNIT, _attend_check, _attend_inputs, _np, _random_tree, _status
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,40 @@ def test_attention_steps_over_a_bad_page_of_eight(cuda, kind, dtype, Q, KV, G, D
     args = _attend_inputs(31, 5, Q, KV, G, D, 8, kind, dtype, [40, 47, 90, 300, 24 + Q])
     for bad in ([[2], [3], [0, 5], [4, 7, 10, 33], []], [[0, 2], [1], [1, 2], [16, 17, 18], [2]]):
         _attend_with_bad_pages(args, bad)
+
+
+# ---- queries of any size ----------------------------------------------------------------------------
+@pytest.mark.parametrize("page", [8, 16, 32])
+@pytest.mark.parametrize("Q,KV,G,D", [(1, 2, 4, 128), (5, 1, 4, 64), (9, 2, 4, 128)])
+@pytest.mark.parametrize("kind", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_attention_of_zero_queries(cuda, dtype, kind, Q, KV, G, D, page):
+    """Zero queries see every token alike: the mean of V, and 0 where there is no token; in every sequence and
+    in one beside others."""
+    ctx = [37, 0, 1, 64, 200, Q]
+    q, kc, vc, ks, vs, tbl, cl = _attend_inputs(Q + page, len(ctx), Q, KV, G, D, page, kind, dtype, ctx)
+    tree = _random_tree(torch.Generator().manual_seed(Q), len(ctx), Q).cuda()
+    zero = torch.zeros_like(q)
+    for t in (None, tree):
+        got = _attend_check(zero, kc, vc, ks, vs, tbl, cl, tree=t)
+        assert (got[1] == 0).all()
+    q[4] = 0
+    _attend_check(q, kc, vc, ks, vs, tbl, cl)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("page", [8, 16, 64])
+@pytest.mark.parametrize("Q,KV,G,D", [(1, 2, 4, 128), (9, 1, 4, 64)])
+@pytest.mark.parametrize("power", [-100, -40, -28, 60, 110])
+def test_attention_of_scaled_bf16_queries(cuda, power, Q, KV, G, D, page):
+    """bf16 queries times a power of two, under sm_scale times its reciprocal, give the same bits (every product
+    and sum is scaled by powers of two alone); tiny ones under the same sm_scale, the mean of V."""
+    import specq
+    q, kc, vc, ks, vs, tbl, cl = _attend_inputs(Q, 5, Q, KV, G, D, page, "int8", torch.bfloat16, [37, 1, 150, 64, Q])
+    ref = _attend_check(q, kc, vc, ks, vs, tbl, cl)
+    small = (q.float() * 2.0 ** power).bfloat16()
+    got = specq.paged_attention_blocks(small, kc, vc, ks, vs, tbl, cl, sm_scale=D ** -0.5 * 2.0 ** -power)
+    assert torch.equal(got, ref)
+    if power < 0:
+        _attend_check(small, kc, vc, ks, vs, tbl, cl)
+    assert _status() == 0
