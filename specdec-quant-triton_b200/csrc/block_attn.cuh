@@ -9,9 +9,11 @@
 //   p = 2^(x - m) = 2^(score - m) * sV,   O = sum p v8,   l = sum p / sV,   out = O / l,
 // so neither scale costs a pass over a tile: sK is a factor of the exponent's fused
 // multiply-add, sV part of its addend, and the normaliser divides by a number that is the same
-// for a whole page.  p is rounded to fp16 for the tensor core; l sums the unrounded p in fp32.
-// q is exact in fp16 (bf16 rows are first scaled by a power of two), and so are k8 and v8; the
-// products accumulate in fp32.  m lags: p may reach 2^8 before the running maximum is raised
+// for a whole page.  What a row may not see becomes -inf after that multiply-add: the factor may
+// underflow, and 0 times -inf is NaN.  p is rounded to fp16 for the tensor core; l sums the unrounded p in fp32.
+// k8 and v8 are exact in fp16, and so is q (bf16 rows are first scaled by a power of two, and keep their 8
+// bits down to 2^-17 of the row's largest element whatever the other rows hold); the products
+// accumulate in fp32.  m lags: p may reach 2^8 before the running maximum is raised
 // (one warp vote a tile), which fp16 holds without loss.
 //
 // Tile.  A tile is 128 tokens (64 up to 16 rows) of one KV head against up to 40 query rows, the work of
@@ -92,7 +94,6 @@ constexpr int kBAMaxStages = 8;
 constexpr float kBARaise = 8.f;         // log2 of how far p may pass 1 before the maximum is raised
 constexpr float kBANone = -1e30f;        // the running maximum of a row that has seen no token: finite, so that a
                                          // masked score, -inf, less it is -inf and not NaN
-constexpr float kBALeastK = 1e-37f;              // the least factor of a score that may be masked
 constexpr float kBALeastV = 8.077935669463161e-28f;   // 2^-90: a smaller V scale reads as this
 
 struct BlockAttnParams {
@@ -618,7 +619,6 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     if (first && warp < NF) copy_queries(warp, sg);
     // ---- Q^T as the B operand: thread (gq, tq) holds row gq of each group, d = 16 c + 4 tq + 0..3
     uint32_t qf[NT][KC][2];
-    float fac = 1.f;
     ok = ok && mbar_wait(&q_full[qat.s], qat.ph, p.status, SPECQ_STATUS_TIMEOUT_PIPELINE);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -632,12 +632,17 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     }
     const uint64_t* tree_rows = reinterpret_cast<const uint64_t*>(qbuf + qat.s * S::Q + S::TREE);
     if (threadIdx.x == 0) SPECQ_TRACE_POINT(9, sg.ta);
+    // bf16 to fp16: under one power of two that brings the largest finite element to [2^15, 2^16), so that a
+    // row 2^15 below it still keeps bf16's 8 bits down to 2^-17 of its own largest element (what is smaller
+    // is off by 2^-25 of it at most).  Rows further apart than that have a power each: no row costs another
+    // its bits.  (Each row its own always: D = 128, 8 x 16384, 36 rows 92 -> 98 us, D = 64 trees 38 -> 41.)
+    float fac = 1.f;
+    float* facs = sm_l + warp * ROWS;        // free until the segment's sums are written
     if (p.bf16) {
-      // to fp16 under one power of two that brings the largest finite one to [1, 2): bf16's 8 bits are
-      // exact down to 2^-17 of it, and what is smaller is off by 2^-25 of it at most
-      uint32_t top = 0;
+      uint32_t tops[NT], hi = 0u, lo = 0x7f80u;
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -647,12 +652,22 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
               const uint32_t mag = (half ? qf[n][c][i] >> 16 : qf[n][c][i]) & 0x7fffu;
               top = max(top, mag >= 0x7f80u ? 0u : mag);
             }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const uint32_t ex = min(max(top >> 7, 1u), 253u);
-      fac = __uint_as_float(ex << 23);
-      const float inv = __uint_as_float((254u - ex) << 23);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));   // the row's elements lie in four lanes
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        tops[n] = top;
+        hi = max(hi, top);
+        lo = min(lo, top == 0u ? 0x7f80u : top);                // a row of zeros goes with any
+      }
+      hi = __reduce_max_sync(0xffffffffu, hi) >> 7;             // biased exponents
+      lo = __reduce_min_sync(0xffffffffu, lo) >> 7;
+      const bool apart = hi > lo + 15u;
+      const uint32_t all = max(hi, 16u);
+      fac = apart ? 0.f : __uint_as_float((all - 15u) << 23);   // 0: look in facs
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int n = 0; n < NT; ++n) {
+        const uint32_t own = min(max(tops[n] >> 7, 1u), 253u);
+        const float inv = __uint_as_float((254u - (apart ? own : all - 15u)) << 23);
+        if (apart && tq == 0) facs[n * 8 + gq] = __uint_as_float(own << 23);
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -661,6 +676,8 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
                                                 __uint_as_float(qf[n][c][i] & 0xffff0000u) * inv);
             qf[n][c][i] = *reinterpret_cast<const uint32_t*>(&y);
           }
+      }
+      __syncwarp();
     }
     float o[MT][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
@@ -699,42 +716,52 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
     BAPlace pl = at;
     auto softmax = [&](int t) {              // of tile t, whose place is pl
       // softmax: rows 2 tq, 2 tq + 1 of each group, tokens gq and gq + 8 of each 16
-      float ck[U], lv[U], lv1[U], iv[U], iv1[U];   // 1: of tokens gq + 8
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float4 w0 = scales[pl.s * S::SC + 2 * (U * gw + u)];
-        ck[u] = w0.x;
-        lv[u] = lv1[u] = w0.y;
-        iv[u] = iv1[u] = w0.z;
-      }
-      // What the scores are multiplied by: one number for 16 tokens, in the sum with lv below.  At page 8 tokens
-      // 8 .. 15 are another page's, with its own scales, and bf16 queries bring their power of two; there the
-      // scores are multiplied here, before any of them is masked, since that number may underflow and 0 times
-      // a masked -inf is NaN (below, its floor keeps it from that: a score under it weighs as 0 does).
-      if (p.bf16 || p.page_log2 == 3) {
+      // x = score in log2 units + log2(sV); what a row may not see is masked after, since a factor that
+      // underflows times a masked -inf would be NaN
+      float iv[U], iv1[U];                   // 1: of tokens gq + 8
+      {
+        float ck[U], lv[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          float c0 = ck[u], c1 = c0;
-          if (p.page_log2 == 3) {
-            const float4 w1 = scales[pl.s * S::SC + 2 * (U * gw + u) + 1];
-            c1 = w1.x;
-            lv1[u] = w1.y;
-            iv1[u] = w1.z;
-          }
-          c0 *= fac;
-          c1 *= fac;
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              sc[u][n][r] *= c0;
-              sc[u][n][2 + r] *= c1;
-            }
-          ck[u] = 1.f;
+          const float4 w0 = scales[pl.s * S::SC + 2 * (U * gw + u)];
+          ck[u] = w0.x;
+          lv[u] = w0.y;
+          iv[u] = iv1[u] = w0.z;
         }
-      } else {
+        if (fac == 0.f || p.page_log2 == 3) {     // a factor for each row; tokens 8 .. 15 are another page's at page 8
+          float ck1[U], lv1[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) ck[u] = fmaxf(ck[u], kBALeastK);
+          for (int u = 0; u < U; ++u) {
+            ck1[u] = ck[u];
+            lv1[u] = lv[u];
+            if (p.page_log2 == 3) {
+              const float4 w1 = scales[pl.s * S::SC + 2 * (U * gw + u) + 1];
+              ck1[u] = w1.x;
+              lv1[u] = w1.y;
+              iv1[u] = w1.z;
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float2 f = fac == 0.f ? *reinterpret_cast<const float2*>(&facs[n * 8 + 2 * tq]) : make_float2(fac, fac);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              sc[u][n][0] = fmaf(sc[u][n][0], ck[u] * f.x, lv[u]);
+              sc[u][n][1] = fmaf(sc[u][n][1], ck[u] * f.y, lv[u]);
+              sc[u][n][2] = fmaf(sc[u][n][2], ck1[u] * f.x, lv1[u]);
+              sc[u][n][3] = fmaf(sc[u][n][3], ck1[u] * f.y, lv1[u]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int u = 0; u < U; ++u) ck[u] *= fac;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sc[u][n][i] = fmaf(sc[u][n][i], ck[u], lv[u]);
+        }
       }
       const int tw = t * TOK + 16 * U * gw;  // the warp's first token
       if (tw + 16 * U > sg.old) {
@@ -778,7 +805,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
           }
         }
       }
-      // x = score in log2 units + log2(sV), against the lagging m; one chain of maxima a group of rows
+      // against the lagging m; one chain of maxima a group of rows
       float tops[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -786,11 +813,7 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            sc[u][n][r] = fmaf(sc[u][n][r], ck[u], lv[u]);
-            sc[u][n][2 + r] = fmaf(sc[u][n][2 + r], ck[u], lv1[u]);
-            tops[n] = fmaxf(tops[n], fmaxf(sc[u][n][r], sc[u][n][2 + r]) - m[n][r]);
-          }
+          for (int r = 0; r < 2; ++r) tops[n] = fmaxf(tops[n], fmaxf(sc[u][n][r], sc[u][n][2 + r]) - m[n][r]);
       }
       float top = tops[0];
 #pragma unroll

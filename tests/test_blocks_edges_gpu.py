@@ -86,3 +86,22 @@ def test_attention_of_scaled_bf16_queries(cuda, power, Q, KV, G, D, page):
     if power < 0:
         _attend_check(small, kc, vc, ks, vs, tbl, cl)
     assert _status() == 0
+
+
+@pytest.mark.parametrize("Q,KV,G,D", [(1, 2, 8, 64), (5, 2, 4, 64), (9, 1, 4, 128)])
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 14, 2.0 ** 16, 2.0 ** 20, 2.0 ** 40, 1e30])
+def test_attention_of_an_outlying_row_leaves_the_others_exact(cuda, size, Q, KV, G, D):
+    """One finite, very large bf16 query row costs the others nothing: they keep the bound."""
+    q, kc, vc, ks, vs, tbl, cl = _attend_inputs(21, 3, Q, KV, G, D, 16, "e4m3", torch.bfloat16, [400, 33, 90])
+    import specq
+    big = q.clone()
+    big[0, Q // 2, 1] *= size
+    big[1, 0, 2, 5] = -size
+    got = specq.paged_attention_blocks(big, kc, vc, ks, vs, tbl, cl)
+    assert torch.isfinite(got).all()
+    keep = torch.ones(q.shape[:3], dtype=torch.bool)
+    keep[0, Q // 2, 1] = keep[1, 0, 2] = False
+    keep = keep.cuda()
+    ref = specq.paged_attention_blocks(q, kc, vc, ks, vs, tbl, cl)
+    _attend_check(q, kc, vc, ks, vs, tbl, cl, out=torch.where(keep[..., None], got, ref))
+    assert _status() == 0
