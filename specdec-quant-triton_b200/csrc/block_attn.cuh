@@ -518,9 +518,11 @@ block_attn_kernel(const __grid_constant__ BlockAttnParams p, const __grid_consta
       for (; t0 < sg.tb;) {
         const int my_tile = t0 + lt * NF, my_tok = tok;
         const bool load = my_tile < sg.tb && tok < sg.ctx;
-        const bool there = pg >= 0 && pg < p.n_pages;          // a bad page reads page 0 and weighs nothing
+        const bool there = pg >= 0 && pg < p.n_pages;
         if (load && !there) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
-        const int page = there ? pg : 0;
+        // a page that is not there weighs nothing: its box lies past the map's last page, which TMA fills with
+        // zeros (another page's bytes may be e4m3 NaN)
+        const int page = there ? pg : p.n_pages;
         float ks = 0.f, vs = 0.f;
         const int t1 = min(sg.tb, t0 + tpb * NF);
         const int tb0 = t0;

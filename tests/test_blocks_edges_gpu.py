@@ -51,6 +51,26 @@ def test_attention_steps_over_a_bad_page_of_eight(cuda, kind, dtype, Q, KV, G, D
         _attend_with_bad_pages(args, bad)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Q,KV,G,D,page", [(1, 2, 4, 128, 16), (9, 1, 4, 64, 32), (2, 2, 4, 128, 128), (3, 1, 8, 64, 8)])
+def test_attention_reads_nothing_for_a_bad_page(cuda, dtype, Q, KV, G, D, page):
+    """Page 0 belongs to no sequence and holds NaN bytes: a bad page number does not bring them in.  A sequence
+    without one good page sees nothing."""
+    ctx = [3 * page + 7 + Q, 300 + Q, page + Q]
+    q, kc, vc, ks, vs, tbl, cl = _attend_inputs(41, 3, Q, KV, G, D, page, "e4m3", dtype, ctx)
+    gen = torch.Generator().manual_seed(7)
+    tbl = (torch.randperm(kc.shape[0] - 1, generator=gen)[: tbl.numel()] + 1).to(torch.int32).view(tbl.shape).cuda()
+    for c in (kc, vc):
+        c[0].view(torch.uint8).fill_(0x7F)
+    ks[0], vs[0] = float("nan"), float("inf")
+    _attend_with_bad_pages((q, kc, vc, ks, vs, tbl, cl), [[1], [0, 2 if page < 64 else 1], [0]])
+    import specq
+    none = torch.full_like(tbl, kc.shape[0])
+    got = specq.paged_attention_blocks(q, kc, vc, ks, vs, none, cl)
+    assert (got == 0).all()
+    assert _status() != 0
+
+
 # ---- queries of any size ----------------------------------------------------------------------------
 @pytest.mark.parametrize("page", [8, 16, 32])
 @pytest.mark.parametrize("Q,KV,G,D", [(1, 2, 4, 128), (5, 1, 4, 64), (9, 2, 4, 128)])
