@@ -34,6 +34,11 @@
 // some 83 MB, 3.2 TB/s (40 warps an SM in place of 28: the same; two to eight heads a warp, the next
 // one's tokens read ahead: 31 to 46; half as many tokens in flight: 31); 8 chains of 9, one layer:
 // 3.0 us, the three loads of its chain.
+//
+// Lengths, tables, scales and numbers are written by the kernels that come before these in a stream, and under
+// programmatic launch a kernel's blocks may be resident while those still run.  They are read by plain
+// loads after the wait; the read-only path (__ldg) is for what no such kernel writes: rotary tables and
+// positions, plans, accepted indices.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -170,7 +175,7 @@ __device__ __forceinline__ void append_queries(const BlockAppendParams& p, uint3
     pos = __ldg(p.pos + t);
   } else {
     const int b = t / q_len;
-    pos = __ldg(p.ctx + b) - q_len + (t - b * q_len);
+    pos = p.ctx[b] - q_len + (t - b * q_len);
   }
   const float* row = rope_row(p.table, pos, p.n_pos, p.rot, p.status);
   const T* x = static_cast<const T*>(p.q) + t * p.qt + h0 * p.qh;
@@ -201,7 +206,7 @@ block_append_kernel(const __grid_constant__ BlockAppendParams p) {
   const int part = static_cast<int>(blockIdx.x) - bw * p.win_blocks;
   const int b = bw / p.n_win, win = bw - b * p.n_win;
   if (b >= n_seqs || q_len == 0) return;
-  const int ctx = __ldg(p.ctx + b);
+  const int ctx = p.ctx[b];
   const int base = ctx - q_len;
   if (base < 0 || ctx > p.bt_cols * page) {                 // tokens outside the table: not written
     if (threadIdx.x == 0 && win == 0 && part == 0) report_status(p.status, SPECQ_STATUS_PLAN_CLAMPED);
@@ -210,7 +215,7 @@ block_append_kernel(const __grid_constant__ BlockAppendParams p) {
   const int col = (base >> p.page_log2) + win;
   const int start = col << p.page_log2;                     // position of the page's slot 0
   if (start >= ctx) return;
-  const int pg = __ldg(p.bt + b * p.bt_sb + col);           // looked at after the rows' loads
+  const int pg = p.bt[b * p.bt_sb + col];           // looked at after the rows' loads
   const int unit = part * (kAppendWarps / wpu) + warp / wpu;
   const bool live = unit < 2 * p.h_kv;
   const bool is_v = unit >= p.h_kv;
@@ -498,7 +503,7 @@ __global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __
   const int32_t* acc = p.accept + b * p.acc_sb;
   const int a0 = lane < p.acc_cols ? __ldg(acc + lane) : 0;
   const int a1 = lane + 32 < p.acc_cols ? __ldg(acc + lane + 32) : 0;
-  const int ctx = __ldg(p.ctx + b);
+  const int ctx = p.ctx[b];
   const int n_raw = __ldg(p.n_accept + b);
   const int base = ctx - p.q_len;
   const int n = min(max(n_raw, 0), min(p.acc_cols, p.q_len));
@@ -506,7 +511,7 @@ __global__ void __launch_bounds__(kCompactThreads) block_compact_kernel(const __
   // the drafts' pages, one a lane
   const int col0 = base >> p.page_log2, n_win = ((ctx - 1) >> p.page_log2) - col0 + 1;
   int pg = 0;
-  if (in_table && lane < n_win) pg = __ldg(p.bt + b * p.bt_sb + col0 + lane);
+  if (in_table && lane < n_win) pg = p.bt[b * p.bt_sb + col0 + lane];
   // accept must grow strictly within the drafts, the drafts lie in the table on pages of the cache
   const int before0 = __shfl_up_sync(0xffffffffu, a0, 1), last0 = __shfl_sync(0xffffffffu, a0, 31);
   const int before1 = __shfl_up_sync(0xffffffffu, a1, 1);

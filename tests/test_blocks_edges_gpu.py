@@ -125,3 +125,53 @@ def test_attention_of_an_outlying_row_leaves_the_others_exact(cuda, size, Q, KV,
     ref = specq.paged_attention_blocks(q, kc, vc, ks, vs, tbl, cl)
     _attend_check(q, kc, vc, ks, vs, tbl, cl, out=torch.where(keep[..., None], got, ref))
     assert _status() == 0
+
+
+# ---- kernels on each other's heels -----------------------------------------------------------------------
+def test_chained_calls_see_each_others_writes(cuda):
+    """Reserve, append, attention and compaction in a stream, each reading what the one before it wrote (tables,
+    scales, numbers, lengths, parts), give the bits that they give with the GPU idle between them."""
+    import specq
+    B, Q, KV, G, D, page, C = 6, 9, 2, 4, 128, 16, 96
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    table = specq.rope_table(C * page, D, device="cuda")
+    steps = 12
+    rows = [torch.randn(B * Q, (KV * G + 2 * KV), D, generator=gen, device="cuda").mul(1 + 3 * (i % 4)).half() for i in range(steps)]
+    prompt = torch.randn(B * 700, 2 * KV, D, generator=gen, device="cuda").half()
+    accept = [torch.stack([torch.randperm(Q, generator=gen, device="cuda")[:4].sort().values for _ in range(B)]).int() for _ in range(steps)]
+    four = torch.full((B,), 4, dtype=torch.int32, device="cuda")
+    start = torch.full((B,), 700, dtype=torch.int32, device="cuda")
+
+    def run(idle):
+        wait = torch.cuda.synchronize if idle else (lambda: None)
+        kc, vc = (torch.zeros(B * C, page, KV, D, dtype=torch.int8, device="cuda") for _ in range(2))
+        ks, vs = (torch.ones(B * C, KV, device="cuda") for _ in range(2))
+        ref = torch.zeros(B * C, dtype=torch.int32, device="cuda")
+        tbl = torch.full((B, C), -1, dtype=torch.int32, device="cuda")
+        held = torch.zeros(B, dtype=torch.int32, device="cuda")
+        lens = [start] + [torch.empty_like(start) for _ in range(steps)]
+        drafts = [torch.empty_like(start) for _ in range(steps)]
+        outs = []
+        specq.pages_reserve(ref, tbl, held, start, page)
+        specq.kv_append_blocks(prompt[:, :KV], prompt[:, KV:], kc, vc, ks, vs, tbl, start, 700, table=table)
+        wait()
+        for i in range(steps):
+            torch.add(lens[i], Q, out=drafts[i])
+            wait()
+            specq.pages_reserve(ref, tbl, held, drafts[i], page)
+            wait()
+            q, k, v = rows[i].split([KV * G, KV, KV], 1)
+            q = specq.kv_append_blocks(k, v, kc, vc, ks, vs, tbl, drafts[i], Q, q=q, table=table)
+            wait()
+            outs.append(specq.paged_attention_blocks(q, kc, vc, ks, vs, tbl, drafts[i], q_len=Q))
+            wait()
+            specq.kv_compact_blocks(kc, vc, ks, vs, tbl, drafts[i], Q, accept[i], four, ctx_out=lens[i + 1])
+            wait()
+            outs.append(specq.paged_attention_blocks(q, kc, vc, ks, vs, tbl, lens[i + 1], q_len=Q))
+            wait()
+        torch.cuda.synchronize()
+        return outs + lens + [kc, vc, ks, vs, tbl, held, ref]
+    want = run(True)
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(run(False), want))
+    assert _status() == 0
