@@ -327,6 +327,7 @@ int specq_block_append(const void* k, int64_t kt, int64_t kh, const void* v, int
 
 /* Attention of the q_len newest tokens of each sequence over the block-scaled cache.
  *   q, out   fp16 or bf16 (dtype) [B, q_len, H, D] with strides; q_sb = 0 (o_sb = 0): packed rows
+ *            [n_seqs * q_len, H, D] (so a batch cannot be broadcast from one sequence's rows)
  *   tree     optional uint64 [B, q_len] (strides tree_sb, tree_st): row qi sees draft token j when
  *            bit j is set (and every token before the drafts); null: the causal window of
  *            specq_paged_attention.  q_len <= 64 with a tree.

@@ -301,6 +301,9 @@ PyObject* paged_attention_blocks(PyObject* const* a) {
     BAD_VALUE("%s: n_seqs=%d of %d, q_len=%d of %d, q %s", who, n_seqs, B, q_len, ql_max, shape(q).c_str());
   if (packed && q.size(0) < (plan != nullptr ? static_cast<int64_t>(B) * ql_max : static_cast<int64_t>(n_seqs) * q_len))
     BAD_VALUE("%s: %lld packed rows for %d sequences of %d tokens", who, (long long)q.size(0), B, ql_max);
+  // to the kernels a batch stride of 0 says packed rows
+  if (!packed && q.stride(0) == 0 && (plan != nullptr ? B : n_seqs) > 1)
+    BAD_VALUE("%s: q is expanded over the sequences (its stride is 0); give each sequence its rows", who);
   const int64_t H = q.size(-2);
   if (q.size(-1) != c.D || c.H == 0 || H % c.H)
     BAD_VALUE("%s: q heads (%lld, %lld) do not fit the cache's (%lld, %lld)", who, (long long)H, (long long)q.size(-1), (long long)c.H,
