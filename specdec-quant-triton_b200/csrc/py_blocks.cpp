@@ -108,6 +108,12 @@ void rows3(const char* who, const char* what, const Tensor& t, bool with_f32) {
     BAD_VALUE("%s: %s must be [rows, heads, dim] with unit inner stride, got %s", who, what, shape(t).c_str());
 }
 
+// A tensor that a kernel writes: no two of its elements share memory by a stride of 0.
+void written(const char* who, const char* what, const Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.stride(i) == 0 && t.size(i) > 1) BAD_VALUE("%s: %s is written and must not be expanded (dimension %lld)", who, what, (long long)i);
+}
+
 // int32, `dims` dimensions, at least n0 (and n1) long (-1: any), unit inner stride
 void int32s(const char* who, const char* what, const Tensor& t, int dims, int64_t n0, int64_t n1 = -1) {
   if (t.scalar_type() != at::kInt) BAD_TYPE("%s: %s must be int32, got %s", who, what, dtype(t));
@@ -124,7 +130,7 @@ struct Cache {
   int64_t s_sl() const { return d ? ks.stride(0) : 0; }
 };
 
-Cache cache(const char* who, PyObject* const* a, bool layers) {
+Cache cache(const char* who, PyObject* const* a, bool layers, bool writes = true) {
   const Tensor &kc = tensor(who, "kc", a[0]), &vc = tensor(who, "vc", a[1]), &ks = tensor(who, "ks", a[2]), &vs = tensor(who, "vs", a[3]);
   if ((kc.scalar_type() != at::kChar && kc.scalar_type() != at::kFloat8_e4m3fn) || vc.scalar_type() != kc.scalar_type())
     BAD_TYPE("%s: kc and vc must both be int8 or both float8_e4m3fn, got %s and %s", who, dtype(kc), dtype(vc));
@@ -138,6 +144,10 @@ Cache cache(const char* who, PyObject* const* a, bool layers) {
   if (!ok || ks.size(d + 1) != kc.size(d + 2))
     BAD_VALUE("%s: ks and vs must be alike, one scale for each page and head of %s, got %s and %s", who, shape(kc).c_str(),
               shape(ks).c_str(), shape(vs).c_str());
+  if (writes) {              // vc and vs are alike
+    written(who, "the cache", kc);
+    written(who, "the cache's scales", ks);
+  }
   return Cache{kc, vc, ks, vs, d, d ? kc.size(0) : 1, kc.size(d), kc.size(d + 1), kc.size(d + 2), kc.size(d + 3)};
 }
 
@@ -209,6 +219,7 @@ PyObject* rope(PyObject* const* a) {
     rows3(who, "out", *given, true);
     if (given->scalar_type() != x.scalar_type() || given->sizes() != x.sizes())
       BAD_VALUE("rope: out must be %s %s, got %s %s", dtype(x), shape(x).c_str(), dtype(*given), shape(*given).c_str());
+    written(who, "out", *given);
   }
   same_device(who, {&x, &pos, &table, given, plan});
   const Tensor out = given != nullptr ? *given : at::empty(x.sizes(), x.options());
@@ -256,6 +267,7 @@ PyObject* kv_append_blocks(PyObject* const* a) {
       rows3(who, "q_out", *q_given, false);
       if (q_given->scalar_type() != q->scalar_type() || q_given->sizes() != q->sizes())
         BAD_VALUE("%s: q_out must be %s %s", who, dtype(*q), shape(*q).c_str());
+      written(who, "q_out", *q_given);
     }
   } else if (q_given != nullptr) {
     BAD_VALUE("%s: q_out without q", who);
@@ -278,7 +290,7 @@ PyObject* kv_append_blocks(PyObject* const* a) {
 PyObject* paged_attention_blocks(PyObject* const* a) {
   // q, kc, vc, ks, vs, block_tbl, ctx_len, q_len, tree, sm_scale, out, plan, n_seqs, ql_max
   const char* who = "paged_attention_blocks";
-  const Cache c = cache(who, a + 1, false);
+  const Cache c = cache(who, a + 1, false, false);
   const Tensor& q = tensor(who, "q", a[0]);
   if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16)
     BAD_TYPE("%s: q must be float16 or bfloat16, got %s", who, dtype(q));
@@ -311,6 +323,7 @@ PyObject* paged_attention_blocks(PyObject* const* a) {
   const Tensor *given = optional(who, "out", a[10]), *tree = optional(who, "tree", a[8]);
   if (given != nullptr && (given->scalar_type() != q.scalar_type() || given->sizes() != q.sizes()))
     BAD_VALUE("%s: out must be %s %s, got %s %s", who, dtype(q), shape(q).c_str(), dtype(*given), shape(*given).c_str());
+  if (given != nullptr) written(who, "out", *given);
   if (q.stride(-1) != 1 || (given != nullptr && given->stride(-1) != 1)) BAD_VALUE("%s: q and out need unit stride along D", who);
   float sm = 1.f / std::sqrt(static_cast<float>(c.D));
   if (a[9] != Py_None) {

@@ -35,3 +35,34 @@ def test_queries_expanded_over_the_sequences_are_refused():
         specq.paged_attention_blocks(q, *cache, tbl, ctx, n_seqs=1)
     with pytest.raises(ValueError, match="CUDA"):
         specq.paged_attention_blocks(one[0, :1].expand(6, -1, -1), *cache, tbl, ctx, q_len=2)
+
+
+def test_written_tensors_whose_elements_share_memory_are_refused():
+    kc, vc, ks, vs = cache = _cache()
+    k = torch.zeros(4, 2, 64, dtype=torch.float16)
+    q = torch.zeros(2, 2, 4, 64, dtype=torch.float16)
+    tbl, ctx = _i32(2, 3), _i32(2)
+    table = specq.rope_table(8, 64, device="cpu")
+    with pytest.raises(ValueError, match="out .*expanded"):
+        specq.rope(k, _i32(4), table, out=k[:1].expand(4, -1, -1))
+    with pytest.raises(ValueError, match="out .*expanded"):
+        specq.rope(k, _i32(4), table, out=k[:, :1].expand(-1, 2, -1))
+    with pytest.raises(ValueError, match="q_out .*expanded"):
+        specq.kv_append_blocks(k, k, *cache, tbl, ctx, 2, q=k, q_out=k[:1].expand(4, -1, -1), table=table)
+    for dim in range(3):
+        shape = [2, 2, 4, 64]
+        shape[dim] = 1
+        with pytest.raises(ValueError, match="out .*expanded"):
+            specq.paged_attention_blocks(q, *cache, tbl, ctx, out=torch.zeros(shape, dtype=torch.float16).expand(2, 2, 4, 64))
+    wide = [t[:1].expand_as(t) for t in cache]
+    pool = _i32(6), tbl, _i32(2)
+    for bad in ((wide[0], wide[1], ks, vs), (kc, vc, wide[2], wide[3]), (kc, vc, ks[:, :1].expand(6, 2), vs[:, :1].expand(6, 2))):
+        with pytest.raises(ValueError, match="expanded"):
+            specq.kv_append_blocks(k, k, *bad, tbl, ctx, 2)
+        with pytest.raises(ValueError, match="expanded"):
+            specq.kv_compact_blocks(*bad, tbl, ctx, 2, _i32(2, 2), _i32(2))
+        with pytest.raises(ValueError, match="expanded"):
+            specq.pages_fork(*bad, *pool, _i32(2), _i32(2))
+    # attention only reads the scales: one for all pages is fine
+    with pytest.raises(ValueError, match="CUDA"):
+        specq.paged_attention_blocks(q, kc, vc, wide[2], wide[3], tbl, ctx)
