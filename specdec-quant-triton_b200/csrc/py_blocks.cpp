@@ -173,9 +173,11 @@ void rotary_table(const char* who, const Tensor& t, int64_t D) {
     BAD_VALUE("%s: table %s needs positions and an even rot <= %lld", who, shape(t).c_str(), static_cast<long long>(D));
 }
 
-const int32_t* plan_of(const char* who, const Tensor* plan) {
+// A plan whose first n values the kernels read.
+const int32_t* plan_of(const char* who, const Tensor* plan, int n) {
   if (plan == nullptr) return nullptr;
   if (plan->scalar_type() != at::kInt) BAD_TYPE("%s: plan must be int32, got %s", who, dtype(*plan));
+  if (plan->numel() < n || !plan->is_contiguous()) BAD_VALUE("%s: plan must be contiguous, %d values or more, got %s", who, n, shape(*plan).c_str());
   return static_cast<const int32_t*>(plan->data_ptr());
 }
 
@@ -215,6 +217,7 @@ PyObject* rope(PyObject* const* a) {
   if (inverse < 0) throw Raised{};
   const Tensor* given = optional(who, "out", a[5]);
   const Tensor* plan = optional(who, "plan", a[6]);
+  const int32_t* plan_at = plan_of(who, plan, 1);
   if (given != nullptr) {
     rows3(who, "out", *given, true);
     if (given->scalar_type() != x.scalar_type() || given->sizes() != x.sizes())
@@ -225,7 +228,7 @@ PyObject* rope(PyObject* const* a) {
   const Tensor out = given != nullptr ? *given : at::empty(x.sizes(), x.options());
   check(lib.rope(x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), row_code(x), ptr<int32_t>(pos),
                  ptr<float>(table), size32(who, table.size(0)), size32(who, x.size(0)), size32(who, x.size(1)), size32(who, x.size(2)),
-                 size32(who, table.size(1)), lay, inverse, plan_of(who, plan), stream()));
+                 size32(who, table.size(1)), lay, inverse, plan_at, stream()));
   return wrap(out);
 }
 
@@ -245,6 +248,7 @@ PyObject* kv_append_blocks(PyObject* const* a) {
   if (n_seqs < 0 || n_seqs > B || q_len < 0 || q_len > ql_max)
     BAD_VALUE("%s: n_seqs=%d of %d, q_len=%d of %d", who, n_seqs, B, q_len, ql_max);
   const Tensor* plan = optional(who, "plan", a[14]);
+  const int32_t* plan_at = plan_of(who, plan, 2);
   const int64_t need = plan != nullptr ? static_cast<int64_t>(B) * ql_max : static_cast<int64_t>(n_seqs) * q_len;
   auto kv = [&](const char* what, const Tensor& t) {
     if (t.scalar_type() != k.scalar_type() || t.size(1) != c.H || t.size(2) != c.D || t.size(0) < need)
@@ -282,7 +286,7 @@ PyObject* kv_append_blocks(PyObject* const* a) {
       qs ? q_out.stride(1) : 0, row_code(k), ptr<float>(table), table ? size32(who, table->size(0)) : 0,
       table ? size32(who, table->size(1)) : 0, lay, ptr<int32_t>(pos), c.kc.data_ptr(), c.vc.data_ptr(), c.kc.stride(0),
       c.kc.stride(1), c.kc.stride(2), cache_code(c.kc), size32(who, c.P), ptr<float>(c.ks), ptr<float>(c.vs), c.ks.stride(0),
-      c.ks.stride(1), ptr<int32_t>(tbl), tbl.stride(0), size32(who, tbl.size(1)), ptr<int32_t>(ctx), plan_of(who, plan), B, n_seqs,
+      c.ks.stride(1), ptr<int32_t>(tbl), tbl.stride(0), size32(who, tbl.size(1)), ptr<int32_t>(ctx), plan_at, B, n_seqs,
       q_len, ql_max, qs ? size32(who, q->size(1)) : 0, size32(who, c.H), size32(who, c.D), size32(who, c.page), stream()));
   return qs ? wrap(q_out) : none();
 }
@@ -304,6 +308,7 @@ PyObject* paged_attention_blocks(PyObject* const* a) {
     BAD_VALUE("%s: q must have 3 or 4 dimensions, got %s", who, shape(q).c_str());
   }
   const Tensor* plan = optional(who, "plan", a[11]);
+  const int32_t* plan_at = plan_of(who, plan, 2);
   const int q_len = packed ? integer(a[7]) : integer_or(a[7], size32(who, q.size(1)));
   if (!packed && (q.size(0) < B || q.size(1) < q_len))
     BAD_VALUE("%s: q is %s for %d sequences of %d tokens", who, shape(q).c_str(), B, q_len);
@@ -352,7 +357,7 @@ PyObject* paged_attention_blocks(PyObject* const* a) {
       c.kc.stride(1), c.kc.stride(2), cache_code(c.kc), size32(who, c.P), ptr<float>(c.ks), ptr<float>(c.vs), c.ks.stride(0), c.ks.stride(1),
       ptr<int32_t>(tbl), tbl.stride(0), cols, ptr<int32_t>(ctx), tree ? reinterpret_cast<const uint64_t*>(tree->data_ptr()) : nullptr,
       tree ? tree->stride(0) : 0, tree ? tree->stride(1) : 0, sm, out.data_ptr(), packed ? 0 : out.stride(0), out.stride(o),
-      out.stride(o + 1), plan_of(who, plan), B, n_seqs, q_len, ql_max, h, hk, D, page, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream()));
+      out.stride(o + 1), plan_at, B, n_seqs, q_len, ql_max, h, hk, D, page, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream()));
   return wrap(out);
 }
 

@@ -66,3 +66,23 @@ def test_written_tensors_whose_elements_share_memory_are_refused():
     # attention only reads the scales: one for all pages is fine
     with pytest.raises(ValueError, match="CUDA"):
         specq.paged_attention_blocks(q, kc, vc, wide[2], wide[3], tbl, ctx)
+
+
+def test_plans_that_are_too_short_are_refused():
+    """rope reads plan[0], append and attention plan[0] and plan[1]."""
+    cache = _cache()
+    k = torch.zeros(4, 2, 64, dtype=torch.float16)
+    tbl, ctx = _i32(2, 3), _i32(2)
+    table = specq.rope_table(8, 64, device="cpu")
+    for plan in (_i32(0), _i32(1), _i32(8)[::4], _i32(3, 2)[:, 0]):
+        with pytest.raises(ValueError, match="plan"):
+            specq.kv_append_blocks(k, k, *cache, tbl, ctx, 2, plan=plan)
+        with pytest.raises(ValueError, match="plan"):
+            specq.paged_attention_blocks(k, *cache, tbl, ctx, q_len=2, plan=plan)
+    with pytest.raises(ValueError, match="plan"):
+        specq.rope(k, _i32(4), table, plan=_i32(0))
+    for plan in (_i32(2), _i32(3), _i32(1, 2).t()):
+        with pytest.raises(ValueError, match="CUDA"):
+            specq.kv_append_blocks(k, k, *cache, tbl, ctx, 2, plan=plan)
+    with pytest.raises(ValueError, match="CUDA"):
+        specq.rope(k, _i32(4), table, plan=_i32(1))
