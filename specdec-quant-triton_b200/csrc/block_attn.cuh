@@ -176,7 +176,7 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   }
 }
 
-// qi of query row rr = qi * group + g (rr * group < 2^32)
+// qi of query row rr = qi * group + g (rr * group < 2^32: check_block_attn_sizes)
 __device__ __forceinline__ int ba_token(const BlockAttnParams& p, int rr) {
   return p.group == 1 ? rr : static_cast<int>(__umulhi(static_cast<uint32_t>(rr), p.group_magic));
 }
@@ -1213,7 +1213,9 @@ inline int check_block_attn_sizes(int B, int n_seqs, int q_len, int ql_max, int 
   if (!page_ok(page)) return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: page %d (a power of two in 8..128)", page);
   if (!plan && (n_seqs > B || q_len > ql_max))
     return fail(SPECQ_ERR_INVALID_ARG, "block_attention: n_seqs/q_len exceed the grid");
-  if (static_cast<int64_t>(bt_cols) * page > 0x7FFFFF00ll || static_cast<int64_t>(ql_max) * H > (1 << 24))
+  const int64_t group = H / H_KV, rows = static_cast<int64_t>(ql_max) * group;
+  if (static_cast<int64_t>(bt_cols) * page > 0x7FFFFF00ll || static_cast<int64_t>(ql_max) * H > (1 << 24) ||
+      (rows + 8 * kBAMaxGroups) * group > 0x100000000ll)   // ba_token's product, a chunk's padding rows included
     return fail(SPECQ_ERR_UNSUPPORTED, "block_attention: %d columns of %d tokens, %d x %d query rows", bt_cols, page, ql_max, H);
   return SPECQ_OK;
 }

@@ -2,10 +2,12 @@
 rotary tables at the ends of their rules.  (Tensors on the CPU are refused last, with "CUDA" in the message, so a
 refusal that names something else comes from the arguments.)"""
 
+import numpy as np
 import pytest
 import torch
 
 import specq
+from specq import _lib
 
 
 def _cache(P=6, page=16, KV=2, D=64, dtype=torch.int8):
@@ -86,3 +88,23 @@ def test_plans_that_are_too_short_are_refused():
             specq.kv_append_blocks(k, k, *cache, tbl, ctx, 2, plan=plan)
     with pytest.raises(ValueError, match="CUDA"):
         specq.rope(k, _i32(4), table, plan=_i32(1))
+
+
+def test_query_groups_that_the_row_arithmetic_cannot_hold_are_refused():
+    """A row's token is a product by ceil(2^32 / group), exact while rows * group <= 2^32: a group of 279 heads
+    goes wrong before the limit of 2^24 query rows does."""
+    group, rows = 279, (1 << 24) // 279 * 279
+    magic = 0xFFFFFFFF // group + 1
+    assert ((rows - 1) * magic) >> 32 != (rows - 1) // group
+    lib = _lib.load()
+    n = _lib.C.c_int64()
+
+    def size(q_len, H, H_KV):
+        return lib.specq_block_attention_workspace(1, 1, q_len, q_len, H, H_KV, 128, 16, 0, 0, n)
+    assert size(60000, 279, 1) == _lib.SPECQ_ERR_UNSUPPORTED
+    assert size(1 << 15, 512, 1) == _lib.SPECQ_ERR_UNSUPPORTED
+    # the largest that are taken: exact for every row (and for the padding of a block)
+    for g in (2, 3, 7, 255, 256, 279, 300, 1000):
+        most = min((1 << 24) // g, (1 << 32) // (g * g) - 1) * g
+        r = np.arange(max(0, most - (1 << 16)), most, dtype=np.uint64)
+        assert ((r * np.uint64(0xFFFFFFFF // g + 1)) >> np.uint64(32) == r // np.uint64(g)).all()
