@@ -41,7 +41,8 @@ def rope_table(n_pos, rot, base=10000.0, scaling=None, device="cuda"):
           pairs that turn fewer than `low` times in n positions are divided by f, those that turn
           more than `high` times are kept, those between are blended
       {"type": "yarn", "factor": f, "original": n, "slow": 1.0, "fast": 32.0, "attention": None}
-          the same with a ramp over the pair index, and cosines and sines times `attention`
+          the same with a ramp over the pair index (its ends rounded outwards, the upper one no further
+          than rot - 1: past the last pair the ramp is cut short), and cosines and sines times `attention`
           (default 0.1 ln f + 1)"""
     if rot < 2 or rot % 2 or n_pos < 1:
         raise ValueError(f"rope_table: n_pos={n_pos} rot={rot} (rot even, both positive)")
@@ -70,7 +71,7 @@ def rope_table(n_pos, rot, base=10000.0, scaling=None, device="cuda"):
 
         def pair_of(turns):   # the pair that turns so many times in n positions
             return rot * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
-        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot // 2 - 1)
+        lo, hi = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot - 1)
         ramp = ((torch.arange(rot // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         inv = inv * (1 - ramp) + inv / f * ramp
         gain = scaling.get("attention")

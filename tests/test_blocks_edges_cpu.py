@@ -1,6 +1,7 @@
 """The block-scaled cache's operators without a GPU: what else is refused before anything is launched, and the
 rotary tables at the ends of their rules.  (Tensors on the CPU are refused last, with "CUDA" in the message, so a
 refusal that names something else comes from the arguments.)"""
+import math
 
 import numpy as np
 import pytest
@@ -108,3 +109,30 @@ def test_query_groups_that_the_row_arithmetic_cannot_hold_are_refused():
         most = min((1 << 24) // g, (1 << 32) // (g * g) - 1) * g
         r = np.arange(max(0, most - (1 << 16)), most, dtype=np.uint64)
         assert ((r * np.uint64(0xFFFFFFFF // g + 1)) >> np.uint64(32) == r // np.uint64(g)).all()
+
+
+def _yarn(n, rot, base, factor, original, fast=32.0, slow=1.0):
+    """Angles a position from the method's definition, in 64 bits: the ramp runs over the pair index between the
+    pairs that turn `fast` and `slow` times in `original` positions, its ends rounded outwards and kept within
+    0 .. rot - 1."""
+    def pair(turns):
+        return rot * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+    lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
+    i = np.arange(rot // 2)
+    inv = base ** (-2.0 * i / rot)
+    ramp = np.clip((i - lo) / max(hi - lo, 1e-3), 0, 1)
+    return inv * (1 - ramp) + inv / factor * ramp
+
+
+@pytest.mark.parametrize("base", [10000.0, 500000.0])
+@pytest.mark.parametrize("rot", [32, 64, 128])
+@pytest.mark.parametrize("original", [2048, 4096, 32768, 65536, 131072, 1 << 20])
+def test_yarn_tables_at_any_original_length(original, rot, base):
+    """Table entries are fp32 roundings of 64-bit cosines: 2^-24 of the gain, and the angle's own 64-bit error."""
+    factor, n = 4.0, 300
+    t = specq.rope_table(n, rot, base=base, device="cpu", scaling={"type": "yarn", "factor": factor, "original": original})
+    ang = np.arange(n)[:, None] * _yarn(n, rot, base, factor, original)
+    gain = 0.1 * math.log(factor) + 1.0
+    t = t.double().numpy()
+    assert np.abs(t[:, : rot // 2] - np.cos(ang) * gain).max() <= 2.0 ** -23
+    assert np.abs(t[:, rot // 2:] - np.sin(ang) * gain).max() <= 2.0 ** -23
