@@ -43,7 +43,7 @@ def rope_table(n_pos, rot, base=10000.0, scaling=None, device="cuda"):
       {"type": "yarn", "factor": f, "original": n, "slow": 1.0, "fast": 32.0, "attention": None}
           the same with a ramp over the pair index (its ends rounded outwards, the upper one no further
           than rot - 1: past the last pair the ramp is cut short), and cosines and sines times `attention`
-          (default 0.1 ln f + 1)"""
+          (default 0.1 ln f + 1, and 1 where f <= 1)"""
     if rot < 2 or rot % 2 or n_pos < 1:
         raise ValueError(f"rope_table: n_pos={n_pos} rot={rot} (rot even, both positive)")
     i = torch.arange(0, rot, 2, dtype=torch.float64)
@@ -75,7 +75,7 @@ def rope_table(n_pos, rot, base=10000.0, scaling=None, device="cuda"):
         ramp = ((torch.arange(rot // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
         inv = inv * (1 - ramp) + inv / f * ramp
         gain = scaling.get("attention")
-        gain = 0.1 * math.log(f) + 1.0 if gain is None else float(gain)
+        gain = 0.1 * math.log(max(f, 1.0)) + 1.0 if gain is None else float(gain)
     elif kind not in (None, "ntk"):
         raise ValueError(f"rope_table: scaling type {kind!r}")
     ang = torch.arange(n_pos, dtype=torch.float64, device=device)[:, None] * inv.to(device)

@@ -136,3 +136,14 @@ def test_yarn_tables_at_any_original_length(original, rot, base):
     t = t.double().numpy()
     assert np.abs(t[:, : rot // 2] - np.cos(ang) * gain).max() <= 2.0 ** -23
     assert np.abs(t[:, rot // 2:] - np.sin(ang) * gain).max() <= 2.0 ** -23
+
+
+def test_yarn_gain_is_one_where_nothing_is_stretched():
+    """The default attention factor is 0.1 ln(factor) + 1 above a factor of 1, and 1 up to it."""
+    for factor in (0.25, 0.5, 1.0):
+        t = specq.rope_table(4, 32, device="cpu", scaling={"type": "yarn", "factor": factor, "original": 4096})
+        assert (t[0, :16] == 1.0).all()
+    t = specq.rope_table(4, 32, device="cpu", scaling={"type": "yarn", "factor": 0.5, "original": 4096, "attention": 0.75})
+    assert (t[0, :16] == 0.75).all()
+    t = specq.rope_table(4, 32, device="cpu", scaling={"type": "yarn", "factor": 2.0, "original": 4096})
+    assert abs(t[0, 0].item() - (0.1 * math.log(2.0) + 1.0)) <= 2.0 ** -23
