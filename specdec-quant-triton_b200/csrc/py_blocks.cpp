@@ -200,6 +200,9 @@ void check(int rc) {
   throw Raised{};
 }
 
+// A new output like x; rows that the call does not reach (all = false) are zeros.
+Tensor new_rows(const Tensor& x, bool all) { return all ? at::empty(x.sizes(), x.options()) : at::zeros(x.sizes(), x.options()); }
+
 Tensor new_int32(const Tensor& like, int64_t n) { return at::empty({n}, like.options().dtype(at::kInt)); }
 
 PyObject* wrap(const Tensor& t) { return THPVariable_Wrap(t); }
@@ -225,7 +228,7 @@ PyObject* rope(PyObject* const* a) {
     written(who, "out", *given);
   }
   same_device(who, {&x, &pos, &table, given, plan});
-  const Tensor out = given != nullptr ? *given : at::empty(x.sizes(), x.options());
+  const Tensor out = given != nullptr ? *given : new_rows(x, plan == nullptr);
   check(lib.rope(x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), row_code(x), ptr<int32_t>(pos),
                  ptr<float>(table), size32(who, table.size(0)), size32(who, x.size(0)), size32(who, x.size(1)), size32(who, x.size(2)),
                  size32(who, table.size(1)), lay, inverse, plan_at, stream()));
@@ -278,7 +281,7 @@ PyObject* kv_append_blocks(PyObject* const* a) {
   }
   same_device(who, {&c.kc, &c.vc, &c.ks, &c.vs, &k, &v, q, q_given, table, pos, &tbl, &ctx, plan});
   Tensor q_out;
-  if (q != nullptr) q_out = q_given != nullptr ? *q_given : at::empty(q->sizes(), q->options());
+  if (q != nullptr) q_out = q_given != nullptr ? *q_given : new_rows(*q, plan == nullptr && q->size(0) == need);
   const bool qs = q != nullptr;
   check(lib.block_append(
       k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), qs ? q->data_ptr() : nullptr,
@@ -340,11 +343,9 @@ PyObject* paged_attention_blocks(PyObject* const* a) {
   if (tree != nullptr && (tree->scalar_type() != at::kLong || tree->dim() != 2 || tree->size(0) < B || tree->size(1) < ql_max))
     BAD_VALUE("%s: tree must be int64 [>= %d, >= %d], got %s %s", who, B, ql_max, dtype(*tree), shape(*tree).c_str());
   same_device(who, {&c.kc, &c.vc, &c.ks, &c.vs, &q, given, &tbl, &ctx, tree, plan});
-  // rows that the call does not reach are zeros in a new output
-  const Tensor out = given != nullptr ? *given
-                     : plan == nullptr && n_seqs == B && (packed ? q.size(0) == static_cast<int64_t>(B) * q_len : q.size(0) == B && q.size(1) == q_len)
-                         ? at::empty(q.sizes(), q.options())
-                         : at::zeros(q.sizes(), q.options());
+  const bool all = plan == nullptr && n_seqs == B &&
+                   (packed ? q.size(0) == static_cast<int64_t>(B) * q_len : q.size(0) == B && q.size(1) == q_len);
+  const Tensor out = given != nullptr ? *given : new_rows(q, all);
   int64_t bytes = 0;
   const int cols = size32(who, tbl.size(1)), h = size32(who, H), hk = size32(who, c.H), D = size32(who, c.D), page = size32(who, c.page);
   check(lib.block_attention_workspace(B, n_seqs, q_len, ql_max, h, hk, D, page, cols, plan != nullptr, &bytes));

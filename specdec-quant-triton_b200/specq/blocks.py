@@ -85,7 +85,8 @@ def rope_table(n_pos, rot, base=10000.0, scaling=None, device="cuda"):
 def rope(x, pos, table, layout="half", inverse=False, out=None, plan=None):
     """Turn the first rot = table.shape[1] elements of every head of x [T, H, D] (float16, bfloat16 or
     float32; any row and head strides) to positions pos [T] int32; `out` may be x.  inverse=True
-    turns back, which is the gradient of the rotation.  With `plan`, only rows < plan[0]."""
+    turns back, which is the gradient of the rotation.  With `plan`, only rows < plan[0]: the others of a
+    new output are 0, those of `out` keep what they hold."""
     return _native.rope(x, pos, table, layout, inverse, out, plan)
 
 
@@ -96,7 +97,8 @@ def kv_append_blocks(k, v, kc, vc, ks, vs, block_tbl, ctx_len, q_len, q=None, q_
                      layout="half", plan=None, n_seqs=None, ql_max=None):
     """Write the K and V [T, H_KV, D] of the q_len newest tokens of each sequence (row b * q_len + t,
     position ctx_len[b] - q_len + t) into the cache, K turned by `table` when one is given, and return
-    the same tokens' queries q [T, H, D] turned (q_out, which may be q; a new tensor by default).
+    the same tokens' queries q [T, H, D] turned (q_out, which may be q; a new tensor by default, 0 in rows
+    that the call does not reach).
 
     A page's scale grows when a new token needs it, and the page's older tokens are requantised.
     `pos` [T] int32: rotary positions other than the tokens' places (a draft tree's depths).  With
@@ -112,8 +114,9 @@ def paged_attention_blocks(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len=None, tr
     q: [B, q_len, H, D], or packed rows [T, H, D] (sequence b's token t at row b * q_len + t; give
     q_len), float16 or bfloat16.  Row qi sees tokens t <= ctx_len[b] - q_len + qi, or, with `tree`
     (int64 [B, q_len] bit sets, q_len <= 64), every token before the drafts and draft j where bit j of
-    tree[b, qi] is set.  A row that sees nothing is 0.  With `plan`, plan[0] sequences of plan[1]
-    tokens are active, ql_max is the most tokens and packed rows follow the active q_len."""
+    tree[b, qi] is set.  A row that sees nothing is 0, and so is one of a new output that the call does
+    not reach.  With `plan`, plan[0] sequences of plan[1] tokens are active, ql_max is the most tokens
+    and packed rows follow the active q_len."""
     return _native.paged_attention_blocks(q, kc, vc, ks, vs, block_tbl, ctx_len, q_len, tree, sm_scale, out, plan, n_seqs,
                                           ql_max)
 

@@ -175,3 +175,34 @@ def test_chained_calls_see_each_others_writes(cuda):
     for _ in range(4):
         assert all(torch.equal(a, b) for a, b in zip(run(False), want))
     assert _status() == 0
+
+
+# ---- rows that a call does not reach ----------------------------------------------------------------------
+def test_new_outputs_are_zero_where_a_call_does_not_reach(cuda):
+    """Queries turned by an append of fewer sequences, or under a plan, and rows past a plan's in rope."""
+    import specq
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    B, Q, KV, H, D, page = 4, 9, 2, 8, 128, 16
+    k, v = (torch.randn(B * Q, KV, D, generator=gen, device="cuda").half() for _ in range(2))
+    q = torch.randn(B * Q + 3, H, D, generator=gen, device="cuda").half()
+    kc, vc = (torch.zeros(B, page, KV, D, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.ones(B, KV, device="cuda") for _ in range(2))
+    tbl = torch.arange(B, dtype=torch.int32, device="cuda")[:, None]
+    ctx = torch.full((B,), Q, dtype=torch.int32, device="cuda")
+    table = specq.rope_table(64, D, device="cuda")
+    pos = torch.arange(B * Q + 3, dtype=torch.int32, device="cuda") % 64
+
+    def poison():
+        junk = [torch.full((B * Q + 3, H, D), float("nan"), dtype=torch.half, device="cuda") for _ in range(4)]
+        torch.cuda.synchronize()
+        del junk
+    for kw, n in ((dict(n_seqs=2), 2 * Q), (dict(), B * Q), (dict(n_seqs=0), 0),
+                  (dict(plan=torch.tensor([3, 5], dtype=torch.int32, device="cuda")), 15)):
+        poison()
+        out = specq.kv_append_blocks(k, v, kc, vc, ks, vs, tbl, ctx, Q, q=q, table=table, **kw)
+        assert out.shape == q.shape and (out[n:] == 0).all() and torch.isfinite(out).all()
+    for n in (0, 5, B * Q + 3):
+        poison()
+        out = specq.rope(q, pos, table, plan=torch.tensor([n], dtype=torch.int32, device="cuda"))
+        assert (out[n:] == 0).all() and torch.equal(out[:n], specq.rope(q, pos, table)[:n])
+    assert _status() == 0
