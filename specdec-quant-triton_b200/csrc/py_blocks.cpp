@@ -11,6 +11,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -226,6 +227,11 @@ PyObject* rope(PyObject* const* a) {
     if (given->scalar_type() != x.scalar_type() || given->sizes() != x.sizes())
       BAD_VALUE("rope: out must be %s %s, got %s %s", dtype(x), shape(x).c_str(), dtype(*given), shape(*given).c_str());
     written(who, "out", *given);
+  }
+  if (c10::GradMode::is_enabled()) {
+    if (given != nullptr && (x.requires_grad() || given->requires_grad())) BAD_VALUE("rope: no out for a tensor that requires grad");
+    if (table.requires_grad()) BAD_VALUE("rope: the table has no gradient");
+    if (x.requires_grad()) Py_RETURN_NOTIMPLEMENTED;   // specq/blocks.py records the gradient and calls again
   }
   same_device(who, {&x, &pos, &table, given, plan});
   const Tensor out = given != nullptr ? *given : new_rows(x, plan == nullptr);

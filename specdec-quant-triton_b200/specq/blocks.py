@@ -85,9 +85,29 @@ def rope_table(n_pos, rot, base=10000.0, scaling=None, device="cuda"):
 def rope(x, pos, table, layout="half", inverse=False, out=None, plan=None):
     """Turn the first rot = table.shape[1] elements of every head of x [T, H, D] (float16, bfloat16 or
     float32; any row and head strides) to positions pos [T] int32; `out` may be x.  inverse=True
-    turns back, which is the gradient of the rotation.  With `plan`, only rows < plan[0]: the others of a
-    new output are 0, those of `out` keep what they hold."""
-    return _native.rope(x, pos, table, layout, inverse, out, plan)
+    turns back, which is the gradient of the rotation: an x that requires grad gets it (without `out`; the
+    table has none).  With `plan`, only rows < plan[0]: the others of a new output are 0, those of `out`
+    keep what they hold."""
+    y = _native.rope(x, pos, table, layout, inverse, out, plan)
+    return y if y is not NotImplemented else _Rope.apply(x, pos, table, layout, inverse, plan)
+
+
+class _Rope(torch.autograd.Function):
+    """The rotation with its gradient, the inverse rotation of the output's (the binding leaves an x that
+    requires grad to it)."""
+
+    @staticmethod
+    def forward(ctx, x, pos, table, layout, inverse, plan):
+        ctx.save_for_backward(pos, table, *(() if plan is None else (plan,)))
+        ctx.layout, ctx.inverse = layout, bool(inverse)
+        return _native.rope(x, pos, table, layout, inverse, None, plan)
+
+    @staticmethod
+    def backward(ctx, g):
+        pos, table, *plan = ctx.saved_tensors
+        if g.stride(-1) != 1:
+            g = g.contiguous()
+        return rope(g, pos, table, ctx.layout, not ctx.inverse, plan=plan[0] if plan else None), None, None, None, None, None
 
 
 # ----------------------------------------------------------------------------------------------

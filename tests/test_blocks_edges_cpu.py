@@ -147,3 +147,18 @@ def test_yarn_gain_is_one_where_nothing_is_stretched():
     assert (t[0, :16] == 0.75).all()
     t = specq.rope_table(4, 32, device="cpu", scaling={"type": "yarn", "factor": 2.0, "original": 4096})
     assert abs(t[0, 0].item() - (0.1 * math.log(2.0) + 1.0)) <= 2.0 ** -23
+
+
+def test_rope_refuses_gradients_that_it_does_not_have():
+    x, pos, table = torch.zeros(4, 2, 64), _i32(4), specq.rope_table(8, 64, device="cpu")
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(ValueError, match="requires grad"):
+        specq.rope(leaf, pos, table, out=torch.zeros(4, 2, 64))
+    with pytest.raises(ValueError, match="requires grad"):
+        specq.rope(x, pos, table, out=leaf)
+    with pytest.raises(ValueError, match="table has no gradient"):
+        specq.rope(x, pos, table.clone().requires_grad_())
+    with pytest.raises(ValueError, match="CUDA"):
+        specq.rope(leaf, pos, table)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        specq.rope(leaf, pos, table, out=torch.zeros(4, 2, 64))

@@ -206,3 +206,45 @@ def test_new_outputs_are_zero_where_a_call_does_not_reach(cuda):
         out = specq.rope(q, pos, table, plan=torch.tensor([n], dtype=torch.int32, device="cuda"))
         assert (out[n:] == 0).all() and torch.equal(out[:n], specq.rope(q, pos, table)[:n])
     assert _status() == 0
+
+
+# ---- the rotation's gradient ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rope_carries_gradients(cuda, layout, dtype):
+    """The gradient of a rotation is the inverse rotation of the output's gradient, and that of the inverse the
+    rotation; under a plan the rows past it have none.  Against difference quotients in fp32: a sum of n products
+    of size about 1 is off by n 2^-23 at most, the quotient by 2^-23 |f| / h more."""
+    import specq
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    T, H, D, rot = 9, 3, 64, 32
+    table = specq.rope_table(64, rot, device="cuda")
+    pos = torch.arange(T, dtype=torch.int32, device="cuda") * 5
+    x, g, d = (torch.randn(T, H, D, generator=gen, device="cuda").to(dtype) for _ in range(3))
+    plan = torch.tensor([4], dtype=torch.int32, device="cuda")
+    for inverse in (False, True):
+        for kw in (dict(), dict(plan=plan)):
+            leaf = x.clone().requires_grad_()
+            y = specq.rope(leaf, pos, table, layout=layout, inverse=inverse, **kw)
+            assert torch.equal(y.detach(), specq.rope(x, pos, table, layout=layout, inverse=inverse, **kw))
+            y.backward(g)
+            assert torch.equal(leaf.grad, specq.rope(g, pos, table, layout=layout, inverse=not inverse, **kw))
+    if dtype == torch.float32:
+        leaf = x.clone().requires_grad_()
+        specq.rope(leaf, pos, table, layout=layout).backward(g)
+        h = 0.25
+        f = lambda t: (g.double() * specq.rope(t, pos, table, layout=layout).double()).sum()  # noqa: E731
+        diff = (f(x + h * d) - f(x - h * d)) / (2 * h)
+        size = (g.abs() * (x.abs() + d.abs())).sum().item()
+        assert abs((diff - (leaf.grad.double() * d.double()).sum()).item()) <= 8 * 2.0 ** -23 * size / h + T * H * D * 2.0 ** -23
+        # the gradient's own gradient
+        leaf, gl = x.clone().requires_grad_(), g.clone().requires_grad_()
+        first, = torch.autograd.grad(specq.rope(leaf, pos, table, layout=layout), leaf, gl, create_graph=True)
+        second, = torch.autograd.grad(first, gl, d)
+        assert torch.equal(second, specq.rope(d, pos, table, layout=layout))
+    leaf = x.clone().requires_grad_()
+    with torch.no_grad():
+        assert not specq.rope(leaf, pos, table, layout=layout).requires_grad
+        buf = torch.empty_like(x)
+        assert specq.rope(leaf, pos, table, layout=layout, out=buf) is buf
+    assert _status() == 0
