@@ -42,10 +42,11 @@
 //
 // Measured (D = 128, 8 KV heads, group 4, page 64): B = 32, q = 1, context 4096: 55.0 us, 4.9 TB/s (heads
 // before slots in a page: 49.5 us, 5.4 TB/s, of the 6.44 that a copy reaches), bound by HBM.  B = 8,
-// q = 9, context 4096: 35 us, of which some 15 are set-up and the join (a launch runs its set-up once,
-// from cold instruction caches), and 2,400 cycles a tile where the products alone would take 1,525: two
+// q = 9, context 4096: 35.4 us (bf16 queries 37.9), of which some 15 are set-up and the join (a launch runs its set-up once,
+// from cold instruction caches), and some 2,400 cycles a tile where the products alone would take 1,525: two
 // warps a quarter of the SM are all that the registers hold (Q and O of 40 rows), too few to cover
-// their own latencies.  D = 64: two blocks of 24 rows an SM were 35 us for q = 9, one of 40 rows is 27.
+// their own latencies.  The registers spill from 17 rows on (-Xptxas -v: 268 to 368 bytes of stores a thread,
+// the feeding warps' among them) and at 9 to 16 rows of D = 128 (128 to 132).  D = 64: two blocks of 24 rows an SM were 35 us for q = 9, one of 40 rows is 27.
 //
 // Work.  The tiles of all (sequence, KV head, row chunk) segments form one line, each segment's after
 // some places that stand for the time its beginning takes; the line is cut into equal pieces, one

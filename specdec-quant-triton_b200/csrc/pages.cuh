@@ -21,7 +21,7 @@
 // it has found enough.  fork is that CTA and beside it others that snapshot the parents' rows, and
 // then a grid that copies the pages (bound by HBM) and rewrites the rows.  The kernels follow one
 // another by programmatic launch.  Measured, release + reserve + fork: 8 rows, one layer 9.2 us; 192 rows in
-// beams of 4, 16 layers of pages of 16 x 8 x 128: 24.1 us, of which the copies' bytes need 8.8.
+// beams of 4, 16 layers of pages of 16 x 8 x 128: 24.5 us, of which the copies' bytes need 8.8.
 #pragma once
 
 #include "sm100.cuh"
