@@ -365,6 +365,7 @@ int specq_block_compact(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_
  * ld) = the rows' pages (-1: none), held int32 [S] = how many each holds.  ref is 16-byte
  * aligned.  Results are functions of the state alone: free pages are taken lowest first.
  *   release  rows with drop[r] != 0 (uint8 [S]) give up their pages
+ *   trim     such rows keep the pages of their first length[r] tokens and give up the others
  *   reserve  row r grows to ceil(want[r] / page) pages; every row or none
  *   fork     row r with parent[r] = p >= 0, p != r becomes row p's first length[p] tokens: full
  *            pages shared, a part-filled last page copied (all L layers, filled slots and scales);
@@ -374,12 +375,96 @@ int specq_block_compact(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_
  */
 int specq_pages_release(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C,
                         const uint8_t* drop, void* stream);
+int specq_pages_trim(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C, const uint8_t* drop,
+                     const int32_t* length, int page, void* stream);
 int specq_pages_reserve(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C,
                         const int32_t* want, int page, int32_t* short_out, void* stream);
 int specq_pages_fork(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int L, float* ks,
                      float* vs, int64_t s_sl, int64_t s_sp, int64_t s_sh, int32_t* ref, int P, int32_t* tbl,
                      int64_t ld, int32_t* held, int S, int C, const int32_t* parent, const int32_t* length,
                      int32_t* scratch, int32_t* short_out, int H_KV, int D, int page, void* stream);
+
+/* RMS norm of every query and key head with its rotary turn:
+ *   r = (mean x^2 + eps)^(-1/2) over a head's D elements,  out = turn(x r w) as specq_rope turns
+ * in fp32 with one rounding.
+ *   q, k     [T, H, D], [T, H_KV, D] of SPECQ_DTYPE_* `dtype`, strides in elements, unit along D; the
+ *            outputs alike (in place with the same strides); D <= 2048
+ *   qw, kw   [D] of the same type, or fp32 with weight_f32 != 0; null: ones
+ *   eps      positive in fp32; table, pos, rot, layout, plan as for specq_rope
+ */
+int specq_qk_norm_rope(const void* q, int64_t qt, int64_t qh, void* q_out, int64_t qot, int64_t qoh, const void* k,
+                       int64_t kt, int64_t kh, void* k_out, int64_t kot, int64_t koh, int dtype, const void* qw,
+                       const void* kw, int weight_f32, float eps, const int32_t* pos, const float* table, int n_pos,
+                       int T, int H, int H_KV, int D, int rot, int layout, const int32_t* plan, void* stream);
+
+/* Its gradients: from gq, gk = dL/d(outputs) the dq, dk (null: not wanted) and dqw, dkw (of the weights' type,
+ * null: not wanted), which are sums over tokens and heads in a fixed order.  workspace: 16-byte aligned device memory of
+ * the bytes that specq_qk_norm_rope_grad_workspace gives, needed where dqw or dkw is wanted.
+ */
+int specq_qk_norm_rope_grad(const void* q, int64_t qt, int64_t qh, const void* gq, int64_t gqt, int64_t gqh, void* dq,
+                            int64_t dqt, int64_t dqh, const void* k, int64_t kt, int64_t kh, const void* gk,
+                            int64_t gkt, int64_t gkh, void* dk, int64_t dkt, int64_t dkh, int dtype, const void* qw,
+                            const void* kw, void* dqw, void* dkw, int weight_f32, float eps, const int32_t* pos,
+                            const float* table, int n_pos, int T, int H, int H_KV, int D, int rot, int layout,
+                            const int32_t* plan, void* workspace, int64_t workspace_bytes, void* stream);
+int specq_qk_norm_rope_grad_workspace(int T, int H, int H_KV, int D, int64_t* bytes);
+
+/* The n best continuations of B requests of K beams each (rows b K .. b K + K - 1).
+ *   logits   [B K, V] of SPECQ_DTYPE_* `dtype`, row stride ld in elements, unit along V
+ *   scores   fp32 [B K]; candidate (k, v) has the total score + logit - ln sum exp logits of its beam
+ *   done     optional uint8 [B K]: a finished beam's one candidate is (k, pad) with the beam's score
+ *   out_*    [B, n]: totals in fp32 in falling order, the candidate's row, its token; equal totals
+ *            (compared in 64 bits) by k V + v.  A total of -inf is no candidate; a place without one has
+ *            score -inf, row b K + j mod K and the pad token.  A NaN logit or score counts as -inf, a
+ *            logit of +inf as the largest finite number, a score of +inf as -inf.
+ * K <= 64, n <= 128, B K <= 65535, K V < 2^31.  workspace as the function below gives, 16-byte aligned.
+ */
+int specq_beam_select(const void* logits, int64_t ld, int dtype, const float* scores, const uint8_t* done, int pad,
+                      float* out_scores, int32_t* out_parent, int32_t* out_token, int B, int K, int V, int n,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+int specq_beam_select_workspace(int B, int K, int V, int n, int dtype, int64_t* bytes);
+
+/* Rows of `states` tensors moved to follow their beams: row r becomes row parent[r] (device int32 [B K]), as
+ * it was, where that is a row of the same request of K <= 64 beams; a negative parent keeps the row, and so does any
+ * other one outside the request (SPECQ_STATUS_BAD_INDEX).  ptr, stride, row_bytes: HOST arrays of
+ * device addresses, bytes between rows and bytes of a row.  No two states share memory.
+ */
+int specq_beam_reorder(void* const* ptr, const int64_t* stride, const int64_t* row_bytes, int states,
+                       const int32_t* parent, int B, int K, void* stream);
+
+/* The attention weight that each cached token gets from the q_len newest tokens' rows, added up:
+ *   mass[b, h, t] = decay mass[b, h, t] + sum over rows and the group's heads of softmax(q k sm_scale)[t]
+ * for t < ctx_len[b], h a KV head; q, cache, table and causal window as for specq_block_attention.
+ *   n_rows   optional int32 [B]: only the first n_rows[b] rows of the sequence count, which stand at the
+ *            places ctx_len[b] - n_rows[b] + i; a sequence without rows or tokens keeps its mass
+ *   mass     fp32 [B, H_KV, >= bt_cols * page], strides (m_sb, m_sh), unit along the tokens
+ * A query row with a NaN or an infinity adds nothing.
+ */
+int specq_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, const void* kc,
+                         int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int cache_dtype, int n_pages, const float* ks,
+                         int64_t s_sp, int64_t s_sh, const int32_t* block_tbl, int64_t bt_sb, int bt_cols,
+                         const int32_t* ctx_len, const int32_t* n_rows, float sm_scale, float decay, float* mass,
+                         int64_t m_sb, int64_t m_sh, int B, int q_len, int H, int H_KV, int D, int page,
+                         void* workspace, int64_t workspace_bytes, void* stream);
+int specq_attention_mass_workspace(int B, int q_len, int H, int H_KV, int D, int page, int bt_cols, int64_t* bytes);
+
+/* Each sequence of more than `keep` tokens cut down, in every layer and KV head by itself, to its `recent`
+ * newest tokens and the keep - recent others of largest mass (fp32 [L, B, H_KV, >= bt_cols * page], strides
+ * (m_sl, m_sb, m_sh); equal ones the earliest first, NaN last).  The kept tokens move to places 0 .. keep - 1 in
+ * their order, their masses with them, and mass is 0 from keep to the old length.  A page's scale becomes the largest
+ * of the pages its tokens come from; numbers of another scale are requantised.
+ *   ref      optional int32 [P] (the pool's counts): a sequence with a page that other rows share stays as it is
+ *   ctx_out  int32 [B], the new lengths (may be ctx_len)
+ * A sequence past its table, with a page outside the cache or a shared one keeps its tokens and its length
+ * (SPECQ_STATUS_BAD_INDEX).
+ */
+int specq_block_evict(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int cache_dtype,
+                      int L, int n_pages, float* ks, float* vs, int64_t s_sl, int64_t s_sp, int64_t s_sh,
+                      const int32_t* block_tbl, int64_t bt_sb, int bt_cols, const int32_t* ctx_len,
+                      const int32_t* ref, float* mass, int64_t m_sl, int64_t m_sb, int64_t m_sh, int keep, int recent,
+                      int32_t* ctx_out, int B, int H_KV, int D, int page, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+int specq_block_evict_workspace(int L, int B, int H_KV, int keep, int64_t* bytes);
 
 /*
  * Pipeline tracing (builds compiled with -DSPECQ_TRACE only; other builds return

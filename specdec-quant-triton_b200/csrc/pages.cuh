@@ -7,6 +7,7 @@
 // integers, whose order does not matter, or claim nothing).
 //
 // release  every held page of a dropped row counts one less; the row empties.
+// trim     the same for the pages past a row's first length[r] tokens.
 // reserve  row r is extended to ceil(want[r] / page) pages.  All rows or, when the free pages
 //          do not suffice, none; short = the missing pages (0: granted).
 // fork     row r with parent[r] = p (p >= 0, p != r) becomes a copy of row p's first
@@ -63,6 +64,28 @@ __global__ void __launch_bounds__(128) pages_release_kernel(const __grid_constan
   }
   __syncthreads();       // every thread has read held[r]
   if (threadIdx.x == 0) p.held[r] = 0;
+}
+
+// Rows r with drop[r] keep the pages of their first length[r] tokens and give up the others.
+__global__ void __launch_bounds__(128) pages_trim_kernel(const __grid_constant__ PagePool p, const uint8_t* drop, const int32_t* length,
+                                                         int page) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int r = blockIdx.x;
+  if (drop[r] == 0) return;
+  const int had = pool_held(p, r), len = length[r], n = min(had, len <= 0 ? 0 : (len - 1) / page + 1);
+  int32_t* row = p.tbl + r * p.ld;
+  for (int c = n + threadIdx.x; c < had; c += 128) {
+    const int pg = row[c];
+    if (pg < 0 || pg >= p.P) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+    else if (atomicSub(p.ref + pg, 1) <= 0) {
+      atomicAdd(p.ref + pg, 1);
+      report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+    }
+    row[c] = -1;
+  }
+  __syncthreads();       // every thread has read held[r]
+  if (threadIdx.x == 0) p.held[r] = n;
 }
 
 // Exclusive sum over the block's threads; total in *sum.  red: 33 ints.
@@ -401,6 +424,18 @@ inline int run_pages_release(int32_t* ref, int P, int32_t* tbl, int64_t ld, int3
   if (drop == nullptr) return fail(SPECQ_ERR_INVALID_ARG, "pages_release: null pointer");
   if (int rc = pool_device(&p)) return rc;
   SPECQ_CUDA_TRY(launch_plain(pages_release_kernel, dim3(S), dim3(128), static_cast<cudaStream_t>(stream), p, drop));
+  return SPECQ_OK;
+}
+
+inline int run_pages_trim(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C, const uint8_t* drop,
+                          const int32_t* length, int page, void* stream) {
+  PagePool p = {};
+  if (page <= 0) return fail(SPECQ_ERR_INVALID_ARG, "pages_trim: page %d", page);
+  if (int rc = make_pool("pages_trim", &p, ref, P, tbl, ld, held, S, C)) return rc;
+  if (S == 0) return SPECQ_OK;
+  if (drop == nullptr || length == nullptr) return fail(SPECQ_ERR_INVALID_ARG, "pages_trim: null pointer");
+  if (int rc = pool_device(&p)) return rc;
+  SPECQ_CUDA_TRY(launch_plain(pages_trim_kernel, dim3(S), dim3(128), static_cast<cudaStream_t>(stream), p, drop, length, page));
   return SPECQ_OK;
 }
 

@@ -20,6 +20,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <string>
+#include <vector>
 
 #include "specq.h"
 
@@ -36,6 +37,17 @@ struct Table {
   decltype(&specq_pages_release) pages_release;
   decltype(&specq_pages_reserve) pages_reserve;
   decltype(&specq_pages_fork) pages_fork;
+  decltype(&specq_pages_trim) pages_trim;
+  decltype(&specq_qk_norm_rope) qk_norm_rope;
+  decltype(&specq_qk_norm_rope_grad) qk_norm_rope_grad;
+  decltype(&specq_qk_norm_rope_grad_workspace) qk_norm_rope_grad_workspace;
+  decltype(&specq_beam_select) beam_select;
+  decltype(&specq_beam_select_workspace) beam_select_workspace;
+  decltype(&specq_beam_reorder) beam_reorder;
+  decltype(&specq_attention_mass) attention_mass;
+  decltype(&specq_attention_mass_workspace) attention_mass_workspace;
+  decltype(&specq_block_evict) block_evict;
+  decltype(&specq_block_evict_workspace) block_evict_workspace;
   decltype(&specq_last_error) last_error;
 } lib;
 PyObject* specq_error = nullptr;   // specq.SpecqError
@@ -411,14 +423,26 @@ Pool pool(const char* who, PyObject* const* a) {
 }
 
 PyObject* pages_release(PyObject* const* a) {
+  // ref, tbl, held, drop, length, page
   const char* who = "pages_release";
   const Pool p = pool(who, a);
   const Tensor& drop = tensor(who, "drop", a[3]);
   if ((drop.scalar_type() != at::kBool && drop.scalar_type() != at::kByte) || drop.dim() != 1 || drop.size(0) < p.S ||
       (drop.size(0) > 1 && drop.stride(0) != 1))
     BAD_VALUE("%s: drop must be a contiguous bool [%d], got %s %s", who, p.S, dtype(drop), shape(drop).c_str());
-  same_device(who, {&p.ref, &p.tbl, &p.held, &drop});
-  check(lib.pages_release(ptr<int32_t>(p.ref), p.P, ptr<int32_t>(p.tbl), p.ld, ptr<int32_t>(p.held), p.S, p.C, ptr<uint8_t>(drop), stream()));
+  const Tensor* length = optional(who, "length", a[4]);
+  if ((length == nullptr) != (a[5] == Py_None)) BAD_VALUE("%s: length and page go together", who);
+  if (length == nullptr) {
+    same_device(who, {&p.ref, &p.tbl, &p.held, &drop});
+    check(lib.pages_release(ptr<int32_t>(p.ref), p.P, ptr<int32_t>(p.tbl), p.ld, ptr<int32_t>(p.held), p.S, p.C, ptr<uint8_t>(drop), stream()));
+    return none();
+  }
+  int32s(who, "length", *length, 1, p.S);
+  const int page = integer(a[5]);
+  if (page < 1) BAD_VALUE("%s: page=%d", who, page);
+  same_device(who, {&p.ref, &p.tbl, &p.held, &drop, length});
+  check(lib.pages_trim(ptr<int32_t>(p.ref), p.P, ptr<int32_t>(p.tbl), p.ld, ptr<int32_t>(p.held), p.S, p.C, ptr<uint8_t>(drop),
+                       ptr<int32_t>(*length), page, stream()));
   return none();
 }
 
@@ -458,6 +482,306 @@ PyObject* pages_fork(PyObject* const* a) {
                        ptr<float>(c.ks), ptr<float>(c.vs), c.s_sl(), c.ks.stride(d), c.ks.stride(d + 1), ptr<int32_t>(p.ref), p.P,
                        ptr<int32_t>(p.tbl), p.ld, ptr<int32_t>(p.held), p.S, p.C, ptr<int32_t>(parent), ptr<int32_t>(length),
                        ptr<int32_t>(scratch), ptr<int32_t>(out), size32(who, c.H), size32(who, c.D), size32(who, c.page), stream()));
+  return wrap(out);
+}
+
+// ---- heads: norm and turn ---------------------------------------------------------------------------
+// q and k rows with their weights and angles, as qk_norm_rope and its gradient take them.
+struct Heads {
+  const Tensor &q, &k, &pos, &table;
+  const Tensor *qw, *kw, *plan;
+  float eps;
+  int layout, weight_f32;
+};
+
+Heads heads(const char* who, PyObject* q_, PyObject* k_, PyObject* qw_, PyObject* kw_, PyObject* pos_, PyObject* table_, PyObject* eps_,
+            PyObject* layout_, PyObject* plan_) {
+  const int lay = layout_code(who, layout_);
+  const Tensor &q = tensor(who, "q", q_), &k = tensor(who, "k", k_), &pos = tensor(who, "pos", pos_), &table = tensor(who, "table", table_);
+  rows3(who, "q", q, true);
+  rows3(who, "k", k, true);
+  if (k.scalar_type() != q.scalar_type() || k.size(0) != q.size(0) || k.size(2) != q.size(2))
+    BAD_VALUE("%s: q and k must be of one type, with as many rows and elements a head, got %s %s and %s %s", who, dtype(q),
+              shape(q).c_str(), dtype(k), shape(k).c_str());
+  const Tensor *qw = optional(who, "q_weight", qw_), *kw = optional(who, "k_weight", kw_);
+  int f32 = -1;
+  for (const Tensor* w : {qw, kw}) {
+    if (w == nullptr) continue;
+    if (w->scalar_type() != q.scalar_type() && w->scalar_type() != at::kFloat)
+      BAD_TYPE("%s: weights must be %s or float32, got %s", who, dtype(q), dtype(*w));
+    if (w->dim() != 1 || w->size(0) != q.size(2) || (w->size(0) > 1 && w->stride(0) != 1))
+      BAD_VALUE("%s: weights must be contiguous [%lld], got %s", who, (long long)q.size(2), shape(*w).c_str());
+    const int is = w->scalar_type() == at::kFloat;
+    if (f32 >= 0 && f32 != is) BAD_TYPE("%s: both weights must be of one type", who);
+    f32 = is;
+  }
+  rotary_table(who, table, q.size(2));
+  int32s(who, "pos", pos, 1, q.size(0));
+  const double eps = PyFloat_AsDouble(eps_);
+  if (eps == -1.0 && PyErr_Occurred()) throw Raised{};
+  if (!(static_cast<float>(eps) > 0.f) || !(eps < 3e38)) BAD_VALUE("%s: eps=%g must be positive and finite", who, eps);
+  const Tensor* plan = optional(who, "plan", plan_);
+  plan_of(who, plan, 1);
+  return Heads{q, k, pos, table, qw, kw, plan, static_cast<float>(eps), lay, f32 > 0};
+}
+
+const void* raw(const Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }
+
+PyObject* pack(std::initializer_list<Tensor> ts) {    // undefined tensors become None
+  PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
+  if (out == nullptr) throw Raised{};
+  Py_ssize_t i = 0;
+  for (const Tensor& t : ts) {
+    PyObject* o = t.defined() ? wrap(t) : none();
+    if (o == nullptr) {
+      Py_DECREF(out);
+      throw Raised{};
+    }
+    PyTuple_SET_ITEM(out, i++, o);
+  }
+  return out;
+}
+
+PyObject* qk_norm_rope(PyObject* const* a) {
+  // q, k, q_weight, k_weight, pos, table, eps, layout, q_out, k_out, plan
+  const char* who = "qk_norm_rope";
+  const Heads x = heads(who, a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7], a[10]);
+  const Tensor *q_given = optional(who, "q_out", a[8]), *k_given = optional(who, "k_out", a[9]);
+  auto out_like = [&](const char* what, const Tensor* out, const Tensor& in) {
+    if (out == nullptr) return;
+    rows3(who, what, *out, true);
+    if (out->scalar_type() != in.scalar_type() || out->sizes() != in.sizes())
+      BAD_VALUE("%s: %s must be %s %s, got %s %s", who, what, dtype(in), shape(in).c_str(), dtype(*out), shape(*out).c_str());
+    written(who, what, *out);
+  };
+  out_like("q_out", q_given, x.q);
+  out_like("k_out", k_given, x.k);
+  if (c10::GradMode::is_enabled()) {
+    const bool needs = x.q.requires_grad() || x.k.requires_grad() || (x.qw != nullptr && x.qw->requires_grad()) ||
+                       (x.kw != nullptr && x.kw->requires_grad());
+    if ((q_given != nullptr || k_given != nullptr) &&
+        (needs || (q_given != nullptr && q_given->requires_grad()) || (k_given != nullptr && k_given->requires_grad())))
+      BAD_VALUE("%s: no q_out or k_out where a gradient is wanted", who);
+    if (x.table.requires_grad()) BAD_VALUE("%s: the table has no gradient", who);
+    if (needs) Py_RETURN_NOTIMPLEMENTED;   // specq/heads.py records the gradient and calls again
+  }
+  same_device(who, {&x.q, &x.k, &x.pos, &x.table, x.qw, x.kw, q_given, k_given, x.plan});
+  const bool all = x.plan == nullptr;
+  const Tensor q_out = q_given != nullptr ? *q_given : new_rows(x.q, all), k_out = k_given != nullptr ? *k_given : new_rows(x.k, all);
+  check(lib.qk_norm_rope(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), x.k.data_ptr(),
+                         x.k.stride(0), x.k.stride(1), k_out.data_ptr(), k_out.stride(0), k_out.stride(1), row_code(x.q), raw(x.qw),
+                         raw(x.kw), x.weight_f32, x.eps, ptr<int32_t>(x.pos), ptr<float>(x.table), size32(who, x.table.size(0)),
+                         size32(who, x.q.size(0)), size32(who, x.q.size(1)), size32(who, x.k.size(1)), size32(who, x.q.size(2)),
+                         size32(who, x.table.size(1)), x.layout, ptr<int32_t>(x.plan), stream()));
+  return pack({q_out, k_out});
+}
+
+PyObject* qk_norm_rope_grad(PyObject* const* a) {
+  // gq, gk, q, k, q_weight, k_weight, pos, table, eps, layout, plan, want (bits: dq, dk, dqw, dkw)
+  const char* who = "qk_norm_rope's gradient";
+  const Heads x = heads(who, a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10]);
+  const Tensor &gq = tensor(who, "gq", a[0]), &gk = tensor(who, "gk", a[1]);
+  rows3(who, "gq", gq, true);
+  rows3(who, "gk", gk, true);
+  if (gq.scalar_type() != x.q.scalar_type() || gk.scalar_type() != x.q.scalar_type() || gq.sizes() != x.q.sizes() || gk.sizes() != x.k.sizes())
+    BAD_VALUE("%s: gradients %s %s and %s %s of outputs like %s and %s", who, dtype(gq), shape(gq).c_str(), dtype(gk), shape(gk).c_str(),
+              shape(x.q).c_str(), shape(x.k).c_str());
+  const int want = integer(a[11]);
+  same_device(who, {&x.q, &x.k, &gq, &gk, &x.pos, &x.table, x.qw, x.kw, x.plan});
+  const int T = size32(who, x.q.size(0)), H = size32(who, x.q.size(1)), HK = size32(who, x.k.size(1)), D = size32(who, x.q.size(2));
+  Tensor dq, dk, dqw, dkw, ws;
+  if (want & 1) dq = new_rows(x.q, x.plan == nullptr);
+  if (want & 2) dk = new_rows(x.k, x.plan == nullptr);
+  if ((want & 4) && x.qw != nullptr) dqw = at::empty(x.qw->sizes(), x.qw->options());
+  if ((want & 8) && x.kw != nullptr) dkw = at::empty(x.kw->sizes(), x.kw->options());
+  int64_t bytes = 0;
+  if (dqw.defined() || dkw.defined()) check(lib.qk_norm_rope_grad_workspace(T, H, HK, D, &bytes));
+  // from torch's allocator on the current stream, as the attention's
+  if (bytes > 0) ws = at::empty({bytes}, x.q.options().dtype(at::kByte));
+  auto p = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  auto st = [](const Tensor& t, int i) { return t.defined() ? t.stride(i) : 0; };
+  check(lib.qk_norm_rope_grad(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), gq.data_ptr(), gq.stride(0), gq.stride(1), p(dq), st(dq, 0),
+                              st(dq, 1), x.k.data_ptr(), x.k.stride(0), x.k.stride(1), gk.data_ptr(), gk.stride(0), gk.stride(1), p(dk),
+                              st(dk, 0), st(dk, 1), row_code(x.q), raw(x.qw), raw(x.kw), p(dqw), p(dkw), x.weight_f32, x.eps,
+                              ptr<int32_t>(x.pos), ptr<float>(x.table), size32(who, x.table.size(0)), T, H, HK, D,
+                              size32(who, x.table.size(1)), x.layout, ptr<int32_t>(x.plan), p(ws), bytes, stream()));
+  return pack({dq, dk, dqw, dkw});
+}
+
+// ---- beams ------------------------------------------------------------------------------------------
+PyObject* beam_select(PyObject* const* a) {
+  // logits, scores, n, done, pad, beams
+  const char* who = "beam_select";
+  const Tensor &x = tensor(who, "logits", a[0]), &scores = tensor(who, "scores", a[1]);
+  if (row_code(x) < 0) BAD_TYPE("%s: logits must be float16, bfloat16 or float32, got %s", who, dtype(x));
+  if (x.dim() != 2 || (x.size(1) > 1 && x.stride(1) != 1)) BAD_VALUE("%s: logits must be [rows, vocabulary] with unit inner stride, got %s", who, shape(x).c_str());
+  if (scores.scalar_type() != at::kFloat || scores.numel() != x.size(0) || !scores.is_contiguous() || scores.dim() > 2)
+    BAD_VALUE("%s: scores must be contiguous float32 [requests, beams] of %lld rows, got %s %s", who, (long long)x.size(0), dtype(scores),
+              shape(scores).c_str());
+  if (a[5] == Py_None && scores.dim() != 2) BAD_VALUE("%s: give beams, or scores as [requests, beams]", who);
+  const int K = a[5] == Py_None ? size32(who, scores.size(1)) : integer(a[5]);
+  if (K < 1 || x.size(0) % K || (scores.dim() == 2 && scores.size(1) != K)) BAD_VALUE("%s: %lld rows of scores %s are no requests of %d beams", who, (long long)x.size(0), shape(scores).c_str(), K);
+  const int n = integer_or(a[2], K), pad = integer(a[4]), V = size32(who, x.size(1)), B = size32(who, x.size(0) / K);
+  if (n < 1 || V < 1) BAD_VALUE("%s: n=%d of a vocabulary of %d", who, n, V);
+  if (x.size(0) > 1 && x.stride(0) < V) BAD_VALUE("%s: logits' rows overlap (stride %lld of %d tokens); give each beam its row", who, (long long)x.stride(0), V);
+  const Tensor* done = optional(who, "done", a[3]);
+  if (done != nullptr && ((done->scalar_type() != at::kBool && done->scalar_type() != at::kByte) || done->numel() != x.size(0) || !done->is_contiguous()))
+    BAD_VALUE("%s: done must be a contiguous bool of %lld rows, got %s %s", who, (long long)x.size(0), dtype(*done), shape(*done).c_str());
+  if (pad < 0 || pad >= V) BAD_VALUE("%s: pad=%d is no token of %d", who, pad, V);
+  if (c10::GradMode::is_enabled() && (x.requires_grad() || scores.requires_grad())) BAD_VALUE("%s: no gradient; detach logits and scores", who);
+  same_device(who, {&x, &scores, done});
+  const Tensor out = at::empty({B, n}, scores.options()), parent = at::empty({B, n}, scores.options().dtype(at::kInt)),
+               token = at::empty({B, n}, scores.options().dtype(at::kInt));
+  int64_t bytes = 0;
+  check(lib.beam_select_workspace(B, K, V, n, row_code(x), &bytes));
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  check(lib.beam_select(x.data_ptr(), x.size(0) > 1 ? x.stride(0) : V, row_code(x), ptr<float>(scores), ptr<uint8_t>(done), pad, ptr<float>(out),
+                        ptr<int32_t>(parent), ptr<int32_t>(token), B, K, V, n, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream()));
+  return pack({out, parent, token});
+}
+
+PyObject* beam_reorder(PyObject* const* a) {
+  // states, parent, beams
+  const char* who = "beam_reorder";
+  if (!PyList_Check(a[0]) && !PyTuple_Check(a[0])) BAD_TYPE("%s: states must be a list or a tuple of tensors", who);
+  const Tensor& parent = tensor(who, "parent", a[1]);
+  if (parent.scalar_type() != at::kInt || !parent.is_contiguous() || parent.dim() < 1 || parent.dim() > 2)
+    BAD_VALUE("%s: parent must be contiguous int32 [rows] or [requests, beams], got %s %s", who, dtype(parent), shape(parent).c_str());
+  const int K = a[2] == Py_None && parent.dim() == 2 ? size32(who, parent.size(1)) : a[2] == Py_None ? 0 : integer(a[2]);
+  const int64_t R = parent.numel();
+  if (K < 1 || R % K) BAD_VALUE("%s: %lld rows are no requests of %d beams (give beams, or parent as [requests, beams])", who, (long long)R, K);
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(a[0]);
+  PyObject** items = PySequence_Fast_ITEMS(a[0]);
+  std::vector<void*> at_(count);
+  std::vector<int64_t> stride(count), bytes(count);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const Tensor& t = tensor(who, "a state", items[i]);
+    if (t.dim() < 1 || t.size(0) != R) BAD_VALUE("%s: state %zd is %s for %lld rows", who, i, shape(t).c_str(), (long long)R);
+    int64_t inner = 1;                                   // a row is one run of memory
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+      if (t.size(d) > 1 && t.stride(d) != inner) BAD_VALUE("%s: state %zd's rows must be contiguous, strides of %s", who, i, shape(t).c_str());
+      inner *= t.size(d);
+    }
+    if (R > 1 && inner > 0 && t.stride(0) < inner) BAD_VALUE("%s: state %zd is written and its rows must not share memory", who, i);
+    if (c10::GradMode::is_enabled() && t.requires_grad()) BAD_VALUE("%s: state %zd requires grad; it is written in place", who, i);
+    at_[i] = t.data_ptr();
+    stride[i] = t.stride(0) * t.element_size();
+    bytes[i] = inner * t.element_size();
+    for (Py_ssize_t j = 0; j < i && bytes[i] > 0; ++j) {     // columns of one buffer are two states, shared bytes are not
+      if (bytes[j] == 0) continue;
+      const int64_t lo = static_cast<char*>(at_[i]) - static_cast<char*>(at_[j]);
+      const int64_t span_i = (R - 1) * stride[i] + bytes[i], span_j = (R - 1) * stride[j] + bytes[j];
+      if (lo >= span_j || -lo >= span_i) continue;
+      bool apart = false;
+      if (stride[i] == stride[j] && R > 1) {
+        const int64_t s = stride[i], off = ((lo % s) + s) % s;
+        apart = off >= bytes[j] && off + bytes[i] <= s;
+      }
+      if (!apart) BAD_VALUE("%s: states %zd and %zd share memory", who, j, i);
+    }
+  }
+  for (Py_ssize_t i = 0; i < count; ++i) same_device(who, {&parent, &THPVariable_Unpack(items[i])});
+  same_device(who, {&parent});
+  check(lib.beam_reorder(at_.data(), stride.data(), bytes.data(), size32(who, count), ptr<int32_t>(parent), size32(who, R / K), K, stream()));
+  return none();
+}
+
+// ---- a bounded cache --------------------------------------------------------------------------------
+// mass: float32, one run of at least `tokens` for each sequence and KV head (and layer)
+void mass_of(const char* who, const Tensor& m, bool layers, int64_t L, int64_t B, int64_t H, int64_t tokens) {
+  const int d = layers ? 1 : 0;
+  if (m.scalar_type() != at::kFloat) BAD_TYPE("%s: mass must be float32, got %s", who, dtype(m));
+  if (m.dim() != 3 + d || (d && m.size(0) != L) || m.size(d) < B || m.size(d + 1) != H || m.size(d + 2) < tokens)
+    BAD_VALUE("%s: mass must be [%s%lld, %lld, >= %lld], got %s", who, d ? (std::to_string(L) + ", ").c_str() : "", (long long)B, (long long)H,
+              (long long)tokens, shape(m).c_str());
+  if (m.size(d + 2) > 1 && m.stride(d + 2) != 1) BAD_VALUE("%s: mass needs unit stride along the tokens", who);
+  written(who, "mass", m);
+  if (c10::GradMode::is_enabled() && m.requires_grad()) BAD_VALUE("%s: mass requires grad; it is written in place", who);
+}
+
+PyObject* attention_mass_blocks(PyObject* const* a) {
+  // q, kc, ks, block_tbl, ctx_len, mass, q_len, n_rows, decay, sm_scale
+  const char* who = "attention_mass_blocks";
+  PyObject* const keys[4] = {a[1], a[1], a[2], a[2]};
+  const Cache c = cache(who, keys, false, false);
+  const Tensor& q = tensor(who, "q", a[0]);
+  if (q.scalar_type() != at::kHalf && q.scalar_type() != at::kBFloat16)
+    BAD_TYPE("%s: q must be float16 or bfloat16, got %s", who, dtype(q));
+  const Tensor &tbl = tensor(who, "block_tbl", a[3]), &ctx = tensor(who, "ctx_len", a[4]), &mass = tensor(who, "mass", a[5]);
+  int32s(who, "block_tbl", tbl, 2, -1);
+  int32s(who, "ctx_len", ctx, 1, tbl.size(0));
+  const int B = size32(who, tbl.size(0)), cols = size32(who, tbl.size(1));
+  const bool packed = q.dim() == 3;
+  if (packed ? a[6] == Py_None : q.dim() != 4) {
+    if (packed) BAD_VALUE("%s: packed queries need q_len", who);
+    BAD_VALUE("%s: q must have 3 or 4 dimensions, got %s", who, shape(q).c_str());
+  }
+  const int q_len = packed ? integer(a[6]) : integer_or(a[6], size32(who, q.size(1)));
+  if (q_len < 0 || (packed ? q.size(0) < static_cast<int64_t>(B) * q_len : q.size(0) < B || q.size(1) < q_len))
+    BAD_VALUE("%s: q is %s for %d sequences of %d tokens", who, shape(q).c_str(), B, q_len);
+  if (!packed && q.stride(0) == 0 && B > 1) BAD_VALUE("%s: q is expanded over the sequences (its stride is 0); give each sequence its rows", who);
+  const int64_t H = q.size(-2);
+  if (q.size(-1) != c.D || c.H == 0 || H < 1 || H % c.H)
+    BAD_VALUE("%s: q heads (%lld, %lld) do not fit the cache's (%lld, %lld)", who, (long long)H, (long long)q.size(-1), (long long)c.H, (long long)c.D);
+  if (q.stride(-1) != 1) BAD_VALUE("%s: q needs unit stride along D", who);
+  const Tensor* n_rows = optional(who, "n_rows", a[7]);
+  if (n_rows != nullptr) int32s(who, "n_rows", *n_rows, 1, B);
+  mass_of(who, mass, false, 1, B, c.H, static_cast<int64_t>(cols) * c.page);
+  const double decay = PyFloat_AsDouble(a[8]);
+  if (decay == -1.0 && PyErr_Occurred()) throw Raised{};
+  if (!(decay >= 0 && decay <= 1)) BAD_VALUE("%s: decay=%g must be in 0..1", who, decay);
+  float sm = 1.f / std::sqrt(static_cast<float>(c.D));
+  if (a[9] != Py_None) {
+    const double v = PyFloat_AsDouble(a[9]);
+    if (v == -1.0 && PyErr_Occurred()) throw Raised{};
+    if (!(v > 0)) BAD_VALUE("%s: sm_scale=%g must be positive", who, v);
+    sm = static_cast<float>(v);
+  }
+  same_device(who, {&c.kc, &c.ks, &q, &tbl, &ctx, n_rows, &mass});
+  const int h = size32(who, H), hk = size32(who, c.H), D = size32(who, c.D), page = size32(who, c.page);
+  int64_t bytes = 0;
+  check(lib.attention_mass_workspace(B, q_len, h, hk, D, page, cols, &bytes));
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  const int o = packed ? 0 : 1;
+  // to the kernels a batch stride of 0 says packed rows; one sequence is one either way
+  check(lib.attention_mass(q.data_ptr(), packed ? 0 : q.stride(0), q.stride(o), q.stride(o + 1), row_code(q), c.kc.data_ptr(), c.kc.stride(0),
+                           c.kc.stride(1), c.kc.stride(2), cache_code(c.kc), size32(who, c.P), ptr<float>(c.ks), c.ks.stride(0), c.ks.stride(1),
+                           ptr<int32_t>(tbl), tbl.stride(0), cols, ptr<int32_t>(ctx), ptr<int32_t>(n_rows), sm, static_cast<float>(decay),
+                           ptr<float>(mass), mass.stride(0), mass.stride(1), B, q_len, h, hk, D, page, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
+                           stream()));
+  Py_INCREF(a[5]);
+  return a[5];
+}
+
+PyObject* kv_evict_blocks(PyObject* const* a) {
+  // kc, vc, ks, vs, block_tbl, ctx_len, mass, keep, recent, ref, ctx_out
+  const char* who = "kv_evict_blocks";
+  const Cache c = cache(who, a, true);
+  const Tensor &tbl = tensor(who, "block_tbl", a[4]), &ctx = tensor(who, "ctx_len", a[5]), &mass = tensor(who, "mass", a[6]);
+  int32s(who, "block_tbl", tbl, 2, -1);
+  const int64_t B = tbl.size(0);
+  int32s(who, "ctx_len", ctx, 1, B);
+  if (c.L == 0) BAD_VALUE("%s: a cache without layers", who);
+  const int keep = integer(a[7]), recent = integer(a[8]);
+  if (keep < 1 || recent < 0 || recent > keep) BAD_VALUE("%s: keep=%d, of these the newest recent=%d", who, keep, recent);
+  mass_of(who, mass, c.d != 0, c.L, B, c.H, tbl.size(1) * c.page);
+  const Tensor *ref = optional(who, "ref", a[9]), *given = optional(who, "ctx_out", a[10]);
+  if (ref != nullptr) int32s(who, "ref", *ref, 1, c.P);
+  if (given != nullptr) int32s(who, "ctx_out", *given, 1, B);
+  same_device(who, {&c.kc, &c.vc, &c.ks, &c.vs, &tbl, &ctx, &mass, ref, given});
+  const Tensor out = given != nullptr ? *given : new_int32(ctx, B);
+  const int L = size32(who, c.L), b = size32(who, B), h = size32(who, c.H), d = c.d;
+  if (b == 0 || h == 0) return wrap(out);
+  int64_t bytes = 0;
+  check(lib.block_evict_workspace(L, b, h, keep, &bytes));
+  const Tensor ws = at::empty({bytes}, c.kc.options().dtype(at::kByte));
+  check(lib.block_evict(c.kc.data_ptr(), c.vc.data_ptr(), c.sl(), c.kc.stride(d), c.kc.stride(d + 1), c.kc.stride(d + 2), cache_code(c.kc), L,
+                        size32(who, c.P), ptr<float>(c.ks), ptr<float>(c.vs), c.s_sl(), c.ks.stride(d), c.ks.stride(d + 1), ptr<int32_t>(tbl),
+                        tbl.stride(0), size32(who, tbl.size(1)), ptr<int32_t>(ctx), ptr<int32_t>(ref), ptr<float>(mass), d ? mass.stride(0) : 0,
+                        mass.stride(d), mass.stride(d + 1), keep, recent, ptr<int32_t>(out), b, h, size32(who, c.D), size32(who, c.page),
+                        ws.data_ptr(), bytes, stream()));
   return wrap(out);
 }
 
@@ -501,6 +825,17 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
       {"specq_pages_release", reinterpret_cast<void**>(&t.pages_release)},
       {"specq_pages_reserve", reinterpret_cast<void**>(&t.pages_reserve)},
       {"specq_pages_fork", reinterpret_cast<void**>(&t.pages_fork)},
+      {"specq_pages_trim", reinterpret_cast<void**>(&t.pages_trim)},
+      {"specq_qk_norm_rope", reinterpret_cast<void**>(&t.qk_norm_rope)},
+      {"specq_qk_norm_rope_grad", reinterpret_cast<void**>(&t.qk_norm_rope_grad)},
+      {"specq_qk_norm_rope_grad_workspace", reinterpret_cast<void**>(&t.qk_norm_rope_grad_workspace)},
+      {"specq_beam_select", reinterpret_cast<void**>(&t.beam_select)},
+      {"specq_beam_select_workspace", reinterpret_cast<void**>(&t.beam_select_workspace)},
+      {"specq_beam_reorder", reinterpret_cast<void**>(&t.beam_reorder)},
+      {"specq_attention_mass", reinterpret_cast<void**>(&t.attention_mass)},
+      {"specq_attention_mass_workspace", reinterpret_cast<void**>(&t.attention_mass_workspace)},
+      {"specq_block_evict", reinterpret_cast<void**>(&t.block_evict)},
+      {"specq_block_evict_workspace", reinterpret_cast<void**>(&t.block_evict_workspace)},
       {"specq_last_error", reinterpret_cast<void**>(&t.last_error)},
   };
   for (const auto& e : names) {
@@ -525,7 +860,13 @@ PyMethodDef methods[] = {
     {"kv_append_blocks", FAST((entry<kv_append_blocks, 17>)), nullptr},
     {"paged_attention_blocks", FAST((entry<paged_attention_blocks, 14>)), nullptr},
     {"kv_compact_blocks", FAST((entry<kv_compact_blocks, 10>)), nullptr},
-    {"pages_release", FAST((entry<pages_release, 4>)), nullptr},
+    {"qk_norm_rope", FAST((entry<qk_norm_rope, 11>)), nullptr},
+    {"qk_norm_rope_grad", FAST((entry<qk_norm_rope_grad, 12>)), nullptr},
+    {"beam_select", FAST((entry<beam_select, 6>)), nullptr},
+    {"beam_reorder", FAST((entry<beam_reorder, 3>)), nullptr},
+    {"attention_mass_blocks", FAST((entry<attention_mass_blocks, 10>)), nullptr},
+    {"kv_evict_blocks", FAST((entry<kv_evict_blocks, 11>)), nullptr},
+    {"pages_release", FAST((entry<pages_release, 6>)), nullptr},
     {"pages_reserve", FAST((entry<pages_reserve, 6>)), nullptr},
     {"pages_fork", FAST((entry<pages_fork, 10>)), nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -16,6 +16,10 @@
 #include "block_cache.cuh"
 #include "block_attn.cuh"
 #include "pages.cuh"
+#include "qk_norm.cuh"
+#include "beams.cuh"
+#include "mass.cuh"
+#include "evict.cuh"
 
 namespace specq {
 
@@ -570,6 +574,90 @@ int specq_pages_fork(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t k
   last_launch_ref() = LaunchRecord();
   return run_pages_fork(kc, vc, kv_sl, kv_sp, kv_so, kv_sh, L, ks, vs, s_sl, s_sp, s_sh, ref, P, tbl, ld, held, S,
                         C, parent, length, scratch, short_out, H_KV, D, page, stream);
+}
+
+int specq_qk_norm_rope(const void* q, int64_t qt, int64_t qh, void* q_out, int64_t qot, int64_t qoh, const void* k,
+                       int64_t kt, int64_t kh, void* k_out, int64_t kot, int64_t koh, int dtype, const void* qw, const
+                       void* kw, int weight_f32, float eps, const int32_t* pos, const float* table, int n_pos, int T,
+                       int H, int H_KV, int D, int rot, int layout, const int32_t* plan, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_qk_norm_rope(q, qt, qh, q_out, qot, qoh, k, kt, kh, k_out, kot, koh, dtype, qw, kw, weight_f32, eps,
+                          pos, table, n_pos, T, H, H_KV, D, rot, layout, plan, stream);
+}
+
+int specq_qk_norm_rope_grad(const void* q, int64_t qt, int64_t qh, const void* gq, int64_t gqt, int64_t gqh, void* dq,
+                            int64_t dqt, int64_t dqh, const void* k, int64_t kt, int64_t kh, const void* gk, int64_t
+                            gkt, int64_t gkh, void* dk, int64_t dkt, int64_t dkh, int dtype, const void* qw, const
+                            void* kw, void* dqw, void* dkw, int weight_f32, float eps, const int32_t* pos, const
+                            float* table, int n_pos, int T, int H, int H_KV, int D, int rot, int layout, const
+                            int32_t* plan, void* workspace, int64_t workspace_bytes, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_qk_norm_rope_grad(q, qt, qh, gq, gqt, gqh, dq, dqt, dqh, k, kt, kh, gk, gkt, gkh, dk, dkt, dkh, dtype,
+                               qw, kw, dqw, dkw, weight_f32, eps, pos, table, n_pos, T, H, H_KV, D, rot, layout, plan,
+                               workspace, workspace_bytes, stream);
+}
+
+int specq_qk_norm_rope_grad_workspace(int T, int H, int H_KV, int D, int64_t* bytes) {
+  last_launch_ref() = LaunchRecord();
+  return run_qk_norm_rope_grad_workspace(T, H, H_KV, D, bytes);
+}
+
+int specq_beam_select(const void* logits, int64_t ld, int dtype, const float* scores, const uint8_t* done, int pad,
+                      float* out_scores, int32_t* out_parent, int32_t* out_token, int B, int K, int V, int n, void*
+                      workspace, int64_t workspace_bytes, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_beam_select(logits, ld, dtype, scores, done, pad, out_scores, out_parent, out_token, B, K, V, n,
+                         workspace, workspace_bytes, stream);
+}
+
+int specq_beam_select_workspace(int B, int K, int V, int n, int dtype, int64_t* bytes) {
+  last_launch_ref() = LaunchRecord();
+  return run_beam_select_workspace(B, K, V, n, dtype, bytes);
+}
+
+int specq_beam_reorder(void* const* ptr, const int64_t* stride, const int64_t* row_bytes, int states, const int32_t*
+                       parent, int B, int K, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_beam_reorder(ptr, stride, row_bytes, states, parent, B, K, stream);
+}
+
+int specq_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, const void* kc, int64_t
+                         kv_sp, int64_t kv_so, int64_t kv_sh, int cache_dtype, int n_pages, const float* ks, int64_t
+                         s_sp, int64_t s_sh, const int32_t* block_tbl, int64_t bt_sb, int bt_cols, const int32_t*
+                         ctx_len, const int32_t* n_rows, float sm_scale, float decay, float* mass, int64_t m_sb,
+                         int64_t m_sh, int B, int q_len, int H, int H_KV, int D, int page, void* workspace, int64_t
+                         workspace_bytes, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_attention_mass(q, q_sb, q_st, q_sh, dtype, kc, kv_sp, kv_so, kv_sh, cache_dtype, n_pages, ks, s_sp,
+                            s_sh, block_tbl, bt_sb, bt_cols, ctx_len, n_rows, sm_scale, decay, mass, m_sb, m_sh, B,
+                            q_len, H, H_KV, D, page, workspace, workspace_bytes, stream);
+}
+
+int specq_attention_mass_workspace(int B, int q_len, int H, int H_KV, int D, int page, int bt_cols, int64_t* bytes) {
+  last_launch_ref() = LaunchRecord();
+  return run_attention_mass_workspace(B, q_len, H, H_KV, D, page, bt_cols, bytes);
+}
+
+int specq_block_evict(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int cache_dtype,
+                      int L, int n_pages, float* ks, float* vs, int64_t s_sl, int64_t s_sp, int64_t s_sh, const
+                      int32_t* block_tbl, int64_t bt_sb, int bt_cols, const int32_t* ctx_len, const int32_t* ref,
+                      float* mass, int64_t m_sl, int64_t m_sb, int64_t m_sh, int keep, int recent, int32_t* ctx_out,
+                      int B, int H_KV, int D, int page, void* workspace, int64_t workspace_bytes, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_block_evict(kc, vc, kv_sl, kv_sp, kv_so, kv_sh, cache_dtype, L, n_pages, ks, vs, s_sl, s_sp, s_sh,
+                         block_tbl, bt_sb, bt_cols, ctx_len, ref, mass, m_sl, m_sb, m_sh, keep, recent, ctx_out, B,
+                         H_KV, D, page, workspace, workspace_bytes, stream);
+}
+
+int specq_block_evict_workspace(int L, int B, int H_KV, int keep, int64_t* bytes) {
+  last_launch_ref() = LaunchRecord();
+  return run_block_evict_workspace(L, B, H_KV, keep, bytes);
+}
+
+int specq_pages_trim(int32_t* ref, int P, int32_t* tbl, int64_t ld, int32_t* held, int S, int C, const uint8_t* drop,
+                     const int32_t* length, int page, void* stream) {
+  last_launch_ref() = LaunchRecord();
+  return run_pages_trim(ref, P, tbl, ld, held, S, C, drop, length, page, stream);
 }
 
 

@@ -9,9 +9,11 @@ import torch
 
 from . import _lib
 from . import fixtures
-from .blocks import (kv_append_blocks, kv_compact_blocks, paged_attention_blocks, pages_fork, pages_release,
-                     pages_reserve, rope, rope_table)
+from .beams import beam_reorder, beam_select
+from .blocks import (attention_mass_blocks, kv_append_blocks, kv_compact_blocks, kv_evict_blocks, paged_attention_blocks,
+                     pages_fork, pages_release, pages_reserve, rope, rope_table)
 from .fixtures import make_paged_kv, paged_attention_ref, quantize_weight_int8
+from .heads import qk_norm_rope
 from .ops import (QUANT_PLAIN, QUANT_RESIDUAL, QUANT_SILU_MUL, KernelHandle, _paged_attn_kernel, _w4a16_kernel,
                   _w8a8_kernel, kv_append, pack_int4, paged_attention, paged_attention_packed, quant_rows,
                   w4a16_matmul, w8a8_accumulator, w8a8_matmul)
@@ -54,5 +56,5 @@ __all__ = [
     "KernelHandle", "get_status", "SpecqError",
     "quant_rows", "kv_append", "pack_int4", "fixtures", "paged_attention_packed", "QUANT_PLAIN", "QUANT_RESIDUAL", "QUANT_SILU_MUL",
     "rope", "rope_table", "kv_append_blocks", "paged_attention_blocks", "kv_compact_blocks", "pages_release",
-    "pages_reserve", "pages_fork",
+    "pages_reserve", "pages_fork", "attention_mass_blocks", "kv_evict_blocks", "qk_norm_rope", "beam_select", "beam_reorder",
 ]

@@ -83,6 +83,25 @@ SIGNATURES = {
     "specq_pages_reserve": (_i32, [_vp, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _i32, _vp, _vp]),
     "specq_pages_fork": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _vp, _i32, _vp,
                     _i64, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
+    "specq_qk_norm_rope": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp,
+                    _vp, _i32, C.c_float, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "specq_qk_norm_rope_grad": (_i32, [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+                    _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i32, C.c_float, _vp, _vp, _i32, _i32,
+                    _i32, _i32, _i32, _i32, _i32, _vp, _vp, _i64, _vp]),
+    "specq_qk_norm_rope_grad_workspace": (_i32, [_i32, _i32, _i32, _i32, C.POINTER(C.c_int64)]),
+    "specq_beam_select": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _i64,
+                    _vp]),
+    "specq_beam_select_workspace": (_i32, [_i32, _i32, _i32, _i32, _i32, C.POINTER(C.c_int64)]),
+    "specq_beam_reorder": (_i32, [_vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp]),
+    "specq_attention_mass": (_i32, [_vp, _i64, _i64, _i64, _i32, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i64, _i64,
+                    _vp, _i64, _i32, _vp, _vp, C.c_float, C.c_float, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32,
+                    _i32, _vp, _i64, _vp]),
+    "specq_attention_mass_workspace": (_i32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, C.POINTER(C.c_int64)]),
+    "specq_block_evict": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i64, _i64, _i64,
+                    _vp, _i64, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _vp,
+                    _i64, _vp]),
+    "specq_block_evict_workspace": (_i32, [_i32, _i32, _i32, _i32, C.POINTER(C.c_int64)]),
+    "specq_pages_trim": (_i32, [_vp, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _i32, _vp]),
     "specq_trace_configure": (_i32, [_vp, _i32]),
 }
 

@@ -5,6 +5,8 @@
     kv_append_blocks(k, v, kc, vc, ks, vs, block_tbl, ctx_len, q_len, q=..., table=...)
     paged_attention_blocks(q, kc, vc, ks, vs, block_tbl, ctx_len, tree=...)
     kv_compact_blocks(kc, vc, ks, vs, block_tbl, ctx_len, q_len, accept, n_accept)
+    attention_mass_blocks(q, kc, ks, block_tbl, ctx_len, mass)    the attention weight each token got, added up
+    kv_evict_blocks(kc, vc, ks, vs, block_tbl, ctx_len, mass, keep, recent)    only the heaviest and newest kept
     pages_release / pages_reserve / pages_fork                the pool of pages
 
 kc, vc [P, page, H_KV, D] int8 or float8_e4m3fn, ks, vs float32 [P, H_KV]; value = number *
@@ -151,12 +153,44 @@ def kv_compact_blocks(kc, vc, ks, vs, block_tbl, ctx_len, q_len, accept, n_accep
 
 
 # ----------------------------------------------------------------------------------------------
+# a bounded cache: accumulated attention weight, eviction
+# ----------------------------------------------------------------------------------------------
+def attention_mass_blocks(q, kc, ks, block_tbl, ctx_len, mass, q_len=None, n_rows=None, decay=1.0, sm_scale=None):
+    """Add to `mass` the attention weight that each cached token gets from the q_len newest tokens' queries:
+
+        mass[b, h, t] = decay * mass[b, h, t] + sum over rows and the heads of group h of softmax(q k)[t]
+
+    for t < ctx_len[b], in place; returned as well.  q, cache, table and causal window are those of
+    paged_attention_blocks (the same q that it is given); mass float32 [B, H_KV, N], N >= the table's tokens.  `n_rows`
+    [B] int32: only the first n_rows[b] rows of a sequence count, the newest n_rows[b] tokens of its ctx_len[b] (a
+    padded batch; the accepted rows of a verification after kv_compact_blocks).  A sequence without
+    rows or tokens keeps its mass.  A query row with a NaN or an infinity adds nothing.  No gradient."""
+    return _native.attention_mass_blocks(q, kc, ks, block_tbl, ctx_len, mass, q_len, n_rows, decay, sm_scale)
+
+
+def kv_evict_blocks(kc, vc, ks, vs, block_tbl, ctx_len, mass, keep, recent=0, ref=None, ctx_out=None):
+    """Cut every sequence of more than `keep` tokens down to `keep`, in each layer and KV head by itself: its
+    `recent` newest tokens and the others of largest mass (equal ones the earliest first, NaN last).  Returns the new
+    lengths int32 [B] (ctx_out, which may be ctx_len).
+
+    The kept tokens move together in their order, and their masses with them; mass is 0 from there to the old end.
+    A page's scale becomes the largest of the pages its tokens come from, and numbers of another scale are
+    requantised.  Positions were turned in before: a later append gives the tokens' own by `pos`.  One layer with mass
+    [B, H_KV, N], or all layers of a cache with mass [L, B, H_KV, N].  With `ref` (the pool's counts)
+    a sequence that shares a page with another row is left as it is, as is one with a page outside the cache, and
+    the status word says so; without it no page may be shared.  The pages past the new length stay the
+    row's: pages_release gives them up."""
+    return _native.kv_evict_blocks(kc, vc, ks, vs, block_tbl, ctx_len, mass, keep, recent, ref, ctx_out)
+
+
+# ----------------------------------------------------------------------------------------------
 # the page pool
 # ----------------------------------------------------------------------------------------------
-def pages_release(ref, tbl, held, drop):
+def pages_release(ref, tbl, held, drop, length=None, page=None):
     """Rows r with drop[r] (bool [S]) give up their pages: ref int32 [P] counts the rows that hold a page,
-    tbl int32 [S, C] has the rows' pages (-1: none), held int32 [S] their number."""
-    return _native.pages_release(ref, tbl, held, drop)
+    tbl int32 [S, C] has the rows' pages (-1: none), held int32 [S] their number.  With `length` (int32 [S])
+    and the page size they keep the pages of their first length[r] tokens."""
+    return _native.pages_release(ref, tbl, held, drop, length, page)
 
 
 def pages_reserve(ref, tbl, held, want_len, page, short=None):
