@@ -416,7 +416,7 @@ int specq_qk_norm_rope_grad_workspace(int T, int H, int H_KV, int D, int64_t* by
  *   out_*    [B, n]: totals in fp32 in falling order, the candidate's row, its token; equal totals
  *            (compared in 64 bits) by k V + v.  A total of -inf is no candidate; a place without one has
  *            score -inf, row b K + j mod K and the pad token.  A NaN logit or score counts as -inf, a
- *            logit of +inf as the largest finite number, a score of +inf as -inf.
+ *            logit of +inf as its type's largest finite number, a score of +inf as -inf.
  * K <= 64, n <= 128, B K <= 65535, K V < 2^31.  workspace as the function below gives, 16-byte aligned.
  */
 int specq_beam_select(const void* logits, int64_t ld, int dtype, const float* scores, const uint8_t* done, int pad,

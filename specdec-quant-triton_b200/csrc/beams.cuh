@@ -5,20 +5,18 @@
 // candidate (k, v) has the total s_k + (x[k, v] - lse_k); a finished beam has one candidate, its pad token
 // with the total s_k.  The n best of a request come out in order, equal totals by k V + v.  A total of -inf
 // (a masked token, an empty beam) is none; places left over have the score -inf, the pad token and
-// the row b K + j mod K.  A NaN logit counts as -inf, +inf as the largest finite number; a NaN or +inf score as -inf.
+// the row b K + j mod K.  A NaN logit counts as -inf, +inf as its type's largest finite number; a NaN or +inf score as -inf.
 //
 // Which candidate comes first is an answer of whole numbers, so totals are compared in 64 bits and lse must
-// be good to some 1e-7: exp is made with the product by log2 e in two parts (the rounding of that product
-// is the error that would not average out), eight values are added in fp32 and the rest in 64 bits.  Within a row
+// be good to some 1e-7: what the rounding of the row's largest logit times log2 e moves is put right in the sum, sixteen values are added in fp32 and the rest in 64 bits.  Within a row
 // the order is that of the logits themselves, which needs no exp.
 //
-// Bound by HBM: one pass over the logits.  A block holds a slice of one row in shared memory (8 or 2
-// 16-byte pieces a thread, which only that thread reads back), so maximum, sum and selection read it once.  Selection: the n-th largest of the
-// threads' maxima is a bound that at least n elements reach and few more; those are ranked by
-// counting.  Where many elements reach it (ties, a constant row) the n-th largest key is found by bisection
-// of its bits and its equals are taken in the order of their index, which bounds the work for every row.  A second
-// launch merges a request's sorted lists, the best of the lists' heads at a time, by one warp up to 128
-// lists, by eight and then one beyond.
+// Bound by HBM: one pass over the logits.  A block holds a slice of one row in shared memory (2 to 16 16-byte pieces a
+// thread, which only that thread reads back), so maximum, sum and selection read it once.  Selection: each warp's
+// t-th largest of its threads' maxima (8 t >= n) gives a bound that at least n elements reach and few more; those are
+// ranked by counting.  Where many elements reach it (ties, a constant row) the n-th largest key is found by bisection of its
+// bits and its equals are taken in the order of their index, which bounds the work for every row.  A second launch
+// takes the best of a request's lists in the same way, or merges the lists where too many totals meet the bound.
 //
 // reorder.  Row r of each state becomes row parent[r], a row of the same request, as it was before the call.  A thread reads
 // its 16 bytes of all the request's moving rows and then writes them: in place without a copy of the state, and
@@ -26,6 +24,7 @@
 #pragma once
 
 #include <cfloat>
+#include <cmath>
 
 #include "rope.cuh"
 
@@ -35,9 +34,7 @@ constexpr int kSelThreads = 256;
 constexpr int kSelMaxN = 128;
 constexpr int kSelMaxBeams = 64;
 constexpr int kSelBuf = 512;       // candidates of a slice that are ranked by counting
-constexpr int kSelPieces = 8;      // 16-byte pieces a thread; kSelFewPieces where there are few rows
-constexpr int kSelFewPieces = 2;
-constexpr int kSelOneWarp = 128;   // lists that one warp merges
+constexpr int kSelMaxPieces = 16;  // 16-byte pieces a thread: 64 KB of a row, three blocks an SM
 constexpr uint32_t kKeyNone = 0x007FFFFFu;   // the key of -inf, which is no candidate
 
 // Unsigned keys in the order of the floats (no NaN; -0 and +0 are one value).
@@ -56,18 +53,85 @@ __device__ __forceinline__ double key64_value(uint64_t k) {
   return __longlong_as_double(static_cast<int64_t>(k & 0x8000000000000000ull ? k ^ 0x8000000000000000ull : ~k));
 }
 
-// A logit as the selection sees it: NaN is -inf, +inf the largest finite number.
-__device__ __forceinline__ float plain_logit(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
+// Two 16-bit logits, or one fp32 one, of a word: the larger of each; the same with NaN kept; and the words that
+// the selection has in place of a NaN (-inf) and of +inf (the type's largest finite number).
+template <typename T>
+struct LogitWord;
+template <>
+struct LogitWord<float> {
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+  static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+    return __float_as_uint(y);
+  }
+  static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ bool strange(uint32_t w) { return !(__uint_as_float(w) < INFINITY); }
+  static __device__ __forceinline__ uint32_t plain(uint32_t w) {
+    const float x = __uint_as_float(w);
+    return __float_as_uint(fminf(fmaxf(x, -INFINITY), FLT_MAX));
+  }
+  static constexpr uint32_t kNone = 0xFF800000u;
+};
+template <>
+struct LogitWord<__half> {
+  static __device__ __forceinline__ __half2 h(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
+  static __device__ __forceinline__ uint32_t u(__half2 w) { return *reinterpret_cast<const uint32_t*>(&w); }
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { return u(__hmax2(h(a), h(b))); }
+  static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) { return u(__hmax2_nan(h(a), h(b))); }
+  static __device__ __forceinline__ float top(uint32_t w) { return fmaxf(__low2float(h(w)), __high2float(h(w))); }
+  static __device__ __forceinline__ bool strange(uint32_t w) { return !(__low2float(h(w)) < INFINITY && __high2float(h(w)) < INFINITY); }
+  static __device__ __forceinline__ uint32_t plain(uint32_t w) { return u(__hmin2(__hmax2(h(w), h(kNone)), h(0x7BFF7BFFu))); }
+  static constexpr uint32_t kNone = 0xFC00FC00u;
+};
+template <>
+struct LogitWord<__nv_bfloat16> {
+  static __device__ __forceinline__ __nv_bfloat162 h(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+  static __device__ __forceinline__ uint32_t u(__nv_bfloat162 w) { return *reinterpret_cast<const uint32_t*>(&w); }
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { return u(__hmax2(h(a), h(b))); }
+  static __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b) { return u(__hmax2_nan(h(a), h(b))); }
+  static __device__ __forceinline__ float top(uint32_t w) { return fmaxf(__low2float(h(w)), __high2float(h(w))); }
+  static __device__ __forceinline__ bool strange(uint32_t w) { return !(__low2float(h(w)) < INFINITY && __high2float(h(w)) < INFINITY); }
+  static __device__ __forceinline__ uint32_t plain(uint32_t w) { return u(__hmin2(__hmax2(h(w), h(kNone)), h(0x7F7F7F7Fu))); }
+  static constexpr uint32_t kNone = 0xFF80FF80u;
+};
 
-// exp(d), d <= 0: 2^(d log2 e) with the product's low part kept.  log2 e = kLog2eHi + kLog2eLo to 2^-50.
-__device__ __forceinline__ float exp_wide(float d) {
-  constexpr float kLog2eHi = 1.44269502162933349609375f, kLog2eLo = 1.92596303e-8f, kLn2 = 0.693147182f;
-  d = fmaxf(d, -200.f);             // exp(-200) is below fp32; -inf would make a NaN of the low part
-  const float hi = d * kLog2eHi;
-  const float lo = fmaf(d, kLog2eLo, fmaf(d, kLog2eHi, -hi));
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(hi));
-  return fmaf(e, lo * kLn2, e);
+// exp(x - top) of two logits added up: 2^(x c - top c), one rounding a term.  `shift` is fp32(top c); what its rounding moves is
+// the same factor in every term, which shift_factor gives.  c is log2 e less 1.9e-8, so a term far below the top is off by 1.3e-8
+// of its distance: in rows alike an error alike, beside which an order of beams is not lost.  (-inf goes through as 0.)
+constexpr float kFarTop = 1024.f;      // above it the moved factor is no longer 1 + a little (and fp32(top c) may be infinite)
+constexpr float kLog2eF = 1.44269502162933349609375f;
+__device__ __forceinline__ void add_exp(float x, float y, float2 minus_shift, float2& sum) {
+  const float2 t = __ffma2_rn(make_float2(x, y), make_float2(kLog2eF, kLog2eF), minus_shift);
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  sum = __fadd2_rn(sum, e);
+}
+__device__ __forceinline__ double shift_factor(float top, float shift) {
+  return 1.0 + 0.6931471805599453 * (static_cast<double>(shift) - static_cast<double>(top) * static_cast<double>(kLog2eF));
+}
+
+// exp(x) for |x| < 700, to 1e-9 of itself: 2^k times Taylor's sum of the rest (|r| <= ln 2 / 2, r^9 / 9! < 2.1e-10); in place of the
+// library's, whose code is longer than all of the merge.
+__device__ __forceinline__ double exp64(double x) {
+  const double k = rint(x * 1.4426950408889634);
+  const double r = fma(k, -0.6931471805599453, x);
+  double y = 1.0 / 40320;
+  y = fma(y, r, 1.0 / 5040);
+  y = fma(y, r, 1.0 / 720);
+  y = fma(y, r, 1.0 / 120);
+  y = fma(y, r, 1.0 / 24);
+  y = fma(y, r, 1.0 / 6);
+  y = fma(y, r, 0.5);
+  y = fma(y, r, 1.0);
+  y = fma(y, r, 1.0);
+  return __longlong_as_double(__double_as_longlong(y) + (static_cast<int64_t>(static_cast<int>(k)) << 52));
+}
+// ln(x), 1 <= x < 2^100: a Newton step for exp(y) = x from fp32's logarithm, which is good to 1e-6.
+__device__ __forceinline__ double log64(double x) {
+  const double y = static_cast<double>(__logf(static_cast<float>(x)));
+  return y + (x * exp64(-y) - 1.0);
 }
 
 struct BeamSelectParams {
@@ -83,6 +147,7 @@ struct BeamSelectParams {
   int* status;
   int64_t ld;
   int K, V, n, S, slice, pieces, pad;
+  uint32_t lists_inv, beams_inv;   // 2^32 / (K S) and / K, rounded up: exact quotients of a staged candidate's index
 };
 
 __device__ __forceinline__ bool beam_alive(float score) { return score > -INFINITY && score < INFINITY; }
@@ -126,112 +191,163 @@ __device__ __forceinline__ int block_before(int v, int* red, int* sum) {
 template <typename T>
 __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const __grid_constant__ BeamSelectParams p) {
   constexpr int E = Row16<T>::N;
+  using W = LogitWord<T>;
   extern __shared__ uint4 held[];                 // [pieces, threads]: a thread reads back its own pieces
   __shared__ uint64_t buf[kSelBuf];
-  __shared__ uint32_t top[kSelThreads];
+  __shared__ uint32_t warp_top[kSelThreads / 32], warp_least[kSelThreads / 32];
   __shared__ double redd[kSelThreads / 32];
   __shared__ int redi[kSelThreads / 32];
-  __shared__ uint32_t bound;
+  __shared__ int found;
   pdl_launch_dependents();
   pdl_wait();
-  const int row = blockIdx.y, s = blockIdx.x, tid = static_cast<int>(threadIdx.x);
+  const int row = blockIdx.y, s = blockIdx.x, tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
   if (!beam_alive(p.scores[row]) || (p.done != nullptr && p.done[row] != 0)) return;   // no logits are needed
   const T* x = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.ld;
-  // pieces begin at the 16-byte boundary before the row: element 0 of the slice is index `first`
+  // pieces begin at the 16-byte boundary before the row: element 0 of the slice is index `first`, and the slices of a row
+  // meet at first + slice
   const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
   const int first = s * p.slice - shift;
-  const int end = min(p.V, first + p.slice);      // the slices of a row meet at first + slice
-  const int begin = max(first, 0);
-  const int pieces = p.pieces;
+  const int NP = p.pieces;                        // even
+  auto fetch = [&](int j, int i) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(held + j * kSelThreads + tid)), "l"(x + i) : "memory");
+  };
+  const bool whole = first >= 0 && first + p.slice <= p.V;
+  if (whole) {
 #pragma unroll 4
-  for (int j = 0; j < pieces; ++j) {
-    const int i = first + (j * kSelThreads + tid) * E;
-    uint4* to = held + j * kSelThreads + tid;
-    if (i >= begin && i + E <= end) {
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(x + i) : "memory");
-    } else {                                      // the row's ends, by elements; -inf outside
-      T* e = reinterpret_cast<T*>(to);
-#pragma unroll
-      for (int k = 0; k < E; ++k) e[k] = i + k >= begin && i + k < end ? x[i + k] : f32_to_row<T>(-INFINITY);
+    for (int j = 0; j < NP; ++j) fetch(j, first + (j * kSelThreads + tid) * E);
+  } else {                                        // a row's ends: -inf outside, its cut pieces by elements
+#pragma unroll 1
+    for (int j = 0; j < NP; ++j) {
+      const int i = first + (j * kSelThreads + tid) * E;
+      if (i >= 0 && i + E <= p.V) fetch(j, i);
+      else if (i >= p.V) held[j * kSelThreads + tid] = make_uint4(W::kNone, W::kNone, W::kNone, W::kNone);
+    }
+    const int last = (p.V - first) / E * E;       // the piece that the row's end cuts, if it does: two warps' lanes take the two
+    const int at = tid < 32 ? lane : last + lane;
+    if (lane < E && (tid < 32 ? first < 0 : tid < 64 && last < p.slice && first + last < p.V)) {
+      const int i = first + at;
+      reinterpret_cast<T*>(held)[at] = i >= 0 && i < p.V ? x[i] : f32_to_row<T>(-INFINITY);
     }
   }
+  if (tid == 0) found = 0;
   asm volatile("cp.async.wait_all;" ::: "memory");
-  auto piece = [&](int j, float (&v)[E]) {
+  if (!whole) __syncthreads();
+  // (loops over the pieces are not unrolled: the kernel is short against its code)
+  float m = -INFINITY;
+  uint32_t seen = W::kNone;
+  auto top_of = [&](const uint4& u) { return W::top(W::max(W::max(u.x, u.y), W::max(u.z, u.w))); };
+#pragma unroll 2
+  for (int j = 0; j < NP; ++j) {
+    const uint4 u = held[j * kSelThreads + tid];
+    seen = W::max_nan(seen, W::max_nan(W::max_nan(u.x, u.y), W::max_nan(u.z, u.w)));
+    m = fmaxf(m, top_of(u));
+  }
+  if (W::strange(seen)) {                         // rewritten once, by the only thread that reads them
+    m = -INFINITY;
+#pragma unroll 1
+    for (int j = 0; j < NP; ++j) {
+      uint4& u = held[j * kSelThreads + tid];
+      u = make_uint4(W::plain(u.x), W::plain(u.y), W::plain(u.z), W::plain(u.w));
+      m = fmaxf(m, top_of(u));
+    }
+  }
+  const uint32_t mine = order_key(m);
+  // Each warp's k-th largest of its threads' maxima, 8 k >= n: at least n elements reach the least of these.
+  {
+    const int k = (p.n + kSelThreads / 32 - 1) / (kSelThreads / 32);
+    uint32_t left = mine, at = 0;
+    for (int i = 0; i < k; ++i) {
+      at = __reduce_max_sync(0xffffffffu, left);
+      if (i == 0 && lane == 0) warp_top[warp] = at;
+      if (lane == __ffs(__ballot_sync(0xffffffffu, left == at)) - 1) left = 0;
+    }
+    if (lane == 0) warp_least[warp] = at;
+  }
+  __syncthreads();
+  uint32_t best = 0, least = 0xffffffffu;
+#pragma unroll
+  for (int w = 0; w < kSelThreads / 32; ++w) {
+    best = max(best, warp_top[w]);
+    least = min(least, warp_least[w]);
+  }
+  least = max(least, kKeyNone + 1);               // fewer than n candidates: every one is taken
+  const float row_max = key_value(best), bound = key_value(least);
+  auto values = [&](int j, float (&v)[E]) {
     Row16<T> r;
     r.raw = held[j * kSelThreads + tid];
     r.get(v);
-#pragma unroll
-    for (int k = 0; k < E; ++k) v[k] = plain_logit(v[k]);
   };
-  float m = -INFINITY;
-#pragma unroll 2
-  for (int j = 0; j < pieces; ++j) {
-    float v[E];
-    piece(j, v);
-#pragma unroll
-    for (int k = 0; k < E; ++k) m = fmaxf(m, v[k]);
-  }
-  const uint32_t mine = order_key(m);
-  top[tid] = mine;
-  if (tid == 0) bound = kKeyNone + 1;             // fewer than n threads with a candidate: every one is taken
-  __syncthreads();
-  // rank of this thread's maximum, equal ones by thread; the block's maximum on the way
-  int rank = 0;
-  uint32_t best = 0;
-  for (int t = 0; t < kSelThreads; t += 4) {
-    const uint4 u = *reinterpret_cast<const uint4*>(top + t);
-    rank += (u.x > mine || (u.x == mine && t < tid)) + (u.y > mine || (u.y == mine && t + 1 < tid)) +
-            (u.z > mine || (u.z == mine && t + 2 < tid)) + (u.w > mine || (u.w == mine && t + 3 < tid));
-    best = max(best, max(max(u.x, u.y), max(u.z, u.w)));
-  }
-  if (rank == p.n - 1 && mine > kKeyNone) bound = mine;
-  const float row_max = key_value(best);
-  double sum = 0.0;
+  // the warp goes through the pieces of its threads that reach the bound, a lane a piece
   if (best > kKeyNone) {
-#pragma unroll 1
-    for (int j = 0; j < pieces; ++j) {
-      float v[E], e8 = 0.f;
-      piece(j, v);
+    for (uint32_t todo = __ballot_sync(0xffffffffu, mine >= least); todo != 0u; todo &= todo - 1u) {
+      const int from = warp * 32 + __ffs(todo) - 1;
+      if (lane >= NP || top_of(held[lane * kSelThreads + from]) < bound) continue;
+      Row16<T> r;
+      float v[E];
+      r.raw = held[lane * kSelThreads + from];
+      r.get(v);
+      uint32_t hits = 0;
 #pragma unroll
-      for (int k = 0; k < E; ++k) e8 += exp_wide(v[k] - row_max);
-      sum += static_cast<double>(e8);
+      for (int k = 0; k < E; ++k) hits |= v[k] >= bound ? 1u << k : 0u;
+      int at = atomicAdd(&found, __popc(hits));   // their order does not matter: they are ranked
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if (hits >> k & 1u) {
+          if (at < kSelBuf) buf[at] = static_cast<uint64_t>(order_key(v[k])) << 32 | static_cast<uint32_t>(~(first + (lane * kSelThreads + from) * E + k));
+          ++at;
+        }
     }
   }
-  sum = block_total(sum, redd);                   // (its barriers publish `bound`)
+  double sum = 0.0;
+  if (best > kKeyNone) {
+    const float shift = row_max * kLog2eF;
+    const float2 minus_shift = make_float2(-shift, -shift);
+    const bool far = fabsf(row_max) > kFarTop;
+#pragma unroll 1
+    for (int j = 0; j < NP; j += 2) {             // two pieces in fp32, the rest in 64 bits
+      float2 e = {0.f, 0.f};
+      if (far) {
+        for (int i = 0; i < 2; ++i) {
+          float v[E];
+          values(j + i, v);
+#pragma unroll
+          for (int k = 0; k < E; ++k) e.x += exp2f((v[k] - row_max) * kLog2eF);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float v[E];
+          values(j + i, v);
+#pragma unroll
+          for (int k = 0; k < E; k += 2) add_exp(v[k], v[k + 1], minus_shift, e);
+        }
+      }
+      sum += static_cast<double>(e.x + e.y);
+    }
+    if (!far) sum *= shift_factor(row_max, shift);
+  }
+  sum = block_total(sum, redd);                   // (its barriers publish buf and found)
   const int64_t list = static_cast<int64_t>(row) * p.S + s;
   if (tid == 0) {
     p.part_max[list] = best > kKeyNone ? row_max : -INFINITY;
     p.part_sum[list] = sum;
   }
-  uint32_t least = bound;
-  auto count_from = [&](uint32_t key) {
-    int c = 0;
+  int total = found;
+  if (total > kSelBuf) {
+    auto count_from = [&](uint32_t key) {
+      int c = 0;
 #pragma unroll 1
-    for (int j = 0; j < pieces; ++j) {
-      float v[E];
-      piece(j, v);
-#pragma unroll
-      for (int k = 0; k < E; ++k) c += order_key(v[k]) >= key;
-    }
-    return c;
-  };
-  auto put = [&](int at, uint32_t key, int index) { buf[at] = static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~index); };
-  int cnt = mine >= least ? count_from(least) : 0, total;
-  int at = block_before(cnt, redi, &total);
-  if (total <= kSelBuf) {
-    if (cnt > 0) {
-#pragma unroll 1
-      for (int j = 0; j < pieces; ++j) {
+      for (int j = 0; j < NP; ++j) {
         float v[E];
-        piece(j, v);
+        values(j, v);
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-          const uint32_t key = order_key(v[k]);
-          if (key >= least) put(at++, key, first + (j * kSelThreads + tid) * E + k);
-        }
+        for (int k = 0; k < E; ++k) c += order_key(v[k]) >= key;
       }
-    }
-  } else {
+      return c;
+    };
+    auto put = [&](int at, uint32_t key, int j, int k) {
+      buf[at] = static_cast<uint64_t>(key) << 32 | static_cast<uint32_t>(~(first + (j * kSelThreads + tid) * E + k));
+    };
     // the n-th largest key: the largest one that at least n elements reach
     uint32_t lo = least, hi = best;
     while (lo < hi) {
@@ -239,18 +355,18 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const __grid_co
       if (block_total(mine >= mid ? count_from(mid) : 0, redi) >= p.n) lo = mid;
       else hi = mid - 1;
     }
-    cnt = mine > lo ? count_from(lo + 1) : 0;     // fewer than n are above it
-    at = block_before(cnt, redi, &total);
+    const int cnt = mine > lo ? count_from(lo + 1) : 0;     // fewer than n are above it
+    int at = block_before(cnt, redi, &total);
     int left = p.n - total, next = total;         // its equals fill up, lowest index first
 #pragma unroll 1
-    for (int j = 0; j < pieces; ++j) {
+    for (int j = 0; j < NP; ++j) {
       float v[E];
-      piece(j, v);
+      values(j, v);
       int same = 0;
 #pragma unroll
       for (int k = 0; k < E; ++k) {
         const uint32_t key = order_key(v[k]);
-        if (key > lo) put(at++, key, first + (j * kSelThreads + tid) * E + k);
+        if (key > lo) put(at++, key, j, k);
         same += key == lo;
       }
       int all;
@@ -258,7 +374,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const __grid_co
 #pragma unroll
       for (int k = 0; k < E; ++k)
         if (order_key(v[k]) == lo) {
-          if (before < left) put(next + before, lo, first + (j * kSelThreads + tid) * E + k);
+          if (before < left) put(next + before, lo, j, k);
           ++before;
         }
       const int took = min(all, left);
@@ -266,12 +382,13 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const __grid_co
       next += took;
     }
     total = next;
+    __syncthreads();
   }
-  __syncthreads();
   uint64_t* out = p.cand + list * p.n;
   for (int c = tid; c < total; c += kSelThreads) {
     const uint64_t me = buf[c];
     int ahead = 0;
+#pragma unroll 4
     for (int o = 0; o < total; ++o) ahead += buf[o] > me;
     if (ahead < p.n) out[ahead] = me;
   }
@@ -279,66 +396,84 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const __grid_co
 }
 
 constexpr int kMergeThreads = 256;
-constexpr int kMergeSmem = 64 * 1024;   // candidates up to this size are staged in shared memory
+constexpr int kMergeWarps = kMergeThreads / 32;
+constexpr int kMergeRank = 256;         // candidates that are ranked by counting
+constexpr int kMergeSmem = 96 * 1024;   // a request's candidates up to this size are staged in shared memory
 
 struct Merged {                         // a candidate of a request
   uint64_t key;                         // order_key64 of its total; 0: none
   uint32_t at;                          // k V + v
-  __device__ __forceinline__ bool before(const Merged& o) const { return key > o.key || (key == o.key && at < o.at); }
 };
 
-// The lane with the warp's first candidate, or -1 when no lane has one; *got: that candidate.
-__device__ __forceinline__ int warp_first(const Merged& mine, Merged* got) {
-  const uint32_t hi = static_cast<uint32_t>(mine.key >> 32), lo = static_cast<uint32_t>(mine.key);
+// The lane with the first of the warp's candidates, or -1 when no lane has one.
+__device__ __forceinline__ int warp_first(const Merged& mine) {
+  const uint32_t hi = static_cast<uint32_t>(mine.key >> 32);
   const uint32_t mh = __reduce_max_sync(0xffffffffu, hi);
   if (mh == 0u) return -1;              // (the key of a finite total has a high word above 0)
-  const uint32_t ml = __reduce_max_sync(0xffffffffu, hi == mh ? lo : 0u);
-  const bool tie = hi == mh && lo == ml;
-  const uint32_t mi = __reduce_min_sync(0xffffffffu, tie ? mine.at : 0xffffffffu);
-  got->key = static_cast<uint64_t>(mh) << 32 | ml;
-  got->at = mi;
-  return __ffs(__ballot_sync(0xffffffffu, tie && mine.at == mi)) - 1;
+  uint32_t who = __ballot_sync(0xffffffffu, hi == mh);
+  if (who & (who - 1)) {
+    const uint32_t lo = static_cast<uint32_t>(mine.key);
+    const uint32_t ml = __reduce_max_sync(0xffffffffu, hi == mh ? lo : 0u);
+    const bool tie = hi == mh && lo == ml;
+    const uint32_t mi = __reduce_min_sync(0xffffffffu, tie ? mine.at : 0xffffffffu);
+    who = __ballot_sync(0xffffffffu, tie && mine.at == mi);
+  }
+  return __ffs(who) - 1;
 }
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_constant__ BeamSelectParams p, int staged) {
-  extern __shared__ uint64_t dyn[];     // staged candidates [K, S, n], then a position for each list
+  extern __shared__ __align__(16) uint8_t dyn[];   // staged: totals' keys [K, S, n] and places [K, S, n]; a position a list
   __shared__ double top[kSelMaxBeams];  // a beam's largest logit and the logarithm of its sum: their sum would round
   __shared__ double ln[kSelMaxBeams];   // the small one away beside logits of 1e16 and more
   __shared__ float score[kSelMaxBeams];
   __shared__ int mode[kSelMaxBeams];    // 0: has lists, 1: finished, 2: no candidate
-  __shared__ Merged warp_list[kMergeThreads / 32][kSelMaxN];
+  __shared__ Merged warp_list[kMergeWarps * kSelMaxN];
+  __shared__ Merged final_list[kSelMaxN];
+  __shared__ uint32_t warp_least[kMergeWarps];
+  __shared__ int found;
   pdl_launch_dependents();
   pdl_wait();
   const int b = blockIdx.x, tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
-  const int lists = p.K * p.S;
-  uint64_t* staged_cand = dyn;
-  int* pos = reinterpret_cast<int*>(dyn + (staged ? static_cast<int64_t>(lists) * p.n : 0));
-  const uint64_t* cand = p.cand + static_cast<int64_t>(b) * lists * p.n;
-  if (staged) {
-    for (int i = tid; i < lists * p.n; i += kMergeThreads) staged_cand[i] = cand[i];
-    cand = staged_cand;
+  const int lists = p.K * p.S, all = lists * p.n;
+  uint64_t* keys = reinterpret_cast<uint64_t*>(dyn);
+  uint32_t* places = reinterpret_cast<uint32_t*>(keys + all);
+  int* pos = staged ? reinterpret_cast<int*>(places + all) : reinterpret_cast<int*>(dyn);
+  const uint64_t* cand = p.cand + static_cast<int64_t>(b) * all;
+  if (tid == 0) found = 0;
+  if (staged) {                         // on their way while the sums are made
+#pragma unroll 4
+    for (int i = tid; i < all; i += kMergeThreads)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(keys + i)), "l"(cand + i) : "memory");
   }
-  for (int i = tid; i < lists; i += kMergeThreads) pos[i] = 0;
   // a warp a beam: maximum and sum over its slices
-  for (int k = warp; k < p.K; k += kMergeThreads / 32) {
+  for (int k = warp; k < p.K; k += kMergeWarps) {
     const int row = b * p.K + k;
     const float sc = p.scores[row];
     int md = !beam_alive(sc) ? 2 : p.done != nullptr && p.done[row] != 0 ? 1 : 0;
     double l = 0.0;
     float m = -INFINITY;
     if (md == 0) {
-      for (int s = lane; s < p.S; s += 32) m = fmaxf(m, p.part_max[static_cast<int64_t>(row) * p.S + s]);
+      const float* pm = p.part_max + static_cast<int64_t>(row) * p.S;
+      const double* ps = p.part_sum + static_cast<int64_t>(row) * p.S;
+      float m0 = lane < p.S ? pm[lane] : -INFINITY;
+      double s0 = lane < p.S ? ps[lane] : 0.0;
+      m = m0;
+      for (int s = lane + 32; s < p.S; s += 32) m = fmaxf(m, pm[s]);
       m = warp_max_f32(m);
-      double sum = 0.0;
-      if (m > -INFINITY)
-        for (int s = lane; s < p.S; s += 32) {
-          const float pm = p.part_max[static_cast<int64_t>(row) * p.S + s];
-          if (pm > -INFINITY) sum += p.part_sum[static_cast<int64_t>(row) * p.S + s] * exp(static_cast<double>(pm) - static_cast<double>(m));
-        }
+      auto share = [&](float v, double sum) {    // below e^-100 it is nothing beside the largest one's
+        const double d = static_cast<double>(v) - static_cast<double>(m);
+        return d > -100.0 ? sum * exp64(d) : 0.0;
+      };
+      if (m > -INFINITY) {
+        double sum = m0 > -INFINITY ? share(m0, s0) : 0.0;
+        for (int s = lane + 32; s < p.S; s += 32)
+          if (pm[s] > -INFINITY) sum += share(pm[s], ps[s]);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (m > -INFINITY) l = log(sum);
-      else md = 2;
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l = log64(sum);
+      } else {
+        md = 2;
+      }
     }
     if (lane == 0) {
       top[k] = static_cast<double>(m);
@@ -347,28 +482,139 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
       mode[k] = md;
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  // the candidate at the head of a list
-  auto head = [&](int list) {
-    const int k = list / p.S, s = list - k * p.S, i = pos[list];
+  // i / d by d's inverse
+  auto div = [](int i, int d, uint32_t inv) { return d == 1 ? i : static_cast<int>(__umulhi(static_cast<uint32_t>(i), inv)); };
+  // candidate i of list `list` of beam k
+  auto total_of = [&](int k, bool first, uint64_t u) {
     Merged c = {0, 0xffffffffu};
     if (mode[k] == 1) {
-      if (s == 0 && i == 0) {
+      if (first) {
         c.key = order_key64(static_cast<double>(score[k]));
         c.at = static_cast<uint32_t>(k) * static_cast<uint32_t>(p.V) + static_cast<uint32_t>(p.pad);
       }
-    } else if (mode[k] == 0 && i < p.n) {
-      const uint64_t u = cand[static_cast<int64_t>(list) * p.n + i];
-      if (u != 0) {
-        c.key = order_key64(static_cast<double>(score[k]) + (static_cast<double>(key_value(static_cast<uint32_t>(u >> 32))) - top[k] - ln[k]));
-        c.at = static_cast<uint32_t>(k) * static_cast<uint32_t>(p.V) + ~static_cast<uint32_t>(u);
-      }
+    } else if (mode[k] == 0 && u != 0) {
+      c.key = order_key64(static_cast<double>(score[k]) + (static_cast<double>(key_value(static_cast<uint32_t>(u >> 32))) - top[k] - ln[k]));
+      c.at = static_cast<uint32_t>(k) * static_cast<uint32_t>(p.V) + ~static_cast<uint32_t>(u);
     }
     return c;
   };
-  auto emit = [&](int j, const Merged& c) {   // c.key 0: a place without a candidate
+  bool ranked = false;
+  if (staged) {
+    // A thread takes its candidates in the order rank, slice, beam, so that each warp sees good ones of all beams.
+    uint32_t high = 0;                        // the high word of this thread's best key
+#pragma unroll 2
+    for (int i = tid; i < all; i += kMergeThreads) {
+      const int j = div(i, lists, p.lists_inv), list = i - j * lists, s = div(list, p.K, p.beams_inv), k = list - s * p.K;
+      const int at = (k * p.S + s) * p.n + j;
+      const Merged c = total_of(k, s == 0 && j == 0, keys[at]);
+      keys[at] = c.key;
+      places[at] = c.at;
+      high = max(high, static_cast<uint32_t>(c.key >> 32));
+    }
+    // As in a slice: the t-th largest of its threads' bests of each of the `full` warps whose threads all have
+    // candidates, t full >= n; n candidates reach the least of these.
+    const int full = min(all / 32, kMergeWarps), t = full > 0 ? (p.n + full - 1) / full : 33;
+    if (warp < full && t <= 32) {
+      uint32_t left = high, at = 0;
+      for (int i = 0; i < t; ++i) {
+        at = __reduce_max_sync(0xffffffffu, left);
+        if (lane == __ffs(__ballot_sync(0xffffffffu, left == at)) - 1) left = 0;
+      }
+      if (lane == 0) warp_least[warp] = at;
+    }
+    __syncthreads();
+    uint32_t bound = t <= 32 ? 0xffffffffu : 0u;
+    for (int w = 0; w < full && t <= 32; ++w) bound = min(bound, warp_least[w]);
+    bound = max(bound, 1u);                   // none has the key 0
+    if (high >= bound)
+      for (int i = tid; i < all; i += kMergeThreads) {
+        const int j = div(i, lists, p.lists_inv), list = i - j * lists, s = div(list, p.K, p.beams_inv), k = list - s * p.K;
+        const int at = (k * p.S + s) * p.n + j;
+        const uint64_t key = keys[at];
+        if (static_cast<uint32_t>(key >> 32) < bound) continue;
+        const int o = atomicAdd(&found, 1);
+        if (o < kMergeRank) warp_list[o] = Merged{key, places[at]};
+      }
+    __syncthreads();
+    const int total = found;
+    if (total <= kMergeRank) {
+      ranked = true;
+      for (int j = total + tid; j < p.n; j += kMergeThreads) final_list[j] = Merged{0, 0xffffffffu};
+      for (int c = tid; c < total; c += kMergeThreads) {
+        const Merged me = warp_list[c];
+        int ahead = 0;
+#pragma unroll 4
+        for (int o = 0; o < total; ++o) {
+          const Merged x = warp_list[o];
+          ahead += x.key > me.key || (x.key == me.key && x.at < me.at);
+        }
+        if (ahead < p.n) final_list[ahead] = me;
+      }
+    }
+  }
+  if (!ranked) {                              // very many candidates, or very many that meet the bound
+    for (int i = tid; i < lists; i += kMergeThreads) pos[i] = 0;
+    __syncthreads();
+  }
+  auto head = [&](int list) {
+    const int i = pos[list];
+    if (i >= p.n) return Merged{0, 0xffffffffu};
+    if (staged) return Merged{keys[list * p.n + i], places[list * p.n + i]};
+    const int k = list / p.S;
+    return total_of(k, list == k * p.S && i == 0, cand[static_cast<int64_t>(list) * p.n + i]);
+  };
+  // a warp merges the lists from, from + step, ..., spread over its lanes
+  auto merge = [&](int from, int step, Merged* out) {
+    Merged mine;
+    int which;
+    auto look = [&]() {                       // the first of this lane's heads
+      mine = Merged{0, 0xffffffffu};
+      which = 0;
+      for (int l = from + lane * step; l < lists; l += 32 * step) {
+        const Merged c = head(l);
+        if (c.key > mine.key || (c.key == mine.key && c.at < mine.at)) mine = c, which = l;
+      }
+    };
+    look();
+    int j = 0;
+    for (; j < p.n; ++j) {
+      const int who = warp_first(mine);
+      if (who < 0) break;
+      if (lane == who) {
+        out[j] = mine;
+        ++pos[which];
+        look();
+      }
+      __syncwarp();
+    }
+    for (j += lane; j < p.n; j += 32) out[j] = Merged{0, 0xffffffffu};
+  };
+  if (!ranked) {
+    merge(warp, kMergeWarps, warp_list + warp * kSelMaxN);
+    __syncthreads();
+    if (warp == 0) {
+      int i = 0, j = 0;
+      const Merged* mine_list = warp_list + lane * kSelMaxN;
+      Merged mine = lane < kMergeWarps ? mine_list[0] : Merged{0, 0xffffffffu};
+      for (; j < p.n; ++j) {
+        const int who = warp_first(mine);
+        if (who < 0) break;
+        if (lane == who) {
+          final_list[j] = mine;
+          ++i;
+          mine = i < p.n ? mine_list[i] : Merged{0, 0xffffffffu};
+        }
+      }
+      for (j += lane; j < p.n; j += 32) final_list[j] = Merged{0, 0xffffffffu};
+    }
+  }
+  __syncthreads();
+  for (int j = tid; j < p.n; j += kMergeThreads) {
+    const Merged c = final_list[j];
     const int64_t o = static_cast<int64_t>(b) * p.n + j;
-    if (c.key == 0) {
+    if (c.key == 0) {                         // a place without a candidate
       p.out_scores[o] = -INFINITY;
       p.out_parent[o] = b * p.K + j % p.K;
       p.out_token[o] = p.pad;
@@ -378,73 +624,28 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
       p.out_parent[o] = b * p.K + static_cast<int>(k);
       p.out_token[o] = static_cast<int>(c.at - k * static_cast<uint32_t>(p.V));
     }
-  };
-  // a warp merges the lists warp0, warp0 + step, ... of its lanes
-  auto merge = [&](int from, int step, auto use) {
-    Merged mine = {0, 0xffffffffu};
-    int which = -1;
-    auto look = [&]() {                       // the first of this lane's heads
-      mine.key = 0;
-      mine.at = 0xffffffffu;
-      for (int l = from + lane * step; l < lists; l += 32 * step) {
-        const Merged c = head(l);
-        if (c.before(mine)) mine = c, which = l;
-      }
-    };
-    look();
-    int j = 0;
-    for (; j < p.n; ++j) {
-      Merged got;
-      const int who = warp_first(mine, &got);
-      if (who < 0) break;
-      if (lane == who) {
-        use(j, got);
-        ++pos[which];
-        look();
-      }
-      __syncwarp();
-    }
-    const Merged no = {0, 0xffffffffu};
-    for (j += lane; j < p.n; j += 32) use(j, no);
-  };
-  if (lists <= kSelOneWarp) {
-    if (warp == 0) merge(0, 1, emit);
-    return;
-  }
-  merge(warp, kMergeThreads / 32, [&](int j, const Merged& c) { warp_list[warp][j] = c; });
-  __syncthreads();
-  if (warp != 0) return;
-  int i = 0;
-  Merged mine = {0, 0xffffffffu};
-  if (lane < kMergeThreads / 32) mine = warp_list[lane][0];
-  for (int j = 0; j < p.n; ++j) {
-    Merged got;
-    const int who = warp_first(mine, &got);
-    if (who < 0) {
-      const Merged no = {0, 0xffffffffu};
-      for (j += lane; j < p.n; j += 32) emit(j, no);
-      return;
-    }
-    if (lane == who) {
-      emit(j, got);
-      ++i;
-      mine = i < p.n ? warp_list[lane][i] : Merged{0, 0xffffffffu};
-    }
   }
 }
 
-// Elements a block takes of a row, and blocks a row.  Small slices while the large ones leave SMs idle.
-inline void beam_slices(int rows, int V, int elem, int sm_count, int* pieces, int* slice, int* S) {
+// Pieces a thread takes of a row, elements a block, and blocks a row: the least of waves * (pieces + what a block costs
+// besides, about twenty pieces' time) and of the merge's work, a few of a block's pieces for each 256 candidates.
+inline void beam_slices(int rows, int K, int V, int n, int elem, int sm_count, int* pieces, int* slice, int* S) {
   const int E = 16 / elem;
-  *pieces = kSelPieces;
-  *slice = kSelThreads * E * kSelPieces;
-  // a row may begin E - 1 elements into its first piece
-  auto count = [&] { return static_cast<int>((static_cast<int64_t>(V) + E - 1 + *slice - 1) / *slice); };
-  if (static_cast<int64_t>(rows) * count() < 2 * sm_count) {
-    *pieces = kSelFewPieces;
-    *slice = kSelThreads * E * kSelFewPieces;
+  double best = 0;
+  *pieces = 0;
+  for (int c = 2; c <= kSelMaxPieces; c += 2) {
+    const int len = kSelThreads * E * c;
+    const int64_t count = (static_cast<int64_t>(V) + E - 1 + len - 1) / len;   // a row may begin E - 1 elements into its first piece
+    const int resident = std::min(5, (227 * 1024) / (c * kSelThreads * 16 + 6 * 1024));
+    const double waves = std::max(1.0, static_cast<double>(rows) * static_cast<double>(count) / (static_cast<double>(resident) * sm_count));
+    const double cost = waves * resident * (c + 20) + 2.0 * static_cast<double>(K) * static_cast<double>(count) * n / 256;
+    if (*pieces == 0 || cost < best) {
+      best = cost;
+      *pieces = c;
+      *slice = len;
+      *S = static_cast<int>(count);
+    }
   }
-  *S = count();
 }
 
 inline int beam_select_check(int B, int K, int V, int n, int dtype) {
@@ -463,7 +664,7 @@ inline int run_beam_select_workspace(int B, int K, int V, int n, int dtype, int6
   DeviceState* dev = nullptr;
   if (int rc = get_device_state(&dev)) return rc;
   int pieces, slice, S;
-  beam_slices(B * K, V, dtype == SPECQ_DTYPE_F32 ? 4 : 2, dev->sm_count, &pieces, &slice, &S);
+  beam_slices(B * K, K, V, n, dtype == SPECQ_DTYPE_F32 ? 4 : 2, dev->sm_count, &pieces, &slice, &S);
   *bytes = static_cast<int64_t>(B) * K * S * (static_cast<int64_t>(n) * 8 + 8 + 4);
   return SPECQ_OK;
 }
@@ -484,7 +685,7 @@ inline int run_beam_select(const void* logits, int64_t ld, int dtype, const floa
   DeviceState* dev = nullptr;
   if (int rc = get_device_state(&dev)) return rc;
   BeamSelectParams p = {};
-  beam_slices(B * K, V, dtype == SPECQ_DTYPE_F32 ? 4 : 2, dev->sm_count, &p.pieces, &p.slice, &p.S);
+  beam_slices(B * K, K, V, n, dtype == SPECQ_DTYPE_F32 ? 4 : 2, dev->sm_count, &p.pieces, &p.slice, &p.S);
   const int64_t lists = static_cast<int64_t>(B) * K * p.S;
   p.logits = logits; p.ld = ld; p.scores = scores; p.done = done; p.status = dev->status;
   p.cand = static_cast<uint64_t*>(workspace);
@@ -492,14 +693,20 @@ inline int run_beam_select(const void* logits, int64_t ld, int dtype, const floa
   p.part_max = reinterpret_cast<float*>(p.part_sum + lists);
   p.out_scores = out_scores; p.out_parent = out_parent; p.out_token = out_token;
   p.K = K; p.V = V; p.n = n; p.pad = pad;
+  // i (ceil(2^32 / d) d - 2^32) < i d < 2^32 for i below the number of staged candidates, 8192, and d up to 8192
+  auto inverse = [](int64_t d) { return static_cast<uint32_t>((0x100000000ll + d - 1) / d); };
+  p.lists_inv = inverse(static_cast<int64_t>(K) * p.S);
+  p.beams_inv = inverse(K);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(p.S, B * K), block(kSelThreads);
-  const size_t held = static_cast<size_t>(p.pieces) * kSelThreads * 16;   // 32 KB at most, below the 48 that need no leave
+  const int held = p.pieces * kSelThreads * 16;
   auto launch = [&](auto kern) {
+    cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), kSelMaxPieces * kSelThreads * 16);
+    if (e != cudaSuccess) return e;
     cudaLaunchConfig_t c = {};
     c.gridDim = grid;
     c.blockDim = block;
-    c.dynamicSmemBytes = held;
+    c.dynamicSmemBytes = static_cast<size_t>(held);
     c.stream = st;
     LaunchAttrs a(1);
     a.apply(c);
@@ -511,8 +718,8 @@ inline int run_beam_select(const void* logits, int64_t ld, int dtype, const floa
   else e = launch(beam_slice_kernel<__nv_bfloat16>);
   SPECQ_CUDA_TRY(e);
   const int64_t lists_b = static_cast<int64_t>(K) * p.S;
-  const int staged = lists_b * n * 8 <= kMergeSmem ? 1 : 0;
-  const int64_t smem = (staged ? lists_b * n * 8 : 0) + lists_b * 4;
+  const int staged = lists_b * n * 12 <= kMergeSmem ? 1 : 0;
+  const int64_t smem = (staged ? lists_b * n * 12 : 0) + lists_b * 4;
   if (smem > dev->max_smem_optin - 32 * 1024) return fail(SPECQ_ERR_UNSUPPORTED, "beam_select: %d beams of %d tokens", K, V);
   SPECQ_CUDA_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(beam_merge_kernel), static_cast<int>(smem)));
   cudaLaunchConfig_t cfg = {};

@@ -26,7 +26,7 @@ def beam_select(logits, scores, n=None, done=None, pad=0, beams=None):
     Returns scores' float32, parent int32 (rows) and token int32, each [B, n], best first; equal totals (in 64
     bits) by beam, then token.  A candidate of total -inf (a masked token) is never chosen: a place that is left
     without one has score -inf, token `pad` and the row b * beams + j % beams, which for j < beams is
-    the place's own.  NaN logits count as -inf, +inf ones as the largest finite number; a NaN or +inf score as -inf.
+    the place's own.  NaN logits count as -inf, +inf ones as their type's largest finite number; a NaN or +inf score as -inf.
     Up to 64 beams and n = 128."""
     return _native.beam_select(logits, scores, n, done, pad, beams)
 
