@@ -627,7 +627,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const __grid_
   }
 }
 
-// Pieces a thread takes of a row, elements a block, and blocks a row: the least of waves * (pieces + what a block costs
+// Pieces a thread takes of a row, elements a block, and blocks a row: the least of an SM's blocks * (pieces + what a block costs
 // besides, about twenty pieces' time) and of the merge's work, a few of a block's pieces for each 256 candidates.
 inline void beam_slices(int rows, int K, int V, int n, int elem, int sm_count, int* pieces, int* slice, int* S) {
   const int E = 16 / elem;
@@ -636,9 +636,8 @@ inline void beam_slices(int rows, int K, int V, int n, int elem, int sm_count, i
   for (int c = 2; c <= kSelMaxPieces; c += 2) {
     const int len = kSelThreads * E * c;
     const int64_t count = (static_cast<int64_t>(V) + E - 1 + len - 1) / len;   // a row may begin E - 1 elements into its first piece
-    const int resident = std::min(5, (227 * 1024) / (c * kSelThreads * 16 + 6 * 1024));
-    const double waves = std::max(1.0, static_cast<double>(rows) * static_cast<double>(count) / (static_cast<double>(resident) * sm_count));
-    const double cost = waves * resident * (c + 20) + 2.0 * static_cast<double>(K) * static_cast<double>(count) * n / 256;
+    const double per_sm = std::max(1.0, static_cast<double>(rows) * static_cast<double>(count) / sm_count);
+    const double cost = per_sm * (c + 20) + 2.0 * static_cast<double>(K) * static_cast<double>(count) * n / 256;
     if (*pieces == 0 || cost < best) {
       best = cost;
       *pieces = c;
