@@ -8,16 +8,20 @@
 // Row i of n stands at place ctx_len - n + i and sees the tokens up to it.  A row with a NaN or an infinity adds
 // nothing, nor does a token of a page outside the cache get anything.
 //
-// The products run on the tensor cores with the tokens on M: the keys' bytes go from global memory into the
-// registers of the thread that the A fragment wants them in (the order of the elements along D is free as long as q
-// has the same), are widened to fp16 there, exactly, and stay for all rows; q stands in shared memory as fp16 (bf16
-// rows times a power of two that brings their largest element to 2^14: exact down to 2^-31 of it).  Scores,
-// maxima and sums are fp32, nothing is rounded in between.
+// The products run on the tensor cores, rows on M and tokens on N.  A warp takes 32 tokens at a time: each lane copies
+// the bytes that the B fragments want in it to shared memory (asynchronously, 16 at a time; nobody else reads them), and
+// widens them to fp16 in its registers, exactly; the order of the elements along D is free as long as q has the
+// same.  q stands in shared memory as fp16 (bf16 rows times a power of two that brings their largest element to
+// 2^14: exact down to 2^-31 of it).  A thread has two rows and eight tokens of a product, so a row's maximum and sum over
+// 32 tokens and a token's sum over rows are nearly all its own.  Scores, maxima and sums are fp32, nothing is
+// rounded in between.
 //
-// A column needs its rows' sums over all tokens first.  Where one cluster of blocks holds the whole context,
-// the blocks exchange their maxima and sums through distributed shared memory and each key is read once;
-// else a first launch leaves each tile's maxima and sums, a second joins them, and a third makes the
-// products again.  No atomics: a token's sum is one thread's, over the rows in their order.
+// A column needs its rows' sums over all tokens first.  Where a cluster of up to 8 blocks of 512 tokens holds the whole
+// table, the blocks exchange their maxima and sums through distributed shared memory and each key is read from
+// HBM once; up to 16 rows the scores stay in registers, more rows' products are made again from the keys in shared
+// memory.  For longer tables a first launch leaves each block's maxima and sums (and, up to 16 rows, the scores: 8 bytes a row and
+// token against D for reading the key again), and a later one takes the sums.  No atomics: a token's sum is made
+// in a fixed order.
 #pragma once
 
 #include "block_cache.cuh"
@@ -26,8 +30,11 @@ namespace specq {
 
 constexpr int kMassThreads = 256;
 constexpr int kMassWarps = kMassThreads / 32;
-constexpr int kMassTile = 32 * kMassWarps;   // tokens of a block
-constexpr int kMassRows = 128;               // rows of q in shared memory at a time
+constexpr int kMassTiles = 2;                // tiles of 32 tokens that a warp takes of a block's
+constexpr int kMassChunk = 32 * kMassWarps * kMassTiles;   // tokens of a block
+constexpr int kMassFew = 16;                 // rows of one product
+constexpr int kMassRows = 128;               // rows of q in shared memory at a time where there are more
+constexpr int kMassCluster = 8;              // blocks that share their sums
 constexpr float kLog2E = 1.44269504f;
 
 struct MassParams {
@@ -38,11 +45,12 @@ struct MassParams {
   const int32_t* ctx;
   const int32_t* n_rows;   // optional [B]
   float* mass;             // [B, H_KV, N]
-  float2* stats;           // workspace [B, H_KV, tiles, rows]: maximum (of score log2 e) and sum
-  float* lse;              // workspace [B, H_KV, rows], log2
+  float2* stats;           // workspace [B, H_KV, chunks, rows]: maximum (of score log2 e) and sum
+  float* lse;              // workspace [B, H_KV, rows], log2 (more than 16 rows)
+  float* score;            // workspace [B, H_KV, rows, chunks * kMassChunk], times log2 e (up to 16 rows)
   int* status;
   int64_t q_sb, q_st, q_sh, kv_sp, kv_so, kv_sh, s_sp, s_sh, bt_sb, m_sb, m_sh;
-  int q_len, group, h_kv, page_log2, n_pages, bt_cols, tiles, rows;   // rows = q_len * group
+  int q_len, group, h_kv, page_log2, n_pages, bt_cols, chunks, rows;   // rows = q_len * group
   float sm_log2, decay;
 };
 
@@ -77,61 +85,16 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// One row of q to fp16 in shared memory, by a warp; *factor: what its scores are to be multiplied by.
-// Returns whether every element is finite (else the row is zeros).
-template <bool BF, int D>
-__device__ __forceinline__ bool mass_query_row(const void* src, __half* dst, float* factor, int lane) {
-  constexpr int E = D / 32;
-  float v[E], top = 0.f;
-  bool finite = true;
-  if constexpr (BF) {
-    const __nv_bfloat16* s = static_cast<const __nv_bfloat16*>(src) + lane * E;
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const __nv_bfloat162 u = *reinterpret_cast<const __nv_bfloat162*>(s + i);
-      v[i] = __low2float(u);
-      v[i + 1] = __high2float(u);
-    }
-  } else {
-    const __half* s = static_cast<const __half*>(src) + lane * E;
-#pragma unroll
-    for (int i = 0; i < E; i += 2) {
-      const __half2 u = *reinterpret_cast<const __half2*>(s + i);
-      v[i] = __low2float(u);
-      v[i + 1] = __high2float(u);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    finite = finite && fabsf(v[i]) < INFINITY;
-    top = fmaxf(top, fabsf(v[i]));
-  }
-  finite = __all_sync(0xffffffffu, finite);
-  *factor = 1.f;
-  if constexpr (BF) {
-    top = warp_max_f32(top);
-    // top 2^k in [2^14, 2^15); 2^126 suffices for what is not zero beside any key
-    const int k = top > 0.f && finite ? min(14 - ilogbf(top), 126) : 0;
-    const float up = __int_as_float((127 + k) << 23);            // k >= 14 - 127
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] *= up;
-    *factor = __int_as_float((127 - k) << 23);
-  }
-#pragma unroll
-  for (int i = 0; i < E; i += 2)
-    *reinterpret_cast<__half2*>(dst + lane * E + i) = finite ? __floats2half2_rn(v[i], v[i + 1]) : __floats2half2_rn(0.f, 0.f);
-  return finite;
-}
-
-template <int D>
+template <int D, int ROWS>
 struct MassSmem {
   static constexpr int kQStride = D + 8;     // halves: 16 more bytes a row put a quarter-warp's reads on all banks
-  __half q[kMassRows * kQStride];
-  float2 part[kMassWarps][kMassRows];        // each warp's maximum and sum for a row
-  float2 all[kMassRows];                     // the block's
-  float lse[kMassRows];
-  float factor[kMassRows];
-  int lim[kMassRows];                        // the last token that a row sees; -1: none
+  uint4 keys[kMassTiles][kMassWarps][D / 16][32];   // the 16-byte pieces of a lane: its token of eight, n-tile by n-tile
+  __half q[ROWS * kQStride];
+  float2 part[kMassWarps][ROWS];             // each warp's maximum and sum for a row
+  float2 all[ROWS];                          // the block's
+  float lse[ROWS];
+  float factor[ROWS];
+  int lim[ROWS];                             // the last token that a row sees; -1: none
 };
 
 __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
@@ -139,234 +102,467 @@ __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
   if (m == -INFINITY) return make_float2(-INFINITY, 0.f);
   return make_float2(m, a.y * exp2_fast(a.x - m) + b.y * exp2_fast(b.x - m));
 }
+// log2 of a row's sum; +inf where it has none, so that exp2(s - lse) is 0
+__device__ __forceinline__ float stats_lse(float2 x) { return x.y > 0.f ? x.x + log2f(x.y) : INFINITY; }
 
-template <bool BF, int CT, int D, int MODE>
-__global__ void __launch_bounds__(kMassThreads, 2) mass_kernel(const __grid_constant__ MassParams p) {
-  using Smem = MassSmem<D>;
+// What a sequence has: tokens (within its table) and counted rows; 0 rows: its mass stays.
+__device__ __forceinline__ void mass_extent(const MassParams& p, int b, bool tell, int& n, int& nr) {
+  n = p.ctx[b];
+  const int most = p.bt_cols << p.page_log2;
+  if (n > most) {
+    if (tell) report_status(p.status, SPECQ_STATUS_PLAN_CLAMPED);
+    n = most;
+  }
+  nr = n <= 0 ? 0 : p.n_rows == nullptr ? p.q_len : min(max(p.n_rows[b], 0), p.q_len);
+}
+
+// `here` rows of q from row `first` of the KV head, padded with zeros to PAD, to fp16 in shared memory; their factors and limits.
+template <bool BF, int D, int ROWS, typename Smem>
+__device__ __forceinline__ void mass_queries(const MassParams& p, Smem& sm, int b, int h, int first, int here, int pad, int base) {
+  constexpr int kPieces = D / 8, kLanes = kMassThreads / ROWS < kPieces ? kMassThreads / ROWS : kPieces, kMine = D / kLanes;   // threads of a row, elements of each
+  const int tid = static_cast<int>(threadIdx.x);
+  for (int i = tid; i < pad * kPieces; i += kMassThreads) {
+    const int r = i / kPieces, c = i - r * kPieces;
+    __half* dst = sm.q + r * Smem::kQStride + c * 8;
+    if (r < here) {
+      const int row = (first + r) / p.group, head = h * p.group + (first + r) - row * p.group;
+      const int64_t at = (p.q_sb != 0 ? b * p.q_sb + row * p.q_st : (static_cast<int64_t>(b) * p.q_len + row) * p.q_st) + head * p.q_sh;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(static_cast<const __half*>(p.q) + at + c * 8) : "memory");
+    } else {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  const int r = tid / kLanes, lane = tid - r * kLanes;
+  if (r < pad) {                       // (pad is a multiple of 16 rows: whole warps)
+    uint4* at = reinterpret_cast<uint4*>(sm.q + r * Smem::kQStride + lane * kMine);
+    uint32_t top = 0u;                 // the larger of the halves' magnitudes, a NaN kept
+#pragma unroll
+    for (int i = 0; i < kMine / 8; ++i) {
+      const uint4 u = at[i];
+      const uint32_t w[4] = {u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu, u.z & 0x7FFF7FFFu, u.w & 0x7FFF7FFFu};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = __vmaxu2(top, w[k]);      // magnitudes order as integers, infinity and NaN last
+    }
+    top = max(top & 0xFFFFu, top >> 16);
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool finite = top < (BF ? 0x7F80u : 0x7C00u);
+    float factor = 1.f;
+    if constexpr (BF) {
+      const float amax = __uint_as_float(top << 16);
+      // amax 2^k in [2^14, 2^15); 2^126 suffices for what is not zero beside any key
+      const int k = top != 0u && finite ? min(14 - ilogbf(amax), 126) : 0;
+      const float up = __int_as_float((127 + k) << 23);           // k >= 14 - 127
+      factor = __int_as_float((127 - k) << 23);
+#pragma unroll
+      for (int i = 0; i < kMine / 8; ++i) {
+        uint4 u = at[i];
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __half2 v = __floats2half2_rn(__uint_as_float(w[j] << 16) * up, __uint_as_float(w[j] & 0xFFFF0000u) * up);
+          w[j] = finite ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
+        }
+        at[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    } else if (!finite) {
+#pragma unroll
+      for (int i = 0; i < kMine / 8; ++i) at[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    if (lane == 0) {
+      sm.factor[r] = factor;
+      sm.lim[r] = r < here && finite ? base + (first + r) / p.group : -1;
+    }
+  }
+  __syncthreads();
+}
+
+template <bool BF, int CT, int D, int ROWS, int MODE>
+__global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_kernel(const __grid_constant__ MassParams p) {
+  using Smem = MassSmem<D, ROWS>;
+  constexpr bool kFew = ROWS == kMassFew;
+  constexpr int C = D / 64;                  // 16-byte pieces of a lane's token
   extern __shared__ __align__(16) uint8_t raw_smem[];
   Smem& sm = *reinterpret_cast<Smem*>(raw_smem);
   pdl_launch_dependents();
   pdl_wait();
-  const int tile = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int lane = static_cast<int>(threadIdx.x & 31), warp = static_cast<int>(threadIdx.x >> 5);
   const int g = lane >> 2, tq = lane & 3;
-  int n = p.ctx[b];
-  const int most = p.bt_cols << p.page_log2;
-  if (n > most) {
-    if (tile == 0 && h == 0 && threadIdx.x == 0) report_status(p.status, SPECQ_STATUS_PLAN_CLAMPED);
-    n = most;
-  }
-  const int nr = p.n_rows == nullptr ? p.q_len : min(max(p.n_rows[b], 0), p.q_len);
-  const bool idle = n <= 0 || nr == 0 || tile * kMassTile >= n;
-  // (a cluster's blocks stay together: an idle one still takes part in the barriers)
-  if (MODE != kMassWhole && idle) return;
-
-  // this lane's four tokens of the warp's 32: page, scale, keys
-  constexpr int C = D / 64;
-  uint32_t a[2][C][4][4];
-  float tscale[2][2];
-  int tok[2][2];             // a token that no row sees: INT_MAX
-  const int t0 = tile * kMassTile + warp * 32;
-  bool good = true;
-  {
-    uint4 w[2][2][C];
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int t = t0 + mt * 16 + half * 8 + g;
-        tok[mt][half] = INT_MAX;
-        tscale[mt][half] = 0.f;
-#pragma unroll
-        for (int c = 0; c < C; ++c) w[mt][half][c] = make_uint4(0u, 0u, 0u, 0u);
-        if (!idle && t < n) {
-          const int pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
-          if (pg >= 0 && pg < p.n_pages) {
-            tok[mt][half] = t;
-            const uint8_t* k = p.kc + pg * p.kv_sp + (t & ((1 << p.page_log2) - 1)) * p.kv_so + h * p.kv_sh + tq * 16;
-#pragma unroll
-            for (int c = 0; c < C; ++c) w[mt][half][c] = *reinterpret_cast<const uint4*>(k + c * 64);
-            tscale[mt][half] = p.ks[pg * p.s_sp + h * p.s_sh] * p.sm_log2;
-          } else {
-            report_status(p.status, SPECQ_STATUS_BAD_INDEX);
-            good = false;
-          }
-        } else {
-          good = false;
-        }
-      }
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const uint32_t* u = reinterpret_cast<const uint32_t*>(&w[mt][0][c]);
-        const uint32_t* v = reinterpret_cast<const uint32_t*>(&w[mt][1][c]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          widen4<CT>(u[j], a[mt][c][j][0], a[mt][c][j][2]);
-          widen4<CT>(v[j], a[mt][c][j][1], a[mt][c][j][3]);
-        }
-      }
-  }
-  const int base = n - nr;
-  good = __all_sync(0xffffffffu, good);
-  float weight[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+  int n, nr;
+  mass_extent(p, b, chunk == 0 && h == 0 && threadIdx.x == 0 && MODE != kMassWeights, n, nr);
+  // A block without tokens leaves; a cluster's barriers count only the threads that have not left, and no
+  // block looks at the sums of one that has no tokens.
+  if (nr == 0 || chunk * kMassChunk >= n) return;
   const int64_t bh = static_cast<int64_t>(b) * p.h_kv + h;
-  const int rows = nr * p.group;
 
-  // scores of eight rows from `r0` of the block, times log2 e; -inf where a row does not see a token
-  auto scores = [&](int r0, float (&s)[2][4]) {
+  // This warp's tiles: a page for each n-tile of eight tokens (a page holds eight or more), its scale, the lane's keys.
+  int t0[kMassTiles];
+  float tscale[kMassTiles][4];
+  uint32_t bad[kMassTiles];                  // bit j: n-tile j is of no page
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+  for (int i = 0; i < kMassTiles; ++i) {
+    t0[i] = chunk * kMassChunk + (i * kMassWarps + warp) * 32;
+    bad[i] = 0u;
+    int pg = -1;
+    float sc = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[mt][i] = 0.f;
-    const __half* qrow = sm.q + (r0 + g) * Smem::kQStride + tq * 16;
+    for (int j = 0; j < 4; ++j) {
+      const int t = t0[i] + j * 8;
+      uint4* dst = &sm.keys[i][warp][j * C][lane];
+      if (j == 0 || (t & ((1 << p.page_log2) - 1)) == 0) {      // another page
+        pg = -1;
+        sc = 0.f;
+        if (t < n) {
+          pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
+          if (pg < 0 || pg >= p.n_pages) {
+            if (lane == 0) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+            pg = -1;
+          } else {
+            sc = p.ks[pg * p.s_sp + h * p.s_sh] * p.sm_log2;
+          }
+        }
+      }
+      tscale[i][j] = sc;
+      if (pg < 0 || t >= n) bad[i] |= 1u << j;
+      if (pg >= 0 && t + g < n) {
+        const uint8_t* k = p.kc + pg * p.kv_sp + ((t + g) & ((1 << p.page_log2) - 1)) * p.kv_so + h * p.kv_sh + tq * 16;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + c * 32)), "l"(k + c * 64) : "memory");
+      } else {
+#pragma unroll
+        for (int c = 0; c < C; ++c) dst[c * 32] = make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
+  }
+  const int base = n - nr, rows = nr * p.group;
+  const int active = min((n - 1) / kMassChunk + 1, static_cast<int>(gridDim.x));   // of this sequence's blocks
+  float weight[kMassTiles][4][2];            // of this thread's tokens, over its rows
+#pragma unroll
+  for (int i = 0; i < kMassTiles; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) weight[i][j][0] = weight[i][j][1] = 0.f;
+
+  // Fragments of q for rows r0 + g and r0 + g + 8.
+  auto fragments = [&](int r0, uint32_t (&a)[C][4][4]) {
+    const __half* lo = sm.q + (r0 + g) * Smem::kQStride + tq * 16;
+    const __half* hi = lo + 8 * Smem::kQStride;
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
-        const uint4 u = *reinterpret_cast<const uint4*>(qrow + c * 64 + jj * 8);
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-          mma_f16(s[mt], a[mt][c][2 * jj], u.x, u.y);
-          mma_f16(s[mt], a[mt][c][2 * jj + 1], u.z, u.w);
-        }
+        const uint4 u = *reinterpret_cast<const uint4*>(lo + c * 64 + jj * 8), v = *reinterpret_cast<const uint4*>(hi + c * 64 + jj * 8);
+        a[c][2 * jj][0] = u.x; a[c][2 * jj][1] = v.x; a[c][2 * jj][2] = u.y; a[c][2 * jj][3] = v.y;
+        a[c][2 * jj + 1][0] = u.z; a[c][2 * jj + 1][1] = v.z; a[c][2 * jj + 1][2] = u.w; a[c][2 * jj + 1][3] = v.w;
       }
-    const float f0 = sm.factor[r0 + 2 * tq], f1 = sm.factor[r0 + 2 * tq + 1];
+  };
+  auto widen = [&](int i, int j, uint32_t (&k)[C][4][2]) {
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        // a NaN among the keys weighs nothing
-        s[mt][2 * half] = fmaxf(s[mt][2 * half] * tscale[mt][half] * (BF ? f0 : 1.f), -INFINITY);
-        s[mt][2 * half + 1] = fmaxf(s[mt][2 * half + 1] * tscale[mt][half] * (BF ? f1 : 1.f), -INFINITY);
-      }
-    if (!good || t0 + 31 > base) {
-      const int l0 = sm.lim[r0 + 2 * tq], l1 = sm.lim[r0 + 2 * tq + 1];
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          if (tok[mt][half] > l0) s[mt][2 * half] = -INFINITY;
-          if (tok[mt][half] > l1) s[mt][2 * half + 1] = -INFINITY;
-        }
+    for (int c = 0; c < C; ++c) {
+      const uint4 u = sm.keys[i][warp][j * C + c][lane];
+      widen4<CT>(u.x, k[c][0][0], k[c][0][1]);
+      widen4<CT>(u.y, k[c][1][0], k[c][1][1]);
+      widen4<CT>(u.z, k[c][2][0], k[c][2][1]);
+      widen4<CT>(u.w, k[c][3][0], k[c][3][1]);
     }
   };
-
-  for (int first = 0; first < rows; first += kMassRows) {
-    const int here = min(kMassRows, rows - first), padded = (here + 7) & ~7;
-    if (first > 0) __syncthreads();
-    for (int r = warp; r < padded; r += kMassWarps) {
-      __half* dst = sm.q + r * Smem::kQStride;
-      if (r < here) {
-        const int i = (first + r) / p.group, head = h * p.group + (first + r) - i * p.group;
-        const int64_t at = (p.q_sb != 0 ? b * p.q_sb + i * p.q_st : (static_cast<int64_t>(b) * p.q_len + i) * p.q_st) + head * p.q_sh;
-        float factor;
-        const bool finite = mass_query_row<BF, D>(static_cast<const __half*>(p.q) + at, dst, &factor, lane);
-        if (lane == 0) {
-          sm.factor[r] = factor;
-          sm.lim[r] = finite ? base + i : -1;
-        }
-      } else {
-        for (int e = lane * 2; e < D; e += 64) *reinterpret_cast<uint32_t*>(dst + e) = 0u;
-        if (lane == 0) {
-          sm.factor[r] = 1.f;
-          sm.lim[r] = -1;
+  auto product = [&](const uint32_t (&a)[C][4][4], const uint32_t (&k)[C][4][2], float (&s)[4]) {
+    s[0] = s[1] = s[2] = s[3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int jj = 0; jj < 4; ++jj) mma_f16(s, a[c][jj], k[c][jj][0], k[c][jj][1]);
+  };
+  // s: rows r0 + g (0, 1) and r0 + g + 8 (2, 3), tokens 8 j + 2 tq + 0, 1, times log2 e; -inf where a row does not see a token
+  auto scale = [&](int i, int r0, float (&s)[4][4]) {
+    const float f0 = BF ? sm.factor[r0 + g] : 1.f, f1 = BF ? sm.factor[r0 + g + 8] : 1.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = tscale[i][j] * f0, y = tscale[i][j] * f1;
+      s[j][0] *= x; s[j][1] *= x;
+      s[j][2] *= y; s[j][3] *= y;
+    }
+    if (bad[i] != 0u || t0[i] + 31 > base) {
+      const int l0 = sm.lim[r0 + g], l1 = sm.lim[r0 + g + 8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = bad[i] >> j & 1u ? INT_MAX - 1 : t0[i] + j * 8 + 2 * tq;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (t + e > l0) s[j][e] = -INFINITY;
+          if (t + e > l1) s[j][2 + e] = -INFINITY;
         }
       }
     }
-    if constexpr (MODE == kMassWeights)
-      for (int r = threadIdx.x; r < padded; r += kMassThreads) sm.lse[r] = r < here ? p.lse[bh * p.rows + first + r] : INFINITY;
+  };
+  // a row's maximum and sum over this thread's eight tokens, then over the quad's 32
+  auto row_stats = [&](const float (&s)[4][4], int e) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(s[j][e], s[j][e + 1]));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const float z = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) l += exp2_fast(s[j][e] - z) + exp2_fast(s[j][e + 1] - z);
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    return make_float2(m, l);
+  };
+  auto add_weights = [&](int i, int r0, const float (&s)[4][4]) {
+    const float l0 = sm.lse[r0 + g], l1 = sm.lse[r0 + g + 8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        weight[i][j][e] += exp2_fast(s[j][e] - l0) + exp2_fast(s[j][2 + e] - l1);
+  };
+  // the warps' sums to the block's, and (a cluster) the blocks' to lse
+  auto block_stats = [&](int first, int here, int pad) {
     __syncthreads();
-    if constexpr (MODE != kMassWeights) {
-      for (int r0 = 0; r0 < padded; r0 += 8) {
-        float s[2][4];
-        scores(r0, s);
-        float m0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2]));
-        float m1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+    for (int r = threadIdx.x; r < pad; r += kMassThreads) {
+      float2 x = make_float2(-INFINITY, 0.f);
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-          m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+      for (int w = 0; w < kMassWarps; ++w) x = join_stats(x, sm.part[w][r]);
+      if (sm.lim[r] < 0) x = make_float2(-INFINITY, 0.f);
+      if (MODE == kMassStats) {
+        if (r < here) p.stats[(bh * p.chunks + chunk) * p.rows + first + r] = x;
+      } else {
+        sm.all[r] = x;
+      }
+    }
+    if (MODE != kMassWhole) return;
+    if (active == 1) {
+      __syncthreads();
+      for (int r = threadIdx.x; r < pad; r += kMassThreads) sm.lse[r] = stats_lse(sm.all[r]);
+    } else {
+      cluster_sync();
+      for (int r = threadIdx.x; r < pad; r += kMassThreads) {
+        const uint32_t mine = smem_u32(&sm.all[r]);
+        float2 x = make_float2(-INFINITY, 0.f);
+#pragma unroll 4
+        for (int c = 0; c < active; ++c) {
+          const uint32_t at = dsmem_map(mine, static_cast<uint32_t>(c));
+          x = join_stats(x, make_float2(dsmem_ld_f32(at), dsmem_ld_f32(at + 4)));
         }
-        const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
-        float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            l0 += exp2_fast(s[mt][2 * half] - z0);
-            l1 += exp2_fast(s[mt][2 * half + 1] - z1);
-          }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          l0 += __shfl_xor_sync(0xffffffffu, l0, o);
-          l1 += __shfl_xor_sync(0xffffffffu, l1, o);
-        }
-        if (g == 0) {
-          sm.part[warp][r0 + 2 * tq] = make_float2(m0, l0);
-          sm.part[warp][r0 + 2 * tq + 1] = make_float2(m1, l1);
-        }
+        sm.lse[r] = stats_lse(x);
       }
       __syncthreads();
-      for (int r = threadIdx.x; r < padded; r += kMassThreads) {
-        float2 x = make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int w = 0; w < kMassWarps; ++w) x = join_stats(x, sm.part[w][r]);
-        if (sm.lim[r] < 0) x = make_float2(-INFINITY, 0.f);
-        if (MODE == kMassStats) {
-          if (r < here) p.stats[(bh * p.tiles + tile) * p.rows + first + r] = x;
-        } else {
-          sm.lse[r] = x.y > 0.f ? x.x + log2f(x.y) : INFINITY;   // +inf: exp2(s - lse) is 0
-        }
-      }
-      if (MODE == kMassWhole) __syncthreads();
+      cluster_arrive();                       // this block has read its peers' sums (waited for before `all` is written again, and at the end)
+      return;
     }
-    if constexpr (MODE != kMassStats) {
-      for (int r0 = 0; r0 < padded; r0 += 8) {
-        float s[2][4];
-        scores(r0, s);
-        const float l0 = sm.lse[r0 + 2 * tq], l1 = sm.lse[r0 + 2 * tq + 1];
+    __syncthreads();
+  };
+
+  if constexpr (kFew) {
+    mass_queries<BF, D, ROWS>(p, sm, b, h, 0, rows, kMassFew, base);   // (its wait is for the keys too)
+    const bool half = rows <= 8;              // rows 8 to 15 are padding
+    float s[kMassTiles][4][4];
+    if (t0[0] < n) {                          // (a warp's first tile is the one that has tokens if any has)
+      uint32_t a[C][4][4];
+      fragments(0, a);
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+      for (int i = 0; i < kMassTiles; ++i) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half)
-            weight[mt][half] += exp2_fast(s[mt][2 * half] - l0) + exp2_fast(s[mt][2 * half + 1] - l1);
+        for (int j = 0; j < 4; ++j) {
+          uint32_t k[C][4][2];
+          widen(i, j, k);
+          product(a, k, s[i][j]);
+        }
+        scale(i, 0, s[i]);
+      }
+    }
+    float top[2] = {0.f, 0.f};                // a quad's largest score of rows g and g + 8: whole, the scores become 2^(s - top)
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      float2 x = make_float2(-INFINITY, 0.f);
+      if (t0[0] < n && !(half && e == 2)) {
+#pragma unroll
+        for (int i = 0; i < kMassTiles; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x.x = fmaxf(x.x, fmaxf(s[i][j][e], s[i][j][e + 1]));
+        x.x = fmaxf(x.x, __shfl_xor_sync(0xffffffffu, x.x, 1));
+        x.x = fmaxf(x.x, __shfl_xor_sync(0xffffffffu, x.x, 2));
+        const float z = x.x == -INFINITY ? 0.f : x.x;
+        top[e / 2] = z;
+#pragma unroll
+        for (int i = 0; i < kMassTiles; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float u = exp2_fast(s[i][j][e] - z), v = exp2_fast(s[i][j][e + 1] - z);
+            x.y += u + v;
+            if constexpr (MODE == kMassWhole) s[i][j][e] = u, s[i][j][e + 1] = v;
+          }
+        x.y += __shfl_xor_sync(0xffffffffu, x.y, 1);
+        x.y += __shfl_xor_sync(0xffffffffu, x.y, 2);
+      }
+      if (tq == 0) sm.part[warp][g + 4 * e] = x;
+    }
+    if constexpr (MODE == kMassStats) {       // the scores stay for the second launch
+      if (t0[0] < n)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const int r = g + 4 * e;
+          if (r < rows) {
+            float* at = p.score + (bh * p.rows + r) * (static_cast<int64_t>(p.chunks) * kMassChunk);
+#pragma unroll
+            for (int i = 0; i < kMassTiles; ++i)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(at + t0[i] + j * 8 + 2 * tq) = make_float2(s[i][j][e], s[i][j][e + 1]);
+          }
+        }
+    }
+    block_stats(0, rows, kMassFew);
+    if constexpr (MODE == kMassWhole) {
+      if (t0[0] < n) {
+        const float f0 = exp2_fast(top[0] - sm.lse[g]), f1 = exp2_fast(top[1] - sm.lse[g + 8]);
+#pragma unroll
+        for (int i = 0; i < kMassTiles; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) weight[i][j][e] = half ? s[i][j][e] * f0 : fmaf(s[i][j][2 + e], f1, s[i][j][e] * f0);
+      }
+    }
+  } else {
+    for (int first = 0; first < rows; first += kMassRows) {
+      const int here = min(kMassRows, rows - first), pad = (here + 15) & ~15;
+      if (first > 0) {
+        __syncthreads();                      // q, lim and lse are no longer read
+        if (MODE == kMassWhole && active > 1) cluster_wait();
+      }
+      mass_queries<BF, D, ROWS>(p, sm, b, h, first, here, pad, base);
+      if constexpr (MODE == kMassWeights) {
+        for (int r = threadIdx.x; r < pad; r += kMassThreads) sm.lse[r] = r < here ? p.lse[bh * p.rows + first + r] : INFINITY;
+        __syncthreads();
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < kMassTiles; ++i) {
+          uint32_t k[4][C][4][2];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) widen(i, j, k[j]);
+#pragma unroll 1
+          for (int r0 = 0; r0 < pad; r0 += 16) {
+            uint32_t a[C][4][4];
+            float s[4][4];
+            fragments(r0, a);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
+            scale(i, r0, s);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const float2 x = row_stats(s, e);
+              float2* at = &sm.part[warp][r0 + g + 4 * e];
+              if (tq == 0) *at = i == 0 ? x : join_stats(*at, x);
+            }
+          }
+        }
+        block_stats(first, here, pad);
+      }
+      if constexpr (MODE != kMassStats) {
+#pragma unroll
+        for (int i = 0; i < kMassTiles; ++i) {
+          uint32_t k[4][C][4][2];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) widen(i, j, k[j]);
+#pragma unroll 1
+          for (int r0 = 0; r0 < pad; r0 += 16) {
+            uint32_t a[C][4][4];
+            float s[4][4];
+            fragments(r0, a);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
+            scale(i, r0, s);
+            add_weights(i, r0, s);
+          }
+        }
       }
     }
   }
   if constexpr (MODE != kMassStats) {
-    if (idle) return;
+    // Eight tokens' sums over the eight lanes of a column, halving: lane g keeps token 8 (g >> 1) + 2 tq + (g & 1).
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int i = 0; i < kMassTiles; ++i) {
+      if (t0[i] >= n) continue;
+      float u[4], v[2];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float w = weight[mt][half];
-        w += __shfl_xor_sync(0xffffffffu, w, 1);
-        w += __shfl_xor_sync(0xffffffffu, w, 2);
-        const int t = t0 + mt * 16 + half * 8 + g;
-        if (tq == 0 && t < n) {
-          float* at = p.mass + b * p.m_sb + h * p.m_sh + t;
-          *at = fmaf(*at, p.decay, w);
-        }
+      for (int j = 0; j < 4; ++j) {           // e by bit 0 of g
+        const bool odd = g & 1;
+        u[j] = (odd ? weight[i][j][1] : weight[i][j][0]) + __shfl_xor_sync(0xffffffffu, odd ? weight[i][j][0] : weight[i][j][1], 4);
       }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {           // n-tiles 2 j, 2 j + 1 by bit 1
+        const bool odd = g & 2;
+        v[j] = (odd ? u[2 * j + 1] : u[2 * j]) + __shfl_xor_sync(0xffffffffu, odd ? u[2 * j] : u[2 * j + 1], 8);
+      }
+      const bool odd = g & 4;
+      const float w = (odd ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, odd ? v[0] : v[1], 16);
+      const int t = t0[i] + 8 * (g >> 1) + 2 * tq + (g & 1);
+      if (t < n) {
+        float* at = p.mass + b * p.m_sb + h * p.m_sh + t;
+        *at = fmaf(*at, p.decay, w);
+      }
+    }
   }
+  if (MODE == kMassWhole && active > 1) cluster_wait();   // the peers have read this block's sums
 }
 
-// log2 of each row's sum from its tiles' maxima and sums, in their order.
-__global__ void __launch_bounds__(128) mass_join_kernel(const __grid_constant__ MassParams p) {
+// log2 of each row's sum from its blocks' maxima and sums: a warp a row.
+__global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ MassParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int r = blockIdx.x * 128 + threadIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int n = min(p.ctx[b], p.bt_cols << p.page_log2);
-  const int nr = p.n_rows == nullptr ? p.q_len : min(max(p.n_rows[b], 0), p.q_len);
-  if (r >= nr * p.group || n <= 0) return;
+  const int r = blockIdx.x * 8 + static_cast<int>(threadIdx.x >> 5), lane = static_cast<int>(threadIdx.x & 31), h = blockIdx.y, b = blockIdx.z;
+  int n, nr;
+  mass_extent(p, b, false, n, nr);
+  if (r >= nr * p.group) return;
   const int64_t bh = static_cast<int64_t>(b) * p.h_kv + h;
-  const int tiles = (n + kMassTile - 1) / kMassTile;
-  const float2* at = p.stats + bh * p.tiles * p.rows + r;
+  const int chunks = (n - 1) / kMassChunk + 1;
   float2 x = make_float2(-INFINITY, 0.f);
-  for (int t = 0; t < tiles; ++t) x = join_stats(x, at[static_cast<int64_t>(t) * p.rows]);
-  p.lse[bh * p.rows + r] = x.y > 0.f ? x.x + log2f(x.y) : INFINITY;
+  for (int c = lane; c < chunks; c += 32) x = join_stats(x, p.stats[(bh * p.chunks + c) * p.rows + r]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = join_stats(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
+  if (lane == 0) p.lse[bh * p.rows + r] = stats_lse(x);
+}
+
+// Up to 16 rows, a table longer than a cluster: the sums over rows from the scores of the first launch.
+constexpr int kMassSumTokens = 4 * kMassThreads;
+__global__ void __launch_bounds__(kMassThreads) mass_sum_kernel(const __grid_constant__ MassParams p) {
+  __shared__ float lse[kMassFew];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int h = blockIdx.y, b = blockIdx.z, lane = static_cast<int>(threadIdx.x & 31), warp = static_cast<int>(threadIdx.x >> 5);
+  int n, nr;
+  mass_extent(p, b, false, n, nr);
+  if (nr == 0 || static_cast<int64_t>(blockIdx.x) * kMassSumTokens >= n) return;
+  const int64_t bh = static_cast<int64_t>(b) * p.h_kv + h;
+  const int chunks = (n - 1) / kMassChunk + 1, rows = nr * p.group;
+  for (int r = warp; r < rows; r += kMassWarps) {
+    float2 x = make_float2(-INFINITY, 0.f);
+    for (int c = lane; c < chunks; c += 32) x = join_stats(x, p.stats[(bh * p.chunks + c) * p.rows + r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = join_stats(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
+    if (lane == 0) lse[r] = stats_lse(x);
+  }
+  __syncthreads();
+  const int64_t width = static_cast<int64_t>(p.chunks) * kMassChunk;
+  const float* score = p.score + bh * p.rows * width;
+  const int t = static_cast<int>(blockIdx.x) * kMassSumTokens + static_cast<int>(threadIdx.x);
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    const float l = lse[r];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (t + i * kMassThreads < n) w[i] += exp2_fast(score[r * width + t + i * kMassThreads] - l);
+  }
+  float* at = p.mass + b * p.m_sb + h * p.m_sh + t;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (t + i * kMassThreads < n) at[i * kMassThreads] = fmaf(at[i * kMassThreads], p.decay, w[i]);
 }
 
 inline int mass_check(int B, int q_len, int H, int H_KV, int D, int page, int bt_cols) {
@@ -375,7 +571,7 @@ inline int mass_check(int B, int q_len, int H, int H_KV, int D, int page, int bt
     return fail(SPECQ_ERR_INVALID_ARG, "%s: B=%d q_len=%d H=%d H_KV=%d bt_cols=%d", who, B, q_len, H, H_KV, bt_cols);
   if (D != 64 && D != 128) return fail(SPECQ_ERR_UNSUPPORTED, "%s: head_dim %d (64 or 128)", who, D);
   if (page < 8 || page > 128 || (page & (page - 1))) return fail(SPECQ_ERR_UNSUPPORTED, "%s: page %d (a power of two, 8 to 128)", who, page);
-  if (B > 65535 || H_KV > 65535 || static_cast<int64_t>(bt_cols) * page > 0x7ffffeffll || static_cast<int64_t>(q_len) * (H / H_KV) > 0x7fffff00ll)
+  if (B > 65535 || H_KV > 65535 || static_cast<int64_t>(bt_cols) * page > 0x7ffff000ll || static_cast<int64_t>(q_len) * (H / H_KV) > 0x7fffff00ll)
     return fail(SPECQ_ERR_UNSUPPORTED, "%s: B=%d H_KV=%d, %d pages of %d, %d rows of %d heads", who, B, H_KV, bt_cols, page, q_len, H / H_KV);
   return SPECQ_OK;
 }
@@ -383,9 +579,10 @@ inline int mass_check(int B, int q_len, int H, int H_KV, int D, int page, int bt
 inline int run_attention_mass_workspace(int B, int q_len, int H, int H_KV, int D, int page, int bt_cols, int64_t* bytes) {
   if (bytes == nullptr) return fail(SPECQ_ERR_INVALID_ARG, "attention_mass_workspace: null pointer");
   if (int rc = mass_check(B, q_len, H, H_KV, D, page, bt_cols)) return rc;
-  const int tiles = ceil_div(bt_cols * page, kMassTile);
+  const int chunks = ceil_div(bt_cols * page, kMassChunk);
   const int64_t rows = static_cast<int64_t>(B) * H_KV * q_len * (H / H_KV);
-  *bytes = tiles > 1 ? rows * tiles * 8 + rows * 4 : 0;
+  const bool few = q_len * (H / H_KV) <= kMassFew;
+  *bytes = chunks <= kMassCluster ? 0 : rows * chunks * 8 + (few ? rows * chunks * kMassChunk * 4 : rows * 4);
   return SPECQ_OK;
 }
 
@@ -416,35 +613,46 @@ inline int run_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t
   p.q_sb = q_sb; p.q_st = q_st; p.q_sh = q_sh; p.kv_sp = kv_sp; p.kv_so = kv_so; p.kv_sh = kv_sh; p.s_sp = s_sp; p.s_sh = s_sh;
   p.bt_sb = bt_sb; p.m_sb = m_sb; p.m_sh = m_sh;
   p.q_len = q_len; p.group = H / H_KV; p.h_kv = H_KV; p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
-  p.n_pages = n_pages; p.bt_cols = bt_cols; p.tiles = ceil_div(bt_cols * page, kMassTile); p.rows = q_len * p.group;
+  p.n_pages = n_pages; p.bt_cols = bt_cols; p.chunks = ceil_div(bt_cols * page, kMassChunk); p.rows = q_len * p.group;
   p.sm_log2 = sm_scale * kLog2E; p.decay = decay;
   p.stats = static_cast<float2*>(workspace);
-  p.lse = reinterpret_cast<float*>(p.stats + (p.tiles > 1 ? static_cast<int64_t>(B) * H_KV * p.tiles * p.rows : 0));
+  p.score = p.lse = reinterpret_cast<float*>(p.stats + (need > 0 ? static_cast<int64_t>(B) * H_KV * p.chunks * p.rows : 0));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(p.tiles, H_KV, B);
+  const bool whole = p.chunks <= kMassCluster;
   auto launch = [&](auto kern, size_t smem) {
-    const cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), static_cast<int>(smem));
+    int cluster = 1;
+    cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), static_cast<int>(smem));
     if (e != cudaSuccess) return e;
+    if (whole) cluster = next_pow2(p.chunks);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
+    cfg.gridDim = dim3(whole ? cluster : p.chunks, H_KV, B);
     cfg.blockDim = dim3(kMassThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    LaunchAttrs at(1);
+    LaunchAttrs at(cluster);
     at.apply(cfg);
     return cudaLaunchKernelEx(&cfg, kern, p);
   };
   auto all = [&](auto bf, auto ct, auto d) -> int {
     constexpr bool BF = decltype(bf)::value;
     constexpr int CT = decltype(ct)::value, DD = decltype(d)::value;
-    const size_t smem = sizeof(MassSmem<DD>);
-    if (p.tiles == 1) {
-      SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassWhole>, smem));
+    const size_t few = sizeof(MassSmem<DD, kMassFew>), many = sizeof(MassSmem<DD, kMassRows>);
+    if (p.rows <= kMassFew) {
+      if (whole) {
+        SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassFew, kMassWhole>, few));
+        return SPECQ_OK;
+      }
+      SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassFew, kMassStats>, few));
+      SPECQ_CUDA_TRY(launch_plain(mass_sum_kernel, dim3(ceil_div(bt_cols * page, kMassSumTokens), H_KV, B), dim3(kMassThreads), st, p));
       return SPECQ_OK;
     }
-    SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassStats>, smem));
-    SPECQ_CUDA_TRY(launch_plain(mass_join_kernel, dim3(ceil_div(p.rows, 128), H_KV, B), dim3(128), st, p));
-    SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassWeights>, smem));
+    if (whole) {
+      SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassRows, kMassWhole>, many));
+      return SPECQ_OK;
+    }
+    SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassRows, kMassStats>, many));
+    SPECQ_CUDA_TRY(launch_plain(mass_join_kernel, dim3(ceil_div(p.rows, 8), H_KV, B), dim3(256), st, p));
+    SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassRows, kMassWeights>, many));
     return SPECQ_OK;
   };
   auto by_d = [&](auto bf, auto ct) { return D == 64 ? all(bf, ct, std::integral_constant<int, 64>{}) : all(bf, ct, std::integral_constant<int, 128>{}); };
