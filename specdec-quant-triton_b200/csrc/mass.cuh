@@ -34,7 +34,9 @@ constexpr int kMassTiles = 2;                // tiles of 32 tokens that a warp t
 constexpr int kMassChunk = 32 * kMassWarps * kMassTiles;   // tokens of a block
 constexpr int kMassFew = 16;                 // rows of one product
 constexpr int kMassRows = 128;               // rows of q in shared memory at a time where there are more
+constexpr int kMassStages = 2;               // tiles of a warp on their way, up to 16 rows
 constexpr int kMassCluster = 8;              // blocks that share their sums
+constexpr int kMassSms = 148;                // how a call is cut does not ask the device: its workspace is known without one
 constexpr float kLog2E = 1.44269504f;
 
 struct MassParams {
@@ -47,10 +49,11 @@ struct MassParams {
   float* mass;             // [B, H_KV, N]
   float2* stats;           // workspace [B, H_KV, chunks, rows]: maximum (of score log2 e) and sum
   float* lse;              // workspace [B, H_KV, rows], log2 (more than 16 rows)
-  float* score;            // workspace [B, H_KV, rows, chunks * kMassChunk], times log2 e (up to 16 rows)
+  float* score;            // workspace [B, H_KV, rows, chunks * chunk_tiles * 256], times log2 e (up to 16 rows)
   int* status;
   int64_t q_sb, q_st, q_sh, kv_sp, kv_so, kv_sh, s_sp, s_sh, bt_sb, m_sb, m_sh;
   int q_len, group, h_kv, page_log2, n_pages, bt_cols, chunks, rows;   // rows = q_len * group
+  int chunk_tiles;         // up to 16 rows in several launches: 256 tokens each, a block's tiles
   float sm_log2, decay;
 };
 
@@ -179,6 +182,46 @@ __device__ __forceinline__ void mass_queries(const MassParams& p, Smem& sm, int 
   __syncthreads();
 }
 
+// The same for up to 16 rows in two steps, so that nothing waits between them: a 16-byte piece for each thread (asked for with the
+// lengths), and later its row's factor and the piece in shared memory (the caller's barrier publishes them).
+template <int D>
+__device__ __forceinline__ uint4 few_queries_load(const MassParams& p, int b, int h) {
+  const int r = static_cast<int>(threadIdx.x) / (D / 8), c = static_cast<int>(threadIdx.x) % (D / 8);
+  if (r >= p.rows) return make_uint4(0u, 0u, 0u, 0u);
+  const int row = r / p.group, head = h * p.group + r - row * p.group;
+  const int64_t at = (p.q_sb != 0 ? b * p.q_sb + row * p.q_st : (static_cast<int64_t>(b) * p.q_len + row) * p.q_st) + head * p.q_sh;
+  return *reinterpret_cast<const uint4*>(static_cast<const __half*>(p.q) + at + c * 8);
+}
+template <bool BF, int D, typename Smem>
+__device__ __forceinline__ void few_queries_store(const MassParams& p, Smem& sm, uint4 u, int rows, int base) {
+  constexpr int kLanes = D / 8;              // threads of a row
+  const int r = static_cast<int>(threadIdx.x) / kLanes, c = static_cast<int>(threadIdx.x) % kLanes;
+  uint32_t w[4] = {u.x, u.y, u.z, u.w}, top = 0u;   // the larger of the halves' magnitudes: infinity and NaN last
+#pragma unroll
+  for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7FFFu, w[k] >> 16 & 0x7FFFu));
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const bool counts = r < rows && top < (BF ? 0x7F80u : 0x7C00u);
+  float factor = 1.f;
+  if constexpr (BF) {
+    // the largest element times 2^k in [2^14, 2^15); 2^126 suffices for what is not zero beside any key
+    const int k = top != 0u && counts ? min(14 - ilogbf(__uint_as_float(top << 16)), 126) : 0;
+    const float up = __int_as_float((127 + k) << 23);             // k >= 14 - 127
+    factor = __int_as_float((127 - k) << 23);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __half2 v = __floats2half2_rn(__uint_as_float(w[j] << 16) * up, __uint_as_float(w[j] & 0xFFFF0000u) * up);
+      w[j] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  }
+  if (r >= kMassFew) return;                 // (D = 64: half the threads have a piece)
+  *reinterpret_cast<uint4*>(sm.q + r * Smem::kQStride + c * 8) = counts ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(0u, 0u, 0u, 0u);
+  if (c == 0) {
+    sm.factor[r] = factor;
+    sm.lim[r] = counts ? base + r / p.group : -1;
+  }
+}
+
 template <bool BF, int CT, int D, int ROWS, int MODE>
 __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_kernel(const __grid_constant__ MassParams p) {
   using Smem = MassSmem<D, ROWS>;
@@ -191,6 +234,8 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
   const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   const int lane = static_cast<int>(threadIdx.x & 31), warp = static_cast<int>(threadIdx.x >> 5);
   const int g = lane >> 2, tq = lane & 3;
+  uint4 my_q = make_uint4(0u, 0u, 0u, 0u);
+  if constexpr (kFew) my_q = few_queries_load<D>(p, b, h);
   int n, nr;
   mass_extent(p, b, chunk == 0 && h == 0 && threadIdx.x == 0 && MODE != kMassWeights, n, nr);
   // A block without tokens leaves; a cluster's barriers count only the threads that have not left, and no
@@ -359,7 +404,9 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
   };
 
   if constexpr (kFew) {
-    mass_queries<BF, D, ROWS>(p, sm, b, h, 0, rows, kMassFew, base);   // (its wait is for the keys too)
+    few_queries_store<BF, D>(p, sm, my_q, rows, base);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
     const bool half = rows <= 8;              // rows 8 to 15 are padding
     float s[kMassTiles][4][4];
     if (t0[0] < n) {                          // (a warp's first tile is the one that has tokens if any has)
@@ -376,7 +423,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
         scale(i, 0, s[i]);
       }
     }
-    float top[2] = {0.f, 0.f};                // a quad's largest score of rows g and g + 8: whole, the scores become 2^(s - top)
+    float top[2] = {0.f, 0.f};                // a quad's largest score of rows g and g + 8; the scores become 2^(s - top)
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
       float2 x = make_float2(-INFINITY, 0.f);
@@ -395,29 +442,16 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
           for (int j = 0; j < 4; ++j) {
             const float u = exp2_fast(s[i][j][e] - z), v = exp2_fast(s[i][j][e + 1] - z);
             x.y += u + v;
-            if constexpr (MODE == kMassWhole) s[i][j][e] = u, s[i][j][e + 1] = v;
+            s[i][j][e] = u;
+            s[i][j][e + 1] = v;
           }
         x.y += __shfl_xor_sync(0xffffffffu, x.y, 1);
         x.y += __shfl_xor_sync(0xffffffffu, x.y, 2);
       }
       if (tq == 0) sm.part[warp][g + 4 * e] = x;
     }
-    if constexpr (MODE == kMassStats) {       // the scores stay for the second launch
-      if (t0[0] < n)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const int r = g + 4 * e;
-          if (r < rows) {
-            float* at = p.score + (bh * p.rows + r) * (static_cast<int64_t>(p.chunks) * kMassChunk);
-#pragma unroll
-            for (int i = 0; i < kMassTiles; ++i)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(at + t0[i] + j * 8 + 2 * tq) = make_float2(s[i][j][e], s[i][j][e + 1]);
-          }
-        }
-    }
     block_stats(0, rows, kMassFew);
-    if constexpr (MODE == kMassWhole) {
+    {
       if (t0[0] < n) {
         const float f0 = exp2_fast(top[0] - sm.lse[g]), f1 = exp2_fast(top[1] - sm.lse[g + 8]);
 #pragma unroll
@@ -528,7 +562,190 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
   if (lane == 0) p.lse[bh * p.rows + r] = stats_lse(x);
 }
 
-// Up to 16 rows, a table longer than a cluster: the sums over rows from the scores of the first launch.
+// Up to 16 rows, a table longer than a cluster: scores, and each block's maxima and sums.  A warp goes through its tiles of
+// 32 tokens with the keys of the next two on their way; what q costs is paid once for all of them.
+template <int D>
+struct MassStreamSmem {
+  static constexpr int kQStride = D + 8;
+  uint4 keys[kMassStages][kMassWarps][D / 16][32];
+  __half q[kMassFew * kQStride];
+  float2 part[kMassWarps][kMassFew];
+  float factor[kMassFew];
+  int lim[kMassFew];
+};
+
+template <bool BF, int CT, int D>
+__global__ void __launch_bounds__(kMassThreads, 2) mass_stream_kernel(const __grid_constant__ MassParams p) {
+  using Smem = MassStreamSmem<D>;
+  constexpr int C = D / 64;
+  extern __shared__ __align__(16) uint8_t raw_smem[];
+  Smem& sm = *reinterpret_cast<Smem*>(raw_smem);
+  pdl_launch_dependents();
+  pdl_wait();
+  const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z, len = p.chunk_tiles * kMassThreads;
+  const int lane = static_cast<int>(threadIdx.x & 31), warp = static_cast<int>(threadIdx.x >> 5);
+  const int g = lane >> 2, tq = lane & 3;
+  const uint4 my_q = few_queries_load<D>(p, b, h);
+  int n, nr;
+  mass_extent(p, b, chunk == 0 && h == 0 && threadIdx.x == 0, n, nr);
+  if (nr == 0 || static_cast<int64_t>(chunk) * len >= n) return;
+  const int64_t bh = static_cast<int64_t>(b) * p.h_kv + h;
+  const int base = n - nr, rows = nr * p.group, first = chunk * len;
+  const int tiles = min(p.chunk_tiles, (n - first + kMassThreads - 1) / kMassThreads);
+  auto start = [&](int i) { return first + (i * kMassWarps + warp) * 32; };
+  // lane's n-tile (lane & 3) of tile i: its page, or -1
+  auto page_of = [&](int i) {
+    const int t = start(i) + 8 * (lane & 3);
+    if (i >= tiles || t >= n) return -1;
+    const int pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
+    if (pg >= 0 && pg < p.n_pages) return pg;
+    if (lane < 4) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
+    return -1;
+  };
+  auto scale_of = [&](int pg) { return pg < 0 ? 0.f : p.ks[pg * p.s_sp + h * p.s_sh] * p.sm_log2; };
+  const int mask = (1 << p.page_log2) - 1;
+  const uint8_t* heads = p.kc + h * p.kv_sh + tq * 16;
+  auto fetch = [&](int stage, int i, int pg) {
+    if (i < tiles) {
+      const int t = start(i) + g;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int of = __shfl_sync(0xffffffffu, pg, j);
+        uint4* dst = &sm.keys[stage][warp][j * C][lane];
+        if (of >= 0 && t + 8 * j < n) {
+          const uint8_t* k = heads + of * p.kv_sp + ((t + 8 * j) & mask) * p.kv_so;
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + c * 32)), "l"(k + c * 64) : "memory");
+        } else {
+#pragma unroll
+          for (int c = 0; c < C; ++c) dst[c * 32] = make_uint4(0u, 0u, 0u, 0u);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int pg[kMassStages];
+  float sc[kMassStages];                      // the lane's n-tile's scale of each tile on its way (0: it has no page)
+#pragma unroll
+  for (int i = 0; i < kMassStages; ++i) pg[i] = page_of(i);
+  int ahead = page_of(kMassStages);
+#pragma unroll
+  for (int i = 0; i < kMassStages; ++i) {
+    fetch(i, i, pg[i]);
+    sc[i] = scale_of(pg[i]);
+  }
+  few_queries_store<BF, D>(p, sm, my_q, rows, base);
+  __syncthreads();
+  uint32_t a[C][4][4];
+  {
+    const __half* lo = sm.q + g * Smem::kQStride + tq * 16;
+    const __half* hi = lo + 8 * Smem::kQStride;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const uint4 u = *reinterpret_cast<const uint4*>(lo + c * 64 + jj * 8), v = *reinterpret_cast<const uint4*>(hi + c * 64 + jj * 8);
+        a[c][2 * jj][0] = u.x; a[c][2 * jj][1] = v.x; a[c][2 * jj][2] = u.y; a[c][2 * jj][3] = v.y;
+        a[c][2 * jj + 1][0] = u.z; a[c][2 * jj + 1][1] = v.z; a[c][2 * jj + 1][2] = u.w; a[c][2 * jj + 1][3] = v.w;
+      }
+  }
+  const float f0 = sm.factor[g], f1 = sm.factor[g + 8];
+  const int l0 = sm.lim[g], l1 = sm.lim[g + 8];
+  const bool half = rows <= 8;
+  const int64_t width = static_cast<int64_t>(p.chunks) * len;
+  float* out0 = p.score + (bh * p.rows + g) * width + 2 * tq;
+  float* out1 = out0 + 8 * width;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  int stage = 0;
+#pragma unroll 1
+  for (int i = 0; i < tiles; ++i) {
+    const int t = start(i);
+    const float scl = sc[0];
+    const bool bad = __any_sync(0xffffffffu, scl == 0.f);       // (a page's scale is positive)
+    asm volatile("cp.async.wait_group %0;" ::"n"(kMassStages - 1) : "memory");
+    float s[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const uint4 u = sm.keys[stage][warp][j * C + c][lane];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          uint32_t b0, b1;
+          widen4<CT>(w[jj], b0, b1);
+          mma_f16(s[j], a[c][jj], b0, b1);
+        }
+      }
+    }
+    // the stage is read: its next tile, and the page after that
+    fetch(stage, i + kMassStages, ahead);
+    stage = stage + 1 == kMassStages ? 0 : stage + 1;
+#pragma unroll
+    for (int k = 0; k + 1 < kMassStages; ++k) sc[k] = sc[k + 1];
+    sc[kMassStages - 1] = scale_of(ahead);
+    ahead = page_of(i + kMassStages + 1);
+    if (t >= n) continue;                     // (the warp has no tokens here)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = __shfl_sync(0xffffffffu, scl, j);
+      s[j][0] *= x * f0; s[j][1] *= x * f0;
+      s[j][2] *= x * f1; s[j][3] *= x * f1;
+    }
+    if (bad || t + 31 > base) {
+      const uint32_t gone = __ballot_sync(0xffffffffu, scl == 0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = gone >> j & 1u ? INT_MAX - 1 : t + 8 * j + 2 * tq;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (at + e > l0) s[j][e] = -INFINITY;
+          if (at + e > l1) s[j][2 + e] = -INFINITY;
+        }
+      }
+    }
+    auto take = [&](int e) {
+      float top = m[e / 2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, fmaxf(s[j][e], s[j][e + 1]));
+      const float z = top == -INFINITY ? 0.f : top;
+      float sum = l[e / 2] * exp2_fast(m[e / 2] - z);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += exp2_fast(s[j][e] - z) + exp2_fast(s[j][e + 1] - z);
+      m[e / 2] = top;
+      l[e / 2] = sum;
+    };
+    take(0);
+    if (g < rows)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(out0 + t + 8 * j) = make_float2(s[j][0], s[j][1]);
+    if (!half) {
+      take(2);
+      if (g + 8 < rows)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(out1 + t + 8 * j) = make_float2(s[j][2], s[j][3]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    float2 x = make_float2(m[e], l[e]);
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) x = join_stats(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
+    if (tq == 0) sm.part[warp][g + 8 * e] = x;
+  }
+  __syncthreads();
+  const int r = threadIdx.x;
+  if (r >= rows) return;
+  float2 x = make_float2(-INFINITY, 0.f);
+#pragma unroll
+  for (int w = 0; w < kMassWarps; ++w) x = join_stats(x, sm.part[w][r]);
+  if (sm.lim[r] < 0) x = make_float2(-INFINITY, 0.f);
+  p.stats[(bh * p.chunks + chunk) * p.rows + r] = x;
+}
+
+// The sums over rows from those scores.
 constexpr int kMassSumTokens = 4 * kMassThreads;
 __global__ void __launch_bounds__(kMassThreads) mass_sum_kernel(const __grid_constant__ MassParams p) {
   __shared__ float lse[kMassFew];
@@ -539,30 +756,41 @@ __global__ void __launch_bounds__(kMassThreads) mass_sum_kernel(const __grid_con
   mass_extent(p, b, false, n, nr);
   if (nr == 0 || static_cast<int64_t>(blockIdx.x) * kMassSumTokens >= n) return;
   const int64_t bh = static_cast<int64_t>(b) * p.h_kv + h;
-  const int chunks = (n - 1) / kMassChunk + 1, rows = nr * p.group;
-  for (int r = warp; r < rows; r += kMassWarps) {
+  const int len = p.chunk_tiles * kMassThreads, chunks = (n - 1) / len + 1, rows = nr * p.group;
+  const int64_t width = static_cast<int64_t>(p.chunks) * len;
+  const int t = static_cast<int>(blockIdx.x) * kMassSumTokens + static_cast<int>(threadIdx.x);
+  const float* score = p.score + bh * p.rows * width + t;
+  float* at = p.mass + b * p.m_sb + h * p.m_sh + t;
+  // the first rows' scores and the masses are on their way while the rows' sums are joined
+  float v[4][4], old[4], w[4] = {0.f, 0.f, 0.f, 0.f};
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[r][i] = r0 + r < rows && t + i * kMassThreads < n ? score[(r0 + r) * width + i * kMassThreads] : -INFINITY;
+  };
+  load(0);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) old[i] = t + i * kMassThreads < n ? at[i * kMassThreads] : 0.f;
+  for (int r = warp; r < kMassFew; r += kMassWarps) {
     float2 x = make_float2(-INFINITY, 0.f);
-    for (int c = lane; c < chunks; c += 32) x = join_stats(x, p.stats[(bh * p.chunks + c) * p.rows + r]);
+    if (r < rows)
+      for (int c = lane; c < chunks; c += 32) x = join_stats(x, p.stats[(bh * p.chunks + c) * p.rows + r]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x = join_stats(x, make_float2(__shfl_xor_sync(0xffffffffu, x.x, o), __shfl_xor_sync(0xffffffffu, x.y, o)));
     if (lane == 0) lse[r] = stats_lse(x);
   }
   __syncthreads();
-  const int64_t width = static_cast<int64_t>(p.chunks) * kMassChunk;
-  const float* score = p.score + bh * p.rows * width;
-  const int t = static_cast<int>(blockIdx.x) * kMassSumTokens + static_cast<int>(threadIdx.x);
-  float w[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int r = 0; r < rows; ++r) {
-    const float l = lse[r];
+  for (int r0 = 0; r0 < rows; r0 += 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (t + i * kMassThreads < n) w[i] += exp2_fast(score[r * width + t + i * kMassThreads] - l);
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] += exp2_fast(v[r][i] - lse[r0 + r]);
+    if (r0 + 4 < rows) load(r0 + 4);
   }
-  float* at = p.mass + b * p.m_sb + h * p.m_sh + t;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (t + i * kMassThreads < n) at[i * kMassThreads] = fmaf(at[i * kMassThreads], p.decay, w[i]);
+    if (t + i * kMassThreads < n) at[i * kMassThreads] = fmaf(old[i], p.decay, w[i]);
 }
 
 inline int mass_check(int B, int q_len, int H, int H_KV, int D, int page, int bt_cols) {
@@ -576,13 +804,30 @@ inline int mass_check(int B, int q_len, int H, int H_KV, int D, int page, int bt
   return SPECQ_OK;
 }
 
+// How a call is cut: whether clusters hold the whole table, else the tokens of a block (chunk_tiles * 256) and blocks a head.
+inline bool mass_plan(int B, int H_KV, int rows, int tokens, int* chunk_tiles, int* chunks) {
+  *chunk_tiles = kMassChunk / kMassThreads;
+  *chunks = ceil_div(tokens, kMassChunk);
+  // up to 16 rows a cluster is the faster only while most SMs would be idle: 1 x 4096 tokens of 8 heads 8.5 us against 9.2, but 8 x 1024
+  // 10.8 against 9.9 and 32 x 4096 76 against 52
+  if (*chunks <= kMassCluster && (rows > kMassFew || *chunks == 1 || static_cast<int64_t>(B) * H_KV * *chunks <= kMassSms / 2)) return true;
+  if (rows <= kMassFew) {            // long blocks pay for q once; three blocks an SM at least, if the call has them
+    int tiles = 8;
+    while (tiles > 2 && static_cast<int64_t>(B) * H_KV * ceil_div(tokens, tiles * kMassThreads) < 3 * kMassSms) tiles /= 2;
+    *chunk_tiles = tiles;
+    *chunks = ceil_div(tokens, tiles * kMassThreads);
+  }
+  return false;
+}
+
 inline int run_attention_mass_workspace(int B, int q_len, int H, int H_KV, int D, int page, int bt_cols, int64_t* bytes) {
   if (bytes == nullptr) return fail(SPECQ_ERR_INVALID_ARG, "attention_mass_workspace: null pointer");
   if (int rc = mass_check(B, q_len, H, H_KV, D, page, bt_cols)) return rc;
-  const int chunks = ceil_div(bt_cols * page, kMassChunk);
-  const int64_t rows = static_cast<int64_t>(B) * H_KV * q_len * (H / H_KV);
-  const bool few = q_len * (H / H_KV) <= kMassFew;
-  *bytes = chunks <= kMassCluster ? 0 : rows * chunks * 8 + (few ? rows * chunks * kMassChunk * 4 : rows * 4);
+  int tiles, chunks;
+  const int rows = q_len * (H / H_KV);
+  const bool whole = mass_plan(B, H_KV, rows, bt_cols * page, &tiles, &chunks);
+  const int64_t all = static_cast<int64_t>(B) * H_KV * rows;
+  *bytes = whole ? 0 : all * chunks * 8 + (rows <= kMassFew ? all * chunks * tiles * kMassThreads * 4 : all * 4);
   return SPECQ_OK;
 }
 
@@ -613,12 +858,12 @@ inline int run_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t
   p.q_sb = q_sb; p.q_st = q_st; p.q_sh = q_sh; p.kv_sp = kv_sp; p.kv_so = kv_so; p.kv_sh = kv_sh; p.s_sp = s_sp; p.s_sh = s_sh;
   p.bt_sb = bt_sb; p.m_sb = m_sb; p.m_sh = m_sh;
   p.q_len = q_len; p.group = H / H_KV; p.h_kv = H_KV; p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
-  p.n_pages = n_pages; p.bt_cols = bt_cols; p.chunks = ceil_div(bt_cols * page, kMassChunk); p.rows = q_len * p.group;
+  p.n_pages = n_pages; p.bt_cols = bt_cols; p.rows = q_len * p.group;
   p.sm_log2 = sm_scale * kLog2E; p.decay = decay;
+  const bool whole = mass_plan(B, H_KV, p.rows, bt_cols * page, &p.chunk_tiles, &p.chunks);
   p.stats = static_cast<float2*>(workspace);
   p.score = p.lse = reinterpret_cast<float*>(p.stats + (need > 0 ? static_cast<int64_t>(B) * H_KV * p.chunks * p.rows : 0));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool whole = p.chunks <= kMassCluster;
   auto launch = [&](auto kern, size_t smem) {
     int cluster = 1;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), static_cast<int>(smem));
@@ -642,7 +887,7 @@ inline int run_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t
         SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassFew, kMassWhole>, few));
         return SPECQ_OK;
       }
-      SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassFew, kMassStats>, few));
+      SPECQ_CUDA_TRY(launch(mass_stream_kernel<BF, CT, DD>, sizeof(MassStreamSmem<DD>)));
       SPECQ_CUDA_TRY(launch_plain(mass_sum_kernel, dim3(ceil_div(bt_cols * page, kMassSumTokens), H_KV, B), dim3(kMassThreads), st, p));
       return SPECQ_OK;
     }

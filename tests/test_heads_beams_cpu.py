@@ -240,7 +240,7 @@ def test_bounded_cache_library_refuses():
                                         1, D, page, None, 0, None)
     for bad in (dict(D=96), dict(page=24), dict(page=4), dict(page=256), dict(B=70000), dict(cols=1 << 27, page=128), dict(q=8), dict(kv=24)):
         assert mass(**bad) == _lib.SPECQ_ERR_UNSUPPORTED, bad
-    for bad in (dict(cache=2), dict(B=-1), dict(q=None), dict(cols=100)):    # (the last: no workspace)
+    for bad in (dict(cache=2), dict(B=-1), dict(q=None), dict(cols=1000)):    # (the last: no workspace)
         assert mass(**bad) == _lib.SPECQ_ERR_INVALID_ARG, bad
 
     def evict(D=64, page=16, L=1, keep=8, recent=2, ws=16, n=1 << 20, kv=64, pages=4):
