@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
           }
         }
       }
-      tscale[i][j] = sc;
+      tscale[i][j] = pg < 0 ? 1.f : sc;
       if (pg < 0 || t >= n) bad[i] |= 1u << j;
       if (pg >= 0 && t + g < n) {
         const uint8_t* k = p.kc + pg * p.kv_sp + ((t + g) & ((1 << p.page_log2) - 1)) * p.kv_so + h * p.kv_sh + tq * 16;
@@ -321,50 +321,59 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
 #pragma unroll
       for (int jj = 0; jj < 4; ++jj) mma_f16(s, a[c][jj], k[c][jj][0], k[c][jj][1]);
   };
-  // s: rows r0 + g (0, 1) and r0 + g + 8 (2, 3), tokens 8 j + 2 tq + 0, 1, times log2 e; -inf where a row does not see a token
-  auto scale = [&](int i, int r0, float (&s)[4][4]) {
+  // s: the products of rows r0 + g (0, 1) and r0 + g + 8 (2, 3) with tokens 8 j + 2 tq + 0, 1.  A score times log2 e is s x, x > 0;
+  // s becomes -inf where a row does not see a token (and x 1, where a page gives none).
+  auto factors = [&](int i, int r0, float (&x)[4], float (&y)[4]) {
     const float f0 = BF ? sm.factor[r0 + g] : 1.f, f1 = BF ? sm.factor[r0 + g + 8] : 1.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float x = tscale[i][j] * f0, y = tscale[i][j] * f1;
-      s[j][0] *= x; s[j][1] *= x;
-      s[j][2] *= y; s[j][3] *= y;
+      x[j] = BF ? tscale[i][j] * f0 : tscale[i][j];
+      y[j] = BF ? tscale[i][j] * f1 : tscale[i][j];
     }
-    if (bad[i] != 0u || t0[i] + 31 > base) {
-      const int l0 = sm.lim[r0 + g], l1 = sm.lim[r0 + g + 8];
+  };
+  auto hide = [&](int i, int r0, float (&s)[4][4]) {
+    if (bad[i] == 0u && t0[i] + 31 <= base) return;
+    const int l0 = sm.lim[r0 + g], l1 = sm.lim[r0 + g + 8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = bad[i] >> j & 1u ? INT_MAX - 1 : t0[i] + j * 8 + 2 * tq;
+    for (int j = 0; j < 4; ++j) {
+      const int t = bad[i] >> j & 1u ? INT_MAX - 1 : t0[i] + j * 8 + 2 * tq;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (t + e > l0) s[j][e] = -INFINITY;
-          if (t + e > l1) s[j][2 + e] = -INFINITY;
-        }
+      for (int e = 0; e < 2; ++e) {
+        if (t + e > l0) s[j][e] = -INFINITY;
+        if (t + e > l1) s[j][2 + e] = -INFINITY;
       }
     }
   };
   // a row's maximum and sum over this thread's eight tokens, then over the quad's 32
-  auto row_stats = [&](const float (&s)[4][4], int e) {
-    float m = -INFINITY;
+  auto row_stats = [&](const float (&s)[4][4], const float (&x)[4], int e) {
+    float m = fmaxf(s[0][e], s[0][e + 1]) * x[0];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = fmaxf(m, fmaxf(s[j][e], s[j][e + 1]));
+    for (int j = 1; j < 4; ++j) m = fmaxf(m, fmaxf(s[j][e], s[j][e + 1]) * x[j]);
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const float z = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
+    const float z = m == -INFINITY ? 0.f : -m;
+    float2 l = {0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) l += exp2_fast(s[j][e] - z) + exp2_fast(s[j][e + 1] - z);
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    return make_float2(m, l);
+    for (int j = 0; j < 4; ++j) {
+      const float2 d = __ffma2_rn(make_float2(s[j][e], s[j][e + 1]), make_float2(x[j], x[j]), make_float2(z, z));
+      l = __fadd2_rn(l, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+    }
+    float sum = l.x + l.y;
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    return make_float2(m, sum);
   };
-  auto add_weights = [&](int i, int r0, const float (&s)[4][4]) {
-    const float l0 = sm.lse[r0 + g], l1 = sm.lse[r0 + g + 8];
+  auto add_weights = [&](int i, int r0, const float (&s)[4][4], const float (&x)[4], const float (&y)[4]) {
+    const float l0 = -sm.lse[r0 + g], l1 = -sm.lse[r0 + g + 8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        weight[i][j][e] += exp2_fast(s[j][e] - l0) + exp2_fast(s[j][2 + e] - l1);
+    for (int j = 0; j < 4; ++j) {
+      const float2 u = __ffma2_rn(make_float2(s[j][0], s[j][1]), make_float2(x[j], x[j]), make_float2(l0, l0));
+      const float2 v = __ffma2_rn(make_float2(s[j][2], s[j][3]), make_float2(y[j], y[j]), make_float2(l1, l1));
+      const float2 w = __fadd2_rn(__fadd2_rn(make_float2(weight[i][j][0], weight[i][j][1]), make_float2(exp2_fast(u.x), exp2_fast(u.y))),
+                                  make_float2(exp2_fast(v.x), exp2_fast(v.y)));
+      weight[i][j][0] = w.x;
+      weight[i][j][1] = w.y;
+    }
   };
   // the warps' sums to the block's, and (a cluster) the blocks' to lse
   auto block_stats = [&](int first, int here, int pad) {
@@ -420,7 +429,14 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
           widen(i, j, k);
           product(a, k, s[i][j]);
         }
-        scale(i, 0, s[i]);
+        hide(i, 0, s[i]);
+        float x[4], y[4];
+        factors(i, 0, x, y);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s[i][j][0] *= x[j]; s[i][j][1] *= x[j];
+          s[i][j][2] *= y[j]; s[i][j][3] *= y[j];
+        }
       }
     }
     float top[2] = {0.f, 0.f};                // a quad's largest score of rows g and g + 8; the scores become 2^(s - top)
@@ -474,7 +490,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
         for (int r = threadIdx.x; r < pad; r += kMassThreads) sm.lse[r] = r < here ? p.lse[bh * p.rows + first + r] : INFINITY;
         __syncthreads();
       } else {
-#pragma unroll 1
+#pragma unroll
         for (int i = 0; i < kMassTiles; ++i) {
           uint32_t k[4][C][4][2];
 #pragma unroll
@@ -486,12 +502,14 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
             fragments(r0, a);
 #pragma unroll
             for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
-            scale(i, r0, s);
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const float2 x = row_stats(s, e);
-              float2* at = &sm.part[warp][r0 + g + 4 * e];
-              if (tq == 0) *at = i == 0 ? x : join_stats(*at, x);
+            hide(i, r0, s);
+            float x[4], y[4];
+            factors(i, r0, x, y);
+            const float2 u = row_stats(s, x, 0), v = row_stats(s, y, 2);
+            if (tq == 0) {
+              float2* at = &sm.part[warp][r0 + g];
+              at[0] = i == 0 ? u : join_stats(at[0], u);
+              at[8] = i == 0 ? v : join_stats(at[8], v);
             }
           }
         }
@@ -510,8 +528,10 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
             fragments(r0, a);
 #pragma unroll
             for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
-            scale(i, r0, s);
-            add_weights(i, r0, s);
+            hide(i, r0, s);
+            float x[4], y[4];
+            factors(i, r0, x, y);
+            add_weights(i, r0, s, x, y);
           }
         }
       }
@@ -690,9 +710,9 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_stream_kernel(const __gr
     if (t >= n) continue;                     // (the warp has no tokens here)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float x = __shfl_sync(0xffffffffu, scl, j);
-      s[j][0] *= x * f0; s[j][1] *= x * f0;
-      s[j][2] *= x * f1; s[j][3] *= x * f1;
+      const float x = __shfl_sync(0xffffffffu, scl, j), x0 = BF ? x * f0 : x, x1 = BF ? x * f1 : x;
+      s[j][0] *= x0; s[j][1] *= x0;
+      s[j][2] *= x1; s[j][3] *= x1;
     }
     if (bad || t + 31 > base) {
       const uint32_t gone = __ballot_sync(0xffffffffu, scl == 0.f);
