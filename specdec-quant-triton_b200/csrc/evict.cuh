@@ -8,7 +8,7 @@
 //   another scale are requantised, rn(q * (s_source / s'))
 // Each number moved from a page of the largest scale keeps its bits, and no maximum over the numbers is needed.
 //
-// A block selects for one (layer, sequence, head): the bound's 32 bits by four histograms of 8, then one
+// A block selects for one (layer, sequence, head): the bound's 32 bits two at a time by counting, then one
 // ordered pass that writes the kept tokens' places in the cache.  A block then moves K or V of one (layer, sequence,
 // head), 16 KB at a time, the next batch read ahead of the writes: a token's place never grows, and the
 // batches hold whole pages, so what is read later lies behind what is written.  Bound by HBM (scattered
@@ -20,7 +20,7 @@
 
 namespace specq {
 
-constexpr int kEvictSelThreads = 512;
+constexpr int kEvictSelThreads = 256;
 constexpr int kEvictRun = 4;                                        // tokens a thread takes in the ordered pass
 constexpr int kEvictStage = 12 * 1024;                              // keys held in shared memory (48 KB)
 constexpr int kEvictMoveThreads = 256;
@@ -43,7 +43,7 @@ struct EvictParams {
   int n_pages, bt_cols, B, h_kv, page_log2, keep, recent, staged;
 };
 
-// Exclusive sum over the 512 threads.
+// Exclusive sum over the block's threads.
 __device__ __forceinline__ int evict_before(int v, int* red, int* sum) {
   const int lane = static_cast<int>(threadIdx.x & 31), warp = static_cast<int>(threadIdx.x >> 5);
   int inc = v;
@@ -67,10 +67,8 @@ __device__ __forceinline__ int evict_before(int v, int* red, int* sum) {
 
 __global__ void __launch_bounds__(kEvictSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ uint32_t staged[];
-  __shared__ int hist[256];
+  __shared__ int4 counts[2][kEvictSelThreads / 32];
   __shared__ int red[kEvictSelThreads / 32];
-  __shared__ uint32_t digit;
-  __shared__ int left;
   __shared__ int lowest;
   pdl_launch_dependents();
   pdl_wait();
@@ -104,35 +102,52 @@ __global__ void __launch_bounds__(kEvictSelThreads) evict_select_kernel(const __
     for (int t = tid; t < others; t += kEvictSelThreads) staged[t] = order_key(fmaxf(mass[t], -INFINITY));
     __syncthreads();
   }
-  // the want-th largest key, digit by digit; `left`: how many of those that share its digits so far are wanted
+  // The want-th largest key, two bits at a time: how many keys reach each of the next three bounds.
   uint32_t bound = 0xffffffffu;
   int equal = 0;                                               // keys equal to the bound that are kept
   if (want > 0) {
     uint32_t prefix = 0;
-    int need = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
+    int above = 0;                                             // keys above prefix's range
+    for (int shift = 30; shift >= 0; shift -= 2) {
+      const uint32_t b1 = prefix + (1u << shift), b2 = prefix + (2u << shift), b3 = prefix + (3u << shift);
+      const uint32_t last = prefix + ((4u << shift) - 1u);     // (wraps to all ones at the top)
+      int n1 = 0, n2 = 0, n3 = 0;
       for (int t = tid; t < others; t += kEvictSelThreads) {
         const uint32_t k = key_at(t);
-        if (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(hist + (k >> shift & 255u), 1);
+        if (k > last) continue;
+        n1 += k >= b1;
+        n2 += k >= b2;
+        n3 += k >= b3;
       }
+      n1 = __reduce_add_sync(0xffffffffu, n1);
+      n2 = __reduce_add_sync(0xffffffffu, n2);
+      n3 = __reduce_add_sync(0xffffffffu, n3);
+      int4* sums = counts[shift >> 1 & 1];                     // the other one may still be read
+      if ((tid & 31) == 0) sums[tid >> 5] = make_int4(n1, n2, n3, 0);
       __syncthreads();
-      // how many keys have a larger digit: thread 255 - d has digit d
-      const int mine = tid < 256 ? hist[255 - tid] : 0;
-      int all;
-      const int above = evict_before(mine, red, &all);
-      if (tid < 256 && above < need && above + mine >= need) {
-        digit = static_cast<uint32_t>(255 - tid);
-        left = need - above;
+      n1 = n2 = n3 = 0;
+#pragma unroll
+      for (int w = 0; w < kEvictSelThreads / 32; ++w) {
+        const int4 u = sums[w];
+        n1 += u.x;
+        n2 += u.y;
+        n3 += u.z;
       }
-      __syncthreads();
-      prefix |= digit << shift;
-      need = left;
-      __syncthreads();
+      // as many as wanted reach a bound: the keys above it less one are the ones
+      const uint32_t exact = above + n3 == want ? b3 : above + n2 == want ? b2 : above + n1 == want ? b1 : 0u;
+      if (exact != 0u) {
+        prefix = exact - 1u;
+        above = want;
+        break;
+      }
+      // the largest bound that `want` keys reach; those at or above the next one are above its range
+      if (above + n3 >= want) prefix = b3;
+      else if (above + n2 >= want) prefix = b2, above += n3;
+      else if (above + n1 >= want) prefix = b1, above += n2;
+      else above += n1;
     }
     bound = prefix;
-    equal = need;
+    equal = want - above;
   }
   if (tid == 0) lowest = keep;
   // kept tokens in order: those above the bound and the first `equal` at it
@@ -189,6 +204,7 @@ template <int CT, int D>
 __global__ void __launch_bounds__(kEvictMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
   constexpr int U = kEvictPieces, kPer = D / 16;                       // pieces of a token
   constexpr int kBatch = kEvictMoveThreads * U / kPer;                 // tokens: 128 (D = 128) or 256
+  static_assert(kEvictMoveThreads % kPer == 0, "a thread's pieces stand at one place of their tokens");
   static_assert(kBatch >= 128 && kBatch <= kEvictMoveThreads, "a batch holds whole pages, a thread a token's scale");
   __shared__ float from[kBatch];
   __shared__ float to[kBatch];
@@ -208,19 +224,24 @@ __global__ void __launch_bounds__(kEvictMoveThreads) evict_move_kernel(const __g
   float* scale = (is_v ? p.vs : p.ks) + l * p.s_sl + h * p.s_sh;
   const int32_t* place = p.place + id * p.keep;
   const int32_t* row = p.bt + b * p.bt_sb;
+  // Batches in registers: the tokens of one while the one before is written, and the places of the one after.
   uint4 w[2][U];
   float s[2];                                       // this thread's token's scale
-  auto load = [&](int j0, uint4 (&v)[U], float& sc) {
+  int at[U], at_scale;
+  auto look = [&](int j0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = u * kEvictMoveThreads + tid, j = j0 + i / kPer;
-      if (j < p.keep) {
-        const int at = place[j];
-        v[u] = *reinterpret_cast<const uint4*>(cache + (at >> p.page_log2) * p.kv_sp + (at & mask) * p.kv_so + (i % kPer) * 16);
-      }
+      const int j = j0 + (u * kEvictMoveThreads + tid) / kPer;
+      at[u] = j < p.keep ? place[j] : -1;
     }
-    sc = 0.f;
-    if (tid < kBatch && j0 + tid < p.keep) sc = scale[(place[j0 + tid] >> p.page_log2) * p.s_sp];
+    at_scale = tid < kBatch && j0 + tid < p.keep ? place[j0 + tid] : -1;
+  };
+  auto load = [&](uint4 (&v)[U], float& sc) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (at[u] >= 0)
+        v[u] = *reinterpret_cast<const uint4*>(cache + (at[u] >> p.page_log2) * p.kv_sp + (at[u] & mask) * p.kv_so + (tid % kPer) * 16);
+    sc = at_scale >= 0 ? scale[(at_scale >> p.page_log2) * p.s_sp] : 0.f;
   };
   auto store = [&](int j0, uint4 (&v)[U], float sc) {
     // the largest scale of each page: over its lanes, then (pages of 64 and 128) its warps
@@ -245,18 +266,22 @@ __global__ void __launch_bounds__(kEvictMoveThreads) evict_move_kernel(const __g
       if (j < p.keep) {
         const float a = from[t], z = to[t];
         const uint4 out = a == z ? v[u] : requant16<CT>(v[u], a / z);
-        *reinterpret_cast<uint4*>(cache + row[j >> p.page_log2] * p.kv_sp + (j & mask) * p.kv_so + (i % kPer) * 16) = out;
+        *reinterpret_cast<uint4*>(cache + row[j >> p.page_log2] * p.kv_sp + (j & mask) * p.kv_so + (tid % kPer) * 16) = out;
       }
     }
   };
   int j0 = first & ~mask;
-  load(j0, w[0], s[0]);
+  look(j0);
+  load(w[0], s[0]);
+  look(j0 + kBatch);
   while (true) {
-    if (j0 + kBatch < p.keep) load(j0 + kBatch, w[1], s[1]);
+    load(w[1], s[1]);                               // (nothing past the last token)
+    look(j0 + 2 * kBatch);
     store(j0, w[0], s[0]);
     j0 += kBatch;
     if (j0 >= p.keep) break;
-    if (j0 + kBatch < p.keep) load(j0 + kBatch, w[0], s[0]);
+    load(w[0], s[0]);
+    look(j0 + 2 * kBatch);
     store(j0, w[1], s[1]);
     j0 += kBatch;
     if (j0 >= p.keep) break;
