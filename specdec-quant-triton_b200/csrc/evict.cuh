@@ -10,7 +10,7 @@
 //
 // A block selects for one (layer, sequence, head): the bound's 32 bits two at a time by counting, then one
 // ordered pass that writes the kept tokens' places in the cache.  A block then moves K or V of one (layer, sequence,
-// head), 16 KB at a time, the next batch read ahead of the writes: a token's place never grows, and the
+// head), 32 KB at a time, the next batch read ahead of the writes: a token's place never grows, and the
 // batches hold whole pages, so what is read later lies behind what is written.  Bound by HBM (scattered
 // runs of D bytes) where there are some hundred (layer, sequence, head)s, by latency below.
 #pragma once
@@ -23,7 +23,7 @@ namespace specq {
 constexpr int kEvictSelThreads = 256;
 constexpr int kEvictRun = 4;                                        // tokens a thread takes in the ordered pass
 constexpr int kEvictStage = 12 * 1024;                              // keys held in shared memory (48 KB)
-constexpr int kEvictMoveThreads = 256;
+constexpr int kEvictMoveThreads = 512;
 constexpr int kEvictPieces = 4;                                     // 16-byte pieces a thread moves at a time
 
 struct EvictParams {
@@ -41,6 +41,7 @@ struct EvictParams {
   int* status;
   int64_t kv_sl, kv_sp, kv_so, kv_sh, s_sl, s_sp, s_sh, bt_sb, m_sl, m_sb, m_sh;
   int n_pages, bt_cols, B, h_kv, page_log2, keep, recent, staged;
+  int linear;              // kv_sp is a page of kv_so
 };
 
 // Exclusive sum over the block's threads.
@@ -194,20 +195,30 @@ __global__ void __launch_bounds__(kEvictSelThreads) evict_select_kernel(const __
   if (tid == 0) p.first[id] = lowest;
 }
 
-// A piece of 16 stored numbers times r, rounded.
+// A piece of 16 stored numbers times r <= 1, rounded: fp32 products, two at a time.
 template <int CT>
 __device__ __forceinline__ uint4 requant16(uint4 w, float r) {
-  return make_uint4(requant4<CT>(w.x, r), requant4<CT>(w.y, r), requant4<CT>(w.z, r), requant4<CT>(w.w, r));
+  uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  const float2 rr = make_float2(r, r);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[4];
+    unpack_cache4<CT>(u[i], v);
+    const float2 a = __fmul2_rn(make_float2(v[0], v[1]), rr), b = __fmul2_rn(make_float2(v[2], v[3]), rr);
+    u[i] = pack_cache4<CT>(a.x, a.y, b.x, b.y);
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
 }
 
 template <int CT, int D>
 __global__ void __launch_bounds__(kEvictMoveThreads) evict_move_kernel(const __grid_constant__ EvictParams p) {
   constexpr int U = kEvictPieces, kPer = D / 16;                       // pieces of a token
-  constexpr int kBatch = kEvictMoveThreads * U / kPer;                 // tokens: 128 (D = 128) or 256
+  constexpr int kBatch = kEvictMoveThreads * U / kPer;                 // tokens: 256 (D = 128) or 512
   static_assert(kEvictMoveThreads % kPer == 0, "a thread's pieces stand at one place of their tokens");
   static_assert(kBatch >= 128 && kBatch <= kEvictMoveThreads, "a batch holds whole pages, a thread a token's scale");
   __shared__ float from[kBatch];
   __shared__ float to[kBatch];
+  __shared__ int dest[kBatch];
   __shared__ float wide[kEvictMoveThreads / 32];
   pdl_launch_dependents();
   pdl_wait();
@@ -228,6 +239,11 @@ __global__ void __launch_bounds__(kEvictMoveThreads) evict_move_kernel(const __g
   uint4 w[2][U];
   float s[2];                                       // this thread's token's scale
   int at[U], at_scale;
+  uint8_t* mine = cache + (tid % kPer) * 16;
+  // where a place of the cache stands; pages that follow one another without gaps need one product
+  auto token = [&](int where) {
+    return p.linear ? where * p.kv_so : (where >> p.page_log2) * p.kv_sp + (where & mask) * p.kv_so;
+  };
   auto look = [&](int j0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -240,7 +256,7 @@ __global__ void __launch_bounds__(kEvictMoveThreads) evict_move_kernel(const __g
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (at[u] >= 0)
-        v[u] = *reinterpret_cast<const uint4*>(cache + (at[u] >> p.page_log2) * p.kv_sp + (at[u] & mask) * p.kv_so + (tid % kPer) * 16);
+        v[u] = *reinterpret_cast<const uint4*>(mine + token(at[u]));
     sc = at_scale >= 0 ? scale[(at_scale >> p.page_log2) * p.s_sp] : 0.f;
   };
   auto store = [&](int j0, uint4 (&v)[U], float sc) {
@@ -257,16 +273,19 @@ __global__ void __launch_bounds__(kEvictMoveThreads) evict_move_kernel(const __g
     if (tid < kBatch) {
       from[tid] = sc;
       to[tid] = m;
-      if ((tid & mask) == 0 && j0 + tid < p.keep) scale[row[(j0 + tid) >> p.page_log2] * p.s_sp] = m;
+      if (j0 + tid < p.keep) {
+        const int pg = row[(j0 + tid) >> p.page_log2];
+        dest[tid] = pg * page + (tid & mask);       // (a batch begins with a page)
+        if ((tid & mask) == 0) scale[pg * p.s_sp] = m;
+      }
     }
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = u * kEvictMoveThreads + tid, t = i / kPer, j = j0 + t;
-      if (j < p.keep) {
+      const int t = (u * kEvictMoveThreads + tid) / kPer;
+      if (j0 + t < p.keep) {
         const float a = from[t], z = to[t];
-        const uint4 out = a == z ? v[u] : requant16<CT>(v[u], a / z);
-        *reinterpret_cast<uint4*>(cache + row[j >> p.page_log2] * p.kv_sp + (j & mask) * p.kv_so + (tid % kPer) * 16) = out;
+        *reinterpret_cast<uint4*>(mine + token(dest[t])) = a == z ? v[u] : requant16<CT>(v[u], a / z);
       }
     }
   };
@@ -335,7 +354,7 @@ inline int run_block_evict(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int
   p.kv_sl = kv_sl; p.kv_sp = kv_sp; p.kv_so = kv_so; p.kv_sh = kv_sh; p.s_sl = s_sl; p.s_sp = s_sp; p.s_sh = s_sh;
   p.bt_sb = bt_sb; p.m_sl = m_sl; p.m_sb = m_sb; p.m_sh = m_sh;
   p.n_pages = n_pages; p.bt_cols = bt_cols; p.B = B; p.h_kv = H_KV; p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
-  p.keep = keep; p.recent = recent;
+  p.keep = keep; p.recent = recent; p.linear = kv_sp == page * kv_so;
   // the keys of rows that the table admits, up to 48 KB; longer rows read their masses again for each digit
   const int64_t tokens = static_cast<int64_t>(bt_cols) * page;
   p.staged = tokens > 0;

@@ -14,11 +14,14 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <optional>
 #include <string>
 #include <vector>
 
@@ -491,7 +494,7 @@ struct Heads {
   const Tensor &q, &k, &pos, &table;
   const Tensor *qw, *kw, *plan;
   float eps;
-  int layout, weight_f32;
+  int layout;
 };
 
 Heads heads(const char* who, PyObject* q_, PyObject* k_, PyObject* qw_, PyObject* kw_, PyObject* pos_, PyObject* table_, PyObject* eps_,
@@ -522,10 +525,8 @@ Heads heads(const char* who, PyObject* q_, PyObject* k_, PyObject* qw_, PyObject
   if (!(static_cast<float>(eps) > 0.f) || !(eps < 3e38)) BAD_VALUE("%s: eps=%g must be positive and finite", who, eps);
   const Tensor* plan = optional(who, "plan", plan_);
   plan_of(who, plan, 1);
-  return Heads{q, k, pos, table, qw, kw, plan, static_cast<float>(eps), lay, f32 > 0};
+  return Heads{q, k, pos, table, qw, kw, plan, static_cast<float>(eps), lay};
 }
-
-const void* raw(const Tensor* t) { return t == nullptr ? nullptr : t->data_ptr(); }
 
 PyObject* pack(std::initializer_list<Tensor> ts) {    // undefined tensors become None
   PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(ts.size()));
@@ -542,6 +543,78 @@ PyObject* pack(std::initializer_list<Tensor> ts) {    // undefined tensors becom
   return out;
 }
 
+int64_t stride_of(const Tensor& t, int i) { return t.defined() ? t.stride(i) : 0; }
+void* raw(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+Tensor or_none(const Tensor* t) { return t == nullptr ? Tensor() : *t; }
+std::optional<Tensor> maybe(const Tensor* t) { return t == nullptr ? std::nullopt : std::optional<Tensor>(*t); }
+
+// The launch of checked tensors (undefined: not given); the library's code.
+int launch_qk_norm_rope(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& pos, const Tensor& table,
+                        const Tensor& plan, float eps, int layout, const Tensor& q_out, const Tensor& k_out) {
+  const int f32 = (qw.defined() && qw.scalar_type() == at::kFloat) || (kw.defined() && kw.scalar_type() == at::kFloat);
+  return lib.qk_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), k.data_ptr(),
+                          k.stride(0), k.stride(1), k_out.data_ptr(), k_out.stride(0), k_out.stride(1), row_code(q), raw(qw), raw(kw),
+                          f32, eps, ptr<int32_t>(pos), ptr<float>(table), static_cast<int>(table.size(0)), static_cast<int>(q.size(0)),
+                          static_cast<int>(q.size(1)), static_cast<int>(k.size(1)), static_cast<int>(q.size(2)),
+                          static_cast<int>(table.size(1)), layout, static_cast<const int32_t*>(raw(plan)), stream());
+}
+
+// Both outputs with the gradients of q, k and the weights.  The backward pass runs without the interpreter's lock, so its errors
+// are C++ exceptions of torch's engine.
+struct QkNormRope : torch::autograd::Function<QkNormRope> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                const std::optional<Tensor>& qw_, const std::optional<Tensor>& kw_, const Tensor& pos,
+                                                const Tensor& table, const std::optional<Tensor>& plan_, double eps, int64_t layout) {
+    const Tensor qw = qw_.value_or(Tensor()), kw = kw_.value_or(Tensor()), plan = plan_.value_or(Tensor());
+    ctx->save_for_backward({q, k, qw, kw, pos, table, plan});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["layout"] = layout;
+    const bool all = !plan.defined();
+    const Tensor q_out = new_rows(q, all), k_out = new_rows(k, all);
+    check(launch_qk_norm_rope(q, k, qw, kw, pos, table, plan, static_cast<float>(eps), static_cast<int>(layout), q_out, k_out));
+    return {q_out, k_out};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &qw = saved[2], &kw = saved[3], &pos = saved[4], &table = saved[5], &plan = saved[6];
+    auto dense = [](const Tensor& g) { return g.stride(2) == 1 || g.size(2) == 1 ? g : g.contiguous(); };
+    const Tensor gq = dense(grads[0]), gk = dense(grads[1]);
+    const bool all = !plan.defined();
+    const int T = static_cast<int>(q.size(0)), H = static_cast<int>(q.size(1)), HK = static_cast<int>(k.size(1)), D = static_cast<int>(q.size(2));
+    Tensor dq, dk, dqw, dkw, ws;
+    if (ctx->needs_input_grad(0)) dq = new_rows(q, all);
+    if (ctx->needs_input_grad(1)) dk = new_rows(k, all);
+    // (weights that are not there are no edges of the graph)
+    if (qw.defined() && ctx->needs_input_grad(2)) dqw = at::empty(qw.sizes(), qw.options());
+    if (kw.defined() && ctx->needs_input_grad(qw.defined() ? 3 : 2)) dkw = at::empty(kw.sizes(), kw.options());
+    int64_t bytes = 0;
+    int rc = SPECQ_OK;
+    if (dqw.defined() || dkw.defined()) rc = lib.qk_norm_rope_grad_workspace(T, H, HK, D, &bytes);
+    // from torch's allocator on the current stream, as the attention's
+    if (rc == SPECQ_OK && bytes > 0) ws = at::empty({bytes}, q.options().dtype(at::kByte));
+    const int f32 = (qw.defined() && qw.scalar_type() == at::kFloat) || (kw.defined() && kw.scalar_type() == at::kFloat);
+    if (rc == SPECQ_OK)
+      rc = lib.qk_norm_rope_grad(q.data_ptr(), q.stride(0), q.stride(1), gq.data_ptr(), gq.stride(0), gq.stride(1), raw(dq), stride_of(dq, 0),
+                                 stride_of(dq, 1), k.data_ptr(), k.stride(0), k.stride(1), gk.data_ptr(), gk.stride(0), gk.stride(1), raw(dk),
+                                 stride_of(dk, 0), stride_of(dk, 1), row_code(q), raw(qw), raw(kw), raw(dqw), raw(dkw), f32,
+                                 static_cast<float>(ctx->saved_data["eps"].toDouble()), ptr<int32_t>(pos), ptr<float>(table),
+                                 static_cast<int>(table.size(0)), T, H, HK, D, static_cast<int>(table.size(1)),
+                                 static_cast<int>(ctx->saved_data["layout"].toInt()), static_cast<const int32_t*>(raw(plan)), raw(ws), bytes,
+                                 stream());
+    if (rc != SPECQ_OK) throw std::runtime_error(std::string("libspecq: ") + lib.last_error());
+    torch::autograd::variable_list out = {dq, dk, dqw, dkw};
+    if (c10::GradMode::is_enabled()) {     // the gradients are no graph of their own: differentiating them is an error, not a zero
+      for (Tensor& t : out)
+        if (t.defined()) t.set_requires_grad(true);
+      auto stop = std::make_shared<torch::autograd::DelayedError>("qk_norm_rope is differentiable once", 4);
+      out = (*stop)(std::move(out));
+    }
+    out.resize(9);
+    return out;
+  }
+};
+
 PyObject* qk_norm_rope(PyObject* const* a) {
   // q, k, q_weight, k_weight, pos, table, eps, layout, q_out, k_out, plan
   const char* who = "qk_norm_rope";
@@ -556,56 +629,27 @@ PyObject* qk_norm_rope(PyObject* const* a) {
   };
   out_like("q_out", q_given, x.q);
   out_like("k_out", k_given, x.k);
+  for (int64_t n : {x.q.size(0), x.q.size(1), x.k.size(1), x.q.size(2), x.table.size(0)}) size32(who, n);
+  bool needs = false;
   if (c10::GradMode::is_enabled()) {
-    const bool needs = x.q.requires_grad() || x.k.requires_grad() || (x.qw != nullptr && x.qw->requires_grad()) ||
-                       (x.kw != nullptr && x.kw->requires_grad());
+    needs = x.q.requires_grad() || x.k.requires_grad() || (x.qw != nullptr && x.qw->requires_grad()) ||
+            (x.kw != nullptr && x.kw->requires_grad());
     if ((q_given != nullptr || k_given != nullptr) &&
         (needs || (q_given != nullptr && q_given->requires_grad()) || (k_given != nullptr && k_given->requires_grad())))
       BAD_VALUE("%s: no q_out or k_out where a gradient is wanted", who);
     if (x.table.requires_grad()) BAD_VALUE("%s: the table has no gradient", who);
-    if (needs) Py_RETURN_NOTIMPLEMENTED;   // specq/heads.py records the gradient and calls again
   }
   same_device(who, {&x.q, &x.k, &x.pos, &x.table, x.qw, x.kw, q_given, k_given, x.plan});
+  const Tensor qw = or_none(x.qw), kw = or_none(x.kw), plan = or_none(x.plan);
+  if (needs) {
+    const auto out = QkNormRope::apply(x.q, x.k, maybe(x.qw), maybe(x.kw), x.pos, x.table, maybe(x.plan), static_cast<double>(x.eps),
+                                       static_cast<int64_t>(x.layout));
+    return pack({out[0], out[1]});
+  }
   const bool all = x.plan == nullptr;
   const Tensor q_out = q_given != nullptr ? *q_given : new_rows(x.q, all), k_out = k_given != nullptr ? *k_given : new_rows(x.k, all);
-  check(lib.qk_norm_rope(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), x.k.data_ptr(),
-                         x.k.stride(0), x.k.stride(1), k_out.data_ptr(), k_out.stride(0), k_out.stride(1), row_code(x.q), raw(x.qw),
-                         raw(x.kw), x.weight_f32, x.eps, ptr<int32_t>(x.pos), ptr<float>(x.table), size32(who, x.table.size(0)),
-                         size32(who, x.q.size(0)), size32(who, x.q.size(1)), size32(who, x.k.size(1)), size32(who, x.q.size(2)),
-                         size32(who, x.table.size(1)), x.layout, ptr<int32_t>(x.plan), stream()));
+  check(launch_qk_norm_rope(x.q, x.k, qw, kw, x.pos, x.table, plan, x.eps, x.layout, q_out, k_out));
   return pack({q_out, k_out});
-}
-
-PyObject* qk_norm_rope_grad(PyObject* const* a) {
-  // gq, gk, q, k, q_weight, k_weight, pos, table, eps, layout, plan, want (bits: dq, dk, dqw, dkw)
-  const char* who = "qk_norm_rope's gradient";
-  const Heads x = heads(who, a[2], a[3], a[4], a[5], a[6], a[7], a[8], a[9], a[10]);
-  const Tensor &gq = tensor(who, "gq", a[0]), &gk = tensor(who, "gk", a[1]);
-  rows3(who, "gq", gq, true);
-  rows3(who, "gk", gk, true);
-  if (gq.scalar_type() != x.q.scalar_type() || gk.scalar_type() != x.q.scalar_type() || gq.sizes() != x.q.sizes() || gk.sizes() != x.k.sizes())
-    BAD_VALUE("%s: gradients %s %s and %s %s of outputs like %s and %s", who, dtype(gq), shape(gq).c_str(), dtype(gk), shape(gk).c_str(),
-              shape(x.q).c_str(), shape(x.k).c_str());
-  const int want = integer(a[11]);
-  same_device(who, {&x.q, &x.k, &gq, &gk, &x.pos, &x.table, x.qw, x.kw, x.plan});
-  const int T = size32(who, x.q.size(0)), H = size32(who, x.q.size(1)), HK = size32(who, x.k.size(1)), D = size32(who, x.q.size(2));
-  Tensor dq, dk, dqw, dkw, ws;
-  if (want & 1) dq = new_rows(x.q, x.plan == nullptr);
-  if (want & 2) dk = new_rows(x.k, x.plan == nullptr);
-  if ((want & 4) && x.qw != nullptr) dqw = at::empty(x.qw->sizes(), x.qw->options());
-  if ((want & 8) && x.kw != nullptr) dkw = at::empty(x.kw->sizes(), x.kw->options());
-  int64_t bytes = 0;
-  if (dqw.defined() || dkw.defined()) check(lib.qk_norm_rope_grad_workspace(T, H, HK, D, &bytes));
-  // from torch's allocator on the current stream, as the attention's
-  if (bytes > 0) ws = at::empty({bytes}, x.q.options().dtype(at::kByte));
-  auto p = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
-  auto st = [](const Tensor& t, int i) { return t.defined() ? t.stride(i) : 0; };
-  check(lib.qk_norm_rope_grad(x.q.data_ptr(), x.q.stride(0), x.q.stride(1), gq.data_ptr(), gq.stride(0), gq.stride(1), p(dq), st(dq, 0),
-                              st(dq, 1), x.k.data_ptr(), x.k.stride(0), x.k.stride(1), gk.data_ptr(), gk.stride(0), gk.stride(1), p(dk),
-                              st(dk, 0), st(dk, 1), row_code(x.q), raw(x.qw), raw(x.kw), p(dqw), p(dkw), x.weight_f32, x.eps,
-                              ptr<int32_t>(x.pos), ptr<float>(x.table), size32(who, x.table.size(0)), T, H, HK, D,
-                              size32(who, x.table.size(1)), x.layout, ptr<int32_t>(x.plan), p(ws), bytes, stream()));
-  return pack({dq, dk, dqw, dkw});
 }
 
 // ---- beams ------------------------------------------------------------------------------------------
@@ -861,7 +905,6 @@ PyMethodDef methods[] = {
     {"paged_attention_blocks", FAST((entry<paged_attention_blocks, 14>)), nullptr},
     {"kv_compact_blocks", FAST((entry<kv_compact_blocks, 10>)), nullptr},
     {"qk_norm_rope", FAST((entry<qk_norm_rope, 11>)), nullptr},
-    {"qk_norm_rope_grad", FAST((entry<qk_norm_rope_grad, 12>)), nullptr},
     {"beam_select", FAST((entry<beam_select, 6>)), nullptr},
     {"beam_reorder", FAST((entry<beam_reorder, 3>)), nullptr},
     {"attention_mass_blocks", FAST((entry<attention_mass_blocks, 10>)), nullptr},

@@ -278,11 +278,28 @@ __global__ void __launch_bounds__(kNormThreads) qk_norm_any_kernel(const __grid_
 }
 
 // ---- gradients ------------------------------------------------------------------------------------
+// A thread's stages: the 16-byte pieces of the units to come, copied asynchronously; nobody else reads them.
+constexpr int kNormStages = 2;
+template <int THREADS, int PIECES>
+struct NormStages {
+  uint4 (*at)[PIECES][THREADS];
+  __device__ __forceinline__ void fetch(int stage, int piece, const void* src) const {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(&at[stage][piece][threadIdx.x])), "l"(src) : "memory");
+  }
+  __device__ __forceinline__ uint4 get(int stage, int piece, bool there) const {
+    return there ? at[stage][piece][threadIdx.x] : make_uint4(0u, 0u, 0u, 0u);
+  }
+};
+__device__ __forceinline__ void norm_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void norm_arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(kNormStages - 1) : "memory"); }
+
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(kNormGradThreads, 2)
     qk_norm_grad_vec_kernel(const __grid_constant__ QkNormParams p, int lane_bits) {
   constexpr int V = Row16<T>::N, HP = kNormGradHeads;
-  extern __shared__ float red[];       // [warps, D]
+  extern __shared__ uint4 ring[];      // [stages, 4 HP, threads]; at the end the warps' sums [warps, D]
+  float* red = reinterpret_cast<float*>(ring);
+  const NormStages<kNormGradThreads, 4 * HP> stages{reinterpret_cast<uint4 (*)[4 * HP][kNormGradThreads]>(ring)};
   pdl_launch_dependents();
   pdl_wait();
   const int rows = rope_active_rows(p.plan, p.T, p.status);
@@ -302,24 +319,49 @@ __global__ void __launch_bounds__(kNormGradThreads, 2)
   load_weights<T, V>(p.w[is_k], p.w_f32, at.b, wb);
 #pragma unroll
   for (int i = 0; i < V; ++i) sa[i] = sb[i] = 0.f;
+  const int mine = static_cast<int>(threadIdx.x) >> lane_bits;
+  auto place = [&](int64_t u0, int& t, int& h0) {    // -> heads
+    const int64_t unit = u0 + mine;
+    t = static_cast<int>(unit / groups);
+    h0 = static_cast<int>(unit - static_cast<int64_t>(t) * groups) * HP;
+    return unit < units ? min(HP, p.heads[is_k] - h0) : 0;
+  };
+  auto fetch = [&](int stage, int64_t u0) {
+    if (u0 < units) {
+      int t, h0;
+      const int n = place(u0, t, h0);
+      const T* x = x0 + t * p.xt[is_k] + h0 * p.xh[is_k];
+      const T* g = g0 + t * p.gt[is_k] + h0 * p.gh[is_k];
+#pragma unroll
+      for (int h = 0; h < HP; ++h)
+        if (h < n) {
+          stages.fetch(stage, 4 * h, x + h * p.xh[is_k] + at.a);
+          stages.fetch(stage, 4 * h + 1, x + h * p.xh[is_k] + at.b);
+          stages.fetch(stage, 4 * h + 2, g + h * p.gh[is_k] + at.a);
+          stages.fetch(stage, 4 * h + 3, g + h * p.gh[is_k] + at.b);
+        }
+    }
+    norm_commit();
+  };
   // a block's lane groups take neighbouring units; all warps make the same number of turns
-  for (int64_t u0 = static_cast<int64_t>(block) * per_block; u0 < units; u0 += step) {
-    const int64_t unit = u0 + (threadIdx.x >> lane_bits);
-    const int t = static_cast<int>(unit / groups), h0 = static_cast<int>(unit - static_cast<int64_t>(t) * groups) * HP;
-    const int n = unit < units ? min(HP, p.heads[is_k] - h0) : 0;
-    const T* x = x0 + t * p.xt[is_k] + h0 * p.xh[is_k];
-    const T* g = g0 + t * p.gt[is_k] + h0 * p.gh[is_k];
+  const int64_t first = static_cast<int64_t>(block) * per_block;
+#pragma unroll
+  for (int i = 0; i < kNormStages - 1; ++i) fetch(i, first + i * step);
+  int stage = 0;
+  for (int64_t u0 = first; u0 < units; u0 += step) {
+    fetch(stage == 0 ? kNormStages - 1 : stage - 1, u0 + (kNormStages - 1) * step);
+    int t, h0;
+    const int n = place(u0, t, h0);
+    norm_arrived();
     Row16<T> xa[HP], xb[HP], ga[HP], gb[HP];
 #pragma unroll
     for (int h = 0; h < HP; ++h) {
-      xa[h].raw = xb[h].raw = ga[h].raw = gb[h].raw = make_uint4(0u, 0u, 0u, 0u);
-      if (h < n) {
-        xa[h].load(x + h * p.xh[is_k] + at.a);
-        xb[h].load(x + h * p.xh[is_k] + at.b);
-        ga[h].load(g + h * p.gh[is_k] + at.a);
-        gb[h].load(g + h * p.gh[is_k] + at.b);
-      }
+      xa[h].raw = stages.get(stage, 4 * h, h < n);
+      xb[h].raw = stages.get(stage, 4 * h + 1, h < n);
+      ga[h].raw = stages.get(stage, 4 * h + 2, h < n);
+      gb[h].raw = stages.get(stage, 4 * h + 3, h < n);
     }
+    stage = stage + 1 == kNormStages ? 0 : stage + 1;
     float c[V], s[V];
     if (at.turned && n > 0) {
       const float* row = rope_row(p.table, __ldg(p.pos + t), p.n_pos, p.rot, p.status);
@@ -383,6 +425,7 @@ __global__ void __launch_bounds__(kNormGradThreads, 2)
     }
   }
   if (p.part[is_k] == nullptr) return;
+  __syncthreads();                     // the stages are read
   // the warp's lanes of one item, then the warps
   for (int o = 16; o >= lanes; o >>= 1)
 #pragma unroll
@@ -590,7 +633,7 @@ inline int launch_qk_norm_grad(QkNormParams p, bool half, cudaStream_t st) {
   const int bits = norm_lane_bits<T>(p);
   const dim3 grid(p.blocks[0] + p.blocks[1]);
   auto launch = [&](auto kern, int threads, int last) {
-    const size_t smem = static_cast<size_t>(threads / 32) * p.D * sizeof(float);
+    const size_t smem = std::max<size_t>(static_cast<size_t>(threads / 32) * p.D * sizeof(float), bits < 0 ? 0 : static_cast<size_t>(kNormStages) * 4 * kNormGradHeads * kNormGradThreads * 16);
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

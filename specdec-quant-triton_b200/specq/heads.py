@@ -8,12 +8,9 @@ no reference counterpart.
 """
 from __future__ import annotations
 
-import torch
-from torch.autograd.function import once_differentiable
-
 from . import _lib
 
-# The argument checks and the calls are in csrc/py_blocks.cpp, in the order of these signatures.
+# The argument checks, the calls and the gradient's record are in csrc/py_blocks.cpp, in the order of this signature.
 _native = _lib.native()
 
 
@@ -27,24 +24,4 @@ def qk_norm_rope(q, k, q_weight, k_weight, pos, table, eps=1e-6, layout="half", 
     differentiable; the table has none): the weights' gradients are sums over all tokens and heads in a fixed order.
     With `plan`, only rows < plan[0]: the others of new outputs and gradients are 0, those of q_out and k_out keep
     what they hold."""
-    y = _native.qk_norm_rope(q, k, q_weight, k_weight, pos, table, eps, layout, q_out, k_out, plan)
-    return y if y is not NotImplemented else _QkNormRope.apply(q, k, q_weight, k_weight, pos, table, eps, layout, plan)
-
-
-class _QkNormRope(torch.autograd.Function):
-    """Both outputs with the gradients of q, k and the weights (the binding leaves tensors that require grad to it)."""
-
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, pos, table, eps, layout, plan):
-        ctx.save_for_backward(q, k, q_weight, k_weight, pos, table, plan)
-        ctx.eps, ctx.layout = eps, layout
-        return _native.qk_norm_rope(q, k, q_weight, k_weight, pos, table, eps, layout, None, None, plan)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, q_weight, k_weight, pos, table, plan = ctx.saved_tensors
-        gq, gk = (g if g.stride(-1) == 1 else g.contiguous() for g in (gq, gk))
-        want = sum(1 << i for i in range(4) if ctx.needs_input_grad[i])
-        d = _native.qk_norm_rope_grad(gq, gk, q, k, q_weight, k_weight, pos, table, ctx.eps, ctx.layout, plan, want)
-        return *d, None, None, None, None, None
+    return _native.qk_norm_rope(q, k, q_weight, k_weight, pos, table, eps, layout, q_out, k_out, plan)

@@ -226,6 +226,30 @@ def test_large_and_small_rows(cuda, dtype):
                 _check_grad(dx, None, x, qw, g, table, pos[:5], "half", 1e-6)
 
 
+def test_differentiable_once(cuda):
+    """A graph of the gradients is no zero but an error, where it is used."""
+    import specq
+    q, k, qw, kw, pos, table, r = _make(5, 2, 1, 64, 64, torch.float32, 12)
+    q.requires_grad_(True)
+    a, _ = specq.qk_norm_rope(q, k, qw, kw, pos, table)
+    g = r(5, 2, 64)
+    (plain,) = torch.autograd.grad(a, q, g, retain_graph=True)
+    (dq,) = torch.autograd.grad(a, q, g, create_graph=True)
+    assert torch.equal(plain, dq)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dq.sum().backward()
+
+
+def test_inputs_changed_before_backward_are_an_error(cuda):
+    import specq
+    q, k, qw, kw, pos, table, r = _make(5, 2, 1, 64, 64, torch.float32, 13)
+    qw.requires_grad_(True)
+    a, _ = specq.qk_norm_rope(q, k, qw, kw, pos, table)
+    q.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(a, qw, r(5, 2, 64))
+
+
 def test_plan_and_empty_calls(cuda):
     import specq
     q, k, qw, kw, pos, table, r = _make(12, 3, 2, 64, 64, torch.float16, 8)
