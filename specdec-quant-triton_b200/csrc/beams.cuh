@@ -214,7 +214,11 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const __grid_co
   const bool whole = first >= 0 && first + p.slice <= p.V;
   if (whole) {
 #pragma unroll 4
-    for (int j = 0; j < NP; ++j) fetch(j, first + (j * kSelThreads + tid) * E);
+    for (int j = 0; j < NP / 2; ++j) fetch(j, first + (j * kSelThreads + tid) * E);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll 4
+    for (int j = NP / 2; j < NP; ++j) fetch(j, first + (j * kSelThreads + tid) * E);
+    asm volatile("cp.async.commit_group;" ::: "memory");
   } else {                                        // a row's ends: -inf outside, its cut pieces by elements
 #pragma unroll 1
     for (int j = 0; j < NP; ++j) {
@@ -230,17 +234,27 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const __grid_co
     }
   }
   if (tid == 0) found = 0;
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  if (!whole) __syncthreads();
   // (loops over the pieces are not unrolled: the kernel is short against its code)
   float m = -INFINITY;
   uint32_t seen = W::kNone;
   auto top_of = [&](const uint4& u) { return W::top(W::max(W::max(u.x, u.y), W::max(u.z, u.w))); };
+  auto look = [&](int j0, int j1) {
 #pragma unroll 2
-  for (int j = 0; j < NP; ++j) {
-    const uint4 u = held[j * kSelThreads + tid];
-    seen = W::max_nan(seen, W::max_nan(W::max_nan(u.x, u.y), W::max_nan(u.z, u.w)));
-    m = fmaxf(m, top_of(u));
+    for (int j = j0; j < j1; ++j) {
+      const uint4 u = held[j * kSelThreads + tid];
+      seen = W::max_nan(seen, W::max_nan(W::max_nan(u.x, u.y), W::max_nan(u.z, u.w)));
+      m = fmaxf(m, top_of(u));
+    }
+  };
+  if (whole) {
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    look(0, NP / 2);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    look(NP / 2, NP);
+  } else {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    look(0, NP);
   }
   if (W::strange(seen)) {                         // rewritten once, by the only thread that reads them
     m = -INFINITY;
@@ -277,25 +291,24 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const __grid_co
     r.raw = held[j * kSelThreads + tid];
     r.get(v);
   };
-  // the warp goes through the pieces of its threads that reach the bound, a lane a piece
+  // the warp goes through the pieces of its threads that reach the bound, a lane half a piece
   if (best > kKeyNone) {
+    static_assert(2 * kSelMaxPieces <= 32, "a lane for each half piece");
+    constexpr int EH = E / 2;
     for (uint32_t todo = __ballot_sync(0xffffffffu, mine >= least); todo != 0u; todo &= todo - 1u) {
       const int from = warp * 32 + __ffs(todo) - 1;
-      if (lane >= NP || top_of(held[lane * kSelThreads + from]) < bound) continue;
-      Row16<T> r;
-      float v[E];
-      r.raw = held[lane * kSelThreads + from];
-      r.get(v);
-      uint32_t hits = 0;
+      if (lane >= 2 * NP) continue;
+      const int slot = (lane >> 1) * kSelThreads + from;
+      const uint2 u = reinterpret_cast<const uint2*>(held + slot)[lane & 1];
+      const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
-      for (int k = 0; k < E; ++k) hits |= v[k] >= bound ? 1u << k : 0u;
-      int at = atomicAdd(&found, __popc(hits));   // their order does not matter: they are ranked
-#pragma unroll
-      for (int k = 0; k < E; ++k)
-        if (hits >> k & 1u) {
-          if (at < kSelBuf) buf[at] = static_cast<uint64_t>(order_key(v[k])) << 32 | static_cast<uint32_t>(~(first + (lane * kSelThreads + from) * E + k));
-          ++at;
+      for (int k = 0; k < EH; ++k) {
+        const float v = weight_to_f32<T>(e[k]);
+        if (v >= bound) {
+          const int at = atomicAdd(&found, 1);    // their order does not matter: they are ranked
+          if (at < kSelBuf) buf[at] = static_cast<uint64_t>(order_key(v)) << 32 | static_cast<uint32_t>(~(first + slot * E + (lane & 1) * EH + k));
         }
+      }
     }
   }
   double sum = 0.0;
