@@ -260,12 +260,9 @@ def _own_mass(s):
 
 def _own_evict(s):
     c = s["case"]
-    # The masses are kept and a copy goes to the call: with those that an eviction leaves behind (the kept tokens' in
-    # front, 0 behind them) another pass over this state would find nearly every token in its place.
-    mass = s["mass"].clone()
-    ctx = _specq().kv_evict_blocks(s["kc"], s["vc"], s["ks"], s["vs"], s["tbl"], s["ctx"], mass, c["keep"],
+    ctx = _specq().kv_evict_blocks(s["kc"], s["vc"], s["ks"], s["vs"], s["tbl"], s["ctx"], s["mass"], c["keep"],
                                    c["recent"])
-    return dict(ctx=ctx, kc=s["kc"], vc=s["vc"], ks=s["ks"], vs=s["vs"], mass=mass)
+    return dict(ctx=ctx, kc=s["kc"], vc=s["vc"], ks=s["ks"], vs=s["vs"], mass=s["mass"])
 
 
 # ---- the plain forms ---------------------------------------------------------------------------
