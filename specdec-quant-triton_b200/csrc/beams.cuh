@@ -709,6 +709,10 @@ inline int run_beam_select(const void* logits, int64_t ld, int dtype, const floa
   auto inverse = [](int64_t d) { return static_cast<uint32_t>((0x100000000ll + d - 1) / d); };
   p.lists_inv = inverse(static_cast<int64_t>(K) * p.S);
   p.beams_inv = inverse(K);
+  const int64_t lists_b = static_cast<int64_t>(K) * p.S;
+  const int staged = lists_b * n * 12 <= kMergeSmem ? 1 : 0;
+  const int64_t smem = (staged ? lists_b * n * 12 : 0) + lists_b * 4;
+  if (smem > dev->max_smem_optin - 32 * 1024) return fail(SPECQ_ERR_UNSUPPORTED, "beam_select: %d beams of %d tokens", K, V);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(p.S, B * K), block(kSelThreads);
   const int held = p.pieces * kSelThreads * 16;
@@ -729,10 +733,6 @@ inline int run_beam_select(const void* logits, int64_t ld, int dtype, const floa
   else if (dtype == SPECQ_DTYPE_F32) e = launch(beam_slice_kernel<float>);
   else e = launch(beam_slice_kernel<__nv_bfloat16>);
   SPECQ_CUDA_TRY(e);
-  const int64_t lists_b = static_cast<int64_t>(K) * p.S;
-  const int staged = lists_b * n * 12 <= kMergeSmem ? 1 : 0;
-  const int64_t smem = (staged ? lists_b * n * 12 : 0) + lists_b * 4;
-  if (smem > dev->max_smem_optin - 32 * 1024) return fail(SPECQ_ERR_UNSUPPORTED, "beam_select: %d beams of %d tokens", K, V);
   SPECQ_CUDA_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(beam_merge_kernel), static_cast<int>(smem)));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(B);

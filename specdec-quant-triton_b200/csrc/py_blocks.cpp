@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -712,6 +713,9 @@ PyObject* beam_reorder(PyObject* const* a) {
     at_[i] = t.data_ptr();
     stride[i] = t.stride(0) * t.element_size();
     bytes[i] = inner * t.element_size();
+    const char *lo_ = static_cast<char*>(at_[i]), *par = static_cast<char*>(parent.data_ptr());
+    if (bytes[i] > 0 && lo_ < par + R * 4 && par < lo_ + (R - 1) * stride[i] + bytes[i])
+      BAD_VALUE("%s: state %zd and parent share memory", who, i);
     for (Py_ssize_t j = 0; j < i && bytes[i] > 0; ++j) {     // columns of one buffer are two states, shared bytes are not
       if (bytes[j] == 0) continue;
       const int64_t lo = static_cast<char*>(at_[i]) - static_cast<char*>(at_[j]);
@@ -808,8 +812,11 @@ PyObject* kv_evict_blocks(PyObject* const* a) {
   const int64_t B = tbl.size(0);
   int32s(who, "ctx_len", ctx, 1, B);
   if (c.L == 0) BAD_VALUE("%s: a cache without layers", who);
-  const int keep = integer(a[7]), recent = integer(a[8]);
+  int keep = integer(a[7]), recent = integer(a[8]);
   if (keep < 1 || recent < 0 || recent > keep) BAD_VALUE("%s: keep=%d, of these the newest recent=%d", who, keep, recent);
+  // more than the table has room for: no row has as many, and none needs a place for them
+  keep = static_cast<int>(std::min<int64_t>(keep, std::max<int64_t>(1, tbl.size(1) * c.page)));
+  recent = std::min(recent, keep);
   mass_of(who, mass, c.d != 0, c.L, B, c.H, tbl.size(1) * c.page);
   const Tensor *ref = optional(who, "ref", a[9]), *given = optional(who, "ctx_out", a[10]);
   if (ref != nullptr) int32s(who, "ref", *ref, 1, c.P);

@@ -294,6 +294,8 @@ def test_evict_leaves_rows_alone(cuda):
     after = [x.clone() for x in (*cache, mass)]
     only = [0, 0, 70, 0, 0, 0]
     _check_evict([x[None] for x in before], [x[None] for x in after], tbl, only, 30, 10, torch.int8, _i32([0, 0, 30, 0, 0, 0]))
+    out = specq.kv_evict_blocks(*cache, tbl[2:3], _i32([90]), mass[2:3], (1 << 31) - 1, (1 << 31) - 1)   # no budget at all
+    assert out.tolist() == [90]
     out = specq.kv_evict_blocks(*cache, tbl, _i32([20, 30, 30, 8, 0, 1]), mass, 30, 10, ref=ref)       # nothing to cut
     assert out.tolist() == [20, 30, 30, 8, 0, 1] and specq.get_status() == 0
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(after, (*cache, mass)))

@@ -160,6 +160,9 @@ def test_reorder_refuses_the_rest():
         specq.beam_reorder([x.view(-1)[:8].view(4, 2), x.view(-1)[6:14].view(4, 2)], _i32(2, 2))
     with pytest.raises(ValueError, match="CUDA"):       # columns of one buffer are two states
         specq.beam_reorder([x[:, :4], x[:, 4:]], _i32(2, 2))
+    parent = _i32(2, 2)
+    with pytest.raises(ValueError, match="parent share memory"):
+        specq.beam_reorder([parent.view(4)], parent)
     with pytest.raises(ValueError, match="parent"):
         specq.beam_reorder([x], torch.zeros(2, 2, dtype=torch.int64))
     with pytest.raises(ValueError, match="beams"):
