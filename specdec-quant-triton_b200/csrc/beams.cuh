@@ -11,16 +11,20 @@
 // be good to some 1e-7: what the rounding of the row's largest logit times log2 e moves is put right in the sum, sixteen values are added in fp32 and the rest in 64 bits.  Within a row
 // the order is that of the logits themselves, which needs no exp.
 //
-// Bound by HBM: one pass over the logits.  A block holds a slice of one row in shared memory (2 to 16 16-byte pieces a
-// thread, which only that thread reads back), so maximum, sum and selection read it once.  Selection: each warp's
-// t-th largest of its threads' maxima (8 t >= n) gives a bound that at least n elements reach and few more; those are
-// ranked by counting.  Where many elements reach it (ties, a constant row) the n-th largest key is found by bisection of its
+// One pass over the logits, bound by HBM in principle.  A block holds a slice of one row in shared memory (2 to 16 16-byte
+// pieces a thread), so maximum, sum and selection read it once.  Selection: each warp's t-th largest of its threads' maxima
+// (8 t >= n) gives a bound that at least n elements reach and few more (37 of 32,768 for n = 16); those are ranked by
+// counting.  Where many elements reach it (ties, a constant row) the n-th largest key is found by bisection of its
 // bits and its equals are taken in the order of their index, which bounds the work for every row.  A second launch
 // takes the best of a request's lists in the same way, or merges the lists where too many totals meet the bound.
+// Measured (B200): 256 rows of 127,999 bf16 logits, n = 16, one in seven finished: 31.4 us, of which the slices 26 (the bytes need 8.5):
+// loads, sums (8 special-function results a piece) and ranks follow one another in a block, and three blocks an SM do
+// not cover them (8 pieces a thread 33 us, 512 threads 33, blocks that stay with the next slice on its way 49).  4 rows of
+// 32,000: 8.2 us, two dependent launches of some ten dependent steps each.
 //
 // reorder.  Row r of each state becomes row parent[r], a row of the same request, as it was before the call.  A thread reads
 // its 16 bytes of all the request's moving rows and then writes them: in place without a copy of the state, and
-// rows that stay cost nothing.  Bound by HBM.
+// rows that stay cost nothing.  Bound by HBM: 384 rows of 135 KB, two thirds of them moving, 15.0 us, 4.6 TB/s.
 #pragma once
 
 #include <cfloat>

@@ -11,8 +11,11 @@
 // A block selects for one (layer, sequence, head): the bound's 32 bits two at a time by counting, then one
 // ordered pass that writes the kept tokens' places in the cache.  A block then moves K or V of one (layer, sequence,
 // head), 32 KB at a time, the next batch read ahead of the writes: a token's place never grows, and the
-// batches hold whole pages, so what is read later lies behind what is written.  Bound by HBM (scattered
-// runs of D bytes) where there are some hundred (layer, sequence, head)s, by latency below.
+// batches hold whole pages, so what is read later lies behind what is written.  Bound by scattered runs of D bytes where
+// there are some hundred (layer, sequence, head)s, by latency below.  Measured (B200): 4 layers, 12 sequences of up to 2500
+// tokens, 8 heads of 128, 1024 kept: 69 us for 206 MB, of which the moves some 47 (4.3 TB/s; runs of 128 bytes 1 KB apart do not
+// get more, whatever is in flight) and the selection the rest; one layer, 8 sequences of up to 700, 256 kept: 13.2 us.
+// (Selection by histograms of 8 bits in place of counting 18 us more; 256 threads in place of 512 for a move 3 more.)
 #pragma once
 
 #include "beams.cuh"

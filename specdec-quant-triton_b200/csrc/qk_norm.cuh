@@ -14,8 +14,13 @@
 // costs log2(lanes) shuffles and the turn none.  A forward thread takes kNormHeads heads of one token,
 // whose loads are in flight together and share angles and weights; short calls take one head a thread.
 // The backward kernel runs a fixed grid whose threads keep the sums for dw of their own elements in
-// registers over all their heads; a block adds its lanes' sums in a fixed order, a second small kernel
-// adds the blocks': no atomics, the same bits each time.
+// registers over all their heads, the next heads' pieces being copied meanwhile; a block adds its lanes' sums in a fixed order, a
+// second small kernel adds the blocks': no atomics, the same bits each time.
+//
+// Measured (B200, 32 + 8 heads of 128, bf16): 8190 tokens forward 37.4 us, 4.5 TB/s: a thread's angles and weights in fp32 take half of
+// its 128 registers, so that 16 warps an SM have loads in flight (2, 1, 8 heads a thread: 42, 46, 46 us; blocks that stay and
+// copy ahead: 47).  4093 tokens forward and backward 54.4 us, of which backward some 30 (without the copies ahead 56, three stages 57,
+// one head a thread 57).  One token: 2.2 us in a stream of launches.
 #pragma once
 
 #include "rope.cuh"
