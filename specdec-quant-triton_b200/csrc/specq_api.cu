@@ -18,7 +18,7 @@
 #include "pages.cuh"
 #include "qk_norm.cuh"
 #include "beams.cuh"
-#include "mass.cuh"
+#include "mass_api.cuh"
 #include "evict.cuh"
 
 namespace specq {

@@ -143,6 +143,36 @@ def test_mass_strange_values(cuda, ctx):
     assert torch.equal(m, one)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind,D,page", [(torch.int8, 128, 16), (torch.float8_e4m3fn, 64, 8)])
+def test_mass_of_many_rows_in_strange_company(cuda, dtype, kind, D, page):
+    """Counted rows that end inside a group of 128, dead rows, pages outside the cache, stale bytes, a tile that ends in a page."""
+    import specq
+    g = torch.Generator(device="cuda").manual_seed(6)
+    B, Q, KV, G, C = 4, 50, 2, 4, 1300 // page
+    kc, _, ks, _ = _cache(B * C + 1, page, KV, D, kind, g)
+    tbl = _table(B, C, B * C + 1, g)
+    q = torch.randn(B, Q, KV * G, D, generator=g, device="cuda").to(dtype)
+    ctx, rows = [1290, 1025, 30, 600], [50, 33, 50, 0]
+    q[0, 7, 1, 3], q[0, 40, 5, 9], q[1, 32, 2, 0] = float("nan"), float("inf"), -float("inf")
+    q[0, 20] = 0
+    for b, n in enumerate(ctx):
+        stale = tbl[b, -(-n // page):].flatten().long()
+        kc.view(torch.uint8)[stale] = 0x7F
+        ks[stale] = float("nan")
+        if n % page:
+            kc.view(torch.uint8)[tbl[b, n // page].long(), n % page:] = 0x7F
+    tbl[0, 3], tbl[1, 1024 // page], tbl[2, 0] = -1, B * C + 1, 1 << 30
+    mass = torch.rand(B, KV, C * page, generator=g, device="cuda")
+    specq.get_status()
+    m = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), mass.clone(), n_rows=_i32(rows), decay=0.75)
+    assert specq.get_status() == specq._lib.SPECQ_STATUS_BAD_INDEX
+    _check_mass(m, q, torch.nan_to_num(kc.float()) if kind != torch.int8 else kc, ks.nan_to_num(), tbl, _i32(ctx), mass, n_rows=rows, decay=0.75)
+    assert torch.equal(m[3], mass[3])
+    again = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), mass.clone(), n_rows=_i32(rows), decay=0.75)
+    assert torch.equal(m, again)
+
+
 def test_mass_context_past_its_table(cuda):
     import specq
     g = torch.Generator(device="cuda").manual_seed(3)
