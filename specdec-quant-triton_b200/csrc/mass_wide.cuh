@@ -4,8 +4,8 @@
 // shared memory (128-byte swizzle) and goes through the rows of q, 128 at a time, the next ones on their way.  Both tiles are
 // K-major, so the same bytes serve as either operand: for the rows' maxima and sums the rows stand on the lanes of
 // tensor memory (A = q, B = keys) and a thread owns a row; for the tokens' sums the tokens stand there (A = keys, B = q) and a thread
-// owns a token.  Neither needs a shuffle.  Four 128 x 128 products fill the tensor memory; one warp issues them, two
-// warpgroups take two each.
+// owns a token.  Neither needs a shuffle.  Four 128 x 128 products fill the tensor memory; one warp issues them, four
+// warpgroups take one each.
 //
 // Bound by the exponentials: one for each score and pass, 16 a clock and SM, against 8192 products; what the block does before
 // its first product (lengths, table, keys, their widening) is not covered by another block of its SM.
@@ -15,7 +15,8 @@
 
 namespace specq {
 
-constexpr int kWideThreads = 288;           // two warpgroups, and a warp that issues the products
+constexpr int kWideWork = 512;              // four warpgroups, one for each product
+constexpr int kWideThreads = kWideWork + 32;   // and a warp that issues the products
 constexpr int kWideTile = 128;
 constexpr int kWideTiles = kMassChunk / kWideTile;
 static_assert(kWideTiles == 4 && kMassRows == kWideTile, "four products of 128 columns fill the tensor memory");
@@ -30,7 +31,7 @@ struct WideSmem {
   float factor[kWideTile];                  // of each row
   float minus_lse[kWideTile];
   int lim[kWideTile];                       // the last token that a row sees; -1: none
-  float2 part[2][kWideTile];                // each warpgroup's maxima and sums
+  float2 part[kWideTiles][kWideTile];       // each warpgroup's maxima and sums
   uint32_t bad[kMassChunk / 8 / 32];        // a bit for each eight tokens that no page gives
   uint64_t full[kWideTiles];
   uint32_t tmem;
@@ -57,7 +58,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   pdl_wait();
   const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = static_cast<int>(threadIdx.x);
-  const int warp = tid >> 5, lane = tid & 31, group = warp >> 2;       // group 2: the issuing warp
+  const int warp = tid >> 5, lane = tid & 31, group = warp >> 2;       // group 4: the issuing warp
   int n, nr;
   mass_extent(p, b, chunk == 0 && h == 0 && tid == 0 && MODE == kMassStats, n, nr);
   const int first_token = chunk * kMassChunk;
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
   const int tiles = min(kWideTiles, (n - first_token + kWideTile - 1) / kWideTile);
   const int mask = (1 << p.page_log2) - 1;
 
-  if (warp == 8) {
+  if (group == 4) {
     tmem_alloc(&sm.tmem, 512u);
     tmem_relinquish();
     if (lane < kWideTiles) mbar_init(&sm.full[lane], 1u);
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
     constexpr int kChunks = D / 8;
     const int here = min(kWideTile, rows - first);
 #pragma unroll
-    for (int i = tid; i < kWideTile * kChunks; i += 256) {
+    for (int i = tid; i < kWideTile * kChunks; i += kWideWork) {
       const int r = i / kChunks, c = i - r * kChunks;
       uint8_t* dst = sm.q[side] + wide_at(r, c);
       if (r < here) {
@@ -90,10 +91,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
       }
     }
   };
-  // each row's factor (and the halves it stands for, in place), limit and lse; two threads a row
+  // each row's factor (and the halves it stands for, in place), limit and lse; four threads a row
   auto finish = [&](int first, int side, float lse) {
-    constexpr int kMine = D / 16;            // chunks of a thread
-    const int r = tid >> 1, c0 = (tid & 1) * kMine, here = min(kWideTile, rows - first);
+    constexpr int kMine = D / 32;            // chunks of a thread
+    const int r = tid >> 2, c0 = (tid & 3) * kMine, here = min(kWideTile, rows - first);
     uint32_t top = 0u;                       // the larger of the halves' magnitudes: infinity and NaN last
 #pragma unroll
     for (int c = 0; c < kMine; ++c) {
@@ -103,6 +104,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
       for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7FFFu, w[k] >> 16 & 0x7FFFu));
     }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const bool finite = top < (BF ? 0x7F80u : 0x7C00u);
     float factor = 1.f;
     if (BF || !finite) {
@@ -126,19 +128,19 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
         *at = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    if ((tid & 1) == 0) {
+    if ((tid & 3) == 0) {
       sm.factor[r] = factor;
       sm.lim[r] = r < here && finite ? base + (first + r) / p.group : -1;
       sm.minus_lse[r] = r < here ? -lse : -INFINITY;
     }
   };
   auto lse_of = [&](int first) {
-    const int r = first + (tid >> 1);
-    return MODE == kMassWeights && tid < 256 && r < rows ? p.lse[bh * p.rows + r] : INFINITY;
+    const int r = first + (tid >> 2);
+    return MODE == kMassWeights && tid < kWideWork && r < rows ? p.lse[bh * p.rows + r] : INFINITY;
   };
 
   float next_lse = lse_of(0);
-  if (tid < 256) {
+  if (tid < kWideWork) {
     request(0, 0);
     // scales of the chunk's 64 runs of eight tokens
     if (tid < kMassChunk / 8) {
@@ -155,34 +157,31 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
       const uint32_t gone = __ballot_sync(0xffffffffu, pg < 0);
       if (lane == 0) sm.bad[warp] = gone;
     }
-    // the keys: 16 bytes a thread and turn, eight turns' loads in flight
-    constexpr int kPer = D / 16, kPieces = kMassChunk * kPer;
-#pragma unroll 1
-    for (int i0 = tid; i0 < kPieces; i0 += 256 * 8) {
-      uint4 w[8];
+    // the keys: 16 bytes a thread and turn, all turns' loads in flight
+    constexpr int kPer = D / 16, kTurns = kMassChunk * kPer / kWideWork;
+    uint4 w[kTurns];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = i0 + j * 256, t = first_token + i / kPer;
-        w[j] = make_uint4(0u, 0u, 0u, 0u);
-        if (t < n) {
-          const int pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
-          if (pg >= 0 && pg < p.n_pages)
-            w[j] = *reinterpret_cast<const uint4*>(p.kc + pg * p.kv_sp + (t & mask) * p.kv_so + h * p.kv_sh + (i % kPer) * 16);
-        }
+    for (int j = 0; j < kTurns; ++j) {
+      const int i = tid + j * kWideWork, t = first_token + i / kPer;
+      w[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (t < n) {
+        const int pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
+        if (pg >= 0 && pg < p.n_pages)
+          w[j] = *reinterpret_cast<const uint4*>(p.kc + pg * p.kv_sp + (t & mask) * p.kv_so + h * p.kv_sh + (i % kPer) * 16);
       }
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = i0 + j * 256, t = i / kPer, c = (i % kPer) * 2;
-        uint4 lo, hi;
-        widen16<CT>(w[j], lo, hi);
-        uint8_t* tile = sm.keys[t / kWideTile];
-        *reinterpret_cast<uint4*>(tile + wide_at(t % kWideTile, c)) = lo;
-        *reinterpret_cast<uint4*>(tile + wide_at(t % kWideTile, c + 1)) = hi;
-      }
+    for (int j = 0; j < kTurns; ++j) {
+      const int i = tid + j * kWideWork, t = i / kPer, c = (i % kPer) * 2;
+      uint4 lo, hi;
+      widen16<CT>(w[j], lo, hi);
+      uint8_t* tile = sm.keys[t / kWideTile];
+      *reinterpret_cast<uint4*>(tile + wide_at(t % kWideTile, c)) = lo;
+      *reinterpret_cast<uint4*>(tile + wide_at(t % kWideTile, c + 1)) = hi;
     }
   }
 
-  float weight[2] = {0.f, 0.f};              // of this thread's tokens, one in each of the group's tiles
+  float weight = 0.f;                        // of this thread's token
   const uint32_t quarter = static_cast<uint32_t>(warp & 3) * 32u;      // this warp's lanes of tensor memory
   const int me = static_cast<int>(quarter) + lane;
   uint32_t tmem = 0, phase = 0;
@@ -194,10 +193,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
     tc_fence_after();
     tmem = sm.tmem;
     if (first == 0) pdl_launch_dependents(); // (tensor memory is taken: what may start now cannot keep it from this block)
-    if (tid < 256) finish(first, side, next_lse);
+    if (tid < kWideWork) finish(first, side, next_lse);
     fence_proxy_async_smem();
     __syncthreads();
-    if (warp == 8) {
+    if (group == 4) {
       if (elect_one()) {
         const uint64_t qd = sdesc_sw128(smem_u32(sm.q[side]), 16u, 1024u);
         const uint32_t idesc = idesc_f16(128u, MODE == kMassStats ? 128u : static_cast<uint32_t>(pad));
@@ -218,12 +217,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
         next_lse = lse_of(first + kWideTile);
       }
       float m = -INFINITY, l = 0.f;
-      const float mine = MODE == kMassStats ? sm.factor[me] : 1.f;
-      const int my_lim = MODE == kMassStats ? sm.lim[me] : 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = group + 2 * i;
-        if (t >= tiles) break;
+      const int t = group;
+      if (t < tiles) {
         (void)mbar_wait(&sm.full[t], phase, p.status, SPECQ_STATUS_TIMEOUT_MMA);
         tc_fence_after();
         const uint32_t at = tmem + (quarter << 16) + 128u * t;
@@ -231,76 +226,76 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
         const uint32_t gone = sm.bad[t >> 1] >> ((t & 1) * 16) & 0xFFFFu;   // 16 runs of eight tokens a tile
         const bool hidden = gone != 0u || token0 + kWideTile - 1 > base;
         if constexpr (MODE == kMassStats) {
-          if (static_cast<int>(quarter) >= here) continue;     // (a warp without rows)
-          const float* scale = sm.scale + t * (kWideTile / 8);
-#pragma unroll 1
-          for (int c = 0; c < kWideTile; c += 32) {
+          if (static_cast<int>(quarter) < here) {              // (a warp with rows)
+            const float* scale = sm.scale + t * (kWideTile / 8);
+            const float mine = sm.factor[me];
+            const int my_lim = sm.lim[me];
             uint32_t v[2][16];
-            tmem_ld16(at + c, v[0]);
-            tmem_ld16(at + c + 16, v[1]);
-            const float4 x4 = *reinterpret_cast<const float4*>(scale + c / 8);
-            const float x[4] = {x4.x * mine, x4.y * mine, x4.z * mine, x4.w * mine};
-            tmem_wait_ld();
-            if (hidden) {
+            tmem_ld16(at, v[0]);
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if ((gone >> ((c + k) / 8) & 1u) != 0u || token0 + c + k > my_lim) v[k / 16][k % 16] = 0xFF800000u;
+            for (int c = 0; c < kWideTile; c += 16) {          // the next 16 columns on their way
+              uint32_t(&u)[16] = v[(c / 16) & 1];
+              tmem_wait_ld();
+              if (c + 16 < kWideTile) tmem_ld16(at + c + 16, v[(c / 16 + 1) & 1]);
+              const float2 xs = *reinterpret_cast<const float2*>(scale + c / 8);
+              const float x[2] = {BF ? xs.x * mine : xs.x, BF ? xs.y * mine : xs.y};
+              if (hidden) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  if ((gone >> ((c + k) / 8) & 1u) != 0u || token0 + c + k > my_lim) u[k] = 0xFF800000u;
+              }
+              float top = m;
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float y = __uint_as_float(u[j * 8]);
+#pragma unroll
+                for (int k = 1; k < 8; ++k) y = fmaxf(y, __uint_as_float(u[j * 8 + k]));
+                top = fmaxf(top, y * x[j]);
+              }
+              const float z = top == -INFINITY ? 0.f : -top;
+              float2 sum = {l * exp2_fast(m + z), 0.f};         // m = -inf: 0
+#pragma unroll
+              for (int k = 0; k < 16; k += 2) {
+                const float2 d = __ffma2_rn(make_float2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), make_float2(x[k / 8], x[k / 8]), make_float2(z, z));
+                sum = __fadd2_rn(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+              }
+              l = sum.x + sum.y;
+              m = top;
             }
-            float top = m;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float u = __uint_as_float(v[j / 2][(j % 2) * 8]);
-#pragma unroll
-              for (int k = 1; k < 8; ++k) u = fmaxf(u, __uint_as_float(v[j / 2][(j % 2) * 8 + k]));
-              top = fmaxf(top, u * x[j]);
-            }
-            const float z = top == -INFINITY ? 0.f : -top;
-            float2 sum = {l * exp2_fast(m + z), 0.f};           // m = -inf: 0
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) {
-              const float2 d = __ffma2_rn(make_float2(__uint_as_float(v[k / 16][k % 16]), __uint_as_float(v[k / 16][k % 16 + 1])),
-                                          make_float2(x[k / 8], x[k / 8]), make_float2(z, z));
-              sum = __fadd2_rn(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
-            }
-            l = sum.x + sum.y;
-            m = top;
           }
         } else {
           const float x = sm.scale[t * (kWideTile / 8) + me / 8];
           float2 sum = {0.f, 0.f};
-#pragma unroll 1
-          for (int c = 0; c < pad; c += 16) {
-            uint32_t v[16];
-            tmem_ld16(at + c, v);
-            float lse[16];
+          uint32_t v[2][16];
+          tmem_ld16(at, v[0]);
+#pragma unroll
+          for (int c = 0; c < kWideTile; c += 16) {
+            if (c >= pad) break;
+            uint32_t(&u)[16] = v[(c / 16) & 1];
+            tmem_wait_ld();
+            if (c + 16 < pad) tmem_ld16(at + c + 16, v[(c / 16 + 1) & 1]);
 #pragma unroll
             for (int k = 0; k < 16; k += 4) {
-              const float4 u = *reinterpret_cast<const float4*>(sm.minus_lse + c + k);
-              lse[k] = u.x; lse[k + 1] = u.y; lse[k + 2] = u.z; lse[k + 3] = u.w;
-            }
-            tmem_wait_ld();
-            if constexpr (BF) {
-#pragma unroll
-              for (int k = 0; k < 16; k += 4) {
-                const float4 u = *reinterpret_cast<const float4*>(sm.factor + c + k);
-                v[k] = __float_as_uint(__uint_as_float(v[k]) * u.x);
-                v[k + 1] = __float_as_uint(__uint_as_float(v[k + 1]) * u.y);
-                v[k + 2] = __float_as_uint(__uint_as_float(v[k + 2]) * u.z);
-                v[k + 3] = __float_as_uint(__uint_as_float(v[k + 3]) * u.w);
+              float4 lse = *reinterpret_cast<const float4*>(sm.minus_lse + c + k);
+              float2 s0 = make_float2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), s1 = make_float2(__uint_as_float(u[k + 2]), __uint_as_float(u[k + 3]));
+              if constexpr (BF) {
+                const float4 f = *reinterpret_cast<const float4*>(sm.factor + c + k);
+                s0 = __fmul2_rn(s0, make_float2(f.x, f.y));
+                s1 = __fmul2_rn(s1, make_float2(f.z, f.w));
               }
-            }
-            if (hidden) {
-#pragma unroll
-              for (int k = 0; k < 16; ++k)
-                if (token0 + me > sm.lim[c + k]) lse[k] = -INFINITY;
-            }
-#pragma unroll
-            for (int k = 0; k < 16; k += 2) {
-              const float2 d = __ffma2_rn(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), make_float2(x, x), make_float2(lse[k], lse[k + 1]));
-              sum = __fadd2_rn(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
+              if (hidden) {
+                const int4 lim = *reinterpret_cast<const int4*>(sm.lim + c + k);
+                if (token0 + me > lim.x) lse.x = -INFINITY;
+                if (token0 + me > lim.y) lse.y = -INFINITY;
+                if (token0 + me > lim.z) lse.z = -INFINITY;
+                if (token0 + me > lim.w) lse.w = -INFINITY;
+              }
+              const float2 d0 = __ffma2_rn(s0, make_float2(x, x), make_float2(lse.x, lse.y)), d1 = __ffma2_rn(s1, make_float2(x, x), make_float2(lse.z, lse.w));
+              sum = __fadd2_rn(sum, make_float2(exp2_fast(d0.x), exp2_fast(d0.y)));
+              sum = __fadd2_rn(sum, make_float2(exp2_fast(d1.x), exp2_fast(d1.y)));
             }
           }
-          if ((gone >> (me / 8) & 1u) == 0u) weight[i] += sum.x + sum.y;
+          if ((gone >> (me / 8) & 1u) == 0u) weight += sum.x + sum.y;
         }
       }
       if constexpr (MODE == kMassStats) sm.part[group][me] = make_float2(m, l);
@@ -308,27 +303,24 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
     if constexpr (MODE == kMassStats) {
       __syncthreads();
       if (tid < here) {
-        float2 x = join_stats(sm.part[0][tid], sm.part[1][tid]);
+        float2 x = sm.part[0][tid];
+#pragma unroll
+        for (int g = 1; g < kWideTiles; ++g) x = join_stats(x, sm.part[g][tid]);
         if (sm.lim[tid] < 0) x = make_float2(-INFINITY, 0.f);
         p.stats[(bh * p.chunks + chunk) * p.rows + first + tid] = x;
       }
     }
   }
   if constexpr (MODE == kMassWeights) {
-    if (warp < 8) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int t = first_token + (group + 2 * i) * kWideTile + me;
-        if (t < n) {
-          float* at = p.mass + b * p.m_sb + h * p.m_sh + t;
-          *at = fmaf(*at, p.decay, weight[i]);
-        }
-      }
+    const int t = first_token + tid;         // group * 128 + me
+    if (tid < kWideWork && t < n) {
+      float* at = p.mass + b * p.m_sb + h * p.m_sh + t;
+      *at = fmaf(*at, p.decay, weight);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (group == 4) {
     tc_fence_after();
     tmem_dealloc(tmem, 512u);
   }
