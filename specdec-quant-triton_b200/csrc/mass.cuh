@@ -59,7 +59,7 @@ struct MassParams {
   int* status;
   int64_t q_sb, q_st, q_sh, kv_sp, kv_so, kv_sh, s_sp, s_sh, bt_sb, m_sb, m_sh;
   int q_len, group, h_kv, page_log2, n_pages, bt_cols, chunks, rows;   // rows = q_len * group
-  int chunk_tiles;         // up to 16 rows in several launches: 256 tokens each, a block's tiles
+  int chunk_tiles;         // a block's tokens in several launches, 256 each
   float sm_log2, decay;
 };
 
@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(256) mass_join_kernel(const __grid_constant__ 
   mass_extent(p, b, false, n, nr);
   if (r >= nr * p.group) return;
   const int64_t bh = static_cast<int64_t>(b) * p.h_kv + h;
-  const int chunks = (n - 1) / kMassChunk + 1;
+  const int chunks = (n - 1) / (p.chunk_tiles * kMassThreads) + 1;
   float2 x = make_float2(-INFINITY, 0.f);
   for (int c = lane; c < chunks; c += 32) x = join_stats(x, p.stats[(bh * p.chunks + c) * p.rows + r]);
 #pragma unroll

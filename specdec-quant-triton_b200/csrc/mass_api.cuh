@@ -24,7 +24,11 @@ inline bool mass_plan(int B, int H_KV, int rows, int tokens, int* chunk_tiles, i
   *chunks = ceil_div(tokens, kMassChunk);
   // up to 16 rows a cluster is the faster only while most SMs would be idle: 1 x 4096 tokens of 8 heads 8.5 us against 9.2, but 8 x 1024
   // 10.8 against 9.9 and 32 x 4096 76 against 52
-  if (rows >= kMassWide) return false;
+  if (rows >= kMassWide) {
+    *chunk_tiles = kWideChunk / kMassThreads;
+    *chunks = ceil_div(tokens, kWideChunk);
+    return false;
+  }
   if (*chunks <= kMassCluster && (rows > kMassFew || *chunks == 1 || static_cast<int64_t>(B) * H_KV * *chunks <= kMassSms / 2)) return true;
   if (rows <= kMassFew) {            // long blocks pay for q once; three blocks an SM at least, if the call has them
     int tiles = 8;

@@ -1,38 +1,41 @@
 // mass_wide.cuh -- the products of many query rows with the cached keys for attention_mass (mass.cuh) on tcgen05.
 //
-// A block takes 512 tokens of one sequence and KV head.  It widens their keys once, exactly, to fp16 tiles of [128 tokens x D] in
-// shared memory (128-byte swizzle) and goes through the rows of q, 128 at a time, the next ones on their way.  Both tiles are
+// A block takes 256 tokens of one sequence and KV head.  It widens their keys once, exactly, to fp16 tiles of [128 tokens x D] in
+// shared memory (128-byte swizzle) and goes through the rows of q, 128 at a time.  Both tiles are
 // K-major, so the same bytes serve as either operand: for the rows' maxima and sums the rows stand on the lanes of
 // tensor memory (A = q, B = keys) and a thread owns a row; for the tokens' sums the tokens stand there (A = keys, B = q) and a thread
-// owns a token.  Neither needs a shuffle.  Four 128 x 128 products fill the tensor memory; one warp issues them, four
-// warpgroups take one each.
+// owns a token.  Neither needs a shuffle.  One warp issues the two 128 x 128 products, two warpgroups take one
+// each; the next rows of q come into their place as soon as both products are done.
 //
-// Bound by the exponentials: one for each score and pass, 16 a clock and SM, against 8192 products; what the block does before
-// its first product (lengths, table, keys, their widening) is not covered by another block of its SM.
+// Bound by the exponentials: one for each score and pass, 16 a clock and SM, against 8192 products.  Two blocks an SM cover
+// for one another what comes before a block's first product (lengths, table, keys, their widening): blocks of 512 tokens,
+// one an SM, took 138 us for the case below.
 #pragma once
+
+#include <type_traits>
 
 #include "mass.cuh"
 
 namespace specq {
 
-constexpr int kWideWork = 512;              // four warpgroups, one for each product
+constexpr int kWideWork = 256;              // two warpgroups, one for each product
 constexpr int kWideThreads = kWideWork + 32;   // and a warp that issues the products
 constexpr int kWideTile = 128;
-constexpr int kWideTiles = kMassChunk / kWideTile;
-static_assert(kWideTiles == 4 && kMassRows == kWideTile, "four products of 128 columns fill the tensor memory");
+constexpr int kWideTiles = kWideWork / kWideTile;
+constexpr int kWideChunk = kWideTiles * kWideTile;   // tokens of a block
+constexpr uint32_t kWideColumns = 128u * kWideTiles; // of tensor memory: half of it
 
 template <int D>
 struct WideSmem {
   static constexpr int kTileBytes = (D / 64) * kWideTile * 128;
   uint8_t keys[kWideTiles][kTileBytes];
-  uint8_t q[2][kTileBytes];
-  float4 dummy_align;
-  float scale[kMassChunk / 8];              // of each eight tokens: their page's scale, times sm_scale log2 e
+  uint8_t q[kTileBytes];
+  float scale[kWideChunk / 8];              // of each eight tokens: their page's scale, times sm_scale log2 e
   float factor[kWideTile];                  // of each row
   float minus_lse[kWideTile];
   int lim[kWideTile];                       // the last token that a row sees; -1: none
   float2 part[kWideTiles][kWideTile];       // each warpgroup's maxima and sums
-  uint32_t bad[kMassChunk / 8 / 32];        // a bit for each eight tokens that no page gives
+  uint32_t bad[(kWideChunk / 8 + 31) / 32]; // a bit for each eight tokens that no page gives
   uint64_t full[kWideTiles];
   uint32_t tmem;
 };
@@ -52,59 +55,63 @@ __device__ __forceinline__ uint32_t wide_at(int r, int c) {
 }
 
 template <bool BF, int CT, int D, int MODE>
-__global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid_constant__ MassParams p) {
+__global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid_constant__ MassParams p) {
   using Smem = WideSmem<D>;
   extern __shared__ uint8_t raw_smem[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   pdl_wait();
   const int chunk = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = static_cast<int>(threadIdx.x);
-  const int warp = tid >> 5, lane = tid & 31, group = warp >> 2;       // group 4: the issuing warp
+  const int warp = tid >> 5, lane = tid & 31, group = warp >> 2;       // the last group: the issuing warp
   int n, nr;
   mass_extent(p, b, chunk == 0 && h == 0 && tid == 0 && MODE == kMassStats, n, nr);
-  const int first_token = chunk * kMassChunk;
+  const int first_token = chunk * kWideChunk;
   if (nr == 0 || first_token >= n) return;
   const int64_t bh = static_cast<int64_t>(b) * p.h_kv + h;
   const int rows = nr * p.group, base = n - nr;
   const int tiles = min(kWideTiles, (n - first_token + kWideTile - 1) / kWideTile);
   const int mask = (1 << p.page_log2) - 1;
 
-  if (group == 4) {
-    tmem_alloc(&sm.tmem, 512u);
+  if (group == kWideTiles) {
+    tmem_alloc(&sm.tmem, kWideColumns);
     tmem_relinquish();
     if (lane < kWideTiles) mbar_init(&sm.full[lane], 1u);
     fence_barrier_init();
   }
-  // q's rows [first, first + 128) of this head, as they are, into buffer `side`; rows past the last are zeros
-  auto request = [&](int first, int side) {
-    constexpr int kChunks = D / 8;
-    const int here = min(kWideTile, rows - first);
+  // q's rows [first, first + 128) of this head, as they are, two threads a row; rows past the last are zeros
+  constexpr int kMine = D / 16;              // 16-byte chunks of a thread
+  const int my_row = tid >> 1, my_chunk = (tid & 1) * kMine;
+  auto request = [&](int first) {
+    const int r = first + my_row;
+    if (r < rows) {
+      const int row = r / p.group, head = h * p.group + r - row * p.group;
+      const __half* src = static_cast<const __half*>(p.q) + my_chunk * 8 + head * p.q_sh +
+                          (p.q_sb != 0 ? b * p.q_sb + row * p.q_st : (static_cast<int64_t>(b) * p.q_len + row) * p.q_st);
 #pragma unroll
-    for (int i = tid; i < kWideTile * kChunks; i += kWideWork) {
-      const int r = i / kChunks, c = i - r * kChunks;
-      uint8_t* dst = sm.q[side] + wide_at(r, c);
-      if (r < here) {
-        const int row = (first + r) / p.group, head = h * p.group + (first + r) - row * p.group;
-        const int64_t at = (p.q_sb != 0 ? b * p.q_sb + row * p.q_st : (static_cast<int64_t>(b) * p.q_len + row) * p.q_st) + head * p.q_sh;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(static_cast<const __half*>(p.q) + at + c * 8) : "memory");
-      } else {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
-      }
+      for (int c = 0; c < kMine; ++c)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(sm.q + wide_at(my_row, my_chunk + c))), "l"(src + c * 8) : "memory");
+    } else {
+#pragma unroll
+      for (int c = 0; c < kMine; ++c) *reinterpret_cast<uint4*>(sm.q + wide_at(my_row, my_chunk + c)) = make_uint4(0u, 0u, 0u, 0u);
     }
   };
-  // each row's factor (and the halves it stands for, in place), limit and lse; four threads a row
-  auto finish = [&](int first, int side, float lse) {
-    constexpr int kMine = D / 32;            // chunks of a thread
-    const int r = tid >> 2, c0 = (tid & 3) * kMine, here = min(kWideTile, rows - first);
-    uint32_t top = 0u;                       // the larger of the halves' magnitudes: infinity and NaN last
+  // each row's factor (and the halves it stands for, in place), limit and lse, by the threads that asked for it
+  auto finish = [&](int first, float lse) {
+    using W2 = typename std::conditional<BF, __nv_bfloat162, __half2>::type;
+    uint32_t seen = 0u;                      // the largest magnitudes, a NaN kept
+    auto add = [&](uint32_t w) {
+      const W2 m = __hmax2_nan(*reinterpret_cast<const W2*>(&seen), __habs2(*reinterpret_cast<const W2*>(&w)));
+      seen = *reinterpret_cast<const uint32_t*>(&m);
+    };
 #pragma unroll
     for (int c = 0; c < kMine; ++c) {
-      const uint4 u = *reinterpret_cast<const uint4*>(sm.q[side] + wide_at(r, c0 + c));
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7FFFu, w[k] >> 16 & 0x7FFFu));
+      const uint4 u = *reinterpret_cast<const uint4*>(sm.q + wide_at(my_row, my_chunk + c));
+      add(u.x);
+      add(u.y);
+      add(u.z);
+      add(u.w);
     }
+    uint32_t top = max(seen & 0x7FFFu, seen >> 16 & 0x7FFFu);     // magnitudes order as integers: infinity and NaN last
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const bool finite = top < (BF ? 0x7F80u : 0x7C00u);
     float factor = 1.f;
     if (BF || !finite) {
@@ -117,7 +124,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
       }
 #pragma unroll
       for (int c = 0; c < kMine; ++c) {
-        uint4* at = reinterpret_cast<uint4*>(sm.q[side] + wide_at(r, c0 + c));
+        uint4* at = reinterpret_cast<uint4*>(sm.q + wide_at(my_row, my_chunk + c));
         const uint4 u = *at;
         uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -128,22 +135,23 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
         *at = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
-    if ((tid & 3) == 0) {
-      sm.factor[r] = factor;
-      sm.lim[r] = r < here && finite ? base + (first + r) / p.group : -1;
-      sm.minus_lse[r] = r < here ? -lse : -INFINITY;
+    if ((tid & 1) == 0) {
+      const bool there = first + my_row < rows;
+      sm.factor[my_row] = factor;
+      sm.lim[my_row] = there && finite ? base + (first + my_row) / p.group : -1;
+      sm.minus_lse[my_row] = there ? -lse : -INFINITY;
     }
   };
   auto lse_of = [&](int first) {
-    const int r = first + (tid >> 2);
+    const int r = first + my_row;
     return MODE == kMassWeights && tid < kWideWork && r < rows ? p.lse[bh * p.rows + r] : INFINITY;
   };
 
   float next_lse = lse_of(0);
   if (tid < kWideWork) {
-    request(0, 0);
-    // scales of the chunk's 64 runs of eight tokens
-    if (tid < kMassChunk / 8) {
+    request(0);
+    // scales of the chunk's 32 runs of eight tokens
+    if (tid < kWideChunk / 8) {
       const int t = first_token + tid * 8;
       int pg = -1;
       if (t < n) {
@@ -157,27 +165,24 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
       const uint32_t gone = __ballot_sync(0xffffffffu, pg < 0);
       if (lane == 0) sm.bad[warp] = gone;
     }
-    // the keys: 16 bytes a thread and turn, all turns' loads in flight
-    constexpr int kPer = D / 16, kTurns = kMassChunk * kPer / kWideWork;
-    uint4 w[kTurns];
+    // the keys, a token a thread
+    static_assert(kWideChunk == kWideWork, "a thread for each token");
+    constexpr int kPieces = D / 16;
+    const int t = first_token + tid;
+    uint4 w[kPieces];
+    int pg = -1;
+    if (t < n) pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
+    const bool there = pg >= 0 && pg < p.n_pages;
+    const uint8_t* src = p.kc + (there ? pg * p.kv_sp + (t & mask) * p.kv_so + h * p.kv_sh : 0);
 #pragma unroll
-    for (int j = 0; j < kTurns; ++j) {
-      const int i = tid + j * kWideWork, t = first_token + i / kPer;
-      w[j] = make_uint4(0u, 0u, 0u, 0u);
-      if (t < n) {
-        const int pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
-        if (pg >= 0 && pg < p.n_pages)
-          w[j] = *reinterpret_cast<const uint4*>(p.kc + pg * p.kv_sp + (t & mask) * p.kv_so + h * p.kv_sh + (i % kPer) * 16);
-      }
-    }
+    for (int j = 0; j < kPieces; ++j) w[j] = there ? *reinterpret_cast<const uint4*>(src + j * 16) : make_uint4(0u, 0u, 0u, 0u);
+    uint8_t* tile = sm.keys[tid / kWideTile];
 #pragma unroll
-    for (int j = 0; j < kTurns; ++j) {
-      const int i = tid + j * kWideWork, t = i / kPer, c = (i % kPer) * 2;
+    for (int j = 0; j < kPieces; ++j) {
       uint4 lo, hi;
       widen16<CT>(w[j], lo, hi);
-      uint8_t* tile = sm.keys[t / kWideTile];
-      *reinterpret_cast<uint4*>(tile + wide_at(t % kWideTile, c)) = lo;
-      *reinterpret_cast<uint4*>(tile + wide_at(t % kWideTile, c + 1)) = hi;
+      *reinterpret_cast<uint4*>(tile + wide_at(tid % kWideTile, 2 * j)) = lo;
+      *reinterpret_cast<uint4*>(tile + wide_at(tid % kWideTile, 2 * j + 1)) = hi;
     }
   }
 
@@ -185,7 +190,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
   const uint32_t quarter = static_cast<uint32_t>(warp & 3) * 32u;      // this warp's lanes of tensor memory
   const int me = static_cast<int>(quarter) + lane;
   uint32_t tmem = 0, phase = 0;
-  for (int first = 0, side = 0; first < rows; first += kWideTile, side ^= 1, phase ^= 1u) {
+  for (int first = 0; first < rows; first += kWideTile, phase ^= 1u) {
     const int here = min(kWideTile, rows - first), pad = (here + 15) & ~15;
     asm volatile("cp.async.wait_all;" ::: "memory");
     tc_fence_before();
@@ -193,12 +198,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
     tc_fence_after();
     tmem = sm.tmem;
     if (first == 0) pdl_launch_dependents(); // (tensor memory is taken: what may start now cannot keep it from this block)
-    if (tid < kWideWork) finish(first, side, next_lse);
+    if (tid < kWideWork) finish(first, next_lse);
     fence_proxy_async_smem();
     __syncthreads();
-    if (group == 4) {
+    if (group == kWideTiles) {
       if (elect_one()) {
-        const uint64_t qd = sdesc_sw128(smem_u32(sm.q[side]), 16u, 1024u);
+        const uint64_t qd = sdesc_sw128(smem_u32(sm.q), 16u, 1024u);
         const uint32_t idesc = idesc_f16(128u, MODE == kMassStats ? 128u : static_cast<uint32_t>(pad));
         for (int t = 0; t < tiles; ++t) {
           const uint64_t kd = sdesc_sw128(smem_u32(sm.keys[t]), 16u, 1024u);
@@ -212,14 +217,16 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
       }
       __syncwarp();
     } else {
-      if (first + kWideTile < rows) {
-        request(first + kWideTile, side ^ 1);
-        next_lse = lse_of(first + kWideTile);
-      }
       float m = -INFINITY, l = 0.f;
       const int t = group;
+      const bool more = first + kWideTile < rows;
+      if (more) {                              // q's place is free when every product has read it
+        for (int i = 0; i < tiles; ++i) (void)mbar_wait(&sm.full[i], phase, p.status, SPECQ_STATUS_TIMEOUT_MMA);
+        request(first + kWideTile);
+        next_lse = lse_of(first + kWideTile);
+      }
       if (t < tiles) {
-        (void)mbar_wait(&sm.full[t], phase, p.status, SPECQ_STATUS_TIMEOUT_MMA);
+        if (!more) (void)mbar_wait(&sm.full[t], phase, p.status, SPECQ_STATUS_TIMEOUT_MMA);
         tc_fence_after();
         const uint32_t at = tmem + (quarter << 16) + 128u * t;
         const int token0 = first_token + t * kWideTile;
@@ -320,9 +327,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) mass_wide_kernel(const __grid
   }
   tc_fence_before();
   __syncthreads();
-  if (group == 4) {
+  if (group == kWideTiles) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512u);
+    tmem_dealloc(tmem, kWideColumns);
   }
 }
 
