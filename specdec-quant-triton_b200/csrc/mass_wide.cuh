@@ -31,9 +31,10 @@ struct WideSmem {
   uint8_t keys[kWideTiles][kTileBytes];
   uint8_t q[kTileBytes];
   float scale[kWideChunk / 8];              // of each eight tokens: their page's scale, times sm_scale log2 e
-  float factor[kWideTile];                  // of each row
-  float minus_lse[kWideTile];
-  int lim[kWideTile];                       // the last token that a row sees; -1: none
+  // of each of the 128 rows at work and, while some warps are not yet done with those, of the next
+  float factor[2][kWideTile];
+  float minus_lse[2][kWideTile];
+  int lim[2][kWideTile];                    // the last token that a row sees; -1: none
   float2 part[kWideTiles][kWideTile];       // each warpgroup's maxima and sums
   uint32_t bad[(kWideChunk / 8 + 31) / 32]; // a bit for each eight tokens that no page gives
   uint64_t full[kWideTiles];
@@ -95,7 +96,7 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
     }
   };
   // each row's factor (and the halves it stands for, in place), limit and lse, by the threads that asked for it
-  auto finish = [&](int first, float lse) {
+  auto finish = [&](int first, int side, float lse) {
     using W2 = typename std::conditional<BF, __nv_bfloat162, __half2>::type;
     uint32_t seen = 0u;                      // the largest magnitudes, a NaN kept
     auto add = [&](uint32_t w) {
@@ -137,9 +138,9 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
     }
     if ((tid & 1) == 0) {
       const bool there = first + my_row < rows;
-      sm.factor[my_row] = factor;
-      sm.lim[my_row] = there && finite ? base + (first + my_row) / p.group : -1;
-      sm.minus_lse[my_row] = there ? -lse : -INFINITY;
+      sm.factor[side][my_row] = factor;
+      sm.lim[side][my_row] = there && finite ? base + (first + my_row) / p.group : -1;
+      sm.minus_lse[side][my_row] = there ? -lse : -INFINITY;
     }
   };
   auto lse_of = [&](int first) {
@@ -165,25 +166,30 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
       const uint32_t gone = __ballot_sync(0xffffffffu, pg < 0);
       if (lane == 0) sm.bad[warp] = gone;
     }
-    // the keys, a token a thread
-    static_assert(kWideChunk == kWideWork, "a thread for each token");
-    constexpr int kPieces = D / 16;
-    const int t = first_token + tid;
-    uint4 w[kPieces];
-    int pg = -1;
-    if (t < n) pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
-    const bool there = pg >= 0 && pg < p.n_pages;
-    const uint8_t* src = p.kc + (there ? pg * p.kv_sp + (t & mask) * p.kv_so + h * p.kv_sh : 0);
+    // the keys, two threads a token, 32 bytes side by side at a time
+    static_assert(kWideChunk == kWideWork, "two tokens for each pair of threads");
+    constexpr int kPieces = D / 32;
+    uint4 w[2][kPieces];
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) w[j] = there ? *reinterpret_cast<const uint4*>(src + j * 16) : make_uint4(0u, 0u, 0u, 0u);
-    uint8_t* tile = sm.keys[tid / kWideTile];
+    for (int i = 0; i < 2; ++i) {
+      const int t = first_token + i * kWideTile + (tid >> 1);
+      int pg = -1;
+      if (t < n) pg = p.bt[b * p.bt_sb + (t >> p.page_log2)];
+      const bool there = pg >= 0 && pg < p.n_pages;
+      const uint8_t* src = p.kc + (there ? pg * p.kv_sp + (t & mask) * p.kv_so + h * p.kv_sh : 0) + (tid & 1) * 16;
 #pragma unroll
-    for (int j = 0; j < kPieces; ++j) {
-      uint4 lo, hi;
-      widen16<CT>(w[j], lo, hi);
-      *reinterpret_cast<uint4*>(tile + wide_at(tid % kWideTile, 2 * j)) = lo;
-      *reinterpret_cast<uint4*>(tile + wide_at(tid % kWideTile, 2 * j + 1)) = hi;
+      for (int j = 0; j < kPieces; ++j) w[i][j] = there ? *reinterpret_cast<const uint4*>(src + j * 32) : make_uint4(0u, 0u, 0u, 0u);
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        const int c = 4 * j + 2 * (tid & 1);
+        uint4 lo, hi;
+        widen16<CT>(w[i][j], lo, hi);
+        *reinterpret_cast<uint4*>(sm.keys[i] + wide_at(tid >> 1, c)) = lo;
+        *reinterpret_cast<uint4*>(sm.keys[i] + wide_at(tid >> 1, c + 1)) = hi;
+      }
   }
 
   float weight = 0.f;                        // of this thread's token
@@ -192,15 +198,15 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
   uint32_t tmem = 0, phase = 0;
   for (int first = 0; first < rows; first += kWideTile, phase ^= 1u) {
     const int here = min(kWideTile, rows - first), pad = (here + 15) & ~15;
+    const int side = static_cast<int>(phase);
     asm volatile("cp.async.wait_all;" ::: "memory");
+    if (tid < kWideWork) finish(first, side, next_lse);   // (a thread's own bytes)
+    fence_proxy_async_smem();
     tc_fence_before();
-    __syncthreads();                         // q's bytes are there; the products before have been read
+    __syncthreads();                         // both operands are there; the products before have been read
     tc_fence_after();
     tmem = sm.tmem;
     if (first == 0) pdl_launch_dependents(); // (tensor memory is taken: what may start now cannot keep it from this block)
-    if (tid < kWideWork) finish(first, next_lse);
-    fence_proxy_async_smem();
-    __syncthreads();
     if (group == kWideTiles) {
       if (elect_one()) {
         const uint64_t qd = sdesc_sw128(smem_u32(sm.q), 16u, 1024u);
@@ -235,8 +241,8 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
         if constexpr (MODE == kMassStats) {
           if (static_cast<int>(quarter) < here) {              // (a warp with rows)
             const float* scale = sm.scale + t * (kWideTile / 8);
-            const float mine = sm.factor[me];
-            const int my_lim = sm.lim[me];
+            const float mine = sm.factor[side][me];
+            const int my_lim = sm.lim[side][me];
             uint32_t v[2][16];
             tmem_ld16(at, v[0]);
 #pragma unroll
@@ -283,15 +289,15 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
             if (c + 16 < pad) tmem_ld16(at + c + 16, v[(c / 16 + 1) & 1]);
 #pragma unroll
             for (int k = 0; k < 16; k += 4) {
-              float4 lse = *reinterpret_cast<const float4*>(sm.minus_lse + c + k);
+              float4 lse = *reinterpret_cast<const float4*>(sm.minus_lse[side] + c + k);
               float2 s0 = make_float2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), s1 = make_float2(__uint_as_float(u[k + 2]), __uint_as_float(u[k + 3]));
               if constexpr (BF) {
-                const float4 f = *reinterpret_cast<const float4*>(sm.factor + c + k);
+                const float4 f = *reinterpret_cast<const float4*>(sm.factor[side] + c + k);
                 s0 = __fmul2_rn(s0, make_float2(f.x, f.y));
                 s1 = __fmul2_rn(s1, make_float2(f.z, f.w));
               }
               if (hidden) {
-                const int4 lim = *reinterpret_cast<const int4*>(sm.lim + c + k);
+                const int4 lim = *reinterpret_cast<const int4*>(sm.lim[side] + c + k);
                 if (token0 + me > lim.x) lse.x = -INFINITY;
                 if (token0 + me > lim.y) lse.y = -INFINITY;
                 if (token0 + me > lim.z) lse.z = -INFINITY;
@@ -313,7 +319,7 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
         float2 x = sm.part[0][tid];
 #pragma unroll
         for (int g = 1; g < kWideTiles; ++g) x = join_stats(x, sm.part[g][tid]);
-        if (sm.lim[tid] < 0) x = make_float2(-INFINITY, 0.f);
+        if (sm.lim[side][tid] < 0) x = make_float2(-INFINITY, 0.f);
         p.stats[(bh * p.chunks + chunk) * p.rows + first + tid] = x;
       }
     }

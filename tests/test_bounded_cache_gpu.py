@@ -51,7 +51,8 @@ def _check_mass(got, q, kc, ks, tbl, ctx, mass, **kw):
 CASES = [  # B, Q, KV, G, D, page, contexts
     (1, 1, 1, 1, 64, 8, [1]), (1, 1, 8, 4, 128, 16, [37]), (3, 1, 2, 8, 64, 32, [5, 256, 257]), (2, 9, 2, 4, 128, 16, [700, 9]),
     (4, 1, 1, 4, 128, 64, [2000, 1, 0, 513]), (2, 64, 1, 8, 64, 128, [900, 64]), (2, 33, 2, 3, 128, 8, [300, 40]),
-    (1, 5, 1, 1, 64, 16, [3]), (2, 300, 1, 2, 64, 32, [400, 300]), (1, 1, 2, 2, 128, 128, [5000]), (3, 2, 4, 1, 64, 64, [4097, 63, 2500])]
+    (1, 5, 1, 1, 64, 16, [3]), (2, 300, 1, 2, 64, 32, [400, 300]), (1, 1, 2, 2, 128, 128, [5000]), (3, 2, 4, 1, 64, 64, [4097, 63, 2500]),
+    (1, 9, 1, 4, 128, 64, [5000]), (2, 20, 1, 4, 64, 8, [4500, 100]), (1, 48, 1, 8, 128, 16, [4700]), (2, 24, 2, 4, 64, 16, [257, 90])]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
