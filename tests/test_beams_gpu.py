@@ -48,7 +48,7 @@ def _rows(B, K, V, dtype, seed, spread=3.0):
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
-@pytest.mark.parametrize("B,K,V,n", [(1, 1, 1, 1), (2, 3, 50, 1), (3, 64, 4, 1), (1, 1, 5, 8), (1, 4, 32000, 4), (3, 5, 999, 10), (2, 8, 50257, 16), (2, 3, 16384, 6),
+@pytest.mark.parametrize("B,K,V,n", [(1, 1, 1, 1), (2, 3, 50, 1), (3, 64, 4, 1), (1, 8, 362, 16), (4, 2, 1299, 4), (1, 3, 25785, 6), (2, 16, 200, 32), (1, 1, 5, 8), (1, 4, 32000, 4), (3, 5, 999, 10), (2, 8, 50257, 16), (2, 3, 16384, 6),
                                      (2, 2, 16385, 128), (5, 64, 333, 128), (1, 64, 20001, 64), (40, 4, 17000, 8), (1, 2, 200003, 4)])
 def test_select_matches_oracle(cuda, dtype, B, K, V, n):
     import specq
