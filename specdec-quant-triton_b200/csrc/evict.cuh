@@ -25,7 +25,11 @@ namespace specq {
 
 constexpr int kEvictSelThreads = 256;
 constexpr int kEvictRun = 4;                                        // tokens a thread takes in the ordered pass
-constexpr int kEvictStage = 12 * 1024;                              // keys held in shared memory (48 KB)
+// Keys held in shared memory: 192 KB of them where the rows leave each SM one block or two, else 48 KB, so that four blocks of
+// a wide table's short rows stay on an SM. (8 rows of 16384 tokens 75 us against 123 with 48 KB, 256 rows of 32768 213 against
+// 278; past the limit each digit reads the masses again.)
+constexpr int kEvictStage = 48 * 1024;
+constexpr int kEvictStageMany = 12 * 1024;
 constexpr int kEvictMoveThreads = 512;
 constexpr int kEvictPieces = 4;                                     // 16-byte pieces a thread moves at a time
 
@@ -43,7 +47,8 @@ struct EvictParams {
   int32_t* first;          // workspace [L, B, H_KV]: the first kept token that moves; keep: none; -1: the row stays
   int* status;
   int64_t kv_sl, kv_sp, kv_so, kv_sh, s_sl, s_sp, s_sh, bt_sb, m_sl, m_sb, m_sh;
-  int n_pages, bt_cols, B, h_kv, page_log2, keep, recent, staged;
+  int n_pages, bt_cols, B, h_kv, page_log2, keep, recent;
+  int staged;              // keys that the shared memory holds
   int linear;              // kv_sp is a page of kv_so
 };
 
@@ -100,7 +105,7 @@ __global__ void __launch_bounds__(kEvictSelThreads) evict_select_kernel(const __
   }
   float* mass = p.mass + l * p.m_sl + b * p.m_sb + h * p.m_sh;
   const int others = n - p.recent, want = keep - p.recent;     // others > want
-  const bool in_smem = p.staged != 0 && others <= kEvictStage;
+  const bool in_smem = p.staged != 0 && others <= p.staged;
   auto key_at = [&](int t) { return in_smem ? staged[t] : order_key(fmaxf(mass[t], -INFINITY)); };
   if (in_smem) {
     for (int t = tid; t < others; t += kEvictSelThreads) staged[t] = order_key(fmaxf(mass[t], -INFINITY));
@@ -358,13 +363,12 @@ inline int run_block_evict(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int
   p.bt_sb = bt_sb; p.m_sl = m_sl; p.m_sb = m_sb; p.m_sh = m_sh;
   p.n_pages = n_pages; p.bt_cols = bt_cols; p.B = B; p.h_kv = H_KV; p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.keep = keep; p.recent = recent; p.linear = kv_sp == page * kv_so;
-  // the keys of rows that the table admits, up to 48 KB; longer rows read their masses again for each digit
-  const int64_t tokens = static_cast<int64_t>(bt_cols) * page;
-  p.staged = tokens > 0;
+  const bool few = static_cast<int64_t>(H_KV) * B * L <= 2 * static_cast<int64_t>(dev->sm_count);
+  p.staged = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(bt_cols) * page, few ? kEvictStage : kEvictStageMany));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(H_KV, B, L);
   cfg.blockDim = dim3(kEvictSelThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(std::min<int64_t>(tokens, kEvictStage)) * 4;
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.staged) * 4;
   cfg.stream = static_cast<cudaStream_t>(stream);
   LaunchAttrs at(1);
   at.apply(cfg);

@@ -267,7 +267,8 @@ def _check_evict(before, after, tbl, ctx, keep, recent, kind, ctx_out):
 @pytest.mark.parametrize("L,B,KV,D,page,ctx,keep,recent", [
     (1, 1, 1, 64, 8, [9], 8, 0), (1, 1, 1, 64, 8, [2], 1, 1), (1, 3, 2, 128, 16, [100, 48, 49], 48, 7), (2, 2, 2, 64, 32, [333, 40], 100, 100),
     (2, 3, 1, 128, 128, [700, 0, 513], 257, 1), (1, 2, 3, 128, 64, [1000, 999], 500, 250), (3, 2, 2, 64, 64, [600, 601], 599, 30),
-    (1, 2, 1, 128, 8, [3000, 2999], 1030, 64), (1, 1, 1, 64, 128, [13000], 4000, 500), (1, 2, 2, 128, 32, [2049, 2048], 2048, 0)])
+    (1, 2, 1, 128, 8, [3000, 2999], 1030, 64), (1, 1, 1, 64, 128, [13000], 4000, 500), (1, 2, 2, 128, 32, [2049, 2048], 2048, 0),
+    (1, 1, 1, 64, 128, [50000], 300, 20), (1, 40, 8, 64, 128, [12700] + [9, 130, 600] * 13, 100, 30)])
 def test_evict_matches_oracle(cuda, kind, L, B, KV, D, page, ctx, keep, recent):
     import specq
     g = torch.Generator(device="cuda").manual_seed(keep + page)
