@@ -19,15 +19,15 @@
 // A column needs its rows' sums over all tokens first.  Where a cluster of up to 8 blocks of 512 tokens holds the whole
 // table, the blocks exchange their maxima and sums through distributed shared memory and each key is read from
 // HBM once; up to 16 rows the scores stay in registers, more rows' products are made again from the keys in shared
-// memory.  For longer tables, and up to 16 rows where the SMs are busy anyway, a first launch leaves each block's maxima and sums (and, up
-// to 16 rows, the scores: 8 bytes a row and token against D for reading the key again), and a later one takes the
-// sums.  No atomics: a token's sum is made in a fixed order.
+// memory.  For longer tables, and up to 16 rows where the SMs are busy anyway, a first launch leaves each block's maxima and
+// sums (and, up to 16 rows, the scores: 8 bytes a row and token against D for reading the key again), and a later one
+// takes the sums.  No atomics: a token's sum is made in a fixed order.
 //
 // Measured (B200, 8 KV heads of 128).  One row of 4 heads: 32 sequences of 1 to 8192 tokens 49 us (2.9 TB/s), 32 x 4096 51, one of
 // 37 tokens 4.9: the bytes need 20; a tile of 32 tokens costs a warp some 450 instructions (128 of them widen bytes, 32 are
-// products of which 12 rows of 16 are padding).  9 rows of 4 heads, 8 x 4096: 44.6 us.  64 rows of 4 heads, two sequences of 12 to
-// 16 thousand tokens: 163 us, of which the products, made twice, need 55 at the warp-level pipe's 8.5 cycles each; the rest is two
-// exponentials and some ten more instructions a score and thread.
+// products of which 12 rows of 16 are padding).  36 rows (9 of 4 heads), 8 x 4096: 45 us; 64 rows of the same: 53.
+// More rows' products are made on tcgen05 (mass_wide.cuh): made here, twice, at the warp-level pipe's 8.5 cycles each, those of
+// 256 rows and two sequences of 12 to 16 thousand tokens took 55 of 163 us.
 #pragma once
 
 #include "block_cache.cuh"
