@@ -616,6 +616,29 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
   }
 };
 
+// Whether two [T, H, D] tensors of one type share no memory: apart altogether, or columns of one buffer by rows or by heads.
+bool apart(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  const int64_t es = a.element_size();
+  auto head = [&](const Tensor& t) { return (t.size(1) - 1) * t.stride(1) + t.size(2); };
+  auto span = [&](const Tensor& t) { return (t.size(0) - 1) * t.stride(0) + head(t); };
+  const int64_t lo = (static_cast<char*>(a.data_ptr()) - static_cast<char*>(b.data_ptr())) / es;
+  if (lo >= span(b) || -lo >= span(a)) return true;
+  auto beside = [&](int64_t stride, int64_t in_a, int64_t in_b) {
+    if (stride <= 0) return false;
+    const int64_t off = ((lo % stride) + stride) % stride;
+    return off >= in_b && off + in_a <= stride;
+  };
+  const int64_t s0 = a.stride(0), s1 = a.stride(1);
+  if (s0 != b.stride(0)) return false;
+  return beside(s0, head(a), head(b)) || (s1 == b.stride(1) && s1 > 0 && s0 % s1 == 0 && beside(s1, a.size(2), b.size(2)));
+}
+
+// The same elements in the same places.
+bool same_place(const Tensor& a, const Tensor& b) {
+  return a.data_ptr() == b.data_ptr() && (a.size(0) < 2 || a.stride(0) == b.stride(0)) && (a.size(1) < 2 || a.stride(1) == b.stride(1));
+}
+
 PyObject* qk_norm_rope(PyObject* const* a) {
   // q, k, q_weight, k_weight, pos, table, eps, layout, q_out, k_out, plan
   const char* who = "qk_norm_rope";
@@ -640,6 +663,11 @@ PyObject* qk_norm_rope(PyObject* const* a) {
       BAD_VALUE("%s: no q_out or k_out where a gradient is wanted", who);
     if (x.table.requires_grad()) BAD_VALUE("%s: the table has no gradient", who);
   }
+  if (q_given != nullptr && ((!same_place(*q_given, x.q) && !apart(*q_given, x.q)) || !apart(*q_given, x.k)))
+    BAD_VALUE("%s: q_out may be q, and else shares no memory with q and k", who);
+  if (k_given != nullptr && ((!same_place(*k_given, x.k) && !apart(*k_given, x.k)) || !apart(*k_given, x.q)))
+    BAD_VALUE("%s: k_out may be k, and else shares no memory with q and k", who);
+  if (q_given != nullptr && k_given != nullptr && !apart(*q_given, *k_given)) BAD_VALUE("%s: q_out and k_out share memory", who);
   same_device(who, {&x.q, &x.k, &x.pos, &x.table, x.qw, x.kw, q_given, k_given, x.plan});
   const Tensor qw = or_none(x.qw), kw = or_none(x.kw), plan = or_none(x.plan);
   if (needs) {

@@ -80,6 +80,32 @@ def test_heads_refuse_an_output_where_a_gradient_is_wanted():
         t.requires_grad_(False)
 
 
+def _views(shape, *slices):
+    x = torch.zeros(shape, dtype=F16)
+    return [x[s] for s in slices]
+
+
+ALL = slice(None)
+
+
+@pytest.mark.parametrize("names,views,match", [
+    ("q q_out", _views((5, 4, 64), slice(0, 4), slice(1, 5)), "q_out may be q"),
+    ("k q_out", _views((4, 4, 64), (ALL, slice(0, 2)), ALL), "q_out may be q"),
+    ("q k_out", _views((4, 4, 64), ALL, (ALL, slice(1, 3))), "k_out may be k"),
+    ("q q_out", _views((4, 4, 96), (ALL, ALL, slice(0, 64)), (ALL, ALL, slice(32, 96))), "q_out may be q"),
+    ("q_out k_out", _views((4, 4, 64), ALL, (ALL, slice(2, 4))), "q_out and k_out"),
+    # allowed, so that the next refusal is met: the heads of one projection's rows, and heads side by side
+    ("q k q_out k_out", _views((4, 8, 64), (ALL, slice(0, 4)), (ALL, slice(4, 6)), (ALL, slice(0, 4)), (ALL, slice(4, 6))), "CUDA"),
+    ("q k k_out", _views((4, 8, 64), (ALL, slice(0, 4)), (ALL, slice(4, 6)), (ALL, slice(6, 8))), "CUDA"),
+    ("q q_out", _views((4, 4, 2, 64), (ALL, ALL, 0), (ALL, ALL, 1)), "CUDA"),
+])
+def test_heads_refuse_outputs_over_inputs(names, views, match):
+    a = dict(q=torch.zeros(4, 4, 64, dtype=F16), k=torch.zeros(4, 2, 64, dtype=F16), q_out=None, k_out=None)
+    a.update(zip(names.split(), views))
+    with pytest.raises(ValueError, match=match):
+        specq.qk_norm_rope(a["q"], a["k"], None, None, _i32(4), torch.zeros(8, 64), q_out=a["q_out"], k_out=a["k_out"])
+
+
 def test_heads_library_refuses():
     lib = _lib.load()
 
