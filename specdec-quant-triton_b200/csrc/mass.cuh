@@ -445,7 +445,9 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
         }
       }
     }
-    float top[2] = {0.f, 0.f};                // a quad's largest score of rows g and g + 8; the scores become 2^(s - top)
+    // a quad's largest score of rows g and g + 8, -inf where they see none of its tokens (their factor is then 0, however small the
+    // rows' sums are); the scores become 2^(s - top)
+    float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int e = 0; e < 4; e += 2) {
       float2 x = make_float2(-INFINITY, 0.f);
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
         x.x = fmaxf(x.x, __shfl_xor_sync(0xffffffffu, x.x, 1));
         x.x = fmaxf(x.x, __shfl_xor_sync(0xffffffffu, x.x, 2));
         const float z = x.x == -INFINITY ? 0.f : x.x;
-        top[e / 2] = z;
+        top[e / 2] = x.x;
 #pragma unroll
         for (int i = 0; i < kMassTiles; ++i)
 #pragma unroll

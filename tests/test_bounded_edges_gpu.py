@@ -1,0 +1,37 @@
+"""attention_mass_blocks where scores, scales and tables are out of the ordinary, in each form that a call is cut into.
+
+Bounds as in test_bounded_cache_gpu.py, whose oracle, cases' makers and check these tests use."""
+import pytest
+import torch
+
+from test_bounded_cache_gpu import _cache, _check_mass, _i32, _table
+
+pytestmark = pytest.mark.gpu
+
+# new tokens, heads of a group, tokens of the table: one launch, one launch of a cluster, a stream of tiles (up to 16 rows), a cluster, two
+# passes (17 to 95), tcgen05 (96 and more)
+FORMS = [(2, 4, 512), (3, 1, 512), (4, 4, 1024), (2, 2, 4608), (4, 4, 4608), (3, 8, 1024), (4, 8, 4608), (3, 32, 1024), (4, 32, 4608)]
+
+
+@pytest.mark.parametrize("missing", [False, True])
+@pytest.mark.parametrize("score", [-100.0, -181.0])
+@pytest.mark.parametrize("kind", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("Q,G,tokens", FORMS)
+def test_mass_of_very_negative_scores(cuda, Q, G, tokens, kind, score, missing):
+    """Every score far below 0, where a row's sum is below 2^-128 of its own and some 32 tokens of a context are seen by none or by the
+    later rows only."""
+    import specq
+    D, page, ctx = 128, 16, [33, 65, 290]
+    C = tokens // page
+    g = torch.Generator(device="cuda").manual_seed(Q * G)
+    kc, _, ks, _ = _cache(3 * C + 1, page, 1, D, kind, g)
+    kc.copy_(torch.full(kc.shape, 4.0, device="cuda").to(kind))
+    ks.fill_(1.0)
+    tbl = _table(3, C, 3 * C + 1, g)
+    if missing:
+        tbl[0, 2], tbl[1, 2:4], tbl[2, 4:6] = -1, 3 * C + 1, -1     # whole tiles, and the only one that the last row alone sees
+    q = torch.full((3, Q, G, D), score / (4 * D ** 0.5), device="cuda").half()
+    mass = torch.rand(3, 1, tokens, generator=g, device="cuda")
+    m = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), mass.clone(), decay=0.5)
+    specq.get_status()
+    _check_mass(m, q, kc, ks, tbl, _i32(ctx), mass, decay=0.5)
