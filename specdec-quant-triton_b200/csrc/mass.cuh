@@ -94,6 +94,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Two products, each rounded.  (Scalar ones: __fmul2_rn and mul.rn.f32x2 came out fused with the sums that they go into.)
+__device__ __forceinline__ float2 mul2_rounded(float2 a, float2 b) { return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)); }
+
 template <int D, int ROWS>
 struct MassSmem {
   static constexpr int kQStride = D + 8;     // halves: 16 more bytes a row put a quarter-warp's reads on all banks
@@ -327,16 +330,22 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
 #pragma unroll
       for (int jj = 0; jj < 4; ++jj) mma_f16(s, a[c][jj], k[c][jj][0], k[c][jj][1]);
   };
-  // s: the products of rows r0 + g (0, 1) and r0 + g + 8 (2, 3) with tokens 8 j + 2 tq + 0, 1.  A score times log2 e is s x, x > 0;
-  // s becomes -inf where a row does not see a token (and x 1, where a page gives none).
-  auto factors = [&](int i, int r0, float (&x)[4], float (&y)[4]) {
+  // s: the products of rows r0 + g (0, 1) and r0 + g + 8 (2, 3) with tokens 8 j + 2 tq + 0, 1, made scores times log2 e.  They are
+  // rounded once here: a maximum of rounded scores leaves its own score with the difference 0, whatever its size, where a fused
+  // s x - max would leave what the rounding cut off (2^36 of 2^60).
+  auto scale = [&](int i, int r0, float (&s)[4][4]) {
     const float f0 = BF ? sm.factor[r0 + g] : 1.f, f1 = BF ? sm.factor[r0 + g + 8] : 1.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      x[j] = BF ? tscale[i][j] * f0 : tscale[i][j];
-      y[j] = BF ? tscale[i][j] * f1 : tscale[i][j];
+      const float x = BF ? tscale[i][j] * f0 : tscale[i][j], y = BF ? tscale[i][j] * f1 : tscale[i][j];
+      const float2 u = mul2_rounded(make_float2(s[j][0], s[j][1]), make_float2(x, x)), v = mul2_rounded(make_float2(s[j][2], s[j][3]), make_float2(y, y));
+      s[j][0] = u.x;
+      s[j][1] = u.y;
+      s[j][2] = v.x;
+      s[j][3] = v.y;
     }
   };
+  // s becomes -inf where a row does not see a token
   auto hide = [&](int i, int r0, float (&s)[4][4]) {
     if (bad[i] == 0u && t0[i] + 31 <= base) return;
     const int l0 = sm.lim[r0 + g], l1 = sm.lim[r0 + g + 8];
@@ -351,17 +360,17 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
     }
   };
   // a row's maximum and sum over this thread's eight tokens, then over the quad's 32
-  auto row_stats = [&](const float (&s)[4][4], const float (&x)[4], int e) {
-    float m = fmaxf(s[0][e], s[0][e + 1]) * x[0];
+  auto row_stats = [&](const float (&s)[4][4], int e) {
+    float m = fmaxf(s[0][e], s[0][e + 1]);
 #pragma unroll
-    for (int j = 1; j < 4; ++j) m = fmaxf(m, fmaxf(s[j][e], s[j][e + 1]) * x[j]);
+    for (int j = 1; j < 4; ++j) m = fmaxf(m, fmaxf(s[j][e], s[j][e + 1]));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
     const float z = m == -INFINITY ? 0.f : -m;
     float2 l = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 d = __ffma2_rn(make_float2(s[j][e], s[j][e + 1]), make_float2(x[j], x[j]), make_float2(z, z));
+      const float2 d = __fadd2_rn(make_float2(s[j][e], s[j][e + 1]), make_float2(z, z));
       l = __fadd2_rn(l, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
     }
     float sum = l.x + l.y;
@@ -369,12 +378,12 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     return make_float2(m, sum);
   };
-  auto add_weights = [&](int i, int r0, const float (&s)[4][4], const float (&x)[4], const float (&y)[4]) {
+  auto add_weights = [&](int i, int r0, const float (&s)[4][4]) {
     const float l0 = -sm.lse[r0 + g], l1 = -sm.lse[r0 + g + 8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 u = __ffma2_rn(make_float2(s[j][0], s[j][1]), make_float2(x[j], x[j]), make_float2(l0, l0));
-      const float2 v = __ffma2_rn(make_float2(s[j][2], s[j][3]), make_float2(y[j], y[j]), make_float2(l1, l1));
+      const float2 u = __fadd2_rn(make_float2(s[j][0], s[j][1]), make_float2(l0, l0));
+      const float2 v = __fadd2_rn(make_float2(s[j][2], s[j][3]), make_float2(l1, l1));
       const float2 w = __fadd2_rn(__fadd2_rn(make_float2(weight[i][j][0], weight[i][j][1]), make_float2(exp2_fast(u.x), exp2_fast(u.y))),
                                   make_float2(exp2_fast(v.x), exp2_fast(v.y)));
       weight[i][j][0] = w.x;
@@ -436,13 +445,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
           product(a, k, s[i][j]);
         }
         hide(i, 0, s[i]);
-        float x[4], y[4];
-        factors(i, 0, x, y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[i][j][0] *= x[j]; s[i][j][1] *= x[j];
-          s[i][j][2] *= y[j]; s[i][j][3] *= y[j];
-        }
+        scale(i, 0, s[i]);
       }
     }
     // a quad's largest score of rows g and g + 8, -inf where they see none of its tokens (their factor is then 0, however small the
@@ -511,9 +514,8 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
 #pragma unroll
             for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
             hide(i, r0, s);
-            float x[4], y[4];
-            factors(i, r0, x, y);
-            const float2 u = row_stats(s, x, 0), v = row_stats(s, y, 2);
+            scale(i, r0, s);
+            const float2 u = row_stats(s, 0), v = row_stats(s, 2);
             if (tq == 0) {
               float2* at = &sm.part[warp][r0 + g];
               at[0] = i == 0 ? u : join_stats(at[0], u);
@@ -537,9 +539,8 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
 #pragma unroll
             for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
             hide(i, r0, s);
-            float x[4], y[4];
-            factors(i, r0, x, y);
-            add_weights(i, r0, s, x, y);
+            scale(i, r0, s);
+            add_weights(i, r0, s);
           }
         }
       }
@@ -719,8 +720,8 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_stream_kernel(const __gr
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float x = __shfl_sync(0xffffffffu, scl, j), x0 = BF ? x * f0 : x, x1 = BF ? x * f1 : x;
-      s[j][0] *= x0; s[j][1] *= x0;
-      s[j][2] *= x1; s[j][3] *= x1;
+      s[j][0] = __fmul_rn(s[j][0], x0); s[j][1] = __fmul_rn(s[j][1], x0);   // rounded once, as by `scale` above
+      s[j][2] = __fmul_rn(s[j][2], x1); s[j][3] = __fmul_rn(s[j][3], x1);
     }
     if (bad || t + 31 > base) {
       const uint32_t gone = __ballot_sync(0xffffffffu, scl == 0.f);

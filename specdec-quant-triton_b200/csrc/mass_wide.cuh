@@ -259,19 +259,18 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
                 for (int k = 0; k < 16; ++k)
                   if ((gone >> ((c + k) / 8) & 1u) != 0u || token0 + c + k > my_lim) u[k] = 0xFF800000u;
               }
+              float2 s[8];                                      // scores, rounded once (see `scale` in mass.cuh)
               float top = m;
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                float y = __uint_as_float(u[j * 8]);
-#pragma unroll
-                for (int k = 1; k < 8; ++k) y = fmaxf(y, __uint_as_float(u[j * 8 + k]));
-                top = fmaxf(top, y * x[j]);
+              for (int k = 0; k < 8; ++k) {
+                s[k] = mul2_rounded(make_float2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1])), make_float2(x[k / 4], x[k / 4]));
+                top = fmaxf(top, fmaxf(s[k].x, s[k].y));
               }
               const float z = top == -INFINITY ? 0.f : -top;
               float2 sum = {l * exp2_fast(m + z), 0.f};         // m = -inf: 0
 #pragma unroll
-              for (int k = 0; k < 16; k += 2) {
-                const float2 d = __ffma2_rn(make_float2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), make_float2(x[k / 8], x[k / 8]), make_float2(z, z));
+              for (int k = 0; k < 8; ++k) {
+                const float2 d = __fadd2_rn(s[k], make_float2(z, z));
                 sum = __fadd2_rn(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
               }
               l = sum.x + sum.y;
@@ -305,7 +304,10 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
                 if (token0 + me > lim.z) lse.z = -INFINITY;
                 if (token0 + me > lim.w) lse.w = -INFINITY;
               }
-              const float2 d0 = __ffma2_rn(s0, make_float2(x, x), make_float2(lse.x, lse.y)), d1 = __ffma2_rn(s1, make_float2(x, x), make_float2(lse.z, lse.w));
+              // (s f) x is s (f x) to the bit, f being a power of two: the scores of the other pass
+              s0 = mul2_rounded(s0, make_float2(x, x));
+              s1 = mul2_rounded(s1, make_float2(x, x));
+              const float2 d0 = __fadd2_rn(s0, make_float2(lse.x, lse.y)), d1 = __fadd2_rn(s1, make_float2(lse.z, lse.w));
               sum = __fadd2_rn(sum, make_float2(exp2_fast(d0.x), exp2_fast(d0.y)));
               sum = __fadd2_rn(sum, make_float2(exp2_fast(d1.x), exp2_fast(d1.y)));
             }

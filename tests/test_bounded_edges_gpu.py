@@ -1,10 +1,12 @@
 """attention_mass_blocks where scores, scales and tables are out of the ordinary, in each form that a call is cut into.
 
 Bounds as in test_bounded_cache_gpu.py, whose oracle, cases' makers and check these tests use."""
+import numpy as np
 import pytest
 import torch
 
-from test_bounded_cache_gpu import _cache, _check_mass, _i32, _table
+from oracle import bounded_oracle as O
+from test_bounded_cache_gpu import _cache, _check_mass, _i32, _numbers, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -35,3 +37,30 @@ def test_mass_of_very_negative_scores(cuda, Q, G, tokens, kind, score, missing):
     m = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), mass.clone(), decay=0.5)
     specq.get_status()
     _check_mass(m, q, kc, ks, tbl, _i32(ctx), mass, decay=0.5)
+
+
+@pytest.mark.parametrize("kind", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("Q,tokens", [(4, 512), (4, 4608), (12, 1024), (12, 4608), (48, 1024), (48, 4608)])
+def test_mass_of_a_large_row_beside_ordinary_ones(cuda, Q, tokens, kind):
+    """Rows of 2^60 and ordinary ones in one call (two heads of a group): a large row puts its weight on one token, and the others lose no
+    bits to it, since each row has its own power of two.  The bound is made from the ordinary rows alone."""
+    import specq
+    D, page, ctx = 64, 16, [33, 65, 290]
+    C = tokens // page
+    g = torch.Generator(device="cuda").manual_seed(Q + 3)
+    kc, _, ks, _ = _cache(3 * C, page, 1, D, kind, g)
+    tbl = _table(3, C, 3 * C, g)
+    q = torch.randn(3, Q, 2, D, generator=g, device="cuda").bfloat16()
+    q[:, :, 1] *= 2.0 ** 60
+    zero = np.zeros((3, 1, tokens))
+
+    def oracle(rows):
+        return O.attention_mass(rows.double().cpu().numpy(), _numbers(kc), ks.cpu().numpy(), tbl.cpu().numpy(), ctx, zero)
+    plain, size = oracle(q[:, :, :1])
+    large, _ = oracle(q[:, :, 1:])
+    assert np.isin(large, np.arange(Q + 1)).all()          # no two of a large row's scores meet
+    m = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), torch.zeros(3, 1, tokens, device="cuda"))
+    rel = 2 * (D + 4) * 2.0 ** -23 * size + 2.0 ** -20 + 2 * Q * 2.0 ** -24
+    err = np.abs(m.double().cpu().numpy() - plain - large)
+    bound = rel * plain + 2.0 ** -23 * (plain + large) + 1e-12
+    assert (err <= bound).all(), (err / bound).max()
