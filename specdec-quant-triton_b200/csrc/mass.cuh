@@ -345,7 +345,8 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
       s[j][3] = v.y;
     }
   };
-  // s becomes -inf where a row does not see a token
+  // s becomes -inf where a row does not see a token: after the scaling, since a scale of 0 (or a product of small ones that leaves
+  // fp32) times -inf is NaN
   auto hide = [&](int i, int r0, float (&s)[4][4]) {
     if (bad[i] == 0u && t0[i] + 31 <= base) return;
     const int l0 = sm.lim[r0 + g], l1 = sm.lim[r0 + g + 8];
@@ -444,8 +445,8 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
           widen(i, j, k);
           product(a, k, s[i][j]);
         }
-        hide(i, 0, s[i]);
         scale(i, 0, s[i]);
+        hide(i, 0, s[i]);
       }
     }
     // a quad's largest score of rows g and g + 8, -inf where they see none of its tokens (their factor is then 0, however small the
@@ -513,8 +514,8 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
             fragments(r0, a);
 #pragma unroll
             for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
-            hide(i, r0, s);
             scale(i, r0, s);
+            hide(i, r0, s);
             const float2 u = row_stats(s, 0), v = row_stats(s, 2);
             if (tq == 0) {
               float2* at = &sm.part[warp][r0 + g];
@@ -538,8 +539,8 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
             fragments(r0, a);
 #pragma unroll
             for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
-            hide(i, r0, s);
             scale(i, r0, s);
+            hide(i, r0, s);
             add_weights(i, r0, s);
           }
         }
@@ -631,7 +632,8 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_stream_kernel(const __gr
     if (lane < 4) report_status(p.status, SPECQ_STATUS_BAD_INDEX);
     return -1;
   };
-  auto scale_of = [&](int pg) { return pg < 0 ? 0.f : p.ks[pg * p.s_sp + h * p.s_sh] * p.sm_log2; };
+  constexpr float kNoPage = -INFINITY;        // (a page's own scale may be 0; a bit beside it in a word of its own cost 1.5 us of 49)
+  auto scale_of = [&](int pg) { return pg < 0 ? kNoPage : p.ks[pg * p.s_sp + h * p.s_sh] * p.sm_log2; };
   const int mask = (1 << p.page_log2) - 1;
   const uint8_t* heads = p.kc + h * p.kv_sh + tq * 16;
   auto fetch = [&](int stage, int i, int pg) {
@@ -655,7 +657,7 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_stream_kernel(const __gr
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   int pg[kMassStages];
-  float sc[kMassStages];                      // the lane's n-tile's scale of each tile on its way (0: it has no page)
+  float sc[kMassStages];                      // the lane's n-tile's scale of each tile on its way, or kNoPage
 #pragma unroll
   for (int i = 0; i < kMassStages; ++i) pg[i] = page_of(i);
   int ahead = page_of(kMassStages);
@@ -691,7 +693,7 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_stream_kernel(const __gr
   for (int i = 0; i < tiles; ++i) {
     const int t = start(i);
     const float scl = sc[0];
-    const bool bad = __any_sync(0xffffffffu, scl == 0.f);       // (a page's scale is positive)
+    const bool bad = __any_sync(0xffffffffu, scl == kNoPage);
     asm volatile("cp.async.wait_group %0;" ::"n"(kMassStages - 1) : "memory");
     float s[4][4];
 #pragma unroll
@@ -724,7 +726,7 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_stream_kernel(const __gr
       s[j][2] = __fmul_rn(s[j][2], x1); s[j][3] = __fmul_rn(s[j][3], x1);
     }
     if (bad || t + 31 > base) {
-      const uint32_t gone = __ballot_sync(0xffffffffu, scl == 0.f);
+      const uint32_t gone = __ballot_sync(0xffffffffu, scl == kNoPage);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int at = gone >> j & 1u ? INT_MAX - 1 : t + 8 * j + 2 * tq;

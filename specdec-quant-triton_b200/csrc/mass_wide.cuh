@@ -254,23 +254,21 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
               if (c + 16 < kWideTile) tmem_ld16(at + c + 16, v[(c / 16 + 1) & 1]);
               const float2 xs = *reinterpret_cast<const float2*>(scale + c / 8);
               const float x[2] = {BF ? xs.x * mine : xs.x, BF ? xs.y * mine : xs.y};
-              if (hidden) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(__fmul_rn(__uint_as_float(u[k]), x[k / 8]));   // see `scale` in mass.cuh
+              if (hidden) {                                     // after the scaling: see `hide` there
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
                   if ((gone >> ((c + k) / 8) & 1u) != 0u || token0 + c + k > my_lim) u[k] = 0xFF800000u;
               }
-              float2 s[8];                                      // scores, rounded once (see `scale` in mass.cuh)
               float top = m;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                s[k] = mul2_rounded(make_float2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1])), make_float2(x[k / 4], x[k / 4]));
-                top = fmaxf(top, fmaxf(s[k].x, s[k].y));
-              }
+              for (int k = 0; k < 16; ++k) top = fmaxf(top, __uint_as_float(u[k]));
               const float z = top == -INFINITY ? 0.f : -top;
               float2 sum = {l * exp2_fast(m + z), 0.f};         // m = -inf: 0
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float2 d = __fadd2_rn(s[k], make_float2(z, z));
+              for (int k = 0; k < 16; k += 2) {
+                const float2 d = __fadd2_rn(make_float2(__uint_as_float(u[k]), __uint_as_float(u[k + 1])), make_float2(z, z));
                 sum = __fadd2_rn(sum, make_float2(exp2_fast(d.x), exp2_fast(d.y)));
               }
               l = sum.x + sum.y;

@@ -64,3 +64,47 @@ def test_mass_of_a_large_row_beside_ordinary_ones(cuda, Q, tokens, kind):
     err = np.abs(m.double().cpu().numpy() - plain - large)
     bound = rel * plain + 2.0 ** -23 * (plain + large) + 1e-12
     assert (err <= bound).all(), (err / bound).max()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("Q,G,tokens", FORMS)
+def test_mass_of_pages_of_scale_zero(cuda, Q, G, tokens, kind, dtype):
+    """A key of a page of scale 0 has the score 0, in tiles that rows see in part and in tiles that they see whole, beside pages outside
+    the cache."""
+    import specq
+    D, page, ctx = 64, 16, [33, 65, 290]
+    C = tokens // page
+    g = torch.Generator(device="cuda").manual_seed(Q * G + 1)
+    kc, _, ks, _ = _cache(3 * C + 1, page, 1, D, kind, g)
+    tbl = _table(3, C, 3 * C + 1, g)
+    for b, n in enumerate(ctx):
+        ks[tbl[b, [0, (n - 1) // page]].long()] = 0.0
+    ks[tbl[2, 4:9].long()] = 0.0                 # whole tiles
+    q = torch.randn(3, Q, G, D, generator=g, device="cuda").to(dtype)
+    mass = torch.rand(3, 1, tokens, generator=g, device="cuda")
+    for missing in (False, True):
+        if missing:
+            tbl[0, 1], tbl[2, 3], tbl[2, 5] = -1, 3 * C + 1, -1
+        m = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), mass.clone(), decay=0.5)
+        _check_mass(m, q, kc, ks, tbl, _i32(ctx), mass, decay=0.5)
+    specq.get_status()
+
+
+@pytest.mark.parametrize("Q,G,tokens", FORMS)
+def test_mass_of_tiny_rows_beside_pages_of_zeros(cuda, Q, G, tokens):
+    """bf16 rows of 2^-120 and the least scale that the append writes: their product leaves fp32, the score is 0."""
+    import specq
+    D, page, ctx = 64, 16, [33, 65, 290]
+    C = tokens // page
+    g = torch.Generator(device="cuda").manual_seed(Q * G + 2)
+    kc, _, ks, _ = _cache(3 * C, page, 1, D, torch.int8, g)
+    tbl = _table(3, C, 3 * C, g)
+    for b, n in enumerate(ctx):
+        last = tbl[b, (n - 1) // page].long()
+        kc[last], ks[last] = 0, 1e-8 / 127
+    q = torch.randn(3, Q, G, D, generator=g, device="cuda").bfloat16()
+    q[:, -1] *= 2.0 ** -120
+    mass = torch.rand(3, 1, tokens, generator=g, device="cuda")
+    m = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), mass.clone())
+    _check_mass(m, q, kc, ks, tbl, _i32(ctx), mass)
