@@ -94,6 +94,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// What a bf16 row's halves times 2^k stand for: 2^-k, but no more than 2^80, so that the scores of rows past 2^94 stay within fp32 (a
+// product of halves and keys is below 2^32).  Such a row's weight is on its largest score either way: its products are multiples of
+// 2^-33, and 2^47 times the least scale that the append writes is beyond the reach of an exponential.
+__device__ __forceinline__ float row_factor(int k) { return __int_as_float((127 + min(-k, 80)) << 23); }
+
 // Two products, each rounded.  (Scalar ones: __fmul2_rn and mul.rn.f32x2 came out fused with the sums that they go into.)
 __device__ __forceinline__ float2 mul2_rounded(float2 a, float2 b) { return make_float2(__fmul_rn(a.x, b.x), __fmul_rn(a.y, b.y)); }
 
@@ -167,7 +172,7 @@ __device__ __forceinline__ void mass_queries(const MassParams& p, Smem& sm, int 
       // amax 2^k in [2^14, 2^15); 2^126 suffices for what is not zero beside any key
       const int k = top != 0u && finite ? min(14 - ilogbf(amax), 126) : 0;
       const float up = __int_as_float((127 + k) << 23);           // k >= 14 - 127
-      factor = __int_as_float((127 - k) << 23);
+      factor = row_factor(k);
 #pragma unroll
       for (int i = 0; i < kMine / 8; ++i) {
         uint4 u = at[i];
@@ -216,7 +221,7 @@ __device__ __forceinline__ void few_queries_store(const MassParams& p, Smem& sm,
     // the largest element times 2^k in [2^14, 2^15); 2^126 suffices for what is not zero beside any key
     const int k = top != 0u && counts ? min(14 - ilogbf(__uint_as_float(top << 16)), 126) : 0;
     const float up = __int_as_float((127 + k) << 23);             // k >= 14 - 127
-    factor = __int_as_float((127 - k) << 23);
+    factor = row_factor(k);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const __half2 v = __floats2half2_rn(__uint_as_float(w[j] << 16) * up, __uint_as_float(w[j] & 0xFFFF0000u) * up);

@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kWideThreads, 2) mass_wide_kernel(const __grid
         // the largest element times 2^k in [2^14, 2^15); 2^126 suffices for what is not zero beside any key
         const int k = top != 0u && finite ? min(14 - ilogbf(__uint_as_float(top << 16)), 126) : 0;
         up = __int_as_float((127 + k) << 23);                      // k >= 14 - 127
-        factor = __int_as_float((127 - k) << 23);
+        factor = row_factor(k);
       }
 #pragma unroll
       for (int c = 0; c < kMine; ++c) {

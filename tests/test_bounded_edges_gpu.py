@@ -39,11 +39,13 @@ def test_mass_of_very_negative_scores(cuda, Q, G, tokens, kind, score, missing):
     _check_mass(m, q, kc, ks, tbl, _i32(ctx), mass, decay=0.5)
 
 
+@pytest.mark.parametrize("power", [60, 120])
 @pytest.mark.parametrize("kind", [torch.int8, torch.float8_e4m3fn])
 @pytest.mark.parametrize("Q,tokens", [(4, 512), (4, 4608), (12, 1024), (12, 4608), (48, 1024), (48, 4608)])
-def test_mass_of_a_large_row_beside_ordinary_ones(cuda, Q, tokens, kind):
-    """Rows of 2^60 and ordinary ones in one call (two heads of a group): a large row puts its weight on one token, and the others lose no
-    bits to it, since each row has its own power of two.  The bound is made from the ordinary rows alone."""
+def test_mass_of_a_large_row_beside_ordinary_ones(cuda, Q, tokens, kind, power):
+    """Rows of 2^60, or of 2^120 (whose scores are past fp32), and ordinary ones in one call (two heads of a group): a large row puts its
+    weight on one token, and the others lose no bits to it, since each row has its own power of two.  The bound is made from the ordinary
+    rows alone."""
     import specq
     D, page, ctx = 64, 16, [33, 65, 290]
     C = tokens // page
@@ -51,7 +53,7 @@ def test_mass_of_a_large_row_beside_ordinary_ones(cuda, Q, tokens, kind):
     kc, _, ks, _ = _cache(3 * C, page, 1, D, kind, g)
     tbl = _table(3, C, 3 * C, g)
     q = torch.randn(3, Q, 2, D, generator=g, device="cuda").bfloat16()
-    q[:, :, 1] *= 2.0 ** 60
+    q[:, :, 1] *= 2.0 ** power
     zero = np.zeros((3, 1, tokens))
 
     def oracle(rows):
