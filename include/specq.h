@@ -438,7 +438,8 @@ int specq_beam_reorder(void* const* ptr, const int64_t* stride, const int64_t* r
  *   n_rows   optional int32 [B]: only the first n_rows[b] rows of the sequence count, which stand at the
  *            places ctx_len[b] - n_rows[b] + i; a sequence without rows or tokens keeps its mass
  *   mass     fp32 [B, H_KV, >= bt_cols * page], strides (m_sb, m_sh), unit along the tokens
- * A query row with a NaN or an infinity adds nothing.
+ * A query row with a NaN or an infinity adds nothing.  A page's scale is 0 or more, and scale * sm_scale below 2^15, so that
+ * scores stay within fp32.  workspace: at most 512 MB, or what one KV head of one sequence takes, as the function below gives.
  */
 int specq_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, int dtype, const void* kc,
                          int64_t kv_sp, int64_t kv_so, int64_t kv_sh, int cache_dtype, int n_pages, const float* ks,

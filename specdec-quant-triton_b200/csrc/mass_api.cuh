@@ -1,4 +1,5 @@
-// mass_api.cuh -- how attention_mass is cut into launches: clusters, streams of tiles, or tcgen05 products, by rows and table.
+// mass_api.cuh -- how attention_mass is cut into launches: clusters, streams of tiles, or tcgen05 products, by rows and table; and into
+// turns over one workspace where its sums or scores would fill more.
 #pragma once
 
 #include "mass_wide.cuh"
@@ -41,14 +42,44 @@ inline bool mass_plan(int B, int H_KV, int rows, int tokens, int* chunk_tiles, i
   return false;
 }
 
+// What a call keeps in its workspace goes by the table's width, whatever is cached of it: 4 bytes for each row and token (up to 16 rows),
+// or 8 for each row and block of 256 or 512 tokens, of every KV head of every sequence.  Past kMassSpace it goes through its sequences, or
+// the KV heads of one, in several turns of one size over the same workspace, which is then at most that or what one KV head of one
+// sequence takes.  (16 rows of 64 sequences, 8 heads and a table of 131072 tokens: 512 MB in place of 4.3 GB.  A turn costs some 10 us: the
+// same rows of 32 sequences of 32768 tokens take 454 us in one turn of 540 MB, 470 in two and 497 in three.)
+constexpr int64_t kMassSpace = 512ll << 20;
+
+struct MassCut {
+  bool whole;                  // in one launch, without a workspace
+  int chunk_tiles, chunks;
+  int seqs, heads;             // of a turn
+  int64_t bytes;               // of a turn
+};
+
+inline MassCut mass_cut(int B, int H_KV, int rows, int tokens) {
+  MassCut c = {};
+  c.whole = mass_plan(B, H_KV, rows, tokens, &c.chunk_tiles, &c.chunks);
+  c.seqs = B;
+  c.heads = H_KV;
+  if (c.whole || B == 0) return c;
+  const int64_t stats = static_cast<int64_t>(rows) * c.chunks * 8;
+  const int64_t one = stats + (rows <= kMassFew ? static_cast<int64_t>(rows) * c.chunks * c.chunk_tiles * kMassThreads * 4 : static_cast<int64_t>(rows) * 4);
+  auto even = [](int n, int64_t most) {            // turns of at most `most`, all but alike
+    const int turns = most >= n ? 1 : static_cast<int>((n + std::max<int64_t>(most, 1) - 1) / std::max<int64_t>(most, 1));
+    return (n + turns - 1) / turns;
+  };
+  if (one > 0) {
+    c.seqs = even(B, kMassSpace / (one * H_KV));
+    if (one * H_KV > kMassSpace) c.heads = even(H_KV, kMassSpace / one);
+  }
+  c.bytes = one * c.seqs * c.heads;
+  return c;
+}
+
 inline int run_attention_mass_workspace(int B, int q_len, int H, int H_KV, int D, int page, int bt_cols, int64_t* bytes) {
   if (bytes == nullptr) return fail(SPECQ_ERR_INVALID_ARG, "attention_mass_workspace: null pointer");
   if (int rc = mass_check(B, q_len, H, H_KV, D, page, bt_cols)) return rc;
-  int tiles, chunks;
-  const int rows = q_len * (H / H_KV);
-  const bool whole = mass_plan(B, H_KV, rows, bt_cols * page, &tiles, &chunks);
-  const int64_t all = static_cast<int64_t>(B) * H_KV * rows;
-  *bytes = whole ? 0 : all * chunks * 8 + (rows <= kMassFew ? all * chunks * tiles * kMassThreads * 4 : all * 4);
+  *bytes = mass_cut(B, H_KV, q_len * (H / H_KV), bt_cols * page).bytes;
   return SPECQ_OK;
 }
 
@@ -74,24 +105,27 @@ inline int run_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t
   DeviceState* dev = nullptr;
   if (int rc = get_device_state(&dev)) return rc;
   MassParams p = {};
-  p.q = q; p.kc = static_cast<const uint8_t*>(kc); p.ks = ks; p.bt = block_tbl; p.ctx = ctx_len; p.n_rows = n_rows; p.mass = mass;
+  p.kc = static_cast<const uint8_t*>(kc);
   p.status = dev->status;
   p.q_sb = q_sb; p.q_st = q_st; p.q_sh = q_sh; p.kv_sp = kv_sp; p.kv_so = kv_so; p.kv_sh = kv_sh; p.s_sp = s_sp; p.s_sh = s_sh;
   p.bt_sb = bt_sb; p.m_sb = m_sb; p.m_sh = m_sh;
-  p.q_len = q_len; p.group = H / H_KV; p.h_kv = H_KV; p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
+  p.q_len = q_len; p.group = H / H_KV; p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.n_pages = n_pages; p.bt_cols = bt_cols; p.rows = q_len * p.group;
   p.sm_log2 = sm_scale * kLog2E; p.decay = decay;
-  const bool whole = mass_plan(B, H_KV, p.rows, bt_cols * page, &p.chunk_tiles, &p.chunks);
+  const MassCut cut = mass_cut(B, H_KV, p.rows, bt_cols * page);
+  const bool whole = cut.whole;
+  p.chunk_tiles = cut.chunk_tiles;
+  p.chunks = cut.chunks;
   p.stats = static_cast<float2*>(workspace);
-  p.score = p.lse = reinterpret_cast<float*>(p.stats + (need > 0 ? static_cast<int64_t>(B) * H_KV * p.chunks * p.rows : 0));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int here = B;                // sequences of this turn (its KV heads: p.h_kv)
   auto launch = [&](auto kern, size_t smem, int threads = kMassThreads) {
     int cluster = 1;
     cudaError_t e = ensure_dyn_smem(reinterpret_cast<const void*>(kern), static_cast<int>(smem));
     if (e != cudaSuccess) return e;
     if (whole) cluster = next_pow2(p.chunks);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(whole ? cluster : p.chunks, H_KV, B);
+    cfg.gridDim = dim3(whole ? cluster : p.chunks, p.h_kv, here);
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -109,13 +143,13 @@ inline int run_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t
         return SPECQ_OK;
       }
       SPECQ_CUDA_TRY(launch(mass_stream_kernel<BF, CT, DD>, sizeof(MassStreamSmem<DD>)));
-      SPECQ_CUDA_TRY(launch_plain(mass_sum_kernel, dim3(ceil_div(bt_cols * page, kMassSumTokens), H_KV, B), dim3(kMassThreads), st, p));
+      SPECQ_CUDA_TRY(launch_plain(mass_sum_kernel, dim3(ceil_div(bt_cols * page, kMassSumTokens), p.h_kv, here), dim3(kMassThreads), st, p));
       return SPECQ_OK;
     }
     if (p.rows >= kMassWide) {
       const size_t wide = sizeof(WideSmem<DD>) + 1024;
       SPECQ_CUDA_TRY(launch(mass_wide_kernel<BF, CT, DD, kMassStats>, wide, kWideThreads));
-      SPECQ_CUDA_TRY(launch_plain(mass_join_kernel, dim3(ceil_div(p.rows, 8), H_KV, B), dim3(256), st, p));
+      SPECQ_CUDA_TRY(launch_plain(mass_join_kernel, dim3(ceil_div(p.rows, 8), p.h_kv, here), dim3(256), st, p));
       SPECQ_CUDA_TRY(launch(mass_wide_kernel<BF, CT, DD, kMassWeights>, wide, kWideThreads));
       return SPECQ_OK;
     }
@@ -124,7 +158,7 @@ inline int run_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t
       return SPECQ_OK;
     }
     SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassRows, kMassStats>, many));
-    SPECQ_CUDA_TRY(launch_plain(mass_join_kernel, dim3(ceil_div(p.rows, 8), H_KV, B), dim3(256), st, p));
+    SPECQ_CUDA_TRY(launch_plain(mass_join_kernel, dim3(ceil_div(p.rows, 8), p.h_kv, here), dim3(256), st, p));
     SPECQ_CUDA_TRY(launch(mass_kernel<BF, CT, DD, kMassRows, kMassWeights>, many));
     return SPECQ_OK;
   };
@@ -132,7 +166,22 @@ inline int run_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t
   auto by_ct = [&](auto bf) {
     return cache_dtype == SPECQ_CACHE_INT8 ? by_d(bf, std::integral_constant<int, 0>{}) : by_d(bf, std::integral_constant<int, 1>{});
   };
-  return dtype == SPECQ_DTYPE_F16 ? by_ct(std::false_type{}) : by_ct(std::true_type{});
+  const MassParams every = p;
+  for (int b0 = 0; b0 < B; b0 += cut.seqs)
+    for (int h0 = 0; h0 < H_KV; h0 += cut.heads) {
+      here = std::min(cut.seqs, B - b0);
+      p.h_kv = std::min(cut.heads, H_KV - h0);
+      p.q = static_cast<const __half*>(q) + b0 * (q_sb != 0 ? q_sb : q_len * q_st) + h0 * every.group * q_sh;
+      p.kc = every.kc + h0 * kv_sh;
+      p.ks = ks + h0 * s_sh;
+      p.bt = block_tbl + b0 * bt_sb;
+      p.ctx = ctx_len + b0;
+      p.n_rows = n_rows == nullptr ? nullptr : n_rows + b0;
+      p.mass = mass + b0 * m_sb + h0 * m_sh;
+      p.score = p.lse = reinterpret_cast<float*>(p.stats + (whole ? 0 : static_cast<int64_t>(here) * p.h_kv * p.chunks * p.rows));
+      if (int rc = dtype == SPECQ_DTYPE_F16 ? by_ct(std::false_type{}) : by_ct(std::true_type{})) return rc;
+    }
+  return SPECQ_OK;
 }
 
 }  // namespace specq

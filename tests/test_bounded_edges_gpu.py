@@ -110,3 +110,29 @@ def test_mass_of_tiny_rows_beside_pages_of_zeros(cuda, Q, G, tokens):
     mass = torch.rand(3, 1, tokens, generator=g, device="cuda")
     m = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), mass.clone())
     _check_mass(m, q, kc, ks, tbl, _i32(ctx), mass)
+
+
+@pytest.mark.parametrize("B,Q,KV,G,cols", [
+    (17, 4, 8, 4, 8192), (1, 4, 8, 4, 131072),        # a stream of tiles: sequences in three turns, heads in three
+    (6, 11, 8, 8, 524288),                            # two passes of 88 rows: sequences in two turns
+    (2, 200, 4, 8, 131072), (1, 300, 4, 8, 131072)])  # tcgen05: sequences in two turns, heads in two
+def test_mass_of_short_contexts_in_a_wide_table(cuda, B, Q, KV, G, cols):
+    """Tables whose scores or sums would fill more than the workspace: sequence by sequence or head by head, with the same result."""
+    import specq
+    D, page = 64, 16
+    ctx = [(37 * b) % 600 for b in range(B - 1)] + [777]
+    g = torch.Generator(device="cuda").manual_seed(B)
+    kc, _, ks, _ = _cache(B * 50, page, KV, D, torch.int8, g)
+    tbl = torch.full((B, cols), -1, dtype=torch.int32, device="cuda")
+    tbl[:, :50] = _table(B, 50, B * 50, g)
+    rows = [Q - b % 2 for b in range(B)]
+    q = torch.randn(B, Q, KV * G, D, generator=g, device="cuda").half()
+    mass = torch.zeros(B, KV, cols * page, device="cuda")
+    mass[:, :, :800] = torch.rand(B, KV, 800, generator=g, device="cuda")
+    before, small = mass.clone(), mass[:, :, :800].contiguous()
+    m = specq.attention_mass_blocks(q, kc, ks, tbl, _i32(ctx), mass, n_rows=_i32(rows), decay=0.5)
+    _check_mass(m[:, :, :800], q, kc, ks, tbl[:, :50], _i32(ctx), small, n_rows=rows, decay=0.5)
+    for b, n in enumerate(ctx):
+        assert torch.equal(m[b, :, n:], before[b, :, n:])
+    packed = specq.attention_mass_blocks(q.flatten(0, 1), kc, ks, tbl, _i32(ctx), before, q_len=Q, n_rows=_i32(rows), decay=0.5)
+    assert torch.equal(packed, m)
