@@ -11,6 +11,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -131,6 +132,13 @@ void written(const char* who, const char* what, const Tensor& t) {
     if (t.stride(i) == 0 && t.size(i) > 1) BAD_VALUE("%s: %s is written and must not be expanded (dimension %lld)", who, what, (long long)i);
 }
 
+// Forward-mode differentiation has no form here: a tensor that carries a tangent is refused, since the result would have none.
+void no_tangent(const char* who, std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    if (t != nullptr && t->_fw_grad(0).defined()) BAD_VALUE("%s: no forward-mode gradient; unpack the dual tensor", who);
+}
+
 // int32, `dims` dimensions, at least n0 (and n1) long (-1: any), unit inner stride
 void int32s(const char* who, const char* what, const Tensor& t, int dims, int64_t n0, int64_t n1 = -1) {
   if (t.scalar_type() != at::kInt) BAD_TYPE("%s: %s must be int32, got %s", who, what, dtype(t));
@@ -244,6 +252,7 @@ PyObject* rope(PyObject* const* a) {
       BAD_VALUE("rope: out must be %s %s, got %s %s", dtype(x), shape(x).c_str(), dtype(*given), shape(*given).c_str());
     written(who, "out", *given);
   }
+  no_tangent(who, {&x, &table, given});
   if (c10::GradMode::is_enabled()) {
     if (given != nullptr && (x.requires_grad() || given->requires_grad())) BAD_VALUE("rope: no out for a tensor that requires grad");
     if (table.requires_grad()) BAD_VALUE("rope: the table has no gradient");
@@ -654,6 +663,7 @@ PyObject* qk_norm_rope(PyObject* const* a) {
   out_like("q_out", q_given, x.q);
   out_like("k_out", k_given, x.k);
   for (int64_t n : {x.q.size(0), x.q.size(1), x.k.size(1), x.q.size(2), x.table.size(0)}) size32(who, n);
+  no_tangent(who, {&x.q, &x.k, x.qw, x.kw, &x.table, q_given, k_given});
   bool needs = false;
   if (c10::GradMode::is_enabled()) {
     needs = x.q.requires_grad() || x.k.requires_grad() || (x.qw != nullptr && x.qw->requires_grad()) ||
@@ -702,6 +712,7 @@ PyObject* beam_select(PyObject* const* a) {
     BAD_VALUE("%s: done must be a contiguous bool of %lld rows, got %s %s", who, (long long)x.size(0), dtype(*done), shape(*done).c_str());
   if (pad < 0 || pad >= V) BAD_VALUE("%s: pad=%d is no token of %d", who, pad, V);
   if (c10::GradMode::is_enabled() && (x.requires_grad() || scores.requires_grad())) BAD_VALUE("%s: no gradient; detach logits and scores", who);
+  no_tangent(who, {&x, &scores});
   same_device(who, {&x, &scores, done});
   const Tensor out = at::empty({B, n}, scores.options()), parent = at::empty({B, n}, scores.options().dtype(at::kInt)),
                token = at::empty({B, n}, scores.options().dtype(at::kInt));
@@ -738,6 +749,7 @@ PyObject* beam_reorder(PyObject* const* a) {
     }
     if (R > 1 && inner > 0 && t.stride(0) < inner) BAD_VALUE("%s: state %zd is written and its rows must not share memory", who, i);
     if (c10::GradMode::is_enabled() && t.requires_grad()) BAD_VALUE("%s: state %zd requires grad; it is written in place", who, i);
+    no_tangent(who, {&t});
     at_[i] = t.data_ptr();
     stride[i] = t.stride(0) * t.element_size();
     bytes[i] = inner * t.element_size();
@@ -774,6 +786,7 @@ void mass_of(const char* who, const Tensor& m, bool layers, int64_t L, int64_t B
   if (m.size(d + 2) > 1 && m.stride(d + 2) != 1) BAD_VALUE("%s: mass needs unit stride along the tokens", who);
   written(who, "mass", m);
   if (c10::GradMode::is_enabled() && m.requires_grad()) BAD_VALUE("%s: mass requires grad; it is written in place", who);
+  no_tangent(who, {&m});
 }
 
 PyObject* attention_mass_blocks(PyObject* const* a) {

@@ -88,7 +88,7 @@ def rope(x, pos, table, layout="half", inverse=False, out=None, plan=None):
     """Turn the first rot = table.shape[1] elements of every head of x [T, H, D] (float16, bfloat16 or
     float32; any row and head strides) to positions pos [T] int32; `out` may be x.  inverse=True
     turns back, which is the gradient of the rotation: an x that requires grad gets it (without `out`; the
-    table has none).  With `plan`, only rows < plan[0]: the others of a new output are 0, those of `out`
+    table has none; no forward mode).  With `plan`, only rows < plan[0]: the others of a new output are 0, those of `out`
     keep what they hold."""
     y = _native.rope(x, pos, table, layout, inverse, out, plan)
     return y if y is not NotImplemented else _Rope.apply(x, pos, table, layout, inverse, plan)

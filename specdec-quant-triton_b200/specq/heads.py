@@ -20,8 +20,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, pos, table, eps=1e-6, layout="half", 
 
     q and k: float16, bfloat16 or float32, any row and head strides (views of a projection's rows), D up to
     2048.  q_weight, k_weight: [D] of the same type, or both float32; None: ones.  fp32 inside, rounded once.
-    `q_out` may be q, `k_out` k; else they share no memory with q and k.  Where q, k or a weight requires grad the outputs record it (without q_out and k_out; once
-    differentiable; the table has none): the weights' gradients are sums over all tokens and heads in a fixed order.
+    `q_out` may be q, `k_out` k; else they share no memory with q and k.  Where q, k or a weight requires grad the
+    outputs record it (without q_out and k_out; once differentiable; the table has none; no forward mode): the
+    weights' gradients are sums over all tokens and heads in a fixed order.
     With `plan`, only rows < plan[0]: the others of new outputs and gradients are 0, those of q_out and k_out keep
     what they hold."""
     return _native.qk_norm_rope(q, k, q_weight, k_weight, pos, table, eps, layout, q_out, k_out, plan)

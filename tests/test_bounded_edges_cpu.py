@@ -1,8 +1,11 @@
-"""The workspace of the operators around a bounded cache, without a GPU."""
+"""Normalised heads, beams and the bounded cache without a GPU: workspaces, and gradients that the operators do not have."""
 import ctypes
 
 import pytest
+import torch
+from torch.autograd import forward_ad
 
+import specq
 from specq import _lib
 
 SPACE = 512 << 20
@@ -29,3 +32,36 @@ def test_workspace_of_ordinary_calls():
     assert _mass(32, 1, 4, 8, 512) == 32 * 8 * 4 * (8192 * 4 + 8192 // 2048 * 8)
     assert _mass(2, 64, 4, 8, 1024) == 2 * 8 * 256 * (16384 // 256 * 8 + 4)
     assert _mass(0, 1, 4, 8, 512) == 0
+
+
+@pytest.mark.parametrize("what", ["q", "k", "q_weight", "k_weight", "x", "logits", "scores", "state", "mass"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(what, grad):
+    """A dual tensor's tangent would be lost without a word."""
+    F16 = torch.float16
+    pos, table, kc = torch.zeros(4, dtype=torch.int32), torch.zeros(8, 64), torch.zeros(2, 16, 2, 64, dtype=torch.int8)
+    a = {"q": torch.zeros(4, 4, 64, dtype=F16), "k": torch.zeros(4, 2, 64, dtype=F16), "q_weight": torch.ones(64, dtype=F16),
+         "k_weight": torch.ones(64, dtype=F16), "x": torch.zeros(4, 4, 64), "logits": torch.zeros(4, 10), "scores": torch.zeros(2, 2),
+         "state": torch.zeros(4, 3), "mass": torch.zeros(1, 2, 32)}
+    i32 = torch.zeros(1, 2, dtype=torch.int32)
+
+    def call(a):
+        if what in ("q", "k", "q_weight", "k_weight"):
+            return specq.qk_norm_rope(a["q"], a["k"], a["q_weight"], a["k_weight"], pos, table)
+        if what == "x":
+            return specq.rope(a["x"], pos, table)
+        if what in ("logits", "scores"):
+            return specq.beam_select(a["logits"], a["scores"])
+        if what == "state":
+            return specq.beam_reorder([a["state"]], pos, beams=2)
+        return specq.attention_mass_blocks(a["q"][:1, None], kc, torch.ones(2, 2), i32, i32[:, 0], a["mass"])
+    if grad and what in ("q", "k", "q_weight", "k_weight", "x"):
+        a[what].requires_grad_(True)
+    with forward_ad.dual_level():
+        dual = dict(a, **{what: forward_ad.make_dual(a[what], torch.ones_like(a[what]))})
+        with pytest.raises(ValueError, match="forward-mode"):
+            call(dual)
+        with forward_ad._set_fwd_grad_enabled(False), pytest.raises(ValueError, match="CUDA"):
+            call(dual)
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        call(a)
