@@ -132,6 +132,12 @@ void written(const char* who, const char* what, const Tensor& t) {
     if (t.stride(i) == 0 && t.size(i) > 1) BAD_VALUE("%s: %s is written and must not be expanded (dimension %lld)", who, what, (long long)i);
 }
 
+// The call has written these tensors of the caller: a backward pass that saved one is to know.
+void wrote(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 // Forward-mode differentiation has no form here: a tensor that carries a tangent is refused, since the result would have none.
 void no_tangent(const char* who, std::initializer_list<const Tensor*> ts) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
@@ -263,6 +269,7 @@ PyObject* rope(PyObject* const* a) {
   check(lib.rope(x.data_ptr(), x.stride(0), x.stride(1), out.data_ptr(), out.stride(0), out.stride(1), row_code(x), ptr<int32_t>(pos),
                  ptr<float>(table), size32(who, table.size(0)), size32(who, x.size(0)), size32(who, x.size(1)), size32(who, x.size(2)),
                  size32(who, table.size(1)), lay, inverse, plan_at, stream()));
+  wrote({given});
   return wrap(out);
 }
 
@@ -322,6 +329,7 @@ PyObject* kv_append_blocks(PyObject* const* a) {
       c.kc.stride(1), c.kc.stride(2), cache_code(c.kc), size32(who, c.P), ptr<float>(c.ks), ptr<float>(c.vs), c.ks.stride(0),
       c.ks.stride(1), ptr<int32_t>(tbl), tbl.stride(0), size32(who, tbl.size(1)), ptr<int32_t>(ctx), plan_at, B, n_seqs,
       q_len, ql_max, qs ? size32(who, q->size(1)) : 0, size32(who, c.H), size32(who, c.D), size32(who, c.page), stream()));
+  wrote({&c.kc, &c.vc, &c.ks, &c.vs, q_given});
   return qs ? wrap(q_out) : none();
 }
 
@@ -390,6 +398,7 @@ PyObject* paged_attention_blocks(PyObject* const* a) {
       ptr<int32_t>(tbl), tbl.stride(0), cols, ptr<int32_t>(ctx), tree ? reinterpret_cast<const uint64_t*>(tree->data_ptr()) : nullptr,
       tree ? tree->stride(0) : 0, tree ? tree->stride(1) : 0, sm, out.data_ptr(), packed ? 0 : out.stride(0), out.stride(o),
       out.stride(o + 1), plan_at, B, n_seqs, q_len, ql_max, h, hk, D, page, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream()));
+  wrote({given});
   return wrap(out);
 }
 
@@ -417,6 +426,7 @@ PyObject* kv_compact_blocks(PyObject* const* a) {
                           c.ks.stride(d + 1), ptr<int32_t>(tbl), tbl.stride(0), size32(who, tbl.size(1)), ptr<int32_t>(ctx),
                           ptr<int32_t>(acc), acc.stride(0), size32(who, acc.size(1)), ptr<int32_t>(n_acc), ptr<int32_t>(out),
                           size32(who, B), q_len, size32(who, c.H), size32(who, c.D), size32(who, c.page), stream()));
+  wrote({&c.kc, &c.vc, &c.ks, &c.vs, given});
   return wrap(out);
 }
 
@@ -448,6 +458,7 @@ PyObject* pages_release(PyObject* const* a) {
   if (length == nullptr) {
     same_device(who, {&p.ref, &p.tbl, &p.held, &drop});
     check(lib.pages_release(ptr<int32_t>(p.ref), p.P, ptr<int32_t>(p.tbl), p.ld, ptr<int32_t>(p.held), p.S, p.C, ptr<uint8_t>(drop), stream()));
+    wrote({&p.ref, &p.tbl, &p.held});
     return none();
   }
   int32s(who, "length", *length, 1, p.S);
@@ -456,6 +467,7 @@ PyObject* pages_release(PyObject* const* a) {
   same_device(who, {&p.ref, &p.tbl, &p.held, &drop, length});
   check(lib.pages_trim(ptr<int32_t>(p.ref), p.P, ptr<int32_t>(p.tbl), p.ld, ptr<int32_t>(p.held), p.S, p.C, ptr<uint8_t>(drop),
                        ptr<int32_t>(*length), page, stream()));
+  wrote({&p.ref, &p.tbl, &p.held});
   return none();
 }
 
@@ -473,6 +485,7 @@ PyObject* pages_reserve(PyObject* const* a) {
   const Tensor out = given != nullptr ? *given : new_int32(p.ref, 1);
   check(lib.pages_reserve(ptr<int32_t>(p.ref), p.P, ptr<int32_t>(p.tbl), p.ld, ptr<int32_t>(p.held), p.S, p.C, ptr<int32_t>(want), page,
                           ptr<int32_t>(out), stream()));
+  wrote({&p.ref, &p.tbl, &p.held, given});
   return wrap(out);
 }
 
@@ -495,6 +508,7 @@ PyObject* pages_fork(PyObject* const* a) {
                        ptr<float>(c.ks), ptr<float>(c.vs), c.s_sl(), c.ks.stride(d), c.ks.stride(d + 1), ptr<int32_t>(p.ref), p.P,
                        ptr<int32_t>(p.tbl), p.ld, ptr<int32_t>(p.held), p.S, p.C, ptr<int32_t>(parent), ptr<int32_t>(length),
                        ptr<int32_t>(scratch), ptr<int32_t>(out), size32(who, c.H), size32(who, c.D), size32(who, c.page), stream()));
+  wrote({&c.kc, &c.vc, &c.ks, &c.vs, &p.ref, &p.tbl, &p.held, given});
   return wrap(out);
 }
 
@@ -688,6 +702,7 @@ PyObject* qk_norm_rope(PyObject* const* a) {
   const bool all = x.plan == nullptr;
   const Tensor q_out = q_given != nullptr ? *q_given : new_rows(x.q, all), k_out = k_given != nullptr ? *k_given : new_rows(x.k, all);
   check(launch_qk_norm_rope(x.q, x.k, qw, kw, x.pos, x.table, plan, x.eps, x.layout, q_out, k_out));
+  wrote({q_given, k_given});
   return pack({q_out, k_out});
 }
 
@@ -772,6 +787,7 @@ PyObject* beam_reorder(PyObject* const* a) {
   for (Py_ssize_t i = 0; i < count; ++i) same_device(who, {&parent, &THPVariable_Unpack(items[i])});
   same_device(who, {&parent});
   check(lib.beam_reorder(at_.data(), stride.data(), bytes.data(), size32(who, count), ptr<int32_t>(parent), size32(who, R / K), K, stream()));
+  for (Py_ssize_t i = 0; i < count; ++i) wrote({&THPVariable_Unpack(items[i])});
   return none();
 }
 
@@ -840,6 +856,7 @@ PyObject* attention_mass_blocks(PyObject* const* a) {
                            ptr<int32_t>(tbl), tbl.stride(0), cols, ptr<int32_t>(ctx), ptr<int32_t>(n_rows), sm, static_cast<float>(decay),
                            ptr<float>(mass), mass.stride(0), mass.stride(1), B, q_len, h, hk, D, page, bytes > 0 ? ws.data_ptr() : nullptr, bytes,
                            stream()));
+  wrote({&mass});
   Py_INCREF(a[5]);
   return a[5];
 }
@@ -874,6 +891,7 @@ PyObject* kv_evict_blocks(PyObject* const* a) {
                         tbl.stride(0), size32(who, tbl.size(1)), ptr<int32_t>(ctx), ptr<int32_t>(ref), ptr<float>(mass), d ? mass.stride(0) : 0,
                         mass.stride(d), mass.stride(d + 1), keep, recent, ptr<int32_t>(out), b, h, size32(who, c.D), size32(who, c.page),
                         ws.data_ptr(), bytes, stream()));
+  wrote({&c.kc, &c.vc, &c.ks, &c.vs, &mass, given});
   return wrap(out);
 }
 

@@ -136,3 +136,48 @@ def test_mass_of_short_contexts_in_a_wide_table(cuda, B, Q, KV, G, cols):
         assert torch.equal(m[b, :, n:], before[b, :, n:])
     packed = specq.attention_mass_blocks(q.flatten(0, 1), kc, ks, tbl, _i32(ctx), before, q_len=Q, n_rows=_i32(rows), decay=0.5)
     assert torch.equal(packed, m)
+
+
+def test_what_is_written_in_place_is_known_to_autograd(cuda):
+    """A tensor that a call has written counts as changed, so that a backward pass that saved it ends in an error, not in a wrong gradient."""
+    import specq
+    g = torch.Generator(device="cuda").manual_seed(9)
+    D, page = 64, 16
+    table, pos = specq.rope_table(32, D), torch.arange(4, dtype=torch.int32, device="cuda")
+    w = torch.ones(D, device="cuda", dtype=torch.float16, requires_grad=True)
+    q, k, v = (torch.randn(4, 2, D, generator=g, device="cuda").half() for _ in range(3))
+    kc, vc, ks, vs = _cache(4, page, 2, D, torch.int8, g)
+    tbl, ctx = _i32([[0, 1], [2, 3]]), _i32([20, 18])
+    mass, state = torch.zeros(2, 2, 32, device="cuda"), torch.zeros(4, 3, device="cuda")
+
+    def saved(call, *written):
+        before = [t._version for t in written]
+        call()
+        return all(t._version > n for t, n in zip(written, before))
+    assert saved(lambda: specq.rope(q, pos, table, out=q), q)
+    assert saved(lambda: specq.qk_norm_rope(q, k, None, None, pos, table, q_out=q, k_out=k), q, k)
+    assert saved(lambda: specq.kv_append_blocks(k, v, kc, vc, ks, vs, tbl, ctx, 2, q=q, q_out=q, table=table), q, kc, vc, ks, vs)
+    out = torch.empty_like(q)
+    assert saved(lambda: specq.paged_attention_blocks(q, kc, vc, ks, vs, tbl, ctx, q_len=2, out=out), out)
+    assert saved(lambda: specq.attention_mass_blocks(q, kc, ks, tbl, ctx, mass, q_len=2), mass)
+    assert saved(lambda: specq.kv_compact_blocks(kc, vc, ks, vs, tbl, ctx, 2, _i32([[0], [1]]), _i32([1, 1])), kc, vc, ks, vs)
+    assert saved(lambda: specq.kv_evict_blocks(kc, vc, ks, vs, tbl, ctx, mass, 8, ctx_out=ctx), kc, vc, ks, vs, mass, ctx)
+    assert saved(lambda: specq.beam_reorder([state, pos], _i32([[1, 0], [2, 2]])), state, pos)
+    ref, held, drop = _i32([1, 1, 1, 1]), _i32([2, 2]), torch.tensor([False, True], device="cuda")
+    assert saved(lambda: specq.pages_release(ref, tbl, held, drop), ref, tbl, held)
+    assert saved(lambda: specq.pages_reserve(ref, tbl, held, _i32([20, 20]), page), ref, tbl, held)
+    assert saved(lambda: specq.pages_fork(kc, vc, ks, vs, ref, tbl, held, _i32([-1, 0]), _i32([20, 20])), kc, vc, ks, vs, ref, tbl, held)
+    assert saved(lambda: specq.pages_release(ref, tbl, held, drop, length=_i32([3, 3]), page=page), ref, tbl, held)
+
+    pos = torch.arange(4, dtype=torch.int32, device="cuda")
+    for change in (lambda: specq.rope(q, pos, table, out=q), lambda: specq.beam_reorder([pos], _i32([1, 0, 2, 3]), beams=4)):
+        a, _ = specq.qk_norm_rope(q, k, w, w, pos, table)
+        change()
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            a.sum().backward()
+    a, _ = specq.qk_norm_rope(q, k, w, w, pos, table)
+    torch.autograd.grad(a.float().sum(), w)
+    with torch.inference_mode():                            # tensors without a count
+        x = q.clone()
+        specq.rope(x, pos, table, out=x)
+    specq.rope(x, pos, table, out=x)
