@@ -414,7 +414,8 @@ int specq_qk_norm_rope_grad_workspace(int T, int H, int H_KV, int D, int64_t* by
  *   scores   fp32 [B K]; candidate (k, v) has the total score + logit - ln sum exp logits of its beam
  *   done     optional uint8 [B K]: a finished beam's one candidate is (k, pad) with the beam's score
  *   out_*    [B, n]: totals in fp32 in falling order, the candidate's row, its token; equal totals
- *            (compared in 64 bits) by k V + v.  A total of -inf is no candidate; a place without one has
+ *            (compared in 64 bits) by k V + v; a beam's log-sum-exp is good to some 1e-7 (2e-6 at worst), and totals
+ *            of two beams that are closer have no order.  A total of -inf is no candidate; a place without one has
  *            score -inf, row b K + j mod K and the pad token.  A NaN logit or score counts as -inf, a
  *            logit of +inf as its type's largest finite number, a score of +inf as -inf.
  * K <= 64, n <= 128, B K <= 65535, K V < 2^31.  workspace as the function below gives, 16-byte aligned.

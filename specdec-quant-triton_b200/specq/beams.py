@@ -24,7 +24,9 @@ def beam_select(logits, scores, n=None, done=None, pad=0, beams=None):
     beam goes on as itself only, by the token `pad` at its own score.
 
     Returns scores' float32, parent int32 (rows) and token int32, each [B, n], best first; equal totals (in 64
-    bits) by beam, then token.  A candidate of total -inf (a masked token) is never chosen: a place that is left
+    bits) by beam, then token.  A beam's log-sum-exp is good to some 1e-7 (2e-6 at worst), so totals of different
+    beams that are closer than that come in either order, those of equal rows too unless the rows begin alike
+    (their addresses modulo 16 bytes); and so do logits of one beam too close for their totals in 64 bits.  A candidate of total -inf (a masked token) is never chosen: a place that is left
     without one has score -inf, token `pad` and the row b * beams + j % beams, which for j < beams is
     the place's own.  NaN logits count as -inf, +inf ones as their type's largest finite number; a NaN or +inf score as -inf.
     Up to 64 beams and n = 128."""
