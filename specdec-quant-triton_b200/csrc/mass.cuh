@@ -39,7 +39,8 @@ constexpr int kMassWarps = kMassThreads / 32;
 constexpr int kMassTiles = 2;                // tiles of 32 tokens that a warp takes of a block's
 constexpr int kMassChunk = 32 * kMassWarps * kMassTiles;   // tokens of a block
 constexpr int kMassFew = 16;                 // rows of one product
-constexpr int kMassRows = 128;               // rows of q in shared memory at a time where there are more
+constexpr int kMassWide = 96;                // rows from which the products go to tcgen05 (mass_wide.cuh)
+constexpr int kMassRows = kMassWide;         // rows of q in shared memory where there are more than kMassFew
 constexpr int kMassStages = 2;               // tiles of a warp on their way, up to 16 rows
 constexpr int kMassCluster = 8;              // blocks that share their sums
 constexpr int kMassSms = 148;                // how a call is cut does not ask the device: its workspace is known without one
@@ -133,16 +134,17 @@ __device__ __forceinline__ void mass_extent(const MassParams& p, int b, bool tel
   nr = n <= 0 ? 0 : p.n_rows == nullptr ? p.q_len : min(max(p.n_rows[b], 0), p.q_len);
 }
 
-// `here` rows of q from row `first` of the KV head, padded with zeros to PAD, to fp16 in shared memory; their factors and limits.
+// A sequence's rows of q of the KV head, padded with zeros to `pad`, to fp16 in shared memory; their factors and limits.
 template <bool BF, int D, int ROWS, typename Smem>
-__device__ __forceinline__ void mass_queries(const MassParams& p, Smem& sm, int b, int h, int first, int here, int pad, int base) {
-  constexpr int kPieces = D / 8, kLanes = kMassThreads / ROWS < kPieces ? kMassThreads / ROWS : kPieces, kMine = D / kLanes;   // threads of a row, elements of each
+__device__ __forceinline__ void mass_queries(const MassParams& p, Smem& sm, int b, int h, int rows, int pad, int base) {
+  constexpr int kPieces = D / 8, kLanes = 2, kMine = D / kLanes;   // threads of a row, elements of each
+  static_assert(ROWS * kLanes <= kMassThreads, "every row has its threads");
   const int tid = static_cast<int>(threadIdx.x);
   for (int i = tid; i < pad * kPieces; i += kMassThreads) {
     const int r = i / kPieces, c = i - r * kPieces;
     __half* dst = sm.q + r * Smem::kQStride + c * 8;
-    if (r < here) {
-      const int row = (first + r) / p.group, head = h * p.group + (first + r) - row * p.group;
+    if (r < rows) {
+      const int row = r / p.group, head = h * p.group + r - row * p.group;
       const int64_t at = (p.q_sb != 0 ? b * p.q_sb + row * p.q_st : (static_cast<int64_t>(b) * p.q_len + row) * p.q_st) + head * p.q_sh;
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(static_cast<const __half*>(p.q) + at + c * 8) : "memory");
     } else {
@@ -190,7 +192,7 @@ __device__ __forceinline__ void mass_queries(const MassParams& p, Smem& sm, int 
     }
     if (lane == 0) {
       sm.factor[r] = factor;
-      sm.lim[r] = r < here && finite ? base + (first + r) / p.group : -1;
+      sm.lim[r] = r < rows && finite ? base + r / p.group : -1;
     }
   }
   __syncthreads();
@@ -397,7 +399,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
     }
   };
   // the warps' sums to the block's, and (a cluster) the blocks' to lse
-  auto block_stats = [&](int first, int here, int pad) {
+  auto block_stats = [&](int pad) {
     __syncthreads();
     for (int r = threadIdx.x; r < pad; r += kMassThreads) {
       float2 x = make_float2(-INFINITY, 0.f);
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
       for (int w = 0; w < kMassWarps; ++w) x = join_stats(x, sm.part[w][r]);
       if (sm.lim[r] < 0) x = make_float2(-INFINITY, 0.f);
       if (MODE == kMassStats) {
-        if (r < here) p.stats[(bh * p.chunks + chunk) * p.rows + first + r] = x;
+        if (r < rows) p.stats[(bh * p.chunks + chunk) * p.rows + r] = x;
       } else {
         sm.all[r] = x;
       }
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
         sm.lse[r] = stats_lse(x);
       }
       __syncthreads();
-      cluster_arrive();                       // this block has read its peers' sums (waited for before `all` is written again, and at the end)
+      cluster_arrive();                       // this block has read its peers' sums (waited for at the end)
       return;
     }
     __syncthreads();
@@ -483,7 +485,7 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
       }
       if (tq == 0) sm.part[warp][g + 4 * e] = x;
     }
-    block_stats(0, rows, kMassFew);
+    block_stats(kMassFew);
     {
       if (t0[0] < n) {
         const float f0 = exp2_fast(top[0] - sm.lse[g]), f1 = exp2_fast(top[1] - sm.lse[g + 8]);
@@ -496,58 +498,54 @@ __global__ void __launch_bounds__(kMassThreads, ROWS == kMassFew ? 3 : 2) mass_k
       }
     }
   } else {
-    for (int first = 0; first < rows; first += kMassRows) {
-      const int here = min(kMassRows, rows - first), pad = (here + 15) & ~15;
-      if (first > 0) {
-        __syncthreads();                      // q, lim and lse are no longer read
-        if (MODE == kMassWhole && active > 1) cluster_wait();
-      }
-      mass_queries<BF, D, ROWS>(p, sm, b, h, first, here, pad, base);
-      if constexpr (MODE == kMassWeights) {
-        for (int r = threadIdx.x; r < pad; r += kMassThreads) sm.lse[r] = r < here ? p.lse[bh * p.rows + first + r] : INFINITY;
-        __syncthreads();
-      } else {
+    const int pad = (rows + 15) & ~15;
+    mass_queries<BF, D, ROWS>(p, sm, b, h, rows, pad, base);
+    if constexpr (MODE == kMassWeights) {
+      for (int r = threadIdx.x; r < pad; r += kMassThreads) sm.lse[r] = r < rows ? p.lse[bh * p.rows + r] : INFINITY;
+      __syncthreads();
+    } else {
 #pragma unroll
-        for (int i = 0; i < kMassTiles; ++i) {
-          uint32_t k[4][C][4][2];
+      for (int i = 0; i < kMassTiles; ++i) {
+        uint32_t k[4][C][4][2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) widen(i, j, k[j]);
+        for (int j = 0; j < 4; ++j) widen(i, j, k[j]);
 #pragma unroll 1
-          for (int r0 = 0; r0 < pad; r0 += 16) {
-            uint32_t a[C][4][4];
-            float s[4][4];
-            fragments(r0, a);
+        for (int r0 = 0; r0 < pad; r0 += 16) {
+          asm volatile("" : "+r"(r0));         // addresses from r0 alone: a pointer each for q, factors, limits and sums spilled (36 rows 49 us)
+          uint32_t a[C][4][4];
+          float s[4][4];
+          fragments(r0, a);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
-            scale(i, r0, s);
-            hide(i, r0, s);
-            const float2 u = row_stats(s, 0), v = row_stats(s, 2);
-            if (tq == 0) {
-              float2* at = &sm.part[warp][r0 + g];
-              at[0] = i == 0 ? u : join_stats(at[0], u);
-              at[8] = i == 0 ? v : join_stats(at[8], v);
-            }
+          for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
+          scale(i, r0, s);
+          hide(i, r0, s);
+          const float2 u = row_stats(s, 0), v = row_stats(s, 2);
+          if (tq == 0) {
+            float2* at = &sm.part[warp][r0 + g];
+            at[0] = i == 0 ? u : join_stats(at[0], u);
+            at[8] = i == 0 ? v : join_stats(at[8], v);
           }
         }
-        block_stats(first, here, pad);
       }
-      if constexpr (MODE != kMassStats) {
+      block_stats(pad);
+    }
+    if constexpr (MODE != kMassStats) {
 #pragma unroll
-        for (int i = 0; i < kMassTiles; ++i) {
-          uint32_t k[4][C][4][2];
+      for (int i = 0; i < kMassTiles; ++i) {
+        uint32_t k[4][C][4][2];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) widen(i, j, k[j]);
+        for (int j = 0; j < 4; ++j) widen(i, j, k[j]);
 #pragma unroll 1
-          for (int r0 = 0; r0 < pad; r0 += 16) {
-            uint32_t a[C][4][4];
-            float s[4][4];
-            fragments(r0, a);
+        for (int r0 = 0; r0 < pad; r0 += 16) {
+          asm volatile("" : "+r"(r0));
+          uint32_t a[C][4][4];
+          float s[4][4];
+          fragments(r0, a);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
-            scale(i, r0, s);
-            hide(i, r0, s);
-            add_weights(i, r0, s);
-          }
+          for (int j = 0; j < 4; ++j) product(a, k[j], s[j]);
+          scale(i, r0, s);
+          hide(i, r0, s);
+          add_weights(i, r0, s);
         }
       }
     }
