@@ -326,10 +326,16 @@ inline int evict_check(int L, int B, int H_KV, int D, int page, int keep, int re
   return SPECQ_OK;
 }
 
+// Sequences of a turn: a place for each token that may be kept, by layers and heads, goes by `keep`, whatever the sequences hold.  (A budget
+// of 131072 tokens in 32 layers of 64 sequences and 8 heads would be 8.6 GB.)
+inline int evict_turn(int L, int B, int H_KV, int keep) {
+  return even_turn(B, kTurnSpace / (static_cast<int64_t>(L) * H_KV * (static_cast<int64_t>(keep) + 1) * 4));
+}
+
 inline int run_block_evict_workspace(int L, int B, int H_KV, int keep, int64_t* bytes) {
   if (bytes == nullptr) return fail(SPECQ_ERR_INVALID_ARG, "block_evict_workspace: null pointer");
   if (int rc = evict_check(L, B, H_KV, 64, 8, keep, 0, 0)) return rc;
-  *bytes = static_cast<int64_t>(L) * B * H_KV * (static_cast<int64_t>(keep) + 1) * 4;
+  *bytes = static_cast<int64_t>(L) * evict_turn(L, B, H_KV, keep) * H_KV * (static_cast<int64_t>(keep) + 1) * 4;
   return SPECQ_OK;
 }
 
@@ -356,32 +362,40 @@ inline int run_block_evict(void* kc, void* vc, int64_t kv_sl, int64_t kv_sp, int
   if (int rc = get_device_state(&dev)) return rc;
   EvictParams p = {};
   p.kc = static_cast<uint8_t*>(kc); p.vc = static_cast<uint8_t*>(vc); p.ks = ks; p.vs = vs;
-  p.bt = block_tbl; p.ctx = ctx_len; p.ref = ref; p.mass = mass; p.ctx_out = ctx_out; p.status = dev->status;
+  p.ref = ref; p.status = dev->status;
   p.place = static_cast<int32_t*>(workspace);
-  p.first = p.place + static_cast<int64_t>(L) * B * H_KV * keep;
   p.kv_sl = kv_sl; p.kv_sp = kv_sp; p.kv_so = kv_so; p.kv_sh = kv_sh; p.s_sl = s_sl; p.s_sp = s_sp; p.s_sh = s_sh;
   p.bt_sb = bt_sb; p.m_sl = m_sl; p.m_sb = m_sb; p.m_sh = m_sh;
-  p.n_pages = n_pages; p.bt_cols = bt_cols; p.B = B; p.h_kv = H_KV; p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
+  p.n_pages = n_pages; p.bt_cols = bt_cols; p.h_kv = H_KV; p.page_log2 = __builtin_ctz(static_cast<unsigned>(page));
   p.keep = keep; p.recent = recent; p.linear = kv_sp == page * kv_so;
-  const bool few = static_cast<int64_t>(H_KV) * B * L <= 2 * static_cast<int64_t>(dev->sm_count);
+  const int turn = evict_turn(L, B, H_KV, keep);
+  const bool few = static_cast<int64_t>(H_KV) * turn * L <= 2 * static_cast<int64_t>(dev->sm_count);
   p.staged = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(bt_cols) * page, few ? kEvictStage : kEvictStageMany));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(H_KV, B, L);
-  cfg.blockDim = dim3(kEvictSelThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(p.staged) * 4;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  LaunchAttrs at(1);
-  at.apply(cfg);
   SPECQ_CUDA_TRY(ensure_dyn_smem(reinterpret_cast<const void*>(evict_select_kernel), kEvictStage * 4));
-  SPECQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
-  cfg.gridDim = dim3(2 * H_KV, B, L);
-  cfg.blockDim = dim3(kEvictMoveThreads);
-  cfg.dynamicSmemBytes = 0;
   const bool i8 = cache_dtype == SPECQ_CACHE_INT8;
-  cudaError_t e;
-  if (D == 64) e = i8 ? cudaLaunchKernelEx(&cfg, evict_move_kernel<0, 64>, p) : cudaLaunchKernelEx(&cfg, evict_move_kernel<1, 64>, p);
-  else e = i8 ? cudaLaunchKernelEx(&cfg, evict_move_kernel<0, 128>, p) : cudaLaunchKernelEx(&cfg, evict_move_kernel<1, 128>, p);
-  SPECQ_CUDA_TRY(e);
+  LaunchAttrs at(1);
+  for (int b0 = 0; b0 < B; b0 += turn) {
+    p.B = std::min(turn, B - b0);
+    p.first = p.place + static_cast<int64_t>(L) * p.B * H_KV * keep;
+    p.bt = block_tbl + b0 * bt_sb;
+    p.ctx = ctx_len + b0;
+    p.ctx_out = ctx_out + b0;
+    p.mass = mass + b0 * m_sb;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(H_KV, p.B, L);
+    cfg.blockDim = dim3(kEvictSelThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(p.staged) * 4;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    at.apply(cfg);
+    SPECQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
+    cfg.gridDim = dim3(2 * H_KV, p.B, L);
+    cfg.blockDim = dim3(kEvictMoveThreads);
+    cfg.dynamicSmemBytes = 0;
+    cudaError_t e;
+    if (D == 64) e = i8 ? cudaLaunchKernelEx(&cfg, evict_move_kernel<0, 64>, p) : cudaLaunchKernelEx(&cfg, evict_move_kernel<1, 64>, p);
+    else e = i8 ? cudaLaunchKernelEx(&cfg, evict_move_kernel<0, 128>, p) : cudaLaunchKernelEx(&cfg, evict_move_kernel<1, 128>, p);
+    SPECQ_CUDA_TRY(e);
+  }
   return SPECQ_OK;
 }
 

@@ -42,11 +42,10 @@ inline bool mass_plan(int B, int H_KV, int rows, int tokens, int* chunk_tiles, i
 }
 
 // What a call keeps in its workspace goes by the table's width, whatever is cached of it: 4 bytes for each row and token (up to 16 rows),
-// or 8 for each row and block of 256 or 512 tokens, of every KV head of every sequence.  Past kMassSpace it goes through its sequences, or
+// or 8 for each row and block of 256 or 512 tokens, of every KV head of every sequence.  Past kTurnSpace it goes through its sequences, or
 // the KV heads of one, in several turns of one size over the same workspace, which is then at most that or what one KV head of one
 // sequence takes.  (16 rows of 64 sequences, 8 heads and a table of 131072 tokens: 512 MB in place of 4.3 GB.  A turn costs some 10 us: the
 // same rows of 32 sequences of 32768 tokens take 454 us in one turn of 540 MB, 470 in two and 497 in three.)
-constexpr int64_t kMassSpace = 512ll << 20;
 
 struct MassCut {
   bool whole;                  // in one launch, without a workspace
@@ -63,13 +62,9 @@ inline MassCut mass_cut(int B, int H_KV, int rows, int tokens) {
   if (c.whole || B == 0) return c;
   const int64_t stats = static_cast<int64_t>(rows) * c.chunks * 8;
   const int64_t one = stats + (rows <= kMassFew ? static_cast<int64_t>(rows) * c.chunks * c.chunk_tiles * kMassThreads * 4 : static_cast<int64_t>(rows) * 4);
-  auto even = [](int n, int64_t most) {            // turns of at most `most`, all but alike
-    const int turns = most >= n ? 1 : static_cast<int>((n + std::max<int64_t>(most, 1) - 1) / std::max<int64_t>(most, 1));
-    return (n + turns - 1) / turns;
-  };
   if (one > 0) {
-    c.seqs = even(B, kMassSpace / (one * H_KV));
-    if (one * H_KV > kMassSpace) c.heads = even(H_KV, kMassSpace / one);
+    c.seqs = even_turn(B, kTurnSpace / (one * H_KV));
+    if (one * H_KV > kTurnSpace) c.heads = even_turn(H_KV, kTurnSpace / one);
   }
   c.bytes = one * c.seqs * c.heads;
   return c;

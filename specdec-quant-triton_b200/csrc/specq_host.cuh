@@ -196,6 +196,15 @@ inline int next_pow2(int x) {
   while (p < x) p <<= 1;
   return p;
 }
+// n things in turns of at most `most` (one at least), all but alike: how many a turn.
+inline int even_turn(int n, int64_t most) {
+  if (n <= 0 || most >= n) return n;
+  const int step = static_cast<int>(std::max<int64_t>(most, 1));
+  return ceil_div(n, ceil_div(n, step));
+}
+// What a call that can go through its sequences in turns takes for its workspace.
+constexpr int64_t kTurnSpace = 512ll << 20;
+
 inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 
 // Programmatic dependent launch: every kernel of this library may be scheduled while the

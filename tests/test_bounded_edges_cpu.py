@@ -26,12 +26,26 @@ def test_workspace_of_a_wide_table_is_bounded(B, KV, tokens, q_len, G):
     assert min(one, 1) <= got <= max(SPACE, one), (one, got)
 
 
+def _evict(L, B, KV, keep):
+    n = ctypes.c_int64(-1)
+    assert _lib.load().specq_block_evict_workspace(L, B, KV, keep, ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("L,B,KV,keep", [(32, 64, 8, 131072), (80, 256, 8, 32768), (1, 65535, 1, 4096), (64, 3, 8, 1 << 20)])
+def test_workspace_of_a_large_budget_is_bounded(L, B, KV, keep):
+    one, got = _evict(L, 1, KV, keep), _evict(L, B, KV, keep)
+    assert one <= got <= max(SPACE, one), (one, got)
+
+
 def test_workspace_of_ordinary_calls():
     """Nothing for what a cluster holds; 8 bytes a row and block and 4 a row and token for a stream of tiles; the sums alone for many rows."""
     assert _mass(1, 1, 4, 8, 4) == 0
     assert _mass(32, 1, 4, 8, 512) == 32 * 8 * 4 * (8192 * 4 + 8192 // 2048 * 8)
     assert _mass(2, 64, 4, 8, 1024) == 2 * 8 * 256 * (16384 // 256 * 8 + 4)
     assert _mass(0, 1, 4, 8, 512) == 0
+    assert _evict(4, 12, 8, 1024) == 4 * 12 * 8 * 1025 * 4
+    assert _evict(4, 0, 8, 1024) == 0
 
 
 @pytest.mark.parametrize("what", ["q", "k", "q_weight", "k_weight", "x", "logits", "scores", "state", "mass"])

@@ -181,3 +181,28 @@ def test_what_is_written_in_place_is_known_to_autograd(cuda):
         x = q.clone()
         specq.rope(x, pos, table, out=x)
     specq.rope(x, pos, table, out=x)
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_evict_of_a_large_budget_goes_in_turns(cuda, given):
+    """260 sequences, 8 heads and a budget of 65536 tokens: more places than the workspace has.  As one sequence after another; the pages are
+    all alike, so that the masses and lengths alone tell the tokens apart."""
+    import specq
+    g = torch.Generator(device="cuda").manual_seed(13)
+    B, KV, D, page, keep, recent = 260, 8, 64, 128, 65536, 100
+    cols = keep // page + 1
+    kc, vc = (torch.zeros(B, page, KV, D, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = torch.ones(B, KV, device="cuda"), torch.ones(B, KV, device="cuda")
+    tbl = torch.arange(B, dtype=torch.int32, device="cuda")[:, None].repeat(1, cols)
+    ctx = _i32([keep + (b * 7) % (page + 1) - 3 for b in range(B)])
+    mass = torch.rand(B, KV, cols * page, generator=g, device="cuda")
+    before, old = mass.clone(), ctx.tolist()
+    out = specq.kv_evict_blocks(kc, vc, ks, vs, tbl, ctx, mass, keep, recent, ctx_out=ctx if given else None)
+    assert out.tolist() == [min(n, keep) for n in old]
+    for b in (0, 1, 64, 129, 130, 200, 258, 259):
+        one = before[b:b + 1].clone()
+        n = specq.kv_evict_blocks(kc, vc, ks, vs, tbl[b:b + 1], _i32(old[b:b + 1]), one, keep, recent)
+        assert n.tolist() == [min(old[b], keep)] and torch.equal(one[0], mass[b])
+        if old[b] > keep:
+            at = O.evict_choice(before[b, 3].cpu().numpy(), old[b], keep, recent)
+            assert torch.equal(mass[b, 3, :keep], before[b, 3, torch.from_numpy(at).cuda()]) and not mass[b, 3, keep:old[b]].any()
