@@ -86,7 +86,7 @@ inline int run_attention_mass(const void* q, int64_t q_sb, int64_t q_st, int64_t
   if (int rc = mass_check(B, q_len, H, H_KV, D, page, bt_cols)) return rc;
   if (dtype != SPECQ_DTYPE_F16 && dtype != SPECQ_DTYPE_BF16) return fail(SPECQ_ERR_INVALID_ARG, "%s: dtype code %d", who, dtype);
   if (cache_dtype != SPECQ_CACHE_INT8 && cache_dtype != SPECQ_CACHE_E4M3) return fail(SPECQ_ERR_INVALID_ARG, "%s: cache dtype code %d", who, cache_dtype);
-  if (!(sm_scale > 0.f)) return fail(SPECQ_ERR_INVALID_ARG, "%s: sm_scale %g", who, static_cast<double>(sm_scale));
+  if (!(sm_scale > 0.f) || !(sm_scale < 2e38f)) return fail(SPECQ_ERR_INVALID_ARG, "%s: sm_scale %g", who, static_cast<double>(sm_scale));
   if (B == 0 || q_len == 0 || bt_cols == 0) return SPECQ_OK;
   if (q == nullptr || kc == nullptr || ks == nullptr || block_tbl == nullptr || ctx_len == nullptr || mass == nullptr)
     return fail(SPECQ_ERR_INVALID_ARG, "%s: null pointer", who);

@@ -840,7 +840,7 @@ PyObject* attention_mass_blocks(PyObject* const* a) {
   if (a[9] != Py_None) {
     const double v = PyFloat_AsDouble(a[9]);
     if (v == -1.0 && PyErr_Occurred()) throw Raised{};
-    if (!(v > 0)) BAD_VALUE("%s: sm_scale=%g must be positive", who, v);
+    if (!(v > 0) || !(v < 2e38)) BAD_VALUE("%s: sm_scale=%g must be positive and finite", who, v);
     sm = static_cast<float>(v);
   }
   same_device(who, {&c.kc, &c.ks, &q, &tbl, &ctx, n_rows, &mass});

@@ -79,3 +79,13 @@ def test_tangents_are_refused(what, grad):
             call(dual)
     with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
         call(a)
+
+
+@pytest.mark.parametrize("sm_scale", [float("inf"), 1e39, float("nan"), -1.0, 0.0])
+def test_mass_refuses_a_scale_that_is_not_finite(sm_scale):
+    """An infinite scale times a score of 0 would be NaN."""
+    kc, i32 = torch.zeros(2, 16, 2, 64, dtype=torch.int8), torch.zeros(1, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="sm_scale"):
+        specq.attention_mass_blocks(torch.zeros(1, 1, 4, 64).half(), kc, torch.ones(2, 2), i32, i32[:, 0], torch.zeros(1, 2, 32), sm_scale=sm_scale)
+    assert _lib.load().specq_attention_mass(16, 64, 64, 64, 0, 16, 64, 64, 64, 0, 4, 16, 1, 1, 16, 2, 2, 16, None, sm_scale, 1.0, 16, 64, 64, 1, 1, 1,
+                                            1, 64, 16, None, 0, None) == _lib.SPECQ_ERR_INVALID_ARG
