@@ -24,6 +24,7 @@
 namespace specq {
 
 constexpr int kEvictSelThreads = 256;
+static_assert(kEvictSelThreads == kSelThreads, "block_before's threads");
 constexpr int kEvictRun = 4;                                        // tokens a thread takes in the ordered pass
 // Keys held in shared memory: 192 KB of them where the rows leave each SM one block or two, else 48 KB, so that four blocks of
 // a wide table's short rows stay on an SM. (8 rows of 16384 tokens 75 us against 123 with 48 KB, 256 rows of 32768 213 against
@@ -51,28 +52,6 @@ struct EvictParams {
   int staged;              // keys that the shared memory holds
   int linear;              // kv_sp is a page of kv_so
 };
-
-// Exclusive sum over the block's threads.
-__device__ __forceinline__ int evict_before(int v, int* red, int* sum) {
-  const int lane = static_cast<int>(threadIdx.x & 31), warp = static_cast<int>(threadIdx.x >> 5);
-  int inc = v;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += up;
-  }
-  if (lane == 31) red[warp] = inc;
-  __syncthreads();
-  int base = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kEvictSelThreads / 32; ++w) {
-    if (w == warp) base = all;
-    all += red[w];
-  }
-  __syncthreads();
-  *sum = all;
-  return base + inc - v;
-}
 
 __global__ void __launch_bounds__(kEvictSelThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ uint32_t staged[];
@@ -179,7 +158,7 @@ __global__ void __launch_bounds__(kEvictSelThreads) evict_select_kernel(const __
       mine += (t < others && k[i] > bound) + (t < others && k[i] == bound ? 1 << 16 : 0);
     }
     int all;
-    const int before = evict_before(mine, red, &all);          // (its barriers: every thread has read its masses)
+    const int before = block_before(mine, red, &all);          // (its barriers: every thread has read its masses)
     int up = above + (before & 0xffff), eq = same + (before >> 16);
 #pragma unroll
     for (int i = 0; i < kEvictRun; ++i) {
