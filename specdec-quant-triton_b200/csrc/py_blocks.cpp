@@ -870,6 +870,9 @@ PyObject* kv_evict_blocks(PyObject* const* a) {
   const int64_t B = tbl.size(0);
   int32s(who, "ctx_len", ctx, 1, B);
   if (c.L == 0) BAD_VALUE("%s: a cache without layers", who);
+  // K and V are moved side by side
+  if ((c.kc.numel() > 0 && c.kc.data_ptr() == c.vc.data_ptr()) || (c.ks.numel() > 0 && c.ks.data_ptr() == c.vs.data_ptr()))
+    BAD_VALUE("%s: kc and vc, and ks and vs, must not be the same memory", who);
   int keep = integer(a[7]), recent = integer(a[8]);
   if (keep < 1 || recent < 0 || recent > keep) BAD_VALUE("%s: keep=%d, of these the newest recent=%d", who, keep, recent);
   // more than the table has room for: no row has as many, and none needs a place for them

@@ -89,3 +89,15 @@ def test_mass_refuses_a_scale_that_is_not_finite(sm_scale):
         specq.attention_mass_blocks(torch.zeros(1, 1, 4, 64).half(), kc, torch.ones(2, 2), i32, i32[:, 0], torch.zeros(1, 2, 32), sm_scale=sm_scale)
     assert _lib.load().specq_attention_mass(16, 64, 64, 64, 0, 16, 64, 64, 64, 0, 4, 16, 1, 1, 16, 2, 2, 16, None, sm_scale, 1.0, 16, 64, 64, 1, 1, 1,
                                             1, 64, 16, None, 0, None) == _lib.SPECQ_ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("same", ["vc", "vs"])
+def test_evict_refuses_one_cache_for_keys_and_values(same):
+    """Both would be moved at once."""
+    kc, i32 = torch.zeros(2, 16, 2, 64, dtype=torch.int8), torch.zeros(1, 2, dtype=torch.int32)
+    a = {"kc": kc, "vc": kc.clone(), "ks": torch.ones(2, 2), "vs": torch.ones(2, 2)}
+    with pytest.raises(ValueError, match="CUDA"):
+        specq.kv_evict_blocks(*a.values(), i32, i32[:, 0], torch.zeros(1, 2, 32), 8)
+    a[same] = a["k" + same[1]]
+    with pytest.raises(ValueError, match="same memory"):
+        specq.kv_evict_blocks(*a.values(), i32, i32[:, 0], torch.zeros(1, 2, 32), 8)
