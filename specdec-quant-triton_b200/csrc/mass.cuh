@@ -6,15 +6,15 @@
 //   s_rt = q_r . k_t sm_scale,   lse_r = ln sum_t exp s_rt   over the tokens that row i sees
 //   mass[b, h, t] <- decay mass[b, h, t] + sum_r exp(s_rt - lse_r)          for t < ctx_len[b]
 // Row i of n stands at place ctx_len - n + i and sees the tokens up to it.  A row with a NaN or an infinity adds
-// nothing, nor does a token of a page outside the cache get anything.
+// nothing, nor does a token of a page outside the cache get anything; a page of scale 0 gives scores of 0.
 //
 // The products run on the tensor cores, rows on M and tokens on N.  A warp takes 32 tokens at a time: each lane copies
 // the bytes that the B fragments want in it to shared memory (asynchronously, 16 at a time; nobody else reads them), and
 // widens them to fp16 in its registers, exactly; the order of the elements along D is free as long as q has the
 // same.  q stands in shared memory as fp16 (bf16 rows times a power of two that brings their largest element to
 // 2^14: exact down to 2^-31 of it).  A thread has two rows and eight tokens of a product, so a row's maximum and sum over
-// 32 tokens and a token's sum over rows are nearly all its own.  Scores, maxima and sums are fp32, nothing is
-// rounded in between.
+// 32 tokens and a token's sum over rows are nearly all its own.  Scores, maxima and sums are fp32; a score is the
+// product times its scale, rounded once, before anything is taken off it.
 //
 // A column needs its rows' sums over all tokens first.  Where a cluster of up to 8 blocks of 512 tokens holds the whole
 // table, the blocks exchange their maxima and sums through distributed shared memory and each key is read from
@@ -24,8 +24,10 @@
 // takes the sums.  No atomics: a token's sum is made in a fixed order.
 //
 // Measured (B200, 8 KV heads of 128).  One row of 4 heads: 32 sequences of 1 to 8192 tokens 49 us (2.9 TB/s), 32 x 4096 51, one of
-// 37 tokens 4.9: the bytes need 20; a tile of 32 tokens costs a warp some 450 instructions (128 of them widen bytes, 32 are
-// products of which 12 rows of 16 are padding).  36 rows (9 of 4 heads), 8 x 4096: 45 us; 64 rows of the same: 53.
+// 37 tokens 4.9: the bytes of the first two need some 22.  Their instructions (a tile of 32 tokens costs a warp some 450, 128 of them to
+// widen bytes) are some 13 us of issue, 38 % of the time: two blocks an SM (registers) do not cover their waits, the blocks are 1.7 to 1.9
+// turns of the machine, and 32 bytes of scores a token go to HBM and back beside 128 of key.  36 rows (9 of 4 heads), 8 x 4096: 44 us
+// where the bytes need 5.5; 64 rows of the same: 52: each product is made twice, on the warp-level pipe, and each key widened twice.
 // More rows' products are made on tcgen05 (mass_wide.cuh): made here, twice, at the warp-level pipe's 8.5 cycles each, those of
 // 256 rows and two sequences of 12 to 16 thousand tokens took 55 of 163 us.
 #pragma once

@@ -17,8 +17,8 @@ inline int mass_check(int B, int q_len, int H, int H_KV, int D, int page, int bt
   return SPECQ_OK;
 }
 
-// Why from kMassWide rows on the products go to tcgen05: 96 rows of one short sequence 16 us against 23, 256 rows of 4 x 1500 tokens 39 against 75,
-// of two long prompts 127 against 163; but 64 rows of 8 x 4096 tokens 73 against 53 (half of the 128 lanes have no row).
+// Why from kMassWide rows on the products go to tcgen05: 96 rows of one short sequence 16 us against 23, 256 rows of 4 x 1500 tokens 40 against 75,
+// of two long prompts 128 against 163; but 64 rows of 8 x 4096 tokens 73 against 52 (half of the 128 lanes have no row).
 
 // How a call is cut: whether clusters hold the whole table, else the tokens of a block (chunk_tiles * 256) and blocks a head.
 inline bool mass_plan(int B, int H_KV, int rows, int tokens, int* chunk_tiles, int* chunks) {

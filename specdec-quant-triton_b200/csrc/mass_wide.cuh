@@ -7,7 +7,7 @@
 // owns a token.  Neither needs a shuffle.  One warp issues the two 128 x 128 products, two warpgroups take one
 // each; the next rows of q come into their place as soon as both products are done.
 //
-// 256 rows (64 of 4 heads), 8 KV heads of 128, two sequences of 12 to 16 thousand tokens, B200: 127 us for both passes (mma.sync
+// 256 rows (64 of 4 heads), 8 KV heads of 128, two sequences of 12 to 16 thousand tokens, B200: 128 us for both passes (mma.sync
 // 163).  The exponentials, one for each score and pass, 16 a clock and SM, are 26 of them and keep their pipe 25 to
 // 30 % busy, the products theirs 13 %; the rest is a block's start (lengths, table, keys, their widening: 9 of its 26
 // thousand cycles) and waits for products and barriers.  Two blocks an SM cover that for one another: blocks of 512 tokens,

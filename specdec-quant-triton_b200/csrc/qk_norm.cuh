@@ -17,9 +17,9 @@
 // registers over all their heads, the next heads' pieces being copied meanwhile; a block adds its lanes' sums in a fixed order, a
 // second small kernel adds the blocks': no atomics, the same bits each time.
 //
-// Measured (B200, 32 + 8 heads of 128, bf16): 8190 tokens forward 37.4 us, 4.5 TB/s: a thread's angles and weights in fp32 take half of
-// its 128 registers, so that 16 warps an SM have loads in flight (2, 1, 8 heads a thread: 42, 46, 46 us; blocks that stay and
-// copy ahead: 47).  4093 tokens forward and backward 54.4 us, of which backward some 30 (without the copies ahead 56, three stages 57,
+// Measured (B200, 32 + 8 heads of 128, bf16): 8190 tokens forward 37.8 us, 4.5 TB/s: a thread's angles and weights in fp32 take half of
+// its 128 registers and are live from before the reduction, though needed after it, so that 16 warps an SM have loads in flight (2, 1,
+// 8 heads a thread: 42, 46, 46 us; blocks that stay and copy ahead: 47; rope.cuh moves the same bytes in 28.7).  4093 tokens forward and backward 54.4 us, of which backward some 30 (without the copies ahead 56, three stages 57,
 // one head a thread 57).  One token: 2.2 us in a stream of launches.
 #pragma once
 

@@ -164,7 +164,8 @@ def attention_mass_blocks(q, kc, ks, block_tbl, ctx_len, mass, q_len=None, n_row
     paged_attention_blocks (the same q that it is given); mass float32 [B, H_KV, N], N >= the table's tokens.  `n_rows`
     [B] int32: only the first n_rows[b] rows of a sequence count, the newest n_rows[b] tokens of its ctx_len[b] (a
     padded batch; the accepted rows of a verification after kv_compact_blocks).  A sequence without
-    rows or tokens keeps its mass.  A query row with a NaN or an infinity adds nothing.  No gradient."""
+    rows or tokens keeps its mass.  A query row with a NaN or an infinity adds nothing; the tokens of a page of scale 0
+    (none is below) have the score 0.  No gradient."""
     return _native.attention_mass_blocks(q, kc, ks, block_tbl, ctx_len, mass, q_len, n_rows, decay, sm_scale)
 
 
